@@ -290,6 +290,62 @@ VRS_API int vrs_knn_search_noalloc(const float* base, int64_t n, int32_t d, cons
  * up as designed, and leaves the device usable. */
 VRS_API int vrs_selftest_bounded_wait(int64_t limit_ns);
 
+/* ------------------------------------------------- training operators */
+/* No counterpart in the reference. What trains and produces the vectors that
+ * an index holds: the layer norm at an encoder's end, and the softmax cross
+ * entropy of a row's scores against every row of a table (the same inner
+ * products that a dot-product search ranks). All buffers are device pointers
+ * on the current device; work is queued on cuda_stream (NULL = default
+ * stream) and the call returns without waiting; nothing is allocated: scratch
+ * is the caller's workspace, whose size the *_workspace calls give, and may
+ * be reused as soon as the stream has passed the call. Strides are in
+ * elements, between consecutive rows; elements of a row are contiguous.
+ * Results do not depend on timing: the same inputs give the same bits. */
+typedef enum vrs_dtype { VRS_F32 = 0, VRS_F16 = 1, VRS_BF16 = 2 } vrs_dtype;
+
+/* y = (x - mean) * rstd * weight + bias per row of d elements (1..32768),
+ * rstd = 1 / sqrt(var + eps), var the mean of (x - mean)^2. x and y in
+ * dtype; weight and bias (NULL: ones, zeros) in dtype or f32 (param_dtype).
+ * mean and rstd (f32[rows], nullable) are what the backward pass needs. */
+VRS_API int vrs_layer_norm_forward(const void* x, int64_t x_stride, int64_t rows, int64_t d, int32_t dtype,
+                                   const void* weight, const void* bias, int32_t param_dtype, float eps, void* y,
+                                   int64_t y_stride, float* mean, float* rstd, void* cuda_stream);
+
+/* Gradients of the above: dx (in dtype), dweight = sum over rows of
+ * dy (x - mean) rstd and dbias = sum over rows of dy (in param_dtype, either
+ * or both NULL). Sums are held in f32. The workspace (4-byte aligned) is
+ * needed for dweight or dbias only. rows == 0 gives zero dweight and dbias. */
+VRS_API int vrs_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_t* out_bytes);
+VRS_API int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const void* x, int64_t x_stride, int64_t rows,
+                                    int64_t d, int32_t dtype, const void* weight, int32_t param_dtype,
+                                    const float* mean, const float* rstd, void* dx, int64_t dx_stride, void* dweight,
+                                    void* dbias, void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
+/* Linear cross entropy: z[v] = scale * (x . table[v]) over all classes,
+ * lse = log sum_v e^z[v], loss = lse - z[target], without keeping z. x is
+ * rows x d, table classes x d, both VRS_F16 or VRS_BF16 (operands of the
+ * tensor cores; sums, lse and loss are f32); scale > 0 (an inverse
+ * temperature). A row whose target is not in 0..classes-1 takes no part,
+ * whatever its values: loss 0, lse 0, no gradient. The workspace must be
+ * 256-byte aligned. `aligned` of the workspace call: 1 when table (and, for
+ * the backward pass, dtable) start on 16 bytes with strides that are
+ * multiples of 8; 0 sizes it for any alignment. */
+VRS_API int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
+                                               int32_t backward, int32_t aligned, int64_t* out_bytes);
+VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t rows, const void* table,
+                                             int64_t table_stride, int64_t classes, int64_t d, int32_t dtype,
+                                             const int64_t* targets, float scale, float* loss, float* lse,
+                                             void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
+/* Gradients of sum over rows of dloss[row] * loss[row], from the forward
+ * pass's lse: dx (rows x d) and dtable (classes x d) in dtype, either NULL.
+ * The scores are computed again, in pieces of the classes. */
+VRS_API int vrs_linear_cross_entropy_backward(const float* dloss, const void* x, int64_t x_stride, int64_t rows,
+                                              const void* table, int64_t table_stride, int64_t classes, int64_t d,
+                                              int32_t dtype, const int64_t* targets, float scale, const float* lse,
+                                              void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride,
+                                              void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
 /* ------------------------------------------------------ streams, profiling */
 /* Makes a single-GPU or rank-mode handle issue its work on `cuda_stream`
  * (a cudaStream_t of the handle's device; NULL restores the handle's own).

@@ -1,0 +1,278 @@
+"""Layer norm (vrs_layer_norm_*, vector_cuda.ops): forward and backward passes
+against the formulas in 64 bits, gradients against differences, refusals.
+
+Tolerances. With u = 2^-24: a 32-bit sum of the kernel adds at most 32 terms a
+thread, then 5 + 3 + 3 levels over lanes, warps and blocks, so its error is
+under 48 u sum|terms|. That bounds the mean's error by 48 u mean|x|, and
+every element of the normalised row by K u (|xh| + rstd mean|x| + 1) with
+K = 160 (three such sums and the roundings of each step). Outputs in 16 bits
+add half an ulp. Column sums over R rows add at most R/(blocks) + blocks terms
+in order: (R + 64) u sum|terms| bounds them whatever the split."""
+import ctypes
+
+import numpy as np
+import pytest
+
+U = 2.0 ** -24
+
+
+def _half_ulp(t):
+    import torch
+    return {torch.float32: U, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[t]
+
+
+def _tiny(t):
+    """Half the spacing of subnormals."""
+    import torch
+    return {torch.float32: 0.0, torch.float16: 2.0 ** -25, torch.bfloat16: 0.0}[t]
+
+
+def _close(got, want, tol, what):
+    import torch
+    got = got.double()
+    tol = torch.as_tensor(tol, dtype=torch.float64, device=got.device)
+    bad = ~((got - want).abs() <= tol)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} off, worst {(got - want).abs().max().item():.3g}"
+
+
+def _check(x, w, b, dy, eps=1e-5):
+    import torch
+    from vector_cuda import ops
+    d = x.shape[-1]
+    X = x.double().reshape(-1, d)
+    W = torch.ones(d, dtype=torch.float64, device=x.device) if w is None else w.double()
+    B = torch.zeros_like(W) if b is None else b.double()
+    mean = X.mean(1, keepdim=True)
+    rstd = ((X - mean).square().mean(1, keepdim=True) + eps).rsqrt()
+    xh = (X - mean) * rstd
+    e = 160 * U * (xh.abs() + rstd * X.abs().mean(1, keepdim=True) + 1.0)  # of xh
+    y, m, r = ops.layer_norm_forward(x, w, b, eps)
+    assert y.shape == x.shape and y.dtype == x.dtype and m.shape == x.shape[:-1] and r.dtype == torch.float32
+    want = xh * W + B
+    o = _half_ulp(x.dtype)
+    _close(y.reshape(-1, d), want, e * W.abs() + 4 * U * want.abs() + o * want.abs() * 1.01 + _tiny(x.dtype), "y")
+    _close(m.reshape(-1, 1), mean, 50 * U * X.abs().mean(1, keepdim=True), "mean")
+    _close(r.reshape(-1, 1), rstd, 160 * U * rstd * (1 + rstd * X.abs().mean(1, keepdim=True)), "rstd")
+    if dy is None:
+        return
+    D = dy.double().reshape(-1, d)
+    G = D * W
+    m0, m1 = G.mean(1, keepdim=True), (G * xh).mean(1, keepdim=True)
+    dx, dw, db = ops.layer_norm_backward(dy, x, w, m, r)
+    want = rstd * (G - m0 - xh * m1)
+    a0, a1 = G.abs().mean(1, keepdim=True), (G * xh).abs().mean(1, keepdim=True)
+    ea = e.amax(1, keepdim=True) * a0
+    er = 160 * U * (1 + rstd * X.abs().mean(1, keepdim=True)) * want.abs()
+    tol = rstd * (8 * U * (G.abs() + a0 + xh.abs() * a1) + 48 * U * (a0 + xh.abs() * a1) + e * a1 + xh.abs() * ea) + er
+    _close(dx.reshape(-1, d), want, tol + o * want.abs() * 1.01 + _tiny(x.dtype), "dx")
+    n = X.shape[0]
+    p = _half_ulp(dw.dtype)
+    sw, sb = (D * xh).sum(0), D.sum(0)
+    _close(dw, sw, (n + 64) * U * (D * xh).abs().sum(0) + (D.abs() * e).sum(0) + p * sw.abs() * 1.01 + _tiny(dw.dtype),
+           "dweight")
+    _close(db, sb, (n + 64) * U * D.abs().sum(0) + p * sb.abs() * 1.01 + _tiny(db.dtype), "dbias")
+
+
+def _make(rows, d, dtype, ptype, seed=0, shift=1.0):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed + rows * 131 + d)
+    x = (torch.randn(rows, d, generator=g, device="cuda") * 1.5 + shift).to(dtype)
+    w = (1 + 0.3 * torch.randn(d, generator=g, device="cuda")).to(ptype)
+    b = (0.2 * torch.randn(d, generator=g, device="cuda")).to(ptype)
+    dy = torch.randn(rows, d, generator=g, device="cuda").to(dtype)
+    return x, w, b, dy
+
+
+TYPES = [("float32", "float32"), ("float16", "float16"), ("float16", "float32"), ("bfloat16", "bfloat16"),
+         ("bfloat16", "float32")]
+
+# One element to the widest row; both sides of every split of a row (512,
+# 1024, 2048, 4096, 8192 elements), odd widths, rows fewer and more than blocks.
+SIZES = [(1, 1), (3, 2), (5, 7), (1, 384), (9, 512), (7, 513), (33, 1000), (300, 1024), (17, 1025), (1000, 96),
+         (5, 2048), (21, 2056), (4, 4096), (3, 4104), (37, 5001), (2, 8192), (3, 8200), (2, 20011), (1, 32768),
+         (4000, 64), (2500, 771)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,d", SIZES)
+@pytest.mark.parametrize("dtype,ptype", TYPES)
+def test_matches_formula(gpu, rows, d, dtype, ptype):
+    import torch
+    x, w, b, dy = _make(rows, d, getattr(torch, dtype), getattr(torch, ptype))
+    _check(x, w, b, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True)])
+def test_without_parameters(gpu, weight, bias):
+    import torch
+    x, w, b, dy = _make(70, 200, torch.bfloat16, torch.bfloat16)
+    _check(x, w if weight else None, b if bias else None, dy)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d,stride,offset", [(256, 264, 0), (256, 300, 0), (256, 257, 0), (255, 256, 0), (256, 264, 1),
+                                             (256, 264, 8), (6000, 6001, 3)])
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+def test_strided_rows(gpu, d, stride, offset, dtype):
+    """Rows inside a wider buffer, on and off 16-byte boundaries; what lies
+    between them is not touched and does not count."""
+    import torch
+    t = getattr(torch, dtype)
+    x, w, b, dy = _make(45, d, t, t)
+    buf = torch.full((46 * stride + offset,), float("nan"), dtype=t, device="cuda")
+    v = buf[offset:offset + 45 * stride].view(45, stride)[:, :d]
+    v.copy_(x)
+    buf2 = buf.clone()
+    v2 = buf2[offset:offset + 45 * stride].view(45, stride)[:, :d]
+    v2.copy_(dy)
+    _check(v, w, b, v2)
+
+
+@pytest.mark.gpu
+def test_other_layouts(gpu):
+    """Leading dimensions, transposed and broadcast inputs."""
+    import torch
+    x, w, b, dy = _make(60, 128, torch.float32, torch.float32)
+    _check(x.view(3, 4, 5, 128), w, b, dy.view(3, 4, 5, 128))
+    _check(x.t().contiguous().t(), w, b, dy)
+    _check(x[:1].expand(60, 128), w, b, dy[:1].expand(60, 128))
+    _check(x[0], w, b, dy[0])
+
+
+@pytest.mark.gpu
+def test_hard_values(gpu):
+    """A mean far above the spread, rows without spread, large and infinite
+    values (which stay within their row)."""
+    import torch
+    x, w, b, dy = _make(64, 300, torch.float32, torch.float32, shift=1000.0)
+    _check(x, w, b, dy)
+    from vector_cuda import ops
+    x[3] = 7.0
+    x[5, 2] = float("inf")
+    x[6, 1] = float("nan")
+    y, m, r = ops.layer_norm_forward(x, w, b)
+    assert torch.equal(y[3], b) and m[3] == 7.0
+    assert not torch.isfinite(y[5]).any() and torch.isnan(y[6]).all()
+    keep = [i for i in range(64) if i not in (3, 5, 6)]
+    y0, _, _ = ops.layer_norm_forward(x[keep], w, b)
+    assert torch.equal(y[keep], y0)
+
+
+@pytest.mark.gpu
+def test_empty_and_repeatable(gpu):
+    import torch
+    from vector_cuda import ops
+    x, w, b, dy = _make(5000, 769, torch.bfloat16, torch.float32)
+    y, m, r = ops.layer_norm_forward(x[:0], w, b)
+    assert y.shape == (0, 769) and m.shape == (0,)
+    dx, dw, db = ops.layer_norm_backward(dy[:0], x[:0], w, m, r)
+    assert dx.shape == (0, 769) and not dw.any() and not db.any()
+    y, m, r = ops.layer_norm_forward(x, w, b)
+    first = ops.layer_norm_backward(dy, x, w, m, r)
+    for _ in range(3):
+        assert all(torch.equal(p, q) for p, q in zip(first, ops.layer_norm_backward(dy, x, w, m, r)))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,d", [(3, 5), (4, 600)])
+def test_gradients_against_differences(gpu, rows, d):
+    """f(x, w, b) = sum c y in 32 bits along a random direction: the central
+    difference with step h errs by O(h^2) and rounding over h; h = 2^-6 keeps
+    both under 1 % of the largest directional derivative here."""
+    import torch
+    from vector_cuda import ops
+    x, w, b, c = _make(rows, d, torch.float32, torch.float32)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    (ops.layer_norm(*leaves) * c).sum().backward()
+    g = torch.Generator(device="cuda").manual_seed(9)
+    for i, leaf in enumerate(leaves):
+        v = torch.randn(leaf.shape, generator=g, device="cuda")
+        v /= v.norm()
+        h = 2.0 ** -6
+        args = [[t.detach() for t in leaves] for _ in range(2)]
+        args[0][i] = args[0][i] + h * v
+        args[1][i] = args[1][i] - h * v
+        f = [(ops.layer_norm_forward(*a)[0].double() * c.double()).sum() for a in args]
+        diff = ((f[0] - f[1]) / (2 * h)).item()
+        want = (leaf.grad.double() * v.double()).sum().item()
+        assert abs(diff - want) <= 0.01 * leaf.grad.norm().item() + 1e-3
+
+
+@pytest.mark.gpu
+def test_stream_and_in_use(gpu):
+    """Work goes to the current stream: results are ready to that stream's
+    later work without any synchronisation."""
+    import torch
+    from vector_cuda import ops
+    x, w, b, _ = _make(4000, 1024, torch.float32, torch.float32)
+    want = ops.layer_norm_forward(x, w, b)[0]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        z = torch.zeros_like(x)
+        for _ in range(20):
+            z.copy_(x)
+            y = ops.layer_norm_forward(z, w, b)[0]
+            z.zero_()
+    torch.cuda.current_stream().wait_stream(s)
+    assert torch.equal(y, want)
+
+
+def _forward_status(vc, **k):
+    a = dict(x=4096, xs=64, rows=4, d=64, dtype=0, w=None, b=None, pt=0, eps=1e-5, y=4096, ys=64)
+    a.update(k)
+    return vc.lib().vrs_layer_norm_forward(a["x"], a["xs"], a["rows"], a["d"], a["dtype"], a["w"], a["b"], a["pt"],
+                                           a["eps"], a["y"], a["ys"], None, None, None)
+
+
+@pytest.mark.parametrize("change", [dict(dtype=3), dict(dtype=-1), dict(dtype=1, pt=2), dict(rows=-1), dict(d=0),
+                                    dict(d=32769), dict(eps=-1.0), dict(eps=float("nan")), dict(x=None), dict(y=None),
+                                    dict(xs=63), dict(ys=10)])
+def test_forward_refuses(vc, change):
+    """Refused on the host, before any device work (the pointers are never used)."""
+    assert _forward_status(vc, **change) == 5
+    assert b"vrs_layer_norm_forward" in vc.lib().vrs_last_error()
+
+
+def test_backward_refuses(vc):
+    L = vc.lib()
+    n = ctypes.c_int64(0)
+    assert L.vrs_layer_norm_backward_workspace(4, 0, ctypes.byref(n)) == 5
+    assert L.vrs_layer_norm_backward_workspace(4, 64, None) == 5
+
+    def call(dy=4096, x=4096, rows=4, d=64, dtype=0, pt=0, mean=4096, dx=4096, dxs=64):
+        return L.vrs_layer_norm_backward(dy, 64, x, 64, rows, d, dtype, None, pt, mean, 4096, dx, dxs, None, None, None,
+                                         0, None)
+
+    for bad in (dict(dy=None), dict(x=None), dict(mean=None), dict(dx=None), dict(dxs=63), dict(dtype=9),
+                dict(dtype=1, pt=2), dict(d=40000), dict(rows=-5)):
+        assert call(**bad) == 5
+        assert b"vrs_layer_norm_backward" in L.vrs_last_error()
+
+
+def test_python_refuses_cpu_tensors():
+    torch = pytest.importorskip("torch")
+    from vector_cuda import ops
+    with pytest.raises(ValueError, match="CUDA"):
+        ops.layer_norm_forward(torch.zeros(3, 4))
+
+
+@pytest.mark.gpu
+def test_python_refusals(gpu):
+    import torch
+    from vector_cuda import ops
+    x = torch.zeros(4, 64, device="cuda")
+    one = torch.ones(64, device="cuda")
+    for bad in (lambda: ops.layer_norm_forward(x.double()), lambda: ops.layer_norm_forward(x, one[:63]),
+                lambda: ops.layer_norm_forward(x, one.half()), lambda: ops.layer_norm_forward(x, one.cpu()),
+                lambda: ops.layer_norm_forward(x[:, :0])):
+        with pytest.raises(ValueError):
+            bad()
+    y, m, r = ops.layer_norm_forward(x, one)
+    for bad in (lambda: ops.layer_norm_backward(y.half(), x, one, m, r),
+                lambda: ops.layer_norm_backward(y[:3], x, one, m, r),
+                lambda: ops.layer_norm_backward(y, x, one, m[:3], r)):
+        with pytest.raises(ValueError):
+            bad()
+    assert np.isfinite(y.cpu().numpy()).all()
