@@ -5,202 +5,628 @@
 // A row whose target lies outside the table takes no part: loss 0, lse 0, no
 // gradient, whatever its values are.
 //
-// CUDA-core tiles (64 x 64, 16 deep), the classes taken in pieces whose
-// gradient of the scores fits a fixed workspace.
+// This file holds the plan of a call and its small kernels; the products are
+// in linear_ce_tc.cu.
+//   forward   pack -> scores (maximum and sum per row and class tile) -> combine
+//   backward  pack -> for each piece of the classes: gradient of the scores in
+//             16 bits -> dx and dtable products -> finish
+// `pack` copies the rows that take part next to one another (their count
+// stays on the device and sets the number of tiles), so rows without a target
+// cost nothing and their values, NaN too, reach no sum. It also gives the
+// products an aligned operand whatever x's stride and address are.
 #include <cmath>
+#include <mutex>
 
-#include "ops_common.cuh"
+#include <cudaTypedefs.h>
+
+#include "linear_ce.cuh"
 
 namespace vrs {
 namespace ops {
 namespace {
 
-constexpr int BT = 64, BK = 16;
-constexpr int64_t kPieceBytes = 256ll << 20;
+constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
-struct CeArgs {
+// Gradient of the scores held at a time.
+constexpr int64_t kPieceBytes = 128ll << 20;
+// CTA pairs that a product is split for (148 SMs). A constant, so that sums
+// are split alike on every device.
+constexpr int kPairs = 74;
+// Up to here each pack block reads all targets itself; above, a first kernel
+// counts them per kSlab rows.
+constexpr int64_t kScanRows = 8192;
+constexpr int kSlab = 1024;
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// ------------------------------------------------------------------- pack
+
+struct Pack1 {
   const void* x;
-  const void* w;
-  int64_t xs, ws;
-  int64_t rows, classes;
-  int d;
+  int64_t xs, rows;
+  int d, dp;
+  bool vec;  // 16-byte reads of x
   const int64_t* targets;
-  float scale;
-  float2* part;  // [row][tile]: maximum and sum of e^(z - maximum)
-  int64_t ntiles;
-  float* zt;
-  const float* lse;
+  int64_t classes;
+  int per_block;
+  const int2* slabs;  // per slab: taking rows, bits of the largest |dloss|; null: read all targets
+  CeHeader* head;
+  void* xc;        // [taking rows, tail zeros to a whole tile][dp]
+  int* index;      // compact row -> row (forward)
+  int* pos;        // row -> compact row or -1 (backward)
+  int* target;
+  // forward
+  float* loss;
+  float* lse_out;
+  // backward
   const float* dloss;
-  float* g;  // [rows][piece]
-  int64_t v0, vn, gp;
+  const float* lse;
+  float scale;
+  bool f16;
+  float* lse2;
+  float* gs;
 };
 
-__device__ __forceinline__ bool takes_part(const CeArgs& a, int64_t r) {
-  return r < a.rows && a.targets[r] >= 0 && a.targets[r] < a.classes;
+__device__ __forceinline__ bool takes_part(const Pack1& a, int64_t r) {
+  const int64_t t = a.targets[r];
+  return t >= 0 && t < a.classes;
 }
 
-// One 64 x 64 tile of the scores; 256 threads, 4 x 4 each. GRAD: the gradient
-// of the scores, else each row's maximum and sum over the tile.
-template <class T, bool GRAD>
-__global__ void __launch_bounds__(256) ce_tile_kernel(const CeArgs a) {
-  __shared__ float sx[BK][BT + 1], sw[BK][BT + 1];
-  __shared__ float sz[BT][BT + 1];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = (int64_t)blockIdx.y * BT, n0 = a.v0 + (int64_t)blockIdx.x * BT, n1 = a.v0 + a.vn;
-  float acc[4][4] = {};
-  for (int k0 = 0; k0 < a.d; k0 += BK) {
-    for (int i = threadIdx.x; i < BT * BK; i += 256) {
-      const int k = i % BK, r = i / BK;
-      const int64_t m = m0 + r, n = n0 + r;
-      sx[k][r] = m < a.rows && k0 + k < a.d ? to_f32(((const T*)a.x)[m * a.xs + k0 + k]) : 0.0f;
-      sw[k][r] = n < n1 && k0 + k < a.d ? to_f32(((const T*)a.w)[n * a.ws + k0 + k]) : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < BK; k++)
-      for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) acc[i][j] = fmaf(sx[k][ty * 4 + i], sw[k][tx * 4 + j], acc[i][j]);
-    __syncthreads();
+// Sum, sum and maximum over a block of 256.
+__device__ __forceinline__ void block_reduce(int& a, int& b, unsigned& m, int (*s)[3]) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    a += __shfl_xor_sync(~0u, a, o);
+    b += __shfl_xor_sync(~0u, b, o);
+    m = max(m, __shfl_xor_sync(~0u, m, o));
   }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      const float z = acc[i][j] * a.scale;
-      if (GRAD) {
-        if (m >= a.rows || n >= n1) continue;
-        float g = 0.0f;
-        if (takes_part(a, m)) g = (expf(z - a.lse[m]) - (a.targets[m] == n ? 1.0f : 0.0f)) * a.dloss[m] * a.scale;
-        a.g[m * a.gp + n - a.v0] = g;
-      } else {
-        sz[ty * 4 + i][tx * 4 + j] = n < n1 ? z : -INFINITY;
-        if (m < a.rows && n < n1 && a.targets[m] == n) a.zt[m] = z;
+  if ((threadIdx.x & 31) == 0) {
+    s[threadIdx.x >> 5][0] = a;
+    s[threadIdx.x >> 5][1] = b;
+    s[threadIdx.x >> 5][2] = (int)m;
+  }
+  __syncthreads();
+  a = b = 0;
+  m = 0;
+#pragma unroll
+  for (int w = 0; w < 8; w++) {
+    a += s[w][0];
+    b += s[w][1];
+    m = max(m, (unsigned)s[w][2]);
+  }
+}
+
+__global__ void __launch_bounds__(256) ce_count_kernel(const Pack1 a, int2* slabs) {
+  __shared__ int s[8][3];
+  int n = 0, none = 0;
+  unsigned m = 0;
+  const int64_t r0 = (int64_t)blockIdx.x * kSlab;
+  for (int64_t r = r0 + threadIdx.x; r < min(a.rows, r0 + kSlab); r += 256)
+    if (takes_part(a, r)) {
+      n++;
+      if (a.dloss) m = max(m, __float_as_uint(fabsf(a.dloss[r])));
+    }
+  block_reduce(n, none, m, s);
+  if (threadIdx.x == 0) slabs[blockIdx.x] = make_int2(n, (int)m);
+}
+
+// 16-bit floats: the score gradients carry a power of two that brings the
+// largest |dloss scale| into [2^13, 2^14), since f16 ends at 2^16 and loses
+// bits below 2^-14. (Non-finite: no power; the gradients are NaN anyway.)
+__device__ __forceinline__ int grad_exponent(unsigned max_bits, float scale) {
+  const float m = __uint_as_float(max_bits) * scale;
+  if (!(m > 0.0f) || !(m < INFINITY)) return 0;
+  return max(-126, min(126, 13 - ilogbf(m)));
+}
+
+template <bool BACK>
+__global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
+  __shared__ int s[8][3];
+  __shared__ int s_warp[8];
+  __shared__ int s_row[256];
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int64_t r0 = (int64_t)blockIdx.x * a.per_block;
+  const int64_t r1 = min(a.rows, r0 + a.per_block);
+  // Taking rows before this block's, and in all.
+  int before = 0, total = 0;
+  unsigned top = 0;
+  if (a.slabs) {
+    const int64_t slab = r0 / kSlab, n = (a.rows + kSlab - 1) / kSlab;
+    for (int64_t i = tid; i < n; i += 256) {
+      const int2 c = a.slabs[i];
+      total += c.x;
+      if (i < slab) before += c.x;
+      top = max(top, (unsigned)c.y);
+    }
+    for (int64_t r = slab * kSlab + tid; r < r0; r += 256) before += takes_part(a, r);
+  } else {
+#pragma unroll 4
+    for (int64_t r = tid; r < a.rows; r += 256)
+      if (takes_part(a, r)) {
+        total++;
+        before += r < r0;
+        if (BACK) top = max(top, __float_as_uint(fabsf(a.dloss[r])));
+      }
+  }
+  block_reduce(before, total, top, s);
+  float gscale = 1.0f;
+  if (BACK && a.f16) gscale = ldexpf(1.0f, grad_exponent(top, a.scale));
+  if (blockIdx.x == 0 && tid == 0) {
+    a.head->taken = total;
+    a.head->inv_gscale = 1.0f / gscale;
+  }
+  // Places of this block's rows, in row order.
+  const int64_t r = r0 + tid;
+  const bool mine = r < r1, in = mine && takes_part(a, r);
+  const unsigned bal = __ballot_sync(~0u, in);
+  if (lane == 0) s_warp[warp] = __popc(bal);
+  __syncthreads();
+  int here = 0, n_in = 0;
+#pragma unroll
+  for (int w = 0; w < 8; w++) {
+    here += w < warp ? s_warp[w] : 0;
+    n_in += s_warp[w];
+  }
+  here += __popc(bal & ((1u << lane) - 1));
+  if (in) {
+    s_row[here] = tid;
+    const int p = before + here;
+    a.target[p] = (int)a.targets[r];
+    if (BACK) {
+      a.lse2[p] = a.lse[r] * kLog2e;
+      a.gs[p] = a.dloss[r] * a.scale * gscale;
+    } else {
+      a.index[p] = (int)r;
+    }
+  }
+  if (mine) {
+    if (BACK) {
+      a.pos[r] = in ? before + here : -1;
+    } else if (!in) {
+      a.loss[r] = 0.0f;
+      a.lse_out[r] = 0.0f;
+    }
+  }
+  __syncthreads();
+  // One warp a row; elements past d are zeros.
+  uint16_t* xc = (uint16_t*)a.xc;
+  const uint16_t* x = (const uint16_t*)a.x;
+  const int chunks = a.dp / 8;
+  for (int i = warp; i < n_in; i += 8) {
+    const uint16_t* from = x + (r0 + s_row[i]) * a.xs;
+    uint4* to = reinterpret_cast<uint4*>(xc + (int64_t)(before + i) * a.dp);
+    if (a.vec) {
+#pragma unroll 4
+      for (int c = lane; c < chunks; c += 32) to[c] = reinterpret_cast<const uint4*>(from)[c];
+    } else {
+      for (int c = lane; c < chunks; c += 32) {
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          const int e = c * 8 + 2 * j;
+          const uint32_t lo = e < a.d ? from[e] : 0, hi = e + 1 < a.d ? from[e + 1] : 0;
+          q[j] = lo | hi << 16;
+        }
+        to[c] = make_uint4(q[0], q[1], q[2], q[3]);
       }
     }
-  if (GRAD) return;
-  __syncthreads();
-  const int64_t m = m0 + threadIdx.x;
-  if (threadIdx.x < BT && m < a.rows) {
-    float top = -INFINITY, sum = 0.0f;
-    for (int j = 0; j < BT; j++) top = fmaxf(top, sz[threadIdx.x][j]);
-    const float sub = top == -INFINITY ? 0.0f : top;
-    for (int j = 0; j < BT; j++) sum += expf(sz[threadIdx.x][j] - sub);
-    a.part[m * a.ntiles + blockIdx.x] = make_float2(top, sum);
+  }
+  const int tail = (total + kCeM - 1) / kCeM * kCeM;
+  for (int64_t p = total + (int64_t)blockIdx.x * 8 + warp; p < tail; p += (int64_t)gridDim.x * 8) {
+    uint4* to = reinterpret_cast<uint4*>(xc + p * a.dp);
+    for (int c = lane; c < chunks; c += 32) to[c] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// loss and lse from the tiles' maxima and sums: one warp a row.
-__global__ void ce_combine_kernel(const CeArgs a, float* loss, float* lse) {
-  const int64_t r = (int64_t)blockIdx.x * 8 + threadIdx.x / 32;
-  const int lane = threadIdx.x & 31;
-  if (r >= a.rows) return;
-  const bool in = takes_part(a, r);
+// A table whose rows TMA cannot address, copied to rows of dp elements.
+__global__ void __launch_bounds__(256)
+    ce_copy_table_kernel(const uint16_t* __restrict__ w, int64_t ws, int64_t classes, int d, int dp, uint16_t* out) {
+  const int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  if (v >= classes) return;
+  for (int c = threadIdx.x & 31; c < dp / 2; c += 32) {
+    const uint32_t lo = 2 * c < d ? w[v * ws + 2 * c] : 0, hi = 2 * c + 1 < d ? w[v * ws + 2 * c + 1] : 0;
+    reinterpret_cast<uint32_t*>(out + v * dp)[c] = lo | hi << 16;
+  }
+}
+
+// --------------------------------------------------------- combine, finish
+
+// loss and lse of a row from its class tiles' maxima and sums, all in units
+// of log 2. The target's score is subtracted before the logarithm is added:
+// where the target is the largest score the difference is exact. 32 or 128
+// threads a row.
+template <int TPR>
+__global__ void __launch_bounds__(128) ce_combine_kernel(const CeGemm a, const int* __restrict__ index, float* loss,
+                                                        float* lse) {
+  __shared__ float s[4][2];
+  const int64_t r = (int64_t)blockIdx.x * (128 / TPR) + threadIdx.x / TPR;
+  if (r >= a.head->taken) return;  // the whole row's threads
+  const int t = threadIdx.x % TPR;
+  const float2* p = a.part + r * a.vtiles;
   float top = -INFINITY, sum = 0.0f;
-  if (in) {
-    for (int64_t t = lane; t < a.ntiles; t += 32) top = fmaxf(top, a.part[r * a.ntiles + t].x);
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(~0u, top, o));
-    const float sub = top == -INFINITY ? 0.0f : top;
-    for (int64_t t = lane; t < a.ntiles; t += 32) {
-      const float2 p = a.part[r * a.ntiles + t];
-      sum += p.y * expf((p.x == -INFINITY ? 0.0f : p.x) - sub);
-    }
-    for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(~0u, sum, o);
+#pragma unroll 4
+  for (int i = t; i < a.vtiles; i += TPR) {
+    const float2 q = p[i];
+    const float m = fmaxf(top, q.x), sub = m == -INFINITY ? 0.0f : m;
+    sum = sum * exp2f(top - sub) + q.y * exp2f(q.x - sub);
+    top = m;
   }
-  if (lane == 0) {
-    const float l = in ? top + logf(sum) : 0.0f;
-    lse[r] = l;
-    loss[r] = in ? l - a.zt[r] : 0.0f;
+#pragma unroll
+  for (int o = 16; o; o >>= 1) {
+    const float qx = __shfl_xor_sync(~0u, top, o), qy = __shfl_xor_sync(~0u, sum, o);
+    const float m = fmaxf(top, qx), sub = m == -INFINITY ? 0.0f : m;
+    sum = sum * exp2f(top - sub) + qy * exp2f(qx - sub);
+    top = m;
+  }
+  if constexpr (TPR == 128) {
+    if ((threadIdx.x & 31) == 0) {
+      s[threadIdx.x >> 5][0] = top;
+      s[threadIdx.x >> 5][1] = sum;
+    }
+    __syncthreads();
+    top = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
+    const float sub = top == -INFINITY ? 0.0f : top;
+    sum = 0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; w++) sum += s[w][1] * exp2f(s[w][0] - sub);
+  }
+  if (t == 0) {
+    const float l = log2f(sum);
+    const int row = index[r];
+    lse[row] = (top + l) * kLn2;
+    loss[row] = ((top - a.zt[r]) + l) * kLn2;
   }
 }
 
-// acc[m][n] (+)= sum_k a[m am + k ak] b[n bn + k bk]; rows of b whose target
-// lies outside the table (`skip`, along k) are left out.
+// out[row] = sum over splits of acc[split][pos[row]], rounded once; rows
+// without a place get zeros. Four columns a thread.
 template <class T>
 __global__ void __launch_bounds__(256)
-    ce_product_kernel(const float* a, int64_t am, int64_t ak, const T* b, int64_t bn, int64_t bk, int64_t M, int64_t N,
-                      int64_t K, CeArgs c, bool skip, float* acc, bool add, T* out, int64_t os) {
-  __shared__ float sa[BK][BT + 1], sb[BK][BT + 1];
-  const int tx = threadIdx.x % 16, ty = threadIdx.x / 16;
-  const int64_t m0 = (int64_t)blockIdx.y * BT, n0 = (int64_t)blockIdx.x * BT;
-  float s[4][4] = {};
-  for (int64_t k0 = 0; k0 < K; k0 += BK) {
-    for (int i = threadIdx.x; i < BT * BK; i += 256) {
-      const int r = i % BT, k = i / BT;
-      const int64_t m = m0 + r, n = n0 + r, kk = k0 + k;
-      const bool in = kk < K && (!skip || takes_part(c, kk));
-      sa[k][r] = in && m < M ? a[m * am + kk * ak] : 0.0f;
-      sb[k][r] = in && n < N ? to_f32(b[n * bn + kk * bk]) : 0.0f;
-    }
-    __syncthreads();
-    for (int k = 0; k < BK; k++)
-      for (int i = 0; i < 4; i++)
-        for (int j = 0; j < 4; j++) s[i][j] = fmaf(sa[k][ty * 4 + i], sb[k][tx * 4 + j], s[i][j]);
-    __syncthreads();
-  }
-  for (int i = 0; i < 4; i++)
-    for (int j = 0; j < 4; j++) {
-      const int64_t m = m0 + ty * 4 + i, n = n0 + tx * 4 + j;
-      if (m >= M || n >= N) continue;
-      if (acc) acc[m * N + n] = (add ? acc[m * N + n] : 0.0f) + s[i][j];
-      else out[m * os + n] = from_f32<T>(s[i][j]);
-    }
-}
-
-// dx from its 32-bit sums; rows that take no part get zeros.
-template <class T>
-__global__ void ce_finish_kernel(const CeArgs a, const float* acc, T* out, int64_t os) {
+    ce_finish_kernel(const float* __restrict__ acc, int splits, int64_t split_rows, int d, int d4, int64_t rows,
+                     const int* __restrict__ pos, const CeHeader* head, T* out, int64_t os, bool vec) {
+  const int quads = d4 / 4;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= a.rows * a.d) return;
-  const int64_t r = i / a.d, c = i % a.d;
-  out[r * os + c] = takes_part(a, r) ? from_f32<T>(acc[i]) : from_f32<T>(0.0f);
+  if (i >= rows * quads) return;
+  const int64_t r = i / quads;
+  const int c = (int)(i - r * quads) * 4;
+  const int64_t p = pos ? pos[r] : r;
+  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+  if (p >= 0) {
+#pragma unroll 4
+    for (int k = 0; k < splits; k++) {
+      const float4 q = *reinterpret_cast<const float4*>(acc + (k * split_rows + p) * d4 + c);
+      v.x += q.x;
+      v.y += q.y;
+      v.z += q.z;
+      v.w += q.w;
+    }
+    const float inv = head->inv_gscale;
+    v.x *= inv;
+    v.y *= inv;
+    v.z *= inv;
+    v.w *= inv;
+  }
+  T* o = out + r * os + c;
+  const float f[4] = {v.x, v.y, v.z, v.w};
+  if (vec) {
+    store_pack<T, 4>(o, f);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      if (c + j < d) o[j] = from_f32<T>(f[j]);
+  }
 }
 
-int64_t piece_of(int64_t rows, int64_t classes) {
-  int64_t vc = kPieceBytes / (4 * rows) / BT * BT;
-  vc = vc < BT ? BT : vc;
-  return vc < classes ? vc : classes;
-}
-
-int64_t up(int64_t b) { return (b + 255) / 256 * 256; }
-
-int check(const char* who, int64_t rows, int64_t classes, int64_t d, int32_t dtype) {
-  if (dtype != VRS_F16 && dtype != VRS_BF16)
-    return invalid(std::string(who) + ": rows and table are f16 or bf16 (operands of the tensor cores)");
-  if (rows < 0 || rows > (1ll << 31) - 512) return invalid(std::string(who) + ": rows must be in 0..2^31-512");
-  if (classes < 1 || classes > (1ll << 31) - 512) return invalid(std::string(who) + ": classes must be in 1..2^31-512");
-  if (d < 1 || d > 65536) return invalid(std::string(who) + ": d must be in 1..65536");
+template <class T>
+int launch_finish(const float* acc, int splits, int64_t split_rows, int d, int d4, int64_t rows, const int* pos,
+                  const CeHeader* head, void* out, int64_t os, cudaStream_t s) {
+  const bool vec = d % 4 == 0 && (rows == 1 || os % 4 == 0) && (uintptr_t)out % 8 == 0;
+  ce_finish_kernel<T><<<(unsigned)((rows * (d4 / 4) + 255) / 256), 256, 0, s>>>(acc, splits, split_rows, d, d4, rows,
+                                                                             pos, head, (T*)out, os, vec);
+  VRS_CUDA(cudaGetLastError());
+  count_launch();
   return VRS_OK;
 }
 
-template <class T>
-int backward(CeArgs a, void* dx, int64_t dxs, void* dtable, int64_t dts, char* ws, cudaStream_t s) {
-  const int64_t piece = piece_of(a.rows, a.classes);
-  a.g = (float*)ws;
-  a.gp = piece;
-  float* acc = (float*)(ws + up(a.rows * piece * 4));
-  for (a.v0 = 0; a.v0 < a.classes; a.v0 += piece) {
-    a.vn = a.classes - a.v0 < piece ? a.classes - a.v0 : piece;
-    const unsigned tv = (unsigned)((a.vn + BT - 1) / BT), tr = (unsigned)((a.rows + BT - 1) / BT),
-                   td = (unsigned)((a.d + BT - 1) / BT);
-    ce_tile_kernel<T, true><<<dim3(tv, tr), 256, 0, s>>>(a);
-    if (dx)
-      ce_product_kernel<T><<<dim3(td, tr), 256, 0, s>>>(a.g, a.gp, 1, (const T*)a.w + a.v0 * a.ws, 1, a.ws, a.rows,
-                                                        a.d, a.vn, a, false, acc, a.v0 > 0, nullptr, 0);
-    if (dtable)
-      ce_product_kernel<T><<<dim3(td, tv), 256, 0, s>>>(a.g, 1, a.gp, (const T*)a.x, 1, a.xs, a.vn, a.d, a.rows, a,
-                                                        true, nullptr, false, (T*)dtable + a.v0 * dts, dts);
-    count_launch(3);
+// ------------------------------------------------------------- host plan
+
+// Offsets into the workspace, and how the work is cut. Nothing here depends on
+// addresses or on which gradients are asked for, so neither do the sums.
+struct Plan {
+  int64_t rows_p, dp, d4;         // rows in whole tiles, row pitches
+  int64_t piece;                  // classes of a piece, whole tiles
+  int64_t vtiles;                 // class tiles in all
+  int splits_dx, splits_dw;
+  int64_t head, slabs, index, pos, target, lse2, gs, xc, wc, part, zt, g, acc_dx, acc_dw, bytes;
+};
+
+Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned) {
+  Plan p{};
+  p.rows_p = up(rows, kCeM);
+  p.dp = up(d, 8);
+  p.d4 = up(d, 4);
+  p.vtiles = (classes + kCeN - 1) / kCeN;
+  int64_t at = 0;
+  auto take = [&](int64_t bytes) {
+    const int64_t o = at;
+    at += up(bytes, 256);
+    return o;
+  };
+  p.head = take(sizeof(CeHeader));
+  p.slabs = take(rows > kScanRows ? (rows + kSlab - 1) / kSlab * (int64_t)sizeof(int2) : 0);
+  p.target = take(rows * 4);
+  p.xc = take(p.rows_p * p.dp * 2);
+  p.wc = take(aligned ? 0 : classes * p.dp * 2);
+  if (!back) {
+    p.index = take(rows * 4);
+    p.zt = take(rows * 4);
+    p.part = take(rows * p.vtiles * (int64_t)sizeof(float2));
+  } else {
+    p.pos = take(rows * 4);
+    p.lse2 = take(rows * 4);
+    p.gs = take(rows * 4);
+    int64_t tiles = kPieceBytes / (p.rows_p * 2) / kCeN;
+    tiles = tiles < 1 ? 1 : tiles < p.vtiles ? tiles : p.vtiles;
+    const int64_t pieces = (p.vtiles + tiles - 1) / tiles;
+    p.piece = (p.vtiles + pieces - 1) / pieces * kCeN;  // pieces of one size
+    p.g = take(p.rows_p * p.piece * 2);
+    // Few tiles: K is split until the pairs have one each, 8 blocks deep at least.
+    auto splits = [](int64_t tiles_, int64_t kblocks) {
+      int64_t s = kPairs / tiles_ < kblocks / 8 ? kPairs / tiles_ : kblocks / 8;
+      return (int)(s < 1 ? 1 : s);
+    };
+    const int64_t nt = (d + kCeN - 1) / kCeN;
+    p.splits_dx = splits(p.rows_p / kCeM * nt, p.piece / kCeK);
+    p.splits_dw = splits(p.piece / kCeM * nt, (rows + kCeK - 1) / kCeK);
+    p.acc_dx = take(p.splits_dx * p.rows_p * p.d4 * 4);
+    p.acc_dw = take(p.splits_dw > 1 || !aligned ? p.splits_dw * p.piece * p.d4 * 4 : 0);
   }
-  if (dx) {
-    ce_finish_kernel<T><<<(unsigned)((a.rows * a.d + 255) / 256), 256, 0, s>>>(a, acc, (T*)dx, dxs);
+  p.bytes = at;
+  return p;
+}
+
+int check(const std::string& who, int64_t rows, int64_t classes, int64_t d, int32_t dtype) {
+  if (dtype != VRS_F16 && dtype != VRS_BF16)
+    return invalid(who + ": rows and table are f16 or bf16 (operands of the tensor cores)");
+  if (rows < 0 || rows > (1ll << 31) - 512) return invalid(who + ": rows must be in 0..2^31-512");
+  if (classes < 1 || classes > (1ll << 31) - 512) return invalid(who + ": classes must be in 1..2^31-512");
+  if (d < 1 || d > 65536) return invalid(who + ": d must be in 1..65536");
+  if (rows > (1ll << 46) / classes) return invalid(who + ": rows x classes must be at most 2^46");
+  return VRS_OK;
+}
+
+int check_scale(const std::string& who, float scale) {
+  if (!(scale > 0.0f) || !std::isfinite(scale)) return invalid(who + ": scale must be positive and finite");
+  return VRS_OK;
+}
+
+int check_workspace(const std::string& who, const void* ws, int64_t have, int64_t need) {
+  if (!ws) return invalid(who + ": null workspace");
+  if ((uintptr_t)ws % 256) return invalid(who + ": workspace must be 256-byte aligned");
+  if (have < need)
+    return invalid(who + ": workspace of " + std::to_string(have) + " bytes, " + std::to_string(need) + " needed");
+  return VRS_OK;
+}
+
+// Rows that TMA can address: 16-byte aligned starts.
+bool tma_rows(const void* p, int64_t stride, int64_t rows) { return aligned16(p) && (rows == 1 || stride % 8 == 0); }
+
+// The word that a device wait which gave up writes: host memory that the
+// device sees, so a later call reads it without waiting for anything.
+int error_word(int** out) {
+  static std::mutex mu;
+  static int* word = nullptr;
+  std::lock_guard<std::mutex> g(mu);
+  if (!word) {
+    void* p = nullptr;
+    VRS_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
+    word = static_cast<int*>(p);
+    *word = 0;
+  }
+  const int code = *(volatile int*)word;
+  if (code) {
+    *(volatile int*)word = 0;
+    set_error(VRS_ERR_TIMEOUT, "linear cross entropy: a device wait of an earlier call gave up (stage code " +
+                                   std::to_string(code) + "); its results are not valid");
+    return VRS_ERR_TIMEOUT;
+  }
+  *out = word;
+  return VRS_OK;
+}
+
+PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
+  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
+        q != cudaDriverEntryPointSuccess)
+      p = nullptr;
+    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
+  }();
+  return fn;
+}
+
+// [rows][inner] row-major with `stride` elements between rows; boxes of 128
+// bytes by box_rows, 128-byte swizzle, zeros outside.
+int make_map(CUtensorMap* m, CUtensorMapDataType type, int bytes, const void* base, int64_t inner, int64_t rows,
+             int64_t stride, int box_rows) {
+  auto fn = encode_fn();
+  if (!fn) {
+    set_error(VRS_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
+    return VRS_ERR_DRIVER;
+  }
+  cuuint64_t dims[2] = {(cuuint64_t)inner, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)(rows == 1 ? up(inner * bytes, 16) : stride * bytes)};
+  cuuint32_t box[2] = {(cuuint32_t)(128 / bytes), (cuuint32_t)box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  const CUresult r = fn(m, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(VRS_ERR_DRIVER, "cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+    return VRS_ERR_DRIVER;
+  }
+  return VRS_OK;
+}
+
+struct Call {
+  const void* x;
+  int64_t xs, rows;
+  const void* table;
+  int64_t ts, classes, d;
+  int32_t dtype;
+  const int64_t* targets;
+  float scale;
+  char* ws;
+  cudaStream_t s;
+};
+
+// Packs the rows (and the table where TMA cannot address it) and fills what
+// both passes' products share.
+int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool back) {
+  int* err = nullptr;
+  VRS_TRY(error_word(&err));
+  int sms = 0;
+  VRS_TRY(sm_count(&sms));
+  k.x = c.x;
+  k.xs = c.rows == 1 ? 0 : c.xs;
+  k.rows = c.rows;
+  k.d = (int)c.d;
+  k.dp = (int)p.dp;
+  k.vec = c.d % 8 == 0 && tma_rows(c.x, c.xs, c.rows);
+  k.targets = c.targets;
+  k.classes = c.classes;
+  k.head = (CeHeader*)(c.ws + p.head);
+  k.xc = c.ws + p.xc;
+  k.target = (int*)(c.ws + p.target);
+  if (c.rows > kScanRows) {
+    int2* slabs = (int2*)(c.ws + p.slabs);
+    ce_count_kernel<<<(unsigned)((c.rows + kSlab - 1) / kSlab), 256, 0, c.s>>>(k, slabs);
+    count_launch();
+    k.slabs = slabs;
+    k.per_block = 64;
+  } else {
+    k.per_block = (int)((c.rows + 2 * sms - 1) / (2 * sms));
+  }
+  const unsigned blocks = (unsigned)((c.rows + k.per_block - 1) / k.per_block);
+  if (back)
+    ce_pack_kernel<true><<<blocks, 256, 0, c.s>>>(k);
+  else
+    ce_pack_kernel<false><<<blocks, 256, 0, c.s>>>(k);
+  count_launch();
+  const void* w = c.table;
+  int64_t ts = c.ts;
+  if (!tma_rows(w, ts, c.classes)) {
+    w = c.ws + p.wc;
+    ts = p.dp;
+    ce_copy_table_kernel<<<(unsigned)((c.classes + 7) / 8), 256, 0, c.s>>>((const uint16_t*)c.table, c.ts, c.classes,
+                                                                          (int)c.d, (int)p.dp, (uint16_t*)(c.ws + p.wc));
     count_launch();
   }
   VRS_CUDA(cudaGetLastError());
+  const bool f16 = c.dtype == VRS_F16;
+  const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  VRS_TRY(make_map(&maps.x, type, 2, k.xc, c.d, p.rows_p, p.dp, 64));
+  VRS_TRY(make_map(&maps.w, type, 2, w, c.d, c.classes, ts, 64));
+  a.head = k.head;
+  a.err = err;
+  a.classes = (int)c.classes;
+  a.d = (int)c.d;
+  a.kblocks = (int)((c.d + kCeK - 1) / kCeK);
+  // kind::f16, f32 accumulator, M = 256; operand types by bits 7 and 10.
+  a.idesc = (1u << 4) | ((uint32_t)(kCeM >> 4) << 24) | (f16 ? 0u : (1u << 7) | (1u << 10));
+  a.target = k.target;
+  a.c2 = c.scale * kLog2e;
   return VRS_OK;
 }
 
-int64_t need_bytes(int64_t rows, int64_t classes, int64_t d, bool back) {
-  if (rows == 0) return 0;
-  const int64_t fwd = up(rows * ((classes + BT - 1) / BT) * 8) + up(rows * 4);
-  return back ? up(rows * piece_of(rows, classes) * 4) + up(rows * d * 4) : fwd;
+int forward(const Call& c, const Plan& p, float* loss, float* lse) {
+  Pack1 k{};
+  CeMaps maps;
+  CeGemm a{};
+  k.index = (int*)(c.ws + p.index);
+  k.loss = loss;
+  k.lse_out = lse;
+  VRS_TRY(start(c, p, k, maps, a, false));
+  a.vn = a.classes;
+  a.vtiles = (int)p.vtiles;
+  a.part = (float2*)(c.ws + p.part);
+  a.zt = (float*)(c.ws + p.zt);
+  VRS_TRY(launch_ce_gemm(kCeLse, c.dtype == VRS_F16, maps, a, p.rows_p / kCeM * p.vtiles, c.s));
+  // 32 threads read a row's tiles in a few turns, or 128 do.
+  if (p.vtiles <= 128)
+    ce_combine_kernel<32><<<(unsigned)((c.rows + 3) / 4), 128, 0, c.s>>>(a, k.index, loss, lse);
+  else
+    ce_combine_kernel<128><<<(unsigned)c.rows, 128, 0, c.s>>>(a, k.index, loss, lse);
+  VRS_CUDA(cudaGetLastError());
+  count_launch();
+  return VRS_OK;
+}
+
+int finish(bool f16, const float* acc, int splits, int64_t split_rows, const Plan& p, int64_t d, int64_t rows,
+           const int* pos, const CeHeader* head, void* out, int64_t os, cudaStream_t s) {
+  return f16 ? launch_finish<ops::f16>(acc, splits, split_rows, (int)d, (int)p.d4, rows, pos, head, out, os, s)
+             : launch_finish<bf16>(acc, splits, split_rows, (int)d, (int)p.d4, rows, pos, head, out, os, s);
+}
+
+int backward(const Call& c, const Plan& p, const float* dloss, const float* lse, void* dx, int64_t dxs, void* dtable,
+             int64_t dts) {
+  const bool f16 = c.dtype == VRS_F16;
+  const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  Pack1 k{};
+  CeMaps maps;
+  CeGemm a{};
+  k.pos = (int*)(c.ws + p.pos);
+  k.dloss = dloss;
+  k.lse = lse;
+  k.scale = c.scale;
+  k.f16 = f16;
+  k.lse2 = (float*)(c.ws + p.lse2);
+  k.gs = (float*)(c.ws + p.gs);
+  VRS_TRY(start(c, p, k, maps, a, true));
+  a.lse2 = k.lse2;
+  a.gs = k.gs;
+  float* acc_dx = (float*)(c.ws + p.acc_dx);
+  float* acc_dw = (float*)(c.ws + p.acc_dw);
+  VRS_TRY(make_map(&maps.g, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 64));
+  VRS_TRY(make_map(&maps.g_out, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 32));
+  a.dx.on = dx != nullptr;
+  a.dw.on = dtable != nullptr;
+  a.dx.ntiles = a.dw.ntiles = (int)((c.d + kCeN - 1) / kCeN);
+  a.dx.splits = p.splits_dx;
+  a.dw.splits = p.splits_dw;
+  a.dx.f32_rows = (int)p.rows_p;
+  if (dx)
+    VRS_TRY(make_map(&maps.dx_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dx, c.d, p.splits_dx * p.rows_p, p.d4, 32));
+  const bool direct = p.splits_dw == 1 && tma_rows(dtable, dts, c.classes);
+  if (dtable) {
+    if (direct) {
+      VRS_TRY(make_map(&maps.dw_out, type, 2, dtable, c.d, c.classes, dts, 32));
+    } else {
+      a.dw.f32_rows = (int)p.piece;
+      VRS_TRY(make_map(&maps.dw_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dw, c.d, p.splits_dw * p.piece, p.d4, 32));
+    }
+  }
+  for (int64_t v0 = 0; v0 < c.classes; v0 += p.piece) {
+    const int64_t vn = c.classes - v0 < p.piece ? c.classes - v0 : p.piece;
+    a.v0 = (int)v0;
+    a.vn = (int)vn;
+    a.vtiles = (int)((vn + kCeN - 1) / kCeN);
+    VRS_TRY(launch_ce_gemm(kCeGrad, f16, maps, a, p.rows_p / kCeM * a.vtiles, c.s));
+    a.dx.kblocks = (int)((vn + kCeK - 1) / kCeK);
+    a.dx.add = v0 > 0;
+    a.dw.mtiles = a.vtiles;
+    a.dw.row0 = (int)v0;
+    a.dw_first = (c.rows + kCeK - 1) / kCeK / a.dw.splits > a.dx.kblocks / a.dx.splits;
+    const int64_t tiles = (dx ? p.rows_p / kCeM * a.dx.ntiles * a.dx.splits : 0) +
+                          (dtable ? (int64_t)a.dw.mtiles * a.dw.ntiles * a.dw.splits : 0);
+    VRS_TRY(launch_ce_gemm(kCeStore, f16, maps, a, tiles, c.s));
+    if (dtable && !direct)
+      VRS_TRY(finish(f16, acc_dw, p.splits_dw, p.piece, p, c.d, vn, nullptr, a.head, (char*)dtable + v0 * dts * 2, dts,
+                     c.s));
+  }
+  if (dx) VRS_TRY(finish(f16, acc_dx, p.splits_dx, p.rows_p, p, c.d, c.rows, k.pos, a.head, dx, dxs, c.s));
+  return VRS_OK;
 }
 
 }  // namespace
@@ -210,10 +636,10 @@ int64_t need_bytes(int64_t rows, int64_t classes, int64_t d, bool back) {
 extern "C" int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
                                                   int32_t backward, int32_t aligned, int64_t* out_bytes) {
   using namespace vrs::ops;
-  (void)aligned;
-  if (!out_bytes) return invalid("vrs_linear_cross_entropy_workspace: null out_bytes");
-  VRS_TRY(check("vrs_linear_cross_entropy_workspace", rows, classes, d, dtype));
-  *out_bytes = need_bytes(rows, classes, d, backward != 0);
+  const char* who = "vrs_linear_cross_entropy_workspace";
+  if (!out_bytes) return invalid(std::string(who) + ": null out_bytes");
+  VRS_TRY(check(who, rows, classes, d, dtype));
+  *out_bytes = rows == 0 ? 0 : make_plan(rows, classes, d, backward != 0, aligned != 0).bytes;
   return VRS_OK;
 }
 
@@ -223,30 +649,21 @@ extern "C" int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride,
                                                 void* workspace, int64_t workspace_bytes, void* cuda_stream) {
   using namespace vrs;
   using namespace vrs::ops;
-  const char* who = "vrs_linear_cross_entropy_forward";
+  const std::string who = "vrs_linear_cross_entropy_forward";
   VRS_TRY(check(who, rows, classes, d, dtype));
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return invalid(std::string(who) + ": scale must be positive and finite");
+  VRS_TRY(check_scale(who, scale));
   if (rows == 0) return VRS_OK;
-  if (!x || !table || !targets || !loss || !lse || !workspace) return invalid(std::string(who) + ": null buffer");
+  if (!x || !table || !targets || !loss || !lse) return invalid(who + ": null buffer");
   if ((rows > 1 && x_stride < d) || (classes > 1 && table_stride < d))
-    return invalid(std::string(who) + ": row strides must be at least d");
-  if ((uintptr_t)workspace % 256) return invalid(std::string(who) + ": workspace must be 256-byte aligned");
-  if (workspace_bytes < need_bytes(rows, classes, d, false)) return invalid(std::string(who) + ": workspace too small");
-  CeArgs a{};
-  a.x = x; a.w = table; a.xs = x_stride; a.ws = table_stride;
-  a.rows = rows; a.classes = classes; a.d = (int)d; a.targets = targets; a.scale = scale;
-  a.ntiles = (classes + BT - 1) / BT;
-  a.part = (float2*)workspace;
-  a.zt = (float*)((char*)workspace + up(rows * a.ntiles * 8));
-  a.v0 = 0; a.vn = classes;
-  cudaStream_t s = (cudaStream_t)cuda_stream;
-  const dim3 grid((unsigned)a.ntiles, (unsigned)((rows + BT - 1) / BT));
-  if (dtype == VRS_F16) ce_tile_kernel<f16, false><<<grid, 256, 0, s>>>(a);
-  else ce_tile_kernel<bf16, false><<<grid, 256, 0, s>>>(a);
-  ce_combine_kernel<<<(unsigned)((rows + 7) / 8), 256, 0, s>>>(a, loss, lse);
-  count_launch(2);
-  VRS_CUDA(cudaGetLastError());
-  return VRS_OK;
+    return invalid(who + ": row strides must be at least d");
+  const Plan p = make_plan(rows, classes, d, false, tma_rows(table, table_stride, classes));
+  VRS_TRY(check_workspace(who, workspace, workspace_bytes, p.bytes));
+  const Call c{x,       x_stride, rows,  table, table_stride, classes, d, dtype, targets, scale, (char*)workspace,
+               (cudaStream_t)cuda_stream};
+  ProfToken t = prof_begin("linear_cross_entropy_forward", c.s);
+  const int st = forward(c, p, loss, lse);
+  prof_end(t, c.s);
+  return st;
 }
 
 extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void* x, int64_t x_stride, int64_t rows,
@@ -256,25 +673,28 @@ extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void*
                                                  void* workspace, int64_t workspace_bytes, void* cuda_stream) {
   using namespace vrs;
   using namespace vrs::ops;
-  const char* who = "vrs_linear_cross_entropy_backward";
+  const std::string who = "vrs_linear_cross_entropy_backward";
   VRS_TRY(check(who, rows, classes, d, dtype));
-  if (!(scale > 0.0f) || !std::isfinite(scale)) return invalid(std::string(who) + ": scale must be positive and finite");
+  VRS_TRY(check_scale(who, scale));
   if ((rows > 1 && (x_stride < d || (dx && dx_stride < d))) ||
       (classes > 1 && (table_stride < d || (dtable && dtable_stride < d))))
-    return invalid(std::string(who) + ": row strides must be at least d");
+    return invalid(who + ": row strides must be at least d");
   cudaStream_t s = (cudaStream_t)cuda_stream;
-  if (rows == 0) {
-    if (dtable) VRS_CUDA(cudaMemset2DAsync(dtable, (classes > 1 ? dtable_stride : d) * 2, 0, d * 2, classes, s));
+  if (rows == 0) {  // sums over no rows
+    if (dtable)
+      VRS_CUDA(cudaMemset2DAsync(dtable, (size_t)(classes > 1 ? dtable_stride : d) * 2, 0, (size_t)d * 2,
+                                 (size_t)classes, s));
     return VRS_OK;
   }
   if (!dx && !dtable) return VRS_OK;
-  if (!dloss || !x || !table || !targets || !lse || !workspace) return invalid(std::string(who) + ": null buffer");
-  if ((uintptr_t)workspace % 256) return invalid(std::string(who) + ": workspace must be 256-byte aligned");
-  if (workspace_bytes < need_bytes(rows, classes, d, true)) return invalid(std::string(who) + ": workspace too small");
-  CeArgs a{};
-  a.x = x; a.w = table; a.xs = x_stride; a.ws = table_stride;
-  a.rows = rows; a.classes = classes; a.d = (int)d; a.targets = targets; a.scale = scale;
-  a.lse = lse; a.dloss = dloss;
-  return dtype == VRS_F16 ? backward<f16>(a, dx, dx_stride, dtable, dtable_stride, (char*)workspace, s)
-                          : backward<bf16>(a, dx, dx_stride, dtable, dtable_stride, (char*)workspace, s);
+  if (!dloss || !x || !table || !targets || !lse) return invalid(who + ": null buffer");
+  const bool aligned =
+      tma_rows(table, table_stride, classes) && (!dtable || tma_rows(dtable, dtable_stride, classes));
+  const Plan p = make_plan(rows, classes, d, true, aligned);
+  VRS_TRY(check_workspace(who, workspace, workspace_bytes, p.bytes));
+  const Call c{x, x_stride, rows, table, table_stride, classes, d, dtype, targets, scale, (char*)workspace, s};
+  ProfToken t = prof_begin("linear_cross_entropy_backward", s);
+  const int st = backward(c, p, dloss, lse, dx, dx_stride, dtable, dtable_stride);
+  prof_end(t, s);
+  return st;
 }

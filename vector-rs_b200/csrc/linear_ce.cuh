@@ -1,0 +1,69 @@
+// linear_ce.cuh -- between the host plan of the linear cross entropy
+// (linear_ce.cu) and its tensor-core products (linear_ce_tc.cu).
+#pragma once
+#include <cuda.h>
+
+#include "ops_common.cuh"
+
+namespace vrs {
+namespace ops {
+
+// A pair of CTAs computes tiles of 256 x 256 (or 256 x 128) over K blocks of 64.
+constexpr int kCeM = 256;
+constexpr int kCeN = 256;
+constexpr int kCeK = 64;
+
+// Written on the device by the first kernel of a call.
+struct CeHeader {
+  int taken;          // rows that take part
+  float inv_gscale;   // 1 / (power of two the score gradients carry in f16)
+};
+
+enum CeMode : int {
+  kCeLse = 0,    // scores; each row's maximum and sum of e^(z - maximum) per class tile
+  kCeGrad = 1,   // scores again; their gradient in 16 bits for one piece of the classes
+  kCeStore = 2,  // the products of the score gradients: dx (rows x d), dtable (classes x d)
+};
+
+// One product of kCeStore. K is split over `splits` tiles with results of
+// their own ([split][rows_out][d4], added later in split order).
+struct CeJob {
+  int on;
+  int mtiles;      // dtable; dx takes its count from the header
+  int ntiles;      // over d
+  int kblocks;     // dx; dtable takes its count from the header
+  int splits;
+  int f32_rows;    // rows of one split's f32 result; 0: 16-bit result, one split
+  int add;         // f32: add to what earlier pieces left
+  int row0;        // 16-bit result: first row (the piece's first class)
+};
+
+struct CeGemm {
+  const CeHeader* head;
+  int* err;          // host-visible word that a wait which gave up writes
+  int classes;       // all classes
+  int v0, vn;        // the piece
+  int d;
+  int kblocks;       // of d
+  int vtiles;        // class tiles of the piece
+  uint32_t idesc;    // types; majorness and N are added per tile
+  // scores
+  const int* target;   // [rows] of the taking rows, tail -1
+  const float* lse2;   // [rows] lse * log2(e), tail 0
+  const float* gs;     // [rows] dloss * scale (times the power of two), tail 0
+  float c2;            // scale * log2(e)
+  float2* part;        // [row][vtiles]: maximum of c2 z and sum of 2^(c2 z - maximum)
+  float* zt;           // [row] c2 * target's score
+  // products
+  CeJob dx, dw;
+  int dw_first;        // dtable's tiles are the longer ones
+};
+
+struct CeMaps {
+  CUtensorMap x, w, g, g_out, dx_out, dw_out;
+};
+
+int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s);
+
+}  // namespace ops
+}  // namespace vrs
