@@ -110,14 +110,15 @@ __global__ void __launch_bounds__(256) ce_count_kernel(const Pack1 a, int2* slab
   if (threadIdx.x == 0) slabs[blockIdx.x] = make_int2(n, (int)m);
 }
 
-// 16-bit floats: the score gradients carry a power of two that brings the
-// largest |dloss scale| into [2^13, 2^14), since f16 ends at 2^16 and loses
-// bits below 2^-14. (Non-finite: no power; the gradients are NaN anyway.)
-__device__ __forceinline__ int grad_exponent(unsigned max_bits, float scale) {
-  const float m = __uint_as_float(max_bits) * scale;
-  if (!(m > 0.0f) || !(m < INFINITY)) return 0;
-  return max(-126, min(126, 13 - ilogbf(m)));
+// The score gradients are rounded to 16 bits relative to the largest
+// |dloss|: with one weight for all rows (a mean) the target's -1 stays exact
+// and no weight's own rounding biases the sums. 0 and non-finite: by 1.
+__device__ __forceinline__ float grad_unit(unsigned max_bits) {
+  const float m = __uint_as_float(max_bits);
+  return m > 0.0f && m < INFINITY ? m : 1.0f;
 }
+// f16 ends at 2^16 and loses bits below 2^-14: its gradients use the range up to 2^13.
+constexpr float kF16Gain = 8192.0f;
 
 template <bool BACK>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
@@ -149,11 +150,10 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
       }
   }
   block_reduce(before, total, top, s);
-  float gscale = 1.0f;
-  if (BACK && a.f16) gscale = ldexpf(1.0f, grad_exponent(top, a.scale));
+  const float unit = BACK ? grad_unit(top) : 1.0f, gain = BACK && a.f16 ? kF16Gain : 1.0f;
   if (blockIdx.x == 0 && tid == 0) {
     a.head->taken = total;
-    a.head->inv_gscale = 1.0f / gscale;
+    a.head->grad_scale = unit * a.scale / gain;
   }
   // Places of this block's rows, in row order.
   const int64_t r = r0 + tid;
@@ -174,7 +174,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
     a.target[p] = (int)a.targets[r];
     if (BACK) {
       a.lse2[p] = a.lse[r] * kLog2e;
-      a.gs[p] = a.dloss[r] * a.scale * gscale;
+      a.gs[p] = a.dloss[r] / unit * gain;
     } else {
       a.index[p] = (int)r;
     }
@@ -300,20 +300,20 @@ __global__ void __launch_bounds__(256)
       v.z += q.z;
       v.w += q.w;
     }
-    const float inv = head->inv_gscale;
-    v.x *= inv;
-    v.y *= inv;
-    v.z *= inv;
-    v.w *= inv;
+    const float f = head->grad_scale;
+    v.x *= f;
+    v.y *= f;
+    v.z *= f;
+    v.w *= f;
   }
   T* o = out + r * os + c;
-  const float f[4] = {v.x, v.y, v.z, v.w};
+  const float e[4] = {v.x, v.y, v.z, v.w};
   if (vec) {
-    store_pack<T, 4>(o, f);
+    store_pack<T, 4>(o, e);
   } else {
 #pragma unroll
     for (int j = 0; j < 4; j++)
-      if (c + j < d) o[j] = from_f32<T>(f[j]);
+      if (c + j < d) o[j] = from_f32<T>(e[j]);
   }
 }
 

@@ -16,7 +16,7 @@ constexpr int kCeK = 64;
 // Written on the device by the first kernel of a call.
 struct CeHeader {
   int taken;          // rows that take part
-  float inv_gscale;   // 1 / (power of two the score gradients carry in f16)
+  float grad_scale;   // what the products of the score gradients are multiplied by
 };
 
 enum CeMode : int {
@@ -48,9 +48,9 @@ struct CeGemm {
   int vtiles;        // class tiles of the piece
   uint32_t idesc;    // types; majorness and N are added per tile
   // scores
-  const int* target;   // [rows] of the taking rows, tail -1
-  const float* lse2;   // [rows] lse * log2(e), tail 0
-  const float* gs;     // [rows] dloss * scale (times the power of two), tail 0
+  const int* target;   // [rows] of the taking rows
+  const float* lse2;   // [rows] lse * log2(e)
+  const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
   float2* part;        // [row][vtiles]: maximum of c2 z and sum of 2^(c2 z - maximum)
   float* zt;           // [row] c2 * target's score

@@ -451,7 +451,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const CUtensorMap* out = t.job ? &maps.dw_out : &maps.dx_out;
         // rows of the f32 result are never past its end: whole tiles
         const int y = f32 ? t.split * j.f32_rows + r0 : j.row0 + r0;
-        const float inv = t.job ? a.head->inv_gscale : 1.0f;
+        const float f = a.head->grad_scale;
         for (int c = 0; c < t.bn / 32; c++) {
           float w[32];
           if (none) {
@@ -475,7 +475,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           } else {
             if ((c & 1) == 0) stage_ready(lane);
 #pragma unroll
-            for (int i = 0; i < 32; i++) w[i] *= inv;
+            for (int i = 0; i < 32; i++) w[i] *= f;
 #pragma unroll
             for (int q = 0; q < 4; q++)
               stage_put(to, lane, (c & 1) * 4 + q,
