@@ -327,9 +327,9 @@ VRS_API int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const voi
  * tensor cores; sums, lse and loss are f32); scale > 0 (an inverse
  * temperature). A row whose target is not in 0..classes-1 takes no part,
  * whatever its values: loss 0, lse 0, no gradient. The workspace must be
- * 256-byte aligned. `aligned` of the workspace call: 1 when table (and, for
- * the backward pass, dtable) start on 16 bytes with strides that are
- * multiples of 8; 0 sizes it for any alignment. */
+ * 256-byte aligned. `aligned` of the workspace call: 1 when table starts on
+ * 16 bytes with a stride that is a multiple of 8; 0 sizes it for any
+ * alignment (room for a copy of the table). */
 VRS_API int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
                                                int32_t backward, int32_t aligned, int64_t* out_bytes);
 VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t rows, const void* table,

@@ -10,6 +10,8 @@
 #pragma once
 #include <cooperative_groups.h>
 
+#include <atomic>
+
 #include "ops_common.cuh"
 
 namespace vrs {
@@ -29,7 +31,10 @@ struct LnArgs {
   const float* rstd_in;
   float* mean;
   float* rstd;
-  float* partial;      // backward: [row blocks][2][d], null without parameter gradients
+  float* partial;      // backward: [row blocks][2][d], null where it is not needed
+  void* dweight;       // backward: written by column blocks (few rows), nullable
+  void* dbias;
+  int col_blocks;      // backward: blocks of the grid that sum columns
   int64_t rows;
   int64_t xs, dys, ys;  // row strides in elements
   int d;
@@ -40,61 +45,81 @@ struct LnPlan {
   int tpr;      // threads of a row within a block (32..256)
   int cluster;  // blocks of a row (1: none)
   bool vec;     // 16-byte accesses
+  bool wide;    // more elements a thread
   int blocks;   // grid, in clusters
 };
 
-// E: elements a thread holds. The fewest threads that hold a row; a row wider
-// than one block takes a cluster, and so do rows so few that blocks alone
-// would leave most SMs idle (each thread still has at least one access).
-inline LnPlan ln_plan(int64_t rows, int d, int e, int vec, bool can_vec, int sms, int blocks_per_sm) {
+// A thread holds `narrow` elements of a row of up to one block of them, else
+// `wide`, of rows_narrow or rows_wide rows at a time. The fewest threads that hold a row; a row wider than one block takes
+// a cluster, and so do rows so few that blocks alone would leave most SMs idle
+// (each thread still has at least one access).
+inline LnPlan ln_plan(int64_t rows, int d, int narrow, int wide, int rows_narrow, int rows_wide, int vec,
+                      bool can_vec, int sms, int narrow_blocks, int wide_blocks) {
   LnPlan p{};
   p.vec = can_vec;
   const int step = can_vec ? vec : 1;
+  p.wide = d > kLnThreads * narrow;
+  const int e = p.wide ? wide : narrow;
   p.tpr = 32;
   while (p.tpr < kLnThreads && p.tpr * e < d) p.tpr *= 2;
   p.cluster = 1;
   if (p.tpr == kLnThreads) {
-    while (p.cluster < kLnMaxCluster && p.cluster * kLnThreads * e < d) p.cluster *= 2;
+    while (p.cluster < kLnMaxCluster && p.cluster * kLnThreads * wide < d) p.cluster *= 2;
     while (p.cluster < kLnMaxCluster && rows * p.cluster * 2 <= sms && (int64_t)p.cluster * 2 * kLnThreads * step <= d)
       p.cluster *= 2;
   }
-  const int groups = kLnThreads / p.tpr;
+  const int groups = kLnThreads / p.tpr * (p.wide || p.cluster > 1 ? rows_wide : rows_narrow);
   const int64_t need = (rows + groups - 1) / groups;
-  const int64_t most = (int64_t)sms * blocks_per_sm / p.cluster;
+  const int64_t most = (int64_t)sms * (p.wide || p.cluster > 1 ? wide_blocks : narrow_blocks) / p.cluster;
   p.blocks = (int)(need < most ? need : most);
   if (p.blocks < 1) p.blocks = 1;
   return p;
 }
 
-// Sums of N values over the threads of a row, the same bits in all of them.
-// `slot` alternates between two buffers, so one barrier a reduction suffices:
-// a buffer is written again only after the next reduction's barrier.
+// Sums of N values (1, 2 or 4) over the threads of a row, the same bits in all
+// of them. Within a warp the values are halved between the lanes while they
+// are added (4 values: 6 shuffles, not 20). `slot` alternates between two
+// buffers, so one barrier a reduction suffices: a buffer is written again only
+// after the next reduction's barrier.
 template <int TPR, bool CL, int N>
 struct LnReduce {
   static constexpr int kWarps = kLnThreads / 32;
-  struct Smem {
+  struct alignas(16) Smem {
     float warp[2][kWarps][N];
     float cta[2][kLnMaxCluster][N];
   };
-  __device__ static __forceinline__ void run(float* v, Smem* s, int slot) {
+  __device__ static __forceinline__ void run(float (&v)[N], Smem* s, int slot) {
+    const int lane = threadIdx.x & 31;
+    float k = v[0];
+    if constexpr (N == 4) {
+      const bool up = lane & 16;
+      float a = up ? v[2] : v[0], b = up ? v[3] : v[1];
+      a += __shfl_xor_sync(0xffffffffu, up ? v[0] : v[2], 16);
+      b += __shfl_xor_sync(0xffffffffu, up ? v[1] : v[3], 16);
+      k = (lane & 8 ? b : a) + __shfl_xor_sync(0xffffffffu, lane & 8 ? a : b, 8);
+    } else if constexpr (N == 2) {
+      k = (lane & 16 ? v[1] : v[0]) + __shfl_xor_sync(0xffffffffu, lane & 16 ? v[0] : v[1], 16);
+    }
+    constexpr int kLanes = 32 / N;  // that hold one value between them
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1)
+    for (int o = kLanes / 2; o > 0; o >>= 1) k += __shfl_xor_sync(0xffffffffu, k, o);
+    if constexpr (TPR == 32) {
 #pragma unroll
-      for (int n = 0; n < N; n++) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
-    if constexpr (TPR > 32) {
-      const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-      if (lane == 0)
-#pragma unroll
-        for (int n = 0; n < N; n++) s->warp[slot][warp][n] = v[n];
+      for (int n = 0; n < N; n++) v[n] = N == 1 ? k : __shfl_sync(0xffffffffu, k, n * kLanes);
+    } else {
+      const int warp = threadIdx.x >> 5;
+      if (lane % kLanes == 0) s->warp[slot][warp][lane / kLanes] = k;
       __syncthreads();
       constexpr int W = TPR / 32;
       const int w0 = warp / W * W;
 #pragma unroll
       for (int n = 0; n < N; n++) v[n] = 0.0f;
 #pragma unroll
-      for (int w = 0; w < W; w++)
+      for (int w = 0; w < W; w++) {
+        const Pack<float, N> p = load_pack<float, N>(&s->warp[slot][w0 + w][0]);
 #pragma unroll
-        for (int n = 0; n < N; n++) v[n] += s->warp[slot][w0 + w][n];
+        for (int n = 0; n < N; n++) v[n] += p.v[n];
+      }
     }
     if constexpr (CL) {
       auto cluster = cooperative_groups::this_cluster();
@@ -115,10 +140,22 @@ struct LnReduce {
 };
 
 template <class K>
-int ln_launch(K kernel, const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+  auto kernel = K::get();
+  const int smem = K::smem();
+  if (smem > 16384) {  // beside up to 32 KB of static shared memory
+    static std::atomic<unsigned> allowed[4];  // a bit per device
+    int dev = 0;
+    VRS_CUDA(cudaGetDevice(&dev));
+    if (dev >= 128 || !(allowed[dev / 32].load() >> (dev % 32) & 1)) {
+      VRS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+      if (dev < 128) allowed[dev / 32].fetch_or(1u << (dev % 32));
+    }
+  }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.blocks * p.cluster));
+  cfg.gridDim = dim3((unsigned)(p.blocks * p.cluster + a.col_blocks));
   cfg.blockDim = dim3(kLnThreads);
+  cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
   cudaLaunchAttribute at[1];
   if (p.cluster > 1) {
@@ -134,32 +171,35 @@ int ln_launch(K kernel, const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   return VRS_OK;
 }
 
-// The instantiation for a plan: K<T, P, VEC, TPR, CL>::get().
-template <template <class, class, int, int, bool> class K, class T, class P, int VEC>
+// The instantiation for a plan.
+template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE, class T, class P, int VEC>
 int ln_dispatch_tpr(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  if (p.cluster > 1) return ln_launch(K<T, P, VEC, kLnThreads, true>::get(), a, p, s);
+  if (p.cluster > 1) return ln_launch<K<T, P, VEC, kLnThreads, WIDE, true>>(a, p, s);
+  if (p.wide) return ln_launch<K<T, P, VEC, kLnThreads, WIDE, false>>(a, p, s);
   switch (p.tpr) {
-    case 32: return ln_launch(K<T, P, VEC, 32, false>::get(), a, p, s);
-    case 64: return ln_launch(K<T, P, VEC, 64, false>::get(), a, p, s);
-    case 128: return ln_launch(K<T, P, VEC, 128, false>::get(), a, p, s);
-    default: return ln_launch(K<T, P, VEC, 256, false>::get(), a, p, s);
+    case 32: return ln_launch<K<T, P, VEC, 32, NARROW, false>>(a, p, s);
+    case 64: return ln_launch<K<T, P, VEC, 64, NARROW, false>>(a, p, s);
+    case 128: return ln_launch<K<T, P, VEC, 128, NARROW, false>>(a, p, s);
+    default: return ln_launch<K<T, P, VEC, 256, NARROW, false>>(a, p, s);
   }
 }
 
-template <template <class, class, int, int, bool> class K, class T, class P>
+template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE, class T, class P>
 int ln_dispatch_vec(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  return p.vec ? ln_dispatch_tpr<K, T, P, 16 / (int)sizeof(T)>(a, p, s) : ln_dispatch_tpr<K, T, P, 1>(a, p, s);
+  return p.vec ? ln_dispatch_tpr<K, NARROW, WIDE, T, P, 16 / (int)sizeof(T)>(a, p, s)
+               : ln_dispatch_tpr<K, NARROW, WIDE, T, P, 1>(a, p, s);
 }
 
-template <template <class, class, int, int, bool> class K>
+template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE>
 int ln_dispatch(int dtype, int param_dtype, const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   switch (dtype) {
-    case VRS_F32: return ln_dispatch_vec<K, float, float>(a, p, s);
+    case VRS_F32: return ln_dispatch_vec<K, NARROW, WIDE, float, float>(a, p, s);
     case VRS_F16:
-      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, f16, float>(a, p, s) : ln_dispatch_vec<K, f16, f16>(a, p, s);
+      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, NARROW, WIDE, f16, float>(a, p, s)
+                                    : ln_dispatch_vec<K, NARROW, WIDE, f16, f16>(a, p, s);
     default:
-      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, bf16, float>(a, p, s)
-                                    : ln_dispatch_vec<K, bf16, bf16>(a, p, s);
+      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, NARROW, WIDE, bf16, float>(a, p, s)
+                                    : ln_dispatch_vec<K, NARROW, WIDE, bf16, bf16>(a, p, s);
   }
 }
 

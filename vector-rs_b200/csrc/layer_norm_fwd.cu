@@ -4,22 +4,22 @@
 // Bound by memory: 2 d elements a row. The row stays in registers between the
 // two sums (mean first, then the squares of x - mean: one pass of
 // sum-of-squares would lose the variance of rows whose mean is large).
-#include <atomic>
-
 #include "layer_norm.cuh"
 
 namespace vrs {
 namespace ops {
 namespace {
 
-// Elements a thread holds: with 32 a warp covers 1,024 elements with no
-// barrier at all.
-constexpr int kE = 32;
+// Elements a thread holds of each of kRows rows.
+constexpr int kNarrow = 16, kWide = 32;
+constexpr int kNarrowRows = 2, kWideRows = 1;
+constexpr int kNarrowBlocks = 3, kWideBlocks = 2;
 
-template <class T, class P, int VEC, int TPR, bool CL>
-__global__ void __launch_bounds__(kLnThreads) ln_fwd_kernel(const LnArgs a) {
-  constexpr int NV = kE / VEC, GROUPS = kLnThreads / TPR;
-  using Red = LnReduce<TPR, CL, 1>;
+template <class T, class P, int VEC, int TPR, int E, bool CL>
+__global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWideBlocks)
+    ln_fwd_kernel(const LnArgs a) {
+  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR, R = E == kNarrow ? kNarrowRows : kWideRows;
+  using Red = LnReduce<TPR, CL, R>;
   __shared__ typename Red::Smem s_red;
   int tt = threadIdx.x % TPR, TT = TPR;
   int64_t first = blockIdx.x, step = gridDim.x;
@@ -32,80 +32,95 @@ __global__ void __launch_bounds__(kLnThreads) ln_fwd_kernel(const LnArgs a) {
   }
   const T* x = (const T*)a.x;
   T* y = (T*)a.y;
-  const P* w = (const P*)a.weight;
-  const P* b = (const P*)a.bias;
   const float inv_d = 1.0f / (float)a.d;
+  // The parameters of the thread's columns stay in registers for all rows;
+  // without them 1 and 0 give the same bits as leaving the steps out (but for
+  // the sign of a zero).
+  Held<P, E, VEC> w, b;
+  w.fill(1.0f);
+  b.fill(0.0f);
+#pragma unroll
+  for (int i = 0; i < NV; i++) {
+    const int c = (i * TT + tt) * VEC;
+    if (a.weight && c < a.d) w.load(i, (const P*)a.weight + c);
+    if (a.bias && c < a.d) b.load(i, (const P*)a.bias + c);
+  }
   int slot = 0;
   // Every thread of a block takes the same number of turns (the barriers
   // inside the reductions); a group past the last row computes on zeros.
-  for (int64_t r0 = first * GROUPS; r0 < a.rows; r0 += step * GROUPS) {
-    const int64_t row = r0 + threadIdx.x / TPR;
-    const bool have = row < a.rows;
-    Pack<T, VEC> k[NV];
-    float v[kE];
+  for (int64_t r0 = first * (GROUPS * R); r0 < a.rows; r0 += step * (GROUPS * R)) {
+    const int64_t row0 = r0 + threadIdx.x / TPR;  // and every GROUPS-th after it
+    Held<T, E, VEC> k[R];
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (i * TT + tt) * VEC;
-      if (have && c < a.d) {
-        k[i] = load_pack<T, VEC>(x + row * a.xs + c);
-      } else {
+    for (int r = 0; r < R; r++) {
+      const int64_t row = row0 + r * GROUPS;
+      k[r].fill(0.0f);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) k[i].v[j] = from_f32<T>(0.0f);
+      for (int i = 0; i < NV; i++) {
+        const int c = (i * TT + tt) * VEC;
+        if (row < a.rows && c < a.d) k[r].load(i, x + row * a.xs + c);
       }
     }
-    float sum = 0.0f;
+    F2 v[R][E / 2];
+    float mean[R], rstd[R];
 #pragma unroll
-    for (int i = 0; i < NV; i++)
+    for (int r = 0; r < R; r++) {
+      F2 s = pack_f2(0.0f);
 #pragma unroll
-      for (int j = 0; j < VEC; j++) sum += v[i * VEC + j] = to_f32(k[i].v[j]);
-    Red::run(&sum, &s_red, slot);
+      for (int q = 0; q < E / 2; q++) s = add2(s, v[r][q] = k[r].pair(q));
+      mean[r] = sum_f2(s);
+    }
+    Red::run(mean, &s_red, slot);
     slot ^= 1;
-    const float mean = sum * inv_d;
-    float sq = 0.0f;
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const bool in = (i * TT + tt) * VEC < a.d;
+    for (int r = 0; r < R; r++) {
+      mean[r] *= inv_d;
+      const F2 m = pack_f2(-mean[r]);
+      F2 s = pack_f2(0.0f);
 #pragma unroll
-      for (int j = 0; j < VEC; j++) {
-        v[i * VEC + j] -= mean;
-        if (in) sq = fmaf(v[i * VEC + j], v[i * VEC + j], sq);
+      for (int q = 0; q < E / 2; q++) {
+        v[r][q] = add2(v[r][q], m);
+        const int c0 = (2 * q / VEC * TT + tt) * VEC, c1 = ((2 * q + 1) / VEC * TT + tt) * VEC;
+        if constexpr (VEC > 1) {
+          if (c0 < a.d) s = fma2(v[r][q], v[r][q], s);
+        } else {
+          float lo, hi;
+          unpack_f2(v[r][q], lo, hi);
+          const F2 in = pack_f2(c0 < a.d ? lo : 0.0f, c1 < a.d ? hi : 0.0f);
+          s = fma2(in, in, s);
+        }
       }
+      rstd[r] = sum_f2(s);
     }
-    Red::run(&sq, &s_red, slot);
+    Red::run(rstd, &s_red, slot);
     slot ^= 1;
-    const float rstd = 1.0f / sqrtf(fmaf(sq, inv_d, a.eps));
-    if (!have) continue;
-    if (tt == 0) {
-      if (a.mean) a.mean[row] = mean;
-      if (a.rstd) a.rstd[row] = rstd;
-    }
 #pragma unroll
-    for (int i = 0; i < NV; i++) {
-      const int c = (i * TT + tt) * VEC;
-      if (c >= a.d) continue;
-      float o[VEC], f[VEC];
-#pragma unroll
-      for (int j = 0; j < VEC; j++) o[j] = v[i * VEC + j] * rstd;
-      if (w) {
-        load_params<P, VEC>(w + c, f);
-#pragma unroll
-        for (int j = 0; j < VEC; j++) o[j] *= f[j];
+    for (int r = 0; r < R; r++) {
+      const int64_t row = row0 + r * GROUPS;
+      if (row >= a.rows) break;
+      rstd[r] = 1.0f / sqrtf(fmaf(rstd[r], inv_d, a.eps));
+      if (tt == 0) {
+        if (a.mean) a.mean[row] = mean[r];
+        if (a.rstd) a.rstd[row] = rstd[r];
       }
-      if (b) {
-        load_params<P, VEC>(b + c, f);
+      const F2 f = pack_f2(rstd[r]);
 #pragma unroll
-        for (int j = 0; j < VEC; j++) o[j] += f[j];
+      for (int q = 0; q < E / 2; q++) v[r][q] = fma2(mul2(v[r][q], f), w.pair(q), b.pair(q));
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int c = (i * TT + tt) * VEC;
+        if (c < a.d) store_held<T, VEC, E>(y + row * a.ys + c, v[r], i);
       }
-      store_pack<T, VEC>(y + row * a.ys + c, o);
     }
   }
   // A block must not leave while another still writes its shared memory.
   if constexpr (CL) cooperative_groups::this_cluster().sync();
 }
 
-template <class T, class P, int VEC, int TPR, bool CL>
+template <class T, class P, int VEC, int TPR, int E, bool CL>
 struct FwdKernel {
-  static auto get() { return &ln_fwd_kernel<T, P, VEC, TPR, CL>; }
+  static auto get() { return &ln_fwd_kernel<T, P, VEC, TPR, E, CL>; }
+  static int smem() { return 0; }
 };
 
 }  // namespace
@@ -167,10 +182,11 @@ extern "C" int vrs_layer_norm_forward(const void* x, int64_t x_stride, int64_t r
                        aligned16(y) && aligned16(weight) && aligned16(bias);
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  const LnPlan p = ln_plan(rows, (int)d, kE, vec, can_vec, sms, 6);
+  const LnPlan p = ln_plan(rows, (int)d, kNarrow, kWide, kNarrowRows, kWideRows, vec, can_vec, sms, kNarrowBlocks,
+                          kWideBlocks);
   cudaStream_t s = (cudaStream_t)cuda_stream;
   ProfToken t = prof_begin("layer_norm_forward", s);
-  const int st = ln_dispatch<FwdKernel>(dtype, param_dtype, a, p, s);
+  const int st = ln_dispatch<FwdKernel, kNarrow, kWide>(dtype, param_dtype, a, p, s);
   prof_end(t, s);
   return st;
 }

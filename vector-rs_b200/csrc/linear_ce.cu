@@ -28,7 +28,7 @@ namespace {
 constexpr float kLog2e = 1.44269504088896341f, kLn2 = 0.693147180559945309f;
 
 // Gradient of the scores held at a time.
-constexpr int64_t kPieceBytes = 128ll << 20;
+constexpr int64_t kPieceBytes = 256ll << 20;
 // CTA pairs that a product is split for (148 SMs). A constant, so that sums
 // are split alike on every device.
 constexpr int kPairs = 74;
@@ -120,8 +120,13 @@ __device__ __forceinline__ float grad_unit(unsigned max_bits) {
 // f16 ends at 2^16 and loses bits below 2^-14: its gradients use the range up to 2^13.
 constexpr float kF16Gain = 8192.0f;
 
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 template <bool BACK>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
+  grid_launch();
+  grid_wait();  // the slab counts, where there are any
   __shared__ int s[8][3];
   __shared__ int s_warp[8];
   __shared__ int s_row[256];
@@ -141,13 +146,17 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
     }
     for (int64_t r = slab * kSlab + tid; r < r0; r += 256) before += takes_part(a, r);
   } else {
-#pragma unroll 4
-    for (int64_t r = tid; r < a.rows; r += 256)
-      if (takes_part(a, r)) {
+    // (Both loads of a row at once, sixteen rows in flight.)
+#pragma unroll 16
+    for (int64_t r = tid; r < a.rows; r += 256) {
+      const int64_t t = a.targets[r];
+      const unsigned g = BACK ? __float_as_uint(fabsf(a.dloss[r])) : 0;
+      if (t >= 0 && t < a.classes) {
         total++;
         before += r < r0;
-        if (BACK) top = max(top, __float_as_uint(fabsf(a.dloss[r])));
+        top = max(top, g);
       }
+    }
   }
   block_reduce(before, total, top, s);
   const float unit = BACK ? grad_unit(top) : 1.0f, gain = BACK && a.f16 ? kF16Gain : 1.0f;
@@ -211,22 +220,60 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
       }
     }
   }
-  const int tail = (total + kCeM - 1) / kCeM * kCeM;
+  // (Past the last row TMA reads zeros itself.)
+  const int64_t tail = min(a.rows, (int64_t)(total + kCeM - 1) / kCeM * kCeM);
   for (int64_t p = total + (int64_t)blockIdx.x * 8 + warp; p < tail; p += (int64_t)gridDim.x * 8) {
     uint4* to = reinterpret_cast<uint4*>(xc + p * a.dp);
     for (int c = lane; c < chunks; c += 32) to[c] = make_uint4(0, 0, 0, 0);
   }
 }
 
-// A table whose rows TMA cannot address, copied to rows of dp elements.
-__global__ void __launch_bounds__(256)
-    ce_copy_table_kernel(const uint16_t* __restrict__ w, int64_t ws, int64_t classes, int d, int dp, uint16_t* out) {
-  const int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (v >= classes) return;
-  for (int c = threadIdx.x & 31; c < dp / 2; c += 32) {
-    const uint32_t lo = 2 * c < d ? w[v * ws + 2 * c] : 0, hi = 2 * c + 1 < d ? w[v * ws + 2 * c + 1] : 0;
-    reinterpret_cast<uint32_t*>(out + v * dp)[c] = lo | hi << 16;
+// A table whose rows TMA cannot address, copied to rows of dp elements: 16
+// bytes out a thread, read as A elements at a time (the rows' alignment).
+template <int A>
+__global__ void __launch_bounds__(256) ce_copy_table_kernel(const uint16_t* __restrict__ w, int64_t ws, int64_t classes,
+                                                           int d, int dp, uint16_t* out) {
+  grid_launch();  // reads inputs and writes what only the products read: nothing to wait for
+  const int chunks = dp / 8, lane = threadIdx.x & 31;
+  for (int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); v < classes; v += (int64_t)gridDim.x * 8) {
+    const uint16_t* from = w + v * ws;
+    uint4* to = reinterpret_cast<uint4*>(out + v * dp);
+#pragma unroll 2
+    for (int c = lane; c < chunks; c += 32) {
+      Pack<uint16_t, 8> q;
+#pragma unroll
+      for (int j = 0; j < 8; j += A) {
+        const int e = c * 8 + j;
+        Pack<uint16_t, A> k;
+        if (e + A <= d) {
+          k = load_pack<uint16_t, A>(from + e);
+        } else {
+#pragma unroll
+          for (int i = 0; i < A; i++) k.v[i] = e + i < d ? from[e + i] : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < A; i++) q.v[j + i] = k.v[i];
+      }
+      to[c] = *reinterpret_cast<uint4*>(&q);
+    }
   }
+}
+
+int copy_table(const void* table, int64_t ts, int64_t classes, int d, int dp, void* out, int sms, cudaStream_t s) {
+  const uint16_t* w = (const uint16_t*)table;
+  uint16_t* o = (uint16_t*)out;
+  const int64_t need = (classes + 7) / 8, most = (int64_t)sms * 8;
+  const unsigned blocks = (unsigned)(need < most ? need : most);
+  const uintptr_t at = (uintptr_t)table | (uintptr_t)(classes == 1 ? 0 : ts * 2);
+  if (at % 8 == 0)
+    ce_copy_table_kernel<4><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
+  else if (at % 4 == 0)
+    ce_copy_table_kernel<2><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
+  else
+    ce_copy_table_kernel<1><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
+  VRS_CUDA(cudaGetLastError());
+  count_launch();
+  return VRS_OK;
 }
 
 // --------------------------------------------------------- combine, finish
@@ -239,13 +286,14 @@ template <int TPR>
 __global__ void __launch_bounds__(128) ce_combine_kernel(const CeGemm a, const int* __restrict__ index, float* loss,
                                                         float* lse) {
   __shared__ float s[4][2];
+  grid_wait();
   const int64_t r = (int64_t)blockIdx.x * (128 / TPR) + threadIdx.x / TPR;
-  if (r >= a.head->taken) return;  // the whole row's threads
+  if (r >= (a.rows >= 0 ? a.rows : a.head->taken)) return;  // the whole row's threads
   const int t = threadIdx.x % TPR;
-  const float2* p = a.part + r * a.vtiles;
+  const float2* p = a.part + r * a.parts;
   float top = -INFINITY, sum = 0.0f;
 #pragma unroll 4
-  for (int i = t; i < a.vtiles; i += TPR) {
+  for (int i = t; i < a.parts; i += TPR) {
     const float2 q = p[i];
     const float m = fmaxf(top, q.x), sub = m == -INFINITY ? 0.0f : m;
     sum = sum * exp2f(top - sub) + q.y * exp2f(q.x - sub);
@@ -272,48 +320,46 @@ __global__ void __launch_bounds__(128) ce_combine_kernel(const CeGemm a, const i
   }
   if (t == 0) {
     const float l = log2f(sum);
-    const int row = index[r];
-    lse[row] = (top + l) * kLn2;
-    loss[row] = ((top - a.zt[r]) + l) * kLn2;
+    const int64_t row = index ? index[r] : r;
+    const bool in = index || (a.targets[r] >= 0 && a.targets[r] < a.classes);
+    lse[row] = in ? (top + l) * kLn2 : 0.0f;
+    loss[row] = in ? ((top - a.zt[r]) + l) * kLn2 : 0.0f;
   }
 }
 
 // out[row] = sum over splits of acc[split][pos[row]], rounded once; rows
-// without a place get zeros. Four columns a thread.
+// without a place get zeros. A warp a row, four columns a lane and turn.
 template <class T>
 __global__ void __launch_bounds__(256)
     ce_finish_kernel(const float* __restrict__ acc, int splits, int64_t split_rows, int d, int d4, int64_t rows,
                      const int* __restrict__ pos, const CeHeader* head, T* out, int64_t os, bool vec) {
-  const int quads = d4 / 4;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i >= rows * quads) return;
-  const int64_t r = i / quads;
-  const int c = (int)(i - r * quads) * 4;
-  const int64_t p = pos ? pos[r] : r;
-  float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  if (p >= 0) {
+  grid_wait();
+  const float f = head->grad_scale;
+  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+    const int64_t p = pos ? pos[r] : r;
+    T* o = out + r * os;
 #pragma unroll 4
-    for (int k = 0; k < splits; k++) {
-      const float4 q = *reinterpret_cast<const float4*>(acc + (k * split_rows + p) * d4 + c);
-      v.x += q.x;
-      v.y += q.y;
-      v.z += q.z;
-      v.w += q.w;
-    }
-    const float f = head->grad_scale;
-    v.x *= f;
-    v.y *= f;
-    v.z *= f;
-    v.w *= f;
-  }
-  T* o = out + r * os + c;
-  const float e[4] = {v.x, v.y, v.z, v.w};
-  if (vec) {
-    store_pack<T, 4>(o, e);
-  } else {
+    for (int c = (threadIdx.x & 31) * 4; c < d4; c += 128) {
+      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      if (p >= 0) {
+#pragma unroll 4
+        for (int k = 0; k < splits; k++) {
+          const float4 q = *reinterpret_cast<const float4*>(acc + (k * split_rows + p) * d4 + c);
+          v.x += q.x;
+          v.y += q.y;
+          v.z += q.z;
+          v.w += q.w;
+        }
+      }
+      const float e[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+      if (vec) {
+        store_pack<T, 4>(o + c, e);
+      } else {
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      if (c + j < d) o[j] = from_f32<T>(e[j]);
+        for (int j = 0; j < 4; j++)
+          if (c + j < d) o[c + j] = from_f32<T>(e[j]);
+      }
+    }
   }
 }
 
@@ -321,9 +367,11 @@ template <class T>
 int launch_finish(const float* acc, int splits, int64_t split_rows, int d, int d4, int64_t rows, const int* pos,
                   const CeHeader* head, void* out, int64_t os, cudaStream_t s) {
   const bool vec = d % 4 == 0 && (rows == 1 || os % 4 == 0) && (uintptr_t)out % 8 == 0;
-  ce_finish_kernel<T><<<(unsigned)((rows * (d4 / 4) + 255) / 256), 256, 0, s>>>(acc, splits, split_rows, d, d4, rows,
-                                                                             pos, head, (T*)out, os, vec);
-  VRS_CUDA(cudaGetLastError());
+  int sms = 0;
+  VRS_TRY(sm_count(&sms));
+  const int64_t need = (rows + 7) / 8, most = (int64_t)sms * 8;
+  VRS_TRY(launch_after(ce_finish_kernel<T>, (unsigned)(need < most ? need : most), 256, 0, s, acc, splits, split_rows, d,
+                       d4, rows, pos, head, (T*)out, os, vec));
   count_launch();
   return VRS_OK;
 }
@@ -336,6 +384,7 @@ struct Plan {
   int64_t rows_p, dp, d4;         // rows in whole tiles, row pitches
   int64_t piece;                  // classes of a piece, whole tiles
   int64_t vtiles;                 // class tiles in all
+  int64_t parts;                  // and parts of 64 classes
   int splits_dx, splits_dw;
   int64_t head, slabs, index, pos, target, lse2, gs, xc, wc, part, zt, g, acc_dx, acc_dw, bytes;
 };
@@ -346,6 +395,7 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
   p.dp = up(d, 8);
   p.d4 = up(d, 4);
   p.vtiles = (classes + kCeN - 1) / kCeN;
+  p.parts = (classes + 63) / 64;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -360,7 +410,7 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
   if (!back) {
     p.index = take(rows * 4);
     p.zt = take(rows * 4);
-    p.part = take(rows * p.vtiles * (int64_t)sizeof(float2));
+    p.part = take(rows * p.parts * (int64_t)sizeof(float2));
   } else {
     p.pos = take(rows * 4);
     p.lse2 = take(rows * 4);
@@ -379,7 +429,7 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
     p.splits_dx = splits(p.rows_p / kCeM * nt, p.piece / kCeK);
     p.splits_dw = splits(p.piece / kCeM * nt, (rows + kCeK - 1) / kCeK);
     p.acc_dx = take(p.splits_dx * p.rows_p * p.d4 * 4);
-    p.acc_dw = take(p.splits_dw > 1 || !aligned ? p.splits_dw * p.piece * p.d4 * 4 : 0);
+    p.acc_dw = take(p.splits_dw > 1 ? p.splits_dw * p.piece * p.d4 * 4 : 0);
   }
   p.bytes = at;
   return p;
@@ -482,7 +532,9 @@ struct Call {
 };
 
 // Packs the rows (and the table where TMA cannot address it) and fills what
-// both passes' products share.
+// both passes' products share. Forward, up to one tile of rows that TMA can
+// address stay where they are: there are no tiles to save, and a row's values
+// reach its own loss only.
 int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool back) {
   int* err = nullptr;
   VRS_TRY(error_word(&err));
@@ -499,34 +551,42 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   k.head = (CeHeader*)(c.ws + p.head);
   k.xc = c.ws + p.xc;
   k.target = (int*)(c.ws + p.target);
-  if (c.rows > kScanRows) {
-    int2* slabs = (int2*)(c.ws + p.slabs);
-    ce_count_kernel<<<(unsigned)((c.rows + kSlab - 1) / kSlab), 256, 0, c.s>>>(k, slabs);
+  const bool packed = back || c.rows > kCeM || !tma_rows(c.x, c.xs, c.rows);
+  a.rows = packed ? -1 : (int)c.rows;
+  if (packed) {
+    if (c.rows > kScanRows) {
+      int2* slabs = (int2*)(c.ws + p.slabs);
+      ce_count_kernel<<<(unsigned)((c.rows + kSlab - 1) / kSlab), 256, 0, c.s>>>(k, slabs);
+      VRS_CUDA(cudaGetLastError());
+      count_launch();
+      k.slabs = slabs;
+      k.per_block = 64;
+    } else {
+      k.per_block = (int)((c.rows + 2 * sms - 1) / (2 * sms));
+    }
+    const unsigned blocks = (unsigned)((c.rows + k.per_block - 1) / k.per_block);
+    if (back)
+      ce_pack_kernel<true><<<blocks, 256, 0, c.s>>>(k);
+    else
+      ce_pack_kernel<false><<<blocks, 256, 0, c.s>>>(k);
+    VRS_CUDA(cudaGetLastError());
     count_launch();
-    k.slabs = slabs;
-    k.per_block = 64;
   } else {
-    k.per_block = (int)((c.rows + 2 * sms - 1) / (2 * sms));
+    a.targets = c.targets;
   }
-  const unsigned blocks = (unsigned)((c.rows + k.per_block - 1) / k.per_block);
-  if (back)
-    ce_pack_kernel<true><<<blocks, 256, 0, c.s>>>(k);
-  else
-    ce_pack_kernel<false><<<blocks, 256, 0, c.s>>>(k);
-  count_launch();
   const void* w = c.table;
   int64_t ts = c.ts;
   if (!tma_rows(w, ts, c.classes)) {
     w = c.ws + p.wc;
     ts = p.dp;
-    ce_copy_table_kernel<<<(unsigned)((c.classes + 7) / 8), 256, 0, c.s>>>((const uint16_t*)c.table, c.ts, c.classes,
-                                                                          (int)c.d, (int)p.dp, (uint16_t*)(c.ws + p.wc));
-    count_launch();
+    VRS_TRY(copy_table(c.table, c.ts, c.classes, (int)c.d, (int)p.dp, c.ws + p.wc, sms, c.s));
   }
-  VRS_CUDA(cudaGetLastError());
   const bool f16 = c.dtype == VRS_F16;
   const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  VRS_TRY(make_map(&maps.x, type, 2, k.xc, c.d, p.rows_p, p.dp, 64));
+  if (packed)
+    VRS_TRY(make_map(&maps.x, type, 2, k.xc, c.d, c.rows, p.dp, 64));
+  else
+    VRS_TRY(make_map(&maps.x, type, 2, c.x, c.d, c.rows, c.xs, 64));
   VRS_TRY(make_map(&maps.w, type, 2, w, c.d, c.classes, ts, 64));
   a.head = k.head;
   a.err = err;
@@ -535,6 +595,7 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   a.kblocks = (int)((c.d + kCeK - 1) / kCeK);
   // kind::f16, f32 accumulator, M = 256; operand types by bits 7 and 10.
   a.idesc = (1u << 4) | ((uint32_t)(kCeM >> 4) << 24) | (f16 ? 0u : (1u << 7) | (1u << 10));
+  a.one_tile_rows = c.rows <= kCeM ? (int)c.rows : 0;
   a.target = k.target;
   a.c2 = c.scale * kLog2e;
   return VRS_OK;
@@ -549,16 +610,22 @@ int forward(const Call& c, const Plan& p, float* loss, float* lse) {
   k.lse_out = lse;
   VRS_TRY(start(c, p, k, maps, a, false));
   a.vn = a.classes;
-  a.vtiles = (int)p.vtiles;
+  // One tile of rows reads the table at the speed of memory: where at most
+  // half of the pairs would have a tile in the last turn, halves of tiles
+  // shorten it.
+  const int64_t rest = p.vtiles % kPairs;
+  a.whole = (int)(c.rows <= kCeM && 2 * rest <= kPairs ? p.vtiles - rest : p.vtiles);
+  a.vtiles = a.whole == p.vtiles ? a.whole : a.whole + (int)((c.classes - a.whole * (int64_t)kCeN + 127) / 128);
+  a.parts = (int)p.parts;
   a.part = (float2*)(c.ws + p.part);
   a.zt = (float*)(c.ws + p.zt);
-  VRS_TRY(launch_ce_gemm(kCeLse, c.dtype == VRS_F16, maps, a, p.rows_p / kCeM * p.vtiles, c.s));
-  // 32 threads read a row's tiles in a few turns, or 128 do.
-  if (p.vtiles <= 128)
-    ce_combine_kernel<32><<<(unsigned)((c.rows + 3) / 4), 128, 0, c.s>>>(a, k.index, loss, lse);
+  VRS_TRY(launch_ce_gemm(kCeLse, c.dtype == VRS_F16, maps, a, p.rows_p / kCeM * a.vtiles, c.s));
+  const int* index = a.rows < 0 ? k.index : nullptr;
+  // 32 threads read a row's parts in a few turns, or 128 do.
+  if (p.parts <= 128)
+    VRS_TRY(launch_after(ce_combine_kernel<32>, (unsigned)((c.rows + 3) / 4), 128, 0, c.s, a, index, loss, lse));
   else
-    ce_combine_kernel<128><<<(unsigned)c.rows, 128, 0, c.s>>>(a, k.index, loss, lse);
-  VRS_CUDA(cudaGetLastError());
+    VRS_TRY(launch_after(ce_combine_kernel<128>, (unsigned)c.rows, 128, 0, c.s, a, index, loss, lse));
   count_launch();
   return VRS_OK;
 }
@@ -598,20 +665,23 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   a.dx.f32_rows = (int)p.rows_p;
   if (dx)
     VRS_TRY(make_map(&maps.dx_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dx, c.d, p.splits_dx * p.rows_p, p.d4, 32));
-  const bool direct = p.splits_dw == 1 && tma_rows(dtable, dts, c.classes);
+  const bool direct = p.splits_dw == 1;
   if (dtable) {
-    if (direct) {
-      VRS_TRY(make_map(&maps.dw_out, type, 2, dtable, c.d, c.classes, dts, 32));
-    } else {
+    if (!direct) {
       a.dw.f32_rows = (int)p.piece;
       VRS_TRY(make_map(&maps.dw_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dw, c.d, p.splits_dw * p.piece, p.d4, 32));
+    } else if (tma_rows(dtable, dts, c.classes)) {
+      VRS_TRY(make_map(&maps.dw_out, type, 2, dtable, c.d, c.classes, dts, 32));
+    } else {
+      a.dw.out = (uint16_t*)dtable;
+      a.dw.out_stride = c.classes == 1 ? 0 : dts;
     }
   }
   for (int64_t v0 = 0; v0 < c.classes; v0 += p.piece) {
     const int64_t vn = c.classes - v0 < p.piece ? c.classes - v0 : p.piece;
     a.v0 = (int)v0;
     a.vn = (int)vn;
-    a.vtiles = (int)((vn + kCeN - 1) / kCeN);
+    a.vtiles = a.whole = (int)((vn + kCeN - 1) / kCeN);
     VRS_TRY(launch_ce_gemm(kCeGrad, f16, maps, a, p.rows_p / kCeM * a.vtiles, c.s));
     a.dx.kblocks = (int)((vn + kCeK - 1) / kCeK);
     a.dx.add = v0 > 0;
@@ -688,9 +758,7 @@ extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void*
   }
   if (!dx && !dtable) return VRS_OK;
   if (!dloss || !x || !table || !targets || !lse) return invalid(who + ": null buffer");
-  const bool aligned =
-      tma_rows(table, table_stride, classes) && (!dtable || tma_rows(dtable, dtable_stride, classes));
-  const Plan p = make_plan(rows, classes, d, true, aligned);
+  const Plan p = make_plan(rows, classes, d, true, tma_rows(table, table_stride, classes));
   VRS_TRY(check_workspace(who, workspace, workspace_bytes, p.bytes));
   const Call c{x, x_stride, rows, table, table_stride, classes, d, dtype, targets, scale, (char*)workspace, s};
   ProfToken t = prof_begin("linear_cross_entropy_backward", s);

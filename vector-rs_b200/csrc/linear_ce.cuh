@@ -36,23 +36,30 @@ struct CeJob {
   int f32_rows;    // rows of one split's f32 result; 0: 16-bit result, one split
   int add;         // f32: add to what earlier pieces left
   int row0;        // 16-bit result: first row (the piece's first class)
+  uint16_t* out;   // 16-bit result that TMA cannot address, else null
+  int64_t out_stride;
 };
 
 struct CeGemm {
   const CeHeader* head;
+  int rows;          // rows that take part, -1: head->taken
+  int whole;         // tiles of 256 columns; those after them have 128 (kCeLse)
+  int one_tile_rows; // scores: the rows where one tile holds them all, else 0
   int* err;          // host-visible word that a wait which gave up writes
   int classes;       // all classes
   int v0, vn;        // the piece
   int d;
   int kblocks;       // of d
   int vtiles;        // class tiles of the piece
+  int parts;         // kCeLse: 64-class parts of a row
   uint32_t idesc;    // types; majorness and N are added per tile
   // scores
-  const int* target;   // [rows] of the taking rows
+  const int64_t* targets;  // [rows] where the rows are not packed, else null
+  const int* target;       // [rows] of the taking rows
   const float* lse2;   // [rows] lse * log2(e)
   const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
-  float2* part;        // [row][vtiles]: maximum of c2 z and sum of 2^(c2 z - maximum)
+  float2* part;        // [row][parts]: maximum of c2 z and sum of 2^(c2 z - maximum)
   float* zt;           // [row] c2 * target's score
   // products
   CeJob dx, dw;
@@ -62,6 +69,24 @@ struct CeGemm {
 struct CeMaps {
   CUtensorMap x, w, g, g_out, dx_out, dw_out;
 };
+
+// A launch that may begin while the kernel before it on the stream ends; the
+// kernel waits for that one's results itself (griddepcontrol.wait).
+template <class... KA, class... A>
+int launch_after(void (*kernel)(KA...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  VRS_CUDA(cudaLaunchKernelEx(&cfg, kernel, KA(args)...));
+  return VRS_OK;
+}
 
 int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s);
 

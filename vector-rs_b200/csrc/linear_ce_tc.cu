@@ -10,11 +10,12 @@
 // A pair owns a tile of 256 rows (128 a CTA: its TMEM lanes) by up to 256
 // columns; each CTA loads its half of both operands, 64 deep, into a ring of
 // stages. One thread of the even CTA issues M = 256 MMAs into one of two
-// accumulators (2 x 256 columns = all of TMEM); two groups of four epilogue
-// warps a CTA take alternate tiles, so a tile is drained, exponentiated and
-// stored while the next one is multiplied. Results leave through swizzled
-// staging tiles and TMA stores, in f32 also as TMA additions to what earlier
-// pieces of the classes left.
+// accumulators (2 x 256 columns = all of TMEM). Sixteen epilogue warps a CTA
+// (TMEM lane quadrant x 64 columns) load a tile into registers and hand its
+// accumulator back at once, so a tile is exponentiated and stored while the
+// next two are multiplied. Results leave through swizzled staging tiles and
+// TMA stores, in f32 also as TMA additions to what earlier pieces of the
+// classes left.
 //
 // Bound by the tensor cores for d of some hundreds and more; by the
 // exponentials for small d (one a score, 16 an SM and clock, against
@@ -30,17 +31,19 @@ namespace {
 
 using namespace vrs::tc;
 
-constexpr int THREADS = 384;          // producer, MMA, TMEM, spare; 8 epilogue warps
-constexpr int EPI_FIRST = 4;
+constexpr int EPI_FIRST = 4;          // producer, MMA, TMEM, spare
+constexpr int EPI_WARPS = 16;
+constexpr int THREADS = 32 * (EPI_FIRST + EPI_WARPS);
+constexpr int QCOLS = 64;             // columns of an epilogue warp
 constexpr uint32_t BOX = 64 * 128;    // bytes of a 64 x 64 tile of 16-bit operands
 constexpr uint32_t STAGE = 4 * BOX;   // a CTA's halves: A 128 x 64, B 128 x 64
 constexpr uint32_t STG = 32 * 128;    // a warp's staging tile: 32 rows of 128 bytes
 constexpr size_t SMEM_BAR = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;
 
-constexpr int stages(int mode) { return mode == kCeLse ? 6 : 5; }
+constexpr int stages(int mode) { return mode == kCeLse ? 7 : 5; }
 constexpr size_t smem_bytes(int mode) {
-  return 1024 + (size_t)stages(mode) * STAGE + (mode == kCeLse ? 0 : 8 * 2 * STG) + SMEM_BAR;
+  return 1024 + (size_t)stages(mode) * STAGE + (mode == kCeLse ? 0 : EPI_WARPS * STG) + SMEM_BAR;
 }
 static_assert(smem_bytes(kCeLse) <= 232448 && smem_bytes(kCeGrad) <= 232448, "above the per-block limit");
 
@@ -82,30 +85,8 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
-// 32 lanes x 32 columns; the values may be used only after tmem_wait.
-__device__ __forceinline__ void tmem_ld_issue(uint32_t taddr, float (&v)[32]) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(taddr)
-      : "memory");
-}
-// The values pass through the wait, so no use of them can move before it.
-__device__ __forceinline__ void tmem_wait(float (&v)[32]) {
-  asm volatile("tcgen05.wait::ld.sync.aligned;"
-               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
-                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
-                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
-                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
-                 "+f"(v[30]), "+f"(v[31])
-               :
-               : "memory");
-}
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
@@ -126,6 +107,16 @@ struct Tile {
   int split;
 };
 
+// Rows that take part: counted by the pack kernel, or all rows where no
+// packing was needed.
+__device__ __forceinline__ int taken_rows(const CeGemm& a) { return a.rows >= 0 ? a.rows : a.head->taken; }
+
+// 64-row boxes of the A operand that a CTA loads in the score modes: with one
+// tile of rows, those that hold rows. The others are zeroed once.
+__device__ __forceinline__ int a_boxes(const CeGemm& a, int cta) {
+  return a.one_tile_rows ? max(0, min(2, (a.one_tile_rows - cta * 128 + 63) / 64)) : 2;
+}
+
 struct Tiles {
   int mtiles;         // rows that take part, in tiles
   int kblocks_rows;   // and in K blocks
@@ -136,7 +127,7 @@ struct Tiles {
 template <int MODE>
 __device__ __forceinline__ Tiles count_tiles(const CeGemm& a) {
   Tiles t;
-  const int rows = a.head->taken;
+  const int rows = taken_rows(a);
   t.mtiles = (rows + kCeM - 1) / kCeM;
   t.kblocks_rows = (rows + kCeK - 1) / kCeK;
   t.n_dx = t.n_dw = 0;
@@ -158,8 +149,9 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
     // and the rows' operand stays in L2.
     t.job = 0;
     t.m = id % c.mtiles;
-    t.n = id / c.mtiles * kCeN;
-    t.bn = kCeN;
+    const int n = id / c.mtiles;
+    t.bn = n < a.whole ? kCeN : kCeN / 2;
+    t.n = n < a.whole ? n * kCeN : a.whole * kCeN + (n - a.whole) * (kCeN / 2);
     t.kb0 = 0;
     t.kb1 = a.kblocks;
     t.split = 0;
@@ -185,61 +177,58 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
 
 // --------------------------------------------------------------- epilogues
 
-// One row's 256 scores: running maximum and sum of powers of two (the scores
-// times scale * log2(e), so that e^z is one ex2), the target's score.
-__device__ __forceinline__ void epi_lse(const CeGemm& a, uint32_t tmem, int n0, int64_t row, bool live, int tgt,
-                                        int vtile) {
-  float top = -INFINITY, sum = 0.0f;
-  const int cols = min(kCeN, a.classes - n0);
-  float v[2][32];
-  tmem_ld_issue(tmem, v[0]);
+// 64 scores of a row: their maximum and the sum of powers of two (the scores
+// times scale * log2(e), so that e^z is one ex2), and the target's score.
+__device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[QCOLS], int n0, int64_t row, bool live, int tgt) {
+  const int cols = a.classes - n0;
+  if (cols <= 0) return;
+  if (cols < QCOLS) {
 #pragma unroll
-  for (int c = 0; c < kCeN / 32; c++) {
-    float(&w)[32] = v[c & 1];
-    tmem_wait(w);
-    if (c + 1 < kCeN / 32) tmem_ld_issue(tmem + (c + 1) * 32, v[(c + 1) & 1]);
-    if (c * 32 >= cols) continue;
-    if (cols - c * 32 < 32) {
-#pragma unroll
-      for (int j = 0; j < 32; j++)
-        if (j >= cols - c * 32) w[j] = -INFINITY;
-    }
-    const int at = tgt - n0 - c * 32;
-    if (at >= 0 && at < 32) {
-      float z = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 32; j++) z = j == at ? w[j] : z;
-      if (live) a.zt[row] = z * a.c2;
-    }
-    float m = fmaxf(w[0], w[1]);
-#pragma unroll
-    for (int j = 2; j < 32; j += 2) m = fmax3(m, w[j], w[j + 1]);
-    m *= a.c2;
-    if (m > top) {
-      sum *= ex2(top - m);
-      top = m;
-    }
-    const float sub = top == -INFINITY ? 0.0f : top;
-    float s0 = 0.0f, s1 = 0.0f;
-#pragma unroll
-    for (int j = 0; j < 32; j += 2) {
-      s0 += ex2(fmaf(w[j], a.c2, -sub));
-      s1 += ex2(fmaf(w[j + 1], a.c2, -sub));
-    }
-    sum += s0 + s1;
+    for (int j = 0; j < QCOLS; j++)
+      if (j >= cols) w[j] = -INFINITY;
   }
-  if (live) a.part[row * a.vtiles + vtile] = make_float2(top, sum);
+  const int at = tgt - n0;
+  if (at >= 0 && at < QCOLS && live) {
+    float z = 0.0f;
+#pragma unroll
+    for (int j = 0; j < QCOLS; j++) z = j == at ? w[j] : z;
+    a.zt[row] = z * a.c2;
+  }
+  float m[4];
+#pragma unroll
+  for (int k = 0; k < 4; k++) {
+    m[k] = fmax3(w[16 * k], w[16 * k + 1], w[16 * k + 2]);
+#pragma unroll
+    for (int j = 3; j < 15; j += 2) m[k] = fmax3(m[k], w[16 * k + j], w[16 * k + j + 1]);
+    m[k] = fmaxf(m[k], w[16 * k + 15]);
+  }
+  const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * a.c2;
+  const float sub = top == -INFINITY ? 0.0f : top;
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+  for (int j = 0; j < QCOLS; j++) sum[j & 3] += ex2(fmaf(w[j], a.c2, -sub));
+  if (live) a.part[row * a.parts + n0 / QCOLS] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
 }
 
-// A staging tile is free again once its last store has read it (of two).
+// A staging tile is free again once its last store has read it.
 __device__ __forceinline__ void stage_ready(int lane) {
-  if (lane == 0) bulk_wait_read<1>();
+  if (lane == 0) bulk_wait_read<0>();
   __syncwarp();
 }
 
 // Row `lane` of a staging tile: 16-byte chunk j, 128-byte swizzle.
 __device__ __forceinline__ void stage_put(uint8_t* stg, int lane, int j, uint4 q) {
   *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = q;
+}
+
+// 64 values of a row in 16 bits into the staging tile.
+template <bool F16>
+__device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, const float (&w)[QCOLS]) {
+#pragma unroll
+  for (int q = 0; q < 8; q++)
+    stage_put(stg, lane, q,
+              make_uint4(pack2<F16>(w[8 * q], w[8 * q + 1]), pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
+                         pack2<F16>(w[8 * q + 4], w[8 * q + 5]), pack2<F16>(w[8 * q + 6], w[8 * q + 7])));
 }
 
 // ------------------------------------------------------------------ kernel
@@ -251,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_stg = smem + (size_t)ST * STAGE;
-  uint64_t* bars = (uint64_t*)(s_stg + (MODE == kCeLse ? 0 : 8 * 2 * STG));
+  uint64_t* bars = (uint64_t*)(s_stg + (MODE == kCeLse ? 0 : EPI_WARPS * STG));
   uint64_t* full = bars;           // [ST] even CTA: both CTAs' bytes
   uint64_t* empty = full + ST;     // [ST] each CTA: MMA commit
   uint64_t* tfull = empty + ST;    // [2] each CTA: MMA commit
@@ -271,16 +260,27 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 8);
+      mbar_init(&tempty[b], 2 * EPI_WARPS);
     }
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc_pair(s_tmem, 512);
+  if (MODE != kCeStore && a.one_tile_rows) {
+    const int skip = a_boxes(a, cta) * (int)BOX;
+    for (int s = 0; s < ST; s++)
+      for (int i = skip + threadIdx.x * 16; i < 2 * (int)BOX; i += THREADS * 16)
+        *reinterpret_cast<uint4*>(smem + s * STAGE + i) = make_uint4(0, 0, 0, 0);
+    fence_async_smem();
+  }
   tc_fence_before();
   cluster_sync();  // barriers initialised and TMEM allocated in both CTAs
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
+  // The set-up above overlaps the end of the kernel before; its results are
+  // there from here on.
+  grid_launch();
+  grid_wait();
   const Tiles cnt = count_tiles<MODE>(a);
 
   if (warp == 0) {
@@ -288,9 +288,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     if (lane == 0) {
       int it = 0;
       bool ok = true;
+      const int na = a_boxes(a, cta);
       for (int id = pair; ok && id < cnt.total; id += npairs) {
         const Tile t = tile_at<MODE>(a, cnt, id);
         const int boxes = t.bn >> 7;  // of B in each CTA
+        const uint32_t bytes = (MODE == kCeStore ? 4 : a_boxes(a, 0) + a_boxes(a, 1)) * BOX + 2u * boxes * BOX;
         const int ra = t.m * kCeM + cta * 128;
         const int rb = t.n + cta * (t.bn >> 1);
         for (int kb = t.kb0; kb < t.kb1; kb++, it++) {
@@ -299,14 +301,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             ok = false;
             break;
           }
-          if (lead) mbar_expect_tx(&full[s], 2u * (2 + boxes) * BOX);
+          if (lead) mbar_expect_tx(&full[s], bytes);
           const uint32_t bar = mapa_shared(&full[s], 0);
           uint8_t* sa = smem + s * STAGE;
           uint8_t* sb = sa + 2 * BOX;
           const int k = kb * kCeK;
           if (MODE != kCeStore) {
-            for (int i = 0; i < 2; i++) tma_load_2d_pair(sa + i * BOX, &maps.x, k, ra + 64 * i, bar);
-            for (int i = 0; i < 2; i++) tma_load_2d_pair(sb + i * BOX, &maps.w, k, a.v0 + rb + 64 * i, bar);
+            for (int i = 0; i < na; i++) tma_load_2d_pair(sa + i * BOX, &maps.x, k, ra + 64 * i, bar);
+            for (int i = 0; i < boxes; i++) tma_load_2d_pair(sb + i * BOX, &maps.w, k, a.v0 + rb + 64 * i, bar);
           } else if (t.job == 0) {
             for (int i = 0; i < 2; i++) tma_load_2d_pair(sa + i * BOX, &maps.g, k, ra + 64 * i, bar);
             for (int i = 0; i < boxes; i++) tma_load_2d_pair(sb + i * BOX, &maps.w, rb + 64 * i, a.v0 + k, bar);
@@ -365,146 +367,136 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else if (warp >= EPI_FIRST) {
     // ---------------------------------------------------- epilogue
-    const int group = (warp - EPI_FIRST) >> 2, quad = warp & 3;
-    uint8_t* stg = s_stg + (warp - EPI_FIRST) * 2 * STG;
-    int puts = 0;
-    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + group * 256;
+    const int quarter = (warp - EPI_FIRST) >> 2, quad = warp & 3;
+    uint8_t* stg = s_stg + (warp - EPI_FIRST) * STG;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int taken = taken_rows(a);
     int tn = 0;
     for (int id = pair; id < cnt.total; id += npairs, tn++) {
-      if ((tn & 1) != group) continue;
       const Tile t = tile_at<MODE>(a, cnt, id);
+      const int b = tn & 1;
       const int r0 = t.m * kCeM + cta * 128 + quad * 32;  // the warp's first row
       const int64_t row = r0 + lane;
+      const int n0 = t.n + quarter * QCOLS;               // and column
+      const bool mine = quarter * QCOLS < t.bn && (MODE != kCeLse || r0 < taken);
+      const bool live = row < taken;
       int tgt = -1;
       float lse2 = 0.0f, gs = 0.0f;
-      const bool any = MODE == kCeStore ? true : r0 < a.head->taken;
-      const bool live = row < a.head->taken;
       if (MODE != kCeStore && live) {
-        tgt = a.target[row];
+        if (a.targets) {  // unpacked rows
+          const int64_t g = a.targets[row];
+          tgt = g >= 0 && g < a.classes ? (int)g : -1;
+        } else {
+          tgt = a.target[row];
+        }
         if (MODE == kCeGrad) {
           lse2 = a.lse2[row];
           gs = a.gs[row];
         }
       }
-      const bool ok = mbar_wait(&tfull[group], (tn >> 1) & 1, s_abort, a.err, 34, WAIT_NS);
+      const bool ok = mbar_wait(&tfull[b], (tn >> 1) & 1, s_abort, a.err, 34, WAIT_NS);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      if (MODE == kCeLse) {
-        if (any) epi_lse(a, taddr, t.n, row, live, tgt, t.n / kCeN);
-      } else if (MODE == kCeGrad) {
-        // g = (2^(c2 z - lse2) - [target]) gs in 16 bits; zeros past the last
-        // class and in the tail rows, which the products read.
-        const int cols = min(kCeN, a.vn - t.n);
-        tgt -= a.v0 + t.n;
-        float v[2][32];
-        if (any) tmem_ld_issue(taddr, v[0]);
-#pragma unroll
-        for (int c = 0; c < kCeN / 32; c++) {
-          float(&w)[32] = v[c & 1];
-          if (any) {
-            tmem_wait(w);
-            if (c + 1 < kCeN / 32) tmem_ld_issue(taddr + (c + 1) * 32, v[(c + 1) & 1]);
-#pragma unroll
-            for (int j = 0; j < 32; j++) w[j] = ex2(fmaf(w[j], a.c2, -lse2));
-            const int at = tgt - c * 32;
-            if (at >= 0 && at < 32) {
-#pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (j == at) w[j] -= 1.0f;
-            }
-#pragma unroll
-            for (int j = 0; j < 32; j++) w[j] *= gs;
-            if (!live) {
-#pragma unroll
-              for (int j = 0; j < 32; j++) w[j] = 0.0f;
-            }
-            if (cols - c * 32 < 32) {
-#pragma unroll
-              for (int j = 0; j < 32; j++)
-                if (j >= cols - c * 32) w[j] = 0.0f;
-            }
-          } else {
-#pragma unroll
-            for (int j = 0; j < 32; j++) w[j] = 0.0f;
-          }
-          uint8_t* to = stg + (puts & 1) * STG;
-          if ((c & 1) == 0) stage_ready(lane);
-#pragma unroll
-          for (int q = 0; q < 4; q++)
-            stage_put(to, lane, (c & 1) * 4 + q,
-                      make_uint4(pack2<F16>(w[8 * q], w[8 * q + 1]), pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
-                                 pack2<F16>(w[8 * q + 4], w[8 * q + 5]), pack2<F16>(w[8 * q + 6], w[8 * q + 7])));
-          if (c & 1) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              tma_store_2d(&maps.g_out, to, t.n + (c - 1) * 32, r0);
-              bulk_commit();
-            }
-            puts++;
-          }
-        }
-      } else {
-        const CeJob& j = t.job ? a.dw : a.dx;
-        const bool none = t.kb0 == t.kb1;
-        const bool f32 = j.f32_rows > 0;
-        const CUtensorMap* out = t.job ? &maps.dw_out : &maps.dx_out;
-        // rows of the f32 result are never past its end: whole tiles
-        const int y = f32 ? t.split * j.f32_rows + r0 : j.row0 + r0;
-        const float f = a.head->grad_scale;
-        for (int c = 0; c < t.bn / 32; c++) {
-          float w[32];
-          if (none) {
-#pragma unroll
-            for (int i = 0; i < 32; i++) w[i] = 0.0f;
-          } else {
-            tmem_ld_issue(taddr + c * 32, w);
-            tmem_wait(w);
-          }
-          if (t.n + c * 32 >= a.d) {
-            if (f32 || (c & 1) == 0) break;  // past the last column; a 16-bit tile half written still goes out
-          }
-          uint8_t* to = stg + (puts & 1) * STG;
-          if (f32) {
-            stage_ready(lane);
-#pragma unroll
-            for (int q = 0; q < 8; q++)
-              stage_put(to, lane, q,
-                        make_uint4(__float_as_uint(w[4 * q]), __float_as_uint(w[4 * q + 1]),
-                                   __float_as_uint(w[4 * q + 2]), __float_as_uint(w[4 * q + 3])));
-          } else {
-            if ((c & 1) == 0) stage_ready(lane);
-#pragma unroll
-            for (int i = 0; i < 32; i++) w[i] *= f;
-#pragma unroll
-            for (int q = 0; q < 4; q++)
-              stage_put(to, lane, (c & 1) * 4 + q,
-                        make_uint4(pack2<F16>(w[8 * q], w[8 * q + 1]), pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
-                                   pack2<F16>(w[8 * q + 4], w[8 * q + 5]), pack2<F16>(w[8 * q + 6], w[8 * q + 7])));
-          }
-          if (f32 || (c & 1)) {
-            fence_async_smem();
-            __syncwarp();
-            if (lane == 0) {
-              if (!f32)
-                tma_store_2d(out, to, t.n + (c - 1) * 32, y);
-              else if (j.add)
-                tma_add_2d(out, to, t.n + c * 32, y);
-              else
-                tma_store_2d(out, to, t.n + c * 32, y);
-              bulk_commit();
-            }
-            puts++;
-          }
-        }
-      }
+      float w[QCOLS];
+      if (mine) tmem_ld64(tmem + lanes + b * 256 + quarter * QCOLS, w);
+      // The columns are in registers: hand the accumulator back.
       tc_fence_before();
       __syncwarp();
       if (lane == 0) {
         if (lead)
-          mbar_arrive(&tempty[group]);
+          mbar_arrive(&tempty[b]);
         else
-          mbar_arrive_cluster(mapa_shared(&tempty[group], 0));
+          mbar_arrive_cluster(mapa_shared(&tempty[b], 0));
+      }
+      if (!mine) continue;
+      if (MODE == kCeLse) {
+        epi_lse(a, w, n0, row, live, tgt);
+      } else if (MODE == kCeGrad) {
+        // g = (2^(c2 z - lse2) - [target]) gs in 16 bits; zeros past the last
+        // class and in the tail rows, which the products read.
+        const int cols = a.vn - n0;
+#pragma unroll
+        for (int j = 0; j < QCOLS; j++) w[j] = ex2(fmaf(w[j], a.c2, -lse2));
+        const int at = tgt - a.v0 - n0;
+        if (at >= 0 && at < QCOLS) {
+#pragma unroll
+          for (int j = 0; j < QCOLS; j++)
+            if (j == at) w[j] -= 1.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < QCOLS; j++) w[j] *= gs;
+        if (cols < QCOLS || !live) {
+#pragma unroll
+          for (int j = 0; j < QCOLS; j++)
+            if (!live || j >= cols) w[j] = 0.0f;
+        }
+        stage_ready(lane);
+        stage_row16<F16>(stg, lane, w);
+        fence_async_smem();
+        __syncwarp();
+        if (lane == 0) {
+          tma_store_2d(&maps.g_out, stg, n0, r0);
+          bulk_commit();
+        }
+      } else {
+        const CeJob& j = t.job ? a.dw : a.dx;
+        const CUtensorMap* out = t.job ? &maps.dw_out : &maps.dx_out;
+        if (n0 >= a.d) continue;  // past the last column
+        if (t.kb0 == t.kb1) {
+#pragma unroll
+          for (int i = 0; i < QCOLS; i++) w[i] = 0.0f;
+        }
+        if (j.f32_rows > 0) {
+          // whole tiles of rows: never past the end of the split's result
+          const int y = t.split * j.f32_rows + r0;
+#pragma unroll
+          for (int h = 0; h < 2; h++) {
+            if (n0 + h * 32 >= a.d) break;
+            stage_ready(lane);
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              stage_put(stg, lane, q,
+                        make_uint4(__float_as_uint(w[32 * h + 4 * q]), __float_as_uint(w[32 * h + 4 * q + 1]),
+                                   __float_as_uint(w[32 * h + 4 * q + 2]), __float_as_uint(w[32 * h + 4 * q + 3])));
+            fence_async_smem();
+            __syncwarp();
+            if (lane == 0) {
+              if (j.add)
+                tma_add_2d(out, stg, n0 + h * 32, y);
+              else
+                tma_store_2d(out, stg, n0 + h * 32, y);
+              bulk_commit();
+            }
+          }
+        } else {
+          const float f = a.head->grad_scale;
+#pragma unroll
+          for (int i = 0; i < QCOLS; i++) w[i] *= f;
+          stage_ready(lane);
+          stage_row16<F16>(stg, lane, w);
+          fence_async_smem();
+          __syncwarp();
+          if (!j.out) {
+            if (lane == 0) {
+              tma_store_2d(out, stg, n0, j.row0 + r0);
+              bulk_commit();
+            }
+          } else {
+            // Rows that TMA cannot address: the warp stores them one by one,
+            // two elements a lane.
+            const int64_t left = a.classes - (j.row0 + (int64_t)r0);
+            uint16_t* o = j.out + (j.row0 + (int64_t)r0) * j.out_stride + n0;
+            const int cols = a.d - n0;
+            for (int r = 0; r < 32 && r < left; r++, o += j.out_stride) {
+#pragma unroll
+              for (int h = 0; h < 2; h++) {
+                const int c = lane + 32 * h;
+                if (c < cols) o[c] = *reinterpret_cast<uint16_t*>(stg + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | (c & 7) << 1));
+              }
+            }
+            __syncwarp();
+          }
+        }
       }
     }
     if (MODE != kCeLse && lane == 0) bulk_wait_all();  // shared memory is read until then
@@ -555,8 +547,7 @@ int launch(const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t
   int pairs = 0;
   VRS_TRY((pairs_of<MODE, F16>(&pairs)));
   const int64_t n = most_tiles < pairs ? most_tiles : pairs;
-  ce_gemm_kernel<MODE, F16><<<(unsigned)(2 * (n < 1 ? 1 : n)), THREADS, smem_bytes(MODE), s>>>(maps, a);
-  VRS_CUDA(cudaGetLastError());
+  VRS_TRY(launch_after(ce_gemm_kernel<MODE, F16>, (unsigned)(2 * (n < 1 ? 1 : n)), THREADS, smem_bytes(MODE), s, maps, a));
   count_launch();
   return VRS_OK;
 }

@@ -37,31 +37,106 @@ __device__ __forceinline__ Pack<T, VEC> load_pack(const T* p) {
   return *reinterpret_cast<const Pack<T, VEC>*>(p);
 }
 
+__device__ __forceinline__ void round_pair(f16* o, float lo, float hi) {
+  *reinterpret_cast<__half2*>(o) = __floats2half2_rn(lo, hi);
+}
+__device__ __forceinline__ void round_pair(bf16* o, float lo, float hi) {
+  *reinterpret_cast<__nv_bfloat162*>(o) = __floats2bfloat162_rn(lo, hi);
+}
+__device__ __forceinline__ void round_pair(float* o, float lo, float hi) {
+  o[0] = lo;
+  o[1] = hi;
+}
+
 template <class T, int VEC>
 __device__ __forceinline__ void store_pack(T* p, const float* v) {
   Pack<T, VEC> o;
+  if constexpr (VEC == 1) {
+    o.v[0] = from_f32<T>(v[0]);
+  } else {
 #pragma unroll
-  for (int j = 0; j < VEC; j++) o.v[j] = from_f32<T>(v[j]);
+    for (int j = 0; j < VEC; j += 2) round_pair(o.v + j, v[j], v[j + 1]);
+  }
   *reinterpret_cast<Pack<T, VEC>*>(p) = o;
 }
 
-// VEC parameters (weights or biases) in 32 bits; a 32-bit parameter array
-// beside 16-bit rows takes two 16-byte loads.
-template <class P, int VEC>
-__device__ __forceinline__ void load_params(const P* p, float* out) {
-  if constexpr (sizeof(P) * VEC > 16) {
-    constexpr int H = 16 / sizeof(P);
+// ---- pairs of floats: sm_100 multiplies and adds two at once (f32x2), which
+// halves the instructions of kernels that are short of issue slots.
+struct F2 {
+  unsigned long long u;
+};
+__device__ __forceinline__ F2 pack_f2(float lo, float hi) {
+  F2 r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.u) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ F2 pack_f2(float v) { return pack_f2(v, v); }
+__device__ __forceinline__ void unpack_f2(F2 a, float& lo, float& hi) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(a.u));
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+  F2 r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.u) : "l"(a.u), "l"(b.u), "l"(c.u));
+  return r;
+}
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+  F2 r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.u) : "l"(a.u), "l"(b.u));
+  return r;
+}
+__device__ __forceinline__ float sum_f2(F2 a) {
+  float lo, hi;
+  unpack_f2(a, lo, hi);
+  return lo + hi;
+}
+
+// E elements of a row or of a parameter array in a thread's registers, in
+// their own type, as NV accesses of VEC.
+template <class T, int E, int VEC>
+struct Held {
+  static constexpr int NV = E / VEC;
+  static_assert(VEC * sizeof(T) <= 16 || VEC * sizeof(T) == 32, "one or two 16-byte accesses");
+  Pack<T, VEC> k[NV];
+  __device__ __forceinline__ void fill(float f) {
+#pragma unroll
+    for (int i = 0; i < NV; i++)
+#pragma unroll
+      for (int j = 0; j < VEC; j++) k[i].v[j] = from_f32<T>(f);
+  }
+  // 32-bit parameters beside 16-bit rows: a pack of 8 takes two accesses.
+  __device__ __forceinline__ void load(int i, const T* p) {
+    constexpr int H = sizeof(T) * VEC > 16 ? 16 / (int)sizeof(T) : VEC;
 #pragma unroll
     for (int h = 0; h < VEC / H; h++) {
-      const Pack<P, H> k = load_pack<P, H>(p + h * H);
+      const Pack<T, H> q = load_pack<T, H>(p + h * H);
 #pragma unroll
-      for (int j = 0; j < H; j++) out[h * H + j] = to_f32(k.v[j]);
+      for (int j = 0; j < H; j++) k[i].v[h * H + j] = q.v[j];
     }
-  } else {
-    const Pack<P, VEC> k = load_pack<P, VEC>(p);
-#pragma unroll
-    for (int j = 0; j < VEC; j++) out[j] = to_f32(k.v[j]);
   }
+  // Elements 2q and 2q + 1 as floats.
+  __device__ __forceinline__ F2 pair(int q) const {
+    return pack_f2(to_f32(k[2 * q / VEC].v[2 * q % VEC]), to_f32(k[(2 * q + 1) / VEC].v[(2 * q + 1) % VEC]));
+  }
+};
+
+// Stores a pair-wise row: VEC elements at access i.
+template <class T, int VEC, int E>
+__device__ __forceinline__ void store_held(T* p, const F2 (&v)[E / 2], int i) {
+  float f[VEC];
+  if constexpr (VEC == 1) {
+    float lo, hi;
+    unpack_f2(v[i / 2], lo, hi);
+    f[0] = i & 1 ? hi : lo;
+  } else {
+#pragma unroll
+    for (int j = 0; j < VEC; j += 2) unpack_f2(v[(i * VEC + j) / 2], f[j], f[j + 1]);
+  }
+  store_pack<T, VEC>(p, f);
 }
 
 inline int dtype_bytes(int dtype) { return dtype == VRS_F32 ? 4 : 2; }

@@ -31,28 +31,29 @@ def _rows(t: torch.Tensor, name: str, d: Optional[int] = None) -> Tuple[torch.Te
         raise ValueError(f"{name} must be a CUDA tensor (there is no CPU fallback)")
     if t.dim() < 1 or t.dtype not in _DTYPES:
         raise ValueError(f"{name} must have rows of float32, float16 or bfloat16, got {t.dtype}")
-    if d is not None and t.shape[-1] != d:
-        raise ValueError(f"{name} has rows of {t.shape[-1]} elements, expected {d}")
-    d = t.shape[-1]
-    if d < 1:
+    have = t.shape[-1]
+    if d is not None and have != d:
+        raise ValueError(f"{name} has rows of {have} elements, expected {d}")
+    if have < 1:
         raise ValueError(f"{name} has rows of no elements")
     if t.dim() != 2:
-        t = t.reshape(-1, d)
-    n, stride = t.shape[0], t.stride(0)
-    if (d > 1 and t.stride(1) != 1) or (n > 1 and stride < d):
+        t = t.reshape(-1, have)
+    n = t.shape[0]
+    stride, one = t.stride()
+    if (have > 1 and one != 1) or (n > 1 and stride < have):
         t = t.contiguous()
-        stride = d
-    return t, n, max(stride, d)
+        stride = have
+    return t, n, stride if stride > have else have
 
 
-def _same(t: torch.Tensor, like: torch.Tensor, name: str, n: Optional[int] = None, dtype=None) -> torch.Tensor:
-    """A one-dimensional tensor beside `like`, contiguous."""
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
-    if n is not None and t.numel() != n:
-        raise ValueError(f"{name} holds {t.numel()} values, expected {n}")
-    if dtype is not None and t.dtype != dtype:
+def _same(t: torch.Tensor, like: torch.Tensor, name: str, n: int, dtype: torch.dtype) -> torch.Tensor:
+    """A tensor of n values beside `like`, contiguous."""
+    if t.dtype != dtype:
         raise ValueError(f"{name} must be {dtype}, got {t.dtype}")
+    if t.numel() != n:
+        raise ValueError(f"{name} holds {t.numel()} values, expected {n}")
+    if t.get_device() != like.get_device():
+        raise ValueError(f"{name} is on {t.device}, expected {like.device}")
     return t if t.is_contiguous() else t.contiguous()
 
 
@@ -64,44 +65,50 @@ def _params(weight, bias, x, d: int):
             if p.dtype != x.dtype and p.dtype != torch.float32:
                 raise ValueError(f"{name} must be {x.dtype} or float32, got {p.dtype}")
             pt = p.dtype
-    weight = None if weight is None else _same(weight, x, "weight", d, pt)
-    bias = None if bias is None else _same(bias, x, "bias", d, pt)
+    if weight is not None:
+        weight = _same(weight, x, "weight", d, pt)
+    if bias is not None:
+        bias = _same(bias, x, "bias", d, pt)
     return weight, bias, pt
+
+
+def _like(t: torch.Tensor, rows: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type (rows: t seen as rows)."""
+    return torch.empty_like(t) if t is rows and t.is_contiguous() else t.new_empty(t.shape)
+
+
+def _column(t: torch.Tensor, n: int) -> torch.Tensor:
+    """An f32 value for each of t's n rows."""
+    v = torch.empty(n, dtype=torch.float32, device=t.device)
+    return v if t.dim() == 2 else v.view(t.shape[:-1])
 
 
 def _p(t: Optional[torch.Tensor]):
     return None if t is None else t.data_ptr()
 
 
-class _On:
-    """The tensors' device made current, and its current stream."""
-
-    __slots__ = ("guard", "stream")
-
-    def __init__(self, t: torch.Tensor):
-        i = t.device.index
-        self.guard = torch.cuda.device(i) if i != torch.cuda.current_device() else None
-        self.stream = torch.cuda.current_stream(i).cuda_stream
-
-    def __enter__(self):
-        if self.guard is not None:
-            self.guard.__enter__()
-        return self.stream
-
-    def __exit__(self, *e):
-        if self.guard is not None:
-            self.guard.__exit__(*e)
+def _call(f, device: int, *args):
+    """f(*args, stream) on the device's current stream, with the device current."""
+    stream = torch.cuda.current_stream(device).cuda_stream
+    if device == torch.cuda.current_device():
+        status = f(*args, stream)
+    else:
+        with torch.cuda.device(device):
+            status = f(*args, stream)
+    if status:
+        _check(status)
 
 
 @functools.lru_cache(maxsize=1024)
 def _norm_workspace(device: int, rows: int, d: int) -> int:
     n = ctypes.c_int64(0)
-    _check(lib().vrs_layer_norm_backward_workspace(rows, d, ctypes.byref(n)))
+    with torch.cuda.device(device):
+        _check(lib().vrs_layer_norm_backward_workspace(rows, d, ctypes.byref(n)))
     return n.value
 
 
 @functools.lru_cache(maxsize=1024)
-def _loss_workspace(device: int, rows: int, classes: int, d: int, dtype: int, backward: bool, aligned: bool) -> int:
+def _loss_workspace(rows: int, classes: int, d: int, dtype: int, backward: bool, aligned: bool) -> int:
     n = ctypes.c_int64(0)
     _check(lib().vrs_linear_cross_entropy_workspace(rows, classes, d, dtype, int(backward), int(aligned),
                                                     ctypes.byref(n)))
@@ -115,17 +122,14 @@ def layer_norm_forward(x: torch.Tensor, weight: Optional[torch.Tensor] = None, b
                        eps: float = 1e-5) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
     """(y, mean, rstd): the norm of x's last dimension, y in x's type and
     shape, mean and rstd float32 of x's leading shape."""
-    shape = x.shape
     xr, n, xs = _rows(x, "x")
-    d = shape[-1]
+    d = xr.shape[1]
     weight, bias, pt = _params(weight, bias, xr, d)
-    y = torch.empty(shape, dtype=xr.dtype, device=xr.device)
-    stats = torch.empty((2, *shape[:-1]), dtype=torch.float32, device=xr.device)
-    mean, rstd = stats[0], stats[1]
-    with _On(xr) as stream:
-        _check(lib().vrs_layer_norm_forward(xr.data_ptr(), xs, n, d, _DTYPES[xr.dtype], _p(weight), _p(bias),
-                                            _DTYPES[pt], eps, y.data_ptr(), d, mean.data_ptr(), rstd.data_ptr(),
-                                            stream))
+    y = _like(x, xr)
+    mean = _column(x, n)
+    rstd = torch.empty_like(mean)
+    _call(lib().vrs_layer_norm_forward, xr.get_device(), xr.data_ptr(), xs, n, d, _DTYPES[xr.dtype], _p(weight),
+          _p(bias), _DTYPES[pt], eps, y.data_ptr(), d, mean.data_ptr(), rstd.data_ptr())
     return y, mean, rstd
 
 
@@ -134,11 +138,10 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
     """(dx, dweight, dbias) from the forward pass's mean and rstd; dweight and
     dbias in weight's type (param_dtype where there is no weight), or None
     each with params false."""
-    shape = x.shape
     xr, n, xs = _rows(x, "x")
-    d = shape[-1]
-    if dy.shape != shape or dy.dtype != xr.dtype or dy.device != xr.device:
-        raise ValueError(f"dy must be like x ({tuple(shape)}, {xr.dtype}), got {tuple(dy.shape)}, {dy.dtype}")
+    d = xr.shape[1]
+    if dy.shape != x.shape or dy.dtype != xr.dtype or dy.get_device() != xr.get_device():
+        raise ValueError(f"dy must be like x ({tuple(x.shape)}, {xr.dtype}), got {tuple(dy.shape)}, {dy.dtype}")
     yr, _, ys = _rows(dy, "dy", d)
     weight, _, pt = _params(weight, None, xr, d)
     if weight is None and param_dtype is not None:
@@ -147,15 +150,17 @@ def layer_norm_backward(dy: torch.Tensor, x: torch.Tensor, weight: Optional[torc
             raise ValueError(f"param_dtype must be {xr.dtype} or float32, got {pt}")
     mean = _same(mean, xr, "mean", n, torch.float32)
     rstd = _same(rstd, xr, "rstd", n, torch.float32)
-    dx = torch.empty(shape, dtype=xr.dtype, device=xr.device)
-    dw = torch.empty(d, dtype=pt, device=xr.device) if params else None
-    db = torch.empty(d, dtype=pt, device=xr.device) if params else None
-    with _On(xr) as stream:
-        need = _norm_workspace(xr.device.index, n, d) if params else 0
-        ws = torch.empty(need, dtype=torch.uint8, device=xr.device) if params else None
-        _check(lib().vrs_layer_norm_backward(yr.data_ptr(), ys, xr.data_ptr(), xs, n, d, _DTYPES[xr.dtype],
-                                             _p(weight), _DTYPES[pt], mean.data_ptr(), rstd.data_ptr(),
-                                             dx.data_ptr(), d, _p(dw), _p(db), _p(ws), need, stream))
+    device = xr.get_device()
+    dx = _like(x, xr)
+    dw = db = ws = None
+    need = 0
+    if params:
+        dw = torch.empty(d, dtype=pt, device=xr.device)
+        db = torch.empty_like(dw)
+        need = _norm_workspace(device, n, d)
+        ws = torch.empty(need, dtype=torch.uint8, device=xr.device)
+    _call(lib().vrs_layer_norm_backward, device, yr.data_ptr(), ys, xr.data_ptr(), xs, n, d, _DTYPES[xr.dtype],
+          _p(weight), _DTYPES[pt], mean.data_ptr(), rstd.data_ptr(), dx.data_ptr(), d, _p(dw), _p(db), _p(ws), need)
     return dx, dw, db
 
 
@@ -192,7 +197,7 @@ def _loss_args(x, table, targets, scale):
         raise ValueError(f"table must be classes x d, got {tuple(table.shape)}")
     d = xr.shape[1]
     tr, classes, ts = _rows(table, "table", d)
-    if tr.dtype != xr.dtype or tr.device != xr.device:
+    if tr.dtype != xr.dtype or tr.get_device() != xr.get_device():
         raise ValueError(f"table must be {xr.dtype} on {xr.device}, got {tr.dtype} on {tr.device}")
     if xr.dtype == torch.float32:
         raise ValueError("x and table must be float16 or bfloat16 (operands of the tensor cores)")
@@ -217,14 +222,12 @@ def linear_cross_entropy_forward(x: torch.Tensor, table: torch.Tensor, targets: 
     not a row of the table take no part: loss 0, lse 0."""
     xr, n, xs, tr, classes, ts, d, tg = _loss_args(x, table, targets, scale)
     dt = _DTYPES[xr.dtype]
-    out = torch.empty((2, *targets.shape), dtype=torch.float32, device=xr.device)
-    loss, lse = out[0], out[1]
-    with _On(xr) as stream:
-        need = _loss_workspace(xr.device.index, n, classes, d, dt, False, _aligned(tr, ts))
-        ws = torch.empty(need, dtype=torch.uint8, device=xr.device)
-        _check(lib().vrs_linear_cross_entropy_forward(xr.data_ptr(), xs, n, tr.data_ptr(), ts, classes, d, dt,
-                                                      tg.data_ptr(), scale, loss.data_ptr(), lse.data_ptr(),
-                                                      ws.data_ptr(), need, stream))
+    loss = _column(x, n)
+    lse = torch.empty_like(loss)
+    need = _loss_workspace(n, classes, d, dt, False, _aligned(tr, ts))
+    ws = torch.empty(need, dtype=torch.uint8, device=xr.device)
+    _call(lib().vrs_linear_cross_entropy_forward, xr.get_device(), xr.data_ptr(), xs, n, tr.data_ptr(), ts, classes, d,
+          dt, tg.data_ptr(), scale, loss.data_ptr(), lse.data_ptr(), ws.data_ptr(), need)
     return loss, lse
 
 
@@ -237,14 +240,13 @@ def linear_cross_entropy_backward(dloss: torch.Tensor, x: torch.Tensor, table: t
     dt = _DTYPES[xr.dtype]
     dloss = _same(dloss, xr, "dloss", n, torch.float32)
     lse = _same(lse, xr, "lse", n, torch.float32)
-    dx = torch.empty(x.shape, dtype=xr.dtype, device=xr.device) if need_dx else None
-    dtable = torch.empty((classes, d), dtype=tr.dtype, device=xr.device) if need_dtable else None
-    with _On(xr) as stream:
-        need = _loss_workspace(xr.device.index, n, classes, d, dt, True, _aligned(tr, ts) and d % 8 == 0)
-        ws = torch.empty(need, dtype=torch.uint8, device=xr.device)
-        _check(lib().vrs_linear_cross_entropy_backward(dloss.data_ptr(), xr.data_ptr(), xs, n, tr.data_ptr(), ts,
-                                                       classes, d, dt, tg.data_ptr(), scale, lse.data_ptr(), _p(dx),
-                                                       d, _p(dtable), d, ws.data_ptr(), need, stream))
+    dx = _like(x, xr) if need_dx else None
+    dtable = _like(table, tr) if need_dtable else None
+    need = _loss_workspace(n, classes, d, dt, True, _aligned(tr, ts))
+    ws = torch.empty(need, dtype=torch.uint8, device=xr.device)
+    _call(lib().vrs_linear_cross_entropy_backward, xr.get_device(), dloss.data_ptr(), xr.data_ptr(), xs, n,
+          tr.data_ptr(), ts, classes, d, dt, tg.data_ptr(), scale, lse.data_ptr(), _p(dx), d, _p(dtable), d,
+          ws.data_ptr(), need)
     return dx, dtable
 
 
