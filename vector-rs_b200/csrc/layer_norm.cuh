@@ -1,7 +1,7 @@
 // layer_norm.cuh -- what the layer norm's forward and backward kernels share:
 // the launch plan, the split of a row over threads, and its reductions.
 //
-// A row of d elements is held in registers by TPR threads (32 to 256) of a
+// A row of d elements is held in registers by TPR threads (4 to 256) of a
 // 256-thread block, or by a cluster of 2 to 8 blocks, E elements a thread, so
 // that it is read from memory once. Thread tt of a row's TT threads holds the
 // vectors i * TT + tt: neighbouring threads read neighbouring 16 bytes. Rows
@@ -9,6 +9,7 @@
 // the same kernels with one element per access.
 #pragma once
 #include <cooperative_groups.h>
+#include <cuda_pipeline_primitives.h>
 
 #include <atomic>
 
@@ -41,36 +42,59 @@ struct LnArgs {
   float eps;
 };
 
+// How a row is held, by its width.
+//   small    up to 256 elements: 4 to 32 threads, 8 elements each, two rows at
+//            a time (their loads and reductions overlap)
+//   narrow   up to 4,096: 32 to 256 threads, 16 elements each
+//   wide     up to 8,192, forward only (the backward pass holds five values an
+//            element): 256 threads, 32 elements each
+//   cluster  2 to 8 blocks, 16 elements a thread, or in the forward pass of
+//            many rows 32 (fewer blocks to a reduction over a cluster: 6,000 x
+//            16,384 in bf16 124 us with clusters of 2, 151 us with 4)
+enum LnClass : int { kLnSmall, kLnNarrow, kLnWide, kLnCluster, kLnWideCluster };
+constexpr int kSmallE = 8, kSmallRows = 2, kNarrowE = 16, kWideE = 32;
+
 struct LnPlan {
-  int tpr;      // threads of a row within a block (32..256)
+  LnClass cls;
+  int tpr;      // threads of a row within a block (4..256)
   int cluster;  // blocks of a row (1: none)
   bool vec;     // 16-byte accesses
-  bool wide;    // more elements a thread
   int blocks;   // grid, in clusters
 };
 
-// A thread holds `narrow` elements of a row of up to one block of them, else
-// `wide`, of rows_narrow or rows_wide rows at a time. The fewest threads that hold a row; a row wider than one block takes
-// a cluster, and so do rows so few that blocks alone would leave most SMs idle
-// (each thread still has at least one access).
-inline LnPlan ln_plan(int64_t rows, int d, int narrow, int wide, int rows_narrow, int rows_wide, int vec,
-                      bool can_vec, int sms, int narrow_blocks, int wide_blocks) {
+// The fewest threads that hold a row; a row wider than one block takes a
+// cluster, and so do rows so few that blocks alone would leave SMs idle (each
+// thread still has at least one access).
+inline LnPlan ln_plan(int64_t rows, int d, bool allow_wide, int vec, bool can_vec, int sms, int blocks_per_sm) {
   LnPlan p{};
   p.vec = can_vec;
   const int step = can_vec ? vec : 1;
-  p.wide = d > kLnThreads * narrow;
-  const int e = p.wide ? wide : narrow;
-  p.tpr = 32;
-  while (p.tpr < kLnThreads && p.tpr * e < d) p.tpr *= 2;
   p.cluster = 1;
-  if (p.tpr == kLnThreads) {
-    while (p.cluster < kLnMaxCluster && p.cluster * kLnThreads * wide < d) p.cluster *= 2;
-    while (p.cluster < kLnMaxCluster && rows * p.cluster * 2 <= sms && (int64_t)p.cluster * 2 * kLnThreads * step <= d)
-      p.cluster *= 2;
+  if (d <= 32 * kSmallE) {
+    p.cls = kLnSmall;
+    p.tpr = 4;
+    while (p.tpr * kSmallE < d) p.tpr *= 2;
+  } else if (d <= kLnThreads * kNarrowE) {
+    p.cls = kLnNarrow;
+    p.tpr = 32;
+    while (p.tpr * kNarrowE < d) p.tpr *= 2;
+  } else {
+    p.cls = kLnCluster;
+    p.tpr = kLnThreads;
+    while (p.cluster * kLnThreads * kNarrowE < d) p.cluster *= 2;
+    if (allow_wide && rows * p.cluster > sms) {
+      p.cluster /= 2;
+      p.cls = p.cluster > 1 ? kLnWideCluster : kLnWide;
+    }
   }
-  const int groups = kLnThreads / p.tpr * (p.wide || p.cluster > 1 ? rows_wide : rows_narrow);
-  const int64_t need = (rows + groups - 1) / groups;
-  const int64_t most = (int64_t)sms * (p.wide || p.cluster > 1 ? wide_blocks : narrow_blocks) / p.cluster;
+  if (p.tpr == kLnThreads && rows * p.cluster <= sms) {
+    while (p.cluster < kLnMaxCluster && rows * p.cluster <= sms && (int64_t)p.cluster * 2 * kLnThreads * step <= d)
+      p.cluster *= 2;
+    if (p.cluster > 1) p.cls = kLnCluster;
+  }
+  const int at_once = kLnThreads / p.tpr * (p.cls == kLnSmall ? kSmallRows : 1);
+  const int64_t need = (rows + at_once - 1) / at_once;
+  const int64_t most = (int64_t)sms * blocks_per_sm / p.cluster;
   p.blocks = (int)(need < most ? need : most);
   if (p.blocks < 1) p.blocks = 1;
   return p;
@@ -89,6 +113,13 @@ struct LnReduce {
     float cta[2][kLnMaxCluster][N];
   };
   __device__ static __forceinline__ void run(float (&v)[N], Smem* s, int slot) {
+    if constexpr (TPR < 32) {
+#pragma unroll
+      for (int o = TPR / 2; o > 0; o >>= 1)
+#pragma unroll
+        for (int n = 0; n < N; n++) v[n] += __shfl_xor_sync(0xffffffffu, v[n], o);
+      return;
+    }
     const int lane = threadIdx.x & 31;
     float k = v[0];
     if constexpr (N == 4) {
@@ -139,6 +170,88 @@ struct LnReduce {
   }
 };
 
+// A ring in shared memory for the rows a thread will hold next: asynchronous
+// 16-byte copies into slots of its own (nobody else reads them, so no barrier
+// is added), DEPTH - 1 turns ahead. R rows and ARRAYS arrays a turn; thread tt
+// of a row's TT holds the accesses i * TT + tt. Columns past the row's end are
+// zeros and stay so. Without 16-byte accesses rows are loaded when needed.
+template <class T, int VEC, int E, int R, int ARRAYS>
+struct LnRing {
+  static constexpr int NV = E / VEC;
+  static constexpr bool kAsync = VEC > 1;
+  static constexpr int kStage = R * ARRAYS * E * (int)sizeof(T) * kLnThreads;  // bytes of a turn
+  static constexpr int kDepth = kStage <= 16384 ? 3 : 2;
+  static constexpr int kBytes = kAsync ? kDepth * kStage : 0;
+
+  const T* base[ARRAYS];
+  int64_t stride[ARRAYS];
+  int64_t rows;
+  int64_t apart;  // rows between those of a turn; a turn is R times as long
+  int d, tt, TT, at;
+
+  __device__ __forceinline__ uint4* slot(int k, int r, int array, int i) const {
+    extern __shared__ uint4 s_ring[];
+    return &s_ring[(((k * R + r) * ARRAYS + array) * NV + i) * kLnThreads + threadIdx.x];
+  }
+  __device__ __forceinline__ void fetch(int64_t row, int k) const {
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int r = 0; r < R; r++) {
+        if (row + r * apart < rows) {
+#pragma unroll
+          for (int m = 0; m < ARRAYS; m++) {
+            const T* p = base[m] + (row + r * apart) * stride[m];
+#pragma unroll
+            for (int i = 0; i < NV; i++) {
+              const int c = (i * TT + tt) * VEC;
+              if (c < d) __pipeline_memcpy_async(slot(k, r, m, i), p + c, 16);
+            }
+          }
+        }
+      }
+      __pipeline_commit();
+    }
+  }
+  __device__ __forceinline__ void start(int64_t row) {
+    at = 0;
+    if constexpr (kAsync) {
+#pragma unroll
+      for (int i = 0; i < NV; i++)
+        if ((i * TT + tt) * VEC >= d)
+          for (int k = 0; k < kDepth * R * ARRAYS; k++)
+            *slot(k / (R * ARRAYS), k / ARRAYS % R, k % ARRAYS, i) = make_uint4(0, 0, 0, 0);
+      for (int k = 0; k < kDepth - 1; k++) fetch(row + k * R * apart, k);
+    }
+  }
+  // Starts the copies of a later turn and waits for those of `row`'s.
+  __device__ __forceinline__ void next(int64_t row) {
+    if constexpr (kAsync) {
+      fetch(row + (kDepth - 1) * R * apart, at == 0 ? kDepth - 1 : at - 1);
+      __pipeline_wait_prior(kDepth - 1);
+    }
+  }
+  __device__ __forceinline__ void done() { at = at + 1 == kDepth ? 0 : at + 1; }
+  // Row r of the turn at `row`; zeros past the last row.
+  __device__ __forceinline__ Held<T, E, VEC> get(int64_t row, int r, int m) const {
+    Held<T, E, VEC> h;
+    h.fill(0.0f);
+    if (row + r * apart < rows) {
+#pragma unroll
+      for (int i = 0; i < NV; i++) {
+        const int c = (i * TT + tt) * VEC;
+        if constexpr (kAsync)
+          h.k[i] = *reinterpret_cast<const Pack<T, VEC>*>(slot(at, r, m, i));
+        else if (c < d)
+          h.load(i, base[m] + (row + r * apart) * stride[m] + c);
+      }
+    }
+    return h;
+  }
+  __device__ __forceinline__ void drain() const {
+    if constexpr (kAsync) __pipeline_wait_prior(0);
+  }
+};
+
 template <class K>
 int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   auto kernel = K::get();
@@ -171,35 +284,43 @@ int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   return VRS_OK;
 }
 
-// The instantiation for a plan.
-template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE, class T, class P, int VEC>
+// The instantiation for a plan: K<T, P, VEC, TPR, E, R, CL>.
+template <template <class, class, int, int, int, int, bool> class K, bool WIDE, class T, class P, int VEC>
 int ln_dispatch_tpr(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  if (p.cluster > 1) return ln_launch<K<T, P, VEC, kLnThreads, WIDE, true>>(a, p, s);
-  if (p.wide) return ln_launch<K<T, P, VEC, kLnThreads, WIDE, false>>(a, p, s);
+  if (p.cls == kLnCluster) return ln_launch<K<T, P, VEC, kLnThreads, kNarrowE, 1, true>>(a, p, s);
+  if constexpr (WIDE) {
+    if (p.cls == kLnWideCluster) return ln_launch<K<T, P, VEC, kLnThreads, kWideE, 1, true>>(a, p, s);
+    if (p.cls == kLnWide) return ln_launch<K<T, P, VEC, kLnThreads, kWideE, 1, false>>(a, p, s);
+  }
+  if (p.cls == kLnSmall) switch (p.tpr) {
+      case 4: return ln_launch<K<T, P, VEC, 4, kSmallE, kSmallRows, false>>(a, p, s);
+      case 8: return ln_launch<K<T, P, VEC, 8, kSmallE, kSmallRows, false>>(a, p, s);
+      case 16: return ln_launch<K<T, P, VEC, 16, kSmallE, kSmallRows, false>>(a, p, s);
+      default: return ln_launch<K<T, P, VEC, 32, kSmallE, kSmallRows, false>>(a, p, s);
+    }
   switch (p.tpr) {
-    case 32: return ln_launch<K<T, P, VEC, 32, NARROW, false>>(a, p, s);
-    case 64: return ln_launch<K<T, P, VEC, 64, NARROW, false>>(a, p, s);
-    case 128: return ln_launch<K<T, P, VEC, 128, NARROW, false>>(a, p, s);
-    default: return ln_launch<K<T, P, VEC, 256, NARROW, false>>(a, p, s);
+    case 32: return ln_launch<K<T, P, VEC, 32, kNarrowE, 1, false>>(a, p, s);
+    case 64: return ln_launch<K<T, P, VEC, 64, kNarrowE, 1, false>>(a, p, s);
+    case 128: return ln_launch<K<T, P, VEC, 128, kNarrowE, 1, false>>(a, p, s);
+    default: return ln_launch<K<T, P, VEC, 256, kNarrowE, 1, false>>(a, p, s);
   }
 }
 
-template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE, class T, class P>
+template <template <class, class, int, int, int, int, bool> class K, bool WIDE, class T, class P>
 int ln_dispatch_vec(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
-  return p.vec ? ln_dispatch_tpr<K, NARROW, WIDE, T, P, 16 / (int)sizeof(T)>(a, p, s)
-               : ln_dispatch_tpr<K, NARROW, WIDE, T, P, 1>(a, p, s);
+  return p.vec ? ln_dispatch_tpr<K, WIDE, T, P, 16 / (int)sizeof(T)>(a, p, s) : ln_dispatch_tpr<K, WIDE, T, P, 1>(a, p, s);
 }
 
-template <template <class, class, int, int, int, bool> class K, int NARROW, int WIDE>
+template <template <class, class, int, int, int, int, bool> class K, bool WIDE>
 int ln_dispatch(int dtype, int param_dtype, const LnArgs& a, const LnPlan& p, cudaStream_t s) {
   switch (dtype) {
-    case VRS_F32: return ln_dispatch_vec<K, NARROW, WIDE, float, float>(a, p, s);
+    case VRS_F32: return ln_dispatch_vec<K, WIDE, float, float>(a, p, s);
     case VRS_F16:
-      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, NARROW, WIDE, f16, float>(a, p, s)
-                                    : ln_dispatch_vec<K, NARROW, WIDE, f16, f16>(a, p, s);
+      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, WIDE, f16, float>(a, p, s)
+                                    : ln_dispatch_vec<K, WIDE, f16, f16>(a, p, s);
     default:
-      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, NARROW, WIDE, bf16, float>(a, p, s)
-                                    : ln_dispatch_vec<K, NARROW, WIDE, bf16, bf16>(a, p, s);
+      return param_dtype == VRS_F32 ? ln_dispatch_vec<K, WIDE, bf16, float>(a, p, s)
+                                    : ln_dispatch_vec<K, WIDE, bf16, bf16>(a, p, s);
   }
 }
 

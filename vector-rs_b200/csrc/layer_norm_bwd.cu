@@ -10,41 +10,23 @@
 // kernel adds in block order, so the result does not depend on timing.
 //
 // The instructions come next after memory (33 an element in a first form kept
-// it at 4.2 TB/s): pairs of floats, and two rows to a reduction.
-//
-// A thread's loads of the next rows are in flight while it reduces the
-// current ones: asynchronous copies into slots of its own in shared memory
-// (nobody else reads them, so no barrier is added).
+// it at 4.2 TB/s): pairs of floats, and shuffles that halve the values.
 //
 // Few rows (at most kColumnRows): the blocks' sums would be as large as the
 // inputs. Further blocks of the same launch then sum the columns straight
 // from x and dy, which L2 still holds.
-#include <cuda_pipeline_primitives.h>
-
 #include "layer_norm.cuh"
 
 namespace vrs {
 namespace ops {
 namespace {
 
-// Elements a thread holds of each row it has at a time, and blocks an SM. 8
-// (two rows) leave room for 24 warps; 16 reach the widest rows with clusters
-// of 8.
-constexpr int kNarrow = 8, kWide = 16;
-constexpr int kNarrowRows = 2, kWideRows = 1;
-constexpr int kNarrowBlocks = 3, kWideBlocks = 2;
+// x, dy, the weight and two column sums an element: 16 elements a thread
+// leave room for two blocks an SM. (Measured at 65,536 x 2,048 in bf16: 144 us;
+// 8 elements, two rows a turn and three blocks 167 us, four blocks 209 us.)
+constexpr int kBlocksPerSm = 2;
 constexpr int64_t kColumnRows = 64;
 constexpr int kColumns = 64;  // of a column block; its 4 strips of threads split the rows
-
-// Asynchronous copies: bytes of a stage (the rows of one turn), and stages.
-template <class T, int E>
-constexpr int stage_bytes() {
-  return (E == kNarrow ? kNarrowRows : kWideRows) * 2 * E * (int)sizeof(T) * kLnThreads;
-}
-template <class T, int E>
-constexpr int stage_count() {
-  return stage_bytes<T, E>() <= 16384 ? 3 : 2;
-}
 
 template <class T, class P>
 __device__ void sum_columns(const LnArgs& a, int block, float (*s)[kColumns][2]) {
@@ -75,17 +57,16 @@ __device__ void sum_columns(const LnArgs& a, int block, float (*s)[kColumns][2])
   }
 }
 
-template <class T, class P, int VEC, int TPR, int E, bool CL>
-__global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWideBlocks)
+template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
+__global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
     ln_bwd_kernel(const LnArgs a) {
-  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR, R = E == kNarrow ? kNarrowRows : kWideRows;
-  constexpr bool ASYNC = VEC > 1;
-  constexpr int DEPTH = stage_count<T, E>();
+  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
+  using Ring = LnRing<T, VEC, E, R, 2>;
   using Red = LnReduce<TPR, CL, 2 * R>;
   __shared__ typename Red::Smem s_red;
-  constexpr int kColFloats = GROUPS > 1 ? 2 * TPR * E : kLnThreads * 2;
+  // Sums of the block's columns, or of a column block's strips.
+  constexpr int kColFloats = GROUPS > 1 && TPR * E > kLnThreads ? 2 * TPR * E : 2 * kLnThreads;
   __shared__ float s_col[kColFloats];
-  extern __shared__ uint4 s_row[];  // ASYNC: [DEPTH][R][2][NV][threads]
   int64_t first = blockIdx.x, step = gridDim.x - a.col_blocks;
   if (first >= step) {  // whole clusters
     sum_columns<T, P>(a, (int)(first - step), reinterpret_cast<float(*)[kColumns][2]>(s_col));
@@ -99,44 +80,20 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
     first /= cluster.num_blocks();
     step /= cluster.num_blocks();
   }
-  const T* x = (const T*)a.x;
-  const T* dy = (const T*)a.dy;
   T* dx = (T*)a.y;
   const float inv_d = 1.0f / (float)a.d;
-  const int64_t turn = step * (GROUPS * R);
-  const int64_t row0 = first * (GROUPS * R) + threadIdx.x / TPR;  // and every GROUPS-th after it
-
-  auto slot_of = [&](int at, int r, int which, int i) {
-    return &s_row[(((at * R + r) * 2 + which) * NV + i) * kLnThreads + threadIdx.x];
-  };
-  auto fetch = [&](int64_t row, int at) {
-    if constexpr (ASYNC) {
-#pragma unroll
-      for (int r = 0; r < R; r++) {
-        if (row + r * GROUPS < a.rows) {
-          const T* px = x + (row + r * GROUPS) * a.xs;
-          const T* py = dy + (row + r * GROUPS) * a.dys;
-#pragma unroll
-          for (int i = 0; i < NV; i++) {
-            const int c = (i * TT + tt) * VEC;
-            if (c < a.d) {
-              __pipeline_memcpy_async(slot_of(at, r, 0, i), px + c, 16);
-              __pipeline_memcpy_async(slot_of(at, r, 1, i), py + c, 16);
-            }
-          }
-        }
-      }
-      __pipeline_commit();
-    }
-  };
-  if constexpr (ASYNC) {
-    // Columns past the row's end are zeros and stay so.
-#pragma unroll
-    for (int i = 0; i < NV; i++)
-      if ((i * TT + tt) * VEC >= a.d)
-        for (int k = 0; k < DEPTH * R * 2; k++) *slot_of(k / (R * 2), k / 2 % R, k % 2, i) = make_uint4(0, 0, 0, 0);
-    for (int k = 0; k < DEPTH - 1; k++) fetch(row0 + k * turn, k);
-  }
+  const int64_t apart = step * GROUPS, row0 = first * GROUPS + threadIdx.x / TPR;
+  Ring ring;
+  ring.base[0] = (const T*)a.x;
+  ring.base[1] = (const T*)a.dy;
+  ring.stride[0] = a.xs;
+  ring.stride[1] = a.dys;
+  ring.rows = a.rows;
+  ring.apart = apart;
+  ring.d = a.d;
+  ring.tt = tt;
+  ring.TT = TT;
+  ring.start(row0);
 
   Held<P, E, VEC> w;
   w.fill(1.0f);
@@ -148,42 +105,34 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
   F2 dw[E / 2], db[E / 2];
 #pragma unroll
   for (int q = 0; q < E / 2; q++) dw[q] = db[q] = pack_f2(0.0f);
-  int slot = 0, at = 0;
+  // A turn's statistics are loaded a turn ahead.
+  float mean_next[R], rstd_next[R];
+  auto stats = [&](int64_t row) {
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+      const bool have = row + r * apart < a.rows;
+      mean_next[r] = have ? a.mean_in[row + r * apart] : 0.0f;
+      rstd_next[r] = have ? a.rstd_in[row + r * apart] : 0.0f;
+    }
+  };
+  stats(row0);
+  int slot = 0;
   // Every thread of a block takes the same number of turns; a row past the
   // last one is zeros (with dy = 0 it adds nothing to any sum).
-  for (int64_t row = row0, r0 = first * (GROUPS * R); r0 < a.rows; row += turn, r0 += turn) {
+  for (int64_t row = row0, r0 = first * GROUPS; r0 < a.rows; row += R * apart, r0 += R * apart) {
     float mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      const bool have = row + r * GROUPS < a.rows;
-      mean[r] = have ? a.mean_in[row + r * GROUPS] : 0.0f;
-      rstd[r] = have ? a.rstd_in[row + r * GROUPS] : 0.0f;
+      mean[r] = mean_next[r];
+      rstd[r] = rstd_next[r];
     }
-    if constexpr (ASYNC) {
-      fetch(row + (DEPTH - 1) * turn, at == 0 ? DEPTH - 1 : at - 1);
-      __pipeline_wait_prior(DEPTH - 1);
-    }
+    stats(row + R * apart);
+    ring.next(row);
     F2 xh[R][E / 2], g[R][E / 2];
     float s[2 * R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      const bool have = row + r * GROUPS < a.rows;
-      Held<T, E, VEC> kx, ky;
-      kx.fill(0.0f);
-      ky.fill(0.0f);
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = (i * TT + tt) * VEC;
-        if constexpr (ASYNC) {
-          if (have) {
-            kx.k[i] = *reinterpret_cast<const Pack<T, VEC>*>(slot_of(at, r, 0, i));
-            ky.k[i] = *reinterpret_cast<const Pack<T, VEC>*>(slot_of(at, r, 1, i));
-          }
-        } else if (have && c < a.d) {
-          kx.load(i, x + (row + r * GROUPS) * a.xs + c);
-          ky.load(i, dy + (row + r * GROUPS) * a.dys + c);
-        }
-      }
+      const Held<T, E, VEC> kx = ring.get(row, r, 0), ky = ring.get(row, r, 1);
       const F2 m = pack_f2(-mean[r]), f = pack_f2(rstd[r]);
       F2 s0 = pack_f2(0.0f), s1 = pack_f2(0.0f);
 #pragma unroll
@@ -199,23 +148,23 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
       s[2 * r] = sum_f2(s0);
       s[2 * r + 1] = sum_f2(s1);
     }
-    if constexpr (ASYNC) at = at + 1 == DEPTH ? 0 : at + 1;
+    ring.done();
     Red::run(s, &s_red, slot);
     slot ^= 1;
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      if (row + r * GROUPS >= a.rows) break;
+      if (row + r * apart >= a.rows) break;
       const F2 f = pack_f2(rstd[r]), m0 = pack_f2(-s[2 * r] * inv_d), m1 = pack_f2(-s[2 * r + 1] * inv_d);
 #pragma unroll
       for (int q = 0; q < E / 2; q++) g[r][q] = mul2(add2(g[r][q], fma2(xh[r][q], m1, m0)), f);
 #pragma unroll
       for (int i = 0; i < NV; i++) {
         const int c = (i * TT + tt) * VEC;
-        if (c < a.d) store_held<T, VEC, E>(dx + (row + r * GROUPS) * a.ys + c, g[r], i);
+        if (c < a.d) store_held<T, VEC, E>(dx + (row + r * apart) * a.ys + c, g[r], i);
       }
     }
   }
-  if constexpr (ASYNC) __pipeline_wait_prior(0);
+  ring.drain();
   if (a.partial) {
     float* out = a.partial + first * 2 * a.d;
     float fw[E], fb[E];
@@ -224,10 +173,21 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
       unpack_f2(dw[q], fw[2 * q], fw[2 * q + 1]);
       unpack_f2(db[q], fb[2 * q], fb[2 * q + 1]);
     }
+    if constexpr (TPR < 32) {
+#pragma unroll
+      for (int o = TPR; o < 32; o *= 2)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+          fw[e] += __shfl_xor_sync(0xffffffffu, fw[e], o);
+          fb[e] += __shfl_xor_sync(0xffffffffu, fb[e], o);
+        }
+    }
     if constexpr (GROUPS > 1) {
-      // The groups of a block add their sums in turn (always in this order).
-      for (int gr = 0; gr < GROUPS; gr++) {
-        if ((int)threadIdx.x / TPR == gr) {
+      // The groups of a block (warps, where a row takes less) add their sums
+      // in turn, always in this order.
+      constexpr int SPAN = TPR < 32 ? 32 : TPR;
+      for (int gr = 0; gr < kLnThreads / SPAN; gr++) {
+        if ((int)threadIdx.x / SPAN == gr && (int)threadIdx.x % SPAN < TPR) {
 #pragma unroll
           for (int e = 0; e < E; e++) {
             const int c = (e / VEC * TT + tt) * VEC + e % VEC;
@@ -258,14 +218,16 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
   if constexpr (CL) cooperative_groups::this_cluster().sync();
 }
 
-template <class T, class P, int VEC, int TPR, int E, bool CL>
+template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 struct BwdKernel {
-  static auto get() { return &ln_bwd_kernel<T, P, VEC, TPR, E, CL>; }
-  static int smem() { return VEC > 1 ? stage_count<T, E>() * stage_bytes<T, E>() : 0; }
+  static auto get() { return &ln_bwd_kernel<T, P, VEC, TPR, E, R, CL>; }
+  static int smem() {
+    return LnRing<T, VEC, E, R, 2>::kBytes;
+  }
 };
 
 LnPlan bwd_plan(int64_t rows, int d, int vec, bool can_vec, int sms) {
-  return ln_plan(rows, d, kNarrow, kWide, kNarrowRows, kWideRows, vec, can_vec, sms, kNarrowBlocks, kWideBlocks);
+  return ln_plan(rows, d, false, vec, can_vec, sms, kBlocksPerSm);
 }
 
 // dweight[c], dbias[c] = sum over blocks of partial[b][0 / 1][c]: 32 columns a
@@ -373,7 +335,7 @@ extern "C" int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const 
   a.ys = dx_stride;
   a.d = (int)d;
   ProfToken t = prof_begin("layer_norm_backward", s);
-  int st = ln_dispatch<BwdKernel, kNarrow, kWide>(dtype, param_dtype, a, p, s);
+  int st = ln_dispatch<BwdKernel, false>(dtype, param_dtype, a, p, s);
   if (st == VRS_OK && a.partial) {
     st = param_dtype == VRS_F32   ? launch_params<float>(a.partial, p.blocks, a.d, dweight, dbias, s)
          : param_dtype == VRS_F16 ? launch_params<f16>(a.partial, p.blocks, a.d, dweight, dbias, s)

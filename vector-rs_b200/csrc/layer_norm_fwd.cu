@@ -10,16 +10,14 @@ namespace vrs {
 namespace ops {
 namespace {
 
-// Elements a thread holds of each of kRows rows.
-constexpr int kNarrow = 16, kWide = 32;
-constexpr int kNarrowRows = 2, kWideRows = 1;
-constexpr int kNarrowBlocks = 3, kWideBlocks = 2;
+constexpr int blocks_per_sm(int e) { return e == kWideE ? 2 : 3; }
 
-template <class T, class P, int VEC, int TPR, int E, bool CL>
-__global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWideBlocks)
+template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
+__global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
     ln_fwd_kernel(const LnArgs a) {
-  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR, R = E == kNarrow ? kNarrowRows : kWideRows;
+  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
   using Red = LnReduce<TPR, CL, R>;
+  using Ring = LnRing<T, VEC, E, R, 1>;
   __shared__ typename Red::Smem s_red;
   int tt = threadIdx.x % TPR, TT = TPR;
   int64_t first = blockIdx.x, step = gridDim.x;
@@ -30,8 +28,17 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
     first /= cluster.num_blocks();
     step /= cluster.num_blocks();
   }
-  const T* x = (const T*)a.x;
   T* y = (T*)a.y;
+  const int64_t apart = step * GROUPS, row_first = first * GROUPS + threadIdx.x / TPR;
+  Ring ring;
+  ring.base[0] = (const T*)a.x;
+  ring.stride[0] = a.xs;
+  ring.rows = a.rows;
+  ring.apart = apart;
+  ring.d = a.d;
+  ring.tt = tt;
+  ring.TT = TT;
+  ring.start(row_first);
   const float inv_d = 1.0f / (float)a.d;
   // The parameters of the thread's columns stay in registers for all rows;
   // without them 1 and 0 give the same bits as leaving the steps out (but for
@@ -48,28 +55,19 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
   int slot = 0;
   // Every thread of a block takes the same number of turns (the barriers
   // inside the reductions); a group past the last row computes on zeros.
-  for (int64_t r0 = first * (GROUPS * R); r0 < a.rows; r0 += step * (GROUPS * R)) {
-    const int64_t row0 = r0 + threadIdx.x / TPR;  // and every GROUPS-th after it
-    Held<T, E, VEC> k[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-      const int64_t row = row0 + r * GROUPS;
-      k[r].fill(0.0f);
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = (i * TT + tt) * VEC;
-        if (row < a.rows && c < a.d) k[r].load(i, x + row * a.xs + c);
-      }
-    }
+  for (int64_t row0 = row_first, r0 = first * GROUPS; r0 < a.rows; row0 += R * apart, r0 += R * apart) {
+    ring.next(row0);
     F2 v[R][E / 2];
     float mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
+      const Held<T, E, VEC> k = ring.get(row0, r, 0);
       F2 s = pack_f2(0.0f);
 #pragma unroll
-      for (int q = 0; q < E / 2; q++) s = add2(s, v[r][q] = k[r].pair(q));
+      for (int q = 0; q < E / 2; q++) s = add2(s, v[r][q] = k.pair(q));
       mean[r] = sum_f2(s);
     }
+    ring.done();
     Red::run(mean, &s_red, slot);
     slot ^= 1;
 #pragma unroll
@@ -96,7 +94,7 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
     slot ^= 1;
 #pragma unroll
     for (int r = 0; r < R; r++) {
-      const int64_t row = row0 + r * GROUPS;
+      const int64_t row = row0 + r * apart;
       if (row >= a.rows) break;
       rstd[r] = 1.0f / sqrtf(fmaf(rstd[r], inv_d, a.eps));
       if (tt == 0) {
@@ -113,14 +111,17 @@ __global__ void __launch_bounds__(kLnThreads, E == kNarrow ? kNarrowBlocks : kWi
       }
     }
   }
+  ring.drain();
   // A block must not leave while another still writes its shared memory.
   if constexpr (CL) cooperative_groups::this_cluster().sync();
 }
 
-template <class T, class P, int VEC, int TPR, int E, bool CL>
+template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 struct FwdKernel {
-  static auto get() { return &ln_fwd_kernel<T, P, VEC, TPR, E, CL>; }
-  static int smem() { return 0; }
+  static auto get() { return &ln_fwd_kernel<T, P, VEC, TPR, E, R, CL>; }
+  static int smem() {
+    return LnRing<T, VEC, E, R, 1>::kBytes;
+  }
 };
 
 }  // namespace
@@ -182,11 +183,10 @@ extern "C" int vrs_layer_norm_forward(const void* x, int64_t x_stride, int64_t r
                        aligned16(y) && aligned16(weight) && aligned16(bias);
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  const LnPlan p = ln_plan(rows, (int)d, kNarrow, kWide, kNarrowRows, kWideRows, vec, can_vec, sms, kNarrowBlocks,
-                          kWideBlocks);
+  const LnPlan p = ln_plan(rows, (int)d, true, vec, can_vec, sms, blocks_per_sm(d > kLnThreads * kNarrowE ? kWideE : 0));
   cudaStream_t s = (cudaStream_t)cuda_stream;
   ProfToken t = prof_begin("layer_norm_forward", s);
-  const int st = ln_dispatch<FwdKernel, kNarrow, kWide>(dtype, param_dtype, a, p, s);
+  const int st = ln_dispatch<FwdKernel, true>(dtype, param_dtype, a, p, s);
   prof_end(t, s);
   return st;
 }

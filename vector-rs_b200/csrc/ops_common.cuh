@@ -95,6 +95,17 @@ __device__ __forceinline__ float sum_f2(F2 a) {
   return lo + hi;
 }
 
+// Two neighbouring elements as floats (a bf16 is the upper half of a float).
+__device__ __forceinline__ F2 pair_of(const float* p) { return pack_f2(p[0], p[1]); }
+__device__ __forceinline__ F2 pair_of(const f16* p) {
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(p));
+  return pack_f2(f.x, f.y);
+}
+__device__ __forceinline__ F2 pair_of(const bf16* p) {
+  const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+  return pack_f2(__uint_as_float(u << 16), __uint_as_float(u & 0xffff0000u));
+}
+
 // E elements of a row or of a parameter array in a thread's registers, in
 // their own type, as NV accesses of VEC.
 template <class T, int E, int VEC>
@@ -120,7 +131,10 @@ struct Held {
   }
   // Elements 2q and 2q + 1 as floats.
   __device__ __forceinline__ F2 pair(int q) const {
-    return pack_f2(to_f32(k[2 * q / VEC].v[2 * q % VEC]), to_f32(k[(2 * q + 1) / VEC].v[(2 * q + 1) % VEC]));
+    if constexpr (VEC > 1)
+      return pair_of(&k[2 * q / VEC].v[2 * q % VEC]);
+    else
+      return pack_f2(to_f32(k[2 * q].v[0]), to_f32(k[2 * q + 1].v[0]));
   }
 };
 
