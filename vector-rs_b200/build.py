@@ -3,17 +3,20 @@
     python vector-rs_b200/build.py [--force] [-v]
 
 Each csrc/*.cu is compiled by nvcc for sm_100a only into _build/, then
-linked with the static CUDA runtime and NCCL into lib/libvrs.so. The
+linked with the static CUDA runtime and NCCL into lib/libvrs.so. Where torch
+is installed, csrc/py_ops.cpp becomes python/vector_cuda/_ops.so. The
 generator (gen_kernels.cu) is compiled without FMA contraction on both the
 device and the host so its output is bit-identical everywhere.
 """
 from __future__ import annotations
 
 import argparse
+import importlib.util
 import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 
 PKG = os.path.dirname(os.path.abspath(__file__))
@@ -22,6 +25,9 @@ CSRC = os.path.join(PKG, "csrc")
 BUILD = os.path.join(PKG, "_build")
 LIBDIR = os.path.join(PKG, "lib")
 LIB = os.path.join(LIBDIR, "libvrs.so")
+# The torch side of vector_cuda.ops (built where torch is installed).
+OPS_SRC = os.path.join(CSRC, "py_ops.cpp")
+OPS = os.path.join(PKG, "python", "vector_cuda", "_ops.so")
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 COMMON = ["-O3", "-std=c++17", "-lineinfo", "--expt-relaxed-constexpr",
@@ -64,11 +70,38 @@ def _compile(src: str, force: bool, verbose: bool) -> str:
     return obj
 
 
+def build_ops(force: bool = False, verbose: bool = False) -> str | None:
+    """_ops.so against the installed torch's headers; None without torch."""
+    spec = importlib.util.find_spec("torch")
+    if spec is None or not spec.submodule_search_locations:
+        return None
+    torch = list(spec.submodule_search_locations)[0]
+    header = os.path.join(ROOT, "include", "vrs.h")
+    if (not force and os.path.exists(OPS)
+            and os.path.getmtime(OPS) >= max(os.path.getmtime(OPS_SRC), os.path.getmtime(header))):
+        return OPS
+    cuda = os.path.dirname(os.path.dirname(nvcc()))
+    inc = [os.path.join(ROOT, "include"), os.path.join(torch, "include"),
+           os.path.join(torch, "include", "torch", "csrc", "api", "include"),
+           os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
+    cmd = ["g++", "-O2", "-std=c++20", "-fPIC", "-shared", "-fvisibility=hidden", *[f"-isystem{i}" for i in inc],
+           OPS_SRC, "-o", OPS, "-L" + os.path.join(torch, "lib"), "-Wl,-rpath," + os.path.join(torch, "lib"),
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"g++ failed on py_ops.cpp:\n{r.stdout}\n{r.stderr}")
+    return OPS
+
+
 def build(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
     with ThreadPoolExecutor(max_workers=os.cpu_count() or 4) as ex:
+        ops = ex.submit(build_ops, force, verbose)
         objs = list(ex.map(lambda s: _compile(s, force, verbose), sources()))
+        ops.result()
     newest = max(os.path.getmtime(o) for o in objs)
     if force or not os.path.exists(LIB) or os.path.getmtime(LIB) < newest:
         cmd = [nvcc(), *ARCH, "-shared", "-o", LIB, *objs, "-cudart", "static", "-lnccl"]
