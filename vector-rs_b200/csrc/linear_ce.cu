@@ -126,7 +126,7 @@ __device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.lau
 template <bool BACK>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
   grid_launch();
-  grid_wait();  // the slab counts, where there are any
+  grid_wait();
   __shared__ int s[8][3];
   __shared__ int s_warp[8];
   __shared__ int s_row[256];
@@ -228,33 +228,27 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
   }
 }
 
-// A table whose rows TMA cannot address, copied to rows of dp elements: 16
-// bytes out a thread, read as A elements at a time (the rows' alignment).
+// A table whose rows TMA cannot address, copied to rows of dp elements: two
+// elements a lane and turn, read by A at a time (the rows' alignment), or four.
 template <int A>
 __global__ void __launch_bounds__(256) ce_copy_table_kernel(const uint16_t* __restrict__ w, int64_t ws, int64_t classes,
                                                            int d, int dp, uint16_t* out) {
   grid_launch();  // reads inputs and writes what only the products read: nothing to wait for
-  const int chunks = dp / 8, lane = threadIdx.x & 31;
+  constexpr int N = A < 2 ? 2 : A;
+  const int lane = threadIdx.x & 31;
   for (int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); v < classes; v += (int64_t)gridDim.x * 8) {
     const uint16_t* from = w + v * ws;
-    uint4* to = reinterpret_cast<uint4*>(out + v * dp);
-#pragma unroll 2
-    for (int c = lane; c < chunks; c += 32) {
-      Pack<uint16_t, 8> q;
+    uint16_t* to = out + v * dp;
+#pragma unroll 8
+    for (int e = lane * N; e < dp; e += 32 * N) {
+      Pack<uint16_t, N> k;
+      if (A > 1 && e + N <= d) {
+        k = load_pack<uint16_t, N>(from + e);
+      } else {
 #pragma unroll
-      for (int j = 0; j < 8; j += A) {
-        const int e = c * 8 + j;
-        Pack<uint16_t, A> k;
-        if (e + A <= d) {
-          k = load_pack<uint16_t, A>(from + e);
-        } else {
-#pragma unroll
-          for (int i = 0; i < A; i++) k.v[i] = e + i < d ? from[e + i] : 0;
-        }
-#pragma unroll
-        for (int i = 0; i < A; i++) q.v[j + i] = k.v[i];
+        for (int i = 0; i < N; i++) k.v[i] = e + i < d ? from[e + i] : 0;
       }
-      to[c] = *reinterpret_cast<uint4*>(&q);
+      *reinterpret_cast<Pack<uint16_t, N>*>(to + e) = k;
     }
   }
 }
@@ -278,52 +272,52 @@ int copy_table(const void* table, int64_t ts, int64_t classes, int d, int dp, vo
 
 // --------------------------------------------------------- combine, finish
 
-// loss and lse of a row from its class tiles' maxima and sums, all in units
-// of log 2. The target's score is subtracted before the logarithm is added:
-// where the target is the largest score the difference is exact. 32 or 128
-// threads a row.
-template <int TPR>
-__global__ void __launch_bounds__(128) ce_combine_kernel(const CeGemm a, const int* __restrict__ index, float* loss,
-                                                        float* lse) {
-  __shared__ float s[4][2];
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// (maximum, sum of powers of two below it) of two sets.
+__device__ __forceinline__ float2 merge(float2 a, float2 b) {
+  const float m = fmaxf(a.x, b.x), sub = m == -INFINITY ? 0.0f : m;
+  return make_float2(m, a.y * ex2(a.x - sub) + b.y * ex2(b.x - sub));
+}
+
+// loss and lse of rows from their parts' maxima and sums, in units of log 2.
+// The target's score is subtracted before the logarithm is added: where the
+// target is the largest score the difference is exact. A block takes R rows
+// (a power of two up to 32), 1024 / R threads each; the parts lie row by row.
+__global__ void __launch_bounds__(1024)
+    ce_combine_kernel(const CeGemm a, int R, const int* __restrict__ index, float* loss, float* lse) {
+  __shared__ float2 s[1024];
   grid_wait();
-  const int64_t r = (int64_t)blockIdx.x * (128 / TPR) + threadIdx.x / TPR;
-  if (r >= (a.rows >= 0 ? a.rows : a.head->taken)) return;  // the whole row's threads
-  const int t = threadIdx.x % TPR;
-  const float2* p = a.part + r * a.parts;
-  float top = -INFINITY, sum = 0.0f;
-#pragma unroll 4
-  for (int i = t; i < a.parts; i += TPR) {
-    const float2 q = p[i];
-    const float m = fmaxf(top, q.x), sub = m == -INFINITY ? 0.0f : m;
-    sum = sum * exp2f(top - sub) + q.y * exp2f(q.x - sub);
-    top = m;
+  const int taken = a.rows >= 0 ? a.rows : a.head->taken;
+  const int64_t r0 = (int64_t)blockIdx.x * R;
+  if (r0 >= taken) return;
+  const int64_t row = r0 + threadIdx.x % R;
+  const int strips = 1024 / R;
+  float2 v = make_float2(-INFINITY, 0.0f);
+  if (row < taken) {
+    const float2* p = a.part + row;
+#pragma unroll 8
+    for (int i = threadIdx.x / R; i < a.parts; i += strips) v = merge(v, p[i * a.part_rows]);
   }
+  s[threadIdx.x] = v;
+  __syncthreads();
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;  // a warp a row
+  if (w >= R || r0 + w >= taken) return;
+  v = make_float2(-INFINITY, 0.0f);
+  for (int k = lane; k < strips; k += 32) v = merge(v, s[k * R + w]);
 #pragma unroll
-  for (int o = 16; o; o >>= 1) {
-    const float qx = __shfl_xor_sync(~0u, top, o), qy = __shfl_xor_sync(~0u, sum, o);
-    const float m = fmaxf(top, qx), sub = m == -INFINITY ? 0.0f : m;
-    sum = sum * exp2f(top - sub) + qy * exp2f(qx - sub);
-    top = m;
-  }
-  if constexpr (TPR == 128) {
-    if ((threadIdx.x & 31) == 0) {
-      s[threadIdx.x >> 5][0] = top;
-      s[threadIdx.x >> 5][1] = sum;
-    }
-    __syncthreads();
-    top = fmaxf(fmaxf(s[0][0], s[1][0]), fmaxf(s[2][0], s[3][0]));
-    const float sub = top == -INFINITY ? 0.0f : top;
-    sum = 0.0f;
-#pragma unroll
-    for (int w = 0; w < 4; w++) sum += s[w][1] * exp2f(s[w][0] - sub);
-  }
-  if (t == 0) {
-    const float l = log2f(sum);
-    const int64_t row = index ? index[r] : r;
+  for (int o = 16; o; o >>= 1) v = merge(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
+  if (lane == 0) {
+    const int64_t r = r0 + w;
+    const float l = log2f(v.y);
+    const int64_t at = index ? index[r] : r;
     const bool in = index || (a.targets[r] >= 0 && a.targets[r] < a.classes);
-    lse[row] = in ? (top + l) * kLn2 : 0.0f;
-    loss[row] = in ? ((top - a.zt[r]) + l) * kLn2 : 0.0f;
+    lse[at] = in ? (v.x + l) * kLn2 : 0.0f;
+    loss[at] = in ? ((v.x - a.zt[r]) + l) * kLn2 : 0.0f;
   }
 }
 
@@ -384,10 +378,37 @@ struct Plan {
   int64_t rows_p, dp, d4;         // rows in whole tiles, row pitches
   int64_t piece;                  // classes of a piece, whole tiles
   int64_t vtiles;                 // class tiles in all
-  int64_t parts;                  // and parts of 64 classes
+  int64_t parts;                  // and parts of 128 classes
   int splits_dx, splits_dw;
   int64_t head, slabs, index, pos, target, lse2, gs, xc, wc, part, zt, g, acc_dx, acc_dw, bytes;
 };
+
+// Class tiles of a piece: few pieces of one size, as many (up to twice the
+// fewest) as make the pairs' last turns fullest. A turn's length is that of its
+// longest tile; the products' tiles are counted as the kernel orders them.
+int64_t piece_of(int64_t rows_p, int64_t vtiles, int64_t ntiles) {
+  int64_t most = kPieceBytes / (rows_p * 2) / kCeN;
+  most = most < 1 ? 1 : most < vtiles ? most : vtiles;
+  const int64_t fewest = (vtiles + most - 1) / most, mt = rows_p / kCeM;
+  int64_t best = most;
+  double best_cost = 0.0;
+  for (int64_t n = fewest; n <= 2 * fewest && n <= vtiles && n < fewest + 16; n++) {
+    const int64_t vt = (vtiles + n - 1) / n;
+    const double grad = (double)((mt * vt + kPairs - 1) / kPairs);
+    // dx: mt * ntiles tiles of vt * 4 K blocks; dtable: vt * ntiles of mt * 4.
+    const double l = (double)(mt > vt ? mt : vt), s = (double)(mt > vt ? vt : mt);
+    const int64_t nl = (mt > vt ? vt : mt) * ntiles, ns = (mt > vt ? mt : vt) * ntiles;
+    const int64_t turns = nl / kPairs, rem = nl % kPairs;
+    const double left = (double)ns - (rem ? (double)(kPairs - rem) * std::floor(l / s + 0.5) : 0.0);
+    const double store = (double)(turns + (rem != 0)) * l + (left > 0 ? std::ceil(left / kPairs) * s : 0.0);
+    const double cost = (double)n * (grad * (double)ntiles + store + 2.0);
+    if (best_cost == 0.0 || cost < best_cost) {
+      best_cost = cost;
+      best = vt;
+    }
+  }
+  return best;
+}
 
 Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned) {
   Plan p{};
@@ -395,7 +416,7 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
   p.dp = up(d, 8);
   p.d4 = up(d, 4);
   p.vtiles = (classes + kCeN - 1) / kCeN;
-  p.parts = (classes + 63) / 64;
+  p.parts = (classes + 127) / 128;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
@@ -415,10 +436,7 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
     p.pos = take(rows * 4);
     p.lse2 = take(rows * 4);
     p.gs = take(rows * 4);
-    int64_t tiles = kPieceBytes / (p.rows_p * 2) / kCeN;
-    tiles = tiles < 1 ? 1 : tiles < p.vtiles ? tiles : p.vtiles;
-    const int64_t pieces = (p.vtiles + tiles - 1) / tiles;
-    p.piece = (p.vtiles + pieces - 1) / pieces * kCeN;  // pieces of one size
+    p.piece = piece_of(p.rows_p, p.vtiles, (d + kCeN - 1) / kCeN) * kCeN;
     p.g = take(p.rows_p * p.piece * 2);
     // Few tiles: K is split until the pairs have one each, 8 blocks deep at least.
     auto splits = [](int64_t tiles_, int64_t kblocks) {
@@ -565,11 +583,7 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
       k.per_block = (int)((c.rows + 2 * sms - 1) / (2 * sms));
     }
     const unsigned blocks = (unsigned)((c.rows + k.per_block - 1) / k.per_block);
-    if (back)
-      ce_pack_kernel<true><<<blocks, 256, 0, c.s>>>(k);
-    else
-      ce_pack_kernel<false><<<blocks, 256, 0, c.s>>>(k);
-    VRS_CUDA(cudaGetLastError());
+    VRS_TRY(launch_after(back ? ce_pack_kernel<true> : ce_pack_kernel<false>, blocks, 256, 0, c.s, k));
     count_launch();
   } else {
     a.targets = c.targets;
@@ -583,11 +597,12 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   }
   const bool f16 = c.dtype == VRS_F16;
   const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
-  if (packed)
-    VRS_TRY(make_map(&maps.x, type, 2, k.xc, c.d, c.rows, p.dp, 64));
-  else
-    VRS_TRY(make_map(&maps.x, type, 2, c.x, c.d, c.rows, c.xs, 64));
-  VRS_TRY(make_map(&maps.w, type, 2, w, c.d, c.classes, ts, 64));
+  // K-major loads of the rows take 128 of them (64 where there are no more),
+  // those of the table 64.
+  a.one_tile_rows = c.rows <= kCeM ? (int)c.rows : 0;
+  const int box = a.one_tile_rows && c.rows <= 64 ? 64 : 128;
+  VRS_TRY(make_map(&maps.a0, type, 2, packed ? k.xc : c.x, c.d, c.rows, packed ? p.dp : c.xs, box));
+  VRS_TRY(make_map(&maps.b0, type, 2, w, c.d, c.classes, ts, 64));
   a.head = k.head;
   a.err = err;
   a.classes = (int)c.classes;
@@ -595,7 +610,6 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   a.kblocks = (int)((c.d + kCeK - 1) / kCeK);
   // kind::f16, f32 accumulator, M = 256; operand types by bits 7 and 10.
   a.idesc = (1u << 4) | ((uint32_t)(kCeM >> 4) << 24) | (f16 ? 0u : (1u << 7) | (1u << 10));
-  a.one_tile_rows = c.rows <= kCeM ? (int)c.rows : 0;
   a.target = k.target;
   a.c2 = c.scale * kLog2e;
   return VRS_OK;
@@ -617,15 +631,15 @@ int forward(const Call& c, const Plan& p, float* loss, float* lse) {
   a.whole = (int)(c.rows <= kCeM && 2 * rest <= kPairs ? p.vtiles - rest : p.vtiles);
   a.vtiles = a.whole == p.vtiles ? a.whole : a.whole + (int)((c.classes - a.whole * (int64_t)kCeN + 127) / 128);
   a.parts = (int)p.parts;
+  a.part_rows = c.rows;
   a.part = (float2*)(c.ws + p.part);
   a.zt = (float*)(c.ws + p.zt);
   VRS_TRY(launch_ce_gemm(kCeLse, c.dtype == VRS_F16, maps, a, p.rows_p / kCeM * a.vtiles, c.s));
   const int* index = a.rows < 0 ? k.index : nullptr;
-  // 32 threads read a row's parts in a few turns, or 128 do.
-  if (p.parts <= 128)
-    VRS_TRY(launch_after(ce_combine_kernel<32>, (unsigned)((c.rows + 3) / 4), 128, 0, c.s, a, index, loss, lse));
-  else
-    VRS_TRY(launch_after(ce_combine_kernel<128>, (unsigned)c.rows, 128, 0, c.s, a, index, loss, lse));
+  // Up to 32 rows a block (whole lines of parts), fewer where blocks are few.
+  int R = 1;
+  while (R < 32 && R < c.rows && (R < 4 || c.rows > R * 256)) R *= 2;
+  VRS_TRY(launch_after(ce_combine_kernel, (unsigned)((c.rows + R - 1) / R), 1024, 0, c.s, a, R, index, loss, lse));
   count_launch();
   return VRS_OK;
 }
@@ -655,8 +669,12 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   a.gs = k.gs;
   float* acc_dx = (float*)(c.ws + p.acc_dx);
   float* acc_dw = (float*)(c.ws + p.acc_dw);
-  VRS_TRY(make_map(&maps.g, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 64));
-  VRS_TRY(make_map(&maps.g_out, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 32));
+  VRS_TRY(make_map(&maps.out0, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 32));
+  CeMaps prod;  // of the products
+  VRS_TRY(make_map(&prod.a0, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 128));
+  VRS_TRY(make_map(&prod.a1, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 64));
+  VRS_TRY(make_map(&prod.b1, type, 2, k.xc, c.d, c.rows, p.dp, 64));
+  prod.b0 = maps.b0;
   a.dx.on = dx != nullptr;
   a.dw.on = dtable != nullptr;
   a.dx.ntiles = a.dw.ntiles = (int)((c.d + kCeN - 1) / kCeN);
@@ -664,14 +682,14 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   a.dw.splits = p.splits_dw;
   a.dx.f32_rows = (int)p.rows_p;
   if (dx)
-    VRS_TRY(make_map(&maps.dx_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dx, c.d, p.splits_dx * p.rows_p, p.d4, 32));
+    VRS_TRY(make_map(&prod.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dx, c.d, p.splits_dx * p.rows_p, p.d4, 32));
   const bool direct = p.splits_dw == 1;
   if (dtable) {
     if (!direct) {
       a.dw.f32_rows = (int)p.piece;
-      VRS_TRY(make_map(&maps.dw_out, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dw, c.d, p.splits_dw * p.piece, p.d4, 32));
+      VRS_TRY(make_map(&prod.out1, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dw, c.d, p.splits_dw * p.piece, p.d4, 32));
     } else if (tma_rows(dtable, dts, c.classes)) {
-      VRS_TRY(make_map(&maps.dw_out, type, 2, dtable, c.d, c.classes, dts, 32));
+      VRS_TRY(make_map(&prod.out1, type, 2, dtable, c.d, c.classes, dts, 32));
     } else {
       a.dw.out = (uint16_t*)dtable;
       a.dw.out_stride = c.classes == 1 ? 0 : dts;
@@ -687,10 +705,9 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
     a.dx.add = v0 > 0;
     a.dw.mtiles = a.vtiles;
     a.dw.row0 = (int)v0;
-    a.dw_first = (c.rows + kCeK - 1) / kCeK / a.dw.splits > a.dx.kblocks / a.dx.splits;
     const int64_t tiles = (dx ? p.rows_p / kCeM * a.dx.ntiles * a.dx.splits : 0) +
                           (dtable ? (int64_t)a.dw.mtiles * a.dw.ntiles * a.dw.splits : 0);
-    VRS_TRY(launch_ce_gemm(kCeStore, f16, maps, a, tiles, c.s));
+    VRS_TRY(launch_ce_gemm(kCeStore, f16, prod, a, tiles, c.s));
     if (dtable && !direct)
       VRS_TRY(finish(f16, acc_dw, p.splits_dw, p.piece, p, c.d, vn, nullptr, a.head, (char*)dtable + v0 * dts * 2, dts,
                      c.s));

@@ -51,7 +51,7 @@ struct CeGemm {
   int d;
   int kblocks;       // of d
   int vtiles;        // class tiles of the piece
-  int parts;         // kCeLse: 64-class parts of a row
+  int parts;         // kCeLse: 128-class parts of a row
   uint32_t idesc;    // types; majorness and N are added per tile
   // scores
   const int64_t* targets;  // [rows] where the rows are not packed, else null
@@ -59,15 +59,17 @@ struct CeGemm {
   const float* lse2;   // [rows] lse * log2(e)
   const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
-  float2* part;        // [row][parts]: maximum of c2 z and sum of 2^(c2 z - maximum)
+  int64_t part_rows;
+  float2* part;        // [part][part_rows]: maximum of c2 z and sum of 2^(c2 z - maximum)
   float* zt;           // [row] c2 * target's score
   // products
   CeJob dx, dw;
-  int dw_first;        // dtable's tiles are the longer ones
 };
 
+// Tensor maps of a launch. Scores: a0 rows, b0 table, out0 their gradient.
+// Products: a0, b0, out0 of dx (A: the score gradients), a1, b1, out1 of dtable.
 struct CeMaps {
-  CUtensorMap x, w, g, g_out, dx_out, dw_out;
+  CUtensorMap a0, b0, out0, a1, b1, out1;
 };
 
 // A launch that may begin while the kernel before it on the stream ends; the

@@ -10,12 +10,11 @@
 // A pair owns a tile of 256 rows (128 a CTA: its TMEM lanes) by up to 256
 // columns; each CTA loads its half of both operands, 64 deep, into a ring of
 // stages. One thread of the even CTA issues M = 256 MMAs into one of two
-// accumulators (2 x 256 columns = all of TMEM). Sixteen epilogue warps a CTA
-// (TMEM lane quadrant x 64 columns) load a tile into registers and hand its
-// accumulator back at once, so a tile is exponentiated and stored while the
-// next two are multiplied. Results leave through swizzled staging tiles and
-// TMA stores, in f32 also as TMA additions to what earlier pieces of the
-// classes left.
+// accumulators (2 x 256 columns = all of TMEM). Two groups of epilogue warps a
+// CTA (TMEM lane quadrant x the tile's columns, or half of them) take alternate
+// tiles and read 32 columns ahead, so that one tile is exponentiated or stored
+// while the other accumulator is written. Results leave through swizzled staging tiles and TMA stores, in f32 also as
+// TMA additions to what earlier pieces of the classes left.
 //
 // Bound by the tensor cores for d of some hundreds and more; by the
 // exponentials for small d (one a score, 16 an SM and clock, against
@@ -31,21 +30,26 @@ namespace {
 
 using namespace vrs::tc;
 
-constexpr int EPI_FIRST = 4;          // producer, MMA, TMEM, spare
-constexpr int EPI_WARPS = 16;
-constexpr int THREADS = 32 * (EPI_FIRST + EPI_WARPS);
-constexpr int QCOLS = 64;             // columns of an epilogue warp
+constexpr int EPI_FIRST = 4;          // producer of A, MMA, TMEM, producer of B
+// Epilogue warps: the scores' exponentials keep 16 busy (1,024 x 300,000 x 128:
+// forward 121 us, with 8 of twice the columns 151 us); storing products takes 8.
+constexpr int epi_warps(int mode) { return mode == kCeStore ? 8 : 16; }
+constexpr int threads(int mode) { return 32 * (EPI_FIRST + epi_warps(mode)); }
+constexpr int CHUNK = 32;             // columns that an epilogue warp loads at a time
+constexpr int PART = 128;             // columns of one maximum and sum of the scores
+constexpr int kTileCost = 4;          // of a tile beside its K blocks, in K blocks
 constexpr uint32_t BOX = 64 * 128;    // bytes of a 64 x 64 tile of 16-bit operands
 constexpr uint32_t STAGE = 4 * BOX;   // a CTA's halves: A 128 x 64, B 128 x 64
 constexpr uint32_t STG = 32 * 128;    // a warp's staging tile: 32 rows of 128 bytes
 constexpr size_t SMEM_BAR = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;
 
-constexpr int stages(int mode) { return mode == kCeLse ? 7 : 5; }
+constexpr int stages(int mode) { return mode == kCeGrad ? 5 : 6; }
 constexpr size_t smem_bytes(int mode) {
-  return 1024 + (size_t)stages(mode) * STAGE + (mode == kCeLse ? 0 : EPI_WARPS * STG) + SMEM_BAR;
+  return 1024 + (size_t)stages(mode) * STAGE + (mode == kCeLse ? 0 : epi_warps(mode) * STG) + SMEM_BAR;
 }
-static_assert(smem_bytes(kCeLse) <= 232448 && smem_bytes(kCeGrad) <= 232448, "above the per-block limit");
+static_assert(smem_bytes(kCeLse) <= 232448 && smem_bytes(kCeGrad) <= 232448 && smem_bytes(kCeStore) <= 232448,
+              "above the per-block limit");
 
 // ------------------------------------------------------------ PTX wrappers
 
@@ -85,6 +89,31 @@ __device__ __forceinline__ float ex2(float x) {
   return r;
 }
 
+// 32 lanes x 32 columns; the values may be used only after tmem_wait.
+__device__ __forceinline__ void tmem_ld_issue(uint32_t taddr, float (&v)[CHUNK]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+// The values pass through the wait, so no use of them can move before it.
+__device__ __forceinline__ void tmem_wait(float (&v)[CHUNK]) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
@@ -111,17 +140,21 @@ struct Tile {
 // packing was needed.
 __device__ __forceinline__ int taken_rows(const CeGemm& a) { return a.rows >= 0 ? a.rows : a.head->taken; }
 
-// 64-row boxes of the A operand that a CTA loads in the score modes: with one
+// Bytes of the A operand that a CTA loads a stage in the score modes: with one
 // tile of rows, those that hold rows. The others are zeroed once.
-__device__ __forceinline__ int a_boxes(const CeGemm& a, int cta) {
-  return a.one_tile_rows ? max(0, min(2, (a.one_tile_rows - cta * 128 + 63) / 64)) : 2;
+__device__ __forceinline__ uint32_t a_bytes(const CeGemm& a, int cta) {
+  if (!a.one_tile_rows) return 2 * BOX;
+  if (cta) return a.one_tile_rows > 128 ? 2 * BOX : 0;
+  return a.one_tile_rows > 64 ? 2 * BOX : BOX;
 }
 
 struct Tiles {
   int mtiles;         // rows that take part, in tiles
   int kblocks_rows;   // and in K blocks
-  int n_dx, n_dw;
   int total;
+  // Order of work in kCeStore: the product with the longer tiles (`job`)
+  // first, one of its tiles as long as `ratio` of the other's.
+  int long_job, n_long, n_short, ratio;
 };
 
 template <int MODE>
@@ -130,15 +163,44 @@ __device__ __forceinline__ Tiles count_tiles(const CeGemm& a) {
   const int rows = taken_rows(a);
   t.mtiles = (rows + kCeM - 1) / kCeM;
   t.kblocks_rows = (rows + kCeK - 1) / kCeK;
-  t.n_dx = t.n_dw = 0;
+  t.long_job = t.n_long = t.n_short = 0;
+  t.ratio = 1;
   if (MODE == kCeStore) {
-    if (a.dx.on) t.n_dx = t.mtiles * a.dx.ntiles * a.dx.splits;
-    if (a.dw.on) t.n_dw = a.dw.mtiles * a.dw.ntiles * a.dw.splits;
-    t.total = t.n_dx + t.n_dw;
+    const int n_dx = a.dx.on ? t.mtiles * a.dx.ntiles * a.dx.splits : 0;
+    const int n_dw = a.dw.on ? a.dw.mtiles * a.dw.ntiles * a.dw.splits : 0;
+    const int k_dx = (a.dx.kblocks + a.dx.splits - 1) / a.dx.splits + kTileCost;
+    const int k_dw = (t.kblocks_rows + a.dw.splits - 1) / a.dw.splits + kTileCost;
+    t.long_job = k_dw > k_dx;
+    t.n_long = t.long_job ? n_dw : n_dx;
+    t.n_short = t.long_job ? n_dx : n_dw;
+    t.ratio = max(1, t.long_job ? (k_dw + k_dx / 2) / k_dx : (k_dx + k_dw / 2) / k_dw);
+    t.total = n_dx + n_dw;
   } else {
     t.total = t.mtiles * a.vtiles;
   }
   return t;
+}
+
+// The i-th tile of a pair, -1 past its last. Scores: every npairs-th. Products:
+// the long tiles first, in turn; the pairs that the last turn of them leaves
+// out take `ratio` short ones meanwhile; the rest of those in turn.
+template <int MODE>
+__device__ __forceinline__ int nth_tile(const Tiles& c, int i, int pair, int npairs) {
+  if (MODE != kCeStore) {
+    const int id = pair + i * npairs;
+    return id < c.total ? id : -1;
+  }
+  const int rem = c.n_long % npairs;
+  const int mine = c.n_long / npairs + (pair < rem);
+  if (i < mine) return pair + i * npairs;
+  i -= mine;
+  const int free_pairs = rem ? npairs - rem : 0;
+  int j;
+  if (free_pairs && pair >= rem && i < c.ratio)
+    j = i * free_pairs + pair - rem;
+  else
+    j = free_pairs * c.ratio + (i - (free_pairs && pair >= rem ? c.ratio : 0)) * npairs + pair;
+  return j < c.n_short ? c.n_long + j : -1;
 }
 
 template <int MODE>
@@ -157,11 +219,9 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
     t.split = 0;
     return t;
   }
-  // The longer product's tiles first, so the shorter ones fill the last turn.
-  const int n_first = a.dw_first ? c.n_dw : c.n_dx;
-  const bool second = id >= n_first;
-  t.job = (a.dw_first != 0) != second;
-  if (second) id -= n_first;
+  const bool second = id >= c.n_long;
+  t.job = second ? !c.long_job : c.long_job;
+  if (second) id -= c.n_long;
   const CeJob& j = t.job ? a.dw : a.dx;
   t.n = id % j.ntiles * kCeN;
   id /= j.ntiles;
@@ -177,37 +237,41 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
 
 // --------------------------------------------------------------- epilogues
 
-// 64 scores of a row: their maximum and the sum of powers of two (the scores
+// 32 scores of a row: the running maximum and sum of powers of two (the scores
 // times scale * log2(e), so that e^z is one ex2), and the target's score.
-__device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[QCOLS], int n0, int64_t row, bool live, int tgt) {
-  const int cols = a.classes - n0;
+__device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[CHUNK], int n0, int cols, int64_t row, bool live,
+                                        int tgt, float& top, float& sum) {
   if (cols <= 0) return;
-  if (cols < QCOLS) {
+  if (cols < CHUNK) {
 #pragma unroll
-    for (int j = 0; j < QCOLS; j++)
+    for (int j = 0; j < CHUNK; j++)
       if (j >= cols) w[j] = -INFINITY;
   }
   const int at = tgt - n0;
-  if (at >= 0 && at < QCOLS && live) {
+  if (at >= 0 && at < CHUNK && live) {
     float z = 0.0f;
 #pragma unroll
-    for (int j = 0; j < QCOLS; j++) z = j == at ? w[j] : z;
+    for (int j = 0; j < CHUNK; j++) z = j == at ? w[j] : z;
     a.zt[row] = z * a.c2;
   }
-  float m[4];
+  float m[2];
 #pragma unroll
-  for (int k = 0; k < 4; k++) {
+  for (int k = 0; k < 2; k++) {
     m[k] = fmax3(w[16 * k], w[16 * k + 1], w[16 * k + 2]);
 #pragma unroll
     for (int j = 3; j < 15; j += 2) m[k] = fmax3(m[k], w[16 * k + j], w[16 * k + j + 1]);
     m[k] = fmaxf(m[k], w[16 * k + 15]);
   }
-  const float top = fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])) * a.c2;
+  const float now = fmaxf(m[0], m[1]) * a.c2;
+  if (now > top) {
+    sum *= ex2(top - now);
+    top = now;
+  }
   const float sub = top == -INFINITY ? 0.0f : top;
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-  for (int j = 0; j < QCOLS; j++) sum[j & 3] += ex2(fmaf(w[j], a.c2, -sub));
-  if (live) a.part[row * a.parts + n0 / QCOLS] = make_float2(top, (sum[0] + sum[1]) + (sum[2] + sum[3]));
+  for (int j = 0; j < CHUNK; j++) s[j & 3] += ex2(fmaf(w[j], a.c2, -sub));
+  sum += (s[0] + s[1]) + (s[2] + s[3]);
 }
 
 // A staging tile is free again once its last store has read it.
@@ -221,12 +285,12 @@ __device__ __forceinline__ void stage_put(uint8_t* stg, int lane, int j, uint4 q
   *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = q;
 }
 
-// 64 values of a row in 16 bits into the staging tile.
+// 32 values of a row in 16 bits into one half of the staging tile.
 template <bool F16>
-__device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, const float (&w)[QCOLS]) {
+__device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, int half, const float (&w)[CHUNK]) {
 #pragma unroll
-  for (int q = 0; q < 8; q++)
-    stage_put(stg, lane, q,
+  for (int q = 0; q < 4; q++)
+    stage_put(stg, lane, half * 4 + q,
               make_uint4(pack2<F16>(w[8 * q], w[8 * q + 1]), pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
                          pack2<F16>(w[8 * q + 4], w[8 * q + 5]), pack2<F16>(w[8 * q + 6], w[8 * q + 7])));
 }
@@ -234,13 +298,14 @@ __device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, const float 
 // ------------------------------------------------------------------ kernel
 
 template <int MODE, bool F16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     ce_gemm_kernel(const __grid_constant__ CeMaps maps, const __grid_constant__ CeGemm a) {
-  constexpr int ST = stages(MODE);
+  constexpr int ST = stages(MODE), EW = epi_warps(MODE);
+  constexpr int HCOLS = 2048 / EW;  // columns of an epilogue warp: the tile's or half of them
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* s_stg = smem + (size_t)ST * STAGE;
-  uint64_t* bars = (uint64_t*)(s_stg + (MODE == kCeLse ? 0 : EPI_WARPS * STG));
+  uint64_t* bars = (uint64_t*)(s_stg + (MODE == kCeLse ? 0 : EW * STG));
   uint64_t* full = bars;           // [ST] even CTA: both CTAs' bytes
   uint64_t* empty = full + ST;     // [ST] each CTA: MMA commit
   uint64_t* tfull = empty + ST;    // [2] each CTA: MMA commit
@@ -260,16 +325,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], 2 * EPI_WARPS);
+      mbar_init(&tempty[b], EW);  // of both CTAs, half of them take the buffer's tiles
     }
     *s_abort = 0;
     fence_mbar_init();
   }
   if (warp == 2) tmem_alloc_pair(s_tmem, 512);
   if (MODE != kCeStore && a.one_tile_rows) {
-    const int skip = a_boxes(a, cta) * (int)BOX;
+    const int skip = (int)a_bytes(a, cta);
     for (int s = 0; s < ST; s++)
-      for (int i = skip + threadIdx.x * 16; i < 2 * (int)BOX; i += THREADS * 16)
+      for (int i = skip + (int)threadIdx.x * 16; i < 2 * (int)BOX; i += threads(MODE) * 16)
         *reinterpret_cast<uint4*>(smem + s * STAGE + i) = make_uint4(0, 0, 0, 0);
     fence_async_smem();
   }
@@ -283,42 +348,61 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   grid_wait();
   const Tiles cnt = count_tiles<MODE>(a);
 
-  if (warp == 0) {
-    // ---------------------------------------------------- TMA producer
+  if (warp == 0 || warp == 3) {
+    // ---------------------------------------------------- TMA producers
+    // One thread issues a K block's A loads, one its B loads: a K block lasts
+    // 512 clocks, which one thread for all of them did not always meet.
     if (lane == 0) {
-      int it = 0;
+      const bool for_a = warp == 0;
+      const uint32_t full0 = mapa_shared(full, 0);
+      const uint32_t bytes_a = MODE == kCeStore ? 4 * BOX : a_bytes(a, 0) + a_bytes(a, 1);
+      const bool load_a = MODE == kCeStore || a_bytes(a, cta) > 0;
+      int s = 0, it = 0;
+      uint32_t phase = 1;
       bool ok = true;
-      const int na = a_boxes(a, cta);
-      for (int id = pair; ok && id < cnt.total; id += npairs) {
+      for (int i = 0, id; ok && (id = nth_tile<MODE>(cnt, i, pair, npairs)) >= 0; i++) {
         const Tile t = tile_at<MODE>(a, cnt, id);
-        const int boxes = t.bn >> 7;  // of B in each CTA
-        const uint32_t bytes = (MODE == kCeStore ? 4 : a_boxes(a, 0) + a_boxes(a, 1)) * BOX + 2u * boxes * BOX;
         const int ra = t.m * kCeM + cta * 128;
         const int rb = t.n + cta * (t.bn >> 1);
+        const bool two = t.bn == 256;  // 64-column boxes of B in each CTA
+        const uint32_t bytes = bytes_a + (two ? 4 : 2) * BOX;
+        const CUtensorMap* map = for_a ? (MODE == kCeStore && t.job ? &maps.a1 : &maps.a0)
+                                       : (MODE == kCeStore && t.job ? &maps.b1 : &maps.b0);
+        const int v0 = MODE == kCeStore && t.job ? 0 : a.v0;
         for (int kb = t.kb0; kb < t.kb1; kb++, it++) {
-          const int s = it % ST;
-          if (!mbar_wait(&empty[s], ((it / ST) & 1) ^ 1, s_abort, a.err, 31, WAIT_NS)) {
+          if (!mbar_wait(&empty[s], phase, s_abort, a.err, 31, WAIT_NS)) {
             ok = false;
             break;
           }
-          if (lead) mbar_expect_tx(&full[s], bytes);
-          const uint32_t bar = mapa_shared(&full[s], 0);
-          uint8_t* sa = smem + s * STAGE;
-          uint8_t* sb = sa + 2 * BOX;
+          uint8_t* to = smem + s * STAGE;
+          const uint32_t bar = full0 + s * 8;
           const int k = kb * kCeK;
-          if (MODE != kCeStore) {
-            for (int i = 0; i < na; i++) tma_load_2d_pair(sa + i * BOX, &maps.x, k, ra + 64 * i, bar);
-            for (int i = 0; i < boxes; i++) tma_load_2d_pair(sb + i * BOX, &maps.w, k, a.v0 + rb + 64 * i, bar);
-          } else if (t.job == 0) {
-            for (int i = 0; i < 2; i++) tma_load_2d_pair(sa + i * BOX, &maps.g, k, ra + 64 * i, bar);
-            for (int i = 0; i < boxes; i++) tma_load_2d_pair(sb + i * BOX, &maps.w, rb + 64 * i, a.v0 + k, bar);
+          if (for_a) {
+            if (lead) mbar_expect_tx(&full[s], bytes);
+            if (MODE != kCeStore) {
+              if (load_a) tma_load_2d_pair(to, map, k, ra, bar);
+            } else if (t.job == 0) {
+              tma_load_2d_pair(to, map, k, ra, bar);
+            } else {
+              tma_load_2d_pair(to, map, ra, k, bar);
+              tma_load_2d_pair(to + BOX, map, ra + 64, k, bar);
+            }
           } else {
-            for (int i = 0; i < 2; i++) tma_load_2d_pair(sa + i * BOX, &maps.g, ra + 64 * i, k, bar);
-            for (int i = 0; i < boxes; i++) tma_load_2d_pair(sb + i * BOX, &maps.x, rb + 64 * i, k, bar);
+            if (MODE != kCeStore) {
+              tma_load_2d_pair(to + 2 * BOX, map, k, v0 + rb, bar);
+              if (two) tma_load_2d_pair(to + 3 * BOX, map, k, v0 + rb + 64, bar);
+            } else {
+              tma_load_2d_pair(to + 2 * BOX, map, rb, v0 + k, bar);
+              if (two) tma_load_2d_pair(to + 3 * BOX, map, rb + 64, v0 + k, bar);
+            }
+          }
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1;
           }
         }
       }
-      if (*s_abort && lead) {
+      if (*s_abort && lead && for_a) {
         // Drain (bounded): both CTAs' loads complete on these barriers.
         volatile int dummy = 0;
         for (int i = max(0, it - ST); i < it; i++)
@@ -328,9 +412,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   } else if (warp == 1) {
     // ---------------------------------------------------- MMA issuer (even CTA)
     if (lane == 0 && lead) {
-      int it = 0, tn = 0, last = -1;
+      // Descriptors of stage 0, K-major and MN-major (shared addresses are
+      // below 2^18: adding 16-byte units does not carry out of the field).
+      const uint64_t ka = smem_desc_sw128(smem), kb_ = smem_desc_sw128(smem + 2 * BOX);
+      const uint64_t ma = desc_mn(smem), mb = desc_mn(smem + 2 * BOX);
+      int s = 0, tn = 0, last = -1;
+      uint32_t phase = 0;
       bool ok = true;
-      for (int id = pair; ok && id < cnt.total; id += npairs, tn++) {
+      for (int id; ok && (id = nth_tile<MODE>(cnt, tn, pair, npairs)) >= 0; tn++) {
         const Tile t = tile_at<MODE>(a, cnt, id);
         const int b = tn & 1;
         if (!mbar_wait(&tempty[b], ((tn >> 1) & 1) ^ 1, s_abort, a.err, 32, WAIT_NS)) break;
@@ -339,23 +428,24 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
         const uint32_t d = tmem + b * 256;
         const bool a_mn = MODE == kCeStore && t.job == 1, b_mn = MODE == kCeStore;
         const uint32_t idesc = a.idesc | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(t.bn >> 3) << 17);
-        for (int kb = t.kb0; kb < t.kb1; kb++, it++) {
-          const int s = it % ST;
-          if (!mbar_wait(&full[s], (it / ST) & 1, s_abort, a.err, 33, WAIT_NS)) {
+        const uint64_t ad0 = a_mn ? ma : ka, bd0 = b_mn ? mb : kb_;
+        // 16 of K: 32 bytes on in a K-major row, 16 rows on in an MN-major box.
+        const uint32_t astep = a_mn ? 2048 >> 4 : 32 >> 4, bstep = b_mn ? 2048 >> 4 : 32 >> 4;
+        for (int kb = t.kb0; kb < t.kb1; kb++) {
+          if (!mbar_wait(&full[s], phase, s_abort, a.err, 33, WAIT_NS)) {
             ok = false;
             break;
           }
           tc_fence_after();
-          uint8_t* sa = smem + s * STAGE;
-          const uint64_t ad = a_mn ? desc_mn(sa) : smem_desc_sw128(sa);
-          const uint64_t bd = b_mn ? desc_mn(sa + 2 * BOX) : smem_desc_sw128(sa + 2 * BOX);
-          // 16 of K: 32 bytes on in a K-major row, 16 rows on in an MN-major
-          // box. (Shared addresses are below 2^18: no carry out of the field.)
-          const uint32_t astep = a_mn ? 2048 >> 4 : 32 >> 4, bstep = b_mn ? 2048 >> 4 : 32 >> 4;
+          const uint64_t ad = ad0 + s * (STAGE >> 4), bd = bd0 + s * (STAGE >> 4);
 #pragma unroll
           for (int ks = 0; ks < 4; ks++)
             mma_f16_pair(d, ad + ks * astep, bd + ks * bstep, idesc, kb > t.kb0 || ks > 0 ? 1u : 0u);
           mma_commit_pair(&empty[s], 0x3);
+          if (++s == ST) {
+            s = 0;
+            phase ^= 1;
+          }
         }
         mma_commit_pair(&tfull[b], 0x3);
         last = tn;
@@ -367,18 +457,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     }
   } else if (warp >= EPI_FIRST) {
     // ---------------------------------------------------- epilogue
-    const int quarter = (warp - EPI_FIRST) >> 2, quad = warp & 3;
-    uint8_t* stg = s_stg + (warp - EPI_FIRST) * STG;
-    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const int ew = warp - EPI_FIRST, group = ew / (EW / 2), half = ew / 4 % (EW / 8), quad = warp & 3;
+    uint8_t* stg = s_stg + ew * STG;
+    const uint32_t taddr = tmem + ((uint32_t)(quad * 32) << 16) + group * 256 + half * HCOLS;
     const int taken = taken_rows(a);
     int tn = 0;
-    for (int id = pair; id < cnt.total; id += npairs, tn++) {
+    for (int id; (id = nth_tile<MODE>(cnt, tn, pair, npairs)) >= 0; tn++) {
+      if ((tn & 1) != group) continue;
       const Tile t = tile_at<MODE>(a, cnt, id);
-      const int b = tn & 1;
       const int r0 = t.m * kCeM + cta * 128 + quad * 32;  // the warp's first row
       const int64_t row = r0 + lane;
-      const int n0 = t.n + quarter * QCOLS;               // and column
-      const bool mine = quarter * QCOLS < t.bn && (MODE != kCeLse || r0 < taken);
+      const int n0 = t.n + half * HCOLS;                  // and column
       const bool live = row < taken;
       int tgt = -1;
       float lse2 = 0.0f, gs = 0.0f;
@@ -394,107 +483,130 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           gs = a.gs[row];
         }
       }
-      const bool ok = mbar_wait(&tfull[b], (tn >> 1) & 1, s_abort, a.err, 34, WAIT_NS);
+      const bool ok = mbar_wait(&tfull[group], (tn >> 1) & 1, s_abort, a.err, 34, WAIT_NS);
       if (!__all_sync(0xffffffffu, ok)) break;
       tc_fence_after();
-      float w[QCOLS];
-      if (mine) tmem_ld64(tmem + lanes + b * 256 + quarter * QCOLS, w);
-      // The columns are in registers: hand the accumulator back.
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) {
-        if (lead)
-          mbar_arrive(&tempty[b]);
-        else
-          mbar_arrive_cluster(mapa_shared(&tempty[b], 0));
-      }
-      if (!mine) continue;
-      if (MODE == kCeLse) {
-        epi_lse(a, w, n0, row, live, tgt);
-      } else if (MODE == kCeGrad) {
-        // g = (2^(c2 z - lse2) - [target]) gs in 16 bits; zeros past the last
-        // class and in the tail rows, which the products read.
-        const int cols = a.vn - n0;
+      // Columns of the warp that exist: the last class or a dx or dtable row may
+      // end within the tile.
+      const int cols = min(t.bn - half * HCOLS, (MODE == kCeStore ? a.d : MODE == kCeGrad ? a.vn : a.classes) - n0);
+      const bool mine = half * HCOLS < t.bn && (MODE == kCeLse ? r0 < taken && cols > 0 : MODE == kCeStore ? cols > 0 : true);
+      const CeJob& job = t.job ? a.dw : a.dx;
+      const CUtensorMap* out = t.job ? &maps.out1 : &maps.out0;
+      const bool none = MODE == kCeStore && t.kb0 == t.kb1;  // a split without K blocks: zeros
+      const float f = MODE == kCeStore ? a.head->grad_scale : 1.0f;
+      float top = -INFINITY, sum = 0.0f;
+      float v[2][CHUNK];
+      if (mine) tmem_ld_issue(taddr, v[0]);
 #pragma unroll
-        for (int j = 0; j < QCOLS; j++) w[j] = ex2(fmaf(w[j], a.c2, -lse2));
-        const int at = tgt - a.v0 - n0;
-        if (at >= 0 && at < QCOLS) {
-#pragma unroll
-          for (int j = 0; j < QCOLS; j++)
-            if (j == at) w[j] -= 1.0f;
+      for (int c = 0; c < HCOLS / CHUNK; c++) {
+        float(&w)[CHUNK] = v[c & 1];
+        if (mine) tmem_wait(w);
+        if (c + 1 < HCOLS / CHUNK) {
+          if (mine) tmem_ld_issue(taddr + (c + 1) * CHUNK, v[(c + 1) & 1]);
+        } else {
+          // The last columns are in registers: hand the accumulator back.
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) {
+            if (lead)
+              mbar_arrive(&tempty[group]);
+            else
+              mbar_arrive_cluster(mapa_shared(&tempty[group], 0));
+          }
         }
+        if (!mine) continue;
+        const int left = cols - c * CHUNK;
+        if (MODE == kCeLse) {
+          epi_lse(a, w, n0 + c * CHUNK, left, row, live, tgt, top, sum);
+          if ((c + 1) * CHUNK % PART == 0) {
+            // Neighbouring lanes (rows) side by side.
+            const int part = (n0 + c * CHUNK) / PART;
+            if (live && left + PART - CHUNK > 0) a.part[(int64_t)part * a.part_rows + row] = make_float2(top, sum);
+            top = -INFINITY;
+            sum = 0.0f;
+          }
+        } else if (MODE == kCeGrad) {
+          // g = (2^(c2 z - lse2) - [target]) gs in 16 bits; zeros past the last
+          // class and in the tail rows, which the products read.
 #pragma unroll
-        for (int j = 0; j < QCOLS; j++) w[j] *= gs;
-        if (cols < QCOLS || !live) {
+          for (int j = 0; j < CHUNK; j++) w[j] = ex2(fmaf(w[j], a.c2, -lse2));
+          const int at = tgt - a.v0 - n0 - c * CHUNK;
+          if (at >= 0 && at < CHUNK) {
 #pragma unroll
-          for (int j = 0; j < QCOLS; j++)
-            if (!live || j >= cols) w[j] = 0.0f;
-        }
-        stage_ready(lane);
-        stage_row16<F16>(stg, lane, w);
-        fence_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          tma_store_2d(&maps.g_out, stg, n0, r0);
-          bulk_commit();
-        }
-      } else {
-        const CeJob& j = t.job ? a.dw : a.dx;
-        const CUtensorMap* out = t.job ? &maps.dw_out : &maps.dx_out;
-        if (n0 >= a.d) continue;  // past the last column
-        if (t.kb0 == t.kb1) {
+            for (int j = 0; j < CHUNK; j++)
+              if (j == at) w[j] -= 1.0f;
+          }
 #pragma unroll
-          for (int i = 0; i < QCOLS; i++) w[i] = 0.0f;
-        }
-        if (j.f32_rows > 0) {
-          // whole tiles of rows: never past the end of the split's result
-          const int y = t.split * j.f32_rows + r0;
+          for (int j = 0; j < CHUNK; j++) w[j] *= gs;
+          if (left < CHUNK || !live) {
 #pragma unroll
-          for (int h = 0; h < 2; h++) {
-            if (n0 + h * 32 >= a.d) break;
-            stage_ready(lane);
-#pragma unroll
-            for (int q = 0; q < 8; q++)
-              stage_put(stg, lane, q,
-                        make_uint4(__float_as_uint(w[32 * h + 4 * q]), __float_as_uint(w[32 * h + 4 * q + 1]),
-                                   __float_as_uint(w[32 * h + 4 * q + 2]), __float_as_uint(w[32 * h + 4 * q + 3])));
+            for (int j = 0; j < CHUNK; j++)
+              if (!live || j >= left) w[j] = 0.0f;
+          }
+          if ((c & 1) == 0) stage_ready(lane);
+          stage_row16<F16>(stg, lane, c & 1, w);
+          if (c & 1) {
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
-              if (j.add)
-                tma_add_2d(out, stg, n0 + h * 32, y);
-              else
-                tma_store_2d(out, stg, n0 + h * 32, y);
+              tma_store_2d(&maps.out0, stg, n0 + (c - 1) * CHUNK, r0);
               bulk_commit();
             }
           }
         } else {
-          const float f = a.head->grad_scale;
+          if (none) {
 #pragma unroll
-          for (int i = 0; i < QCOLS; i++) w[i] *= f;
-          stage_ready(lane);
-          stage_row16<F16>(stg, lane, w);
-          fence_async_smem();
-          __syncwarp();
-          if (!j.out) {
+            for (int i = 0; i < CHUNK; i++) w[i] = 0.0f;
+          }
+          if (job.f32_rows > 0) {
+            if (left <= 0) continue;
+            // whole tiles of rows: never past the end of the split's result
+            const int y = t.split * job.f32_rows + r0;
+            stage_ready(lane);
+#pragma unroll
+            for (int q = 0; q < 8; q++)
+              stage_put(stg, lane, q,
+                        make_uint4(__float_as_uint(w[4 * q]), __float_as_uint(w[4 * q + 1]),
+                                   __float_as_uint(w[4 * q + 2]), __float_as_uint(w[4 * q + 3])));
+            fence_async_smem();
+            __syncwarp();
             if (lane == 0) {
-              tma_store_2d(out, stg, n0, j.row0 + r0);
+              if (job.add)
+                tma_add_2d(out, stg, n0 + c * CHUNK, y);
+              else
+                tma_store_2d(out, stg, n0 + c * CHUNK, y);
               bulk_commit();
             }
           } else {
-            // Rows that TMA cannot address: the warp stores them one by one,
-            // two elements a lane.
-            const int64_t left = a.classes - (j.row0 + (int64_t)r0);
-            uint16_t* o = j.out + (j.row0 + (int64_t)r0) * j.out_stride + n0;
-            const int cols = a.d - n0;
-            for (int r = 0; r < 32 && r < left; r++, o += j.out_stride) {
+            if (left + (c & 1) * CHUNK <= 0) continue;  // the 64 columns of a staging tile
 #pragma unroll
-              for (int h = 0; h < 2; h++) {
-                const int c = lane + 32 * h;
-                if (c < cols) o[c] = *reinterpret_cast<uint16_t*>(stg + r * 128 + ((((c >> 3) ^ (r & 7)) << 4) | (c & 7) << 1));
-              }
-            }
+            for (int i = 0; i < CHUNK; i++) w[i] *= f;
+            if ((c & 1) == 0) stage_ready(lane);
+            stage_row16<F16>(stg, lane, c & 1, w);
+            if ((c & 1) == 0) continue;
+            fence_async_smem();
             __syncwarp();
+            if (!job.out) {
+              if (lane == 0) {
+                tma_store_2d(out, stg, n0 + (c - 1) * CHUNK, job.row0 + r0);
+                bulk_commit();
+              }
+            } else {
+              // Rows that TMA cannot address: the warp stores them one by one,
+              // two elements a lane.
+              const int64_t first = job.row0 + (int64_t)r0, rows = a.classes - first;
+              uint16_t* o = job.out + first * job.out_stride + n0 + (c - 1) * CHUNK;
+              const int here = left + CHUNK;
+              for (int r = 0; r < 32 && r < rows; r++, o += job.out_stride) {
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                  const int e = lane + 32 * h;
+                  if (e < here)
+                    o[e] = *reinterpret_cast<uint16_t*>(stg + r * 128 + ((((e >> 3) ^ (r & 7)) << 4) | (e & 7) << 1));
+                }
+              }
+              __syncwarp();
+            }
           }
         }
       }
@@ -520,11 +632,12 @@ int pairs_of(int* out) {
   int n = dev < 128 ? cached[dev].load() : 0;
   if (n == 0) {
     auto kernel = ce_gemm_kernel<MODE, F16>;
-    VRS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(MODE)));
+    constexpr int kSmem = (int)smem_bytes(MODE);
+    VRS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = smem_bytes(MODE);
+    cfg.blockDim = dim3(threads(MODE));
+    cfg.dynamicSmemBytes = kSmem;
     cudaLaunchAttribute at[1];
     at[0].id = cudaLaunchAttributeClusterDimension;
     at[0].val.clusterDim.x = 2;
@@ -547,7 +660,8 @@ int launch(const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t
   int pairs = 0;
   VRS_TRY((pairs_of<MODE, F16>(&pairs)));
   const int64_t n = most_tiles < pairs ? most_tiles : pairs;
-  VRS_TRY(launch_after(ce_gemm_kernel<MODE, F16>, (unsigned)(2 * (n < 1 ? 1 : n)), THREADS, smem_bytes(MODE), s, maps, a));
+  VRS_TRY(launch_after(ce_gemm_kernel<MODE, F16>, (unsigned)(2 * (n < 1 ? 1 : n)), threads(MODE), smem_bytes(MODE),
+                       s, maps, a));
   count_launch();
   return VRS_OK;
 }
