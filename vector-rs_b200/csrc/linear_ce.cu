@@ -49,6 +49,10 @@ struct Pack1 {
   const int64_t* targets;
   int64_t classes;
   int per_block;
+  int pack_blocks;  // the grid's other blocks copy the table
+  const uint16_t* table;
+  int64_t ts;
+  uint16_t* table_out;
   const int2* slabs;  // per slab: taking rows, bits of the largest |dloss|; null: read all targets
   CeHeader* head;
   void* xc;        // [taking rows, tail zeros to a whole tile][dp]
@@ -123,10 +127,75 @@ constexpr float kF16Gain = 8192.0f;
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
+// One row of d elements at any address, copied by a warp to `to` (16-byte
+// aligned, dp elements, zeros past d). Where whole 16-byte words around the row
+// may be read (`inside`), each lane reads the two that its 16 bytes lie in and
+// shifts them into place; else the row is read element by element.
+__device__ __forceinline__ void copy_row(const uint16_t* from, int d, int dp, uint16_t* to, bool inside) {
+  const int lane = threadIdx.x & 31, chunks = dp / 8;
+  uint4* out = reinterpret_cast<uint4*>(to);
+  if (!inside) {
+    for (int c = lane; c < chunks; c += 32) {
+      Pack<uint16_t, 8> q;
+#pragma unroll
+      for (int j = 0; j < 8; j++) q.v[j] = c * 8 + j < d ? from[c * 8 + j] : 0;
+      out[c] = *reinterpret_cast<uint4*>(&q);
+    }
+    return;
+  }
+  const uint4* in = reinterpret_cast<const uint4*>((uintptr_t)from & ~(uintptr_t)15);
+  const int shift = (int)((uintptr_t)from & 15);  // bytes, even; the same for the warp
+  constexpr int U = 4;
+  for (int c0 = lane; c0 < chunks; c0 += 32 * U) {
+    uint4 lo[U], hi[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int c = c0 + 32 * u;
+      if (c < chunks) {
+        lo[u] = in[c];
+        hi[u] = make_uint4(0, 0, 0, 0);
+        if (2 * (d - c * 8) > 16 - shift) hi[u] = in[c + 1];  // else no element lies in it
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int c = c0 + 32 * u;
+      if (c >= chunks) continue;
+      uint32_t w[8] = {lo[u].x, lo[u].y, lo[u].z, lo[u].w, hi[u].x, hi[u].y, hi[u].z, hi[u].w};
+      if (shift & 8) {
+#pragma unroll
+        for (int j = 0; j < 6; j++) w[j] = w[j + 2];
+      }
+      if (shift & 4) {
+#pragma unroll
+        for (int j = 0; j < 5; j++) w[j] = w[j + 1];
+      }
+      if (shift & 2) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = __funnelshift_r(w[j], w[j + 1], 16);
+      }
+      const int left = d - c * 8;
+      if (left < 8) {
+#pragma unroll
+        for (int j = 0; j < 4; j++) w[j] = left >= 2 * j + 2 ? w[j] : left == 2 * j + 1 ? w[j] & 0xffffu : 0u;
+      }
+      out[c] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  }
+}
+
 template <bool BACK>
 __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
   grid_launch();
   grid_wait();
+  if ((int)blockIdx.x >= a.pack_blocks) {
+    // The table's rows, a warp each. The 16-byte words around a row belong to
+    // the table but for its first and last rows (and rows shorter than a word).
+    const int64_t step = (int64_t)(gridDim.x - a.pack_blocks) * 8;
+    for (int64_t v = (int64_t)(blockIdx.x - a.pack_blocks) * 8 + (threadIdx.x >> 5); v < a.classes; v += step)
+      copy_row(a.table + v * a.ts, a.d, a.dp, a.table_out + v * a.dp, v > 0 && v < a.classes - 1 && a.d >= 8);
+    return;
+  }
   __shared__ int s[8][3];
   __shared__ int s_warp[8];
   __shared__ int s_row[256];
@@ -202,72 +271,22 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
   const uint16_t* x = (const uint16_t*)a.x;
   const int chunks = a.dp / 8;
   for (int i = warp; i < n_in; i += 8) {
-    const uint16_t* from = x + (r0 + s_row[i]) * a.xs;
-    uint4* to = reinterpret_cast<uint4*>(xc + (int64_t)(before + i) * a.dp);
+    const int64_t row = r0 + s_row[i];
+    uint16_t* to = xc + (int64_t)(before + i) * a.dp;
     if (a.vec) {
+      const uint4* from = reinterpret_cast<const uint4*>(x + row * a.xs);
 #pragma unroll 4
-      for (int c = lane; c < chunks; c += 32) to[c] = reinterpret_cast<const uint4*>(from)[c];
+      for (int c = lane; c < chunks; c += 32) reinterpret_cast<uint4*>(to)[c] = from[c];
     } else {
-      for (int c = lane; c < chunks; c += 32) {
-        uint32_t q[4];
-#pragma unroll
-        for (int j = 0; j < 4; j++) {
-          const int e = c * 8 + 2 * j;
-          const uint32_t lo = e < a.d ? from[e] : 0, hi = e + 1 < a.d ? from[e + 1] : 0;
-          q[j] = lo | hi << 16;
-        }
-        to[c] = make_uint4(q[0], q[1], q[2], q[3]);
-      }
+      copy_row(x + row * a.xs, a.d, a.dp, to, row > 0 && row < a.rows - 1 && a.d >= 8);
     }
   }
   // (Past the last row TMA reads zeros itself.)
   const int64_t tail = min(a.rows, (int64_t)(total + kCeM - 1) / kCeM * kCeM);
-  for (int64_t p = total + (int64_t)blockIdx.x * 8 + warp; p < tail; p += (int64_t)gridDim.x * 8) {
+  for (int64_t p = total + (int64_t)blockIdx.x * 8 + warp; p < tail; p += (int64_t)a.pack_blocks * 8) {
     uint4* to = reinterpret_cast<uint4*>(xc + p * a.dp);
     for (int c = lane; c < chunks; c += 32) to[c] = make_uint4(0, 0, 0, 0);
   }
-}
-
-// A table whose rows TMA cannot address, copied to rows of dp elements: two
-// elements a lane and turn, read by A at a time (the rows' alignment), or four.
-template <int A>
-__global__ void __launch_bounds__(256) ce_copy_table_kernel(const uint16_t* __restrict__ w, int64_t ws, int64_t classes,
-                                                           int d, int dp, uint16_t* out) {
-  grid_launch();  // reads inputs and writes what only the products read: nothing to wait for
-  constexpr int N = A < 2 ? 2 : A;
-  const int lane = threadIdx.x & 31;
-  for (int64_t v = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); v < classes; v += (int64_t)gridDim.x * 8) {
-    const uint16_t* from = w + v * ws;
-    uint16_t* to = out + v * dp;
-#pragma unroll 8
-    for (int e = lane * N; e < dp; e += 32 * N) {
-      Pack<uint16_t, N> k;
-      if (A > 1 && e + N <= d) {
-        k = load_pack<uint16_t, N>(from + e);
-      } else {
-#pragma unroll
-        for (int i = 0; i < N; i++) k.v[i] = e + i < d ? from[e + i] : 0;
-      }
-      *reinterpret_cast<Pack<uint16_t, N>*>(to + e) = k;
-    }
-  }
-}
-
-int copy_table(const void* table, int64_t ts, int64_t classes, int d, int dp, void* out, int sms, cudaStream_t s) {
-  const uint16_t* w = (const uint16_t*)table;
-  uint16_t* o = (uint16_t*)out;
-  const int64_t need = (classes + 7) / 8, most = (int64_t)sms * 8;
-  const unsigned blocks = (unsigned)(need < most ? need : most);
-  const uintptr_t at = (uintptr_t)table | (uintptr_t)(classes == 1 ? 0 : ts * 2);
-  if (at % 8 == 0)
-    ce_copy_table_kernel<4><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
-  else if (at % 4 == 0)
-    ce_copy_table_kernel<2><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
-  else
-    ce_copy_table_kernel<1><<<blocks, 256, 0, s>>>(w, ts, classes, d, dp, o);
-  VRS_CUDA(cudaGetLastError());
-  count_launch();
-  return VRS_OK;
 }
 
 // --------------------------------------------------------- combine, finish
@@ -569,7 +588,10 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   k.head = (CeHeader*)(c.ws + p.head);
   k.xc = c.ws + p.xc;
   k.target = (int*)(c.ws + p.target);
-  const bool packed = back || c.rows > kCeM || !tma_rows(c.x, c.xs, c.rows);
+  const void* w = c.table;
+  int64_t ts = c.ts;
+  const bool copied = !tma_rows(w, ts, c.classes);
+  const bool packed = back || copied || c.rows > kCeM || !tma_rows(c.x, c.xs, c.rows);
   a.rows = packed ? -1 : (int)c.rows;
   if (packed) {
     if (c.rows > kScanRows) {
@@ -582,18 +604,21 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
     } else {
       k.per_block = (int)((c.rows + 2 * sms - 1) / (2 * sms));
     }
-    const unsigned blocks = (unsigned)((c.rows + k.per_block - 1) / k.per_block);
-    VRS_TRY(launch_after(back ? ce_pack_kernel<true> : ce_pack_kernel<false>, blocks, 256, 0, c.s, k));
+    k.pack_blocks = (int)((c.rows + k.per_block - 1) / k.per_block);
+    int64_t blocks = k.pack_blocks;
+    if (copied) {
+      k.table = (const uint16_t*)w;
+      k.ts = ts;
+      k.table_out = (uint16_t*)(c.ws + p.wc);
+      const int64_t need = (c.classes + 7) / 8, most = (int64_t)sms * 16;
+      blocks += need < most ? need : most;
+      w = k.table_out;
+      ts = p.dp;
+    }
+    VRS_TRY(launch_after(back ? ce_pack_kernel<true> : ce_pack_kernel<false>, (unsigned)blocks, 256, 0, c.s, k));
     count_launch();
   } else {
     a.targets = c.targets;
-  }
-  const void* w = c.table;
-  int64_t ts = c.ts;
-  if (!tma_rows(w, ts, c.classes)) {
-    w = c.ws + p.wc;
-    ts = p.dp;
-    VRS_TRY(copy_table(c.table, c.ts, c.classes, (int)c.d, (int)p.dp, c.ws + p.wc, sms, c.s));
   }
   const bool f16 = c.dtype == VRS_F16;
   const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
