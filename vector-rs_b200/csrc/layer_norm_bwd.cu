@@ -68,6 +68,8 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
   constexpr int kColFloats = GROUPS > 1 && TPR * E > kLnThreads ? 2 * TPR * E : 2 * kLnThreads;
   __shared__ float s_col[kColFloats];
   int64_t first = blockIdx.x, step = gridDim.x - a.col_blocks;
+  grid_launch();
+  grid_wait();
   if (first >= step) {  // whole clusters
     sum_columns<T, P>(a, (int)(first - step), reinterpret_cast<float(*)[kColumns][2]>(s_col));
     return;
@@ -238,6 +240,8 @@ template <class P>
 __global__ void __launch_bounds__(32 * kStrips) ln_param_kernel(const float* __restrict__ partial, int nblk, int d,
                                                        P* __restrict__ dweight, P* __restrict__ dbias) {
   __shared__ float s[kStrips][33];
+  grid_launch();
+  grid_wait();
   const int lane = threadIdx.x & 31, strip = threadIdx.x >> 5;
   const int64_t c = (int64_t)blockIdx.x * 32 + lane, n = 2 * (int64_t)d;
   float v = 0.0f;
@@ -258,8 +262,8 @@ __global__ void __launch_bounds__(32 * kStrips) ln_param_kernel(const float* __r
 
 template <class P>
 int launch_params(const float* partial, int nblk, int d, void* dw, void* db, cudaStream_t s) {
-  ln_param_kernel<P><<<(unsigned)((2 * (int64_t)d + 31) / 32), 32 * kStrips, 0, s>>>(partial, nblk, d, (P*)dw, (P*)db);
-  VRS_CUDA(cudaGetLastError());
+  VRS_TRY(launch_after(ln_param_kernel<P>, (unsigned)((2 * (int64_t)d + 31) / 32), 32 * kStrips, 0, s, partial, nblk, d,
+                       (P*)dw, (P*)db));
   count_launch();
   return VRS_OK;
 }

@@ -28,6 +28,8 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
     first /= cluster.num_blocks();
     step /= cluster.num_blocks();
   }
+  grid_launch();
+  grid_wait();
   T* y = (T*)a.y;
   const int64_t apart = step * GROUPS, row_first = first * GROUPS + threadIdx.x / TPR;
   Ring ring;

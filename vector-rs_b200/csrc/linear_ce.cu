@@ -124,9 +124,6 @@ __device__ __forceinline__ float grad_unit(unsigned max_bits) {
 // f16 ends at 2^16 and loses bits below 2^-14: its gradients use the range up to 2^13.
 constexpr float kF16Gain = 8192.0f;
 
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 // One row of d elements at any address, copied by a warp to `to` (16-byte
 // aligned, dp elements, zeros past d). Where whole 16-byte words around the row
 // may be read (`inside`), each lane reads the two that its 16 bytes lie in and

@@ -72,24 +72,6 @@ struct CeMaps {
   CUtensorMap a0, b0, out0, a1, b1, out1;
 };
 
-// A launch that may begin while the kernel before it on the stream ends; the
-// kernel waits for that one's results itself (griddepcontrol.wait).
-template <class... KA, class... A>
-int launch_after(void (*kernel)(KA...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
-  cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3(blocks);
-  cfg.blockDim = dim3(threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = s;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  VRS_CUDA(cudaLaunchKernelEx(&cfg, kernel, KA(args)...));
-  return VRS_OK;
-}
-
 int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s);
 
 }  // namespace ops

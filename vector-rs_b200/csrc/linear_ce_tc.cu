@@ -114,9 +114,6 @@ __device__ __forceinline__ void tmem_wait(float (&v)[CHUNK]) {
                : "memory");
 }
 
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-
 template <bool F16>
 __device__ __forceinline__ uint32_t pack2(float lo, float hi) {
   uint32_t r;

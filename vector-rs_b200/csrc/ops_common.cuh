@@ -153,6 +153,29 @@ __device__ __forceinline__ void store_held(T* p, const F2 (&v)[E / 2], int i) {
   store_pack<T, VEC>(p, f);
 }
 
+// ---- dependent launches. A kernel started by launch_after may begin while the
+// one before it on the stream ends: it waits (grid_wait) before it touches
+// memory, for that kernel and, since every kernel here does so, for all before
+// it. grid_launch lets the next one begin once all blocks have come so far.
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void grid_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+template <class... KA, class... A>
+int launch_after(void (*kernel)(KA...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t s, const A&... args) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(blocks);
+  cfg.blockDim = dim3(threads);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = s;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  VRS_CUDA(cudaLaunchKernelEx(&cfg, kernel, KA(args)...));
+  return VRS_OK;
+}
+
 inline int dtype_bytes(int dtype) { return dtype == VRS_F32 ? 4 : 2; }
 
 inline int invalid(const std::string& m) {
