@@ -338,37 +338,39 @@ __global__ void __launch_bounds__(1024)
 }
 
 // out[row] = sum over splits of acc[split][pos[row]], rounded once; rows
-// without a place get zeros. A warp a row, four columns a lane and turn.
+// without a place get zeros. A warp takes 128 columns of a row at a time.
 template <class T>
 __global__ void __launch_bounds__(256)
     ce_finish_kernel(const float* __restrict__ acc, int splits, int64_t split_rows, int d, int d4, int64_t rows,
                      const int* __restrict__ pos, const CeHeader* head, T* out, int64_t os, bool vec) {
   grid_wait();
   const float f = head->grad_scale;
-  for (int64_t r = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); r < rows; r += (int64_t)gridDim.x * 8) {
+  const int chunks = (d4 + 127) / 128;
+  const int64_t step = (int64_t)gridDim.x * 8, units = rows * chunks;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += step) {
+    const int64_t r = units < (1ll << 31) ? (int64_t)((uint32_t)u / (uint32_t)chunks) : u / chunks;
+    const int c = (int)(u - r * chunks) * 128 + (threadIdx.x & 31) * 4;
+    if (c >= d4) continue;
     const int64_t p = pos ? pos[r] : r;
-    T* o = out + r * os;
-#pragma unroll 4
-    for (int c = (threadIdx.x & 31) * 4; c < d4; c += 128) {
-      float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-      if (p >= 0) {
-#pragma unroll 4
-        for (int k = 0; k < splits; k++) {
-          const float4 q = *reinterpret_cast<const float4*>(acc + (k * split_rows + p) * d4 + c);
-          v.x += q.x;
-          v.y += q.y;
-          v.z += q.z;
-          v.w += q.w;
-        }
+    T* o = out + r * os + c;
+    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (p >= 0) {
+#pragma unroll 8
+      for (int k = 0; k < splits; k++) {
+        const float4 q = *reinterpret_cast<const float4*>(acc + (k * split_rows + p) * d4 + c);
+        v.x += q.x;
+        v.y += q.y;
+        v.z += q.z;
+        v.w += q.w;
       }
-      const float e[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
-      if (vec) {
-        store_pack<T, 4>(o + c, e);
-      } else {
+    }
+    const float e[4] = {v.x * f, v.y * f, v.z * f, v.w * f};
+    if (vec) {
+      store_pack<T, 4>(o, e);
+    } else {
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-          if (c + j < d) o[c + j] = from_f32<T>(e[j]);
-      }
+      for (int j = 0; j < 4; j++)
+        if (c + j < d) o[j] = from_f32<T>(e[j]);
     }
   }
 }
@@ -379,7 +381,7 @@ int launch_finish(const float* acc, int splits, int64_t split_rows, int d, int d
   const bool vec = d % 4 == 0 && (rows == 1 || os % 4 == 0) && (uintptr_t)out % 8 == 0;
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  const int64_t need = (rows + 7) / 8, most = (int64_t)sms * 8;
+  const int64_t need = (rows * ((d4 + 127) / 128) + 7) / 8, most = (int64_t)sms * 8;
   VRS_TRY(launch_after(ce_finish_kernel<T>, (unsigned)(need < most ? need : most), 256, 0, s, acc, splits, split_rows, d,
                        d4, rows, pos, head, (T*)out, os, vec));
   count_launch();
@@ -702,19 +704,18 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   a.dx.ntiles = a.dw.ntiles = (int)((c.d + kCeN - 1) / kCeN);
   a.dx.splits = p.splits_dx;
   a.dw.splits = p.splits_dw;
+  a.d4 = (int)p.d4;
+  a.dx.f32 = acc_dx;
   a.dx.f32_rows = (int)p.rows_p;
-  if (dx)
-    VRS_TRY(make_map(&prod.out0, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dx, c.d, p.splits_dx * p.rows_p, p.d4, 32));
   const bool direct = p.splits_dw == 1;
   if (dtable) {
     if (!direct) {
+      a.dw.f32 = acc_dw;
       a.dw.f32_rows = (int)p.piece;
-      VRS_TRY(make_map(&prod.out1, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 4, acc_dw, c.d, p.splits_dw * p.piece, p.d4, 32));
-    } else if (tma_rows(dtable, dts, c.classes)) {
-      VRS_TRY(make_map(&prod.out1, type, 2, dtable, c.d, c.classes, dts, 32));
     } else {
       a.dw.out = (uint16_t*)dtable;
       a.dw.out_stride = c.classes == 1 ? 0 : dts;
+      a.dw.out_vec = c.d % 8 == 0 && tma_rows(dtable, dts, c.classes);
     }
   }
   for (int64_t v0 = 0; v0 < c.classes; v0 += p.piece) {

@@ -33,11 +33,13 @@ struct CeJob {
   int ntiles;      // over d
   int kblocks;     // dx; dtable takes its count from the header
   int splits;
-  int f32_rows;    // rows of one split's f32 result; 0: 16-bit result, one split
+  float* f32;      // [split][f32_rows][d4], or null: 16-bit result, one split
+  int f32_rows;
   int add;         // f32: add to what earlier pieces left
   int row0;        // 16-bit result: first row (the piece's first class)
-  uint16_t* out;   // 16-bit result that TMA cannot address, else null
+  uint16_t* out;   // 16-bit result
   int64_t out_stride;
+  int out_vec;     // its rows take 16-byte stores
 };
 
 struct CeGemm {
@@ -48,7 +50,7 @@ struct CeGemm {
   int* err;          // host-visible word that a wait which gave up writes
   int classes;       // all classes
   int v0, vn;        // the piece
-  int d;
+  int d, d4;         // d4: pitch of f32 results, d in whole fours
   int kblocks;       // of d
   int vtiles;        // class tiles of the piece
   int parts;         // kCeLse: 128-class parts of a row
@@ -67,9 +69,9 @@ struct CeGemm {
 };
 
 // Tensor maps of a launch. Scores: a0 rows, b0 table, out0 their gradient.
-// Products: a0, b0, out0 of dx (A: the score gradients), a1, b1, out1 of dtable.
+// Products: a0, b0 of dx (A: the score gradients), a1, b1 of dtable.
 struct CeMaps {
-  CUtensorMap a0, b0, out0, a1, b1, out1;
+  CUtensorMap a0, b0, out0, a1, b1;
 };
 
 int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s);

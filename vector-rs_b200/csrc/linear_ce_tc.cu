@@ -69,10 +69,9 @@ __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void*
                "r"(x), "r"(y), "r"(smem_u32(src))
                : "memory");
 }
-__device__ __forceinline__ void tma_add_2d(const CUtensorMap* map, const void* src, int x, int y) {
-  asm volatile("cp.reduce.async.bulk.tensor.2d.global.shared::cta.add.bulk_group [%0, {%1, %2}], [%3];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(smem_u32(src))
+__device__ __forceinline__ void add_f32x4(float* to, uint4 v) {
+  asm volatile("red.relaxed.gpu.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(to), "f"(__uint_as_float(v.x)),
+               "f"(__uint_as_float(v.y)), "f"(__uint_as_float(v.z)), "f"(__uint_as_float(v.w))
                : "memory");
 }
 __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
@@ -80,7 +79,6 @@ template <int N>
 __device__ __forceinline__ void bulk_wait_read() {
   asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
 }
-__device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ float ex2(float x) {
@@ -200,6 +198,24 @@ __device__ __forceinline__ int nth_tile(const Tiles& c, int i, int pair, int npa
   return j < c.n_short ? c.n_long + j : -1;
 }
 
+// By value, field by field: a reference chosen at run time would read the
+// kernel's parameters through memory, again after every asm statement.
+__device__ __forceinline__ CeJob job_of(const CeGemm& a, bool dw) {
+  CeJob j;
+  j.mtiles = dw ? a.dw.mtiles : a.dx.mtiles;
+  j.ntiles = dw ? a.dw.ntiles : a.dx.ntiles;
+  j.kblocks = dw ? a.dw.kblocks : a.dx.kblocks;
+  j.splits = dw ? a.dw.splits : a.dx.splits;
+  j.f32 = dw ? a.dw.f32 : a.dx.f32;
+  j.f32_rows = dw ? a.dw.f32_rows : a.dx.f32_rows;
+  j.add = dw ? a.dw.add : a.dx.add;
+  j.row0 = dw ? a.dw.row0 : a.dx.row0;
+  j.out = dw ? a.dw.out : a.dx.out;
+  j.out_stride = dw ? a.dw.out_stride : a.dx.out_stride;
+  j.out_vec = dw ? a.dw.out_vec : a.dx.out_vec;
+  return j;
+}
+
 template <int MODE>
 __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id) {
   Tile t;
@@ -219,7 +235,7 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
   const bool second = id >= c.n_long;
   t.job = second ? !c.long_job : c.long_job;
   if (second) id -= c.n_long;
-  const CeJob& j = t.job ? a.dw : a.dx;
+  const CeJob j = job_of(a, t.job);
   t.n = id % j.ntiles * kCeN;
   id /= j.ntiles;
   t.split = id % j.splits;
@@ -282,6 +298,10 @@ __device__ __forceinline__ void stage_put(uint8_t* stg, int lane, int j, uint4 q
   *reinterpret_cast<uint4*>(stg + lane * 128 + ((j ^ (lane & 7)) << 4)) = q;
 }
 
+__device__ __forceinline__ uint4 stage_get(const uint8_t* stg, int row, int j) {
+  return *reinterpret_cast<const uint4*>(stg + row * 128 + ((j ^ (row & 7)) << 4));
+}
+
 // 32 values of a row in 16 bits into one half of the staging tile.
 template <bool F16>
 __device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, int half, const float (&w)[CHUNK]) {
@@ -326,6 +346,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     }
     *s_abort = 0;
     fence_mbar_init();
+  }
+  if (threadIdx.x == 32 * 3) {
+    prefetch_tmap(&maps.a0);
+    prefetch_tmap(&maps.b0);
+    if (MODE == kCeStore) {
+      prefetch_tmap(&maps.a1);
+      prefetch_tmap(&maps.b1);
+    }
+    if (MODE == kCeGrad) prefetch_tmap(&maps.out0);
   }
   if (warp == 2) tmem_alloc_pair(s_tmem, 512);
   if (MODE != kCeStore && a.one_tile_rows) {
@@ -487,19 +516,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
       // end within the tile.
       const int cols = min(t.bn - half * HCOLS, (MODE == kCeStore ? a.d : MODE == kCeGrad ? a.vn : a.classes) - n0);
       const bool mine = half * HCOLS < t.bn && (MODE == kCeLse ? r0 < taken && cols > 0 : MODE == kCeStore ? cols > 0 : true);
-      const CeJob& job = t.job ? a.dw : a.dx;
-      const CUtensorMap* out = t.job ? &maps.out1 : &maps.out0;
+      const CeJob job = job_of(a, t.job);
       const bool none = MODE == kCeStore && t.kb0 == t.kb1;  // a split without K blocks: zeros
       const float f = MODE == kCeStore ? a.head->grad_scale : 1.0f;
       float top = -INFINITY, sum = 0.0f;
       float v[2][CHUNK];
       if (mine) tmem_ld_issue(taddr, v[0]);
+      // (Two chunks a turn and no more unrolling: in a small problem this code
+      // runs once, and fetching it was half of the kernel's time.)
+#pragma unroll 1
+      for (int c0 = 0; c0 < HCOLS / CHUNK; c0 += 2)
 #pragma unroll
-      for (int c = 0; c < HCOLS / CHUNK; c++) {
-        float(&w)[CHUNK] = v[c & 1];
+      for (int h = 0; h < 2; h++) {
+        const int c = c0 + h;
+        float(&w)[CHUNK] = v[h];
         if (mine) tmem_wait(w);
         if (c + 1 < HCOLS / CHUNK) {
-          if (mine) tmem_ld_issue(taddr + (c + 1) * CHUNK, v[(c + 1) & 1]);
+          if (mine) tmem_ld_issue(taddr + (c + 1) * CHUNK, v[1 - h]);
         } else {
           // The last columns are in registers: hand the accumulator back.
           tc_fence_before();
@@ -540,9 +573,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
             for (int j = 0; j < CHUNK; j++)
               if (!live || j >= left) w[j] = 0.0f;
           }
-          if ((c & 1) == 0) stage_ready(lane);
-          stage_row16<F16>(stg, lane, c & 1, w);
-          if (c & 1) {
+          if (h == 0) stage_ready(lane);
+          stage_row16<F16>(stg, lane, h, w);
+          if (h == 1) {
             fence_async_smem();
             __syncwarp();
             if (lane == 0) {
@@ -555,60 +588,66 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
 #pragma unroll
             for (int i = 0; i < CHUNK; i++) w[i] = 0.0f;
           }
-          if (job.f32_rows > 0) {
-            if (left <= 0) continue;
-            // whole tiles of rows: never past the end of the split's result
-            const int y = t.split * job.f32_rows + r0;
-            stage_ready(lane);
+          if (job.f32) {
+            // Through the staging tile, so that a warp's store covers whole
+            // lines. Whole tiles of rows: never past the end of the split's
+            // result. Each value has one writer a launch, so additions come in
+            // launch order.
 #pragma unroll
-            for (int q = 0; q < 8; q++)
+            for (int q = 0; q < CHUNK / 4; q++)
               stage_put(stg, lane, q,
                         make_uint4(__float_as_uint(w[4 * q]), __float_as_uint(w[4 * q + 1]),
                                    __float_as_uint(w[4 * q + 2]), __float_as_uint(w[4 * q + 3])));
-            fence_async_smem();
             __syncwarp();
-            if (lane == 0) {
-              if (job.add)
-                tma_add_2d(out, stg, n0 + c * CHUNK, y);
-              else
-                tma_store_2d(out, stg, n0 + c * CHUNK, y);
-              bulk_commit();
+            float* o = job.f32 + (t.split * (int64_t)job.f32_rows + r0) * a.d4 + n0 + c * CHUNK;
+            const int col = (lane & 7) * 4;
+#pragma unroll
+            for (int q = 0; q < 8; q++) {
+              const int r = q * 4 + (lane >> 3);
+              const uint4 k = stage_get(stg, r, lane & 7);
+              if (col < left) {
+                if (job.add)
+                  add_f32x4(o + (int64_t)r * a.d4 + col, k);
+                else
+                  *reinterpret_cast<uint4*>(o + (int64_t)r * a.d4 + col) = k;
+              }
             }
+            __syncwarp();
           } else {
-            if (left + (c & 1) * CHUNK <= 0) continue;  // the 64 columns of a staging tile
+            if (left + h * CHUNK <= 0) continue;  // the 64 columns of a staging tile
 #pragma unroll
             for (int i = 0; i < CHUNK; i++) w[i] *= f;
-            if ((c & 1) == 0) stage_ready(lane);
-            stage_row16<F16>(stg, lane, c & 1, w);
-            if ((c & 1) == 0) continue;
-            fence_async_smem();
+            stage_row16<F16>(stg, lane, h, w);
+            if (h == 0) continue;
             __syncwarp();
-            if (!job.out) {
-              if (lane == 0) {
-                tma_store_2d(out, stg, n0 + (c - 1) * CHUNK, job.row0 + r0);
-                bulk_commit();
+            const int64_t first = job.row0 + (int64_t)r0, rows = a.classes - first;
+            uint16_t* o = job.out + first * job.out_stride + n0 + c0 * CHUNK;
+            const int here = left + CHUNK;  // of the staging tile's 64 columns
+            if (job.out_vec) {
+              const int col = (lane & 7) * 8;
+#pragma unroll
+              for (int q = 0; q < 8; q++) {
+                const int r = q * 4 + (lane >> 3);
+                const uint4 k = stage_get(stg, r, lane & 7);
+                if (r < rows && col < here) *reinterpret_cast<uint4*>(o + r * job.out_stride + col) = k;
               }
             } else {
-              // Rows that TMA cannot address: the warp stores them one by one,
-              // two elements a lane.
-              const int64_t first = job.row0 + (int64_t)r0, rows = a.classes - first;
-              uint16_t* o = job.out + first * job.out_stride + n0 + (c - 1) * CHUNK;
-              const int here = left + CHUNK;
+              // Rows that 16-byte stores cannot address, two elements a lane.
               for (int r = 0; r < 32 && r < rows; r++, o += job.out_stride) {
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                  const int e = lane + 32 * h;
+                for (int k = 0; k < 2; k++) {
+                  const int e = lane + 32 * k;
                   if (e < here)
                     o[e] = *reinterpret_cast<uint16_t*>(stg + r * 128 + ((((e >> 3) ^ (r & 7)) << 4) | (e & 7) << 1));
                 }
               }
-              __syncwarp();
             }
+            __syncwarp();
           }
         }
       }
     }
-    if (MODE != kCeLse && lane == 0) bulk_wait_all();  // shared memory is read until then
+    if (MODE == kCeGrad && lane == 0) bulk_wait_read<0>();  // shared memory must stay until then
   }
   tc_fence_before();
   __syncthreads();
