@@ -632,8 +632,8 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   a.classes = (int)c.classes;
   a.d = (int)c.d;
   a.kblocks = (int)((c.d + kCeK - 1) / kCeK);
-  // kind::f16, f32 accumulator, M = 256; operand types by bits 7 and 10.
-  a.idesc = (1u << 4) | ((uint32_t)(kCeM >> 4) << 24) | (f16 ? 0u : (1u << 7) | (1u << 10));
+  // kind::f16, f32 accumulator; operand types by bits 7 and 10.
+  a.idesc = (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10));
   a.target = k.target;
   a.c2 = c.scale * kLog2e;
   return VRS_OK;
@@ -649,10 +649,10 @@ int forward(const Call& c, const Plan& p, float* loss, float* lse) {
   VRS_TRY(start(c, p, k, maps, a, false));
   a.vn = a.classes;
   // One tile of rows reads the table at the speed of memory: where at most
-  // half of the pairs would have a tile in the last turn, halves of tiles
-  // shorten it.
-  const int64_t rest = p.vtiles % kPairs;
-  a.whole = (int)(c.rows <= kCeM && 2 * rest <= kPairs ? p.vtiles - rest : p.vtiles);
+  // half of the CTAs or pairs would have a tile in the last turn, halves of
+  // tiles shorten it.
+  const int64_t units = ce_single(a.one_tile_rows) ? 2 * kPairs : kPairs, rest = p.vtiles % units;
+  a.whole = (int)(c.rows <= kCeM && 2 * rest <= units ? p.vtiles - rest : p.vtiles);
   a.vtiles = a.whole == p.vtiles ? a.whole : a.whole + (int)((c.classes - a.whole * (int64_t)kCeN + 127) / 128);
   a.parts = (int)p.parts;
   a.part_rows = c.rows;

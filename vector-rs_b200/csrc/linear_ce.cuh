@@ -54,7 +54,7 @@ struct CeGemm {
   int kblocks;       // of d
   int vtiles;        // class tiles of the piece
   int parts;         // kCeLse: 128-class parts of a row
-  uint32_t idesc;    // types; majorness and N are added per tile
+  uint32_t idesc;    // types; majorness, M and N are added by the kernel
   // scores
   const int64_t* targets;  // [rows] where the rows are not packed, else null
   const int* target;       // [rows] of the taking rows
@@ -73,6 +73,9 @@ struct CeGemm {
 struct CeMaps {
   CUtensorMap a0, b0, out0, a1, b1;
 };
+
+// Whether the score modes run on single CTAs (twice as many tiles at a time).
+inline bool ce_single(int one_tile_rows) { return one_tile_rows > 0 && one_tile_rows <= 128; }
 
 int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s);
 

@@ -39,16 +39,19 @@ constexpr int CHUNK = 32;             // columns that an epilogue warp loads at 
 constexpr int PART = 128;             // columns of one maximum and sum of the scores
 constexpr int kTileCost = 4;          // of a tile beside its K blocks, in K blocks
 constexpr uint32_t BOX = 64 * 128;    // bytes of a 64 x 64 tile of 16-bit operands
-constexpr uint32_t STAGE = 4 * BOX;   // a CTA's halves: A 128 x 64, B 128 x 64
+// A CTA's A, 128 x 64, and its half of B, 128 x 64, or without a partner all 256 x 64.
+constexpr uint32_t stage_bytes(bool pair) { return (pair ? 4 : 6) * BOX; }
 constexpr uint32_t STG = 32 * 128;    // a warp's staging tile: 32 rows of 128 bytes
 constexpr size_t SMEM_BAR = 512;
 constexpr uint64_t WAIT_NS = 2000000000ull;
 
-constexpr int stages(int mode) { return mode == kCeGrad ? 5 : 6; }
-constexpr size_t smem_bytes(int mode) {
-  return 1024 + (size_t)stages(mode) * STAGE + (mode == kCeLse ? 0 : epi_warps(mode) * STG) + SMEM_BAR;
+constexpr int stages(int mode, bool pair) { return pair ? mode == kCeGrad ? 5 : 6 : mode == kCeGrad ? 3 : 4; }
+constexpr size_t smem_bytes(int mode, bool pair) {
+  return 1024 + (size_t)stages(mode, pair) * stage_bytes(pair) + (mode == kCeLse ? 0 : epi_warps(mode) * STG) + SMEM_BAR;
 }
-static_assert(smem_bytes(kCeLse) <= 232448 && smem_bytes(kCeGrad) <= 232448 && smem_bytes(kCeStore) <= 232448,
+static_assert(smem_bytes(kCeLse, true) <= 232448 && smem_bytes(kCeGrad, true) <= 232448 &&
+                  smem_bytes(kCeStore, true) <= 232448 && smem_bytes(kCeLse, false) <= 232448 &&
+                  smem_bytes(kCeGrad, false) <= 232448,
               "above the per-block limit");
 
 // ------------------------------------------------------------ PTX wrappers
@@ -61,6 +64,41 @@ __device__ __forceinline__ uint64_t desc_mn(const void* p) {
   d &= ~((uint64_t)0x3FFF << 16);
   d |= (uint64_t)(BOX >> 4) << 16;
   return d;
+}
+
+// A load that completes on a barrier of the pair's even CTA, or of this CTA.
+template <bool PAIR>
+__device__ __forceinline__ void tma_load(void* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  if (PAIR) {
+    tma_load_2d_pair(dst, map, x, y, bar);
+  } else {
+    asm volatile(
+        "cp.async.bulk.tensor.2d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];" ::"r"(
+            smem_u32(dst)),
+        "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar)
+        : "memory");
+  }
+}
+template <bool PAIR>
+__device__ __forceinline__ void mma(uint32_t d, uint64_t ad, uint64_t bd, uint32_t idesc, uint32_t accumulate) {
+  if (PAIR)
+    mma_f16_pair(d, ad, bd, idesc, accumulate);
+  else
+    mma_f16(d, ad, bd, idesc, accumulate);
+}
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint64_t* bar) {
+  if (PAIR)
+    mma_commit_pair(bar, 0x3);
+  else
+    mma_commit(bar);
+}
+template <bool PAIR>
+__device__ __forceinline__ void sync_all() {
+  if (PAIR)
+    cluster_sync();
+  else
+    __syncthreads();
 }
 
 __device__ __forceinline__ void tma_store_2d(const CUtensorMap* map, const void* src, int x, int y) {
@@ -314,10 +352,14 @@ __device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, int half, co
 
 // ------------------------------------------------------------------ kernel
 
-template <int MODE, bool F16>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
+// PAIR: as the head of this file says. Else, scores of up to 128 rows: a CTA by
+// itself, M = 128, takes tiles of its own; a partner would multiply zeros, and
+// these calls wait for the table to come from memory.
+template <int MODE, bool F16, bool PAIR>
+__global__ void __launch_bounds__(threads(MODE), 1)
     ce_gemm_kernel(const __grid_constant__ CeMaps maps, const __grid_constant__ CeGemm a) {
-  constexpr int ST = stages(MODE), EW = epi_warps(MODE);
+  constexpr int ST = stages(MODE, PAIR), EW = epi_warps(MODE);
+  constexpr uint32_t STAGE = stage_bytes(PAIR);
   constexpr int HCOLS = 2048 / EW;  // columns of an epilogue warp: the tile's or half of them
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = (uint8_t*)(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -331,9 +373,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
   volatile int* s_abort = (volatile int*)(s_tmem + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int cta = (int)cluster_ctarank();
+  const int cta = PAIR ? (int)cluster_ctarank() : 0;
   const bool lead = cta == 0;
-  const int pair = blockIdx.x >> 1, npairs = gridDim.x >> 1;
+  const int pair = PAIR ? blockIdx.x >> 1 : blockIdx.x, npairs = PAIR ? gridDim.x >> 1 : gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; s++) {
@@ -342,7 +384,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     }
     for (int b = 0; b < 2; b++) {
       mbar_init(&tfull[b], 1);
-      mbar_init(&tempty[b], EW);  // of both CTAs, half of them take the buffer's tiles
+      mbar_init(&tempty[b], PAIR ? EW : EW / 2);  // half of a CTA's take the buffer's tiles
     }
     *s_abort = 0;
     fence_mbar_init();
@@ -356,7 +398,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     }
     if (MODE == kCeGrad) prefetch_tmap(&maps.out0);
   }
-  if (warp == 2) tmem_alloc_pair(s_tmem, 512);
+  if (warp == 2) {
+    if (PAIR)
+      tmem_alloc_pair(s_tmem, 512);
+    else
+      tmem_alloc(s_tmem, 512);
+  }
   if (MODE != kCeStore && a.one_tile_rows) {
     const int skip = (int)a_bytes(a, cta);
     for (int s = 0; s < ST; s++)
@@ -365,7 +412,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     fence_async_smem();
   }
   tc_fence_before();
-  cluster_sync();  // barriers initialised and TMEM allocated in both CTAs
+  sync_all<PAIR>();  // barriers initialised and TMEM allocated in both CTAs
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
   // The set-up above overlaps the end of the kernel before; its results are
@@ -380,7 +427,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
     // 512 clocks, which one thread for all of them did not always meet.
     if (lane == 0) {
       const bool for_a = warp == 0;
-      const uint32_t full0 = mapa_shared(full, 0);
+      const uint32_t full0 = PAIR ? mapa_shared(full, 0) : smem_u32(full);
       const uint32_t bytes_a = MODE == kCeStore ? 4 * BOX : a_bytes(a, 0) + a_bytes(a, 1);
       const bool load_a = MODE == kCeStore || a_bytes(a, cta) > 0;
       int s = 0, it = 0;
@@ -389,9 +436,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
       for (int i = 0, id; ok && (id = nth_tile<MODE>(cnt, i, pair, npairs)) >= 0; i++) {
         const Tile t = tile_at<MODE>(a, cnt, id);
         const int ra = t.m * kCeM + cta * 128;
-        const int rb = t.n + cta * (t.bn >> 1);
-        const bool two = t.bn == 256;  // 64-column boxes of B in each CTA
-        const uint32_t bytes = bytes_a + (two ? 4 : 2) * BOX;
+        const int boxes = PAIR ? t.bn >> 7 : t.bn >> 6;  // of 64 columns of B in each CTA
+        const int rb = t.n + cta * boxes * 64;
+        const bool two = boxes == 2;
+        const uint32_t bytes = bytes_a + (t.bn >> 6) * BOX;
         const CUtensorMap* map = for_a ? (MODE == kCeStore && t.job ? &maps.a1 : &maps.a0)
                                        : (MODE == kCeStore && t.job ? &maps.b1 : &maps.b0);
         const int v0 = MODE == kCeStore && t.job ? 0 : a.v0;
@@ -406,7 +454,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
           if (for_a) {
             if (lead) mbar_expect_tx(&full[s], bytes);
             if (MODE != kCeStore) {
-              if (load_a) tma_load_2d_pair(to, map, k, ra, bar);
+              if (load_a) tma_load<PAIR>(to, map, k, ra, bar);
             } else if (t.job == 0) {
               tma_load_2d_pair(to, map, k, ra, bar);
             } else {
@@ -415,8 +463,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
             }
           } else {
             if (MODE != kCeStore) {
-              tma_load_2d_pair(to + 2 * BOX, map, k, v0 + rb, bar);
-              if (two) tma_load_2d_pair(to + 3 * BOX, map, k, v0 + rb + 64, bar);
+              for (int i = 0; i < boxes; i++) tma_load<PAIR>(to + (2 + i) * BOX, map, k, v0 + rb + 64 * i, bar);
             } else {
               tma_load_2d_pair(to + 2 * BOX, map, rb, v0 + k, bar);
               if (two) tma_load_2d_pair(to + 3 * BOX, map, rb + 64, v0 + k, bar);
@@ -453,7 +500,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
         // (A split without K blocks commits at once: its epilogue stores zeros.)
         const uint32_t d = tmem + b * 256;
         const bool a_mn = MODE == kCeStore && t.job == 1, b_mn = MODE == kCeStore;
-        const uint32_t idesc = a.idesc | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(t.bn >> 3) << 17);
+        const uint32_t idesc = a.idesc | ((uint32_t)a_mn << 15) | ((uint32_t)b_mn << 16) | ((uint32_t)(t.bn >> 3) << 17) |
+                               ((PAIR ? 256u : 128u) >> 4 << 24);
         const uint64_t ad0 = a_mn ? ma : ka, bd0 = b_mn ? mb : kb_;
         // 16 of K: 32 bytes on in a K-major row, 16 rows on in an MN-major box.
         const uint32_t astep = a_mn ? 2048 >> 4 : 32 >> 4, bstep = b_mn ? 2048 >> 4 : 32 >> 4;
@@ -466,14 +514,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
           const uint64_t ad = ad0 + s * (STAGE >> 4), bd = bd0 + s * (STAGE >> 4);
 #pragma unroll
           for (int ks = 0; ks < 4; ks++)
-            mma_f16_pair(d, ad + ks * astep, bd + ks * bstep, idesc, kb > t.kb0 || ks > 0 ? 1u : 0u);
-          mma_commit_pair(&empty[s], 0x3);
+            mma<PAIR>(d, ad + ks * astep, bd + ks * bstep, idesc, kb > t.kb0 || ks > 0 ? 1u : 0u);
+          commit<PAIR>(&empty[s]);
           if (++s == ST) {
             s = 0;
             phase ^= 1;
           }
         }
-        mma_commit_pair(&tfull[b], 0x3);
+        commit<PAIR>(&tfull[b]);
         last = tn;
       }
       if (*s_abort && last >= 0) {
@@ -651,36 +699,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(threads(MODE), 1)
   }
   tc_fence_before();
   __syncthreads();
-  cluster_sync();  // no MMA, load or remote arrival of either CTA is still pending
+  if (PAIR) cluster_sync();  // no MMA, load or remote arrival of either CTA is still pending
   if (warp == 2) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    if (PAIR)
+      tmem_dealloc_pair(tmem, 512);
+    else
+      tmem_dealloc(tmem, 512);
   }
 }
 
-// Pairs of the kernel that the current device runs at the same time, asked
-// once per device (with the shared memory that the kernel needs allowed).
-template <int MODE, bool F16>
-int pairs_of(int* out) {
+// CTAs (or pairs) of the kernel that the current device runs at the same time,
+// asked once per device, with the shared memory that it needs allowed.
+template <int MODE, bool F16, bool PAIR>
+int units_of(const cudaLaunchConfig_t& cfg, int* out) {
   static std::atomic<int> cached[128];
   int dev = 0;
   VRS_CUDA(cudaGetDevice(&dev));
   int n = dev < 128 ? cached[dev].load() : 0;
   if (n == 0) {
-    auto kernel = ce_gemm_kernel<MODE, F16>;
-    constexpr int kSmem = (int)smem_bytes(MODE);
-    VRS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(2);
-    cfg.blockDim = dim3(threads(MODE));
-    cfg.dynamicSmemBytes = kSmem;
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = 2;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    VRS_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    auto kernel = ce_gemm_kernel<MODE, F16, PAIR>;
+    VRS_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem_bytes(MODE, PAIR)));
+    if (PAIR)
+      VRS_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+    else
+      VRS_TRY(sm_count(&n));
     if (n < 1) {
       set_error(VRS_ERR_DRIVER, "linear cross entropy: no CTA pair of the product kernel fits this device");
       return VRS_ERR_DRIVER;
@@ -691,24 +734,48 @@ int pairs_of(int* out) {
   return VRS_OK;
 }
 
-template <int MODE, bool F16>
+template <int MODE, bool F16, bool PAIR>
 int launch(const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s) {
-  int pairs = 0;
-  VRS_TRY((pairs_of<MODE, F16>(&pairs)));
-  const int64_t n = most_tiles < pairs ? most_tiles : pairs;
-  VRS_TRY(launch_after(ce_gemm_kernel<MODE, F16>, (unsigned)(2 * (n < 1 ? 1 : n)), threads(MODE), smem_bytes(MODE),
-                       s, maps, a));
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(PAIR ? 2 : 1);
+  cfg.blockDim = dim3(threads(MODE));
+  cfg.dynamicSmemBytes = smem_bytes(MODE, PAIR);
+  cfg.stream = s;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = PAIR ? 2 : 1;
+  at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  int units = 0;
+  VRS_TRY((units_of<MODE, F16, PAIR>(cfg, &units)));
+  const int64_t n = most_tiles < units ? most_tiles : units;
+  cfg.gridDim = dim3((unsigned)((PAIR ? 2 : 1) * (n < 1 ? 1 : n)));
+  cfg.numAttrs = 2;
+  VRS_CUDA(cudaLaunchKernelEx(&cfg, ce_gemm_kernel<MODE, F16, PAIR>, maps, a));
   count_launch();
   return VRS_OK;
+}
+
+template <int MODE, bool PAIR>
+int launch_type(bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s) {
+  return is_f16 ? launch<MODE, true, PAIR>(maps, a, most_tiles, s) : launch<MODE, false, PAIR>(maps, a, most_tiles, s);
 }
 
 }  // namespace
 
 int launch_ce_gemm(int mode, bool is_f16, const CeMaps& maps, const CeGemm& a, int64_t most_tiles, cudaStream_t s) {
+  const bool pair = !ce_single(a.one_tile_rows);
   switch (mode) {
-    case kCeLse: return is_f16 ? launch<kCeLse, true>(maps, a, most_tiles, s) : launch<kCeLse, false>(maps, a, most_tiles, s);
-    case kCeGrad: return is_f16 ? launch<kCeGrad, true>(maps, a, most_tiles, s) : launch<kCeGrad, false>(maps, a, most_tiles, s);
-    default: return is_f16 ? launch<kCeStore, true>(maps, a, most_tiles, s) : launch<kCeStore, false>(maps, a, most_tiles, s);
+    case kCeLse:
+      return pair ? launch_type<kCeLse, true>(is_f16, maps, a, most_tiles, s)
+                  : launch_type<kCeLse, false>(is_f16, maps, a, most_tiles, s);
+    case kCeGrad:
+      return pair ? launch_type<kCeGrad, true>(is_f16, maps, a, most_tiles, s)
+                  : launch_type<kCeGrad, false>(is_f16, maps, a, most_tiles, s);
+    default: return launch_type<kCeStore, true>(is_f16, maps, a, most_tiles, s);
   }
 }
 
