@@ -245,6 +245,40 @@ def test_many_pieces(gpu):
     assert ((dw.double() - want).abs() <= lim).all()
 
 
+# Tiles enough for several turns of the CTAs (up to 128 rows) and of the pairs,
+# with last turns that are full, half full and shorter.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d", [(64, 38000, 24), (65, 50000, 40), (128, 39000, 72), (129, 20000, 33),
+                                            (200, 38100, 64), (256, 19000, 130), (257, 9700, 64), (700, 6500, 320)])
+def test_several_turns(gpu, rows, classes, d):
+    _check(*_make(rows, classes, d, "bfloat16", ignored=0.1))
+
+
+# More rows than a block counts by itself (8,192), with pieces of the classes.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d,ignored", [(8193, 600, 40, 0.0), (9500, 700, 96, 0.5), (20000, 9000, 16, 0.2),
+                                                    (12345, 3, 264, 0.9)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_many_rows(gpu, rows, classes, d, ignored, dtype):
+    _check(*_make(rows, classes, d, dtype, ignored=ignored))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [8, 9, 15, 127, 129, 500, 1001])
+def test_alignments_of_rows(gpu, d):
+    """Every start of a row within 16 bytes: contiguous odd widths, and tables
+    that begin off a 16-byte boundary."""
+    import torch
+    x, w, t, dl = _make(150, 400, d, "float16", ignored=0.2)
+    for o in range(0, 8, 3):
+        bx = torch.zeros(x.numel() + o, dtype=x.dtype, device="cuda")
+        bw = torch.zeros(w.numel() + o, dtype=x.dtype, device="cuda")
+        vx, vw = bx[o:].view_as(x), bw[o:].view_as(w)
+        vx.copy_(x)
+        vw.copy_(w)
+        _check(vx, vw, t, dl)
+
+
 @pytest.mark.gpu
 def test_repeatable_and_empty(gpu):
     import torch
