@@ -32,6 +32,13 @@ constexpr int64_t kPieceBytes = 256ll << 20;
 // CTA pairs that a product is split for (148 SMs). A constant, so that sums
 // are split alike on every device.
 constexpr int kPairs = 74;
+// Products of up to this many multiply-adds take the score gradients as two
+// 16-bit values each, the rounded one and the rest: the products then add
+// nothing to the results' own rounding (error of 8 x 1,398 x 75 in f16 against
+// 64 bits 3.2e-4 with one, PLANES2 with two), for up to a microsecond. Larger ones
+// average the rounding over more terms (at most sqrt 2 of the results' own) and
+// would take half as long again.
+constexpr int64_t kTwoPlanes = 1ll << 28;
 // Up to here each pack block reads all targets itself; above, a first kernel
 // counts them per kSlab rows.
 constexpr int64_t kScanRows = 8192;
@@ -50,7 +57,7 @@ struct Pack1 {
   int64_t classes;
   int per_block;
   int pack_blocks;  // the grid's other blocks copy the table
-  const uint16_t* table;
+  const uint16_t* table;  // as given
   int64_t ts;
   uint16_t* table_out;
   const int2* slabs;  // per slab: taking rows, bits of the largest |dloss|; null: read all targets
@@ -69,6 +76,7 @@ struct Pack1 {
   bool f16;
   float* lse2;
   float* gs;
+  float* gy;
 };
 
 __device__ __forceinline__ bool takes_part(const Pack1& a, int64_t r) {
@@ -277,6 +285,12 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
     } else {
       copy_row(x + row * a.xs, a.d, a.dp, to, row > 0 && row < a.rows - 1 && a.d >= 8);
     }
+    if (BACK) {
+      const uint16_t *from = x + row * a.xs, *w = a.table + a.targets[row] * a.ts;
+      const bool vec = (((uintptr_t)from | (uintptr_t)w) & 15) == 0;
+      const float z = a.f16 ? dot_rows<true>(from, w, a.d, vec) : dot_rows<false>(from, w, a.d, vec);
+      if (lane == 0) a.gy[before + i] = exp2f(z * a.scale * kLog2e - a.lse[row] * kLog2e) - 1.0f;
+    }
   }
   // (Past the last row TMA reads zeros itself.)
   const int64_t tail = min(a.rows, (int64_t)(total + kCeM - 1) / kCeM * kCeM);
@@ -300,10 +314,14 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
   return make_float2(m, a.y * ex2(a.x - sub) + b.y * ex2(b.x - sub));
 }
 
-// loss and lse of rows from their parts' maxima and sums, in units of log 2.
-// The target's score is subtracted before the logarithm is added: where the
-// target is the largest score the difference is exact. A block takes R rows
-// (a power of two up to 32), 1024 / R threads each; the parts lie row by row.
+// loss and lse of rows from their parts' maxima and sums (in units of log 2) and
+// the target's score z: with r the sum of the others' powers relative to the
+// target's, lse = z + log(1 + r) where the target is the largest. loss = lse - z
+// of the 32-bit values that lse and z are, as whoever takes it from the lse
+// handed out would get it. A block takes R rows (a power of two up to 32), 1024
+// / R threads each; the parts lie row by row. One warp a row multiplies the
+// target's score out while the others' loads are on their way.
+template <bool F16>
 __global__ void __launch_bounds__(1024)
     ce_combine_kernel(const CeGemm a, int R, const int* __restrict__ index, float* loss, float* lse) {
   __shared__ float2 s[1024];
@@ -311,6 +329,17 @@ __global__ void __launch_bounds__(1024)
   const int taken = a.rows >= 0 ? a.rows : a.head->taken;
   const int64_t r0 = (int64_t)blockIdx.x * R;
   if (r0 >= taken) return;
+  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const bool mine = w < R && r0 + w < taken;  // this warp's row
+  int64_t tgt = -1;
+  float z = 0.0f;
+  if (mine) {
+    tgt = index ? a.target[r0 + w] : a.targets[r0 + w];
+    if (tgt >= 0 && tgt < a.classes)
+      z = dot_rows<F16>(a.x + (r0 + w) * a.xs, a.w + tgt * a.ws, a.d, true) * a.scale;
+    else
+      tgt = -1;
+  }
   const int64_t row = r0 + threadIdx.x % R;
   const int strips = 1024 / R;
   float2 v = make_float2(-INFINITY, 0.0f);
@@ -321,19 +350,20 @@ __global__ void __launch_bounds__(1024)
   }
   s[threadIdx.x] = v;
   __syncthreads();
-  const int w = threadIdx.x >> 5, lane = threadIdx.x & 31;  // a warp a row
-  if (w >= R || r0 + w >= taken) return;
+  if (!mine) return;
   v = make_float2(-INFINITY, 0.0f);
   for (int k = lane; k < strips; k += 32) v = merge(v, s[k * R + w]);
 #pragma unroll
   for (int o = 16; o; o >>= 1) v = merge(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
   if (lane == 0) {
-    const int64_t r = r0 + w;
-    const float l = log2f(v.y);
-    const int64_t at = index ? index[r] : r;
-    const bool in = index || (a.targets[r] >= 0 && a.targets[r] < a.classes);
-    lse[at] = in ? (v.x + l) * kLn2 : 0.0f;
-    loss[at] = in ? ((v.x - a.zt[r]) + l) * kLn2 : 0.0f;
+    const int64_t at = index ? index[r0 + w] : r0 + w;
+    float all = 0.0f;
+    if (tgt >= 0) {
+      const float z2 = z * kLog2e;
+      all = v.x <= z2 ? z + log1pf(v.y * exp2f(v.x - z2)) : (v.x + log2f(v.y + exp2f(z2 - v.x))) * kLn2;
+    }
+    lse[at] = all;
+    loss[at] = tgt >= 0 ? all - z : 0.0f;
   }
 }
 
@@ -398,7 +428,8 @@ struct Plan {
   int64_t vtiles;                 // class tiles in all
   int64_t parts;                  // and parts of 128 classes
   int splits_dx, splits_dw;
-  int64_t head, slabs, index, pos, target, lse2, gs, xc, wc, part, zt, g, acc_dx, acc_dw, bytes;
+  int planes;                     // of the score gradients
+  int64_t head, slabs, index, pos, target, lse2, gs, gy, xc, wc, part, g, acc_dx, acc_dw, bytes;
 };
 
 // Class tiles of a piece: few pieces of one size, as many (up to twice the
@@ -448,22 +479,23 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
   p.wc = take(aligned ? 0 : classes * p.dp * 2);
   if (!back) {
     p.index = take(rows * 4);
-    p.zt = take(rows * 4);
     p.part = take(rows * p.parts * (int64_t)sizeof(float2));
   } else {
     p.pos = take(rows * 4);
     p.lse2 = take(rows * 4);
     p.gs = take(rows * 4);
+    p.gy = take(rows * 4);
     p.piece = piece_of(p.rows_p, p.vtiles, (d + kCeN - 1) / kCeN) * kCeN;
-    p.g = take(p.rows_p * p.piece * 2);
+    p.planes = rows * classes <= kTwoPlanes / d ? 2 : 1;
+    p.g = take(p.planes * p.rows_p * p.piece * 2);
     // Few tiles: K is split until the pairs have one each, 8 blocks deep at least.
     auto splits = [](int64_t tiles_, int64_t kblocks) {
       int64_t s = kPairs / tiles_ < kblocks / 8 ? kPairs / tiles_ : kblocks / 8;
       return (int)(s < 1 ? 1 : s);
     };
     const int64_t nt = (d + kCeN - 1) / kCeN;
-    p.splits_dx = splits(p.rows_p / kCeM * nt, p.piece / kCeK);
-    p.splits_dw = splits(p.piece / kCeM * nt, (rows + kCeK - 1) / kCeK);
+    p.splits_dx = splits(p.rows_p / kCeM * nt, p.planes * (p.piece / kCeK));
+    p.splits_dw = splits(p.piece / kCeM * nt, p.planes * ((rows + kCeK - 1) / kCeK));
     p.acc_dx = take(p.splits_dx * p.rows_p * p.d4 * 4);
     p.acc_dw = take(p.splits_dw > 1 ? p.splits_dw * p.piece * p.d4 * 4 : 0);
   }
@@ -605,9 +637,9 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
     }
     k.pack_blocks = (int)((c.rows + k.per_block - 1) / k.per_block);
     int64_t blocks = k.pack_blocks;
+    k.table = (const uint16_t*)w;
+    k.ts = c.classes == 1 ? 0 : ts;
     if (copied) {
-      k.table = (const uint16_t*)w;
-      k.ts = ts;
       k.table_out = (uint16_t*)(c.ws + p.wc);
       const int64_t need = (c.classes + 7) / 8, most = (int64_t)sms * 16;
       blocks += need < most ? need : most;
@@ -627,6 +659,10 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   const int box = a.one_tile_rows && c.rows <= 64 ? 64 : 128;
   VRS_TRY(make_map(&maps.a0, type, 2, packed ? k.xc : c.x, c.d, c.rows, packed ? p.dp : c.xs, box));
   VRS_TRY(make_map(&maps.b0, type, 2, w, c.d, c.classes, ts, 64));
+  a.x = (const uint16_t*)(packed ? k.xc : c.x);
+  a.xs = packed ? p.dp : c.rows == 1 ? 0 : c.xs;
+  a.w = (const uint16_t*)w;
+  a.ws = c.classes == 1 ? 0 : ts;
   a.head = k.head;
   a.err = err;
   a.classes = (int)c.classes;
@@ -635,6 +671,7 @@ int start(const Call& c, const Plan& p, Pack1& k, CeMaps& maps, CeGemm& a, bool 
   // kind::f16, f32 accumulator; operand types by bits 7 and 10.
   a.idesc = (1u << 4) | (f16 ? 0u : (1u << 7) | (1u << 10));
   a.target = k.target;
+  a.scale = c.scale;
   a.c2 = c.scale * kLog2e;
   return VRS_OK;
 }
@@ -657,13 +694,13 @@ int forward(const Call& c, const Plan& p, float* loss, float* lse) {
   a.parts = (int)p.parts;
   a.part_rows = c.rows;
   a.part = (float2*)(c.ws + p.part);
-  a.zt = (float*)(c.ws + p.zt);
   VRS_TRY(launch_ce_gemm(kCeLse, c.dtype == VRS_F16, maps, a, p.rows_p / kCeM * a.vtiles, c.s));
   const int* index = a.rows < 0 ? k.index : nullptr;
   // Up to 32 rows a block (whole lines of parts), fewer where blocks are few.
   int R = 1;
   while (R < 32 && R < c.rows && (R < 4 || c.rows > R * 256)) R *= 2;
-  VRS_TRY(launch_after(ce_combine_kernel, (unsigned)((c.rows + R - 1) / R), 1024, 0, c.s, a, R, index, loss, lse));
+  VRS_TRY(launch_after(c.dtype == VRS_F16 ? ce_combine_kernel<true> : ce_combine_kernel<false>,
+                       (unsigned)((c.rows + R - 1) / R), 1024, 0, c.s, a, R, index, loss, lse));
   count_launch();
   return VRS_OK;
 }
@@ -688,15 +725,21 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   k.f16 = f16;
   k.lse2 = (float*)(c.ws + p.lse2);
   k.gs = (float*)(c.ws + p.gs);
+  k.gy = (float*)(c.ws + p.gy);
   VRS_TRY(start(c, p, k, maps, a, true));
   a.lse2 = k.lse2;
   a.gs = k.gs;
+  a.gy = k.gy;
   float* acc_dx = (float*)(c.ws + p.acc_dx);
   float* acc_dw = (float*)(c.ws + p.acc_dw);
   VRS_TRY(make_map(&maps.out0, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 32));
   CeMaps prod;  // of the products
-  VRS_TRY(make_map(&prod.a0, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 128));
-  VRS_TRY(make_map(&prod.a1, type, 2, c.ws + p.g, p.piece, p.rows_p, p.piece, 64));
+  VRS_TRY(make_map(&prod.a0, type, 2, c.ws + p.g, p.piece, p.planes * p.rows_p, p.piece, 128));
+  VRS_TRY(make_map(&prod.a1, type, 2, c.ws + p.g, p.piece, p.planes * p.rows_p, p.piece, 64));
+  a.planes = p.planes;
+  a.plane_rows = (int)p.rows_p;
+  a.g = (uint16_t*)(c.ws + p.g);
+  a.g_pitch = p.piece;
   VRS_TRY(make_map(&prod.b1, type, 2, k.xc, c.d, c.rows, p.dp, 64));
   prod.b0 = maps.b0;
   a.dx.on = dx != nullptr;

@@ -59,14 +59,51 @@ struct CeGemm {
   const int64_t* targets;  // [rows] where the rows are not packed, else null
   const int* target;       // [rows] of the taking rows
   const float* lse2;   // [rows] lse * log2(e)
+  const float* gy;     // [row] the target's probability - 1
   const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
   int64_t part_rows;
   float2* part;        // [part][part_rows]: maximum of c2 z and sum of 2^(c2 z - maximum)
-  float* zt;           // [row] c2 * target's score
+  float scale;
+  const uint16_t* x;   // the rows and the table for the targets' scores, 16-byte aligned
+  int64_t xs;
+  const uint16_t* w;
+  int64_t ws;
   // products
   CeJob dx, dw;
+  int planes;          // of the score gradients: 1, or 2 (rounded value, and what rounding left)
+  int plane_rows;      // rows of a plane
+  uint16_t* g;
+  int64_t g_pitch;
 };
+
+// The product of two rows of d 16-bit floats by one warp, rounded to nearest at
+// every step. The tensor cores' sums are cut off instead: over d terms of one
+// sign, as a trained row's product with its target has, some d / 16 half units
+// of the last place, all downwards. A loss that is small against the target's
+// score, and a probability near 1, would show them (2e-3 of the loss at
+// d = 1,700), so the target's score is computed apart; another class's error is
+// one of many. vec: both rows start on 16 bytes.
+template <bool F16>
+__device__ __forceinline__ float dot_rows(const uint16_t* x, const uint16_t* w, int d, bool vec) {
+  auto value = [](uint16_t u) {
+    return F16 ? __half2float(__ushort_as_half(u)) : __uint_as_float((uint32_t)u << 16);
+  };
+  const int lane = threadIdx.x & 31;
+  float s[2] = {0.0f, 0.0f};
+  int e = vec ? d / 8 * 8 : 0;  // first element read one by one
+  for (int c = lane * 8; c < e; c += 256) {
+    const Pack<uint16_t, 8> p = load_pack<uint16_t, 8>(x + c), q = load_pack<uint16_t, 8>(w + c);
+#pragma unroll
+    for (int j = 0; j < 8; j++) s[j & 1] = fmaf(value(p.v[j]), value(q.v[j]), s[j & 1]);
+  }
+#pragma unroll 4
+  for (e += lane; e < d; e += 32) s[0] = fmaf(value(x[e]), value(w[e]), s[0]);
+  float t = s[0] + s[1];
+#pragma unroll
+  for (int o = 16; o; o >>= 1) t += __shfl_xor_sync(0xffffffffu, t, o);
+  return t;
+}
 
 // Tensor maps of a launch. Scores: a0 rows, b0 table, out0 their gradient.
 // Products: a0, b0 of dx (A: the score gradients), a1, b1 of dtable.

@@ -190,6 +190,13 @@ struct Tiles {
   int long_job, n_long, n_short, ratio;
 };
 
+// A taking row's target; -1 for an unpacked row that takes no part.
+__device__ __forceinline__ int target_of(const CeGemm& a, int64_t row) {
+  if (!a.targets) return a.target[row];
+  const int64_t t = a.targets[row];
+  return t >= 0 && t < a.classes ? (int)t : -1;
+}
+
 template <int MODE>
 __device__ __forceinline__ Tiles count_tiles(const CeGemm& a) {
   Tiles t;
@@ -201,8 +208,8 @@ __device__ __forceinline__ Tiles count_tiles(const CeGemm& a) {
   if (MODE == kCeStore) {
     const int n_dx = a.dx.on ? t.mtiles * a.dx.ntiles * a.dx.splits : 0;
     const int n_dw = a.dw.on ? a.dw.mtiles * a.dw.ntiles * a.dw.splits : 0;
-    const int k_dx = (a.dx.kblocks + a.dx.splits - 1) / a.dx.splits + kTileCost;
-    const int k_dw = (t.kblocks_rows + a.dw.splits - 1) / a.dw.splits + kTileCost;
+    const int k_dx = (a.planes * a.dx.kblocks + a.dx.splits - 1) / a.dx.splits + kTileCost;
+    const int k_dw = (a.planes * t.kblocks_rows + a.dw.splits - 1) / a.dw.splits + kTileCost;
     t.long_job = k_dw > k_dx;
     t.n_long = t.long_job ? n_dw : n_dx;
     t.n_short = t.long_job ? n_dx : n_dw;
@@ -279,7 +286,7 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
   t.split = id % j.splits;
   t.m = id / j.splits;
   t.bn = a.d - t.n > 128 ? 256 : 128;
-  const int kb = t.job ? c.kblocks_rows : j.kblocks;
+  const int kb = a.planes * (t.job ? c.kblocks_rows : j.kblocks);
   const int per = (kb + j.splits - 1) / j.splits;
   t.kb0 = min(kb, t.split * per);
   t.kb1 = min(kb, t.kb0 + per);
@@ -289,9 +296,10 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
 // --------------------------------------------------------------- epilogues
 
 // 32 scores of a row: the running maximum and sum of powers of two (the scores
-// times scale * log2(e), so that e^z is one ex2), and the target's score.
-__device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[CHUNK], int n0, int cols, int64_t row, bool live,
-                                        int tgt, float& top, float& sum) {
+// times scale * log2(e), so that e^z is one ex2). The target's own score is
+// left out: the combining kernel computes it apart.
+__device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[CHUNK], int n0, int cols, int tgt, float& top,
+                                        float& sum) {
   if (cols <= 0) return;
   if (cols < CHUNK) {
 #pragma unroll
@@ -299,11 +307,10 @@ __device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[CHUNK], int 
       if (j >= cols) w[j] = -INFINITY;
   }
   const int at = tgt - n0;
-  if (at >= 0 && at < CHUNK && live) {
-    float z = 0.0f;
+  if (at >= 0 && at < CHUNK) {
 #pragma unroll
-    for (int j = 0; j < CHUNK; j++) z = j == at ? w[j] : z;
-    a.zt[row] = z * a.c2;
+    for (int j = 0; j < CHUNK; j++)
+      if (j == at) w[j] = -INFINITY;
   }
   float m[2];
 #pragma unroll
@@ -319,10 +326,15 @@ __device__ __forceinline__ void epi_lse(const CeGemm& a, float (&w)[CHUNK], int 
     top = now;
   }
   const float sub = top == -INFINITY ? 0.0f : top;
-  float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+  F2 s[2] = {pack_f2(0.0f), pack_f2(0.0f)};
+  const F2 cc = pack_f2(a.c2), dd = pack_f2(-sub);
 #pragma unroll
-  for (int j = 0; j < CHUNK; j++) s[j & 3] += ex2(fmaf(w[j], a.c2, -sub));
-  sum += (s[0] + s[1]) + (s[2] + s[3]);
+  for (int q = 0; q < CHUNK / 2; q++) {
+    float lo, hi;
+    unpack_f2(fma2(pack_f2(w[2 * q], w[2 * q + 1]), cc, dd), lo, hi);
+    s[q & 1] = add2(s[q & 1], pack_f2(ex2(lo), ex2(hi)));
+  }
+  sum += sum_f2(add2(s[0], s[1]));
 }
 
 // A staging tile is free again once its last store has read it.
@@ -348,6 +360,24 @@ __device__ __forceinline__ void stage_row16(uint8_t* stg, int lane, int half, co
     stage_put(stg, lane, half * 4 + q,
               make_uint4(pack2<F16>(w[8 * q], w[8 * q + 1]), pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
                          pack2<F16>(w[8 * q + 4], w[8 * q + 5]), pack2<F16>(w[8 * q + 6], w[8 * q + 7])));
+}
+
+// What rounding to 16 bits leaves of 32 values, itself rounded.
+template <bool F16>
+__device__ __forceinline__ void store_rest(uint16_t* to, const float (&w)[CHUNK]) {
+#pragma unroll
+  for (int q = 0; q < CHUNK / 8; q++) {
+    uint32_t k[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+      const float lo = w[8 * q + 2 * i], hi = w[8 * q + 2 * i + 1];
+      const uint32_t u = pack2<F16>(lo, hi);
+      const float rl = F16 ? __half2float(__ushort_as_half(u & 0xffff)) : __uint_as_float(u << 16);
+      const float rh = F16 ? __half2float(__ushort_as_half(u >> 16)) : __uint_as_float(u & 0xffff0000u);
+      k[i] = pack2<F16>(lo - rl, hi - rh);
+    }
+    *reinterpret_cast<uint4*>(to + 8 * q) = make_uint4(k[0], k[1], k[2], k[3]);
+  }
 }
 
 // ------------------------------------------------------------------ kernel
@@ -450,16 +480,23 @@ __global__ void __launch_bounds__(threads(MODE), 1)
           }
           uint8_t* to = smem + s * STAGE;
           const uint32_t bar = full0 + s * 8;
-          const int k = kb * kCeK;
+          int k = kb * kCeK, plane = 0;
+          if (MODE == kCeStore) {
+            const int kb_plane = t.job ? cnt.kblocks_rows : a.dx.kblocks;
+            if (kb >= kb_plane) {  // the second plane, against the same rows or classes
+              k -= kb_plane * kCeK;
+              plane = a.plane_rows;
+            }
+          }
           if (for_a) {
             if (lead) mbar_expect_tx(&full[s], bytes);
             if (MODE != kCeStore) {
               if (load_a) tma_load<PAIR>(to, map, k, ra, bar);
             } else if (t.job == 0) {
-              tma_load_2d_pair(to, map, k, ra, bar);
+              tma_load_2d_pair(to, map, k, plane + ra, bar);
             } else {
-              tma_load_2d_pair(to, map, ra, k, bar);
-              tma_load_2d_pair(to + BOX, map, ra + 64, k, bar);
+              tma_load_2d_pair(to, map, ra, plane + k, bar);
+              tma_load_2d_pair(to + BOX, map, ra + 64, plane + k, bar);
             }
           } else {
             if (MODE != kCeStore) {
@@ -544,17 +581,13 @@ __global__ void __launch_bounds__(threads(MODE), 1)
       const int n0 = t.n + half * HCOLS;                  // and column
       const bool live = row < taken;
       int tgt = -1;
-      float lse2 = 0.0f, gs = 0.0f;
+      float lse2 = 0.0f, gs = 0.0f, gy = 0.0f;
       if (MODE != kCeStore && live) {
-        if (a.targets) {  // unpacked rows
-          const int64_t g = a.targets[row];
-          tgt = g >= 0 && g < a.classes ? (int)g : -1;
-        } else {
-          tgt = a.target[row];
-        }
+        tgt = target_of(a, row);
         if (MODE == kCeGrad) {
           lse2 = a.lse2[row];
           gs = a.gs[row];
+          gy = a.gy[row];
         }
       }
       const bool ok = mbar_wait(&tfull[group], (tn >> 1) & 1, s_abort, a.err, 34, WAIT_NS);
@@ -595,7 +628,7 @@ __global__ void __launch_bounds__(threads(MODE), 1)
         if (!mine) continue;
         const int left = cols - c * CHUNK;
         if (MODE == kCeLse) {
-          epi_lse(a, w, n0 + c * CHUNK, left, row, live, tgt, top, sum);
+          epi_lse(a, w, n0 + c * CHUNK, left, tgt, top, sum);
           if ((c + 1) * CHUNK % PART == 0) {
             // Neighbouring lanes (rows) side by side.
             const int part = (n0 + c * CHUNK) / PART;
@@ -612,7 +645,7 @@ __global__ void __launch_bounds__(threads(MODE), 1)
           if (at >= 0 && at < CHUNK) {
 #pragma unroll
             for (int j = 0; j < CHUNK; j++)
-              if (j == at) w[j] -= 1.0f;
+              if (j == at) w[j] = gy;
           }
 #pragma unroll
           for (int j = 0; j < CHUNK; j++) w[j] *= gs;
@@ -621,6 +654,7 @@ __global__ void __launch_bounds__(threads(MODE), 1)
             for (int j = 0; j < CHUNK; j++)
               if (!live || j >= left) w[j] = 0.0f;
           }
+          if (a.planes > 1) store_rest<F16>(a.g + (a.plane_rows + row) * a.g_pitch + n0 + c * CHUNK, w);
           if (h == 0) stage_ready(lane);
           stage_row16<F16>(stg, lane, h, w);
           if (h == 1) {
