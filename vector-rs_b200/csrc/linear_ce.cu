@@ -5,6 +5,11 @@
 // A row whose target lies outside the table takes no part: loss 0, lse 0, no
 // gradient, whatever its values are.
 //
+// Forward it reads rows and table once (from memory; the products' tiles again
+// from L2) and does 2 rows classes d operations, backward three times that:
+// the scores are computed again rather than kept (rows x classes values would
+// be read and written at some twice the products' time for d of some hundreds).
+//
 // This file holds the plan of a call and its small kernels; the products are
 // in linear_ce_tc.cu.
 //   forward   pack -> scores (maximum and sum per row and class tile) -> combine
@@ -33,12 +38,14 @@ constexpr int64_t kPieceBytes = 256ll << 20;
 // are split alike on every device.
 constexpr int kPairs = 74;
 // Products of up to this many multiply-adds take the score gradients as two
-// 16-bit values each, the rounded one and the rest: the products then add
-// nothing to the results' own rounding (error of 8 x 1,398 x 75 in f16 against
-// 64 bits 3.2e-4 with one, PLANES2 with two), for up to a microsecond. Larger ones
-// average the rounding over more terms (at most sqrt 2 of the results' own) and
-// would take half as long again.
-constexpr int64_t kTwoPlanes = 1ll << 28;
+// 16-bit values each, the rounded one and the rest, and then add nothing to the
+// results' own rounding: there a result is a sum of so few terms of weight that
+// one term's rounding can show (8 x 1,398 x 75 in f16 against 64 bits: up to
+// 3.2e-4 with one, 2.0e-4 with two, as rounding the exact result leaves). Larger
+// ones average it (at most sqrt 2 of the results' own) and would pay more:
+// backward 8 x 1,398 x 75 23.5 us with one, 28.0 with two; 128 x 8,192 x 256
+// 25.9 and 32.0; 1,024 x 8,192 x 256 40 and 57.
+constexpr int64_t kTwoPlanes = 1ll << 24;
 // Up to here each pack block reads all targets itself; above, a first kernel
 // counts them per kSlab rows.
 constexpr int64_t kScanRows = 8192;

@@ -13,8 +13,13 @@
 // accumulators (2 x 256 columns = all of TMEM). Two groups of epilogue warps a
 // CTA (TMEM lane quadrant x the tile's columns, or half of them) take alternate
 // tiles and read 32 columns ahead, so that one tile is exponentiated or stored
-// while the other accumulator is written. Results leave through swizzled staging tiles and TMA stores, in f32 also as
-// TMA additions to what earlier pieces of the classes left.
+// while the other accumulator is written. The gradient of the scores leaves
+// through swizzled staging tiles and TMA stores; the products, whose rows may
+// start anywhere, through staging tiles that a warp reads back by whole lines,
+// dx adding in f32 to what earlier pieces of the classes left.
+//
+// A row's target takes no part in the sums here, and its gradient is handed in:
+// its score comes from dot_rows, which says why.
 //
 // Bound by the tensor cores for d of some hundreds and more; by the
 // exponentials for small d (one a score, 16 an SM and clock, against
@@ -352,10 +357,10 @@ __device__ __forceinline__ uint4 stage_get(const uint8_t* stg, int row, int j) {
   return *reinterpret_cast<const uint4*>(stg + row * 128 + ((j ^ (row & 7)) << 4));
 }
 
-// Rows first, first + STEP, ... (first < STEP) of a staging tile of 16-bit values to rows that
-// start on (ODD: between) 4-byte words; `here` of their 64 elements. Between
-// words a lane's word holds elements of two lanes, and the first and the last
-// element go by themselves.
+// Rows first, first + STEP, ... (first < STEP) of a staging tile of 16-bit
+// values to rows that start on (ODD: between) 4-byte words; `here` of their 64
+// elements. Between words a lane's word holds elements of two lanes, and the
+// first and the last element go by themselves.
 template <int ODD, int STEP>
 __device__ __forceinline__ void store_rows(uint16_t* o, int64_t pitch, const uint8_t* stg, int first, int all,
                                            int here, int lane) {
@@ -635,8 +640,8 @@ __global__ void __launch_bounds__(threads(MODE), 1)
       float top = -INFINITY, sum = 0.0f;
       float v[2][CHUNK];
       if (mine) tmem_ld_issue(taddr, v[0]);
-      // (Two chunks a turn and no more unrolling: in a small problem this code
-      // runs once, and fetching it was half of the kernel's time.)
+      // Two chunks a turn (one read ahead of the other) and no more unrolling:
+      // in a small problem this code runs once, and its fetch would show.
 #pragma unroll 1
       for (int c0 = 0; c0 < HCOLS / CHUNK; c0 += 2)
 #pragma unroll
