@@ -296,11 +296,17 @@ VRS_API int vrs_selftest_bounded_wait(int64_t limit_ns);
  * entropy of a row's scores against every row of a table (the same inner
  * products that a dot-product search ranks). All buffers are device pointers
  * on the current device; work is queued on cuda_stream (NULL = default
- * stream) and the call returns without waiting; nothing is allocated: scratch
- * is the caller's workspace, whose size the *_workspace calls give, and may
- * be reused as soon as the stream has passed the call. Strides are in
+ * stream) and the call returns without waiting; no device memory is allocated:
+ * scratch is the caller's workspace, whose size the *_workspace calls give, and
+ * may be reused as soon as the stream has passed the call. Strides are in
  * elements, between consecutive rows; elements of a row are contiguous.
- * Results do not depend on timing: the same inputs give the same bits. */
+ * Outputs and workspace overlap neither one another nor the inputs.
+ * Results do not depend on timing: the same inputs give the same bits.
+ * Calls may be captured in a CUDA graph; the first call of each kind on a
+ * device (it sets kernel attributes up, and in a process takes a word of
+ * pinned host memory) should precede the capture. Stage names of
+ * vrs_profile_read: "layer_norm_forward", "layer_norm_backward",
+ * "linear_cross_entropy_forward", "linear_cross_entropy_backward". */
 typedef enum vrs_dtype { VRS_F32 = 0, VRS_F16 = 1, VRS_BF16 = 2 } vrs_dtype;
 
 /* y = (x - mean) * rstd * weight + bias per row of d elements (1..32768),
@@ -329,7 +335,11 @@ VRS_API int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const voi
  * whatever its values: loss 0, lse 0, no gradient. The workspace must be
  * 256-byte aligned. `aligned` of the workspace call: 1 when table starts on
  * 16 bytes with a stride that is a multiple of 8; 0 sizes it for any
- * alignment (room for a copy of the table). */
+ * alignment (room for a copy of the table). Limits: d 1..65536, rows and
+ * classes below 2^31 - 512, rows x classes at most 2^46. The loss is the
+ * difference of the 32-bit lse and target's score. Waits on the device are
+ * bounded; one that gave up (which no correct launch does) is reported as
+ * VRS_ERR_TIMEOUT by the next call of these two functions. */
 VRS_API int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
                                                int32_t backward, int32_t aligned, int64_t* out_bytes);
 VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t rows, const void* table,

@@ -6,6 +6,9 @@ Names, argument meaning and error behaviour follow the Rust crate
 ``DistributedKMeansEngine``, ``DistanceMetric``, ``SearchResult``,
 ``CudaError``. Every call goes through the C ABI in include/vrs.h; there is
 no CPU fallback -- a missing library or GPU raises.
+
+``vector_cuda.ops`` (imported by itself; it needs torch) holds the training
+operators: layer norm and the linear cross entropy.
 """
 from __future__ import annotations
 
