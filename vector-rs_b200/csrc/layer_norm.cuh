@@ -14,13 +14,17 @@
 #include <atomic>
 
 #include "ops_common.cuh"
+#include "tc_common.cuh"
 
 namespace vrs {
 namespace ops {
 
 constexpr int kLnThreads = 256;
 constexpr int kLnMaxCluster = 8;
+constexpr int kLnDevices = 16;  // whose answers are kept
 constexpr int64_t kLnMaxD = 32768;
+constexpr uint64_t kLnWaitNs = 2000000000ull;
+constexpr int kLnWaitCode = 41;
 
 struct LnArgs {
   const void* x;
@@ -40,6 +44,7 @@ struct LnArgs {
   int64_t xs, dys, ys;  // row strides in elements
   int d;
   float eps;
+  int* err;            // host-visible word that a wait which gave up writes
 };
 
 // How a row is held, by its width.
@@ -48,9 +53,11 @@ struct LnArgs {
 //   narrow   up to 4,096: 32 to 256 threads, 16 elements each
 //   wide     up to 8,192, forward only (the backward pass holds five values an
 //            element): 256 threads, 32 elements each
-//   cluster  2 to 8 blocks, 16 elements a thread, or in the forward pass of
-//            many rows 32 (fewer blocks to a reduction over a cluster: 6,000 x
-//            16,384 in bf16 124 us with clusters of 2, 151 us with 4)
+//   cluster  the fewest of 2 to 8 blocks (2,248 x 20,016 in bf16: forward 61 us
+//            with 3 and backward 136 with 5, powers of two, 4 and 8, 110 and 181), 16
+//            elements a thread, or in the forward pass of many rows 32 (fewer
+//            blocks to a reduction over a cluster: 6,000 x 16,384 in bf16 124 us
+//            with clusters of 2, 151 us with 4)
 enum LnClass : int { kLnSmall, kLnNarrow, kLnWide, kLnCluster, kLnWideCluster };
 constexpr int kSmallE = 8, kSmallRows = 2, kNarrowE = 16, kWideE = 32;
 
@@ -59,7 +66,7 @@ struct LnPlan {
   int tpr;      // threads of a row within a block (4..256)
   int cluster;  // blocks of a row (1: none)
   bool vec;     // 16-byte accesses
-  int blocks;   // grid, in clusters
+  int blocks;   // grid, in clusters: at most so many
 };
 
 // The fewest threads that hold a row; a row wider than one block takes a
@@ -81,14 +88,15 @@ inline LnPlan ln_plan(int64_t rows, int d, bool allow_wide, int vec, bool can_ve
   } else {
     p.cls = kLnCluster;
     p.tpr = kLnThreads;
-    while (p.cluster * kLnThreads * kNarrowE < d) p.cluster *= 2;
+    p.cluster = (d + kLnThreads * kNarrowE - 1) / (kLnThreads * kNarrowE);
     if (allow_wide && rows * p.cluster > sms) {
-      p.cluster /= 2;
+      p.cluster = (d + kLnThreads * kWideE - 1) / (kLnThreads * kWideE);
       p.cls = p.cluster > 1 ? kLnWideCluster : kLnWide;
     }
   }
   if (p.tpr == kLnThreads && rows * p.cluster <= sms) {
-    while (p.cluster < kLnMaxCluster && rows * p.cluster <= sms && (int64_t)p.cluster * 2 * kLnThreads * step <= d)
+    while (p.cluster * 2 <= kLnMaxCluster && rows * p.cluster <= sms &&
+           (int64_t)p.cluster * 2 * kLnThreads * step <= d)
       p.cluster *= 2;
     if (p.cluster > 1) p.cls = kLnCluster;
   }
@@ -105,14 +113,38 @@ inline LnPlan ln_plan(int64_t rows, int d, bool allow_wide, int vec, bool can_ve
 // are added (4 values: 6 shuffles, not 20). `slot` alternates between two
 // buffers, so one barrier a reduction suffices: a buffer is written again only
 // after the next reduction's barrier.
+//
+// Between the blocks of a cluster the sums travel as asynchronous stores that
+// complete on a barrier of the block they go to. (A cluster barrier in their
+// place would wait for each thread's own stores of the row before: FIG_CL.)
+// A block sends its next-but-one sums only after it has all blocks' next ones,
+// which they send after they have read the last ones: two buffers suffice here
+// too. A wait that gives up says so and goes on with NaN, so that all threads
+// take the same turns.
 template <int TPR, bool CL, int N>
 struct LnReduce {
   static constexpr int kWarps = kLnThreads / 32;
   struct alignas(16) Smem {
     float warp[2][kWarps][N];
     float cta[2][kLnMaxCluster][N];
+    alignas(8) uint64_t bar[2];
+    volatile int abort;
   };
-  __device__ static __forceinline__ void run(float (&v)[N], Smem* s, int slot) {
+  // Before the first reduction, by all threads of a cluster.
+  __device__ static __forceinline__ void start(Smem* s) {
+    if constexpr (CL) {
+      if (threadIdx.x == 0) {
+        tc::mbar_init(&s->bar[0], 1);
+        tc::mbar_init(&s->bar[1], 1);
+        s->abort = 0;
+        tc::fence_mbar_init();
+      }
+      cooperative_groups::this_cluster().sync();
+    }
+  }
+  // The turn-th reduction.
+  __device__ static __forceinline__ void run(float (&v)[N], Smem* s, int turn, int* err) {
+    const int slot = turn & 1;
     if constexpr (TPR < 32) {
 #pragma unroll
       for (int o = TPR / 2; o > 0; o >>= 1)
@@ -153,16 +185,26 @@ struct LnReduce {
       }
     }
     if constexpr (CL) {
+      static_assert(N <= 2, "sums of one row");
       auto cluster = cooperative_groups::this_cluster();
       const int c = (int)cluster.num_blocks(), r = (int)cluster.block_rank();
-      if ((int)threadIdx.x < c) {
-        float* to = cluster.map_shared_rank(&s->cta[slot][r][0], threadIdx.x);
-#pragma unroll
-        for (int n = 0; n < N; n++) to[n] = v[n];
+      if ((int)threadIdx.x < c && !s->abort) {
+        if (threadIdx.x == 0) tc::mbar_expect_tx(&s->bar[slot], c * N * 4);
+        const uint32_t to = tc::mapa_shared(&s->cta[slot][r][0], threadIdx.x);
+        const uint32_t bar = tc::mapa_shared(&s->bar[slot], threadIdx.x);
+        if constexpr (N == 1)
+          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.f32 [%0], %1, [%2];" ::"r"(to), "f"(v[0]),
+                       "r"(bar)
+                       : "memory");
+        else
+          asm volatile("st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::"r"(to),
+                       "f"(v[0]), "f"(v[N - 1]), "r"(bar)
+                       : "memory");
       }
-      cluster.sync();
+      const bool ok = tc::mbar_try_wait(&s->bar[slot], turn >> 1 & 1) ||
+                      (!s->abort && tc::mbar_wait(&s->bar[slot], turn >> 1 & 1, &s->abort, err, kLnWaitCode, kLnWaitNs));
 #pragma unroll
-      for (int n = 0; n < N; n++) v[n] = 0.0f;
+      for (int n = 0; n < N; n++) v[n] = ok ? 0.0f : NAN;
       for (int b = 0; b < c; b++)
 #pragma unroll
         for (int n = 0; n < N; n++) v[n] += s->cta[slot][b][n];
@@ -171,14 +213,18 @@ struct LnReduce {
 };
 
 // A ring in shared memory for the rows a thread will hold next: asynchronous
-// 16-byte copies into slots of its own (nobody else reads them, so no barrier
-// is added), DEPTH - 1 turns ahead. R rows and ARRAYS arrays a turn; thread tt
+// copies of 16 bytes, or of one 32-bit element, into slots of its own (nobody
+// else reads them, so no barrier is added), DEPTH - 1 turns ahead. R rows and ARRAYS arrays a turn; thread tt
 // of a row's TT holds the accesses i * TT + tt. Columns past the row's end are
-// zeros and stay so. Without 16-byte accesses rows are loaded when needed.
-template <class T, int VEC, int E, int R, int ARRAYS>
+// zeros and stay so. Single elements are copied so where a cluster's turn is long
+// (8193 floats: forward 162 us, loaded when needed 229; 1,023 floats, backward,
+// the other way 117 and 98); 16-bit ones cannot be.
+template <class T, int VEC, int E, int R, int ARRAYS, bool CL>
 struct LnRing {
   static constexpr int NV = E / VEC;
-  static constexpr bool kAsync = VEC > 1;
+  static constexpr int kUnit = VEC * (int)sizeof(T);  // bytes of a copy
+  static constexpr bool kAsync = VEC > 1 || (CL && kUnit >= 4);
+  using Unit = Pack<uint32_t, kAsync ? kUnit / 4 : 1>;
   static constexpr int kStage = R * ARRAYS * E * (int)sizeof(T) * kLnThreads;  // bytes of a turn
   static constexpr int kDepth = kStage <= 16384 ? 3 : 2;
   static constexpr int kBytes = kAsync ? kDepth * kStage : 0;
@@ -189,9 +235,9 @@ struct LnRing {
   int64_t apart;  // rows between those of a turn; a turn is R times as long
   int d, tt, TT, at;
 
-  __device__ __forceinline__ uint4* slot(int k, int r, int array, int i) const {
+  __device__ __forceinline__ Unit* slot(int k, int r, int array, int i) const {
     extern __shared__ uint4 s_ring[];
-    return &s_ring[(((k * R + r) * ARRAYS + array) * NV + i) * kLnThreads + threadIdx.x];
+    return reinterpret_cast<Unit*>(s_ring) + (((k * R + r) * ARRAYS + array) * NV + i) * kLnThreads + threadIdx.x;
   }
   __device__ __forceinline__ void fetch(int64_t row, int k) const {
     if constexpr (kAsync) {
@@ -204,7 +250,7 @@ struct LnRing {
 #pragma unroll
             for (int i = 0; i < NV; i++) {
               const int c = (i * TT + tt) * VEC;
-              if (c < d) __pipeline_memcpy_async(slot(k, r, m, i), p + c, 16);
+              if (c < d) __pipeline_memcpy_async(slot(k, r, m, i), p + c, kUnit);
             }
           }
         }
@@ -219,7 +265,7 @@ struct LnRing {
       for (int i = 0; i < NV; i++)
         if ((i * TT + tt) * VEC >= d)
           for (int k = 0; k < kDepth * R * ARRAYS; k++)
-            *slot(k / (R * ARRAYS), k / ARRAYS % R, k % ARRAYS, i) = make_uint4(0, 0, 0, 0);
+            *slot(k / (R * ARRAYS), k / ARRAYS % R, k % ARRAYS, i) = Unit{};
       for (int k = 0; k < kDepth - 1; k++) fetch(row + k * R * apart, k);
     }
   }
@@ -252,8 +298,12 @@ struct LnRing {
   }
 };
 
+// Clusters take the rows in turn, so no more are launched than run at a time (an
+// SM group of the device holds whole clusters only: 1,373 x 32,767 in bf16,
+// backward 203 us, with as many as the SMs' sum would hold 316); p.blocks says
+// how many.
 template <class K>
-int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+int ln_launch(const LnArgs& a, LnPlan& p, cudaStream_t s) {
   auto kernel = K::get();
   const int smem = K::smem();
   if (smem > 16384) {  // beside up to 32 KB of static shared memory
@@ -266,7 +316,6 @@ int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
     }
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(p.blocks * p.cluster + a.col_blocks));
   cfg.blockDim = dim3(kLnThreads);
   cfg.dynamicSmemBytes = (size_t)smem;
   cfg.stream = s;
@@ -281,7 +330,19 @@ int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
     at[1].val.clusterDim.y = 1;
     at[1].val.clusterDim.z = 1;
     cfg.numAttrs = 2;
+    static std::atomic<int> active[kLnDevices][kLnMaxCluster + 1];  // zero: not asked yet
+    int dev = 0;
+    VRS_CUDA(cudaGetDevice(&dev));
+    int n = dev < kLnDevices ? active[dev][p.cluster].load() : 0;
+    if (n == 0) {
+      cfg.gridDim = dim3((unsigned)p.cluster);
+      VRS_CUDA(cudaOccupancyMaxActiveClusters(&n, kernel, &cfg));
+      if (n < 1) n = 1;
+      if (dev < kLnDevices) active[dev][p.cluster].store(n);
+    }
+    if (p.blocks > n) p.blocks = n;
   }
+  cfg.gridDim = dim3((unsigned)(p.blocks * p.cluster + a.col_blocks));
   VRS_CUDA(cudaLaunchKernelEx(&cfg, kernel, a));
   count_launch();
   return VRS_OK;
@@ -289,7 +350,7 @@ int ln_launch(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
 
 // The instantiation for a plan: K<T, P, VEC, TPR, E, R, CL>.
 template <template <class, class, int, int, int, int, bool> class K, bool WIDE, class T, class P, int VEC>
-int ln_dispatch_tpr(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+int ln_dispatch_tpr(const LnArgs& a, LnPlan& p, cudaStream_t s) {
   if (p.cls == kLnCluster) return ln_launch<K<T, P, VEC, kLnThreads, kNarrowE, 1, true>>(a, p, s);
   if constexpr (WIDE) {
     if (p.cls == kLnWideCluster) return ln_launch<K<T, P, VEC, kLnThreads, kWideE, 1, true>>(a, p, s);
@@ -310,12 +371,12 @@ int ln_dispatch_tpr(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
 }
 
 template <template <class, class, int, int, int, int, bool> class K, bool WIDE, class T, class P>
-int ln_dispatch_vec(const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+int ln_dispatch_vec(const LnArgs& a, LnPlan& p, cudaStream_t s) {
   return p.vec ? ln_dispatch_tpr<K, WIDE, T, P, 16 / (int)sizeof(T)>(a, p, s) : ln_dispatch_tpr<K, WIDE, T, P, 1>(a, p, s);
 }
 
 template <template <class, class, int, int, int, int, bool> class K, bool WIDE>
-int ln_dispatch(int dtype, int param_dtype, const LnArgs& a, const LnPlan& p, cudaStream_t s) {
+int ln_dispatch(int dtype, int param_dtype, const LnArgs& a, LnPlan& p, cudaStream_t s) {
   switch (dtype) {
     case VRS_F32: return ln_dispatch_vec<K, WIDE, float, float>(a, p, s);
     case VRS_F16:

@@ -61,7 +61,7 @@ template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
     ln_bwd_kernel(const LnArgs a) {
   constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
-  using Ring = LnRing<T, VEC, E, R, 2>;
+  using Ring = LnRing<T, VEC, E, R, 2, CL>;
   using Red = LnReduce<TPR, CL, 2 * R>;
   __shared__ typename Red::Smem s_red;
   // Sums of the block's columns, or of a column block's strips.
@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
   ring.tt = tt;
   ring.TT = TT;
   ring.start(row0);
+  Red::start(&s_red);
 
   Held<P, E, VEC> w;
   w.fill(1.0f);
@@ -118,7 +119,7 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
     }
   };
   stats(row0);
-  int slot = 0;
+  int turn = 0;
   // Every thread of a block takes the same number of turns; a row past the
   // last one is zeros (with dy = 0 it adds nothing to any sum).
   for (int64_t row = row0, r0 = first * GROUPS; r0 < a.rows; row += R * apart, r0 += R * apart) {
@@ -151,8 +152,7 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
       s[2 * r + 1] = sum_f2(s1);
     }
     ring.done();
-    Red::run(s, &s_red, slot);
-    slot ^= 1;
+    Red::run(s, &s_red, turn++, a.err);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       if (row + r * apart >= a.rows) break;
@@ -224,7 +224,7 @@ template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 struct BwdKernel {
   static auto get() { return &ln_bwd_kernel<T, P, VEC, TPR, E, R, CL>; }
   static int smem() {
-    return LnRing<T, VEC, E, R, 2>::kBytes;
+    return LnRing<T, VEC, E, R, 2, CL>::kBytes;
   }
 };
 
@@ -310,7 +310,7 @@ extern "C" int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const 
                        aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(weight);
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  const LnPlan p = bwd_plan(rows, (int)d, vec, can_vec, sms);
+  LnPlan p = bwd_plan(rows, (int)d, vec, can_vec, sms);
   const bool params = dweight || dbias;
   const bool columns = params && rows <= kColumnRows;
   if (params) {
@@ -338,6 +338,7 @@ extern "C" int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const 
   a.dys = dy_stride;
   a.ys = dx_stride;
   a.d = (int)d;
+  VRS_TRY(error_word(&a.err));
   ProfToken t = prof_begin("layer_norm_backward", s);
   int st = ln_dispatch<BwdKernel, false>(dtype, param_dtype, a, p, s);
   if (st == VRS_OK && a.partial) {

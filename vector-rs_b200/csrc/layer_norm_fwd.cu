@@ -17,7 +17,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
     ln_fwd_kernel(const LnArgs a) {
   constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
   using Red = LnReduce<TPR, CL, R>;
-  using Ring = LnRing<T, VEC, E, R, 1>;
+  using Ring = LnRing<T, VEC, E, R, 1, CL>;
   __shared__ typename Red::Smem s_red;
   int tt = threadIdx.x % TPR, TT = TPR;
   int64_t first = blockIdx.x, step = gridDim.x;
@@ -41,6 +41,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
   ring.tt = tt;
   ring.TT = TT;
   ring.start(row_first);
+  Red::start(&s_red);
   const float inv_d = 1.0f / (float)a.d;
   // The parameters of the thread's columns stay in registers for all rows;
   // without them 1 and 0 give the same bits as leaving the steps out (but for
@@ -54,7 +55,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
     if (a.weight && c < a.d) w.load(i, (const P*)a.weight + c);
     if (a.bias && c < a.d) b.load(i, (const P*)a.bias + c);
   }
-  int slot = 0;
+  int turn = 0;
   // Every thread of a block takes the same number of turns (the barriers
   // inside the reductions); a group past the last row computes on zeros.
   for (int64_t row0 = row_first, r0 = first * GROUPS; r0 < a.rows; row0 += R * apart, r0 += R * apart) {
@@ -70,8 +71,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
       mean[r] = sum_f2(s);
     }
     ring.done();
-    Red::run(mean, &s_red, slot);
-    slot ^= 1;
+    Red::run(mean, &s_red, turn++, a.err);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       mean[r] *= inv_d;
@@ -92,8 +92,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
       }
       rstd[r] = sum_f2(s);
     }
-    Red::run(rstd, &s_red, slot);
-    slot ^= 1;
+    Red::run(rstd, &s_red, turn++, a.err);
 #pragma unroll
     for (int r = 0; r < R; r++) {
       const int64_t row = row0 + r * apart;
@@ -122,28 +121,11 @@ template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 struct FwdKernel {
   static auto get() { return &ln_fwd_kernel<T, P, VEC, TPR, E, R, CL>; }
   static int smem() {
-    return LnRing<T, VEC, E, R, 1>::kBytes;
+    return LnRing<T, VEC, E, R, 1, CL>::kBytes;
   }
 };
 
 }  // namespace
-
-int sm_count(int* out) {
-  static std::atomic<int> cached[128];  // zero: not read yet
-  int dev = 0;
-  VRS_CUDA(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 128 || !cached[dev]) {
-    int n = 0;
-    VRS_CUDA(cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, dev));
-    if (dev < 0 || dev >= 128) {
-      *out = n;
-      return VRS_OK;
-    }
-    cached[dev] = n;
-  }
-  *out = cached[dev];
-  return VRS_OK;
-}
 
 int ln_check(const char* who, int64_t rows, int64_t d, int32_t dtype, int32_t param_dtype) {
   if (dtype < VRS_F32 || dtype > VRS_BF16) return invalid(std::string(who) + ": dtype must be f32, f16 or bf16");
@@ -185,7 +167,8 @@ extern "C" int vrs_layer_norm_forward(const void* x, int64_t x_stride, int64_t r
                        aligned16(y) && aligned16(weight) && aligned16(bias);
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  const LnPlan p = ln_plan(rows, (int)d, true, vec, can_vec, sms, blocks_per_sm(d > kLnThreads * kNarrowE ? kWideE : 0));
+  VRS_TRY(error_word(&a.err));
+  LnPlan p = ln_plan(rows, (int)d, true, vec, can_vec, sms, blocks_per_sm(d > kLnThreads * kNarrowE ? kWideE : 0));
   cudaStream_t s = (cudaStream_t)cuda_stream;
   ProfToken t = prof_begin("layer_norm_forward", s);
   const int st = ln_dispatch<FwdKernel, true>(dtype, param_dtype, a, p, s);

@@ -20,7 +20,6 @@
 // cost nothing and their values, NaN too, reach no sum. It also gives the
 // products an aligned operand whatever x's stride and address are.
 #include <cmath>
-#include <mutex>
 
 #include <cudaTypedefs.h>
 
@@ -535,29 +534,6 @@ int check_workspace(const std::string& who, const void* ws, int64_t have, int64_
 
 // Rows that TMA can address: 16-byte aligned starts.
 bool tma_rows(const void* p, int64_t stride, int64_t rows) { return aligned16(p) && (rows == 1 || stride % 8 == 0); }
-
-// The word that a device wait which gave up writes: host memory that the
-// device sees, so a later call reads it without waiting for anything.
-int error_word(int** out) {
-  static std::mutex mu;
-  static int* word = nullptr;
-  std::lock_guard<std::mutex> g(mu);
-  if (!word) {
-    void* p = nullptr;
-    VRS_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
-    word = static_cast<int*>(p);
-    *word = 0;
-  }
-  const int code = *(volatile int*)word;
-  if (code) {
-    *(volatile int*)word = 0;
-    set_error(VRS_ERR_TIMEOUT, "linear cross entropy: a device wait of an earlier call gave up (stage code " +
-                                   std::to_string(code) + "); its results are not valid");
-    return VRS_ERR_TIMEOUT;
-  }
-  *out = word;
-  return VRS_OK;
-}
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
   static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {

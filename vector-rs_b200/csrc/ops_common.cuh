@@ -188,5 +188,10 @@ inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 // SMs of the current device (148 on B200), read once per device.
 int sm_count(int* out);
 
+// The word that a device wait which gave up writes: host memory that the
+// device sees, so a later call reads it without waiting for anything. An
+// earlier call's gives VRS_ERR_TIMEOUT once.
+int error_word(int** out);
+
 }  // namespace ops
 }  // namespace vrs
