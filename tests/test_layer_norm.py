@@ -276,3 +276,73 @@ def test_python_refusals(gpu):
         with pytest.raises(ValueError):
             bad()
     assert np.isfinite(y.cpu().numpy()).all()
+
+
+# (rows, d, stride - d, offset): rows of 16-bit elements that all start on 4-byte
+# words, all between them, and alternately (odd strides, with even and odd
+# starts), one row and fewer rows than a turn, each width class, a last row whose
+# end is the tensor's.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,d,gap,offset", [
+    (1, 1, 0, 1), (3, 1, 0, 1), (5, 2, 0, 0), (5, 2, 1, 1), (7, 7, 0, 0), (70, 30, 0, 1), (301, 255, 0, 0),
+    (301, 256, 0, 1), (90, 256, 1, 0), (77, 257, 0, 1), (700, 511, 2, 0), (150, 512, 0, 1), (333, 1023, 0, 1),
+    (65, 4095, 0, 0), (66, 4096, 0, 1), (67, 4097, 0, 0), (130, 8192, 0, 1), (131, 8193, 0, 1), (3, 9001, 0, 0),
+    (70, 32767, 0, 1), (66, 32768, 0, 1)])
+@pytest.mark.parametrize("dtype,ptype", [("float16", "float16"), ("bfloat16", "float32")])
+def test_rows_at_any_element(gpu, vc, rows, d, gap, offset, dtype, ptype):
+    import torch
+    t, p = getattr(torch, dtype), getattr(torch, ptype)
+    code = {"float32": 0, "float16": 1, "bfloat16": 2}
+    x, w, b, dy = _make(rows, d, t, p)
+    stride = d + gap
+    span = (rows - 1) * stride + d
+
+    def inside(values=None):
+        """rows x d within NaN, starting `offset` elements on."""
+        whole = torch.full((span + 16,), float("nan"), dtype=t, device="cuda")
+        part = torch.as_strided(whole, (rows, d), (stride, 1), 8 + offset)
+        if values is not None:
+            part.copy_(values)
+        return whole, part
+
+    def beside(whole, part):
+        """Whether the elements around the rows are what they were."""
+        seen = torch.isnan(whole)
+        torch.as_strided(seen, (rows, d), (stride, 1), 8 + offset).fill_(True)
+        return bool(seen.all())
+
+    (xw, xp), (yw, yp), (gw, gp), (dw_, dp) = inside(x), inside(), inside(dy), inside()
+    mean, rstd = torch.empty(rows, device="cuda"), torch.empty(rows, device="cuda")
+    dweight, dbias = torch.empty(d, dtype=p, device="cuda"), torch.empty(d, dtype=p, device="cuda")
+    L, P, I = vc.lib(), ctypes.c_void_p, ctypes.c_int64
+    n = ctypes.c_int64()
+    assert L.vrs_layer_norm_backward_workspace(I(rows), I(d), ctypes.byref(n)) == 0
+    ws = torch.empty(max(1, n.value), dtype=torch.uint8, device="cuda")
+    torch.cuda.synchronize()
+    assert L.vrs_layer_norm_forward(P(xp.data_ptr()), I(stride), I(rows), I(d), code[dtype], P(w.data_ptr()),
+                                    P(b.data_ptr()), code[ptype], ctypes.c_float(1e-5), P(yp.data_ptr()), I(stride),
+                                    P(mean.data_ptr()), P(rstd.data_ptr()), None) == 0
+    assert L.vrs_layer_norm_backward(P(gp.data_ptr()), I(stride), P(xp.data_ptr()), I(stride), I(rows), I(d),
+                                     code[dtype], P(w.data_ptr()), code[ptype], P(mean.data_ptr()),
+                                     P(rstd.data_ptr()), P(dp.data_ptr()), I(stride), P(dweight.data_ptr()),
+                                     P(dbias.data_ptr()), P(ws.data_ptr()), I(n.value), None) == 0
+    torch.cuda.synchronize()
+    assert beside(yw, yp) and beside(dw_, dp)
+    X, W, B, D = x.double(), w.double(), b.double(), dy.double()
+    m = X.mean(1, keepdim=True)
+    r = ((X - m).square().mean(1, keepdim=True) + 1e-5).rsqrt()
+    xh, G = (X - m) * r, D * W
+    e = 160 * U * (xh.abs() + r * X.abs().mean(1, keepdim=True) + 1.0)
+    o = _half_ulp(t)
+    want = xh * W + B
+    _close(yp, want, e * W.abs() + 4 * U * want.abs() + o * want.abs() * 1.01 + _tiny(t), "y")
+    want = r * (G - G.mean(1, keepdim=True) - xh * (G * xh).mean(1, keepdim=True))
+    a0, a1 = G.abs().mean(1, keepdim=True), (G * xh).abs().mean(1, keepdim=True)
+    er = 160 * U * (1 + r * X.abs().mean(1, keepdim=True)) * want.abs()
+    tol = r * (8 * U * (G.abs() + a0 + xh.abs() * a1) + 48 * U * (a0 + xh.abs() * a1) + e * a1 +
+               xh.abs() * e.amax(1, keepdim=True) * a0) + er
+    _close(dp, want, tol + o * want.abs() * 1.01 + _tiny(t), "dx")
+    sw, sb, q = (D * xh).sum(0), D.sum(0), _half_ulp(p)
+    _close(dweight, sw, (rows + 64) * U * (D * xh).abs().sum(0) + (D.abs() * e).sum(0) + q * sw.abs() * 1.01 + _tiny(p),
+           "dweight")
+    _close(dbias, sb, (rows + 64) * U * D.abs().sum(0) + q * sb.abs() * 1.01 + _tiny(p), "dbias")

@@ -60,7 +60,7 @@ __device__ void sum_columns(const LnArgs& a, int block, float (*s)[kColumns][2])
 template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
     ln_bwd_kernel(const LnArgs a) {
-  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
+  constexpr int GROUPS = kLnThreads / TPR;
   using Ring = LnRing<T, VEC, E, R, 2, CL>;
   using Red = LnReduce<TPR, CL, 2 * R>;
   __shared__ typename Red::Smem s_red;
@@ -84,7 +84,11 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
   }
   T* dx = (T*)a.y;
   const float inv_d = 1.0f / (float)a.d;
-  const int64_t apart = step * GROUPS, row0 = first * GROUPS + threadIdx.x / TPR;
+  const int64_t apart = step * GROUPS;
+  LnPlace<VEC> at;
+  at.tt = tt;
+  at.TT = TT;
+  const int64_t row0 = at.start(a, first, GROUPS, threadIdx.x / TPR);
   Ring ring;
   ring.base[0] = (const T*)a.x;
   ring.base[1] = (const T*)a.dy;
@@ -92,19 +96,13 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
   ring.stride[1] = a.dys;
   ring.rows = a.rows;
   ring.apart = apart;
-  ring.d = a.d;
-  ring.tt = tt;
-  ring.TT = TT;
+  ring.at_columns = at;
   ring.start(row0);
   Red::start(&s_red);
 
   Held<P, E, VEC> w;
   w.fill(1.0f);
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = (i * TT + tt) * VEC;
-    if (a.weight && c < a.d) w.load(i, (const P*)a.weight + c);
-  }
+  at.load(w, a.weight);
   F2 dw[E / 2], db[E / 2];
 #pragma unroll
   for (int q = 0; q < E / 2; q++) dw[q] = db[q] = pack_f2(0.0f);
@@ -122,7 +120,7 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
   int turn = 0;
   // Every thread of a block takes the same number of turns; a row past the
   // last one is zeros (with dy = 0 it adds nothing to any sum).
-  for (int64_t row = row0, r0 = first * GROUPS; r0 < a.rows; row += R * apart, r0 += R * apart) {
+  for (int64_t row = row0, r0 = at.first; r0 < a.rows; row += R * apart, r0 += R * apart) {
     float mean[R], rstd[R];
 #pragma unroll
     for (int r = 0; r < R; r++) {
@@ -159,11 +157,7 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
       const F2 f = pack_f2(rstd[r]), m0 = pack_f2(-s[2 * r] * inv_d), m1 = pack_f2(-s[2 * r + 1] * inv_d);
 #pragma unroll
       for (int q = 0; q < E / 2; q++) g[r][q] = mul2(add2(g[r][q], fma2(xh[r][q], m1, m0)), f);
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = (i * TT + tt) * VEC;
-        if (c < a.d) store_held<T, VEC, E>(dx + (row + r * apart) * a.ys + c, g[r], i);
-      }
+      at.template store<T, E>(dx + (row + r * apart) * a.ys, g[r]);
     }
   }
   ring.drain();
@@ -192,8 +186,8 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
         if ((int)threadIdx.x / SPAN == gr && (int)threadIdx.x % SPAN < TPR) {
 #pragma unroll
           for (int e = 0; e < E; e++) {
-            const int c = (e / VEC * TT + tt) * VEC + e % VEC;
-            if (c < a.d) {
+            const int c = at.column(e / VEC) + e % VEC;
+            if (at.has(e / VEC, e % VEC)) {
               s_col[c] = (gr ? s_col[c] : 0.0f) + fw[e];
               s_col[TPR * E + c] = (gr ? s_col[TPR * E + c] : 0.0f) + fb[e];
             }
@@ -208,8 +202,8 @@ __global__ void __launch_bounds__(kLnThreads, kBlocksPerSm)
     } else {
 #pragma unroll
       for (int e = 0; e < E; e++) {
-        const int c = (e / VEC * TT + tt) * VEC + e % VEC;
-        if (c < a.d) {
+        const int c = at.column(e / VEC) + e % VEC;
+        if (at.has(e / VEC, e % VEC)) {
           out[c] = fw[e];
           out[a.d + c] = fb[e];
         }
@@ -228,8 +222,8 @@ struct BwdKernel {
   }
 };
 
-LnPlan bwd_plan(int64_t rows, int d, int vec, bool can_vec, int sms) {
-  return ln_plan(rows, d, false, vec, can_vec, sms, kBlocksPerSm);
+LnPlan bwd_plan(int64_t rows, int d, int vec, LnAccess access, int sms) {
+  return ln_plan(rows, d, false, vec, access, sms, kBlocksPerSm);
 }
 
 // dweight[c], dbias[c] = sum over blocks of partial[b][0 / 1][c]: 32 columns a
@@ -278,11 +272,14 @@ extern "C" int vrs_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_
   VRS_TRY(ln_check("vrs_layer_norm_backward_workspace", rows, d, VRS_F32, VRS_F32));
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  // The plan with and without 16-byte accesses differs in the cluster only,
-  // which lowers the block count.
-  const LnPlan p = bwd_plan(rows, (int)d, 1, false, sms);
-  const LnPlan q = bwd_plan(rows, (int)d, 8, true, sms);
-  *out_bytes = (int64_t)(p.blocks > q.blocks ? p.blocks : q.blocks) * 2 * d * (int64_t)sizeof(float);
+  // How the rows can be reached decides the cluster of few rows and whether
+  // the count of blocks is even.
+  int blocks = 0;
+  for (LnAccess access : {kLnElements, kLn16Bytes, kLnPairs}) {
+    const LnPlan p = bwd_plan(rows, (int)d, 8, access, sms);
+    blocks = blocks > p.blocks ? blocks : p.blocks;
+  }
+  *out_bytes = (int64_t)blocks * 2 * d * (int64_t)sizeof(float);
   return VRS_OK;
 }
 
@@ -304,13 +301,12 @@ extern "C" int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const 
   if (!dy || !x || !mean || !rstd || !dx) return invalid("vrs_layer_norm_backward: null buffer");
   if (rows > 1 && (x_stride < d || dy_stride < d || dx_stride < d))
     return invalid("vrs_layer_norm_backward: row strides must be at least d");
-  const int vec = 16 / dtype_bytes(dtype);
-  const bool can_vec = d % vec == 0 &&
-                       (rows == 1 || (x_stride % vec == 0 && dy_stride % vec == 0 && dx_stride % vec == 0)) &&
-                       aligned16(x) && aligned16(dy) && aligned16(dx) && aligned16(weight);
+  const int bytes = dtype_bytes(dtype);
+  const LnRows arrays[] = {{x, x_stride}, {dy, dy_stride}, {dx, dx_stride}};
+  const LnAccess access = ln_access(arrays, rows, d, bytes, aligned16(weight));
   int sms = 0;
   VRS_TRY(sm_count(&sms));
-  LnPlan p = bwd_plan(rows, (int)d, vec, can_vec, sms);
+  LnPlan p = bwd_plan(rows, (int)d, 16 / bytes, access, sms);
   const bool params = dweight || dbias;
   const bool columns = params && rows <= kColumnRows;
   if (params) {

@@ -15,7 +15,7 @@ constexpr int blocks_per_sm(int e) { return e == kWideE ? 2 : 3; }
 template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
     ln_fwd_kernel(const LnArgs a) {
-  constexpr int NV = E / VEC, GROUPS = kLnThreads / TPR;
+  constexpr int GROUPS = kLnThreads / TPR;
   using Red = LnReduce<TPR, CL, R>;
   using Ring = LnRing<T, VEC, E, R, 1, CL>;
   __shared__ typename Red::Smem s_red;
@@ -31,15 +31,17 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
   grid_launch();
   grid_wait();
   T* y = (T*)a.y;
-  const int64_t apart = step * GROUPS, row_first = first * GROUPS + threadIdx.x / TPR;
+  const int64_t apart = step * GROUPS;
+  LnPlace<VEC> at;
+  at.tt = tt;
+  at.TT = TT;
+  const int64_t row_first = at.start(a, first, GROUPS, threadIdx.x / TPR);
   Ring ring;
   ring.base[0] = (const T*)a.x;
   ring.stride[0] = a.xs;
   ring.rows = a.rows;
   ring.apart = apart;
-  ring.d = a.d;
-  ring.tt = tt;
-  ring.TT = TT;
+  ring.at_columns = at;
   ring.start(row_first);
   Red::start(&s_red);
   const float inv_d = 1.0f / (float)a.d;
@@ -49,16 +51,12 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
   Held<P, E, VEC> w, b;
   w.fill(1.0f);
   b.fill(0.0f);
-#pragma unroll
-  for (int i = 0; i < NV; i++) {
-    const int c = (i * TT + tt) * VEC;
-    if (a.weight && c < a.d) w.load(i, (const P*)a.weight + c);
-    if (a.bias && c < a.d) b.load(i, (const P*)a.bias + c);
-  }
+  at.load(w, a.weight);
+  at.load(b, a.bias);
   int turn = 0;
   // Every thread of a block takes the same number of turns (the barriers
   // inside the reductions); a group past the last row computes on zeros.
-  for (int64_t row0 = row_first, r0 = first * GROUPS; r0 < a.rows; row0 += R * apart, r0 += R * apart) {
+  for (int64_t row0 = row_first, r0 = at.first; r0 < a.rows; row0 += R * apart, r0 += R * apart) {
     ring.next(row0);
     F2 v[R][E / 2];
     float mean[R], rstd[R];
@@ -80,13 +78,13 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
 #pragma unroll
       for (int q = 0; q < E / 2; q++) {
         v[r][q] = add2(v[r][q], m);
-        const int c0 = (2 * q / VEC * TT + tt) * VEC, c1 = ((2 * q + 1) / VEC * TT + tt) * VEC;
-        if constexpr (VEC > 1) {
-          if (c0 < a.d) s = fma2(v[r][q], v[r][q], s);
+        if constexpr (VEC > 2) {
+          if (at.column(2 * q / VEC) < a.d) s = fma2(v[r][q], v[r][q], s);
         } else {
           float lo, hi;
           unpack_f2(v[r][q], lo, hi);
-          const F2 in = pack_f2(c0 < a.d ? lo : 0.0f, c1 < a.d ? hi : 0.0f);
+          const F2 in = pack_f2(at.has(2 * q / VEC, 2 * q % VEC) ? lo : 0.0f,
+                                at.has((2 * q + 1) / VEC, (2 * q + 1) % VEC) ? hi : 0.0f);
           s = fma2(in, in, s);
         }
       }
@@ -105,11 +103,7 @@ __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
       const F2 f = pack_f2(rstd[r]);
 #pragma unroll
       for (int q = 0; q < E / 2; q++) v[r][q] = fma2(mul2(v[r][q], f), w.pair(q), b.pair(q));
-#pragma unroll
-      for (int i = 0; i < NV; i++) {
-        const int c = (i * TT + tt) * VEC;
-        if (c < a.d) store_held<T, VEC, E>(y + row * a.ys + c, v[r], i);
-      }
+      at.template store<T, E>(y + row * a.ys, v[r]);
     }
   }
   ring.drain();
@@ -162,13 +156,13 @@ extern "C" int vrs_layer_norm_forward(const void* x, int64_t x_stride, int64_t r
   a.ys = y_stride;
   a.d = (int)d;
   a.eps = eps;
-  const int vec = 16 / dtype_bytes(dtype);
-  const bool can_vec = d % vec == 0 && (rows == 1 || (x_stride % vec == 0 && y_stride % vec == 0)) && aligned16(x) &&
-                       aligned16(y) && aligned16(weight) && aligned16(bias);
+  const int bytes = dtype_bytes(dtype);
+  const LnRows arrays[] = {{x, x_stride}, {y, y_stride}};
+  const LnAccess access = ln_access(arrays, rows, d, bytes, aligned16(weight) && aligned16(bias));
   int sms = 0;
   VRS_TRY(sm_count(&sms));
   VRS_TRY(error_word(&a.err));
-  LnPlan p = ln_plan(rows, (int)d, true, vec, can_vec, sms, blocks_per_sm(d > kLnThreads * kNarrowE ? kWideE : 0));
+  LnPlan p = ln_plan(rows, (int)d, true, 16 / bytes, access, sms, blocks_per_sm(d > kLnThreads * kNarrowE ? kWideE : 0));
   cudaStream_t s = (cudaStream_t)cuda_stream;
   ProfToken t = prof_begin("layer_norm_forward", s);
   const int st = ln_dispatch<FwdKernel, true>(dtype, param_dtype, a, p, s);
