@@ -307,13 +307,13 @@ struct LnReduce {
 };
 
 // A ring in shared memory for the rows a thread will hold next: asynchronous
-// copies of 16 bytes, or of one 32-bit element, into slots of its own (nobody
-// else reads them, so no barrier is added), DEPTH - 1 turns ahead. R rows and ARRAYS arrays a turn; thread tt
-// of a row's TT holds the accesses i * TT + tt. Columns past the row's end are
-// zeros and stay so. Single 32-bit elements are copied so
-// where a row takes a cluster, whose turns are long (5,492 x 8,193 forward in f32
-// 162 us; in bf16 by elements, which are loaded when needed, 227), and loaded
-// when needed elsewhere (43,988 x 1,023 backward in f32 98 us, copied 117).
+// copies of 16 bytes, a pair or a 32-bit element into slots of its own (nobody
+// else reads them, so no barrier is added), DEPTH - 1 turns ahead. R rows and
+// ARRAYS arrays a turn. Columns past the row's end are zeros and stay so. Single
+// 32-bit elements are copied so where a row takes a cluster, whose turns are long
+// (5,492 x 8,193 forward in f32 162 us; in bf16 by elements, which are loaded
+// when needed, 227), and loaded when needed elsewhere (43,988 x 1,023 backward in
+// f32 98 us, copied 117).
 template <class T, int VEC, int E, int R, int ARRAYS, bool CL>
 struct LnRing {
   static constexpr int NV = E / VEC;
