@@ -301,7 +301,9 @@ VRS_API int vrs_selftest_bounded_wait(int64_t limit_ns);
  * may be reused as soon as the stream has passed the call. Strides are in
  * elements, between consecutive rows; elements of a row are contiguous.
  * Outputs and workspace overlap neither one another nor the inputs.
- * Results do not depend on timing: the same inputs give the same bits.
+ * Results do not depend on timing: on one device the same inputs give the same
+ * bits. Waits within the kernels are bounded; one that gave up (which no correct
+ * launch does) is reported as VRS_ERR_TIMEOUT by the next call of an operator.
  * Calls may be captured in a CUDA graph; the first call of each kind on a
  * device (it sets kernel attributes up, and in a process takes a word of
  * pinned host memory) should precede the capture. Stage names of
@@ -337,9 +339,7 @@ VRS_API int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const voi
  * 16 bytes with a stride that is a multiple of 8; 0 sizes it for any
  * alignment (room for a copy of the table). Limits: d 1..65536, rows and
  * classes below 2^31 - 512, rows x classes at most 2^46. The loss is the
- * difference of the 32-bit lse and target's score. Waits on the device are
- * bounded; one that gave up (which no correct launch does) is reported as
- * VRS_ERR_TIMEOUT by the next call of these two functions. */
+ * difference of the 32-bit lse and target's score. */
 VRS_API int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
                                                int32_t backward, int32_t aligned, int64_t* out_bytes);
 VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t rows, const void* table,
