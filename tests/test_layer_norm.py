@@ -346,3 +346,14 @@ def test_rows_at_any_element(gpu, vc, rows, d, gap, offset, dtype, ptype):
     _close(dweight, sw, (rows + 64) * U * (D * xh).abs().sum(0) + (D.abs() * e).sum(0) + q * sw.abs() * 1.01 + _tiny(p),
            "dweight")
     _close(dbias, sb, (rows + 64) * U * D.abs().sum(0) + q * sb.abs() * 1.01 + _tiny(p), "dbias")
+
+
+# Rows enough to fill the device: widths between powers of two, and odd ones.
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,d", [(12000, 96), (10001, 71), (6000, 136), (3000, 384), (3001, 383), (1300, 700),
+                                    (700, 1500), (401, 3000), (333, 3071)])
+@pytest.mark.parametrize("dtype,ptype", TYPES)
+def test_many_rows(gpu, rows, d, dtype, ptype):
+    import torch
+    x, w, b, dy = _make(rows, d, getattr(torch, dtype), getattr(torch, ptype))
+    _check(x, w, b, dy)

@@ -59,15 +59,19 @@ struct LnArgs {
 //   small    up to 256 elements: 4 to 32 threads, 8 elements each, two rows at
 //            a time (their loads and reductions overlap)
 //   narrow   up to 4,096: 32 to 256 threads, 16 elements each
+//   between  up to 3,072, many rows, forward only: 4 to 128 threads, 24 elements
+//            each, where that leaves fewer idle (45 M elements in bf16: width 136
+//            36 us, as small 82; 768 33, as narrow 45; 1,536 35 and 44)
 //   wide     up to 8,192, forward only (the backward pass holds five values an
 //            element): 256 threads, 32 elements each
 //   cluster  the fewest of 2 to 8 blocks (2,248 x 20,016 in bf16: forward 61 us
 //            with 3 and backward 136 with 5, powers of two, 4 and 8, 110 and 181), 16
 //            elements a thread, or in the forward pass of many rows 32 (fewer
-//            blocks to a reduction over a cluster: 6,000 x 16,384 in bf16 124 us
-//            with clusters of 2, 151 us with 4)
-enum LnClass : int { kLnSmall, kLnNarrow, kLnWide, kLnCluster, kLnWideCluster };
-constexpr int kSmallE = 8, kSmallRows = 2, kNarrowE = 16, kWideE = 32;
+//            blocks to a reduction over a cluster: 3,747 x 12,008 in bf16 57 us
+//            with clusters of 2, 80 us with 3)
+enum LnClass : int { kLnSmall, kLnNarrow, kLnBetween, kLnWide, kLnCluster, kLnWideCluster };
+constexpr int kBetweenBlocks = 2;  // of an SM
+constexpr int kSmallE = 8, kSmallRows = 2, kNarrowE = 16, kBetweenE = 24, kWideE = 32;
 
 enum LnAccess : int { kLnElements, kLn16Bytes, kLnPairs };
 
@@ -106,6 +110,15 @@ inline LnPlan ln_plan(int64_t rows, int d, bool allow_wide, int vec, LnAccess ac
     if (allow_wide && rows * p.cluster > sms) {
       p.cluster = (d + kLnThreads * kWideE - 1) / (kLnThreads * kWideE);
       p.cls = p.cluster > 1 ? kLnWideCluster : kLnWide;
+    }
+  }
+  if (allow_wide && d <= kLnThreads / 2 * kBetweenE) {
+    int t = 4;
+    while (t * kBetweenE < d) t *= 2;
+    if (t * kBetweenE < p.tpr * (p.cls == kLnSmall ? kSmallE : kNarrowE) && rows * t > (int64_t)sms * kLnThreads) {
+      p.cls = kLnBetween;
+      p.tpr = t;
+      blocks_per_sm = kBetweenBlocks;
     }
   }
   if (p.tpr == kLnThreads && rows * p.cluster <= sms) {
@@ -477,6 +490,15 @@ int ln_dispatch_tpr(const LnArgs& a, LnPlan& p, cudaStream_t s) {
     if (p.cls == kLnWideCluster) return ln_launch<K<T, P, VEC, kLnThreads, kWideE, 1, true>>(a, p, s);
     if (p.cls == kLnWide) return ln_launch<K<T, P, VEC, kLnThreads, kWideE, 1, false>>(a, p, s);
   }
+  if constexpr (WIDE)
+    if (p.cls == kLnBetween) switch (p.tpr) {
+        case 4: return ln_launch<K<T, P, VEC, 4, kBetweenE, 1, false>>(a, p, s);
+        case 8: return ln_launch<K<T, P, VEC, 8, kBetweenE, 1, false>>(a, p, s);
+        case 16: return ln_launch<K<T, P, VEC, 16, kBetweenE, 1, false>>(a, p, s);
+        case 32: return ln_launch<K<T, P, VEC, 32, kBetweenE, 1, false>>(a, p, s);
+        case 64: return ln_launch<K<T, P, VEC, 64, kBetweenE, 1, false>>(a, p, s);
+        default: return ln_launch<K<T, P, VEC, 128, kBetweenE, 1, false>>(a, p, s);
+      }
   if (p.cls == kLnSmall) switch (p.tpr) {
       case 4: return ln_launch<K<T, P, VEC, 4, kSmallE, kSmallRows, false>>(a, p, s);
       case 8: return ln_launch<K<T, P, VEC, 8, kSmallE, kSmallRows, false>>(a, p, s);

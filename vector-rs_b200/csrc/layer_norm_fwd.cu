@@ -10,7 +10,7 @@ namespace vrs {
 namespace ops {
 namespace {
 
-constexpr int blocks_per_sm(int e) { return e == kWideE ? 2 : 3; }
+constexpr int blocks_per_sm(int e) { return e == kWideE ? 2 : e == kBetweenE ? kBetweenBlocks : 3; }
 
 template <class T, class P, int VEC, int TPR, int E, int R, bool CL>
 __global__ void __launch_bounds__(kLnThreads, blocks_per_sm(E))
