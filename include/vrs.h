@@ -338,8 +338,9 @@ VRS_API int vrs_layer_norm_backward(const void* dy, int64_t dy_stride, const voi
  * 256-byte aligned. `aligned` of the workspace call: 1 when table starts on
  * 16 bytes with a stride that is a multiple of 8; 0 sizes it for any
  * alignment (room for a copy of the table). Limits: d 1..65536, rows and
- * classes below 2^31 - 512, rows x classes at most 2^46. The loss is the
- * difference of the 32-bit lse and target's score. */
+ * classes below 2^31 - 512, rows x classes at most 2^46. The loss is not
+ * lse - z[target] of the 32-bit values: a loss that is small against the
+ * scores keeps its own digits. */
 VRS_API int vrs_linear_cross_entropy_workspace(int64_t rows, int64_t classes, int64_t d, int32_t dtype,
                                                int32_t backward, int32_t aligned, int64_t* out_bytes);
 VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, int64_t rows, const void* table,

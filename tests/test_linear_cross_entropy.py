@@ -457,3 +457,63 @@ def test_python_refusals(gpu):
         ops.linear_cross_entropy(x, w, t, 1.0, "median")
     with pytest.raises(ValueError):
         ops.linear_cross_entropy_backward(dl.half(), x, w, t, dl)
+
+
+# ------------------------------------------------ rows that are predicted well
+
+
+def _sure(rows, classes, d, dtype, noise, seed=0, offset=0):
+    """Unit rows near their targets, as a trained encoder gives them; `offset`
+    elements off a 16-byte boundary."""
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed + rows * 7 + classes * 3 + d)
+    t = torch.randint(0, classes, (rows,), generator=g, device="cuda")
+    w = torch.randn(classes, d, generator=g, device="cuda")
+    w /= w.norm(dim=1, keepdim=True)
+    x = w[t] + torch.randn(rows, d, generator=g, device="cuda") * (noise / d ** 0.5)
+    x /= x.norm(dim=1, keepdim=True)
+
+    def placed(m):
+        b = torch.zeros(m.numel() + offset, dtype=getattr(torch, dtype), device="cuda")
+        return b[offset:].view_as(m).copy_(m)
+
+    return placed(x), placed(w), t
+
+
+def _sure64(x, w, t, scale):
+    """In 64 bits: loss, the score gradients (the target's without a difference)
+    and a bound on the relative error of the other classes' weight r = sum of
+    e^(z - z[target]) in 32 bits: two scores' errors (as at the head of this file),
+    the rounding of the target's score and of both exponents (2^-22 of the score
+    each), and the exponentials and sums."""
+    import torch
+    X, W = x.double(), w.double()
+    at = t[:, None]
+    z = scale * (X @ W.t())
+    zt = z.gather(1, at)
+    q = torch.exp(z - zt).scatter_(1, at, 0.0)
+    r = q.sum(1, keepdim=True)
+    g = (q / (1 + r)).scatter_(1, at, -r / (1 + r))
+    ez = (x.shape[1] + 2) * 2.0 ** -22 * scale * (X.abs() @ W.abs().t()).amax(1)
+    rel = 2 * ez + 3 * 2.0 ** -22 * zt[:, 0].abs() + 2.0 ** -20
+    return torch.log1p(r)[:, 0], g, rel
+
+
+SURE = [(90, 1000, 64, 0.5, 20.0, 0), (90, 1000, 65, 0.5, 20.0, 0), (300, 700, 33, 0.2, 20.0, 3), (64, 1000, 64, 0.3, 100.0, 0),
+        (40, 300, 71, 0.7, 100.0, 1), (300, 20, 512, 1.0, 20.0, 0), (5, 2, 16, 0.1, 20.0, 0)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d,noise,scale,offset", SURE)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_small_losses_keep_their_digits(gpu, rows, classes, d, noise, scale, offset, dtype):
+    """The loss of a row whose target clearly wins, relative to itself:
+    log(1 + r) errs by at most r's relative error and a rounding (2^-22 with
+    the logarithm's); below 2^-120 32 bits hold no more digits."""
+    from vector_cuda import ops
+    x, w, t = _sure(rows, classes, d, dtype, noise, offset=offset)
+    want, _, rel = _sure64(x, w, t, scale)
+    assert want.median() < 0.02  # (what the case is for)
+    loss, lse = ops.linear_cross_entropy_forward(x, w, t, scale)
+    off = (loss.double() - want).abs()
+    assert (off <= (rel + 2.0 ** -22) * want + 2.0 ** -120).all(), f"worst {(off / want).max().item():.3g} of the loss"

@@ -322,11 +322,14 @@ __device__ __forceinline__ float2 merge(float2 a, float2 b) {
 
 // loss and lse of rows from their parts' maxima and sums (in units of log 2) and
 // the target's score z: with r the sum of the others' powers relative to the
-// target's, lse = z + log(1 + r) where the target is the largest. loss = lse - z
-// of the 32-bit values that lse and z are, as whoever takes it from the lse
-// handed out would get it. A block takes R rows (a power of two up to 32), 1024
-// / R threads each; the parts lie row by row. One warp a row multiplies the
-// target's score out while the others' loads are on their way.
+// target's, loss = log(1 + r) where the target is the largest, and then lse = z +
+// loss. (lse - z would leave a loss that is small against z the last bits of lse
+// only: 1e-2 of a loss of 1e-4 at a score of 18.) Else the differences to z are
+// taken before the logarithm's sum is rounded. z is rounded by itself, not within
+// a sum, so that the backward pass can form the same lse - z. A block takes R
+// rows (a power of two up to 32), 1024 / R threads each; the parts lie row by row.
+// One warp a row multiplies the target's score out while the others' loads are
+// on their way.
 template <bool F16>
 __global__ void __launch_bounds__(1024)
     ce_combine_kernel(const CeGemm a, int R, const int* __restrict__ index, float* loss, float* lse) {
@@ -342,7 +345,7 @@ __global__ void __launch_bounds__(1024)
   if (mine) {
     tgt = index ? a.target[r0 + w] : a.targets[r0 + w];
     if (tgt >= 0 && tgt < a.classes)
-      z = dot_rows<F16>(a.x + (r0 + w) * a.xs, a.w + tgt * a.ws, a.d, true) * a.scale;
+      z = __fmul_rn(dot_rows<F16>(a.x + (r0 + w) * a.xs, a.w + tgt * a.ws, a.d, true), a.scale);
     else
       tgt = -1;
   }
@@ -363,13 +366,20 @@ __global__ void __launch_bounds__(1024)
   for (int o = 16; o; o >>= 1) v = merge(v, make_float2(__shfl_xor_sync(~0u, v.x, o), __shfl_xor_sync(~0u, v.y, o)));
   if (lane == 0) {
     const int64_t at = index ? index[r0 + w] : r0 + w;
-    float all = 0.0f;
+    float all = 0.0f, less = 0.0f;
     if (tgt >= 0) {
       const float z2 = z * kLog2e;
-      all = v.x <= z2 ? z + log1pf(v.y * exp2f(v.x - z2)) : (v.x + log2f(v.y + exp2f(z2 - v.x))) * kLn2;
+      if (v.x <= z2) {
+        less = log1pf(v.y * exp2f(v.x - z2));
+        all = z + less;
+        if (isinf(z)) less = all - z;  // no loss: NaN
+      } else {
+        all = (v.x + log2f(v.y + exp2f(z2 - v.x))) * kLn2;
+        less = ((v.x - z2) + log2f(v.y + exp2f(z2 - v.x))) * kLn2;
+      }
     }
     lse[at] = all;
-    loss[at] = tgt >= 0 ? all - z : 0.0f;
+    loss[at] = less;
   }
 }
 
