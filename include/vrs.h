@@ -350,12 +350,22 @@ VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, in
 
 /* Gradients of sum over rows of dloss[row] * loss[row], from the forward
  * pass's lse: dx (rows x d) and dtable (classes x d) in dtype, either NULL.
- * The scores are computed again, in pieces of the classes. */
+ * The scores are computed again, in pieces of the classes. The score gradient of
+ * a row's target, e^-loss - 1, is taken from lse - z[target] here, which is off by
+ * half of lse's last place: 5e-7 at lse 8 to 16, as much as the gradient itself
+ * where the loss is that small. ..._with_loss takes the forward pass's loss as
+ * well (NULL: as without it), has that gradient exact however small, and does not
+ * multiply the targets' scores out again. */
 VRS_API int vrs_linear_cross_entropy_backward(const float* dloss, const void* x, int64_t x_stride, int64_t rows,
                                               const void* table, int64_t table_stride, int64_t classes, int64_t d,
                                               int32_t dtype, const int64_t* targets, float scale, const float* lse,
                                               void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride,
                                               void* workspace, int64_t workspace_bytes, void* cuda_stream);
+VRS_API int vrs_linear_cross_entropy_backward_with_loss(
+    const float* dloss, const void* x, int64_t x_stride, int64_t rows, const void* table, int64_t table_stride,
+    int64_t classes, int64_t d, int32_t dtype, const int64_t* targets, float scale, const float* lse, const float* loss,
+    void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride, void* workspace, int64_t workspace_bytes,
+    void* cuda_stream);
 
 /* ------------------------------------------------------ streams, profiling */
 /* Makes a single-GPU or rank-mode handle issue its work on `cuda_stream`

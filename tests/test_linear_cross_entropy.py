@@ -517,3 +517,100 @@ def test_small_losses_keep_their_digits(gpu, rows, classes, d, noise, scale, off
     loss, lse = ops.linear_cross_entropy_forward(x, w, t, scale)
     off = (loss.double() - want).abs()
     assert (off <= (rel + 2.0 ** -22) * want + 2.0 ** -120).all(), f"worst {(off / want).max().item():.3g} of the loss"
+
+
+def _sure_gradients(x, w, t, dl, scale, dx, dw):
+    """dx and dtable of sure rows against 64 bits, relative to what they are made
+    of: score gradients in 16 bits (half an ulp; in f16 2^-38 of the largest
+    dloss at least, where their range ends) with r's relative error, against the
+    other operand, the sums' own error, and the result's half ulp."""
+    import torch
+    h = HALF[str(x.dtype).replace("torch.", "")]
+    f16 = x.dtype == torch.float16
+    X, W = x.double(), w.double()
+    _, g, rel = _sure64(x, w, t, scale)
+    up = dl.double()[:, None] * scale
+    g = g * up
+    ge = (1.01 * h + 2 * rel[:, None]) * g.abs() + (2.0 ** -38 * up.abs().max() if f16 else 0.0)
+    for got, want, e, what in ((dx, g @ W, ge @ W.abs() + (len(w) + 2) * 2.0 ** -22 * (g.abs() @ W.abs()), "dx"),
+                               (dw, g.t() @ X, ge.t() @ X.abs() + (len(t) + 2) * 2.0 ** -22 * (g.abs().t() @ X.abs()), "dtable")):
+        lim = e + 1.01 * h * want.abs() + (2.0 ** -25 if f16 else 0.0) + 2.0 ** -120
+        off = (got.double() - want).abs()
+        assert (off <= lim).all(), f"{what}: {int((off > lim).sum())} of {off.numel()} off, worst {(off / lim).max().item():.3g}x"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d,noise,scale,offset", SURE)
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_gradients_of_small_losses(gpu, rows, classes, d, noise, scale, offset, dtype):
+    """Through autograd. (f16 with a loss scale, as its training has.)"""
+    import torch
+    from vector_cuda import ops
+    x, w, t = _sure(rows, classes, d, dtype, noise, offset=offset)
+    dl = torch.full((rows,), 1024.0 if dtype == "float16" else 1.0, device="cuda")
+    leaves = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    (ops.linear_cross_entropy(*leaves, t, scale, "none") * dl).sum().backward()
+    _sure_gradients(x, w, t, dl, scale, leaves[0].grad, leaves[1].grad)
+
+
+@pytest.mark.gpu
+def test_backward_takes_the_loss(gpu):
+    """The pass by itself, given the loss, is autograd's; without it the target's
+    gradient comes from lse - z, off by no more than half of lse's last place
+    (2^-24 of it) and what sure rows lose otherwise."""
+    import torch
+    from vector_cuda import ops
+    x, w, t = _sure(200, 900, 65, "bfloat16", 0.5)
+    dl = torch.ones(200, device="cuda")
+    leaves = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    ops.linear_cross_entropy(*leaves, t, 20.0, "sum").backward()
+    loss, lse = ops.linear_cross_entropy_forward(x, w, t, 20.0)
+    dx, dw = ops.linear_cross_entropy_backward(dl, x, w, t, lse, 20.0, loss=loss)
+    assert torch.equal(dx, leaves[0].grad) and torch.equal(dw, leaves[1].grad)
+    dx, _ = ops.linear_cross_entropy_backward(dl, x, w, t, lse, 20.0, need_dtable=False)
+    h = HALF["bfloat16"]
+    _, g, rel = _sure64(x, w, t, 20.0)
+    ge = (1.01 * h + 2 * rel[:, None]) * g.abs()
+    ge.scatter_add_(1, t[:, None], 2.0 ** -24 * lse.double().abs()[:, None])
+    want = 20.0 * (g @ w.double())
+    lim = 20.0 * ((ge + 902 * 2.0 ** -22 * g.abs()) @ w.double().abs()) + 1.01 * h * want.abs()
+    assert ((dx.double() - want).abs() <= lim).all()
+
+
+@pytest.mark.gpu
+def test_losses_changed_in_place(gpu):
+    """reduction "none" hands the losses out; what becomes of them does not
+    reach the gradients."""
+    import torch
+    from vector_cuda import ops
+    x, w, t = _sure(50, 300, 64, "bfloat16", 0.5)
+    grads = []
+    for change in (False, True):
+        leaf = x.detach().requires_grad_(True)
+        loss = ops.linear_cross_entropy(leaf, w, t, 20.0, "none")
+        if change:
+            loss *= 1.0
+            loss += 3.0
+        loss.sum().backward()
+        grads.append(leaf.grad)
+    assert torch.equal(*grads)
+
+
+@pytest.mark.parametrize("change", [dict(dl=None), dict(lse=None), dict(loss=None, lse=None), dict(scale=0.0), dict(dws=63)])
+def test_backward_with_loss_refuses(vc, change):
+    a = dict(dl=4096, scale=1.0, lse=4096, loss=4096, dws=64)
+    a.update(change)
+    assert vc.lib().vrs_linear_cross_entropy_backward_with_loss(
+        a["dl"], 4096, 64, 4, 4096, 64, 10, 64, 2, 4096, a["scale"], a["lse"], a["loss"], 4096, 64, 4096, a["dws"], 4096,
+        1 << 40, None) == 5
+    assert b"vrs_linear_cross_entropy_backward" in vc.lib().vrs_last_error()
+
+
+@pytest.mark.gpu
+def test_python_refuses_another_loss(gpu):
+    import torch
+    from vector_cuda import ops
+    x, w, t, dl = _make(8, 20, 16, "bfloat16")
+    for loss in (dl[:7], dl.double(), dl.cpu(), 3.0):
+        with pytest.raises(ValueError):
+            ops.linear_cross_entropy_backward(dl, x, w, t, dl, loss=loss)

@@ -3,7 +3,8 @@
 //   z = scale x w_v, lse = log sum_v e^z, loss = lse - z[target]
 //   g = (e^(z - lse) - [v = target]) dloss scale, dx = g table, dtable = g^T x.
 // A row whose target lies outside the table takes no part: loss 0, lse 0, no
-// gradient, whatever its values are.
+// gradient, whatever its values are. For v = target the bracket is e^-loss - 1,
+// from the forward pass's loss: its difference to 1 would be lost in e^(z - lse).
 //
 // Forward it reads rows and table once (from memory; the products' tiles again
 // from L2) and does 2 rows classes d operations, backward three times that:
@@ -78,6 +79,7 @@ struct Pack1 {
   // backward
   const float* dloss;
   const float* lse;
+  const float* losses;  // null: the target's scores are multiplied out again
   float scale;
   bool f16;
   float* lse2;
@@ -264,6 +266,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
     if (BACK) {
       a.lse2[p] = a.lse[r] * kLog2e;
       a.gs[p] = a.dloss[r] / unit * gain;
+      if (a.losses) a.gy[p] = expm1f(-a.losses[r]);
     } else {
       a.index[p] = (int)r;
     }
@@ -291,11 +294,11 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
     } else {
       copy_row(x + row * a.xs, a.d, a.dp, to, row > 0 && row < a.rows - 1 && a.d >= 8);
     }
-    if (BACK) {
+    if (BACK && !a.losses) {
       const uint16_t *from = x + row * a.xs, *w = a.table + a.targets[row] * a.ts;
       const bool vec = (((uintptr_t)from | (uintptr_t)w) & 15) == 0;
-      const float z = a.f16 ? dot_rows<true>(from, w, a.d, vec) : dot_rows<false>(from, w, a.d, vec);
-      if (lane == 0) a.gy[before + i] = exp2f(z * a.scale * kLog2e - a.lse[row] * kLog2e) - 1.0f;
+      const float z = __fmul_rn(a.f16 ? dot_rows<true>(from, w, a.d, vec) : dot_rows<false>(from, w, a.d, vec), a.scale);
+      if (lane == 0) a.gy[before + i] = expm1f(z - a.lse[row]);
     }
   }
   // (Past the last row TMA reads zeros itself.)
@@ -704,8 +707,8 @@ int finish(bool f16, const float* acc, int splits, int64_t split_rows, const Pla
              : launch_finish<bf16>(acc, splits, split_rows, (int)d, (int)p.d4, rows, pos, head, out, os, s);
 }
 
-int backward(const Call& c, const Plan& p, const float* dloss, const float* lse, void* dx, int64_t dxs, void* dtable,
-             int64_t dts) {
+int backward(const Call& c, const Plan& p, const float* dloss, const float* lse, const float* losses, void* dx,
+             int64_t dxs, void* dtable, int64_t dts) {
   const bool f16 = c.dtype == VRS_F16;
   const CUtensorMapDataType type = f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
   Pack1 k{};
@@ -714,6 +717,7 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   k.pos = (int*)(c.ws + p.pos);
   k.dloss = dloss;
   k.lse = lse;
+  k.losses = losses;
   k.scale = c.scale;
   k.f16 = f16;
   k.lse2 = (float*)(c.ws + p.lse2);
@@ -812,11 +816,11 @@ extern "C" int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride,
   return st;
 }
 
-extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void* x, int64_t x_stride, int64_t rows,
-                                                 const void* table, int64_t table_stride, int64_t classes, int64_t d,
-                                                 int32_t dtype, const int64_t* targets, float scale, const float* lse,
-                                                 void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride,
-                                                 void* workspace, int64_t workspace_bytes, void* cuda_stream) {
+extern "C" int vrs_linear_cross_entropy_backward_with_loss(
+    const float* dloss, const void* x, int64_t x_stride, int64_t rows, const void* table, int64_t table_stride,
+    int64_t classes, int64_t d, int32_t dtype, const int64_t* targets, float scale, const float* lse, const float* loss,
+    void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride, void* workspace, int64_t workspace_bytes,
+    void* cuda_stream) {
   using namespace vrs;
   using namespace vrs::ops;
   const std::string who = "vrs_linear_cross_entropy_backward";
@@ -838,7 +842,17 @@ extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void*
   VRS_TRY(check_workspace(who, workspace, workspace_bytes, p.bytes));
   const Call c{x, x_stride, rows, table, table_stride, classes, d, dtype, targets, scale, (char*)workspace, s};
   ProfToken t = prof_begin("linear_cross_entropy_backward", s);
-  const int st = backward(c, p, dloss, lse, dx, dx_stride, dtable, dtable_stride);
+  const int st = backward(c, p, dloss, lse, loss, dx, dx_stride, dtable, dtable_stride);
   prof_end(t, s);
   return st;
+}
+
+extern "C" int vrs_linear_cross_entropy_backward(const float* dloss, const void* x, int64_t x_stride, int64_t rows,
+                                                 const void* table, int64_t table_stride, int64_t classes, int64_t d,
+                                                 int32_t dtype, const int64_t* targets, float scale, const float* lse,
+                                                 void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride,
+                                                 void* workspace, int64_t workspace_bytes, void* cuda_stream) {
+  return vrs_linear_cross_entropy_backward_with_loss(dloss, x, x_stride, rows, table, table_stride, classes, d, dtype,
+                                                     targets, scale, lse, nullptr, dx, dx_stride, dtable, dtable_stride,
+                                                     workspace, workspace_bytes, cuda_stream);
 }

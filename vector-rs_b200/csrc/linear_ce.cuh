@@ -59,7 +59,7 @@ struct CeGemm {
   const int64_t* targets;  // [rows] where the rows are not packed, else null
   const int* target;       // [rows] of the taking rows
   const float* lse2;   // [rows] lse * log2(e)
-  const float* gy;     // [row] the target's probability - 1
+  const float* gy;     // [rows] the target's probability - 1
   const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
   int64_t part_rows;
@@ -83,7 +83,8 @@ struct CeGemm {
 // of the last place, all downwards. A loss that is small against the target's
 // score, and a probability near 1, would show them (2e-3 of the loss at
 // d = 1,700), so the target's score is computed apart; another class's error is
-// one of many. vec: both rows start on 16 bytes.
+// one of many. vec: both rows start on 16 bytes; the order of the sums is the same
+// either way, so that both passes get one score from packed and unpacked rows.
 template <bool F16>
 __device__ __forceinline__ float dot_rows(const uint16_t* x, const uint16_t* w, int d, bool vec) {
   auto value = [](uint16_t u) {
@@ -91,13 +92,22 @@ __device__ __forceinline__ float dot_rows(const uint16_t* x, const uint16_t* w, 
   };
   const int lane = threadIdx.x & 31;
   float s[2] = {0.0f, 0.0f};
-  int e = vec ? d / 8 * 8 : 0;  // first element read one by one
+  int e = d / 8 * 8;  // first element of the tail
   for (int c = lane * 8; c < e; c += 256) {
-    const Pack<uint16_t, 8> p = load_pack<uint16_t, 8>(x + c), q = load_pack<uint16_t, 8>(w + c);
+    Pack<uint16_t, 8> p, q;
+    if (vec) {
+      p = load_pack<uint16_t, 8>(x + c);
+      q = load_pack<uint16_t, 8>(w + c);
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; j++) {
+        p.v[j] = x[c + j];
+        q.v[j] = w[c + j];
+      }
+    }
 #pragma unroll
     for (int j = 0; j < 8; j++) s[j & 1] = fmaf(value(p.v[j]), value(q.v[j]), s[j & 1]);
   }
-#pragma unroll 4
   for (e += lane; e < d; e += 32) s[0] = fmaf(value(x[e]), value(w[e]), s[0]);
   float t = s[0] + s[1];
 #pragma unroll

@@ -26,7 +26,7 @@ struct Bound {
   decltype(&vrs_layer_norm_backward) norm_backward;
   decltype(&vrs_layer_norm_backward_workspace) norm_workspace;
   decltype(&vrs_linear_cross_entropy_forward) loss_forward;
-  decltype(&vrs_linear_cross_entropy_backward) loss_backward;
+  decltype(&vrs_linear_cross_entropy_backward_with_loss) loss_backward;
   decltype(&vrs_linear_cross_entropy_workspace) loss_workspace;
   PyObject* check;  // raises CudaError for a status
 } g{};
@@ -278,12 +278,14 @@ PyObject* linear_cross_entropy_forward(PyObject* const* args) {
   return to_tuple({loss, lse});
 }
 
-// (dloss, x, table, targets, lse, scale, need dx, need dtable) -> (dx, dtable)
+// (dloss, x, table, targets, lse, scale, need dx, need dtable, loss or None) -> (dx, dtable)
 PyObject* linear_cross_entropy_backward(PyObject* const* args) {
   const LossArgs a = loss_args(args[1], args[2], args[3], args[5]);
   const at::Tensor &x = THPVariable_Unpack(args[1]), &table = THPVariable_Unpack(args[2]);
   const at::Tensor dloss = beside(tensor_arg(args[0], "dloss"), a.x.t, "dloss", a.x.n, at::kFloat);
   const at::Tensor lse = beside(tensor_arg(args[4], "lse"), a.x.t, "lse", a.x.n, at::kFloat);
+  auto loss = optional_arg(args[8], "loss");
+  if (loss) loss = beside(*loss, a.x.t, "loss", a.x.n, at::kFloat);
   std::optional<at::Tensor> dx, dtable;
   if (bool_arg(args[6])) dx = at::empty(x.sizes(), a.x.t.options());
   if (bool_arg(args[7])) dtable = at::empty(table.sizes(), a.table.t.options());
@@ -294,8 +296,8 @@ PyObject* linear_cross_entropy_backward(PyObject* const* args) {
   check_status(unlocked([&] {
     return g.loss_backward((const float*)dloss.data_ptr(), a.x.t.data_ptr(), a.x.stride, a.x.n, a.table.t.data_ptr(),
                            a.table.stride, a.table.n, a.x.d, code_of(a.x.t.scalar_type()),
-                           (const int64_t*)a.targets.data_ptr(), a.scale, (const float*)lse.data_ptr(), ptr(dx), a.x.d,
-                           ptr(dtable), a.x.d, ws.data_ptr(), need, stream);
+                           (const int64_t*)a.targets.data_ptr(), a.scale, (const float*)lse.data_ptr(),
+                           (const float*)ptr(loss), ptr(dx), a.x.d, ptr(dtable), a.x.d, ws.data_ptr(), need, stream);
   }));
   return to_tuple({dx, dtable});
 }
@@ -357,7 +359,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, 
                          VRS_METHOD(layer_norm_forward, 4),
                          VRS_METHOD(layer_norm_backward, 7),
                          VRS_METHOD(linear_cross_entropy_forward, 4),
-                         VRS_METHOD(linear_cross_entropy_backward, 8),
+                         VRS_METHOD(linear_cross_entropy_backward, 9),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -189,6 +189,8 @@ def lib() -> ctypes.CDLL:
                                                        i64, vp]
         L.vrs_linear_cross_entropy_backward.argtypes = [vp, vp, i64, i64, vp, i64, i64, i64, i32, vp, f32, vp, vp,
                                                         i64, vp, i64, vp, i64, vp]
+        L.vrs_linear_cross_entropy_backward_with_loss.argtypes = [vp, vp, i64, i64, vp, i64, i64, i64, i32, vp, f32,
+                                                                  vp, vp, vp, i64, vp, i64, vp, i64, vp]
         _lib_handle = L
     return _lib_handle
 

@@ -30,7 +30,8 @@ except ImportError as e:
 def _bind():
     L = lib()
     names = ("layer_norm_forward", "layer_norm_backward", "layer_norm_backward_workspace",
-             "linear_cross_entropy_forward", "linear_cross_entropy_backward", "linear_cross_entropy_workspace")
+             "linear_cross_entropy_forward", "linear_cross_entropy_backward_with_loss",
+             "linear_cross_entropy_workspace")
     _ops.bind(*(ctypes.cast(getattr(L, "vrs_" + n), ctypes.c_void_p).value for n in names), _check)
 
 
@@ -94,27 +95,30 @@ def linear_cross_entropy_forward(x: torch.Tensor, table: torch.Tensor, targets: 
 
 def linear_cross_entropy_backward(dloss: torch.Tensor, x: torch.Tensor, table: torch.Tensor, targets: torch.Tensor,
                                   lse: torch.Tensor, scale: float = 1.0, need_dx: bool = True,
-                                  need_dtable: bool = True):
+                                  need_dtable: bool = True, loss: Optional[torch.Tensor] = None):
     """(dx, dtable): gradients of sum(dloss * loss), in x's and table's type;
-    None for one that is not needed. lse is the forward pass's."""
-    return _ops.linear_cross_entropy_backward(dloss, x, table, targets, lse, scale, need_dx, need_dtable)
+    None for one that is not needed. lse is the forward pass's, and so is loss:
+    with it the gradient of the target's score is exact for rows whose loss is
+    small; without it, it is off by up to half of lse's last place."""
+    return _ops.linear_cross_entropy_backward(dloss, x, table, targets, lse, scale, need_dx, need_dtable, loss)
 
 
 class _LinearCrossEntropy(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, table, targets, scale):
+    def forward(ctx, x, table, targets, scale, handed_out):
         loss, lse = linear_cross_entropy_forward(x, table, targets, scale)
-        ctx.save_for_backward(x, table, targets, lse)
+        # Losses that the caller gets may change in place.
+        ctx.save_for_backward(x, table, targets, lse, loss.clone() if handed_out else loss)
         ctx.scale = scale
         return loss
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dloss):
-        x, table, targets, lse = ctx.saved_tensors
+        x, table, targets, lse, loss = ctx.saved_tensors
         dx, dtable = linear_cross_entropy_backward(dloss, x, table, targets, lse, ctx.scale,
-                                                   ctx.needs_input_grad[0], ctx.needs_input_grad[1])
-        return dx, dtable, None, None
+                                                   ctx.needs_input_grad[0], ctx.needs_input_grad[1], loss)
+        return dx, dtable, None, None, None
 
 
 def linear_cross_entropy(x: torch.Tensor, table: torch.Tensor, targets: torch.Tensor, scale: float = 1.0,
@@ -125,7 +129,7 @@ def linear_cross_entropy(x: torch.Tensor, table: torch.Tensor, targets: torch.Te
     that take part (0 where there are none), "sum" or "none"."""
     if reduction not in ("mean", "sum", "none"):
         raise ValueError(f"unknown reduction {reduction!r}")
-    loss = _LinearCrossEntropy.apply(x, table, targets, scale)
+    loss = _LinearCrossEntropy.apply(x, table, targets, scale, reduction == "none")
     if reduction == "none":
         return loss
     total = loss.sum()
