@@ -614,3 +614,25 @@ def test_python_refuses_another_loss(gpu):
     for loss in (dl[:7], dl.double(), dl.cpu(), 3.0):
         with pytest.raises(ValueError):
             ops.linear_cross_entropy_backward(dl, x, w, t, dl, loss=loss)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows", [60, 700, 9000])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("bad", [float("inf"), -float("inf"), float("nan")])
+def test_one_row_of_no_finite_weight(gpu, rows, dtype, bad):
+    """An infinite or NaN dloss stays in its row of dx: the other rows are
+    rounded and scaled as if that row had weight 0."""
+    import torch
+    from vector_cuda import ops
+    x, w, t, dl = _make(rows, 500, 64, dtype, ignored=0.1)
+    dl *= 1024.0
+    at = int((t >= 0).nonzero()[3])
+    _, lse = ops.linear_cross_entropy_forward(x, w, t)
+    dl[at] = 0.0
+    want, _ = ops.linear_cross_entropy_backward(dl, x, w, t, lse, need_dtable=False)
+    dl[at] = bad
+    got, _ = ops.linear_cross_entropy_backward(dl, x, w, t, lse, need_dtable=False)
+    assert not torch.isfinite(got[at]).any()
+    got[at] = want[at]
+    assert torch.isfinite(got).all() and torch.equal(got, want)

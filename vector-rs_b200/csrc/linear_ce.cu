@@ -67,7 +67,7 @@ struct Pack1 {
   const uint16_t* table;  // as given
   int64_t ts;
   uint16_t* table_out;
-  const int2* slabs;  // per slab: taking rows, bits of the largest |dloss|; null: read all targets
+  const int2* slabs;  // per slab: taking rows, bits of the largest finite |dloss|; null: read all targets
   CeHeader* head;
   void* xc;        // [taking rows, tail zeros to a whole tile][dp]
   int* index;      // compact row -> row (forward)
@@ -90,6 +90,13 @@ struct Pack1 {
 __device__ __forceinline__ bool takes_part(const Pack1& a, int64_t r) {
   const int64_t t = a.targets[r];
   return t >= 0 && t < a.classes;
+}
+
+// What a row's weight adds to the largest |dloss|: one that is not finite spoils
+// its own row and must not scale the others'.
+__device__ __forceinline__ unsigned weight_bits(float dloss) {
+  const unsigned u = __float_as_uint(fabsf(dloss));
+  return u < 0x7f800000u ? u : 0u;
 }
 
 // Sum, sum and maximum over a block of 256.
@@ -124,18 +131,18 @@ __global__ void __launch_bounds__(256) ce_count_kernel(const Pack1 a, int2* slab
   for (int64_t r = r0 + threadIdx.x; r < min(a.rows, r0 + kSlab); r += 256)
     if (takes_part(a, r)) {
       n++;
-      if (a.dloss) m = max(m, __float_as_uint(fabsf(a.dloss[r])));
+      if (a.dloss) m = max(m, weight_bits(a.dloss[r]));
     }
   block_reduce(n, none, m, s);
   if (threadIdx.x == 0) slabs[blockIdx.x] = make_int2(n, (int)m);
 }
 
 // The score gradients are rounded to 16 bits relative to the largest
-// |dloss|: with one weight for all rows (a mean) the target's -1 stays exact
-// and no weight's own rounding biases the sums. 0 and non-finite: by 1.
+// finite |dloss|: with one weight for all rows (a mean) the target's -1 stays
+// exact and no weight's own rounding biases the sums. Where it is 0: to 1.
 __device__ __forceinline__ float grad_unit(unsigned max_bits) {
   const float m = __uint_as_float(max_bits);
-  return m > 0.0f && m < INFINITY ? m : 1.0f;
+  return m > 0.0f ? m : 1.0f;
 }
 // f16 ends at 2^16 and loses bits below 2^-14: its gradients use the range up to 2^13.
 constexpr float kF16Gain = 8192.0f;
@@ -232,7 +239,7 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
 #pragma unroll 16
     for (int64_t r = tid; r < a.rows; r += 256) {
       const int64_t t = a.targets[r];
-      const unsigned g = BACK ? __float_as_uint(fabsf(a.dloss[r])) : 0;
+      const unsigned g = BACK ? weight_bits(a.dloss[r]) : 0;
       if (t >= 0 && t < a.classes) {
         total++;
         before += r < r0;

@@ -60,7 +60,7 @@ struct CeGemm {
   const int* target;       // [rows] of the taking rows
   const float* lse2;   // [rows] lse * log2(e)
   const float* gy;     // [rows] the target's probability - 1
-  const float* gs;     // [rows] dloss over the largest |dloss| (f16: times a gain)
+  const float* gs;     // [rows] dloss over the largest finite |dloss| (f16: times a gain)
   float c2;            // scale * log2(e)
   int64_t part_rows;
   float2* part;        // [part][part_rows]: maximum of c2 z and sum of 2^(c2 z - maximum)
