@@ -636,3 +636,64 @@ def test_one_row_of_no_finite_weight(gpu, rows, dtype, bad):
     assert not torch.isfinite(got[at]).any()
     got[at] = want[at]
     assert torch.isfinite(got).all() and torch.equal(got, want)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d", [(8, 1398, 75), (1, 1000, 64), (1, 30011, 768), (3, 20000, 500), (64, 5000, 130), (64, 5000, 60),
+                                            (1, 300000, 64), (3, 100000, 72), (40, 9000, 264)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_table_gradients_of_few_rows(gpu, rows, classes, d, dtype):
+    """A row of dtable is a sum over rows: with few of them the 16-bit rounding of
+    the score gradients has little to average with, so it must not be there: only
+    the square of half an ulp (what two 16-bit parts leave), the scores' errors,
+    and the result's own half ulp."""
+    _few_terms(rows, classes, d, dtype, False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("rows,classes,d", [(8, 1398, 75), (1000, 2, 64), (5000, 3, 600), (300, 64, 1000), (20000, 17, 130)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_row_gradients_of_few_classes(gpu, rows, classes, d, dtype):
+    """And a row of dx is a sum over classes."""
+    _few_terms(rows, classes, d, dtype, True)
+
+
+def _few_terms(rows, classes, d, dtype, dx):
+    import torch
+    from vector_cuda import ops
+    x, w, t, dl = _make(rows, classes, d, dtype)
+    loss, lse = ops.linear_cross_entropy_forward(x, w, t)
+    leaves = x.detach().requires_grad_(dx), w.detach().requires_grad_(not dx)
+    (ops.linear_cross_entropy(*leaves, t, 1.0, "none") * dl).sum().backward()
+    got = leaves[0].grad if dx else leaves[1].grad
+    h, f16 = HALF[dtype], dtype == "float16"
+    X, W = x.double(), w.double()
+    _, g, rel = _sure64(x, w, t, 1.0)
+    up = dl.double()[:, None]
+    g = g * up
+    ge = (1.01 * h * h + 2 * rel[:, None]) * g.abs() + (2.0 ** -38 * up.max() if f16 else 0.0)
+    e = (ge + (len(w if dx else t) + 2) * 2.0 ** -22 * g.abs())
+    want, e = (g @ W, e @ W.abs()) if dx else (g.t() @ X, e.t() @ X.abs())
+    lim = e + 1.01 * h * want.abs() + (2.0 ** -25 if f16 else 0.0)
+    off = (got.double() - want).abs()
+    assert (off <= lim).all(), f"{int((off > lim).sum())} of {off.numel()} off, worst {(off / lim).max().item():.3g}x"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("which,rows,classes,d", [("dtable", 60, 2000, 300), ("dtable", 64, 5000, 130), ("dtable", 60, 700, 100),
+                                                  ("dx", 2000, 40, 300), ("dx", 200, 500, 100), ("dx", 3000, 64, 100)])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_few_terms_in_the_mean(gpu, which, rows, classes, d, dtype):
+    """The error's norm over the result's. Rounding values of a normal distribution
+    to the nearest gives 0.43 half ulps; score gradients rounded likewise would
+    add as much again, 0.6 in all. Half is between."""
+    import torch
+    from vector_cuda import ops
+    x, w, t, dl = _make(rows, classes, d, dtype)
+    dl *= 1024.0
+    leaves = x.detach().requires_grad_(which == "dx"), w.detach().requires_grad_(which == "dtable")
+    (ops.linear_cross_entropy(*leaves, t, 1.0, "none") * dl).sum().backward()
+    _, g, _ = _sure64(x, w, t, 1.0)
+    g = g * dl.double()[:, None]
+    got, want = (leaves[0].grad, g @ w.double()) if which == "dx" else (leaves[1].grad, g.t() @ x.double())
+    assert (got.double() - want).norm() <= 0.5 * HALF[dtype] * want.norm()

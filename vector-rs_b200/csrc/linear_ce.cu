@@ -37,14 +37,21 @@ constexpr int64_t kPieceBytes = 256ll << 20;
 // CTA pairs that a product is split for (148 SMs). A constant, so that sums
 // are split alike on every device.
 constexpr int kPairs = 74;
-// Products of up to this many multiply-adds take the score gradients as two
-// 16-bit values each, the rounded one and the rest, and then add nothing to the
-// results' own rounding: there a result is a sum of so few terms of weight that
-// one term's rounding can show (8 x 1,398 x 75 in f16 against 64 bits: up to
-// 3.2e-4 with one, 2.0e-4 with two, as rounding the exact result leaves). Larger
-// ones average it (at most sqrt 2 of the results' own) and would pay more:
-// backward 8 x 1,398 x 75 23.5 us with one, 28.0 with two; 128 x 8,192 x 256
-// 25.9 and 32.0; 1,024 x 8,192 x 256 40 and 57.
+// A product takes the score gradients as two 16-bit values each, the rounded one
+// and the rest, and then adds nothing to the result's own rounding, where that
+// rounding would show: in sums of up to kFewTerms terms (dtable: rows, dx:
+// classes), and in problems of up to kTwoPlanes multiply-adds. One rounding of a
+// lone term's gradient is common to a whole row of the result and at worst as
+// large as the result's own half ulp; over n terms of one sign the roundings
+// average to 1 / sqrt n of it, over terms of random signs they stay (in the
+// root mean square) as large as the result's own, but differ between its elements.
+// Few terms are one K block, so the second plane costs its writing and one K
+// block more: backward 64 x 100,000 x 256 88 us with one, 95 with two; 20,000 x 17 x
+// 130 64 and 69. Small problems show it in dx and dtable (8 x 1,398 x 75 in f16
+// against 64 bits: up to 3.2e-4 with one, 2.0e-4 with two, as rounding the exact
+// result leaves), larger ones would pay more: 128 x 8,192 x 256 25.9 and 32.0 us,
+// 1,024 x 8,192 x 256 40 and 57.
+constexpr int kFewTerms = kCeK;
 constexpr int64_t kTwoPlanes = 1ll << 24;
 // Up to here each pack block reads all targets itself; above, a first kernel
 // counts them per kSlab rows.
@@ -454,15 +461,15 @@ struct Plan {
   int64_t vtiles;                 // class tiles in all
   int64_t parts;                  // and parts of 128 classes
   int splits_dx, splits_dw;
-  int planes;                     // of the score gradients
+  int planes, planes_dx, planes_dw;  // of the score gradients: written, and taken by each product
   int64_t head, slabs, index, pos, target, lse2, gs, gy, xc, wc, part, g, acc_dx, acc_dw, bytes;
 };
 
 // Class tiles of a piece: few pieces of one size, as many (up to twice the
 // fewest) as make the pairs' last turns fullest. A turn's length is that of its
 // longest tile; the products' tiles are counted as the kernel orders them.
-int64_t piece_of(int64_t rows_p, int64_t vtiles, int64_t ntiles) {
-  int64_t most = kPieceBytes / (rows_p * 2) / kCeN;
+int64_t piece_of(int64_t rows_p, int planes, int64_t vtiles, int64_t ntiles) {
+  int64_t most = kPieceBytes / (planes * rows_p * 2) / kCeN;
   most = most < 1 ? 1 : most < vtiles ? most : vtiles;
   const int64_t fewest = (vtiles + most - 1) / most, mt = rows_p / kCeM;
   int64_t best = most;
@@ -511,8 +518,11 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
     p.lse2 = take(rows * 4);
     p.gs = take(rows * 4);
     p.gy = take(rows * 4);
-    p.piece = piece_of(p.rows_p, p.vtiles, (d + kCeN - 1) / kCeN) * kCeN;
-    p.planes = rows * classes <= kTwoPlanes / d ? 2 : 1;
+    const bool small = rows * classes <= kTwoPlanes / d;
+    p.planes_dx = small || classes <= kFewTerms ? 2 : 1;
+    p.planes_dw = small || rows <= kFewTerms ? 2 : 1;
+    p.planes = p.planes_dx > p.planes_dw ? p.planes_dx : p.planes_dw;
+    p.piece = piece_of(p.rows_p, p.planes, p.vtiles, (d + kCeN - 1) / kCeN) * kCeN;
     p.g = take(p.planes * p.rows_p * p.piece * 2);
     // Few tiles: K is split until the pairs have one each, 8 blocks deep at least.
     auto splits = [](int64_t tiles_, int64_t kblocks) {
@@ -520,8 +530,8 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
       return (int)(s < 1 ? 1 : s);
     };
     const int64_t nt = (d + kCeN - 1) / kCeN;
-    p.splits_dx = splits(p.rows_p / kCeM * nt, p.planes * (p.piece / kCeK));
-    p.splits_dw = splits(p.piece / kCeM * nt, p.planes * ((rows + kCeK - 1) / kCeK));
+    p.splits_dx = splits(p.rows_p / kCeM * nt, p.planes_dx * (p.piece / kCeK));
+    p.splits_dw = splits(p.piece / kCeM * nt, p.planes_dw * ((rows + kCeK - 1) / kCeK));
     p.acc_dx = take(p.splits_dx * p.rows_p * p.d4 * 4);
     p.acc_dw = take(p.splits_dw > 1 ? p.splits_dw * p.piece * p.d4 * 4 : 0);
   }
@@ -751,6 +761,8 @@ int backward(const Call& c, const Plan& p, const float* dloss, const float* lse,
   a.dx.ntiles = a.dw.ntiles = (int)((c.d + kCeN - 1) / kCeN);
   a.dx.splits = p.splits_dx;
   a.dw.splits = p.splits_dw;
+  a.dx.planes = p.planes_dx;
+  a.dw.planes = p.planes_dw;
   a.d4 = (int)p.d4;
   a.dx.f32 = acc_dx;
   a.dx.f32_rows = (int)p.rows_p;

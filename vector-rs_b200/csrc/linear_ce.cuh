@@ -33,6 +33,7 @@ struct CeJob {
   int ntiles;      // over d
   int kblocks;     // dx; dtable takes its count from the header
   int splits;
+  int planes;      // of the score gradients that it takes
   float* f32;      // [split][f32_rows][d4], or null: 16-bit result, one split
   int f32_rows;
   int add;         // f32: add to what earlier pieces left
@@ -71,7 +72,7 @@ struct CeGemm {
   int64_t ws;
   // products
   CeJob dx, dw;
-  int planes;          // of the score gradients: 1, or 2 (rounded value, and what rounding left)
+  int planes;          // of the score gradients written: 1, or 2 (rounded value, and what rounding left)
   int plane_rows;      // rows of a plane
   uint16_t* g;
   int64_t g_pitch;

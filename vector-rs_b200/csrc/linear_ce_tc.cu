@@ -213,8 +213,8 @@ __device__ __forceinline__ Tiles count_tiles(const CeGemm& a) {
   if (MODE == kCeStore) {
     const int n_dx = a.dx.on ? t.mtiles * a.dx.ntiles * a.dx.splits : 0;
     const int n_dw = a.dw.on ? a.dw.mtiles * a.dw.ntiles * a.dw.splits : 0;
-    const int k_dx = (a.planes * a.dx.kblocks + a.dx.splits - 1) / a.dx.splits + kTileCost;
-    const int k_dw = (a.planes * t.kblocks_rows + a.dw.splits - 1) / a.dw.splits + kTileCost;
+    const int k_dx = (a.dx.planes * a.dx.kblocks + a.dx.splits - 1) / a.dx.splits + kTileCost;
+    const int k_dw = (a.dw.planes * t.kblocks_rows + a.dw.splits - 1) / a.dw.splits + kTileCost;
     t.long_job = k_dw > k_dx;
     t.n_long = t.long_job ? n_dw : n_dx;
     t.n_short = t.long_job ? n_dx : n_dw;
@@ -256,6 +256,7 @@ __device__ __forceinline__ CeJob job_of(const CeGemm& a, bool dw) {
   j.ntiles = dw ? a.dw.ntiles : a.dx.ntiles;
   j.kblocks = dw ? a.dw.kblocks : a.dx.kblocks;
   j.splits = dw ? a.dw.splits : a.dx.splits;
+  j.planes = dw ? a.dw.planes : a.dx.planes;
   j.f32 = dw ? a.dw.f32 : a.dx.f32;
   j.f32_rows = dw ? a.dw.f32_rows : a.dx.f32_rows;
   j.add = dw ? a.dw.add : a.dx.add;
@@ -291,7 +292,7 @@ __device__ __forceinline__ Tile tile_at(const CeGemm& a, const Tiles& c, int id)
   t.split = id % j.splits;
   t.m = id / j.splits;
   t.bn = a.d - t.n > 128 ? 256 : 128;
-  const int kb = a.planes * (t.job ? c.kblocks_rows : j.kblocks);
+  const int kb = j.planes * (t.job ? c.kblocks_rows : j.kblocks);
   const int per = (kb + j.splits - 1) / j.splits;
   t.kb0 = min(kb, t.split * per);
   t.kb1 = min(kb, t.kb0 + per);
@@ -659,7 +660,9 @@ __global__ void __launch_bounds__(threads(MODE), 1)
       // Columns of the warp that exist: the last class or a dx or dtable row may
       // end within the tile.
       const int cols = min(t.bn - half * HCOLS, (MODE == kCeStore ? a.d : MODE == kCeGrad ? a.vn : a.classes) - n0);
-      const bool mine = half * HCOLS < t.bn && (MODE == kCeLse ? r0 < taken && cols > 0 : MODE == kCeStore ? cols > 0 : true);
+      // Rows that exist; of the score gradients, those in dtable's last K block too.
+      const bool rows = MODE == kCeLse ? r0 < taken : MODE == kCeGrad ? r0 < (taken + kCeK - 1) / kCeK * kCeK : true;
+      const bool mine = half * HCOLS < t.bn && rows && (MODE == kCeGrad || cols > 0);
       const CeJob job = job_of(a, t.job);
       const bool none = MODE == kCeStore && t.kb0 == t.kb1;  // a split without K blocks: zeros
       const float f = MODE == kCeStore ? a.head->grad_scale : 1.0f;
@@ -701,7 +704,9 @@ __global__ void __launch_bounds__(threads(MODE), 1)
           }
         } else if (MODE == kCeGrad) {
           // g = (2^(c2 z - lse2) - [target]) gs in 16 bits; zeros past the last
-          // class and in the tail rows, which the products read.
+          // class and in the rest of the last K block of rows. (dx's product reads
+          // the whole tile of rows; what those further down hold reaches rows of its
+          // result that nobody reads.)
 #pragma unroll
           for (int j = 0; j < CHUNK; j++) w[j] = ex2(fmaf(w[j], a.c2, -lse2));
           const int at = tgt - a.v0 - n0 - c * CHUNK;
@@ -765,7 +770,7 @@ __global__ void __launch_bounds__(threads(MODE), 1)
             stage_row16<F16>(stg, lane, h, w);
             if (h == 0) continue;
             __syncwarp();
-            const int64_t first = job.row0 + (int64_t)r0, rows = a.classes - first;
+            const int64_t first = job.row0 + (int64_t)r0, past = a.classes - first;
             uint16_t* o = job.out + first * job.out_stride + n0 + c0 * CHUNK;
             const int here = left + CHUNK;  // of the staging tile's 64 columns
             if (job.out_vec) {
@@ -774,14 +779,14 @@ __global__ void __launch_bounds__(threads(MODE), 1)
               for (int q = 0; q < 8; q++) {
                 const int r = q * 4 + (lane >> 3);
                 const uint4 k = stage_get(stg, r, lane & 7);
-                if (r < rows && col < here) *reinterpret_cast<uint4*>(o + r * job.out_stride + col) = k;
+                if (r < past && col < here) *reinterpret_cast<uint4*>(o + r * job.out_stride + col) = k;
               }
             } else {
               // Rows that 16-byte stores cannot address: a word a lane, the rows
               // that start on a word and the others apart. Few warps store, so
               // the instructions and latencies of a row count (10 x 150,379 x
               // 798, 120 M elements of dtable: 198 us; element by element 346).
-              const int all = (int)min((int64_t)32, rows);
+              const int all = (int)min((int64_t)32, past);
               const int odd = (int)(reinterpret_cast<uintptr_t>(o) >> 1 & 1);
               if ((job.out_stride & 1) == 0) {
                 if (odd)
