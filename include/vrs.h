@@ -297,8 +297,9 @@ VRS_API int vrs_selftest_bounded_wait(int64_t limit_ns);
  * products that a dot-product search ranks). All buffers are device pointers
  * on the current device; work is queued on cuda_stream (NULL = default
  * stream) and the call returns without waiting; no device memory is allocated:
- * scratch is the caller's workspace, whose size the *_workspace calls give, and
- * may be reused as soon as the stream has passed the call. Strides are in
+ * scratch is the caller's workspace, whose size the *_workspace calls give (it
+ * never falls as a size grows: one for the largest rows, classes and d serves
+ * every smaller call of that pass), and may be reused as soon as the stream has passed the call. Strides are in
  * elements, between consecutive rows; elements of a row are contiguous.
  * Outputs and workspace overlap neither one another nor the inputs.
  * Results do not depend on timing: on one device the same inputs give the same

@@ -357,3 +357,23 @@ def test_many_rows(gpu, rows, d, dtype, ptype):
     import torch
     x, w, b, dy = _make(rows, d, getattr(torch, dtype), getattr(torch, ptype))
     _check(x, w, b, dy)
+
+
+@pytest.mark.gpu
+def test_workspace_grows_with_every_size(gpu, vc):
+    """A workspace for the largest sizes serves every smaller call."""
+    n = ctypes.c_int64(0)
+
+    def size(rows, d):
+        assert vc.lib().vrs_layer_norm_backward_workspace(rows, d, ctypes.byref(n)) == 0
+        return n.value
+
+    widths = sorted({w for k in range(16) for w in (2 ** k - 1, 2 ** k, 2 ** k + 1) if 1 <= w <= 32768} |
+                    {4096 * k + o for k in range(1, 8) for o in (-1, 0, 1)} | {771, 6000, 20011, 32767, 32768})
+    counts = [1, 2, 3, 17, 18, 19, 20, 36, 37, 38, 64, 65, 73, 74, 75, 98, 99, 148, 149, 200, 295, 296, 297, 1000, 10 ** 6]
+    for rows in counts:
+        for narrow, wide in zip(widths, widths[1:]):
+            assert size(rows, narrow) <= size(rows, wide), (rows, narrow, wide)
+    for d in widths:
+        for few, many in zip(counts, counts[1:]):
+            assert size(few, d) <= size(many, d), (few, many, d)

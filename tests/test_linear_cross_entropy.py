@@ -697,3 +697,29 @@ def test_few_terms_in_the_mean(gpu, which, rows, classes, d, dtype):
     g = g * dl.double()[:, None]
     got, want = (leaves[0].grad, g @ w.double()) if which == "dx" else (leaves[1].grad, g.t() @ x.double())
     assert (got.double() - want).norm() <= 0.5 * HALF[dtype] * want.norm()
+
+
+@pytest.mark.parametrize("backward", [0, 1])
+@pytest.mark.parametrize("aligned", [0, 1])
+def test_workspace_grows_with_every_size(vc, backward, aligned):
+    """A workspace for the largest sizes serves every smaller call: the answer
+    never falls as a size grows."""
+    import math
+    import random
+    n = ctypes.c_int64(0)
+
+    def size(rows, classes, d):
+        assert vc.lib().vrs_linear_cross_entropy_workspace(rows, classes, d, 2, backward, aligned, ctypes.byref(n)) == 0
+        return n.value
+
+    rng = random.Random(3)
+    pairs = [((2048, 48000, 1024), (4096, 48000, 1024)), ((1, 1000000, 16), (1, 1000000, 17)),
+             ((64, 70000, 64), (65, 70000, 64)), ((256, 70000, 64), (257, 70000, 64)), ((300, 64, 500), (300, 65, 500))]
+    for _ in range(4000):
+        most = (2 ** 20, 2 ** 21, 2 ** 14)
+        a = [round(2 ** rng.uniform(0, math.log2(m))) for m in most]
+        b = [max(v, min(m, round(v * 2 ** rng.choice([0, 0, rng.uniform(0, 0.2), rng.uniform(0, 6)])) + rng.choice([0, 0, 1])))
+             for v, m in zip(a, most)]
+        pairs.append((tuple(a), tuple(b)))
+    for a, b in pairs:
+        assert size(*a) <= size(*b), f"{a} needs {size(*a)}, {b} {size(*b)}"

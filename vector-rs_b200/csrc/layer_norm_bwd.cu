@@ -273,13 +273,26 @@ extern "C" int vrs_layer_norm_backward_workspace(int64_t rows, int64_t d, int64_
   int sms = 0;
   VRS_TRY(sm_count(&sms));
   // How the rows can be reached decides the cluster of few rows and whether
-  // the count of blocks is even.
-  int blocks = 0;
-  for (LnAccess access : {kLnElements, kLn16Bytes, kLnPairs}) {
-    const LnPlan p = bwd_plan(rows, (int)d, 8, access, sms);
-    blocks = blocks > p.blocks ? blocks : p.blocks;
+  // the count of blocks is even. Rows in wider clusters have fewer of them, and so
+  // may more rows than SMs: the answer is the largest of all widths up to d and of
+  // both counts of rows, so that a workspace for the largest sizes serves all
+  // smaller ones.
+  auto bytes = [&](int64_t width) {
+    int blocks = 0;
+    for (int64_t n : {rows, rows < sms ? rows : (int64_t)sms})
+      for (LnAccess access : {kLnElements, kLn16Bytes, kLnPairs}) {
+        const LnPlan p = bwd_plan(n, (int)width, 8, access, sms);
+        blocks = blocks > p.blocks ? blocks : p.blocks;
+      }
+    return (int64_t)((blocks + 1) / 2 * 2) * 2 * width * (int64_t)sizeof(float);
+  };
+  constexpr int64_t kOne = kLnThreads * kNarrowE;  // elements that a block of a cluster holds
+  int64_t most = bytes(d);
+  for (int64_t w = kOne; w < d; w += kOne) {
+    const int64_t b = bytes(w);
+    most = most > b ? most : b;
   }
-  *out_bytes = (int64_t)blocks * 2 * d * (int64_t)sizeof(float);
+  *out_bytes = most;
   return VRS_OK;
 }
 

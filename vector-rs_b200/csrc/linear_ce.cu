@@ -454,7 +454,9 @@ int launch_finish(const float* acc, int splits, int64_t split_rows, int d, int d
 // ------------------------------------------------------------- host plan
 
 // Offsets into the workspace, and how the work is cut. Nothing here depends on
-// addresses or on which gradients are asked for, so neither do the sums.
+// addresses or on which gradients are asked for, so neither do the sums. The room
+// for what depends on the cut is a bound that never falls as a size grows, so that
+// a workspace for the largest sizes serves all smaller ones.
 struct Plan {
   int64_t rows_p, dp, d4;         // rows in whole tiles, row pitches
   int64_t piece;                  // classes of a piece, whole tiles
@@ -500,6 +502,11 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
   p.vtiles = (classes + kCeN - 1) / kCeN;
   p.parts = (classes + 127) / 128;
   int64_t at = 0;
+  // The smaller of what all of it takes and a limit, but room for one piece at least.
+  auto most = [](int64_t all, int64_t limit, int64_t least) {
+    const int64_t b = all < limit ? all : limit;
+    return b > least ? b : least;
+  };
   auto take = [&](int64_t bytes) {
     const int64_t o = at;
     at += up(bytes, 256);
@@ -523,7 +530,8 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
     p.planes_dw = small || rows <= kFewTerms ? 2 : 1;
     p.planes = p.planes_dx > p.planes_dw ? p.planes_dx : p.planes_dw;
     p.piece = piece_of(p.rows_p, p.planes, p.vtiles, (d + kCeN - 1) / kCeN) * kCeN;
-    p.g = take(p.planes * p.rows_p * p.piece * 2);
+    // Room for two planes whether a problem has them or not.
+    p.g = take(most(2 * p.rows_p * 2 * kCeN * p.vtiles, kPieceBytes, 2 * p.rows_p * 2 * kCeN));
     // Few tiles: K is split until the pairs have one each, 8 blocks deep at least.
     auto splits = [](int64_t tiles_, int64_t kblocks) {
       int64_t s = kPairs / tiles_ < kblocks / 8 ? kPairs / tiles_ : kblocks / 8;
@@ -532,8 +540,13 @@ Plan make_plan(int64_t rows, int64_t classes, int64_t d, bool back, bool aligned
     const int64_t nt = (d + kCeN - 1) / kCeN;
     p.splits_dx = splits(p.rows_p / kCeM * nt, p.planes_dx * (p.piece / kCeK));
     p.splits_dw = splits(p.piece / kCeM * nt, p.planes_dw * ((rows + kCeK - 1) / kCeK));
-    p.acc_dx = take(p.splits_dx * p.rows_p * p.d4 * 4);
-    p.acc_dw = take(p.splits_dw > 1 ? p.splits_dw * p.piece * p.d4 * 4 : 0);
+    // A split product's tiles are at most kPairs, and its splits one per eight K blocks.
+    const int64_t row_bytes = p.d4 * 4, tiles_bytes = kPairs * (int64_t)kCeM * kCeN * 4;
+    const int64_t most_dx = 2 * (p.vtiles * kCeN / kCeK) / 8, most_dw = 2 * ((rows + kCeK - 1) / kCeK) / 8;
+    const int64_t one = p.rows_p * row_bytes;
+    p.acc_dx = take(most((most_dx < kPairs ? most_dx : kPairs) * one, tiles_bytes, one));
+    p.acc_dw = take(most_dw < 2 ? 0
+                                : most((most_dw < kPairs ? most_dw : kPairs) * p.vtiles * kCeN * row_bytes, tiles_bytes, 0));
   }
   p.bytes = at;
   return p;
