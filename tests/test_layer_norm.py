@@ -377,3 +377,42 @@ def test_workspace_grows_with_every_size(gpu, vc):
     for d in widths:
         for few, many in zip(counts, counts[1:]):
             assert size(few, d) <= size(many, d), (few, many, d)
+
+
+@pytest.mark.gpu
+def test_gradients_have_their_parameters_shape(gpu):
+    """Any shape of d values is taken for weight and bias; gradients come back in it."""
+    import torch
+    from vector_cuda import ops
+    x, w, b, dy = _make(6, 40, torch.float32, torch.float32)
+    flat = [t.clone().requires_grad_(True) for t in (x, w, b)]
+    shaped = [x.clone().requires_grad_(True), w.view(1, 40).clone().requires_grad_(True),
+              b.view(4, 10).clone().requires_grad_(True)]
+    (ops.layer_norm(*flat) * dy).sum().backward()
+    (ops.layer_norm(*shaped) * dy).sum().backward()
+    for p, q in zip(flat, shaped):
+        assert q.grad.shape == q.shape and torch.equal(q.grad.reshape(p.shape), p.grad)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("weight,bias", [(False, False), (True, False), (False, True), (True, True)])
+@pytest.mark.parametrize("dtype,ptype", [("float32", "float32"), ("bfloat16", "float32"), ("float16", "float16")])
+@pytest.mark.parametrize("wanted", ["x", "parameters", "all"])
+def test_autograd_without_some(gpu, weight, bias, dtype, ptype, wanted):
+    """Parameters that are missing, or whose gradient nobody asks for."""
+    import torch
+    from vector_cuda import ops
+    x, w, b, dy = _make(30, 136, getattr(torch, dtype), getattr(torch, ptype))
+    w, b = w if weight else None, b if bias else None
+    if w is None and b is None and wanted == "parameters":
+        pytest.skip("no gradient at all")
+    y, m, r = ops.layer_norm_forward(x, w, b)
+    want = ops.layer_norm_backward(dy, x, w, m, r, None if b is None else b.dtype)
+    leaves = [None if t is None else t.clone().requires_grad_(wanted != ("parameters" if i == 0 else "x"))
+              for i, t in enumerate((x, w, b))]
+    ops.layer_norm(*leaves).backward(dy)
+    for leaf, g in zip(leaves, want):
+        if leaf is None:
+            continue
+        assert (leaf.grad is None) == (not leaf.requires_grad)
+        assert leaf.grad is None or (leaf.grad.dtype == leaf.dtype and torch.equal(leaf.grad, g))

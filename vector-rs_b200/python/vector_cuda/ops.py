@@ -64,6 +64,7 @@ class _LayerNorm(torch.autograd.Function):
         y, mean, rstd = layer_norm_forward(x, weight, bias, eps)
         ctx.save_for_backward(x, weight, mean, rstd)
         ctx.bias_dtype = None if bias is None else bias.dtype
+        ctx.bias_shape = None if bias is None else bias.shape
         return y
 
     @staticmethod
@@ -72,13 +73,15 @@ class _LayerNorm(torch.autograd.Function):
         x, weight, mean, rstd = ctx.saved_tensors
         want = ctx.needs_input_grad[1] or ctx.needs_input_grad[2]
         dx, dw, db = layer_norm_backward(dy, x, weight, mean, rstd, ctx.bias_dtype, want)
-        return dx, dw if ctx.needs_input_grad[1] else None, db if ctx.needs_input_grad[2] else None, None
+        return (dx, dw.view(weight.shape) if ctx.needs_input_grad[1] else None,
+                db.view(ctx.bias_shape) if ctx.needs_input_grad[2] else None, None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
                eps: float = 1e-5) -> torch.Tensor:
     """(x - mean) / sqrt(var + eps) * weight + bias over x's last dimension
-    (at most 32,768 elements). weight and bias are in x's type or float32."""
+    (at most 32,768 elements). weight and bias hold one value a column, both in
+    x's type or both in float32."""
     return _LayerNorm.apply(x, weight, bias, eps)
 
 
