@@ -64,6 +64,8 @@ def main(items: int = 20000, dim: int = 128, batch: int = 1024, steps: int = 60,
         if not quiet and step % 20 == 0:
             print(f"step {step}: loss {losses[-1].item():.4f}")
 
+    ops.check()
+
     # The same encoder at the start of a search: the index answers from the learned table.
     with torch.no_grad():
         x, ids = queries(512)

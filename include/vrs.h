@@ -304,12 +304,21 @@ VRS_API int vrs_selftest_bounded_wait(int64_t limit_ns);
  * Outputs and workspace overlap neither one another nor the inputs.
  * Results do not depend on timing: on one device the same inputs give the same
  * bits. Waits within the kernels are bounded; one that gave up (which no correct
- * launch does) is reported as VRS_ERR_TIMEOUT by the next call of an operator.
+ * launch does) leaves results that are not valid, and is reported as
+ * VRS_ERR_TIMEOUT once, by the next call of an operator or by vrs_operators_status.
  * Calls may be captured in a CUDA graph; the first call of each kind on a
  * device (it sets kernel attributes up, and in a process takes a word of
  * pinned host memory) should precede the capture. Stage names of
  * vrs_profile_read: "layer_norm_forward", "layer_norm_backward",
  * "linear_cross_entropy_forward", "linear_cross_entropy_backward". */
+
+/* Whether a device wait of an operator call has given up: call it after
+ * synchronising with the last call's stream. It waits for nothing itself. */
+VRS_API int vrs_operators_status(void);
+/* Test hook: queues the operators' bounded wait on a barrier that nothing arrives
+ * on. limit_ns in [1 us, 1 s]. */
+VRS_API int vrs_selftest_operator_wait(int64_t limit_ns, void* cuda_stream);
+
 typedef enum vrs_dtype { VRS_F32 = 0, VRS_F16 = 1, VRS_BF16 = 2 } vrs_dtype;
 
 /* y = (x - mean) * rstd * weight + bias per row of d elements (1..32768),

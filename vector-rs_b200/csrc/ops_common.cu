@@ -24,26 +24,40 @@ int sm_count(int* out) {
   return VRS_OK;
 }
 
+namespace {
+
+std::mutex g_word_lock;
+int* g_word = nullptr;  // taken by the first call
+
+// What a wait left in the word, once. (With the lock held.)
+int word_status() {
+  const int code = g_word ? *(volatile int*)g_word : 0;
+  if (!code) return VRS_OK;
+  *(volatile int*)g_word = 0;
+  set_error(VRS_ERR_TIMEOUT, "training operators: a device wait of an earlier call gave up (stage code " +
+                                 std::to_string(code) + "); its results are not valid");
+  return VRS_ERR_TIMEOUT;
+}
+
+}  // namespace
+
 int error_word(int** out) {
-  static std::mutex mu;
-  static int* word = nullptr;
-  std::lock_guard<std::mutex> g(mu);
-  if (!word) {
+  std::lock_guard<std::mutex> g(g_word_lock);
+  if (!g_word) {
     void* p = nullptr;
     VRS_CUDA(cudaHostAlloc(&p, sizeof(int), cudaHostAllocPortable | cudaHostAllocMapped));
-    word = static_cast<int*>(p);
-    *word = 0;
+    g_word = static_cast<int*>(p);
+    *g_word = 0;
   }
-  const int code = *(volatile int*)word;
-  if (code) {
-    *(volatile int*)word = 0;
-    set_error(VRS_ERR_TIMEOUT, "training operators: a device wait of an earlier call gave up (stage code " +
-                                   std::to_string(code) + "); its results are not valid");
-    return VRS_ERR_TIMEOUT;
-  }
-  *out = word;
+  VRS_TRY(word_status());
+  *out = g_word;
   return VRS_OK;
 }
 
 }  // namespace ops
 }  // namespace vrs
+
+extern "C" int vrs_operators_status(void) {
+  std::lock_guard<std::mutex> g(vrs::ops::g_word_lock);
+  return vrs::ops::word_status();
+}

@@ -190,7 +190,7 @@ int sm_count(int* out);
 
 // The word that a device wait which gave up writes: host memory that the
 // device sees, so a later call reads it without waiting for anything. An
-// earlier call's gives VRS_ERR_TIMEOUT once.
+// earlier call's gives VRS_ERR_TIMEOUT once, here or from vrs_operators_status.
 int error_word(int** out);
 
 }  // namespace ops

@@ -6,7 +6,10 @@
 // hanging the GPU; the host then reports VRS_ERR_TIMEOUT. This file runs
 // that exact helper on an mbarrier that nothing ever arrives on (no TMA copy
 // or tensor-core work is in flight), so a test can watch the limit expire
-// and the status reach the C ABI, with the context still usable afterwards.
+// and the status reach the C ABI, with the context still usable afterwards: of a
+// call that waits for its own result, and of the training operators, which do
+// not wait and report through their error word in host memory.
+#include "ops_common.cuh"
 #include "tc_common.cuh"
 #include "vrs_internal.cuh"
 
@@ -14,8 +17,9 @@ namespace vrs {
 namespace {
 
 constexpr int kSelftestCode = 99;
+constexpr int kOperatorCode = 98;
 
-__global__ void bounded_wait_selftest_kernel(uint64_t limit_ns, int* err) {
+__global__ void bounded_wait_selftest_kernel(uint64_t limit_ns, int* err, int code) {
   __shared__ uint64_t bar;
   __shared__ int s_abort;
   if (threadIdx.x == 0) {
@@ -24,24 +28,38 @@ __global__ void bounded_wait_selftest_kernel(uint64_t limit_ns, int* err) {
     tc::fence_mbar_init();
   }
   __syncthreads();
-  if (threadIdx.x == 0) tc::mbar_wait(&bar, 0, (volatile int*)&s_abort, err, kSelftestCode, limit_ns);
+  if (threadIdx.x == 0) tc::mbar_wait(&bar, 0, (volatile int*)&s_abort, err, code, limit_ns);
+}
+
+int check_limit(const char* who, int64_t limit_ns) {
+  if (limit_ns >= 1000 && limit_ns <= 1000000000LL) return VRS_OK;
+  set_error(VRS_ERR_INVALID_CONFIG, std::string(who) + ": limit must be in [1 us, 1 s]");
+  return VRS_ERR_INVALID_CONFIG;
 }
 
 }  // namespace
 }  // namespace vrs
 
+extern "C" int vrs_selftest_operator_wait(int64_t limit_ns, void* cuda_stream) {
+  using namespace vrs;
+  VRS_TRY(check_limit("vrs_selftest_operator_wait", limit_ns));
+  int* err = nullptr;
+  VRS_TRY(ops::error_word(&err));
+  bounded_wait_selftest_kernel<<<1, 32, 0, (cudaStream_t)cuda_stream>>>((uint64_t)limit_ns, err, kOperatorCode);
+  VRS_CUDA(cudaGetLastError());
+  count_launch();
+  return VRS_OK;
+}
+
 extern "C" int vrs_selftest_bounded_wait(int64_t limit_ns) {
   using namespace vrs;
-  if (limit_ns < 1000 || limit_ns > 1000000000LL) {
-    set_error(VRS_ERR_INVALID_CONFIG, "vrs_selftest_bounded_wait: limit must be in [1 us, 1 s]");
-    return VRS_ERR_INVALID_CONFIG;
-  }
+  VRS_TRY(check_limit("vrs_selftest_bounded_wait", limit_ns));
   int* d_err = nullptr;
   VRS_CUDA(cudaMalloc(&d_err, sizeof(int)));
   int h_err = 0;
   cudaError_t e = cudaMemset(d_err, 0, sizeof(int));
   if (e == cudaSuccess) {
-    bounded_wait_selftest_kernel<<<1, 32>>>((uint64_t)limit_ns, d_err);
+    bounded_wait_selftest_kernel<<<1, 32>>>((uint64_t)limit_ns, d_err, kSelftestCode);
     count_launch();
     e = cudaGetLastError();
   }

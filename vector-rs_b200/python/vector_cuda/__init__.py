@@ -180,6 +180,7 @@ def lib() -> ctypes.CDLL:
         L.vrs_ivfpq_destroy.argtypes = [c.c_void_p]
         L.vrs_ivfpq_destroy.restype = None
         vp, i64, i32, f32 = c.c_void_p, c.c_int64, c.c_int32, c.c_float
+        L.vrs_selftest_operator_wait.argtypes = [i64, vp]
         L.vrs_layer_norm_forward.argtypes = [vp, i64, i64, i64, i32, vp, vp, i32, f32, vp, i64, vp, vp, vp]
         L.vrs_layer_norm_backward_workspace.argtypes = [i64, i64, P(i64)]
         L.vrs_layer_norm_backward.argtypes = [vp, i64, vp, i64, i64, i64, i32, vp, i32, vp, vp, vp, i64, vp, vp,

@@ -38,6 +38,14 @@ def _bind():
 _bind()
 
 
+def check() -> None:
+    """Waits for the current device and raises CudaError where a device wait of an
+    earlier call gave up, whose results are then not valid. (No correct launch
+    does that. Without this the next call raises it, a program's last none.)"""
+    torch.cuda.synchronize()
+    _check(lib().vrs_operators_status())
+
+
 # ---------------------------------------------------------------- layer norm
 
 
@@ -142,5 +150,5 @@ def linear_cross_entropy(x: torch.Tensor, table: torch.Tensor, targets: torch.Te
     return total / taken.clamp(min=1)
 
 
-__all__ = ["layer_norm", "layer_norm_forward", "layer_norm_backward", "linear_cross_entropy",
+__all__ = ["check", "layer_norm", "layer_norm_forward", "layer_norm_backward", "linear_cross_entropy",
            "linear_cross_entropy_forward", "linear_cross_entropy_backward"]
