@@ -325,12 +325,6 @@ __global__ void __launch_bounds__(256) ce_pack_kernel(const Pack1 a) {
 
 // --------------------------------------------------------- combine, finish
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // (maximum, sum of powers of two below it) of two sets.
 __device__ __forceinline__ float2 merge(float2 a, float2 b) {
   const float m = fmaxf(a.x, b.x), sub = m == -INFINITY ? 0.0f : m;

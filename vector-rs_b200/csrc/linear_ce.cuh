@@ -78,6 +78,13 @@ struct CeGemm {
   int64_t g_pitch;
 };
 
+// 2^x, the score exponentials' instruction.
+__device__ __forceinline__ float ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
 // The product of two rows of d 16-bit floats by one warp, rounded to nearest at
 // every step. The tensor cores' sums are cut off instead: over d terms of one
 // sign, as a trained row's product with its target has, some d / 16 half units

@@ -124,12 +124,6 @@ __device__ __forceinline__ void bulk_wait_read() {
 }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
-__device__ __forceinline__ float ex2(float x) {
-  float r;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
-  return r;
-}
-
 // 32 lanes x 32 columns; the values may be used only after tmem_wait.
 __device__ __forceinline__ void tmem_ld_issue(uint32_t taddr, float (&v)[CHUNK]) {
   asm volatile(
