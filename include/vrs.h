@@ -363,7 +363,8 @@ VRS_API int vrs_linear_cross_entropy_forward(const void* x, int64_t x_stride, in
  * The scores are computed again, in pieces of the classes, and their gradients
  * held in 16 bits (two such parts where few terms make up a sum) relative to the
  * largest finite |dloss|: VRS_F16 keeps them down to 2^-38 of that, so rows whose
- * weight is less than some 2^-20 of another's lose digits. The score gradient of
+ * weight is less than some 2^-20 of another's lose digits. A probability below
+ * 2^-126 counts as 0. The score gradient of
  * a row's target, e^-loss - 1, is taken from lse - z[target] here, which is off by
  * half of lse's last place: 5e-7 at lse 8 to 16, as much as the gradient itself
  * where the loss is that small. ..._with_loss takes the forward pass's loss as
