@@ -381,6 +381,70 @@ VRS_API int vrs_linear_cross_entropy_backward_with_loss(
     void* dx, int64_t dx_stride, void* dtable, int64_t dtable_stride, void* workspace, int64_t workspace_bytes,
     void* cuda_stream);
 
+/* ------------------------------------------------- encoder operators */
+/* No counterpart in the reference. What a text encoder needs beside the layer
+ * norm: its attention with the norms and rotation of queries and keys before
+ * it, and the norm and clipping of a training step's gradients. Everything said
+ * of the training operators holds here: buffers, streams, workspaces (which
+ * never shrink as a size grows), determinism, errors, capture. Stage names of vrs_profile_read: "attention_forward",
+ * "attention_backward", "qk_norm_rope_forward", "qk_norm_rope_backward",
+ * "grad_norm", "clip_grad_norm". */
+
+/* tokens x heads x d elements: `stride` between tokens, `head_stride` between
+ * heads, both in elements; the d elements of a head are contiguous. */
+typedef struct vrs_heads {
+  void* data;
+  int64_t stride, head_stride;
+} vrs_heads;
+
+/* The RMS norm of each head's query and key (x / sqrt(mean x^2 + eps) * weight),
+ * then the rotation to its position of the first `rotary` elements (even, 0..d):
+ * pair i turns by position * base^(-2 i / rotary), pairs being elements i and
+ * i + rotary / 2 or, interleaved, 2 i and 2 i + 1. q and k in dtype, d even and at
+ * most 256; weights (d values, NULL: ones) in dtype or f32 (param_dtype); q_out
+ * and k_out tokens x heads x d without gaps. Angles are computed in 64 bits:
+ * any position below 2^31 keeps its place in a turn to 2^-21. */
+VRS_API int vrs_qk_norm_rope_forward(const vrs_heads* q, int64_t heads, const vrs_heads* k, int64_t kv_heads,
+                                     int64_t tokens, int64_t d, int32_t dtype, const int64_t* positions,
+                                     const void* q_weight, const void* k_weight, int32_t param_dtype, double base,
+                                     int64_t rotary, int32_t interleaved, float eps, void* q_out, void* k_out,
+                                     void* cuda_stream);
+
+/* Gradients of the above from those of q_out and k_out: dq and dk (in dtype,
+ * without gaps), dq_weight and dk_weight (in param_dtype, either or both NULL;
+ * sums are held in f32). The workspace (4-byte aligned) is needed for the
+ * weights' gradients only. tokens == 0 gives zero dq_weight and dk_weight. */
+VRS_API int vrs_qk_norm_rope_backward_workspace(int64_t tokens, int64_t d, int64_t* out_bytes);
+VRS_API int vrs_qk_norm_rope_backward(const vrs_heads* dq_out, const vrs_heads* dk_out, const vrs_heads* q,
+                                      int64_t heads, const vrs_heads* k, int64_t kv_heads, int64_t tokens, int64_t d,
+                                      int32_t dtype, const int64_t* positions, const void* q_weight,
+                                      const void* k_weight, int32_t param_dtype, double base, int64_t rotary,
+                                      int32_t interleaved, float eps, void* dq, void* dk, void* dq_weight,
+                                      void* dk_weight, void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
+/* One tensor of a list of gradients: `count` elements in dtype, one after
+ * another; its result in the same type or in f32. out == grad: in place. */
+typedef struct vrs_grad {
+  const void* grad;
+  void* out; /* vrs_clip_grad_norm only */
+  int64_t count;
+  int32_t dtype, out_dtype;
+} vrs_grad;
+
+/* norm (f32[1]) = unscale * sqrt(sum of all squares); unscale is the inverse of
+ * a loss scale. Squares are added in f64 wherever f32 could lose them, so any
+ * list whose norm is a float has it. The list is read during the call. The
+ * workspace must be 8-byte aligned. At most 2^42 elements. */
+VRS_API int vrs_grad_norm_workspace(int64_t tensors, int64_t* out_bytes);
+VRS_API int vrs_grad_norm(const vrs_grad* grads, int64_t tensors, float unscale, float* norm, void* workspace,
+                          int64_t workspace_bytes, void* cuda_stream);
+/* The norm as above, and out = grad * unscale * min(1, max_norm / (norm + 1e-6)).
+ * An infinite norm gives zeros, and NaN where the gradient is not finite; a NaN
+ * norm gives NaN. In place nothing is written where the factor is 1. Results
+ * overlap neither one another nor other gradients. */
+VRS_API int vrs_clip_grad_norm(const vrs_grad* grads, int64_t tensors, float max_norm, float unscale, float* norm,
+                               void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
 /* ------------------------------------------------------ streams, profiling */
 /* Makes a single-GPU or rank-mode handle issue its work on `cuda_stream`
  * (a cudaStream_t of the handle's device; NULL restores the handle's own).

@@ -1,0 +1,266 @@
+"""The norm over a list of gradients and their clipping (vrs_grad_norm,
+vrs_clip_grad_norm, vector_cuda.ops) against 64 bits, and refusals.
+
+Tolerances, e = 2^-24. Up to 8 squares are added in 32 bits (9 e of their sum at
+most), the rest in 64: the sum is off by 9 e of itself, the norm by 4.5 e and the
+rounding of the result, e. unscale and max_norm travel as 32-bit numbers, which
+the formula here takes too. The factor is off by 4.5 e and its rounding, a
+result by that, the product's rounding and half an ulp of its type."""
+import ctypes
+import math
+
+import pytest
+
+HALF = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+TINY = {"float32": 2.0 ** -149, "float16": 2.0 ** -25, "bfloat16": 2.0 ** -133}
+E = 2.0 ** -24
+
+
+def _f32(v):
+    return ctypes.c_float(v).value
+
+
+def _want(grads, max_norm=None, unscale=1.0):
+    u = _f32(unscale)
+    norm = math.sqrt(math.fsum(float(t.double().square().sum()) for t in grads)) * u
+    factor = None if max_norm is None else min(1.0, _f32(max_norm) / (norm + 1e-6)) * u
+    return norm, factor
+
+
+def _near_norm(norm, want):
+    assert norm.shape == () and str(norm.dtype) == "torch.float32"
+    assert abs(norm.item() - want) <= 6 * E * want + 2.0 ** -149
+
+
+def _near(got, grad, factor):
+    name = str(got.dtype).replace("torch.", "")
+    want = grad.double() * factor
+    off = (got.double() - want).abs()
+    assert (off <= (7 * E + 1.01 * HALF[name]) * want.abs() + TINY[name]).all(), (off / want.abs()).max()
+
+
+def _list(shapes, dtypes, seed=0, size=1.0):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return [(torch.randn(s, generator=g, device="cuda") * size).to(getattr(torch, dtypes[i % len(dtypes)]))
+            for i, s in enumerate(shapes)]
+
+
+SHAPES = [[1], [(3, 5)], [0, 7, 0], [4096, 4097, 8191, 1, 8193], [(64, 384), 384, (384, 1536), 1536],
+          [2 ** 20 + 3, 17, 300000], [5] * 40, [1 + 37 * i for i in range(300)], [1 + i % 9 for i in range(2300)]]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtypes", [["float32"], ["float16"], ["bfloat16"], ["bfloat16", "float32", "float16"]])
+@pytest.mark.parametrize("shapes", SHAPES, ids=[str(i) for i in range(len(SHAPES))])
+def test_norm_and_clip(gpu, shapes, dtypes):
+    import torch
+    from vector_cuda import ops
+    grads = _list(shapes, dtypes)
+    norm, factor = _want(grads, 0.5, 0.25)
+    _near_norm(ops.grad_norm(grads, 0.25), norm)
+    # into 32 bits, into the same types, in place
+    before = [t.clone() for t in grads]
+    for kind in ("wide", "same", "place"):
+        out = None if kind == "place" else [torch.full_like(t, 7, dtype=torch.float32 if kind == "wide" else t.dtype)
+                                            for t in grads]
+        _near_norm(ops.clip_grad_norm(grads, 0.5, out, 0.25), norm)
+        for a, b in zip(grads if out is None else out, before):
+            _near(a, b, factor)
+        if out is not None:
+            assert all(torch.equal(a, b) for a, b in zip(grads, before))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,out", [("float32", None), ("float16", None), ("bfloat16", "float32"), ("float16", "float32"),
+                                       ("float32", "float32")])
+@pytest.mark.parametrize("offset", [0, 1, 2, 3, 5, 7])
+def test_views_of_flat_buffers(gpu, dtype, out, offset):
+    """Tensors at any element of a flat buffer, and results at others; what lies between stays."""
+    import torch
+    from vector_cuda import ops
+    sizes = [1, 2, 3, 4095, 9000, 16, 5, 12289]
+    g = torch.Generator(device="cuda").manual_seed(3)
+    gap = 3
+
+    def views(dt, first):
+        flat = torch.full((first + sum(sizes) + gap * len(sizes),), 7.0, dtype=dt, device="cuda")
+        at, vs, mask = first, [], torch.ones(flat.numel(), dtype=torch.bool, device="cuda")
+        for n in sizes:
+            vs.append(flat[at:at + n])
+            mask[at:at + n] = False
+            at += n + gap
+        return flat, vs, mask
+
+    flat, grads, between = views(getattr(torch, dtype), offset)
+    for t in grads:
+        t.copy_(torch.randn(t.shape, generator=g, device="cuda"))
+    before = [t.clone() for t in grads]
+    norm, factor = _want(grads, 1.0)
+    if out:
+        flat, results, between = views(getattr(torch, out), 2 * offset % 5)
+        _near_norm(ops.clip_grad_norm(grads, 1.0, results), norm)
+    else:
+        results = grads
+        _near_norm(ops.clip_grad_norm(grads, 1.0), norm)
+    for a, b in zip(results, before):
+        _near(a, b, factor)
+    assert (flat[between] == 7.0).all()
+
+
+@pytest.mark.gpu
+def test_orders_and_gaps(gpu):
+    """Transposed, channels last, rows with gaps, expanded gradients."""
+    import torch
+    from vector_cuda import ops
+    base = _list([(40, 30), (2, 3, 8, 9), (50, 20), (7,)], ["float32"])
+    buffer = torch.full((50, 33), 7.0, device="cuda")
+    grads = [base[0].t(), base[1].to(memory_format=torch.channels_last), buffer[:, 5:25], base[3]]
+    grads[2].copy_(base[2])
+    one = torch.full((), 0.5, device="cuda").expand(6, 11)
+    before = [t.clone() for t in grads]
+    norm, factor = _want([*grads, one], 2.0)
+    out = [torch.empty(t.shape, device="cuda") for t in [*grads, one]]
+    _near_norm(ops.clip_grad_norm([*grads, one], 2.0, out), norm)
+    for a, b in zip(out, [*before, one]):
+        _near(a, b, factor)
+    with pytest.raises(ValueError, match="expanded"):
+        ops.clip_grad_norm([one], 2.0)
+    norm, factor = _want(grads, 2.0)
+    _near_norm(ops.clip_grad_norm(grads, 2.0), norm)
+    for a, b in zip(grads, before):
+        _near(a, b, factor)
+    assert (buffer[:, :5] == 7.0).all() and (buffer[:, 25:] == 7.0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("size", [2.0 ** -140, 2.0 ** -120, 2.0 ** -75, 2.0 ** -50, 1.0, 2.0 ** 62, 2.0 ** 80, 2.0 ** 115])
+def test_any_size(gpu, dtype, size):
+    """Squares beyond a 32-bit float's range on both sides; also one large value among small ones."""
+    import torch
+    from vector_cuda import ops
+    if dtype == "bfloat16" and size < 2.0 ** -130:
+        size = 2.0 ** -125
+    grads = [(t.double() * size).to(getattr(torch, dtype)) for t in _list([1000, 4099, 3], ["float32"])]
+    norm, factor = _want(grads, size, 0.5)
+    _near_norm(ops.grad_norm(grads, 0.5), norm)
+    out = [torch.empty_like(t, dtype=torch.float32) for t in grads]
+    ops.clip_grad_norm(grads, size, out, 0.5)
+    if norm > 1e-3:  # (below, the formula's 1e-6 decides and the factor is unscale)
+        for a, b in zip(out, grads):
+            _near(a, b, factor)
+    grads[1][5] = 2.0 ** 100
+    norm, _ = _want(grads)
+    _near_norm(ops.grad_norm(grads), norm)
+
+
+@pytest.mark.gpu
+def test_factor_one_leaves_the_bits(gpu):
+    import torch
+    from vector_cuda import ops
+    grads = _list([1000, 5000], ["float32", "bfloat16"], size=1e-3)
+    before = [t.clone() for t in grads]
+    norm, _ = _want(grads)
+    _near_norm(ops.clip_grad_norm(grads, 100.0), norm)
+    assert all(torch.equal(a, b) for a, b in zip(grads, before))
+    # a negative zero and a NaN's bits too
+    grads[0][3] = -0.0
+    ops.clip_grad_norm(grads, 100.0)
+    assert math.copysign(1, grads[0][3].item()) == -1
+
+
+@pytest.mark.gpu
+def test_not_finite(gpu):
+    import torch
+    from vector_cuda import ops
+    for dtype in ("float32", "float16", "bfloat16"):
+        grads = _list([1000, 3], [dtype])
+        grads[0][17] = float("inf")
+        out = [torch.empty_like(t) for t in grads]
+        assert ops.clip_grad_norm(grads, 1.0, out).item() == math.inf
+        assert out[0][17].isnan() and not out[0][:17].any() and not out[1].any()
+        grads[1][0] = float("nan")
+        assert ops.clip_grad_norm(grads, 1.0, out).isnan()
+        assert all(t.isnan().all() for t in out)
+        zeros = [torch.zeros_like(t) for t in grads]
+        assert ops.clip_grad_norm(zeros, 0.0).item() == 0.0 and not zeros[0].any()
+
+
+@pytest.mark.gpu
+def test_same_bits_captured_and_on_another_stream(gpu):
+    import torch
+    from vector_cuda import ops
+    grads = _list([300000, 77, 2 ** 21 + 1], ["bfloat16", "float32"])
+    out = [torch.empty_like(t) for t in grads]
+    norm = ops.clip_grad_norm(grads, 1.0, out)
+    want = [norm.clone(), *(t.clone() for t in out)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        norm = ops.clip_grad_norm(grads, 1.0, out)
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, [norm, *out]))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = ops.clip_grad_norm(grads, 1.0, out)
+    for t in out:
+        t.zero_()
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(want, [norm, *out]))
+
+
+@pytest.mark.gpu
+def test_autograd_notices(gpu):
+    import torch
+    from vector_cuda import ops
+    x = torch.ones(5, device="cuda", requires_grad=True)
+    w = torch.full((5,), 3.0, device="cuda")
+    y = (x * w).sum()
+    ops.clip_grad_norm([w], 1.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+
+
+@pytest.mark.gpu
+def test_python_refusals(gpu):
+    import torch
+    from vector_cuda import ops
+    t = torch.ones(8, device="cuda")
+    for bad in (lambda: ops.grad_norm([]), lambda: ops.grad_norm([t.cpu()]), lambda: ops.grad_norm([t.double()]),
+                lambda: ops.grad_norm(3), lambda: ops.grad_norm([3]), lambda: ops.clip_grad_norm([t], -1.0),
+                lambda: ops.clip_grad_norm([t], math.nan), lambda: ops.clip_grad_norm([t], 1.0, unscale=0.0),
+                lambda: ops.clip_grad_norm([t], 1.0, unscale=math.inf), lambda: ops.clip_grad_norm([t], 1.0, []),
+                lambda: ops.clip_grad_norm([t], 1.0, [t.half()]), lambda: ops.clip_grad_norm([t], 1.0, [t[:4]]),
+                lambda: ops.clip_grad_norm([t, t], 1.0), lambda: ops.clip_grad_norm([t[:5], t[4:]], 1.0),
+                lambda: ops.clip_grad_norm([t[:4], t[4:]], 1.0, [t[2:6], torch.empty(4, device="cuda")])):
+        with pytest.raises(ValueError):
+            bad()
+    assert (t == 1).all()
+
+
+class Grad(ctypes.Structure):
+    _fields_ = [("grad", ctypes.c_void_p), ("out", ctypes.c_void_p), ("count", ctypes.c_int64),
+                ("dtype", ctypes.c_int32), ("out_dtype", ctypes.c_int32)]
+
+
+def test_c_refusals(vc):
+    """Wrong arguments are told by status before anything is queued (no GPU needed)."""
+    L, i64, f = vc.lib(), ctypes.c_int64, ctypes.c_float
+    n = i64(0)
+    assert L.vrs_grad_norm_workspace(i64(5), ctypes.byref(n)) == 0
+    small = n.value
+    assert L.vrs_grad_norm_workspace(i64(5000), ctypes.byref(n)) == 0 and n.value >= small > 0
+    assert L.vrs_grad_norm_workspace(i64(-1), ctypes.byref(n)) == 5
+    assert L.vrs_grad_norm_workspace(i64(1), None) == 5
+
+    def call(g=Grad(256, 512, 8, 1, 0), tensors=1, limit=1.0, unscale=1.0, norm=256, ws=256, need=small):
+        return L.vrs_clip_grad_norm(ctypes.byref(g) if g else None, i64(tensors), f(limit), f(unscale),
+                                    ctypes.c_void_p(norm), ctypes.c_void_p(ws), i64(need), None)
+
+    for bad in (dict(g=None), dict(tensors=-1), dict(limit=-1.0), dict(limit=math.nan), dict(unscale=0.0),
+                dict(unscale=math.inf), dict(norm=None), dict(ws=None), dict(ws=260), dict(need=small - 1),
+                dict(g=Grad(None, 512, 8, 1, 0)), dict(g=Grad(256, None, 8, 1, 0)), dict(g=Grad(257, 512, 8, 1, 0)),
+                dict(g=Grad(256, 514, 8, 1, 0)), dict(g=Grad(256, 512, -1, 1, 0)), dict(g=Grad(256, 512, 8, 3, 0)),
+                dict(g=Grad(256, 512, 8, 1, 2)), dict(g=Grad(256, 256, 8, 1, 0)), dict(g=Grad(256, 512, 1 << 43, 1, 0))):
+        assert call(**bad) == 5, bad

@@ -1,0 +1,299 @@
+"""Norms and rotation of queries and keys (vrs_qk_norm_rope_*, vector_cuda.ops):
+both passes against the formulas in 64 bits, differences, refusals.
+
+Tolerances, e = 2^-24. A sum of d squares in 32 bits is off by at most (d + 2) e
+of itself, rstd by half of that and 4 roundings, so xhat w by (d / 2 + 8) e. An
+angle is exact in 64 bits but for its remainder's rounding to 32 (at most
+e pi / 2 ... taken as 2 e of a radian) and sincospi's 2 ulps: each product of a
+rotation is off by 8 e of its factors' size. Together a result is off by
+E = (d + 24) e times |a| + |b| of its pair, and half an ulp of its type.
+Backward the turned gradient has the same error times the pair's |dy|; mean(g w
+xhat) adds d e of the terms' sizes. A weight's gradient is a sum of N = tokens x
+heads terms, off by at most (N + d + 40) e of the sum of their sizes."""
+import ctypes
+import math
+
+import pytest
+
+HALF = {"float32": 2.0 ** -24, "float16": 2.0 ** -11, "bfloat16": 2.0 ** -8}
+TINY = {"float32": 2.0 ** -149, "float16": 2.0 ** -25, "bfloat16": 2.0 ** -133}
+
+
+def _make(tokens, heads, kv, d, dtype, params, seed=0, far=0):
+    import torch
+    g = torch.Generator(device="cuda").manual_seed(seed + tokens + 31 * d)
+    dt, pt = getattr(torch, dtype), getattr(torch, params)
+
+    def normal(*s):
+        return torch.randn(*s, generator=g, device="cuda")
+
+    return {"q": (normal(tokens, heads, d) * 1.3 + 0.1).to(dt), "k": (normal(tokens, kv, d) * 0.7).to(dt),
+            "positions": torch.randint(0, 5000, (tokens,), generator=g, device="cuda") + far,
+            "q_weight": (1 + 0.3 * normal(d)).to(pt), "k_weight": (1 + 0.3 * normal(d)).to(pt),
+            "dq_out": normal(tokens, heads, d).to(dt), "dk_out": normal(tokens, kv, d).to(dt)}
+
+
+def _pairs(d, rotary, interleaved):
+    """The other element of each one's pair (itself where it is not turned), and which is first."""
+    import torch
+    half = rotary // 2
+    other, first, index = list(range(d)), [False] * d, [0] * d
+    for i in range(half):
+        a, b = (2 * i, 2 * i + 1) if interleaved else (i, i + half)
+        other[a], other[b], first[a], index[a], index[b] = b, a, True, i, i
+    return (torch.tensor(other, device="cuda"), torch.tensor(first, device="cuda"),
+            torch.tensor(index, device="cuda"))
+
+
+def _turn(x, positions, base, rotary, interleaved, back=False):
+    """(turned, |a| + |b| of each element's pair), in 64 bits."""
+    import torch
+    d = x.shape[-1]
+    other, first, index = _pairs(d, rotary, interleaved)
+    moved = other != torch.arange(d, device="cuda")
+    power = torch.tensor([base ** (-2.0 * i / max(1, rotary)) for i in range(max(1, rotary // 2))],
+                         dtype=torch.float64, device="cuda")
+    angle = positions.double().view(-1, 1, 1) * power[index] * moved
+    sign = torch.where(first, -1.0, 1.0) * (-1.0 if back else 1.0) * moved
+    return x * torch.cos(angle) + x[..., other] * torch.sin(angle) * sign, x.abs() + x[..., other].abs() * moved
+
+
+def _check(s, base=10000.0, rotary=None, interleaved=False, eps=1e-6, shape=None):
+    import torch
+    from vector_cuda import ops
+    d = s["q"].shape[-1]
+    r = d if rotary is None else rotary
+    name = str(s["q"].dtype).replace("torch.", "")
+    h, tiny, e = HALF[name], TINY[name], 2.0 ** -24
+    args = (s["q"], s["k"], s["positions"], s["q_weight"], s["k_weight"], base, rotary, interleaved, eps)
+    got = dict(zip(("q", "k"), ops.qk_norm_rope_forward(*args)))
+    grads = dict(zip(("dq", "dk", "dq_weight", "dk_weight"),
+                     ops.qk_norm_rope_backward(s["dq_out"], s["dk_out"], *args)))
+
+    def near(a, want, lim, what, half=h, small=tiny):
+        assert a.dtype == (s["q_weight"].dtype if "weight" in what else s["q"].dtype)
+        off, lim = (a.double() - want).abs(), lim + 1.01 * half * want.abs() + small
+        assert (off <= lim).all(), f"{what}: {int((off > lim).sum())} of {off.numel()} off, worst {(off / lim).max().item():.3g}x"
+
+    for n in ("q", "k"):
+        x, w, dy = s[n].double(), s[n + "_weight"].double().flatten(), s[f"d{n}_out"].double()
+        x, dy = x.reshape(-1, *x.shape[-2:]), dy.reshape(-1, *dy.shape[-2:])
+        rstd = (x.square().mean(-1, keepdim=True) + eps).rsqrt()
+        xhat = x * rstd
+        y, size = _turn(xhat * w, s["positions"].flatten(), base, r, interleaved)
+        near(got[n].reshape(y.shape), y, (d + 24) * e * size, n)
+        assert got[n].shape == s[n].shape and got[n].is_contiguous()
+        g, gsize = _turn(dy, s["positions"].flatten(), base, r, interleaved, back=True)
+        terms = x.shape[0] * x.shape[1]
+        wname = str(s[n + "_weight"].dtype).replace("torch.", "")
+        near(grads[f"d{n}_weight"], (g * xhat).sum((0, 1)), (terms + d + 40) * e * (gsize * xhat.abs()).sum((0, 1)),
+             f"d{n}_weight", HALF[wname], TINY[wname])
+        mean = (g * w * xhat).mean(-1, keepdim=True)
+        dx = rstd * (g * w - xhat * mean)
+        lim = (2 * d + 64) * e * rstd * (gsize * w.abs() + xhat.abs() * (gsize * w.abs() * xhat.abs()).mean(-1, keepdim=True))
+        near(grads["d" + n].reshape(dx.shape), dx, lim, "d" + n)
+        assert grads["d" + n].shape == s[n].shape
+    return got, grads
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype,params", [("float32", "float32"), ("float16", "float16"), ("float16", "float32"),
+                                          ("bfloat16", "bfloat16"), ("bfloat16", "float32")])
+@pytest.mark.parametrize("tokens,heads,kv,d", [(1, 1, 1, 2), (1, 12, 12, 64), (13, 3, 1, 6), (300, 7, 7, 80),
+                                               (257, 4, 2, 128), (65, 2, 1, 256), (40, 5, 3, 46), (33, 2, 2, 254),
+                                               (3, 20, 4, 16), (5000, 2, 1, 32), (31, 1, 1, 72)])
+def test_matches_formula(gpu, tokens, heads, kv, d, dtype, params):
+    _check(_make(tokens, heads, kv, d, dtype, params))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("d,rotary", [(64, 64), (64, 32), (64, 0), (64, 2), (80, 40), (128, 64), (128, 26), (256, 128),
+                                      (30, 10), (96, 96)])
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+def test_part_of_a_head(gpu, d, rotary, interleaved, dtype):
+    _check(_make(70, 6, 2, d, dtype, dtype), rotary=rotary, interleaved=interleaved)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("far", [1 << 20, (1 << 31) - 6000, -100000])
+@pytest.mark.parametrize("base", [10000.0, 1e6, 2.0])
+def test_far_positions(gpu, far, base):
+    _check(_make(50, 2, 2, 64, "float32", "float32", far=far), base=base)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float32", "float16"])
+@pytest.mark.parametrize("gap,offset", [(0, 0), (8, 8), (4, 4), (3, 1), (2, 0), (0, 1)])
+def test_views(gpu, gap, offset, dtype):
+    """Parts of one projection's result, with gaps and at any element."""
+    import torch
+    s = _make(37, 6, 2, 64, dtype, "float32")
+    wide = 10 * 64 + gap
+    flat = torch.full((37 * wide + offset,), float("nan"), dtype=s["q"].dtype, device="cuda")
+    rows = flat[offset:].view(37, wide)
+    v = dict(s)
+    v["q"], v["k"] = rows[:, :384].view(37, 6, 64), rows[:, 384:512].view(37, 2, 64)
+    v["q"].copy_(s["q"])
+    v["k"].copy_(s["k"])
+    _check(v)  # (narrow accesses add a head's squares in another order: not the same bits)
+
+
+@pytest.mark.gpu
+def test_other_orders(gpu):
+    """Heads before tokens, a batch of sequences, elements that are not contiguous."""
+    import torch
+    s = _make(48, 4, 2, 64, "bfloat16", "bfloat16")
+    want, wantg = _check(s)
+    v = dict(s)
+    v["q"] = s["q"].transpose(0, 1).contiguous().transpose(0, 1)
+    v["k"] = s["k"].transpose(1, 2).contiguous().transpose(1, 2)
+    v["dq_out"] = s["dq_out"].transpose(0, 1).contiguous().transpose(0, 1)
+    got, gotg = _check(v)
+    assert all(torch.equal(want[n], got[n]) for n in want) and all(torch.equal(wantg[n], gotg[n]) for n in wantg)
+    v = {n: t.view(3, 16, *t.shape[1:]) if t.shape[0] == 48 else t for n, t in s.items()}
+    got, gotg = _check(v)
+    assert all(torch.equal(want[n], got[n].view(want[n].shape)) for n in want)
+    # the gradient of a sum is one number seen through strides of 0
+    v = dict(s)
+    v["dq_out"] = torch.ones((), dtype=torch.bfloat16, device="cuda").expand(48, 4, 64)
+    _check(v)
+
+
+@pytest.mark.gpu
+def test_no_weights_and_no_tokens(gpu):
+    import torch
+    from vector_cuda import ops
+    s = _make(20, 3, 1, 32, "float16", "float16")
+    ones = dict(s)
+    ones["q_weight"], ones["k_weight"] = (torch.ones(32, dtype=torch.float16, device="cuda") for _ in range(2))
+    want, wantg = _check(ones)
+    q, k = ops.qk_norm_rope_forward(s["q"], s["k"], s["positions"])
+    dq, dk, a, b = ops.qk_norm_rope_backward(s["dq_out"], s["dk_out"], s["q"], s["k"], s["positions"])
+    assert a is None and b is None
+    assert torch.equal(q, want["q"]) and torch.equal(k, want["k"])
+    assert torch.equal(dq, wantg["dq"]) and torch.equal(dk, wantg["dk"])
+    dq, dk, a, b = ops.qk_norm_rope_backward(s["dq_out"], s["dk_out"], s["q"], s["k"], s["positions"], s["q_weight"])
+    assert a is not None and b is None
+    empty = {n: t[:0] if t.shape[0] == 20 else t for n, t in s.items()}
+    q, k = ops.qk_norm_rope_forward(empty["q"], empty["k"], empty["positions"])
+    assert q.shape == (0, 3, 32) and k.shape == (0, 1, 32)
+    dq, dk, a, b = ops.qk_norm_rope_backward(empty["dq_out"], empty["dk_out"], empty["q"], empty["k"],
+                                             empty["positions"], s["q_weight"], s["k_weight"])
+    assert not a.any() and not b.any() and dq.shape == (0, 3, 32)
+
+
+@pytest.mark.gpu
+def test_values_that_are_not_finite_stay_in_their_head(gpu):
+    import torch
+    from vector_cuda import ops
+    s = _make(30, 4, 2, 64, "bfloat16", "float32")
+    a = ops.qk_norm_rope_forward(s["q"], s["k"], s["positions"], s["q_weight"], s["k_weight"])
+    s["q"][3, 1, 5] = float("nan")
+    s["k"][7, 1, 0] = float("inf")
+    b = ops.qk_norm_rope_forward(s["q"], s["k"], s["positions"], s["q_weight"], s["k_weight"])
+    assert b[0][3, 1].isnan().all() and not torch.isfinite(b[1][7, 1, 0])
+    for x, y, t, h in ((a[0], b[0], 3, 1), (a[1], b[1], 7, 1)):
+        keep = torch.ones(x.shape[:2], dtype=torch.bool)
+        keep[t, h] = False
+        assert torch.equal(x[keep], y[keep])
+
+
+@pytest.mark.gpu
+def test_gradients_against_differences(gpu):
+    import torch
+    from vector_cuda import ops
+    s = _make(6, 2, 1, 16, "float32", "float32")
+    leaves = [s[n].clone().requires_grad_(True) for n in ("q", "k", "q_weight", "k_weight")]
+
+    def f(q, k, a, b):
+        x, y = ops.qk_norm_rope(q, k, s["positions"], a, b, rotary_dim=12)
+        return (x.double() * s["dq_out"].double()).sum() + (y.double() * s["dk_out"].double()).sum()
+
+    f(*leaves).backward()
+    g = torch.Generator(device="cuda").manual_seed(5)
+    for i, leaf in enumerate(leaves):
+        u = torch.randn(leaf.shape, generator=g, device="cuda")
+        step = 1e-2
+        ends = []
+        for sign in (1, -1):
+            at = [x.detach() for x in leaves]
+            at[i] = at[i] + sign * step * u
+            ends.append(f(*at).item())
+        want = (leaf.grad.double() * u.double()).sum().item()
+        # third derivatives times step^2 / 6, and rounding 1e-5 / step
+        assert abs((ends[0] - ends[1]) / (2 * step) - want) < 5e-3 * (1 + abs(want))
+
+
+@pytest.mark.gpu
+def test_same_bits_captured_and_on_another_stream(gpu):
+    import torch
+    from vector_cuda import ops
+    s = _make(700, 8, 2, 128, "bfloat16", "bfloat16")
+    rest = (s["q"], s["k"], s["positions"], s["q_weight"], s["k_weight"])
+
+    def both():
+        return (*ops.qk_norm_rope_forward(*rest), *ops.qk_norm_rope_backward(s["dq_out"], s["dk_out"], *rest))
+
+    want = both()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = both()
+    torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+def test_python_refusals(gpu):
+    import torch
+    from vector_cuda import ops
+    s = _make(5, 2, 1, 16, "float32", "float32")
+    q, k, p, w = s["q"], s["k"], s["positions"], s["q_weight"]
+    bad = [dict(q=q.cpu()), dict(q=q.double()), dict(k=k.half()), dict(k=k[:4]), dict(p=p.int()), dict(p=p[:4]),
+           dict(w=w[:8]), dict(w=w.half()), dict(q=q[..., :15]), dict(q=q[0]), dict(p=p.cpu())]
+    for b in bad:
+        a = {"q": q, "k": k, "p": p, "w": w, **b}
+        with pytest.raises(ValueError):
+            ops.qk_norm_rope(a["q"], a["k"], a["p"], a["w"])
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope_backward(s["dq_out"][:4], s["dk_out"], q, k, p)
+    with pytest.raises(Exception):
+        ops.qk_norm_rope(q, k, p, rotary_dim=17)
+    with pytest.raises(Exception):
+        ops.qk_norm_rope(q, k, p, rotary_dim=18)
+
+
+def test_c_refusals(vc):
+    """Wrong arguments are told by status before anything is queued (no GPU needed)."""
+    L = vc.lib()
+
+    class Heads(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("stride", ctypes.c_int64), ("head", ctypes.c_int64)]
+
+    h = ctypes.byref(Heads(256, 64, 32))
+    none = ctypes.byref(Heads(None, 64, 32))
+    d_, f_ = ctypes.c_double, ctypes.c_float
+
+    def call(q=h, heads=2, k=h, kv=2, tokens=3, d=32, dtype=1, pos=256, pt=1, base=1e4, rotary=32, eps=1e-6, qo=256):
+        return L.vrs_qk_norm_rope_forward(q, ctypes.c_int64(heads), k, ctypes.c_int64(kv), ctypes.c_int64(tokens),
+                                          ctypes.c_int64(d), dtype, ctypes.c_void_p(pos), None, None, pt, d_(base),
+                                          ctypes.c_int64(rotary), 0, f_(eps), ctypes.c_void_p(qo), ctypes.c_void_p(256), None)
+
+    for bad in (dict(dtype=3), dict(dtype=0, pt=1), dict(d=31), dict(d=258), dict(rotary=34), dict(rotary=7), dict(heads=0),
+                dict(kv=-1), dict(tokens=-1), dict(base=0.0), dict(base=math.inf), dict(base=math.nan), dict(eps=-1.0),
+                dict(eps=math.nan), dict(q=None), dict(q=none), dict(k=none), dict(pos=None), dict(qo=None)):
+        assert call(**bad) == 5, bad
+    assert call(tokens=0) == 0
+    n = ctypes.c_int64(0)
+    assert L.vrs_qk_norm_rope_backward_workspace(ctypes.c_int64(-1), ctypes.c_int64(64), ctypes.byref(n)) == 5
+    assert L.vrs_qk_norm_rope_backward_workspace(ctypes.c_int64(5), ctypes.c_int64(64), ctypes.byref(n)) == 0
+    a = n.value
+    assert L.vrs_qk_norm_rope_backward_workspace(ctypes.c_int64(5000), ctypes.c_int64(128), ctypes.byref(n)) == 0
+    assert n.value >= a > 0

@@ -13,9 +13,12 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <optional>
 #include <sstream>
 #include <string>
+#include <utility>
+#include <vector>
 
 #include "vrs.h"
 
@@ -28,6 +31,12 @@ struct Bound {
   decltype(&vrs_linear_cross_entropy_forward) loss_forward;
   decltype(&vrs_linear_cross_entropy_backward_with_loss) loss_backward;
   decltype(&vrs_linear_cross_entropy_workspace) loss_workspace;
+  decltype(&vrs_qk_norm_rope_forward) rope_forward;
+  decltype(&vrs_qk_norm_rope_backward) rope_backward;
+  decltype(&vrs_qk_norm_rope_backward_workspace) rope_workspace;
+  decltype(&vrs_grad_norm) grad_norm;
+  decltype(&vrs_clip_grad_norm) clip_norm;
+  decltype(&vrs_grad_norm_workspace) clip_workspace;
   PyObject* check;  // raises CudaError for a status
 } g{};
 
@@ -302,6 +311,244 @@ PyObject* linear_cross_entropy_backward(PyObject* const* args) {
   return to_tuple({dx, dtable});
 }
 
+// A tensor as tokens x heads x d over its leading dimensions. Tokens that are
+// evenly spaced and heads whose elements are contiguous are used where they
+// are, others are copied.
+struct HeadRows {
+  at::Tensor t;  // tokens x heads x d
+  int64_t tokens, n, d;
+  vrs_heads h;
+};
+
+HeadRows heads_of(const at::Tensor& in, const char* name, bool half_only = false) {
+  if (!in.is_cuda()) bad(name, " must be a CUDA tensor (there is no CPU fallback)");
+  const auto type = in.scalar_type();
+  if (in.dim() < 3) bad(name, " must be tokens x heads x d, got ", in.sizes());
+  if (half_only ? type != at::kHalf && type != at::kBFloat16
+                : type != at::kFloat && type != at::kHalf && type != at::kBFloat16)
+    bad(name, half_only ? " must be float16 or bfloat16 (operands of the tensor cores), got "
+                        : " must be float32, float16 or bfloat16, got ", name_of(type));
+  HeadRows r;
+  r.n = in.size(-2);
+  r.d = in.size(-1);
+  if (r.n < 1 || r.d < 1) bad(name, " has no heads or no elements: ", in.sizes());
+  r.t = in.dim() == 3 ? in : in.reshape({in.numel() / (r.n * r.d), r.n, r.d});
+  r.tokens = r.t.size(0);
+  if ((r.d > 1 && r.t.stride(2) != 1) || (r.n > 1 && r.t.stride(1) < r.d) || (r.tokens > 1 && r.t.stride(0) < r.d))
+    r.t = r.t.contiguous();
+  r.h = {r.t.data_ptr(), r.t.stride(0), r.t.stride(1)};
+  return r;
+}
+
+// `in` shaped like `like`, of its type and device.
+void check_like(const at::Tensor& in, const at::Tensor& like, const char* name, const char* what) {
+  if (in.sizes() != like.sizes() || in.scalar_type() != like.scalar_type() || in.device() != like.device())
+    bad(name, " must be like ", what, " (", like.sizes(), ", ", name_of(like.scalar_type()), " on ",
+        like.device().str(), "), got ", in.sizes(), ", ", name_of(in.scalar_type()), " on ", in.device().str());
+}
+
+int64_t int_arg(PyObject* o, const char* name) {
+  const long long v = PyLong_AsLongLong(o);
+  if (v == -1 && PyErr_Occurred()) {
+    PyErr_Clear();
+    bad(name, " must be an integer");
+  }
+  return v;
+}
+
+struct RopeArgs {
+  HeadRows q, k;
+  at::Tensor positions;
+  std::optional<at::Tensor> qw, kw;
+  at::ScalarType pt;
+  double base;
+  int64_t rotary;
+  bool interleaved;
+  float eps;
+};
+
+// (q, k, positions, q_weight, k_weight, base, rotary or None, interleaved, eps)
+RopeArgs rope_args(PyObject* const* args) {
+  RopeArgs a;
+  const at::Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"),
+                   &positions = tensor_arg(args[2], "positions");
+  a.q = heads_of(q, "q");
+  a.k = heads_of(k, "k");
+  if (a.k.d != a.q.d || a.k.t.scalar_type() != a.q.t.scalar_type() || a.k.t.device() != a.q.t.device() ||
+      q.sizes().slice(0, q.dim() - 2) != k.sizes().slice(0, k.dim() - 2))
+    bad("k must be like q but for its heads (", q.sizes(), ", ", name_of(q.scalar_type()), "), got ", k.sizes(), ", ",
+        name_of(k.scalar_type()));
+  if (positions.sizes() != q.sizes().slice(0, q.dim() - 2))
+    bad("positions have shape ", positions.sizes(), ", expected ", q.sizes().slice(0, q.dim() - 2));
+  a.positions = beside(positions, a.q.t, "positions", a.q.tokens, at::kLong);
+  a.qw = optional_arg(args[3], "q_weight");
+  a.kw = optional_arg(args[4], "k_weight");
+  a.pt = a.q.t.scalar_type();
+  std::pair<const char*, std::optional<at::Tensor>*> both[] = {{"q_weight", &a.qw}, {"k_weight", &a.kw}};
+  for (auto& [name, p] : both)
+    if (*p) {
+      const auto t = (*p)->scalar_type();
+      if (t != a.q.t.scalar_type() && t != at::kFloat)
+        bad(name, " must be ", name_of(a.q.t.scalar_type()), " or torch.float32, got ", name_of(t));
+      a.pt = t;
+    }
+  for (auto& [name, p] : both)
+    if (*p) *p = beside(**p, a.q.t, name, a.q.d, a.pt);
+  a.base = float_arg(args[5]);
+  a.rotary = args[6] == Py_None ? a.q.d : int_arg(args[6], "rotary_dim");
+  a.interleaved = bool_arg(args[7]);
+  a.eps = (float)float_arg(args[8]);
+  return a;
+}
+
+// (q, k, positions, q_weight, k_weight, base, rotary, interleaved, eps) -> (q_out, k_out)
+PyObject* qk_norm_rope_forward(PyObject* const* args) {
+  const RopeArgs a = rope_args(args);
+  at::Tensor qo = at::empty(THPVariable_Unpack(args[0]).sizes(), a.q.t.options());
+  at::Tensor ko = at::empty(THPVariable_Unpack(args[1]).sizes(), a.q.t.options());
+  const c10::cuda::CUDAGuard guard(a.q.t.device());
+  void* stream = c10::cuda::getCurrentCUDAStream(a.q.t.get_device()).stream();
+  check_status(unlocked([&] {
+    return g.rope_forward(&a.q.h, a.q.n, &a.k.h, a.k.n, a.q.tokens, a.q.d, code_of(a.q.t.scalar_type()),
+                          (const int64_t*)a.positions.data_ptr(), ptr(a.qw), ptr(a.kw), code_of(a.pt), a.base, a.rotary,
+                          a.interleaved, a.eps, qo.data_ptr(), ko.data_ptr(), stream);
+  }));
+  return to_tuple({qo, ko});
+}
+
+// (dq_out, dk_out, then as forward) -> (dq, dk, dq_weight, dk_weight)
+PyObject* qk_norm_rope_backward(PyObject* const* args) {
+  const RopeArgs a = rope_args(args + 2);
+  const at::Tensor &dqo = tensor_arg(args[0], "dq_out"), &dko = tensor_arg(args[1], "dk_out");
+  const at::Tensor &q = THPVariable_Unpack(args[2]), &k = THPVariable_Unpack(args[3]);
+  check_like(dqo, q, "dq_out", "q");
+  check_like(dko, k, "dk_out", "k");
+  const HeadRows gq = heads_of(dqo, "dq_out"), gk = heads_of(dko, "dk_out");
+  at::Tensor dq = at::empty(q.sizes(), a.q.t.options()), dk = at::empty(k.sizes(), a.q.t.options());
+  const c10::cuda::CUDAGuard guard(a.q.t.device());
+  std::optional<at::Tensor> dqw, dkw, ws;
+  int64_t need = 0;
+  if (a.qw || a.kw) {
+    check_status(g.rope_workspace(a.q.tokens, a.q.d, &need));
+    if (a.qw) dqw = at::empty({a.q.d}, a.q.t.options().dtype(a.pt));
+    if (a.kw) dkw = at::empty({a.q.d}, a.q.t.options().dtype(a.pt));
+    ws = at::empty({need}, a.q.t.options().dtype(at::kByte));
+  }
+  void* stream = c10::cuda::getCurrentCUDAStream(a.q.t.get_device()).stream();
+  check_status(unlocked([&] {
+    return g.rope_backward(&gq.h, &gk.h, &a.q.h, a.q.n, &a.k.h, a.k.n, a.q.tokens, a.q.d, code_of(a.q.t.scalar_type()),
+                           (const int64_t*)a.positions.data_ptr(), ptr(a.qw), ptr(a.kw), code_of(a.pt), a.base, a.rotary,
+                           a.interleaved, a.eps, dq.data_ptr(), dk.data_ptr(), ptr(dqw), ptr(dkw), ptr(ws), need, stream);
+  }));
+  return to_tuple({dq, dk, dqw, dkw});
+}
+
+// (gradients, results or None (in place), max_norm or None (the norm alone),
+// unscale) -> norm
+PyObject* clip_grad_norm(PyObject* const* args) {
+  struct List {  // a sequence of tensors, held
+    PyObject* o;
+    explicit List(PyObject* in, const char* name) : o(PySequence_Fast(in, "")) {
+      if (o) return;
+      PyErr_Clear();
+      bad(name, " must be a sequence of tensors");
+    }
+    ~List() { Py_XDECREF(o); }
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(o); }
+    PyObject* at(Py_ssize_t i) const { return PySequence_Fast_GET_ITEM(o, i); }
+  };
+  const List grads(args[0], "grads");
+  const bool clip = args[2] != Py_None, in_place = args[1] == Py_None;
+  std::optional<List> results;
+  if (clip && !in_place) {
+    results.emplace(args[1], "out");
+    if (results->size() != grads.size()) bad("out holds ", results->size(), " tensors, expected ", grads.size());
+  }
+  const double max_norm = clip ? float_arg(args[2]) : 0.0, unscale = float_arg(args[3]);
+  if (clip && !(max_norm >= 0.0)) bad("max_norm must be at least 0, got ", max_norm);
+  if (!(unscale > 0.0) || !((float)unscale > 0.0f) || !((float)unscale < INFINITY))
+    bad("unscale must be positive and finite, got ", unscale);
+  if (grads.size() < 1) bad("grads holds no tensors");
+  std::vector<vrs_grad> list;
+  std::vector<at::Tensor> kept, changed;                    // copies of what has gaps; results
+  std::vector<std::pair<at::Tensor, at::Tensor>> back;      // results to copy back
+  std::vector<std::pair<uintptr_t, uintptr_t>> written;
+  std::optional<at::Tensor> first;
+  for (Py_ssize_t i = 0; i < grads.size(); i++) {
+    at::Tensor t = tensor_arg(grads.at(i), "every gradient");
+    const auto type = t.scalar_type();
+    if (!t.is_cuda()) bad("gradient ", i, " must be a CUDA tensor (there is no CPU fallback)");
+    if (type != at::kFloat && type != at::kHalf && type != at::kBFloat16)
+      bad("gradient ", i, " must be float32, float16 or bfloat16, got ", name_of(type));
+    if (!first) first = t;
+    if (t.device() != first->device()) bad("gradient ", i, " is on ", t.device().str(), ", expected ", first->device().str());
+    vrs_grad e{};
+    e.count = t.numel();
+    e.dtype = e.out_dtype = code_of(type);
+    if (!clip) {
+      if (!t.is_non_overlapping_and_dense()) kept.push_back(t = t.contiguous());
+    } else {
+      at::Tensor o = in_place ? t : tensor_arg(results->at(i), "every result");
+      if (!in_place) {
+        const auto ot = o.scalar_type();
+        if (o.sizes() != t.sizes() || o.device() != t.device() || (ot != type && ot != at::kFloat))
+          bad("result ", i, " must be ", t.sizes(), ", ", name_of(type), " or torch.float32 on ", t.device().str(),
+              ", got ", o.sizes(), ", ", name_of(ot), " on ", o.device().str());
+        e.out_dtype = code_of(ot);
+      }
+      changed.push_back(o);
+      if (!o.is_non_overlapping_and_dense()) {
+        // Elements with gaps between them: through a copy. Elements that share
+        // memory cannot each hold a result.
+        for (int64_t d = 0; d < o.dim(); d++)
+          if (o.size(d) > 1 && o.stride(d) == 0) bad(in_place ? "gradient " : "result ", i, " is expanded: its elements share memory");
+        at::Tensor c = in_place ? o.contiguous() : at::empty(o.sizes(), o.options());
+        back.emplace_back(o, c);
+        o = c;
+        if (in_place) t = c;
+      }
+      // One order of the elements for both sides.
+      if (!in_place && (!t.is_non_overlapping_and_dense() || t.strides() != o.strides())) {
+        at::Tensor c = at::empty_strided(t.sizes(), o.strides(), t.options());
+        c.copy_(t);
+        kept.push_back(t = c);
+      }
+      e.out = o.data_ptr();
+      if (e.count) written.emplace_back((uintptr_t)e.out, (uintptr_t)e.out + e.count * o.element_size());
+    }
+    e.grad = t.data_ptr();
+    list.push_back(e);
+  }
+  // Two results in one place, or a result over another tensor's gradient.
+  std::sort(written.begin(), written.end());
+  for (size_t i = 1; i < written.size(); i++)
+    if (written[i].first < written[i - 1].second) bad("two results share memory");
+  if (!in_place)
+    for (const auto& e : list) {
+      if (!clip || !e.count || e.grad == e.out) continue;
+      const uintptr_t from = (uintptr_t)e.grad, to = from + e.count * (e.dtype == VRS_F32 ? 4 : 2);
+      auto it = std::upper_bound(written.begin(), written.end(), std::make_pair(from, UINTPTR_MAX));
+      if ((it != written.end() && it->first < to) || (it != written.begin() && std::prev(it)->second > from))
+        bad("a result shares memory with a gradient");
+    }
+  const c10::cuda::CUDAGuard guard(first->device());
+  int64_t need = 0;
+  check_status(g.clip_workspace((int64_t)list.size(), &need));
+  const auto options = first->options();
+  at::Tensor norm = at::empty({}, options.dtype(at::kFloat)), ws = at::empty({need}, options.dtype(at::kByte));
+  void* stream = c10::cuda::getCurrentCUDAStream(first->get_device()).stream();
+  check_status(unlocked([&] {
+    return clip ? g.clip_norm(list.data(), (int64_t)list.size(), (float)max_norm, (float)unscale, (float*)norm.data_ptr(),
+                              ws.data_ptr(), need, stream)
+                : g.grad_norm(list.data(), (int64_t)list.size(), (float)unscale, (float*)norm.data_ptr(), ws.data_ptr(),
+                              need, stream);
+  }));
+  for (auto& [to, from] : back) to.copy_(from);
+  for (auto& t : changed)  // autograd notices that a saved tensor was written
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  return THPVariable_Wrap(norm);
+}
+
 // Every call: the argument count, no autograd inside, C++ errors as Python's.
 template <PyObject* (*F)(PyObject* const*), int N>
 PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
@@ -326,14 +573,15 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// bind(addresses of the six entry points in the order of Bound, check)
+// bind(addresses of the entry points in the order of Bound, check)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  if (n != 7) {
-    PyErr_SetString(PyExc_TypeError, "bind takes six addresses and a function");
+  constexpr int N = 12;
+  if (n != N + 1) {
+    PyErr_Format(PyExc_TypeError, "bind takes %d addresses and a function", N);
     return nullptr;
   }
-  void* at[6];
-  for (int i = 0; i < 6; i++) {
+  void* at[N];
+  for (int i = 0; i < N; i++) {
     at[i] = PyLong_AsVoidPtr(args[i]);
     if (!at[i]) {
       if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "null address");
@@ -346,9 +594,15 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g.loss_forward = (decltype(g.loss_forward))at[3];
   g.loss_backward = (decltype(g.loss_backward))at[4];
   g.loss_workspace = (decltype(g.loss_workspace))at[5];
-  Py_INCREF(args[6]);
+  g.rope_forward = (decltype(g.rope_forward))at[6];
+  g.rope_backward = (decltype(g.rope_backward))at[7];
+  g.rope_workspace = (decltype(g.rope_workspace))at[8];
+  g.grad_norm = (decltype(g.grad_norm))at[9];
+  g.clip_norm = (decltype(g.clip_norm))at[10];
+  g.clip_workspace = (decltype(g.clip_workspace))at[11];
+  Py_INCREF(args[N]);
   Py_XDECREF(g.check);
-  g.check = args[6];
+  g.check = args[N];
   Py_RETURN_NONE;
 }
 
@@ -360,6 +614,9 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, 
                          VRS_METHOD(layer_norm_backward, 7),
                          VRS_METHOD(linear_cross_entropy_forward, 4),
                          VRS_METHOD(linear_cross_entropy_backward, 9),
+                         VRS_METHOD(qk_norm_rope_forward, 9),
+                         VRS_METHOD(qk_norm_rope_backward, 11),
+                         VRS_METHOD(clip_grad_norm, 4),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

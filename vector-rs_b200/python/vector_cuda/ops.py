@@ -14,7 +14,7 @@ and returns without waiting. There is no CPU fallback.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional, Tuple
+from typing import Optional, Sequence, Tuple
 
 import torch
 
@@ -31,7 +31,8 @@ def _bind():
     L = lib()
     names = ("layer_norm_forward", "layer_norm_backward", "layer_norm_backward_workspace",
              "linear_cross_entropy_forward", "linear_cross_entropy_backward_with_loss",
-             "linear_cross_entropy_workspace")
+             "linear_cross_entropy_workspace", "qk_norm_rope_forward", "qk_norm_rope_backward",
+             "qk_norm_rope_backward_workspace", "grad_norm", "clip_grad_norm", "grad_norm_workspace")
     _ops.bind(*(ctypes.cast(getattr(L, "vrs_" + n), ctypes.c_void_p).value for n in names), _check)
 
 
@@ -150,5 +151,75 @@ def linear_cross_entropy(x: torch.Tensor, table: torch.Tensor, targets: torch.Te
     return total / taken.clamp(min=1)
 
 
+# --------------------------------------- norms and rotation of heads
+
+
+def qk_norm_rope_forward(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor,
+                         q_weight: Optional[torch.Tensor] = None, k_weight: Optional[torch.Tensor] = None,
+                         base: float = 10000.0, rotary_dim: Optional[int] = None, interleaved: bool = False,
+                         eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(q, k) normed and rotated: see qk_norm_rope."""
+    return _ops.qk_norm_rope_forward(q, k, positions, q_weight, k_weight, base, rotary_dim, interleaved, eps)
+
+
+def qk_norm_rope_backward(dq_out: torch.Tensor, dk_out: torch.Tensor, q: torch.Tensor, k: torch.Tensor,
+                          positions: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                          k_weight: Optional[torch.Tensor] = None, base: float = 10000.0,
+                          rotary_dim: Optional[int] = None, interleaved: bool = False, eps: float = 1e-6):
+    """(dq, dk, dq_weight, dk_weight) from the gradients of both results and the
+    forward pass's arguments; None for a weight that there is not."""
+    return _ops.qk_norm_rope_backward(dq_out, dk_out, q, k, positions, q_weight, k_weight, base, rotary_dim,
+                                      interleaved, eps)
+
+
+class _QkNormRope(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, positions, q_weight, k_weight, base, rotary_dim, interleaved, eps):
+        ctx.save_for_backward(q, k, positions, q_weight, k_weight)
+        ctx.rest = (base, rotary_dim, interleaved, eps)
+        return qk_norm_rope_forward(q, k, positions, q_weight, k_weight, *ctx.rest)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dq_out, dk_out):
+        q, k, positions, q_weight, k_weight = ctx.saved_tensors
+        dq, dk, dqw, dkw = qk_norm_rope_backward(dq_out, dk_out, q, k, positions, q_weight, k_weight, *ctx.rest)
+        return (dq, dk, None, None if dqw is None else dqw.view(q_weight.shape),
+                None if dkw is None else dkw.view(k_weight.shape), None, None, None, None)
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_weight: Optional[torch.Tensor] = None,
+                 k_weight: Optional[torch.Tensor] = None, base: float = 10000.0, rotary_dim: Optional[int] = None,
+                 interleaved: bool = False, eps: float = 1e-6) -> Tuple[torch.Tensor, torch.Tensor]:
+    """The RMS norm of every head's query and key, x / sqrt(mean x^2 + eps) *
+    weight, then the rotation to its position. q is ... x heads x d, k ... x
+    kv_heads x d (d even, at most 256), positions int64 of the leading shape;
+    weights hold d values in q's type or float32, both alike. Of the first
+    rotary_dim elements (all by default) pair i turns by position * base^(-2 i /
+    rotary_dim): elements i and i + rotary_dim / 2, or neighbours where
+    interleaved."""
+    return _QkNormRope.apply(q, k, positions, q_weight, k_weight, base, rotary_dim, interleaved, eps)
+
+
+# ------------------------------------------------------ norm of gradients
+
+
+def grad_norm(grads: Sequence[torch.Tensor], unscale: float = 1.0) -> torch.Tensor:
+    """unscale * sqrt(sum of all squares) over a list of tensors, float32 on
+    their device. Tensors may differ in type and shape."""
+    return _ops.clip_grad_norm(grads, None, None, unscale)
+
+
+def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional[Sequence[torch.Tensor]] = None,
+                   unscale: float = 1.0) -> torch.Tensor:
+    """Multiplies all gradients by unscale * min(1, max_norm / (norm + 1e-6)),
+    in place or into out (tensors of the same shapes, in the gradients' types
+    or float32), and returns the norm: unscale * sqrt(sum of all squares).
+    unscale is the inverse of a loss scale. Nothing waits for the device; a norm
+    that is infinite gives zeros and NaN, one that is NaN gives NaN."""
+    return _ops.clip_grad_norm(grads, out, max_norm, unscale)
+
+
 __all__ = ["check", "layer_norm", "layer_norm_forward", "layer_norm_backward", "linear_cross_entropy",
-           "linear_cross_entropy_forward", "linear_cross_entropy_backward"]
+           "linear_cross_entropy_forward", "linear_cross_entropy_backward", "qk_norm_rope", "qk_norm_rope_forward",
+           "qk_norm_rope_backward", "grad_norm", "clip_grad_norm"]
