@@ -397,6 +397,25 @@ typedef struct vrs_heads {
   int64_t stride, head_stride;
 } vrs_heads;
 
+/* Attention over packed sequences: out_i = sum_j e^(scale q_i . k_j - lse_i) v_j
+ * over the keys j of i's sequence (causal: j <= i), lse_i = log of the sum of the
+ * e^(scale q_i . k_j). heads is a multiple of kv_heads: query head h reads key head
+ * h / (heads / kv_heads). All in VRS_F16 or VRS_BF16 (operands of the tensor cores;
+ * sums are f32, lse is f32[heads][tokens]), d a multiple of 8 up to 128; arrays
+ * start on 16 bytes with strides that are multiples of 8. Sequence b is
+ * tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (device memory, sequences + 1
+ * values that do not fall; other values give results without meaning and reach
+ * no other memory); cu_seqlens NULL: `sequences` of equal length. A token that no
+ * sequence holds (behind the last one, say) has out 0 and lse -inf. What a row does
+ * not see has no effect on it, infinities and NaN included. The weights e^(...) are
+ * rounded to 16 bits for the product with v. The workspace (256-byte aligned) is
+ * needed with cu_seqlens only. */
+VRS_API int vrs_attention_forward_workspace(int64_t tokens, int64_t* out_bytes);
+VRS_API int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const vrs_heads* v, int64_t tokens,
+                                  int64_t heads, int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,
+                                  int64_t sequences, int32_t causal, float scale, const vrs_heads* out, float* lse,
+                                  void* workspace, int64_t workspace_bytes, void* cuda_stream);
+
 /* The RMS norm of each head's query and key (x / sqrt(mean x^2 + eps) * weight),
  * then the rotation to its position of the first `rotary` elements (even, 0..d):
  * pair i turns by position * base^(-2 i / rotary), pairs being elements i and

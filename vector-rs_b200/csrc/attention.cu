@@ -1,0 +1,188 @@
+// attention.cu -- the plan of an attention call: checks, tensor maps, each
+// token's sequence, and the launches of attention_fwd.cu and attention_bwd.cu.
+#include <algorithm>
+#include <cmath>
+
+#include "attention.cuh"
+
+namespace vrs {
+namespace ops {
+namespace {
+
+int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
+
+// Each token's sequence [first, past its last): the last bound at or below the
+// token, by bisection. Whatever cu holds, the interval contains the token and
+// lies within 0..tokens.
+__global__ void __launch_bounds__(256) attention_sequences_kernel(const int* cu, int sequences, int tokens, int2* seg) {
+  grid_launch();
+  grid_wait();
+  const int t = blockIdx.x * 256 + threadIdx.x;
+  if (t >= tokens) return;
+  int lo = 0, hi = sequences;
+  if (sequences < 1 || cu[0] > t || cu[sequences] <= t) {
+    seg[t] = make_int2(0, 0);
+    return;
+  }
+  while (hi - lo > 1) {  // cu[lo] <= t < cu[hi]
+    const int mid = (lo + hi) >> 1;
+    if (cu[mid] <= t)
+      lo = mid;
+    else
+      hi = mid;
+  }
+  seg[t] = make_int2(max(cu[lo], 0), min(cu[hi], tokens));
+}
+
+// d, heads and tokens as a 3-D map of 64 x 1 x `rows`, the smaller stride first.
+int make_map(CUtensorMap* m, bool f16, const vrs_heads& h, int64_t tokens, int64_t heads, int64_t d, int rows,
+             int* tokens_last) {
+  auto fn = tensor_map_encoder();
+  if (!fn) {
+    set_error(VRS_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
+    return VRS_ERR_DRIVER;
+  }
+  // (The stride of a dimension of one is never used.)
+  const int64_t sh = heads > 1 ? h.head_stride : up(d, 8), st = tokens > 1 ? h.stride : up(std::max(d, sh * heads), 8);
+  const bool last = st >= sh;
+  *tokens_last = last;
+  const cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)(last ? heads : tokens), (cuuint64_t)(last ? tokens : heads)};
+  const cuuint64_t strides[2] = {(cuuint64_t)(last ? sh : st) * 2, (cuuint64_t)(last ? st : sh) * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)(last ? 1 : rows), (cuuint32_t)(last ? rows : 1)};
+  const cuuint32_t one[3] = {1, 1, 1};
+  const CUresult r = fn(m, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, h.data, dims,
+                        strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    set_error(VRS_ERR_DRIVER, "attention: cuTensorMapEncodeTiled failed: " + std::to_string((int)r));
+    return VRS_ERR_DRIVER;
+  }
+  return VRS_OK;
+}
+
+struct Call {
+  int64_t tokens, heads, kv_heads, d;
+  int32_t dtype;
+  const int32_t* cu;
+  int64_t sequences;
+  int32_t causal;
+  float scale;
+};
+
+int check(const std::string& w, const Call& c) {
+  if (c.dtype != VRS_F16 && c.dtype != VRS_BF16)
+    return invalid(w + ": dtype must be f16 or bf16 (operands of the tensor cores)");
+  if (c.d < 8 || c.d > 128 || c.d % 8) return invalid(w + ": d must be a multiple of 8 in 8..128");
+  if (c.kv_heads < 1 || c.heads < 1 || c.heads > 65536 || c.heads % c.kv_heads)
+    return invalid(w + ": heads must be a multiple of kv_heads, both at least 1");
+  if (c.tokens < 0 || c.tokens > (1ll << 31) - 512) return invalid(w + ": tokens must be in 0..2^31 - 512");
+  if (c.heads * (c.tokens / kAttTile + 1) > (1ll << 30)) return invalid(w + ": heads x tokens must be below 2^37");
+  if (!(c.scale > 0.0f) || !(c.scale < INFINITY)) return invalid(w + ": scale must be positive and finite");
+  if (c.sequences < 0 || c.sequences > (1ll << 31) - 512) return invalid(w + ": sequences must be in 0..2^31 - 512");
+  if (c.tokens && !c.cu && (c.sequences < 1 || c.tokens % c.sequences))
+    return invalid(w + ": without cu_seqlens, tokens must divide into sequences");
+  return VRS_OK;
+}
+
+// One array that TMA reads or writes.
+int check_heads(const std::string& w, const char* name, const vrs_heads* h, int64_t tokens, int64_t heads, int64_t d) {
+  if (!h || !h->data) return invalid(w + ": null " + name);
+  if ((uintptr_t)h->data % 16 || (tokens > 1 && h->stride % 8) || (heads > 1 && h->head_stride % 8))
+    return invalid(w + ": " + name + " must start on 16 bytes with strides that are multiples of 8");
+  if ((tokens > 1 && (h->stride < d || h->stride >= 1ll << 38)) || (heads > 1 && (h->head_stride < d || h->head_stride >= 1ll << 38)))
+    return invalid(w + ": strides of " + name + " must be at least d and below 2^38");
+  return VRS_OK;
+}
+
+// What the passes share; cu_seqlens become a token's sequence in the workspace.
+int start(const Call& c, void* seg, AttArgs& a, cudaStream_t s) {
+  a.tokens = (int)c.tokens;
+  a.heads = (int)c.heads;
+  a.kv_heads = (int)c.kv_heads;
+  a.group = (int)(c.heads / c.kv_heads);
+  a.d = (int)c.d;
+  a.tiles = (int)((c.tokens + kAttTile - 1) / kAttTile);
+  a.causal = c.causal != 0;
+  a.scale = c.scale;
+  a.c2 = c.scale * 1.44269504088896341f;
+  a.seq_len = c.cu ? 0 : (int)(c.tokens / c.sequences);
+  a.seg = nullptr;
+  VRS_TRY(error_word(&a.err));
+  if (!c.cu) return VRS_OK;
+  a.seg = (const int2*)seg;
+  VRS_TRY(launch_after(attention_sequences_kernel, (unsigned)((c.tokens + 255) / 256), 256, 0, s, (const int*)c.cu,
+                       (int)c.sequences, (int)c.tokens, (int2*)seg));
+  count_launch();
+  return VRS_OK;
+}
+
+int check_workspace(const std::string& w, const void* ws, int64_t have, int64_t need) {
+  if (need && (!ws || (uintptr_t)ws % 256 || have < need)) return invalid(w + ": workspace missing, off 256 bytes or too small");
+  return VRS_OK;
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace vrs
+
+extern "C" int vrs_attention_forward_workspace(int64_t tokens, int64_t* out_bytes) {
+  using namespace vrs::ops;
+  if (tokens < 0 || tokens > (1ll << 31) - 512 || !out_bytes)
+    return invalid("vrs_attention_forward_workspace: tokens must be in 0..2^31 - 512, out_bytes not null");
+  *out_bytes = up(tokens * 8, 256);
+  return VRS_OK;
+}
+
+extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const vrs_heads* v, int64_t tokens,
+                                     int64_t heads, int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,
+                                     int64_t sequences, int32_t causal, float scale, const vrs_heads* out, float* lse,
+                                     void* workspace, int64_t workspace_bytes, void* cuda_stream) {
+  using namespace vrs;
+  using namespace vrs::ops;
+  const std::string w = "vrs_attention_forward";
+  const Call c{tokens, heads, kv_heads, d, dtype, cu_seqlens, sequences, causal, scale};
+  VRS_TRY(check(w, c));
+  if (tokens == 0) return VRS_OK;
+  VRS_TRY(check_heads(w, "q", q, tokens, heads, d));
+  VRS_TRY(check_heads(w, "k", k, tokens, kv_heads, d));
+  VRS_TRY(check_heads(w, "v", v, tokens, kv_heads, d));
+  VRS_TRY(check_heads(w, "out", out, tokens, heads, d));
+  if (!lse) return invalid(w + ": null lse");
+  int64_t need = 0;
+  VRS_TRY(vrs_attention_forward_workspace(tokens, &need));
+  if (cu_seqlens) VRS_TRY(check_workspace(w, workspace, workspace_bytes, need));
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  int sms = 0;
+  VRS_TRY(sm_count(&sms));
+  const bool f16 = dtype == VRS_F16;
+  AttFwdMaps maps;
+  AttFwd a{};
+  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, kAttTile, &a.q_last));
+  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, kAttTile, &a.k_last));
+  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, kAttTile, &a.v_last));
+  VRS_TRY(make_map(&maps.out, f16, *out, tokens, heads, d, 32, &a.out_last));
+  ProfToken t = prof_begin("attention_forward", s);
+  int st = start(c, workspace, a, s);
+  if (st == VRS_OK) {
+    a.lse = lse;
+    a.v = (const uint16_t*)v->data;
+    a.vs = v->stride;
+    a.vh = v->head_stride;
+    // Pairs of tiles halve the loads of keys and values; single ones where pairs
+    // would leave SMs without work.
+    const int64_t single = (int64_t)a.tiles * heads;
+    if (single <= sms) {
+      a.pairing = kAttSingle;
+      a.items = (int)single;
+    } else if (a.group % 2 == 0) {
+      a.pairing = kAttTwoHeads;
+      a.items = (int)(single / 2);
+    } else {
+      a.pairing = kAttTwoTiles;
+      a.items = (int)((a.tiles + 1) / 2 * heads);
+    }
+    st = launch_attention_forward(f16, d <= 64 ? 64 : 128, maps, a, sms, s);
+  }
+  prof_end(t, s);
+  return st;
+}

@@ -1,0 +1,337 @@
+// attention.cuh -- what the passes of the attention share: arguments, the rows'
+// intervals of keys, tiles in shared memory, tensor-memory and store wrappers.
+//
+// The token axis is cut into tiles of 128 without regard to the sequences. A
+// query row i sees the keys of an interval [lo, hi) of the same axis (its
+// sequence; causal: up to itself), a key row j the queries of one, and a tile of
+// rows meets the tiles that the union of its rows' intervals touches. So many
+// short sequences share a tile, a long one needs no tiles of its own, and every
+// tile starts where TMA wants it. A pair of tiles that some row does not see
+// whole is masked element by element ("masked" below).
+//
+// Operands of a masked pair of tiles may hold values that are not finite in rows
+// that others do not see; their weight is 0, and 0 times such a value would reach
+// the others through the matrix product. The cleaning warps look such a tile
+// through in shared memory before it is multiplied, set what is not finite to 0
+// and raise a flag; rows of results then add the values that they do see.
+#pragma once
+#include <cuda.h>
+
+#include "ops_common.cuh"
+#include "tc_common.cuh"
+
+namespace vrs {
+namespace ops {
+
+constexpr int kAttTile = 128;                    // tokens of a tile
+constexpr uint32_t kAttBox = 64 * 2 * kAttTile;  // bytes of 64 elements of a tile's rows
+constexpr uint64_t kAttWaitNs = 2000000000ull;
+constexpr int kAttFlags = 16;                    // items that the "not finite" flags tell apart
+
+struct AttArgs {
+  int tokens, heads, kv_heads, group, d, tiles;
+  int causal;
+  int seq_len;        // of every sequence, where seg is null
+  const int2* seg;    // per token: its sequence's first token and the one past its last
+  float c2;           // scale * log2 e
+  float scale;
+  float* lse;         // [heads][tokens]
+  // Values that are not finite are read again from here.
+  const uint16_t *q, *k, *v, *dout;
+  int64_t qs, qh, ks, kh, vs, vh, dos, doh;
+  int* err;
+};
+
+__device__ __forceinline__ float att_ex2(float x) {
+  float r;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(x));
+  return r;
+}
+
+// Rows [lo, hi) that row i meets: the keys of a query (KEYS), or the queries of a
+// key. Empty for a row that no sequence holds. Whatever seg says, within 0..tokens.
+template <bool KEYS>
+__device__ __forceinline__ int2 att_interval(const AttArgs& a, int i) {
+  if (i >= a.tokens) return make_int2(0, 0);
+  int2 r;
+  if (a.seg) {
+    r = a.seg[i];
+  } else {
+    r.x = i / a.seq_len * a.seq_len;
+    r.y = r.x + a.seq_len;
+  }
+  if (a.causal) {
+    if (KEYS)
+      r.y = min(r.y, i + 1);
+    else
+      r.x = max(r.x, i);
+  }
+  return r.x < r.y ? r : make_int2(0, 0);
+}
+
+// What a tile of 128 rows meets; by a whole warp.
+struct AttSpan {
+  int first, end;        // tiles [first, end) with a row that some row here meets
+  int low_max, high_min;  // rows [low_max, high_min) are met by all rows here
+};
+template <bool KEYS>
+__device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
+  const int lane = threadIdx.x & 31;
+  int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
+#pragma unroll
+  for (int r = 0; r < 4; r++) {
+    const int i = tile * kAttTile + r * 32 + lane;
+    const int2 v = att_interval<KEYS>(a, i);
+    if (v.x < v.y) {
+      lo_min = min(lo_min, v.x);
+      lo_max = max(lo_max, v.x);
+      hi_min = min(hi_min, v.y);
+      hi_max = max(hi_max, v.y);
+    } else if (i < a.tokens) {
+      lo_max = INT_MAX;  // a row that meets nothing
+    }
+  }
+  lo_min = __reduce_min_sync(~0u, lo_min);
+  lo_max = __reduce_max_sync(~0u, lo_max);
+  hi_min = __reduce_min_sync(~0u, hi_min);
+  hi_max = __reduce_max_sync(~0u, hi_max);
+  AttSpan s;
+  s.first = hi_max > 0 ? lo_min / kAttTile : 0;
+  s.end = (hi_max + kAttTile - 1) / kAttTile;
+  s.low_max = lo_max;
+  s.high_min = hi_min;
+  return s;
+}
+
+// Whether some row of a span does not meet all of tile t. (The tile's rows past
+// the last token are zeros, and masked.)
+__device__ __forceinline__ bool att_masked(int low_max, int high_min, int t) {
+  return t * kAttTile < low_max || (t + 1) * kAttTile > high_min;
+}
+
+// 3-D tiles: 64 elements of one head of 128 (stored: 32) tokens. tokens_last: the
+// map's dimensions are d, heads, tokens, else d, tokens, heads.
+__device__ __forceinline__ void att_load(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+          tc::smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
+      : "memory");
+}
+__device__ __forceinline__ void att_store(const CUtensorMap* map, const void* src, int x, int y, int z) {
+  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
+                   reinterpret_cast<uint64_t>(map)),
+               "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(src))
+               : "memory");
+}
+__device__ __forceinline__ void att_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+__device__ __forceinline__ void att_store_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void att_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+// A tile of one head: boxes of 64 elements, one after another.
+template <int DP>
+__device__ __forceinline__ void att_load_tile(uint8_t* to, const CUtensorMap* map, int tokens_last, int head, int token,
+                                              uint64_t* bar) {
+#pragma unroll
+  for (int b = 0; b < DP / 64; b++)
+    att_load(to + b * kAttBox, map, b * 64, tokens_last ? head : token, tokens_last ? token : head, bar);
+}
+
+// ---- operand descriptors of a tile (128 tokens x DP): its rows as M or N
+// (K-major, K = the elements), or its elements as N (MN-major, K = the tokens).
+__device__ __forceinline__ uint64_t att_desc_mn(const void* p) {
+  uint64_t d = tc::smem_desc_sw128(p);
+  d &= ~((uint64_t)0x3FFF << 16);
+  d |= (uint64_t)(kAttBox >> 4) << 16;  // the next 64 elements
+  return d;
+}
+// 16 of K further: 32 bytes in a row, the next box every 64; or 16 rows.
+__device__ __forceinline__ uint32_t att_k_step(int k) { return (k >> 2) * (kAttBox >> 4) + (k & 3) * 2; }
+__device__ __forceinline__ uint32_t att_mn_step(int k) { return k * (2048 >> 4); }
+
+// D (+)= A B^T, A in tensor memory: a row a lane, two 16-bit values a column.
+__device__ __forceinline__ void att_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// Instruction descriptor: 16-bit operands of one type, f32 sums, M = 128.
+template <bool F16>
+__host__ __device__ constexpr uint32_t att_idesc(int n, bool b_mn) {
+  return (1u << 4) | (F16 ? 0u : (1u << 7) | (1u << 10)) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) |
+         (128u >> 4 << 24);
+}
+
+// ---- tensor memory: 32 lanes x 32 columns; loaded values may be used only
+// after att_tm_wait, which they pass through.
+__device__ __forceinline__ void att_tm_load(uint32_t taddr, float* v) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+      "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(taddr)
+      : "memory");
+}
+__device__ __forceinline__ void att_tm_wait(float* v) {
+  asm volatile("tcgen05.wait::ld.sync.aligned;"
+               : "+f"(v[0]), "+f"(v[1]), "+f"(v[2]), "+f"(v[3]), "+f"(v[4]), "+f"(v[5]), "+f"(v[6]), "+f"(v[7]),
+                 "+f"(v[8]), "+f"(v[9]), "+f"(v[10]), "+f"(v[11]), "+f"(v[12]), "+f"(v[13]), "+f"(v[14]), "+f"(v[15]),
+                 "+f"(v[16]), "+f"(v[17]), "+f"(v[18]), "+f"(v[19]), "+f"(v[20]), "+f"(v[21]), "+f"(v[22]),
+                 "+f"(v[23]), "+f"(v[24]), "+f"(v[25]), "+f"(v[26]), "+f"(v[27]), "+f"(v[28]), "+f"(v[29]),
+                 "+f"(v[30]), "+f"(v[31])
+               :
+               : "memory");
+}
+__device__ __forceinline__ void att_tm_store(uint32_t taddr, const float* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+      "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+      "f"(v[0]), "f"(v[1]), "f"(v[2]), "f"(v[3]), "f"(v[4]), "f"(v[5]), "f"(v[6]), "f"(v[7]), "f"(v[8]), "f"(v[9]),
+      "f"(v[10]), "f"(v[11]), "f"(v[12]), "f"(v[13]), "f"(v[14]), "f"(v[15]), "f"(v[16]), "f"(v[17]), "f"(v[18]),
+      "f"(v[19]), "f"(v[20]), "f"(v[21]), "f"(v[22]), "f"(v[23]), "f"(v[24]), "f"(v[25]), "f"(v[26]), "f"(v[27]),
+      "f"(v[28]), "f"(v[29]), "f"(v[30]), "f"(v[31])
+      : "memory");
+}
+__device__ __forceinline__ void att_tm_store16(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void att_tm_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <bool F16>
+__device__ __forceinline__ uint32_t att_pack2(float lo, float hi) {
+  uint32_t r;
+  if (F16)
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+
+// ---- values that are not finite: an exponent field of ones. Bits 15 and 31 of
+// the result tell it of both halves (adding one to such a field carries into the
+// sign's place, which the mask left 0).
+template <bool F16>
+__device__ __forceinline__ uint32_t att_not_finite(uint32_t u) {
+  return F16 ? ((u & 0x7c007c00u) + 0x04000400u) & 0x80008000u : ((u & 0x7f807f80u) + 0x00800080u) & 0x80008000u;
+}
+template <bool F16>
+__device__ __forceinline__ uint32_t att_clear(uint32_t u) {
+  const uint32_t bad = att_not_finite<F16>(u);
+  if (bad & 0x8000u) u &= 0xffff0000u;
+  if (bad & 0x80000000u) u &= 0x0000ffffu;
+  return u;
+}
+
+// A warp's share of a tile in shared memory, `part` of `parts`: values that are
+// not finite become 0. Whether there were any. (What the swizzle does within a
+// row is of no concern.)
+template <int DP, bool F16>
+__device__ __forceinline__ bool att_clean(uint8_t* tile, int part, int parts) {
+  const int lane = threadIdx.x & 31;
+  uint4* p = reinterpret_cast<uint4*>(tile);
+  constexpr int kVecs = DP * kAttTile * 2 / 16;
+  uint32_t any = 0;
+#pragma unroll 4
+  for (int i = part * 32 + lane; i < kVecs; i += parts * 32) {
+    const uint4 u = p[i];
+    const uint32_t bad = att_not_finite<F16>(u.x) | att_not_finite<F16>(u.y) | att_not_finite<F16>(u.z) | att_not_finite<F16>(u.w);
+    if (bad) p[i] = make_uint4(att_clear<F16>(u.x), att_clear<F16>(u.y), att_clear<F16>(u.z), att_clear<F16>(u.w));
+    any |= bad;
+  }
+  return __any_sync(~0u, any != 0);
+}
+
+// Adds to 32 results of a row (elements [c0, c0 + 32) of d) the values that are
+// not finite of the rows in [lo, hi) of `m`: what the cleaned tiles left out.
+// (Rows of tiles that were not cleaned have had their effect; once more changes
+// nothing.)
+template <bool F16>
+__device__ __forceinline__ void att_add_not_finite(float* o, const uint16_t* m, int64_t stride, int lo, int hi, int c0,
+                                                   int d) {
+#pragma unroll 1
+  for (int j = lo; j < hi; j++) {
+    const uint4* row = reinterpret_cast<const uint4*>(m + j * stride + c0);
+#pragma unroll
+    for (int q = 0; q < 4; q++) {
+      if (c0 + 8 * q >= d) break;
+      const uint4 u = row[q];
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+      for (int k = 0; k < 4; k++) {
+        const uint32_t bad = att_not_finite<F16>(w[k]);
+        const uint16_t a = (uint16_t)w[k], b = (uint16_t)(w[k] >> 16);
+        if (bad & 0x8000u) o[8 * q + 2 * k] += F16 ? __half2float(__ushort_as_half(a)) : __uint_as_float((uint32_t)a << 16);
+        if (bad & 0x80000000u)
+          o[8 * q + 2 * k + 1] += F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+      }
+    }
+  }
+}
+
+// Row `row` of a staging tile (boxes of 64 elements, 128-byte swizzle): 32
+// results from element c0 on in 16 bits.
+template <bool F16>
+__device__ __forceinline__ void att_stage_row(uint8_t* tile, int row, int c0, const float* w) {
+  uint8_t* to = tile + (c0 >> 6) * kAttBox + row * 128;
+  const int j0 = (c0 & 63) >> 3;
+#pragma unroll
+  for (int q = 0; q < 4; q++)
+    *reinterpret_cast<uint4*>(to + (((j0 + q) ^ (row & 7)) << 4)) =
+        make_uint4(att_pack2<F16>(w[8 * q], w[8 * q + 1]), att_pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
+                   att_pack2<F16>(w[8 * q + 4], w[8 * q + 5]), att_pack2<F16>(w[8 * q + 6], w[8 * q + 7]));
+}
+
+// A warp's 32 rows of a staging tile to memory; the wait is for the reads only.
+template <int DP>
+__device__ __forceinline__ void att_store_rows(const AttArgs& a, const CUtensorMap* map, int tokens_last, uint8_t* tile,
+                                               int row, int head, int token) {
+  att_fence_async();
+  __syncwarp();
+  if ((threadIdx.x & 31) == 0 && token < a.tokens) {
+#pragma unroll
+    for (int b = 0; b < DP / 64; b++)
+      if (b * 64 < a.d)
+        att_store(map, tile + b * kAttBox + row * 128, b * 64, tokens_last ? head : token, tokens_last ? token : head);
+    att_store_commit();
+    att_store_wait();
+  }
+  __syncwarp();
+}
+
+// Set-up that the kernels share: dynamic shared memory on a 1,024-byte boundary.
+__device__ __forceinline__ uint8_t* att_align(uint8_t* p) {
+  return (uint8_t*)(((uintptr_t)p + 1023) & ~(uintptr_t)1023);
+}
+
+// The forward pass's order of work: items of up to two query tiles that share
+// their keys and values' head: two heads of one group (even groups), two
+// neighbouring tiles of one head, or a single tile where items would not fill the
+// device otherwise.
+enum AttPairing { kAttSingle = 0, kAttTwoHeads = 1, kAttTwoTiles = 2 };
+
+struct AttFwdMaps {
+  CUtensorMap q, k, v, out;
+};
+struct AttFwd : AttArgs {
+  int pairing, items;
+  int q_last, k_last, v_last, out_last;  // maps whose last dimension is the tokens
+};
+int launch_attention_forward(bool f16, int dp, const AttFwdMaps& maps, const AttFwd& a, int sms, cudaStream_t s);
+
+}  // namespace ops
+}  // namespace vrs

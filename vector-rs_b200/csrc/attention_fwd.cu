@@ -1,0 +1,476 @@
+// attention_fwd.cu -- attention over packed sequences on tcgen05:
+//   s_ij = scale q_i . k_j over the keys j that row i sees, out_i = sum_j p_ij v_j,
+//   p_ij = e^(s_ij - lse_i), lse_i = log sum_j e^s_ij.
+// One pass over the keys with a running reference m and sum l of the powers of
+// two: p' = 2^(c2 q.k - m), out = (sum p' v) / l, lse = (m + log2 l) ln 2.
+//
+// A CTA takes an item of up to two query tiles (128 rows each) that share the
+// head of their keys, so that each tile of keys and values is loaded once for 256
+// rows. Two groups of four warps, a thread a row, take a tile of scores each from
+// tensor memory, and while one takes exponentials the tensor cores multiply for
+// the other. P goes back to tensor memory in 16 bits, over the scores' columns, as
+// the A operand of the product with V. Because MMAs run in issue order, a tile of
+// scores that has come says that the product before it is complete: the sums in
+// tensor memory may then be scaled without another wait, which happens only when
+// a row's reference has to grow by more than 2^8.
+//
+// Bound for d = 128 by the tensor cores and the exponentials alike: a pair of
+// tiles takes 128 x 128 x 128 x 2 multiply-adds (4,096 an SM and clock: 1,024
+// clocks) and 128 x 128 exponentials (16 an SM and clock: 1,024 clocks).
+#include <atomic>
+
+#include "attention.cuh"
+
+namespace vrs {
+namespace ops {
+namespace {
+
+using namespace vrs::tc;
+
+constexpr int kThreads = 384;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;  // and 11
+constexpr int kColS = 0, kColO = 256;  // of tile 0; tile 1: 128 further
+
+template <int DP>
+constexpr int stages() { return DP == 128 ? 4 : 8; }
+template <int DP>
+constexpr uint32_t tile_bytes() { return DP / 64 * kAttBox; }
+template <int DP>
+constexpr size_t smem_bytes() { return 1024 + (2 + stages<DP>()) * (size_t)tile_bytes<DP>() + 512; }
+static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "above the per-block limit");
+
+// Powers of two kept in 16 bits: f16 ends at 2^16 and loses digits below 2^-14, so
+// its P is 2^7 larger, up to 2^15 where the reference lags by 2^8.
+template <bool F16>
+constexpr float kLift = F16 ? 7.0f : 0.0f;
+constexpr float kLag = 8.0f;
+
+struct Item {
+  int tile[2], head[2];
+  bool live[2];
+  int kv;
+};
+
+__device__ __forceinline__ Item item_at(const AttFwd& a, int id) {
+  Item t;
+  t.live[0] = true;
+  if (a.pairing == kAttTwoHeads) {
+    const int pairs = a.heads / 2;
+    t.tile[0] = t.tile[1] = a.tiles - 1 - id / pairs;
+    t.head[0] = id % pairs * 2;
+    t.head[1] = t.head[0] + 1;
+    t.live[1] = true;
+  } else if (a.pairing == kAttTwoTiles) {
+    const int n = (a.tiles + 1) / 2 - 1 - id / a.heads;
+    t.tile[0] = 2 * n;
+    t.tile[1] = 2 * n + 1;
+    t.head[0] = t.head[1] = id % a.heads;
+    t.live[1] = t.tile[1] < a.tiles;
+  } else {
+    t.tile[0] = t.tile[1] = a.tiles - 1 - id / a.heads;
+    t.head[0] = t.head[1] = id % a.heads;
+    t.live[1] = false;
+  }
+  t.kv = t.head[0] / a.group;
+  return t;
+}
+
+// The tiles of keys that an item's tiles meet, and their union.
+struct Range {
+  int first[2], end[2];
+  int t0, t1;
+  int low_max, high_min;
+  __device__ __forceinline__ bool active(int s, int t) const { return t >= first[s] && t < end[s]; }
+};
+__device__ __forceinline__ Range range_of(const AttFwd& a, const Item& it) {
+  Range r;
+  r.t0 = INT_MAX;
+  r.t1 = 0;
+  r.low_max = 0;
+  r.high_min = INT_MAX;
+#pragma unroll
+  for (int s = 0; s < 2; s++) {
+    r.first[s] = r.end[s] = 0;
+    if (!it.live[s]) continue;
+    if (s == 1 && it.tile[1] == it.tile[0]) {
+      r.first[1] = r.first[0];
+      r.end[1] = r.end[0];
+      continue;
+    }
+    const AttSpan p = att_span<true>(a, it.tile[s]);
+    r.first[s] = p.first;
+    r.end[s] = p.end;
+    if (p.first < p.end) {
+      r.t0 = min(r.t0, p.first);
+      r.t1 = max(r.t1, p.end);
+      r.low_max = max(r.low_max, p.low_max);
+      r.high_min = min(r.high_min, p.high_min);
+    }
+  }
+  if (r.t1 == 0) r.t0 = 0;
+  return r;
+}
+
+template <int DP, bool F16>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_forward_kernel(const __grid_constant__ AttFwdMaps maps, const __grid_constant__ AttFwd a) {
+  constexpr int ST = stages<DP>();
+  constexpr uint32_t TILE = tile_bytes<DP>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = att_align(smem_raw);
+  uint8_t* s_q = smem;              // two tiles; then the results
+  uint8_t* s_kv = smem + 2 * TILE;  // ring of keys and values by turns
+  uint64_t* bars = (uint64_t*)(s_kv + ST * TILE);
+  uint64_t* full = bars;            // [ST] the tile has come
+  uint64_t* empty = full + ST;      // [ST] multiplied, and looked through
+  uint64_t* clean = empty + ST;     // [ST] a masked tile of values is clean
+  uint64_t* q_full = clean + ST;    // [2]
+  uint64_t* q_empty = q_full + 2;   // [2] the results have left
+  uint64_t* s_full = q_empty + 2;   // [2] scores
+  uint64_t* p_full = s_full + 2;    // [2] P in tensor memory
+  uint64_t* o_full = p_full + 2;    // [2] all products
+  uint64_t* drain = o_full + 2;     // of a run that gave up
+  uint32_t* s_tmem = (uint32_t*)(drain + 1);
+  volatile int* s_abort = (volatile int*)(s_tmem + 1);
+  volatile int* s_flag = s_abort + 1;  // [kAttFlags]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 3);
+      mbar_init(&clean[s], 2);
+    }
+    for (int s = 0; s < 2; s++) {
+      mbar_init(&q_full[s], 1);
+      mbar_init(&q_empty[s], 4);
+      mbar_init(&s_full[s], 1);
+      mbar_init(&p_full[s], 128);
+      mbar_init(&o_full[s], 1);
+    }
+    mbar_init(drain, 1);
+    *s_abort = 0;
+    for (int i = 0; i < kAttFlags; i++) s_flag[i] = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 32 * kLoadWarp) {
+    prefetch_tmap(&maps.q);
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+    prefetch_tmap(&maps.out);
+  }
+  if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  grid_launch();
+  grid_wait();
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads
+    int use = 0, q_use[2] = {0, 0};
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Item it = item_at(a, id);
+      const Range r = range_of(a, it);
+      if (lane == 0) {
+        // The first keys and values before the queries: their places in the ring
+        // come free earlier than the queries', which the results leave through.
+        const int i0 = 2 * r.t0, i1 = 2 * r.t1;
+        for (int i = i0; ok && i <= max(i1 - 1, i0 + 2); i++) {
+          if (i == min(i1, i0 + 2)) {
+            for (int s = 0; s < 2 && ok; s++) {
+              if (!it.live[s]) continue;
+              ok = mbar_wait(&q_empty[s], (q_use[s] & 1) ^ 1, s_abort, a.err, 41, kAttWaitNs);
+              if (!ok) break;
+              mbar_expect_tx(&q_full[s], TILE);
+              att_load_tile<DP>(s_q + s * TILE, &maps.q, a.q_last, it.head[s], it.tile[s] * kAttTile, &q_full[s]);
+              q_use[s]++;
+            }
+          }
+          if (!ok || i >= i1) break;
+          const int st = use % ST;
+          ok = mbar_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 42, kAttWaitNs);
+          if (!ok) break;
+          mbar_expect_tx(&full[st], TILE);
+          const bool val = i & 1;
+          att_load_tile<DP>(s_kv + st * TILE, val ? &maps.v : &maps.k, val ? a.v_last : a.k_last, it.kv,
+                            (i >> 1) * kAttTile, &full[st]);
+          use++;
+        }
+      }
+      ok = __shfl_sync(~0u, ok, 0);
+    }
+    if (lane == 0 && *s_abort) {
+      // Drain (bounded) before shared memory goes.
+      volatile int dummy = 0;
+      for (int i = max(0, use - ST); i < use; i++) mbar_wait(&full[i % ST], i / ST & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+      for (int s = 0; s < 2; s++)
+        if (q_use[s]) mbar_wait(&q_full[s], (q_use[s] - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ products
+    const uint64_t qd = smem_desc_sw128(s_q), kd = smem_desc_sw128(s_kv), vd = att_desc_mn(s_kv);
+    constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_o = att_idesc<F16>(DP, true);
+    int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
+    uint32_t cleaned = 0;  // parity of each stage's cleanings
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Item it = item_at(a, id);
+      const Range r = range_of(a, it);
+      if (lane == 0 && r.t0 < r.t1) {
+        auto scores = [&](int s, int st) {
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++)
+            mma_f16(tmem + kColS + s * 128, qd + s * (TILE >> 4) + att_k_step(k), kd + st * (TILE >> 4) + att_k_step(k),
+                    idesc_s, k > 0);
+          mma_commit(&s_full[s]);
+        };
+        for (int s = 0; s < 2 && ok; s++)
+          if (r.first[s] < r.end[s]) ok = mbar_wait(&q_full[s], q_use[s] & 1, s_abort, a.err, 43, kAttWaitNs);
+        // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
+        if (ok) ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 44, kAttWaitNs);
+        if (ok) {
+          tc_fence_after();
+          for (int s = 0; s < 2; s++)
+            if (r.active(s, r.t0)) scores(s, use % ST);
+          mma_commit(&empty[use % ST]);
+        }
+        for (int t = r.t0; ok && t < r.t1; t++) {
+          const int uv = use + 2 * (t - r.t0) + 1, uk = uv + 1, sv = uv % ST, sk = uk % ST;
+          const bool more = t + 1 < r.t1;
+          ok = mbar_wait(&full[sv], uv / ST & 1, s_abort, a.err, 45, kAttWaitNs);
+          if (ok && att_masked(r.low_max, r.high_min, t)) {
+            ok = mbar_wait(&clean[sv], cleaned >> sv & 1, s_abort, a.err, 46, kAttWaitNs);
+            cleaned ^= 1u << sv;
+          }
+          bool keys = false;
+          for (int s = 0; s < 2 && ok; s++) {
+            if (r.active(s, t)) {
+              ok = mbar_wait(&p_full[s], p_use[s] & 1, s_abort, a.err, 47, kAttWaitNs);
+              if (!ok) break;
+              p_use[s]++;
+              tc_fence_after();
+#pragma unroll
+              for (int k = 0; k < kAttTile / 16; k++)
+                att_mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + k * 8, vd + sv * (TILE >> 4) + att_mn_step(k),
+                           idesc_o, t > r.first[s] || k > 0);
+              if (t + 1 == r.end[s]) mma_commit(&o_full[s]);
+            }
+            if (more && r.active(s, t + 1)) {
+              if (!keys) ok = mbar_wait(&full[sk], uk / ST & 1, s_abort, a.err, 48, kAttWaitNs);
+              if (!ok) break;
+              keys = true;
+              tc_fence_after();
+              scores(s, sk);
+            }
+          }
+          if (!ok) break;
+          mma_commit(&empty[sv]);
+          if (more) {
+            if (!keys) ok = mbar_wait(&full[sk], uk / ST & 1, s_abort, a.err, 48, kAttWaitNs);
+            mma_commit(&empty[sk]);
+          }
+        }
+        use += 2 * (r.t1 - r.t0);
+        for (int s = 0; s < 2; s++)
+          if (r.first[s] < r.end[s]) q_use[s]++;
+      }
+      if (lane == 0)
+        for (int s = 0; s < 2; s++)
+          if (it.live[s] && r.first[s] >= r.end[s]) q_use[s]++;
+      ok = __shfl_sync(~0u, ok, 0);
+    }
+    if (lane == 0 && *s_abort) {
+      // MMAs in flight must not outlive the block's tensor memory: one more
+      // commit, waited for (bounded).
+      volatile int dummy = 0;
+      mma_commit(drain);
+      mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
+    }
+  } else if (warp >= kCleanWarp) {
+    // ------------------------------------------------------------ cleaning
+    int use = 0, count = 0;
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Item it = item_at(a, id);
+      const Range r = range_of(a, it);
+      for (int i = 2 * r.t0; ok && i < 2 * r.t1; i++, use++) {
+        const int st = use % ST;
+        // (Keys too are waited for: an arrival before the tile has come could
+        // count for the tile before it.)
+        ok = mbar_wait(&full[st], use / ST & 1, s_abort, a.err, 49, kAttWaitNs);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        if (i & 1) {
+          // A later item's flag: the ring holds at most four tiles of values, so
+          // the other cleaning warp is at most four items ahead, and the item
+          // eight before this one, which had the flag last, has its results.
+          if (i == 2 * r.t0 + 1 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
+          if (att_masked(r.low_max, r.high_min, i >> 1)) {
+            if (att_clean<DP, F16>(s_kv + st * TILE, warp - kCleanWarp, 2) && lane == 0) s_flag[count % kAttFlags] = 1;
+            att_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&clean[st]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+      }
+      if (r.t0 < r.t1) count++;
+    }
+  } else {
+    // ------------------------------------------------------------ softmax
+    const int s = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + lanes + kColS + s * 128, to = tmem + lanes + kColO + s * 128;
+    uint8_t* stage = s_q + s * TILE;
+    int s_use = 0, o_use = 0, q_use = 0, count = 0;
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Item it = item_at(a, id);
+      const Range r = range_of(a, it);
+      if (!it.live[s]) {
+        if (r.t0 < r.t1) count++;
+        continue;
+      }
+      const int i = it.tile[s] * kAttTile + row;
+      const int2 seen = att_interval<true>(a, i);
+      float m = -INFINITY, l = 0.0f;
+      for (int t = r.first[s]; t < r.end[s]; t++) {
+        ok = mbar_wait(&s_full[s], s_use & 1, s_abort, a.err, 50, kAttWaitNs);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        s_use++;
+        tc_fence_after();
+        float v[128];
+#pragma unroll
+        for (int c = 0; c < 4; c++) att_tm_load(ts + 32 * c, v + 32 * c);
+#pragma unroll
+        for (int c = 0; c < 4; c++) att_tm_wait(v + 32 * c);
+        const int off = seen.x - t * kAttTile;
+        const unsigned len = (unsigned)(seen.y - seen.x);
+        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+#pragma unroll
+          for (int c = 0; c < 128; c++) v[c] = (unsigned)(c - off) < len ? v[c] : -INFINITY;
+        }
+        float top[4];
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+          top[k] = fmax3(v[32 * k], v[32 * k + 1], v[32 * k + 2]);
+#pragma unroll
+          for (int j = 3; j < 31; j += 2) top[k] = fmax3(top[k], v[32 * k + j], v[32 * k + j + 1]);
+          top[k] = fmaxf(top[k], v[32 * k + 31]);
+        }
+        const float now = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * a.c2;
+        const bool grow = now > m + kLag;
+        if (__any_sync(~0u, grow)) {
+          const float f = grow ? att_ex2(m - now) : 1.0f;
+          if (grow) m = now;
+          l *= f;
+          if (t > r.first[s]) {
+#pragma unroll 1
+            for (int c = 0; c < DP; c += 32) {
+              float o[32];
+              att_tm_load(to + c, o);
+              att_tm_wait(o);
+#pragma unroll
+              for (int j = 0; j < 32; j++) o[j] *= f;
+              att_tm_store(to + c, o);
+            }
+          }
+        }
+        const float sub = m == -INFINITY ? 0.0f : m;
+        const F2 cc = pack_f2(a.c2), dd = pack_f2(kLift<F16> - sub);
+        F2 sum[2] = {pack_f2(0.0f), pack_f2(0.0f)};
+#pragma unroll
+        for (int c = 0; c < 4; c++) {
+          uint32_t p[16];
+#pragma unroll
+          for (int j = 0; j < 16; j++) {
+            float lo, hi;
+            unpack_f2(fma2(pack_f2(v[32 * c + 2 * j], v[32 * c + 2 * j + 1]), cc, dd), lo, hi);
+            lo = att_ex2(lo);
+            hi = att_ex2(hi);
+            sum[j & 1] = add2(sum[j & 1], pack_f2(lo, hi));
+            p[j] = att_pack2<F16>(lo, hi);
+          }
+          att_tm_store16(ts + 16 * c, p);
+        }
+        l += sum_f2(add2(sum[0], sum[1]));
+        att_tm_store_wait();
+        tc_fence_before();
+        mbar_arrive(&p_full[s]);
+      }
+      if (!ok) break;
+      // The row's result: sums over l; 0 for a row that sees nothing.
+      const bool none = r.first[s] >= r.end[s];
+      if (none)
+        ok = mbar_wait(&q_full[s], q_use & 1, s_abort, a.err, 51, kAttWaitNs);
+      else
+        ok = mbar_wait(&o_full[s], o_use & 1, s_abort, a.err, 52, kAttWaitNs);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      q_use++;
+      tc_fence_after();
+      if (!none) o_use++;
+      const float f = seen.x < seen.y ? 1.0f / l : 0.0f;
+      const bool flagged = r.t0 < r.t1 && s_flag[count % kAttFlags];
+#pragma unroll 1
+      for (int c = 0; c < DP; c += 32) {
+        float o[32];
+        if (none) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = 0.0f;
+        } else {
+          att_tm_load(to + c, o);
+          att_tm_wait(o);
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] *= f;
+          if (flagged) att_add_not_finite<F16>(o, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
+        }
+        att_stage_row<F16>(stage, row, c, o);
+      }
+      tc_fence_before();
+      if (i < a.tokens)
+        a.lse[(int64_t)it.head[s] * a.tokens + i] =
+            seen.x < seen.y ? (m - kLift<F16> + log2f(l)) * 0.693147180559945309f : -INFINITY;
+      att_store_rows<DP>(a, &maps.out, a.out_last, stage, quad * 32, it.head[s], it.tile[s] * kAttTile + quad * 32);
+      if (lane == 0) mbar_arrive(&q_empty[s]);
+      if (r.t0 < r.t1) count++;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+template <int DP, bool F16>
+int launch(const AttFwdMaps& maps, const AttFwd& a, int sms, cudaStream_t s) {
+  static std::atomic<bool> set[128];
+  int dev = 0;
+  VRS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 128 || !set[dev].load()) {
+    VRS_CUDA(cudaFuncSetAttribute(attention_forward_kernel<DP, F16>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)smem_bytes<DP>()));
+    if (dev < 128) set[dev].store(true);
+  }
+  VRS_TRY(launch_after(attention_forward_kernel<DP, F16>, (unsigned)(a.items < sms ? a.items : sms), kThreads,
+                       smem_bytes<DP>(), s, maps, a));
+  count_launch();
+  return VRS_OK;
+}
+
+}  // namespace
+
+int launch_attention_forward(bool f16, int dp, const AttFwdMaps& maps, const AttFwd& a, int sms, cudaStream_t s) {
+  if (dp == 64) return f16 ? launch<64, true>(maps, a, sms, s) : launch<64, false>(maps, a, sms, s);
+  return f16 ? launch<128, true>(maps, a, sms, s) : launch<128, false>(maps, a, sms, s);
+}
+
+}  // namespace ops
+}  // namespace vrs

@@ -22,8 +22,6 @@
 // products an aligned operand whatever x's stride and address are.
 #include <cmath>
 
-#include <cudaTypedefs.h>
-
 #include "linear_ce.cuh"
 
 namespace vrs {
@@ -572,23 +570,11 @@ int check_workspace(const std::string& who, const void* ws, int64_t have, int64_
 // Rows that TMA can address: 16-byte aligned starts.
 bool tma_rows(const void* p, int64_t stride, int64_t rows) { return aligned16(p) && (rows == 1 || stride % 8 == 0); }
 
-PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
-  static PFN_cuTensorMapEncodeTiled_v12000 fn = [] {
-    cudaDriverEntryPointQueryResult q;
-    void* p = nullptr;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess ||
-        q != cudaDriverEntryPointSuccess)
-      p = nullptr;
-    return reinterpret_cast<PFN_cuTensorMapEncodeTiled_v12000>(p);
-  }();
-  return fn;
-}
-
 // [rows][inner] row-major with `stride` elements between rows; boxes of 128
 // bytes by box_rows, 128-byte swizzle, zeros outside.
 int make_map(CUtensorMap* m, CUtensorMapDataType type, int bytes, const void* base, int64_t inner, int64_t rows,
              int64_t stride, int box_rows) {
-  auto fn = encode_fn();
+  auto fn = tensor_map_encoder();
   if (!fn) {
     set_error(VRS_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
     return VRS_ERR_DRIVER;

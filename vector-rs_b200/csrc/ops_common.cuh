@@ -3,6 +3,7 @@
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+#include <cudaTypedefs.h>
 
 #include "vrs_internal.cuh"
 
@@ -184,6 +185,9 @@ inline int invalid(const std::string& m) {
 }
 
 inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The driver's cuTensorMapEncodeTiled; null where there is none.
+PFN_cuTensorMapEncodeTiled_v12000 tensor_map_encoder();
 
 // SMs of the current device (148 on B200), read once per device.
 int sm_count(int* out);

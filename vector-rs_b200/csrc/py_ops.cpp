@@ -14,6 +14,7 @@
 #include <c10/cuda/CUDAStream.h>
 
 #include <algorithm>
+#include <cmath>
 #include <optional>
 #include <sstream>
 #include <string>
@@ -37,6 +38,8 @@ struct Bound {
   decltype(&vrs_grad_norm) grad_norm;
   decltype(&vrs_clip_grad_norm) clip_norm;
   decltype(&vrs_grad_norm_workspace) clip_workspace;
+  decltype(&vrs_attention_forward) attention_forward;
+  decltype(&vrs_attention_forward_workspace) attention_forward_workspace;
   PyObject* check;  // raises CudaError for a status
 } g{};
 
@@ -69,6 +72,7 @@ std::string name_of(at::ScalarType t) {
     case at::kHalf: return "torch.float16";
     case at::kBFloat16: return "torch.bfloat16";
     case at::kLong: return "torch.int64";
+    case at::kInt: return "torch.int32";
     default: return c10::toString(t);
   }
 }
@@ -443,6 +447,95 @@ PyObject* qk_norm_rope_backward(PyObject* const* args) {
   return to_tuple({dq, dk, dqw, dkw});
 }
 
+// Heads as the attention reads them: on 16 bytes with strides that are multiples
+// of 8, elements a multiple of 8 (padded with zeros, which add nothing to a
+// product), or copied to be so.
+HeadRows tiled_heads_of(const at::Tensor& in, const char* name) {
+  HeadRows r = heads_of(in, name, true);
+  if (r.d > 128) bad(name, " has heads of ", r.d, " elements, at most 128 are supported");
+  const int64_t d = (r.d + 7) / 8 * 8;
+  if (d == r.d && (uintptr_t)r.t.data_ptr() % 16 == 0 && (r.tokens <= 1 || r.t.stride(0) % 8 == 0) &&
+      (r.n <= 1 || r.t.stride(1) % 8 == 0) && r.t.stride(0) >= r.d)
+    return r;
+  at::Tensor c = d == r.d ? at::empty({r.tokens, r.n, d}, r.t.options()) : at::zeros({r.tokens, r.n, d}, r.t.options());
+  c.narrow(2, 0, r.d).copy_(r.t);
+  r.t = c;
+  r.d = d;
+  r.h = {c.data_ptr(), c.stride(0), c.stride(1)};
+  return r;
+}
+
+struct AttentionArgs {
+  HeadRows q, k, v;
+  std::optional<at::Tensor> cu;
+  int64_t sequences, d;  // d as given
+  bool causal;
+  float scale;
+};
+
+// (q, k, v, cu_seqlens or None, causal, scale or None)
+AttentionArgs attention_args(PyObject* const* args) {
+  AttentionArgs a;
+  const at::Tensor &q = tensor_arg(args[0], "q"), &k = tensor_arg(args[1], "k"), &v = tensor_arg(args[2], "v");
+  a.cu = optional_arg(args[3], "cu_seqlens");
+  if (q.dim() != 3 && q.dim() != 4) bad("q must be tokens x heads x d or batch x tokens x heads x d, got ", q.sizes());
+  if (a.cu && q.dim() != 3) bad("with cu_seqlens q must be tokens x heads x d, got ", q.sizes());
+  a.d = q.size(-1);
+  const std::pair<const char*, const at::Tensor*> both[] = {{"k", &k}, {"v", &v}};
+  for (auto& [name, t] : both)
+    if (t->dim() != q.dim() || t->size(-1) != a.d || t->size(-2) < 1 || q.size(-2) % t->size(-2) ||
+        t->size(-2) != k.size(-2) || t->sizes().slice(0, q.dim() - 2) != q.sizes().slice(0, q.dim() - 2) ||
+        t->scalar_type() != q.scalar_type() || t->device() != q.device())
+      bad(name, " must be like q but for its heads, of which q has a multiple (", q.sizes(), ", ", name_of(q.scalar_type()),
+          " on ", q.device().str(), "), got ", t->sizes(), ", ", name_of(t->scalar_type()), " on ", t->device().str());
+  a.q = tiled_heads_of(q, "q");
+  a.k = tiled_heads_of(k, "k");
+  a.v = tiled_heads_of(v, "v");
+  a.sequences = q.dim() == 4 ? q.size(0) : 1;
+  if (a.cu) {
+    if (a.cu->dim() != 1 || a.cu->numel() < 1) bad("cu_seqlens must hold one bound more than sequences, got ", a.cu->sizes());
+    a.sequences = a.cu->numel() - 1;
+    a.cu = beside(*a.cu, a.q.t, "cu_seqlens", a.cu->numel(), at::kInt);
+  }
+  a.causal = bool_arg(args[4]);
+  const double scale = args[5] == Py_None ? 1.0 / std::sqrt((double)a.d) : float_arg(args[5]);
+  a.scale = (float)scale;
+  if (!(scale > 0.0) || !(a.scale > 0.0f) || !(a.scale < INFINITY)) bad("scale must be positive and finite, got ", scale);
+  return a;
+}
+
+// A result of tokens x n x d that the caller sees in the shape of `like`.
+struct HeadResult {
+  at::Tensor t;
+  vrs_heads h;
+  HeadResult(const HeadRows& r) : t(at::empty({r.tokens, r.n, r.d}, r.t.options())), h{t.data_ptr(), r.n * r.d, r.d} {}
+  at::Tensor as(at::IntArrayRef sizes) const {
+    const int64_t d = sizes.back();
+    return (d == t.size(2) ? t : t.narrow(2, 0, d).contiguous()).view(sizes);
+  }
+};
+
+// (q, k, v, cu_seqlens, causal, scale) -> (out, lse)
+PyObject* attention_forward(PyObject* const* args) {
+  const AttentionArgs a = attention_args(args);
+  const HeadResult out(a.q);
+  at::Tensor lse = at::empty({a.q.n, a.q.tokens}, a.q.t.options().dtype(at::kFloat));
+  const c10::cuda::CUDAGuard guard(a.q.t.device());
+  int64_t need = 0;
+  std::optional<at::Tensor> ws;
+  if (a.cu) {
+    check_status(g.attention_forward_workspace(a.q.tokens, &need));
+    ws = at::empty({need}, a.q.t.options().dtype(at::kByte));
+  }
+  void* stream = c10::cuda::getCurrentCUDAStream(a.q.t.get_device()).stream();
+  check_status(unlocked([&] {
+    return g.attention_forward(&a.q.h, &a.k.h, &a.v.h, a.q.tokens, a.q.n, a.k.n, a.q.d, code_of(a.q.t.scalar_type()),
+                               (const int32_t*)ptr(a.cu), a.sequences, a.causal, a.scale, &out.h, (float*)lse.data_ptr(),
+                               ptr(ws), need, stream);
+  }));
+  return to_tuple({out.as(THPVariable_Unpack(args[0]).sizes()), lse});
+}
+
 // (gradients, results or None (in place), max_norm or None (the norm alone),
 // unscale) -> norm
 PyObject* clip_grad_norm(PyObject* const* args) {
@@ -575,7 +668,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // bind(addresses of the entry points in the order of Bound, check)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int N = 12;
+  constexpr int N = 14;
   if (n != N + 1) {
     PyErr_Format(PyExc_TypeError, "bind takes %d addresses and a function", N);
     return nullptr;
@@ -600,6 +693,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g.grad_norm = (decltype(g.grad_norm))at[9];
   g.clip_norm = (decltype(g.clip_norm))at[10];
   g.clip_workspace = (decltype(g.clip_workspace))at[11];
+  g.attention_forward = (decltype(g.attention_forward))at[12];
+  g.attention_forward_workspace = (decltype(g.attention_forward_workspace))at[13];
   Py_INCREF(args[N]);
   Py_XDECREF(g.check);
   g.check = args[N];
@@ -617,6 +712,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, 
                          VRS_METHOD(qk_norm_rope_forward, 9),
                          VRS_METHOD(qk_norm_rope_backward, 11),
                          VRS_METHOD(clip_grad_norm, 4),
+                         VRS_METHOD(attention_forward, 6),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

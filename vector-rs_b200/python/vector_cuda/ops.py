@@ -32,7 +32,8 @@ def _bind():
     names = ("layer_norm_forward", "layer_norm_backward", "layer_norm_backward_workspace",
              "linear_cross_entropy_forward", "linear_cross_entropy_backward_with_loss",
              "linear_cross_entropy_workspace", "qk_norm_rope_forward", "qk_norm_rope_backward",
-             "qk_norm_rope_backward_workspace", "grad_norm", "clip_grad_norm", "grad_norm_workspace")
+             "qk_norm_rope_backward_workspace", "grad_norm", "clip_grad_norm", "grad_norm_workspace",
+             "attention_forward", "attention_forward_workspace")
     _ops.bind(*(ctypes.cast(getattr(L, "vrs_" + n), ctypes.c_void_p).value for n in names), _check)
 
 
@@ -201,6 +202,16 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, positions: torch.Tensor, q_we
     return _QkNormRope.apply(q, k, positions, q_weight, k_weight, base, rotary_dim, interleaved, eps)
 
 
+# -------------------------------------------------------------- attention
+
+
+def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+                      causal: bool = True, scale: Optional[float] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(out, lse): out in q's type and shape, lse = log sum_j exp(scale q_i .
+    k_j) in float32, heads x tokens (all tokens of a batch); see attention."""
+    return _ops.attention_forward(q, k, v, cu_seqlens, causal, scale)
+
+
 # ------------------------------------------------------ norm of gradients
 
 
@@ -222,4 +233,4 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
 
 __all__ = ["check", "layer_norm", "layer_norm_forward", "layer_norm_backward", "linear_cross_entropy",
            "linear_cross_entropy_forward", "linear_cross_entropy_backward", "qk_norm_rope", "qk_norm_rope_forward",
-           "qk_norm_rope_backward", "grad_norm", "clip_grad_norm"]
+           "qk_norm_rope_backward", "attention_forward", "grad_norm", "clip_grad_norm"]
