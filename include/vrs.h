@@ -416,6 +416,20 @@ VRS_API int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const 
                                   int64_t sequences, int32_t causal, float scale, const vrs_heads* out, float* lse,
                                   void* workspace, int64_t workspace_bytes, void* cuda_stream);
 
+/* Gradients of the above from that of out, with the forward pass's out and lse: dq
+ * (NULL: not wanted), dk and dv (both or neither NULL), in dtype. Weights and
+ * their gradients are formed again and rounded to 16 bits as operands of the
+ * products: VRS_F16 keeps the latter relative to the largest row of dout times
+ * the largest row of v, down to 2^-38 of that. Tokens that no sequence holds have
+ * gradients 0. */
+VRS_API int vrs_attention_backward_workspace(int64_t tokens, int64_t heads, int64_t* out_bytes);
+VRS_API int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q, const vrs_heads* k, const vrs_heads* v,
+                                   const vrs_heads* out, const float* lse, int64_t tokens, int64_t heads,
+                                   int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,
+                                   int64_t sequences, int32_t causal, float scale, const vrs_heads* dq,
+                                   const vrs_heads* dk, const vrs_heads* dv, void* workspace, int64_t workspace_bytes,
+                                   void* cuda_stream);
+
 /* The RMS norm of each head's query and key (x / sqrt(mean x^2 + eps) * weight),
  * then the rotation to its position of the first `rotary` elements (even, 0..d):
  * pair i turns by position * base^(-2 i / rotary), pairs being elements i and

@@ -146,3 +146,408 @@ def test_forward_matches_formula(gpu, lengths, heads, kv, d, behind, causal, dty
                                                 ([1500], 40, 40, 32), ([60] * 30, 24, 12, 128)])
 def test_forward_many_items(gpu, lengths, heads, kv, d, causal):
     _check(*_make(lengths, heads, kv, d, "bfloat16", 5), lengths, causal, back=False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths,heads,kv,d,behind", CASES, ids=[str(i) for i in range(len(CASES))])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_gradients_match_formula(gpu, lengths, heads, kv, d, behind, causal, dtype):
+    _check(*_make(lengths, heads, kv, d, dtype, behind, seed=1), lengths, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("lengths,heads,kv,d", [([900, 1300], 16, 4, 64), ([700, 31, 900], 27, 9, 128),
+                                                ([1500], 14, 14, 32), ([60] * 30, 24, 12, 128)])
+def test_gradients_many_items(gpu, lengths, heads, kv, d, causal):
+    _check(*_make(lengths, heads, kv, d, "bfloat16", 5), lengths, causal)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("scale", [1e-3, 0.5, 3.0])
+def test_scale(gpu, scale, dtype):
+    """From nearly even weights to single keys whose scores are some hundreds: the running reference has to grow."""
+    _check(*_make([300, 150], 2, 1, 64, dtype), [300, 150], True, scale)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_growing_scores(gpu, dtype):
+    """Each tile of keys has larger scores than all before it, and the other way round."""
+    import torch
+    q, k, v, do = _make([700], 2, 1, 64, dtype)
+    steps = torch.linspace(0.05, 4.0, 700, device="cuda").to(q.dtype)[:, None, None]
+    q = q.abs()
+    _check(q, k.abs() * steps, v, do, [700], False)
+    _check(q, k.abs() * steps.flip(0), v, do, [700], False)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** -20, 2.0 ** -12, 2.0 ** 8])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+def test_gradients_of_any_size(gpu, size, dtype):
+    """dout far from 1 (2^-20 is below float16's normal numbers)."""
+    q, k, v, do = _make([260, 70], 4, 2, 64, dtype)
+    _check(q, k, v, do * size, [260, 70])
+
+
+@pytest.mark.gpu
+def test_rows_of_very_different_weight(gpu):
+    q, k, v, do = _make([200], 2, 2, 64, "float16")
+    do[::2] *= 2.0 ** -10
+    do[7] = 0.0
+    _check(q, k, v, do, [200])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+def test_batch_is_sequences_of_one_length(gpu, causal):
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([150] * 5, 6, 3, 64, "bfloat16")
+    want = _check(q, k, v, do, [150] * 5, causal)
+    b = [t.view(5, 150, *t.shape[1:]) for t in (q, k, v, do)]
+    out, lse = ops.attention_forward(*b[:3], causal=causal)
+    grads = ops.attention_backward(b[3], *b[:3], out, lse, causal=causal)
+    assert out.shape == b[0].shape and grads[1].shape == b[1].shape
+    for a, w in zip((out, lse, *grads), want):
+        assert torch.equal(a.reshape(w.shape), w)
+    # one sequence without bounds
+    want = _check(q, k, v, do, [750], causal)
+    assert torch.equal(ops.attention_forward(q, k, v, causal=causal)[0], want[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("way", ["projection", "gaps", "odd", "heads first", "elements apart", "expanded"])
+def test_views(gpu, way):
+    import torch
+    from vector_cuda import ops
+    lengths, heads, kv, d = [130, 71], 4, 2, 64
+    q, k, v, do = _make(lengths, heads, kv, d, "float16")
+    want = _check(q, k, v, do, lengths)
+    t = 201
+    if way == "projection":
+        w = torch.cat((q, k, v), 1)
+        q, k, v = w[:, :4], w[:, 4:6], w[:, 6:]
+    elif way in ("gaps", "odd"):
+        pad = 16 if way == "gaps" else 3
+        def inside(x):
+            b = torch.full((t, x.shape[1] * d + pad), float("nan"), dtype=x.dtype, device="cuda")
+            s = b[:, pad // 2:pad // 2 + x.shape[1] * d] if way == "odd" else b[:, :x.shape[1] * d]
+            s = s.view(t, x.shape[1], d)
+            s.copy_(x)
+            return s
+        q, k, v, do = (inside(x) for x in (q, k, v, do))
+    elif way == "heads first":
+        q, k, v, do = (x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v, do))
+    elif way == "elements apart":
+        q, k, v, do = (x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v, do))
+    else:
+        do = torch.ones((), dtype=q.dtype, device="cuda").expand(t, heads, d)
+        want = _check(q, k, v, do.contiguous(), lengths)
+    cu = _bounds(lengths)
+    out, lse = ops.attention_forward(q, k, v, cu)
+    got = (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu))
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [1, 7, 20, 33, 100, 127])
+def test_widths_that_no_eight_divides(gpu, d):
+    _check(*_make([140, 9], 2, 1, d, "bfloat16"), [140, 9])
+
+
+@pytest.mark.gpu
+def test_either_gradient_alone(gpu):
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([200, 90], 4, 2, 64, "bfloat16")
+    cu = _bounds([200, 90])
+    out, lse = ops.attention_forward(q, k, v, cu)
+    dq, dk, dv = ops.attention_backward(do, q, k, v, out, lse, cu)
+    a = ops.attention_backward(do, q, k, v, out, lse, cu, need_dkv=False)
+    b = ops.attention_backward(do, q, k, v, out, lse, cu, need_dq=False)
+    assert torch.equal(a[0], dq) and a[1] is None and a[2] is None
+    assert b[0] is None and torch.equal(b[1], dk) and torch.equal(b[2], dv)
+    assert ops.attention_backward(do, q, k, v, out, lse, cu, need_dq=False, need_dkv=False) == (None, None, None)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("causal,lengths,at", [(True, [300], 299), (True, [300], 140), (True, [90, 100, 60], 130),
+                                               (False, [90, 100, 60], 130), (False, [200, 300, 7, 200], 505), (True, [40], 0)])
+def test_not_finite_reaches_only_what_sees_it(gpu, causal, lengths, at, dtype, value):
+    """A token whose key, value, query or output gradient is not finite: rows that
+    do not see it keep their bits, rows that do say so."""
+    import torch
+    from vector_cuda import ops
+    heads, kv, d = 4, 2, 64
+    clean = list(_make(lengths, heads, kv, d, dtype, behind=9))
+    tokens = clean[0].shape[0]
+    cu = _bounds(lengths)
+
+    def run(q, k, v, do):
+        out, lse = ops.attention_forward(q, k, v, cu, causal)
+        return (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu, causal))
+
+    want = run(*clean)
+    seen = _seen(tokens, lengths, causal)
+    sees = seen[:, at]          # queries that see the token
+    back = seen[sees].any(0)    # keys that those see
+    own = seen[at]              # keys that the token sees
+    for which in range(4):
+        bad = [t.clone() for t in clean]
+        bad[which][at, 1, 5] = value
+        out, lse, dq, dk, dv = run(*bad)
+        same = lambda a, b, rows: torch.equal(a[rows].view(torch.int16), b[rows].view(torch.int16))
+        if which == 0:    # a query: its own row, and the keys it sees
+            rows, keys = torch.arange(tokens, device="cuda") == at, own
+        elif which == 3:
+            rows, keys = torch.arange(tokens, device="cuda") == at, own
+            assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+        else:
+            rows, keys = sees, back
+        assert same(out, want[0], ~rows) and same(dq, want[2], ~rows)
+        assert same(dk, want[3], ~keys) and same(dv, want[4], ~keys)
+        assert torch.equal(lse[:, ~rows], want[1][:, ~rows])
+        # the heads that do not use it keep everything
+        group = slice(2, 4) if which in (1, 2) else slice(1, 2)
+        others = [h for h in range(heads) if not (group.start <= h < group.stop)]
+        assert same(out[:, others], want[0][:, others], torch.ones(tokens, dtype=torch.bool))
+        if which == 3:
+            # dout reaches dv of every key it sees (weights are above 0 here)
+            assert not torch.isfinite(dv[own, 0, 5]).any()
+        elif which == 2:
+            assert not torch.isfinite(out[sees][:, 2:4, 5]).any()
+        elif math.isnan(value):
+            assert out[rows][:, group].isnan().all() and dq[rows][:, group].isnan().all()
+
+
+@pytest.mark.gpu
+def test_everything_not_finite(gpu):
+    """A training run that has gone wrong ends with NaN, in a bounded time."""
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = (torch.full_like(t, float("nan")) for t in _make([700, 300, 90], 4, 2, 128, "bfloat16"))
+    cu = _bounds([700, 300, 90])
+    out, lse = ops.attention_forward(q, k, v, cu)
+    grads = ops.attention_backward(do, q, k, v, out, lse, cu)
+    assert all(t.isnan().all() for t in (out, lse, *grads))
+
+
+@pytest.mark.gpu
+def test_bounds_without_meaning_reach_no_other_memory(gpu):
+    """cu_seqlens that fall, are negative or lie past the end: results without meaning, nothing else."""
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([300], 2, 1, 64, "bfloat16")
+    for bounds in ([0, 200, 100, 300], [-50, 100, 1000], [2 ** 31 - 1, -2 ** 31], [5, 5, 5], [300, 0], [7]):
+        cu = torch.tensor(bounds, dtype=torch.int32, device="cuda")
+        out, lse = ops.attention_forward(q, k, v, cu)
+        ops.attention_backward(do, q, k, v, out, lse, cu)
+    ops.check()
+    _check(q, k, v, do, [300])
+
+
+@pytest.mark.gpu
+def test_rows_between_and_around_results_stay(gpu, vc):
+    """C entry: results with strides of their own; what lies between is left alone."""
+    import torch
+    from vector_cuda import ops
+    lengths, heads, kv, d = [150, 60], 4, 2, 72
+    q, k, v, do = _make(lengths, heads, kv, d, "float16", behind=3)
+    want = _check(q, k, v, do, lengths)
+    L, i64, cu, t = vc.lib(), ctypes.c_int64, _bounds(lengths), 213
+
+    class Heads(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("stride", i64), ("head", i64)]
+
+    def of(x):
+        return Heads(x.data_ptr(), x.stride(0), x.stride(1))
+
+    def wide(n):
+        b = torch.full((t + 2, n * 80 + 24), 7.0, dtype=q.dtype, device="cuda")
+        return b, b[1:-1, 8:8 + n * 80].view(t, n, 80)[:, :, :72]
+
+    rest = (i64(t), i64(heads), i64(kv), i64(d), 1, ctypes.c_void_p(cu.data_ptr()), i64(2), 1, ctypes.c_float(72 ** -0.5))
+    n = i64(0)
+    assert L.vrs_attention_forward_workspace(i64(t), ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    bo, o = wide(heads)
+    lse = torch.empty(heads, t, device="cuda")
+    r = ctypes.byref
+    assert L.vrs_attention_forward(r(of(q)), r(of(k)), r(of(v)), *rest, r(of(o)), ctypes.c_void_p(lse.data_ptr()),
+                                   ctypes.c_void_p(ws.data_ptr()), n, None) == 0, L.vrs_last_error()
+    torch.cuda.synchronize()
+    assert L.vrs_attention_backward_workspace(i64(t), i64(heads), ctypes.byref(n)) == 0
+    ws = torch.empty(n.value, dtype=torch.uint8, device="cuda")
+    (bq, gq), (bk, gk), (bv, gv) = wide(heads), wide(kv), wide(kv)
+    assert L.vrs_attention_backward(r(of(do)), r(of(q)), r(of(k)), r(of(v)), r(of(o)), ctypes.c_void_p(lse.data_ptr()), *rest,
+                                    r(of(gq)), r(of(gk)), r(of(gv)), ctypes.c_void_p(ws.data_ptr()), n, None) == 0, L.vrs_last_error()
+    torch.cuda.synchronize()
+    assert torch.equal(lse, want[1])
+    for b, x, w in ((bo, o, want[0]), (bq, gq, want[2]), (bk, gk, want[3]), (bv, gv, want[4])):
+        assert torch.equal(x, w)
+        x.fill_(7.0)
+        assert (b == 7.0).all()
+
+
+@pytest.mark.gpu
+def test_same_bits_captured_and_on_another_stream(gpu):
+    import torch
+    from vector_cuda import ops
+    lengths = [700, 33, 600]
+    q, k, v, do = _make(lengths, 8, 2, 128, "float16", behind=40)
+    cu = _bounds(lengths)
+
+    def both():
+        out, lse = ops.attention_forward(q, k, v, cu)
+        return (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu))
+
+    want = both()
+    for _ in range(3):
+        assert all(torch.equal(a, b) for a, b in zip(want, both()))
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for side in sides:  # two calls at once
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            got.append(both())
+    for side in sides:
+        torch.cuda.current_stream().wait_stream(side)
+    assert all(torch.equal(a, b) for g in got for a, b in zip(want, g))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = both()
+    for _ in range(2):
+        graph.replay()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # other lengths in the captured call: the bounds are read by the device
+    cu.copy_(_bounds([100, 1000, 10]))
+    graph.replay()
+    got = [t.clone() for t in got]
+    assert all(torch.equal(a, b) for a, b in zip(both(), got))
+    ops.check()
+
+
+@pytest.mark.gpu
+def test_autograd_against_differences(gpu):
+    import torch
+    from vector_cuda import ops
+    g = torch.Generator(device="cuda").manual_seed(3)
+    lengths, heads, kv, d = [9, 20], 2, 1, 16
+    cu = _bounds(lengths)
+    x = [(torch.randn(29, n, d, generator=g, device="cuda") * 0.5).half().requires_grad_(True) for n in (heads, kv, kv)]
+    w = torch.randn(29, heads, d, generator=g, device="cuda").half()
+    (ops.attention(*x, cu) * w).sum().backward()
+
+    def f(q, k, v):
+        z = torch.where(_seen(29, lengths, True)[None], torch.einsum("ihd,jhd->hij", q, k.expand(-1, heads, -1)) / 4.0, -math.inf)
+        return (torch.einsum("hij,jhd->ihd", torch.softmax(z, 2), v.expand(-1, heads, -1)) * w.double()).sum().item()
+
+    at = [t.detach().double() for t in x]
+    for i, t in enumerate(x):
+        u = torch.randn(t.shape, generator=g, device="cuda").double()
+        step = 1e-4
+        ends = [f(*[a + s * step * u if j == i else a for j, a in enumerate(at)]) for s in (1, -1)]
+        want = (ends[0] - ends[1]) / (2 * step)
+        # half ulps of the result, of p, ds and out: each at most 2^-11 of a term
+        lim = 2.0 ** -8 * (t.grad.double().abs() * u.abs()).sum().item() + 1e-3
+        assert abs((t.grad.double() * u).sum().item() - want) <= lim
+
+
+@pytest.mark.gpu
+def test_autograd_needs(gpu):
+    """Leaves that want no gradient get none; the others' bits do not change."""
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([70], 2, 1, 64, "bfloat16")
+    cu = _bounds([70])
+    out, lse = ops.attention_forward(q, k, v, cu)
+    want = ops.attention_backward(do, q, k, v, out, lse, cu)
+    for mask in range(1, 8):
+        x = [t.clone().requires_grad_(bool(mask >> i & 1)) for i, t in enumerate((q, k, v))]
+        ops.attention(*x, cu).backward(do)
+        for i, t in enumerate(x):
+            assert (t.grad is None) if not mask >> i & 1 else torch.equal(t.grad, want[i])
+
+
+@pytest.mark.gpu
+def test_no_tokens(gpu):
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = (torch.zeros(0, n, 64, dtype=torch.bfloat16, device="cuda") for n in (4, 2, 2, 4))
+    for cu in (None, torch.zeros(3, dtype=torch.int32, device="cuda")):
+        out, lse = ops.attention_forward(q, k, v, cu)
+        assert out.shape == q.shape and lse.shape == (4, 0)
+        assert [t.shape for t in ops.attention_backward(do, q, k, v, out, lse, cu)] == [q.shape, k.shape, v.shape]
+
+
+@pytest.mark.gpu
+def test_python_refusals(gpu):
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([20], 4, 2, 64, "float16")
+    cu = _bounds([20])
+    for a in ((q.float(), k.float(), v.float(), cu), (q, k.bfloat16(), v, cu), (q, k[:, :1], v, cu), (q[:, :3], k, v, cu),
+              (q, k[:19], v, cu), (q.cpu(), k.cpu(), v.cpu(), cu), (q, k, v, cu.long()), (q, k, v, cu.cpu()),
+              (q, k, v, cu[:0]), (q, k, v, cu[None]), (q[None], k[None], v[None], cu), (q[0], k[0], v[0], cu),
+              (q, k, v[..., :32], cu)):
+        with pytest.raises(ValueError):
+            ops.attention(*a)
+    for scale in (0.0, -1.0, math.inf, math.nan, 1e-60):
+        with pytest.raises(ValueError):
+            ops.attention(q, k, v, cu, True, scale)
+    wide = torch.zeros(5, 2, 136, dtype=torch.float16, device="cuda")
+    with pytest.raises(ValueError, match="128"):
+        ops.attention(wide, wide, wide)
+    out, lse = ops.attention_forward(q, k, v, cu)
+    for a in ((do[:19], q, k, v, out, lse), (do, q, k, v, out[:, :2], lse), (do, q, k, v, out, lse[:, :5]),
+              (do.bfloat16(), q, k, v, out, lse), (do, q, k, v, out, lse.double())):
+        with pytest.raises(ValueError):
+            ops.attention_backward(*a, cu)
+
+
+def test_c_refusals(vc):
+    """Wrong arguments are told by status before anything is queued (no GPU needed)."""
+    L, i64, r = vc.lib(), ctypes.c_int64, ctypes.byref
+
+    class Heads(ctypes.Structure):
+        _fields_ = [("data", ctypes.c_void_p), ("stride", i64), ("head", i64)]
+
+    n = i64(0)
+    assert L.vrs_attention_forward_workspace(i64(100), r(n)) == 0
+    small = n.value
+    assert L.vrs_attention_forward_workspace(i64(1000), r(n)) == 0 and n.value >= small > 0
+    assert L.vrs_attention_forward_workspace(i64(-1), r(n)) == 5
+    sizes = []
+    for t, h in ((100, 2), (100, 4), (1000, 4)):
+        assert L.vrs_attention_backward_workspace(i64(t), i64(h), r(n)) == 0
+        sizes.append(n.value)
+    assert sizes == sorted(sizes) and L.vrs_attention_backward_workspace(i64(5), i64(0), r(n)) == 5
+    ok = Heads(256, 256, 64)
+
+    def call(q=ok, k=ok, v=ok, o=ok, tokens=100, heads=4, kv=2, d=64, dtype=1, cu=256, sequences=2, scale=0.5, lse=256,
+             ws=256, need=small, back=False, dq=ok, dk=ok, dv=ok):
+        h = [r(x) if x else None for x in (q, k, v)]
+        rest = (i64(tokens), i64(heads), i64(kv), i64(d), dtype, ctypes.c_void_p(cu), i64(sequences), 1, ctypes.c_float(scale))
+        if back:
+            g = [r(x) if x else None for x in (dq, dk, dv)]
+            return L.vrs_attention_backward(r(ok), *h, r(o) if o else None, ctypes.c_void_p(lse), *rest, *g,
+                                            ctypes.c_void_p(ws), i64(need), None)
+        return L.vrs_attention_forward(*h, *rest, r(o) if o else None, ctypes.c_void_p(lse), ctypes.c_void_p(ws), i64(need), None)
+
+    for bad in (dict(dtype=0), dict(dtype=3), dict(d=4), dict(d=60), dict(d=136), dict(heads=3), dict(heads=0), dict(kv=0),
+                dict(tokens=-1), dict(tokens=2 ** 31), dict(scale=0.0), dict(scale=math.nan), dict(scale=math.inf),
+                dict(sequences=-1), dict(cu=None, sequences=0), dict(cu=None, sequences=3), dict(q=None), dict(k=None),
+                dict(o=None), dict(v=Heads(None, 256, 64)), dict(q=Heads(264, 256, 64)), dict(k=Heads(256, 260, 64)),
+                dict(v=Heads(256, 256, 60)), dict(o=Heads(256, 256, 56)), dict(q=Heads(256, 56, 64)), dict(lse=None),
+                dict(ws=None), dict(ws=264), dict(need=small - 1)):
+        assert call(**bad) == 5, bad
+    for bad in (dict(dk=None), dict(dv=None), dict(dq=None, dk=None, dv=None), dict(dq=Heads(264, 256, 64)), dict(ws=None),
+                dict(need=sizes[1] - 1), dict(lse=None), dict(o=None)):
+        assert call(**{"back": True, "need": sizes[1], **bad}) == 5, bad
+    assert call(tokens=0) == 0 and call(tokens=0, back=True) == 0

@@ -14,10 +14,13 @@ int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 // Each token's sequence [first, past its last): the last bound at or below the
 // token, by bisection. Whatever cu holds, the interval contains the token and
 // lies within 0..tokens.
-__global__ void __launch_bounds__(256) attention_sequences_kernel(const int* cu, int sequences, int tokens, int2* seg) {
+__global__ void __launch_bounds__(256) attention_sequences_kernel(const int* cu, int sequences, int tokens, int2* seg,
+                                                                  unsigned* zero) {
   grid_launch();
   grid_wait();
   const int t = blockIdx.x * 256 + threadIdx.x;
+  if (zero && t < 2) zero[t] = 0;
+  if (!cu) return;
   if (t >= tokens) return;
   int lo = 0, hi = sequences;
   if (sequences < 1 || cu[0] > t || cu[sequences] <= t) {
@@ -94,8 +97,9 @@ int check_heads(const std::string& w, const char* name, const vrs_heads* h, int6
   return VRS_OK;
 }
 
-// What the passes share; cu_seqlens become a token's sequence in the workspace.
-int start(const Call& c, void* seg, AttArgs& a, cudaStream_t s) {
+// What the passes share; cu_seqlens become a token's sequence in the workspace,
+// `zero` (two words, null: none) is cleared.
+int start(const Call& c, void* seg, unsigned* zero, AttArgs& a, cudaStream_t s) {
   a.tokens = (int)c.tokens;
   a.heads = (int)c.heads;
   a.kv_heads = (int)c.kv_heads;
@@ -108,10 +112,10 @@ int start(const Call& c, void* seg, AttArgs& a, cudaStream_t s) {
   a.seq_len = c.cu ? 0 : (int)(c.tokens / c.sequences);
   a.seg = nullptr;
   VRS_TRY(error_word(&a.err));
-  if (!c.cu) return VRS_OK;
-  a.seg = (const int2*)seg;
-  VRS_TRY(launch_after(attention_sequences_kernel, (unsigned)((c.tokens + 255) / 256), 256, 0, s, (const int*)c.cu,
-                       (int)c.sequences, (int)c.tokens, (int2*)seg));
+  if (!c.cu && !zero) return VRS_OK;
+  if (c.cu) a.seg = (const int2*)seg;
+  VRS_TRY(launch_after(attention_sequences_kernel, c.cu ? (unsigned)((c.tokens + 255) / 256) : 1u, 256, 0, s,
+                       (const int*)c.cu, (int)c.sequences, (int)c.tokens, (int2*)seg, zero));
   count_launch();
   return VRS_OK;
 }
@@ -162,7 +166,7 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
   VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, kAttTile, &a.v_last));
   VRS_TRY(make_map(&maps.out, f16, *out, tokens, heads, d, 32, &a.out_last));
   ProfToken t = prof_begin("attention_forward", s);
-  int st = start(c, workspace, a, s);
+  int st = start(c, workspace, nullptr, a, s);
   if (st == VRS_OK) {
     a.lse = lse;
     a.v = (const uint16_t*)v->data;
@@ -182,6 +186,126 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
       a.items = (int)((a.tiles + 1) / 2 * heads);
     }
     st = launch_attention_forward(f16, d <= 64 ? 64 : 128, maps, a, sms, s);
+  }
+  prof_end(t, s);
+  return st;
+}
+
+namespace vrs {
+namespace ops {
+namespace {
+
+// The backward pass's workspace.
+struct BwdSpace {
+  int64_t padded, seg, lse2, delta, bound, bytes;
+};
+BwdSpace bwd_space(int64_t tokens, int64_t heads) {
+  BwdSpace p;
+  p.padded = up(tokens, kAttTile);
+  p.seg = 0;
+  p.lse2 = up(tokens * 8, 256);
+  p.delta = p.lse2 + heads * p.padded * 4;  // (padded: a multiple of 128)
+  p.bound = p.delta + heads * p.padded * 4;
+  p.bytes = p.bound + 256;
+  return p;
+}
+
+}  // namespace
+}  // namespace ops
+}  // namespace vrs
+
+extern "C" int vrs_attention_backward_workspace(int64_t tokens, int64_t heads, int64_t* out_bytes) {
+  using namespace vrs::ops;
+  if (tokens < 0 || tokens > (1ll << 31) - 512 || heads < 1 || heads > 65536 || !out_bytes)
+    return invalid("vrs_attention_backward_workspace: tokens must be in 0..2^31 - 512, heads in 1..65536, out_bytes not null");
+  *out_bytes = bwd_space(tokens, heads).bytes;
+  return VRS_OK;
+}
+
+extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q, const vrs_heads* k, const vrs_heads* v,
+                                      const vrs_heads* out, const float* lse, int64_t tokens, int64_t heads,
+                                      int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,
+                                      int64_t sequences, int32_t causal, float scale, const vrs_heads* dq,
+                                      const vrs_heads* dk, const vrs_heads* dv, void* workspace, int64_t workspace_bytes,
+                                      void* cuda_stream) {
+  using namespace vrs;
+  using namespace vrs::ops;
+  const std::string w = "vrs_attention_backward";
+  const Call c{tokens, heads, kv_heads, d, dtype, cu_seqlens, sequences, causal, scale};
+  VRS_TRY(check(w, c));
+  if (tokens == 0) return VRS_OK;
+  VRS_TRY(check_heads(w, "dout", dout, tokens, heads, d));
+  VRS_TRY(check_heads(w, "q", q, tokens, heads, d));
+  VRS_TRY(check_heads(w, "k", k, tokens, kv_heads, d));
+  VRS_TRY(check_heads(w, "v", v, tokens, kv_heads, d));
+  VRS_TRY(check_heads(w, "out", out, tokens, heads, d));
+  if (!lse) return invalid(w + ": null lse");
+  if (!dq && (!dk || !dv)) return invalid(w + ": dk and dv come together, and without dq nothing else is left");
+  if ((dk != nullptr) != (dv != nullptr)) return invalid(w + ": dk and dv come together");
+  if (dq) VRS_TRY(check_heads(w, "dq", dq, tokens, heads, d));
+  if (dk) {
+    VRS_TRY(check_heads(w, "dk", dk, tokens, kv_heads, d));
+    VRS_TRY(check_heads(w, "dv", dv, tokens, kv_heads, d));
+  }
+  const BwdSpace p = bwd_space(tokens, heads);
+  VRS_TRY(check_workspace(w, workspace, workspace_bytes, p.bytes));
+  cudaStream_t s = (cudaStream_t)cuda_stream;
+  int sms = 0;
+  VRS_TRY(sm_count(&sms));
+  const bool f16 = dtype == VRS_F16;
+  char* ws = (char*)workspace;
+  AttBwdMaps maps{}, maps_q;
+  AttBwd a{}, aq;
+  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, kAttTile, &a.q_last));
+  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, kAttTile, &a.k_last));
+  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, kAttTile, &a.v_last));
+  VRS_TRY(make_map(&maps.dout, f16, *dout, tokens, heads, d, kAttTile, &a.dout_last));
+  a.out1_last = a.out2_last = 0;
+  maps.out1 = maps.out2 = maps.q;
+  maps_q = maps;
+  int dq_last = 0;
+  if (dq) VRS_TRY(make_map(&maps_q.out1, f16, *dq, tokens, heads, d, 32, &dq_last));
+  if (dk) {
+    VRS_TRY(make_map(&maps.out1, f16, *dk, tokens, kv_heads, d, 32, &a.out1_last));
+    VRS_TRY(make_map(&maps.out2, f16, *dv, tokens, kv_heads, d, 32, &a.out2_last));
+  }
+  ProfToken t = prof_begin("attention_backward", s);
+  unsigned* bound = f16 ? (unsigned*)(ws + p.bound) : nullptr;
+  int st = start(c, ws + p.seg, bound, a, s);
+  if (st == VRS_OK) {
+    a.lse = const_cast<float*>(lse);
+    auto rows = [](const vrs_heads* h, const uint16_t** at, int64_t* stride, int64_t* head) {
+      *at = (const uint16_t*)h->data;
+      *stride = h->stride;
+      *head = h->head_stride;
+    };
+    rows(q, &a.q, &a.qs, &a.qh);
+    rows(k, &a.k, &a.ks, &a.kh);
+    rows(v, &a.v, &a.vs, &a.vh);
+    rows(dout, &a.dout, &a.dos, &a.doh);
+    a.padded = (int)p.padded;
+    a.lse2 = (const float*)(ws + p.lse2);
+    a.delta = (const float*)(ws + p.delta);
+    a.bound = bound;
+    AttStats b{};
+    b.a = a;
+    rows(out, &b.out, &b.os, &b.oh);
+    b.padded = a.padded;
+    b.lse2 = (float*)(ws + p.lse2);
+    b.delta = (float*)(ws + p.delta);
+    b.bound = bound;
+    st = launch_attention_stats(f16, b, sms, s);
+  }
+  const int dp = d <= 64 ? 64 : 128;
+  if (st == VRS_OK && dk) {
+    a.items = a.tiles * (int)kv_heads;
+    st = launch_attention_backward(f16, dp, true, maps, a, sms, s);
+  }
+  if (st == VRS_OK && dq) {
+    aq = a;
+    aq.items = a.tiles * (int)heads;
+    aq.out1_last = dq_last;
+    st = launch_attention_backward(f16, dp, false, maps_q, aq, sms, s);
   }
   prof_end(t, s);
   return st;

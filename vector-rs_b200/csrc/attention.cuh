@@ -333,5 +333,30 @@ struct AttFwd : AttArgs {
 };
 int launch_attention_forward(bool f16, int dp, const AttFwdMaps& maps, const AttFwd& a, int sms, cudaStream_t s);
 
+// The backward pass: statistics of the query rows, then a kernel for dk and dv
+// (items are tiles of keys) and one for dq (tiles of queries).
+struct AttBwdMaps {
+  CUtensorMap q, k, v, dout, out1, out2;  // out1: dk or dq, out2: dv
+};
+struct AttBwd : AttArgs {
+  int items;
+  int q_last, k_last, v_last, dout_last, out1_last, out2_last;
+  int padded;             // tokens, up to whole tiles
+  const float* lse2;      // [heads][padded]: lse log2 e, +inf where nothing is seen
+  const float* delta;     // [heads][padded]
+  const unsigned* bound;  // f16: bits of the largest |dout row|^2 and |v row|^2
+};
+struct AttStats {
+  AttArgs a;
+  const uint16_t* out;
+  int64_t os, oh;
+  int padded;
+  float* lse2;
+  float* delta;
+  unsigned* bound;  // null: not needed
+};
+int launch_attention_stats(bool f16, const AttStats& a, int sms, cudaStream_t s);
+int launch_attention_backward(bool f16, int dp, bool keys, const AttBwdMaps& maps, const AttBwd& a, int sms, cudaStream_t s);
+
 }  // namespace ops
 }  // namespace vrs

@@ -1,0 +1,616 @@
+// attention_bwd.cu -- gradients of the attention on tcgen05. With p_ij =
+// e^(scale q_i . k_j - lse_i) formed again, dp_ij = dout_i . v_j and
+// delta_i = dout_i . out_i (which is sum_j p_ij dp_ij):
+//   ds = p (dp - delta), dq = scale ds k, dk = scale ds^T q, dv = p^T dout,
+// the last two summed over the query heads that share the key's.
+//
+// Two kernels of one form: a CTA keeps a tile of 128 rows (keys and values: dk and
+// dv; queries and output gradients: dq) and passes over the tiles that its rows
+// meet. So every result has one writer that adds in one order, without atomics or
+// an array of partial sums, for two products more than the five that the formulas
+// have (scores and dp twice). The tile's rows are the lanes of tensor memory and a
+// thread has half a row of scores; p and ds go back to tensor memory in 16 bits, as
+// the A operands of the products, over the columns that they came from.
+//
+// The tensor cores run in issue order, so the scores of the next tile are issued
+// after the product that reads this tile's p, and dp after the one that reads ds:
+// while the threads work on p, dp is multiplied, and while they work on ds, the
+// next scores are. Bound by the tensor cores: 4 x 512 clocks a pair of tiles for
+// dk and dv, 3 x 512 for dq (d = 128).
+#include <atomic>
+
+#include "attention.cuh"
+
+namespace vrs {
+namespace ops {
+namespace {
+
+using namespace vrs::tc;
+
+constexpr int kThreads = 384;
+constexpr int kCompute = 256;
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;  // and 11
+constexpr int kColS = 0, kColDp = 128, kCol1 = 256, kCol2 = 384;
+
+template <int DP>
+constexpr int stages() { return DP == 128 ? 2 : 4; }
+template <int DP>
+constexpr uint32_t tile_bytes() { return DP / 64 * kAttBox; }
+constexpr uint32_t kStatBytes = 2 * kAttTile * 4;
+template <int DP>
+constexpr size_t smem_bytes() {
+  return 1024 + (2 + 2 * stages<DP>()) * (size_t)tile_bytes<DP>() + stages<DP>() * (size_t)kStatBytes + 512;
+}
+static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "above the per-block limit");
+
+// f16 ends at 2^16 and loses digits below 2^-14: p, at most 1, is kept 2^14
+// larger, ds times a power of two that brings the bound 2 |dout| |v| of all of them
+// to 2^13 .. 2^14.
+template <bool F16>
+constexpr float kLift = F16 ? 14.0f : 0.0f;
+
+__device__ __forceinline__ float gain_of(const unsigned* bound) {
+  const float b = 2.0f * sqrtf(__uint_as_float(bound[0])) * sqrtf(__uint_as_float(bound[1]));
+  if (!(b > 0.0f)) return 1.0f;
+  int e;
+  frexpf(b, &e);  // b < 2^e
+  return exp2f((float)max(-100, min(100, 14 - e)));
+}
+
+// KEYS: rows are keys and values, results dk and dv; else queries, result dq.
+template <int DP, bool F16, bool KEYS>
+__global__ void __launch_bounds__(kThreads, 1)
+    attention_backward_kernel(const __grid_constant__ AttBwdMaps maps, const __grid_constant__ AttBwd a) {
+  constexpr int ST = stages<DP>();
+  constexpr uint32_t TILE = tile_bytes<DP>();
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = att_align(smem_raw);
+  uint8_t* s_a = smem;               // the rows' two tiles (k, v or q, dout); then the results
+  uint8_t* s_b = smem + 2 * TILE;    // ring of pairs of tiles (q, dout or k, v)
+  float* s_stat = (float*)(s_b + 2 * ST * TILE);  // [ST][lse2, delta][128]
+  uint64_t* bars = (uint64_t*)((uint8_t*)s_stat + ST * kStatBytes);
+  uint64_t* full = bars;             // [ST] both tiles and the statistics have come
+  uint64_t* empty = full + ST;       // [ST] multiplied, and looked through
+  uint64_t* done = empty + ST;       // [ST] scores and dp are multiplied
+  uint64_t* clean = done + ST;       // [ST][2] the pair's tiles are clean
+  uint64_t* a_full = clean + 2 * ST;
+  uint64_t* a_empty = a_full + 1;    // the results have left
+  uint64_t* s_full = a_empty + 1;
+  uint64_t* p_full = s_full + 1;     // scores read, and p written (KEYS)
+  uint64_t* dp_full = p_full + 1;
+  uint64_t* ds_full = dp_full + 1;
+  uint64_t* r_full = ds_full + 1;    // results
+  uint64_t* drain = r_full + 1;
+  uint32_t* s_tmem = (uint32_t*)(drain + 1);
+  volatile int* s_abort = (volatile int*)(s_tmem + 1);
+  volatile int* s_flag = s_abort + 1;  // [kAttFlags]
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < ST; s++) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 3);
+      mbar_init(&done[s], 1);
+      mbar_init(&clean[2 * s], 2);
+      mbar_init(&clean[2 * s + 1], 2);
+    }
+    mbar_init(a_full, 1);
+    mbar_init(a_empty, 8);
+    mbar_init(s_full, 1);
+    mbar_init(p_full, kCompute);
+    mbar_init(dp_full, 1);
+    mbar_init(ds_full, kCompute);
+    mbar_init(r_full, 1);
+    mbar_init(drain, 1);
+    *s_abort = 0;
+    for (int i = 0; i < kAttFlags; i++) s_flag[i] = 0;
+    fence_mbar_init();
+  }
+  if (threadIdx.x == 32 * kLoadWarp) {
+    prefetch_tmap(&maps.q);
+    prefetch_tmap(&maps.k);
+    prefetch_tmap(&maps.v);
+    prefetch_tmap(&maps.dout);
+    prefetch_tmap(&maps.out1);
+    if (KEYS) prefetch_tmap(&maps.out2);
+  }
+  if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *s_tmem;
+  grid_launch();
+  grid_wait();
+
+  // Items: causal, the tiles with the longest passes first (a key's queries are
+  // those after it).
+  const int heads = KEYS ? a.kv_heads : a.heads;
+  auto tile_of = [&](int id) { return KEYS ? id / heads : a.tiles - 1 - id / heads; };
+  const int per = KEYS ? a.group : 1;  // passes over the tiles: the query heads of a key's
+
+  if (warp == kLoadWarp) {
+    // ------------------------------------------------------------ loads
+    int use = 0, a_use = 0;
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const int tile = tile_of(id), head = id % heads;
+      const AttSpan r = att_span<!KEYS>(a, tile);
+      if (lane == 0) {
+        const int n = max(0, r.end - r.first), total = n * per;
+        auto rows = [&] {
+          ok = mbar_wait(a_empty, (a_use & 1) ^ 1, s_abort, a.err, 61, kAttWaitNs);
+          if (!ok) return;
+          mbar_expect_tx(a_full, 2 * TILE);
+          att_load_tile<DP>(s_a, KEYS ? &maps.k : &maps.q, KEYS ? a.k_last : a.q_last, head, tile * kAttTile, a_full);
+          att_load_tile<DP>(s_a + TILE, KEYS ? &maps.v : &maps.dout, KEYS ? a.v_last : a.dout_last, head, tile * kAttTile,
+                            a_full);
+          a_use++;
+        };
+        const int kv = KEYS ? 0 : head / a.group;
+        int t = r.first, g = 0;
+        for (int i = 0; ok && i < total; i++, use++) {
+          const int st = use % ST;
+          ok = mbar_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 62, kAttWaitNs);
+          if (!ok) break;
+          uint8_t* to = s_b + 2 * st * TILE;
+          if (KEYS) {
+            const int h = head * a.group + g;
+            mbar_expect_tx(&full[st], 2 * TILE + kStatBytes);
+            att_load_tile<DP>(to, &maps.q, a.q_last, h, t * kAttTile, &full[st]);
+            att_load_tile<DP>(to + TILE, &maps.dout, a.dout_last, h, t * kAttTile, &full[st]);
+            const int64_t at = (int64_t)h * a.padded + t * kAttTile;
+            bulk_copy_g2s(s_stat + st * 2 * kAttTile, a.lse2 + at, kAttTile * 4, &full[st]);
+            bulk_copy_g2s(s_stat + st * 2 * kAttTile + kAttTile, a.delta + at, kAttTile * 4, &full[st]);
+          } else {
+            mbar_expect_tx(&full[st], 2 * TILE);
+            att_load_tile<DP>(to, &maps.k, a.k_last, kv, t * kAttTile, &full[st]);
+            att_load_tile<DP>(to + TILE, &maps.v, a.v_last, kv, t * kAttTile, &full[st]);
+          }
+          if (++t == r.end) {
+            t = r.first;
+            g++;
+          }
+          if (i == 0) rows();  // (the first pair's place comes free before the rows')
+        }
+        if (total == 0) rows();
+      }
+      ok = __shfl_sync(~0u, ok, 0);
+    }
+    if (lane == 0 && *s_abort) {
+      // Drain (bounded) before shared memory goes.
+      volatile int dummy = 0;
+      for (int i = max(0, use - ST); i < use; i++) mbar_wait(&full[i % ST], i / ST & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+      if (a_use) mbar_wait(a_full, (a_use - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+    }
+  } else if (warp == kMmaWarp) {
+    // ------------------------------------------------------------ products
+    const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
+    const uint64_t bk = smem_desc_sw128(s_b), bm = att_desc_mn(s_b);
+    constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
+    constexpr uint32_t PAIR = 2 * TILE >> 4;
+    int use = 0, a_use = 0, p_use = 0, ds_use = 0;
+    uint32_t cleaned = 0;
+    bool ok = true;
+    auto scores = [&](int st) {  // rows x (q or k)
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+        mma_f16(tmem + kColS, a1 + att_k_step(k), bk + st * PAIR + att_k_step(k), idesc_s, k > 0);
+      mma_commit(s_full);
+    };
+    auto dps = [&](int st) {  // rows x (dout or v)
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+        mma_f16(tmem + kColDp, a2 + att_k_step(k), bk + st * PAIR + (TILE >> 4) + att_k_step(k), idesc_s, k > 0);
+      mma_commit(dp_full);
+      mma_commit(&done[st]);
+    };
+    // (p or ds over its own columns, each half of a row in its half of them) x (tile `second` of the pair)
+    auto product = [&](uint32_t to, uint32_t from, int st, int second, bool add) {
+#pragma unroll
+      for (int k = 0; k < kAttTile / 16; k++)
+        att_mma_ts(tmem + to, tmem + from + (k >> 2) * 64 + (k & 3) * 8,
+                   bm + st * PAIR + second * (TILE >> 4) + att_mn_step(k), idesc_r, add || k > 0);
+    };
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const AttSpan r = att_span<!KEYS>(a, tile_of(id));
+      if (lane == 0) {
+        const int n = max(0, r.end - r.first), total = n * per;
+        if (total > 0) {
+          ok = mbar_wait(a_full, a_use & 1, s_abort, a.err, 63, kAttWaitNs) &&
+               mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 64, kAttWaitNs);
+          if (ok) {
+            tc_fence_after();
+            scores(use % ST);
+            dps(use % ST);
+          }
+        }
+        int t = r.first;
+        for (int i = 0; ok && i < total; i++, use++) {
+          const int st = use % ST, next = (use + 1) % ST;
+          const bool more = i + 1 < total, masked = att_masked(r.low_max, r.high_min, t);
+          ok = mbar_wait(p_full, p_use++ & 1, s_abort, a.err, 65, kAttWaitNs);
+          if (!ok) break;
+          if (KEYS) {
+            if (masked && !(ok = mbar_wait(&clean[2 * st + 1], cleaned >> st & 1, s_abort, a.err, 66, kAttWaitNs))) break;
+            tc_fence_after();
+            product(kCol2, kColS, st, 1, i > 0);
+          }
+          if (more) {
+            ok = mbar_wait(&full[next], (use + 1) / ST & 1, s_abort, a.err, 67, kAttWaitNs);
+            if (!ok) break;
+            tc_fence_after();
+            scores(next);
+          }
+          ok = mbar_wait(ds_full, ds_use++ & 1, s_abort, a.err, 68, kAttWaitNs);
+          if (ok && masked) {
+            ok = mbar_wait(&clean[2 * st], cleaned >> st & 1, s_abort, a.err, 69, kAttWaitNs);
+            cleaned ^= 1u << st;
+          }
+          if (!ok) break;
+          tc_fence_after();
+          product(kCol1, kColDp, st, 0, i > 0);
+          mma_commit(&empty[st]);
+          if (more)
+            dps(next);
+          else
+            mma_commit(r_full);
+          if (++t == r.end) t = r.first;
+        }
+        a_use++;
+      }
+      ok = __shfl_sync(~0u, ok, 0);
+    }
+    if (lane == 0 && *s_abort) {
+      // MMAs in flight must not outlive the block's tensor memory: one more
+      // commit, waited for (bounded).
+      volatile int dummy = 0;
+      mma_commit(drain);
+      mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
+    }
+  } else if (warp >= kCleanWarp) {
+    // ------------------------------------------------------------ cleaning
+    int use = 0, count = 0;
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const AttSpan r = att_span<!KEYS>(a, tile_of(id));
+      const int total = max(0, r.end - r.first) * per;
+      int t = r.first;
+      for (int i = 0; ok && i < total; i++, use++) {
+        const int st = use % ST;
+        ok = mbar_wait(&full[st], use / ST & 1, s_abort, a.err, 70, kAttWaitNs);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        // A later item's flag: the other cleaning warp is at most ST items ahead,
+        // and the item eight before this one, which had the flag last, has its results.
+        if (i == 0 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
+        if (att_masked(r.low_max, r.high_min, t)) {
+          // Scores and dp are of the values as they are.
+          ok = mbar_wait(&done[st], use / ST & 1, s_abort, a.err, 71, kAttWaitNs);
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+          bool any = false;
+#pragma unroll 1
+          for (int second = KEYS ? 1 : 0; second >= 0; second--) {
+            any |= att_clean<DP, F16>(s_b + (2 * st + second) * TILE, warp - kCleanWarp, 2);
+            if (any && lane == 0) s_flag[count % kAttFlags] = 1;
+            att_fence_async();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&clean[2 * st + second]);
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[st]);
+        if (++t == r.end) t = r.first;
+      }
+      if (total > 0) count++;
+    }
+  } else {
+    // ------------------------------------------------------------ p, ds, results
+    const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
+    const uint32_t lanes = (uint32_t)(quad * 32) << 16;
+    const uint32_t ts = tmem + lanes + kColS + half * 64, tdp = tmem + lanes + kColDp + half * 64;
+    const float gain = F16 ? gain_of(a.bound) : 1.0f;
+    const float ds_scale = F16 ? gain * 0x1p-14f : 1.0f;
+    int use = 0, s_use = 0, a_use = 0, r_use = 0, count = 0;
+    bool ok = true;
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const int tile = tile_of(id), head = id % heads;
+      const AttSpan r = att_span<!KEYS>(a, tile);
+      const int total = max(0, r.end - r.first) * per;
+      const int i_row = tile * kAttTile + row;
+      const int2 seen = att_interval<!KEYS>(a, i_row);
+      const unsigned len = (unsigned)(seen.y - seen.x);
+      float lse2 = 0.0f, delta = 0.0f;
+      if (!KEYS) {
+        const int64_t at = (int64_t)head * a.padded + i_row;
+        lse2 = a.lse2[at];
+        delta = a.delta[at];
+      }
+      int t = r.first;
+      for (int i = 0; i < total; i++, use++) {
+        const float* stat = s_stat + use % ST * 2 * kAttTile + half * 64;
+        ok = mbar_wait(s_full, s_use & 1, s_abort, a.err, 72, kAttWaitNs);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        tc_fence_after();
+        float p[64];
+        att_tm_load(ts, p);
+        att_tm_load(ts + 32, p + 32);
+        att_tm_wait(p);
+        att_tm_wait(p + 32);
+        if (!KEYS) {
+          tc_fence_before();
+          mbar_arrive(p_full);  // the next scores may come
+        } else {
+          // (The statistics came with the tiles, by the async proxy: this thread
+          // has to have seen that barrier itself.)
+          ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 73, kAttWaitNs);
+          ok = __all_sync(~0u, ok);
+          if (!ok) break;
+        }
+        const F2 cc = pack_f2(a.c2);
+#pragma unroll
+        for (int c = 0; c < 64; c += 4) {
+          float e[4];
+          F2 lo, hi;
+          if (KEYS) {
+            const float4 z = *reinterpret_cast<const float4*>(stat + c);
+            lo = pack_f2(kLift<F16> - z.x, kLift<F16> - z.y);
+            hi = pack_f2(kLift<F16> - z.z, kLift<F16> - z.w);
+          } else {
+            lo = hi = pack_f2(kLift<F16> - lse2);
+          }
+          unpack_f2(fma2(pack_f2(p[c], p[c + 1]), cc, lo), e[0], e[1]);
+          unpack_f2(fma2(pack_f2(p[c + 2], p[c + 3]), cc, hi), e[2], e[3]);
+#pragma unroll
+          for (int j = 0; j < 4; j++) p[c + j] = att_ex2(e[j]);
+        }
+        const int off = seen.x - t * kAttTile;
+        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+#pragma unroll
+          for (int c = 0; c < 64; c++) p[c] = (unsigned)(c + half * 64 - off) < len ? p[c] : 0.0f;
+        }
+        if (KEYS) {
+#pragma unroll
+          for (int c = 0; c < 2; c++) {
+            uint32_t w[16];
+#pragma unroll
+            for (int j = 0; j < 16; j++) w[j] = att_pack2<F16>(p[32 * c + 2 * j], p[32 * c + 2 * j + 1]);
+            att_tm_store16(ts + 16 * c, w);
+          }
+          att_tm_store_wait();
+          tc_fence_before();
+          mbar_arrive(p_full);
+        }
+        ok = mbar_wait(dp_full, s_use & 1, s_abort, a.err, 74, kAttWaitNs);
+        ok = __all_sync(~0u, ok);
+        if (!ok) break;
+        s_use++;
+        tc_fence_after();
+        const F2 gg = pack_f2(ds_scale);
+        uint32_t w[32];
+#pragma unroll
+        for (int c0 = 0; c0 < 64; c0 += 32) {
+          float v[32];
+          att_tm_load(tdp + c0, v);
+          att_tm_wait(v);
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            F2 lo, hi;
+            if (KEYS) {
+              const float4 z = *reinterpret_cast<const float4*>(stat + kAttTile + c0 + c);
+              lo = pack_f2(-z.x, -z.y);
+              hi = pack_f2(-z.z, -z.w);
+            } else {
+              lo = hi = pack_f2(-delta);
+            }
+            lo = add2(pack_f2(v[c], v[c + 1]), lo);
+            hi = add2(pack_f2(v[c + 2], v[c + 3]), hi);
+            if (F16) {
+              lo = mul2(lo, gg);
+              hi = mul2(hi, gg);
+            }
+            float x, y;
+            unpack_f2(mul2(lo, pack_f2(p[c0 + c], p[c0 + c + 1])), x, y);
+            w[(c0 + c) / 2] = att_pack2<F16>(x, y);
+            unpack_f2(mul2(hi, pack_f2(p[c0 + c + 2], p[c0 + c + 3])), x, y);
+            w[(c0 + c) / 2 + 1] = att_pack2<F16>(x, y);
+          }
+        }
+        // Masked places: p is 0, but dp and delta may hold anything.
+        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+#pragma unroll
+          for (int c = 0; c < 32; c++) {
+            const bool x = (unsigned)(2 * c + half * 64 - off) < len, y = (unsigned)(2 * c + 1 + half * 64 - off) < len;
+            w[c] &= (x ? 0xffffu : 0u) | (y ? 0xffff0000u : 0u);
+          }
+        }
+        att_tm_store16(tdp, w);
+        att_tm_store16(tdp + 16, w + 16);
+        att_tm_store_wait();
+        tc_fence_before();
+        mbar_arrive(ds_full);
+        if (++t == r.end) t = r.first;
+      }
+      if (!ok) break;
+      // Results: dk by the first four warps and dv by the others; dq by the first
+      // four (d up to 64), or half its columns each.
+      if (total == 0)
+        ok = mbar_wait(a_full, a_use & 1, s_abort, a.err, 75, kAttWaitNs);
+      else
+        ok = mbar_wait(r_full, r_use & 1, s_abort, a.err, 76, kAttWaitNs);
+      ok = __all_sync(~0u, ok);
+      if (!ok) break;
+      a_use++;
+      if (total > 0) r_use++;
+      tc_fence_after();
+      const bool flagged = total > 0 && s_flag[count % kAttFlags];
+      if (total > 0) count++;
+      const bool dv = KEYS && half;
+      const uint32_t from = tmem + lanes + (dv ? kCol2 : kCol1);
+      const float f = dv ? (F16 ? 0x1p-14f : 1.0f) : a.scale / gain;
+      uint8_t* stage = s_a + (dv ? TILE : 0);
+      const int c0 = KEYS || DP == 64 ? 0 : half * 64, c1 = KEYS ? DP : DP == 64 ? (half ? 0 : 64) : c0 + 64;
+#pragma unroll 1
+      for (int c = c0; c < c1; c += 32) {
+        float o[32];
+        if (total == 0) {
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] = 0.0f;
+        } else {
+          att_tm_load(from + c, o);
+          att_tm_wait(o);
+#pragma unroll
+          for (int j = 0; j < 32; j++) o[j] *= f;
+          if (flagged) {
+            if (!KEYS) {
+              att_add_not_finite<F16>(o, a.k + head / a.group * a.kh, a.ks, seen.x, seen.y, c, a.d);
+            } else {
+#pragma unroll 1
+              for (int g = 0; g < per; g++) {
+                const int h = head * a.group + g;
+                att_add_not_finite<F16>(o, dv ? a.dout + h * a.doh : a.q + h * a.qh, dv ? a.dos : a.qs, seen.x, seen.y, c, a.d);
+              }
+            }
+          }
+        }
+        att_stage_row<F16>(stage, row, c, o);
+      }
+      tc_fence_before();
+      att_fence_async();
+      __syncwarp();
+      const int token = tile * kAttTile + quad * 32;
+      if (lane == 0 && token < a.tokens && c0 < c1) {
+        const CUtensorMap* map = dv ? &maps.out2 : &maps.out1;
+        const int last = dv ? a.out2_last : a.out1_last;
+        for (int c = c0; c < c1 && c < a.d; c += 64)
+          att_store(map, stage + (c >> 6) * kAttBox + quad * 32 * 128, c, last ? head : token, last ? token : head);
+        att_store_commit();
+        att_store_wait();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(a_empty);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == kMmaWarp) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 512);
+  }
+}
+
+// Per query row: lse in powers of two, and delta = dout . out. A warp takes 32
+// tokens of a head, `lanes` = 16 lanes a row. Values that are not finite become NaN,
+// so that p and ds say so wherever the row is seen. f16: the largest squares of
+// rows of dout and v too (rows that are not finite left out).
+template <bool F16>
+__device__ __forceinline__ void dot8(uint4 x, uint4 y, float& xy, float& xx) {
+  const uint32_t a[4] = {x.x, x.y, x.z, x.w}, b[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+  for (int i = 0; i < 4; i++) {
+    float p, q, r, s;
+    if (F16) {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&a[i]));
+      const float2 g = __half22float2(*reinterpret_cast<const __half2*>(&b[i]));
+      p = f.x, q = f.y, r = g.x, s = g.y;
+    } else {
+      p = __uint_as_float(a[i] << 16), q = __uint_as_float(a[i] & 0xffff0000u);
+      r = __uint_as_float(b[i] << 16), s = __uint_as_float(b[i] & 0xffff0000u);
+    }
+    xy = fmaf(p, r, fmaf(q, s, xy));
+    xx = fmaf(p, p, fmaf(q, q, xx));
+  }
+}
+
+template <bool F16>
+__global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_constant__ AttStats b) {
+  const AttArgs& a = b.a;
+  grid_launch();
+  grid_wait();
+  const int lane = threadIdx.x & 31, gl = lane & 15, group = lane >> 4;
+  const int blocks = b.padded / 32, rows = a.heads + (F16 ? a.kv_heads : 0);
+  const int64_t units = (int64_t)rows * blocks;
+  float top_do = 0.0f, top_v = 0.0f;
+  for (int64_t u = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5); u < units; u += (int64_t)gridDim.x * 8) {
+    const int h = (int)(u / blocks), t0 = (int)(u % blocks) * 32;
+    const bool value = h >= a.heads;  // a head of v
+    const int hv = h - a.heads;
+    const uint16_t* x = value ? a.v + hv * a.vh : a.dout + h * a.doh;
+    const uint16_t* y = value ? x : b.out + h * b.oh;
+    const int64_t xs = value ? a.vs : a.dos, ys = value ? a.vs : b.os;
+    float mine = 0.0f, top = 0.0f;
+#pragma unroll 4
+    for (int r = 0; r < 16; r++) {
+      const int t = t0 + 2 * r + group;
+      float xy = 0.0f, xx = 0.0f;
+      if (t < a.tokens && gl * 8 < a.d)
+        dot8<F16>(*reinterpret_cast<const uint4*>(x + t * xs + gl * 8), *reinterpret_cast<const uint4*>(y + t * ys + gl * 8), xy, xx);
+#pragma unroll
+      for (int o = 8; o; o >>= 1) {
+        xy += __shfl_xor_sync(~0u, xy, o);
+        if (F16) xx += __shfl_xor_sync(~0u, xx, o);
+      }
+      if (F16 && xx < INFINITY) top = fmaxf(top, xx);
+      const float lo = __shfl_sync(~0u, xy, 0), hi = __shfl_sync(~0u, xy, 16);
+      if (lane >> 1 == r) mine = lane & 1 ? hi : lo;
+    }
+    if (value) {
+      top_v = fmaxf(top_v, top);
+      continue;
+    }
+    top_do = fmaxf(top_do, top);
+    const int t = t0 + lane;
+    const int64_t at = (int64_t)h * b.padded + t;
+    const float lse = t < a.tokens ? a.lse[(int64_t)h * a.tokens + t] : -INFINITY;
+    const bool none = att_interval<true>(a, t).y == 0;
+    b.lse2[at] = none ? INFINITY : fabsf(lse) < INFINITY ? lse * 1.44269504088896341f : NAN;
+    b.delta[at] = none ? 0.0f : fabsf(mine) < INFINITY ? mine : NAN;
+  }
+  if (F16) {
+    // (A maximum does not depend on the order.)
+    atomicMax(b.bound, __float_as_uint(top_do));
+    atomicMax(b.bound + 1, __float_as_uint(top_v));
+  }
+}
+
+template <int DP, bool F16, bool KEYS>
+int launch(const AttBwdMaps& maps, const AttBwd& a, int sms, cudaStream_t s) {
+  static std::atomic<bool> set[128];
+  int dev = 0;
+  VRS_CUDA(cudaGetDevice(&dev));
+  if (dev >= 128 || !set[dev].load()) {
+    VRS_CUDA(cudaFuncSetAttribute(attention_backward_kernel<DP, F16, KEYS>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                  (int)smem_bytes<DP>()));
+    if (dev < 128) set[dev].store(true);
+  }
+  VRS_TRY(launch_after(attention_backward_kernel<DP, F16, KEYS>, (unsigned)(a.items < sms ? a.items : sms), kThreads,
+                       smem_bytes<DP>(), s, maps, a));
+  count_launch();
+  return VRS_OK;
+}
+
+template <int DP, bool F16>
+int launch_keys(bool keys, const AttBwdMaps& maps, const AttBwd& a, int sms, cudaStream_t s) {
+  return keys ? launch<DP, F16, true>(maps, a, sms, s) : launch<DP, F16, false>(maps, a, sms, s);
+}
+
+}  // namespace
+
+int launch_attention_backward(bool f16, int dp, bool keys, const AttBwdMaps& maps, const AttBwd& a, int sms, cudaStream_t s) {
+  if (dp == 64) return f16 ? launch_keys<64, true>(keys, maps, a, sms, s) : launch_keys<64, false>(keys, maps, a, sms, s);
+  return f16 ? launch_keys<128, true>(keys, maps, a, sms, s) : launch_keys<128, false>(keys, maps, a, sms, s);
+}
+
+int launch_attention_stats(bool f16, const AttStats& b, int sms, cudaStream_t s) {
+  const int64_t units = (int64_t)(b.a.heads + (f16 ? b.a.kv_heads : 0)) * (b.padded / 32);
+  const int64_t blocks = (units + 7) / 8;
+  const unsigned grid = (unsigned)(blocks < (int64_t)sms * 16 ? blocks : (int64_t)sms * 16);
+  VRS_TRY(f16 ? launch_after(attention_stats_kernel<true>, grid, 256, 0, s, b)
+              : launch_after(attention_stats_kernel<false>, grid, 256, 0, s, b));
+  count_launch();
+  return VRS_OK;
+}
+
+}  // namespace ops
+}  // namespace vrs

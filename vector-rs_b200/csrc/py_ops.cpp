@@ -40,6 +40,8 @@ struct Bound {
   decltype(&vrs_grad_norm_workspace) clip_workspace;
   decltype(&vrs_attention_forward) attention_forward;
   decltype(&vrs_attention_forward_workspace) attention_forward_workspace;
+  decltype(&vrs_attention_backward) attention_backward;
+  decltype(&vrs_attention_backward_workspace) attention_backward_workspace;
   PyObject* check;  // raises CudaError for a status
 } g{};
 
@@ -536,6 +538,41 @@ PyObject* attention_forward(PyObject* const* args) {
   return to_tuple({out.as(THPVariable_Unpack(args[0]).sizes()), lse});
 }
 
+// (dout, out, lse, then as forward, need dq, need dk and dv) -> (dq, dk, dv)
+PyObject* attention_backward(PyObject* const* args) {
+  const AttentionArgs a = attention_args(args + 3);
+  const at::Tensor &dout = tensor_arg(args[0], "dout"), &out = tensor_arg(args[1], "out");
+  const at::Tensor &q = THPVariable_Unpack(args[3]), &k = THPVariable_Unpack(args[4]);
+  check_like(dout, q, "dout", "q");
+  check_like(out, q, "out", "q");
+  const HeadRows gr = tiled_heads_of(dout, "dout"), o = tiled_heads_of(out, "out");
+  const at::Tensor lse = beside(tensor_arg(args[2], "lse"), a.q.t, "lse", a.q.n * a.q.tokens, at::kFloat);
+  const bool need_q = bool_arg(args[9]), need_kv = bool_arg(args[10]);
+  if (!need_q && !need_kv) return to_tuple({std::nullopt, std::nullopt, std::nullopt});
+  std::optional<HeadResult> dq, dk, dv;
+  if (need_q) dq.emplace(a.q);
+  if (need_kv) {
+    dk.emplace(a.k);
+    dv.emplace(a.v);
+  }
+  const c10::cuda::CUDAGuard guard(a.q.t.device());
+  int64_t need = 0;
+  check_status(g.attention_backward_workspace(a.q.tokens, a.q.n, &need));
+  const at::Tensor ws = at::empty({need}, a.q.t.options().dtype(at::kByte));
+  void* stream = c10::cuda::getCurrentCUDAStream(a.q.t.get_device()).stream();
+  check_status(unlocked([&] {
+    return g.attention_backward(&gr.h, &a.q.h, &a.k.h, &a.v.h, &o.h, (const float*)lse.data_ptr(), a.q.tokens, a.q.n,
+                                a.k.n, a.q.d, code_of(a.q.t.scalar_type()), (const int32_t*)ptr(a.cu), a.sequences,
+                                a.causal, a.scale, dq ? &dq->h : nullptr, dk ? &dk->h : nullptr, dv ? &dv->h : nullptr,
+                                ws.data_ptr(), need, stream);
+  }));
+  std::optional<at::Tensor> rq, rk, rv;
+  if (dq) rq = dq->as(q.sizes());
+  if (dk) rk = dk->as(k.sizes());
+  if (dv) rv = dv->as(k.sizes());
+  return to_tuple({rq, rk, rv});
+}
+
 // (gradients, results or None (in place), max_norm or None (the norm alone),
 // unscale) -> norm
 PyObject* clip_grad_norm(PyObject* const* args) {
@@ -668,7 +705,7 @@ PyObject* entry(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 // bind(addresses of the entry points in the order of Bound, check)
 PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
-  constexpr int N = 14;
+  constexpr int N = 16;
   if (n != N + 1) {
     PyErr_Format(PyExc_TypeError, "bind takes %d addresses and a function", N);
     return nullptr;
@@ -695,6 +732,8 @@ PyObject* bind(PyObject*, PyObject* const* args, Py_ssize_t n) {
   g.clip_workspace = (decltype(g.clip_workspace))at[11];
   g.attention_forward = (decltype(g.attention_forward))at[12];
   g.attention_forward_workspace = (decltype(g.attention_forward_workspace))at[13];
+  g.attention_backward = (decltype(g.attention_backward))at[14];
+  g.attention_backward_workspace = (decltype(g.attention_backward_workspace))at[15];
   Py_INCREF(args[N]);
   Py_XDECREF(g.check);
   g.check = args[N];
@@ -713,6 +752,7 @@ PyMethodDef methods[] = {{"bind", (PyCFunction)(void (*)())bind, METH_FASTCALL, 
                          VRS_METHOD(qk_norm_rope_backward, 11),
                          VRS_METHOD(clip_grad_norm, 4),
                          VRS_METHOD(attention_forward, 6),
+                         VRS_METHOD(attention_backward, 11),
                          {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_ops", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

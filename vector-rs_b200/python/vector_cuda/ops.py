@@ -33,7 +33,7 @@ def _bind():
              "linear_cross_entropy_forward", "linear_cross_entropy_backward_with_loss",
              "linear_cross_entropy_workspace", "qk_norm_rope_forward", "qk_norm_rope_backward",
              "qk_norm_rope_backward_workspace", "grad_norm", "clip_grad_norm", "grad_norm_workspace",
-             "attention_forward", "attention_forward_workspace")
+             "attention_forward", "attention_forward_workspace", "attention_backward", "attention_backward_workspace")
     _ops.bind(*(ctypes.cast(getattr(L, "vrs_" + n), ctypes.c_void_p).value for n in names), _check)
 
 
@@ -212,6 +212,44 @@ def attention_forward(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seql
     return _ops.attention_forward(q, k, v, cu_seqlens, causal, scale)
 
 
+def attention_backward(dout: torch.Tensor, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out: torch.Tensor,
+                       lse: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None, causal: bool = True,
+                       scale: Optional[float] = None, need_dq: bool = True, need_dkv: bool = True):
+    """(dq, dk, dv) from the gradient of out and the forward pass's out and lse;
+    None for what is not needed."""
+    return _ops.attention_backward(dout, out, lse, q, k, v, cu_seqlens, causal, scale, need_dq, need_dkv)
+
+
+class _Attention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, cu_seqlens, causal, scale):
+        out, lse = attention_forward(q, k, v, cu_seqlens, causal, scale)
+        ctx.save_for_backward(q, k, v, cu_seqlens, out, lse)
+        ctx.rest = (causal, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout):
+        q, k, v, cu_seqlens, out, lse = ctx.saved_tensors
+        dq, dk, dv = attention_backward(dout, q, k, v, out, lse, cu_seqlens, *ctx.rest, ctx.needs_input_grad[0],
+                                        ctx.needs_input_grad[1] or ctx.needs_input_grad[2])
+        return (dq, dk if ctx.needs_input_grad[1] else None, dv if ctx.needs_input_grad[2] else None, None, None, None)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: Optional[torch.Tensor] = None,
+              causal: bool = True, scale: Optional[float] = None) -> torch.Tensor:
+    """softmax(scale * q k^T) v of every head over packed sequences. q is tokens
+    x heads x d, k and v tokens x kv_heads x d (heads a multiple of kv_heads, d at
+    most 128), all float16 or bfloat16; scale is 1 / sqrt(d) by default. Sequence b
+    is tokens cu_seqlens[b] .. cu_seqlens[b + 1] - 1 (int32 on the device, not
+    falling); a token that no sequence holds has output 0. Without cu_seqlens the
+    tokens are one sequence, or batch x tokens x heads x d a batch of them. causal:
+    a token sees itself and those before it, else all of its sequence. What a
+    token does not see has no effect on it, NaN included."""
+    return _Attention.apply(q, k, v, cu_seqlens, causal, scale)
+
+
 # ------------------------------------------------------ norm of gradients
 
 
@@ -233,4 +271,4 @@ def clip_grad_norm(grads: Sequence[torch.Tensor], max_norm: float, out: Optional
 
 __all__ = ["check", "layer_norm", "layer_norm_forward", "layer_norm_backward", "linear_cross_entropy",
            "linear_cross_entropy_forward", "linear_cross_entropy_backward", "qk_norm_rope", "qk_norm_rope_forward",
-           "qk_norm_rope_backward", "attention_forward", "grad_norm", "clip_grad_norm"]
+           "qk_norm_rope_backward", "attention", "attention_forward", "attention_backward", "grad_norm", "clip_grad_norm"]
