@@ -551,3 +551,22 @@ def test_c_refusals(vc):
                 dict(need=sizes[1] - 1), dict(lse=None), dict(o=None)):
         assert call(**{"back": True, "need": sizes[1], **bad}) == 5, bad
     assert call(tokens=0) == 0 and call(tokens=0, back=True) == 0
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("d", [64, 80])
+@pytest.mark.parametrize("heads,kv", [(7, 7), (12, 3)])
+def test_items_after_empty_ones(gpu, heads, kv, d, causal):
+    """Tiles that no sequence touches come first and last in the order of work, others
+    after them on the same SMs: results do not depend on how long anything takes."""
+    import torch
+    from vector_cuda import ops
+    lengths = [700, 450, 0, 900, 129, 1000]
+    q, k, v, do = _make(lengths, heads, kv, d, "float16", behind=700)
+    want = _check(q, k, v, do, lengths, causal)
+    cu = _bounds(lengths)
+    for _ in range(100):
+        out, lse = ops.attention_forward(q, k, v, cu, causal)
+        got = (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu, causal))
+        assert all(torch.equal(a, b) for a, b in zip(want, got))

@@ -215,9 +215,11 @@ __global__ void __launch_bounds__(kThreads, 1)
       const AttSpan r = att_span<!KEYS>(a, tile_of(id));
       if (lane == 0) {
         const int n = max(0, r.end - r.first), total = n * per;
-        if (total > 0) {
-          ok = mbar_wait(a_full, a_use & 1, s_abort, a.err, 63, kAttWaitNs) &&
-               mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 64, kAttWaitNs);
+        // (The rows are waited for where nothing is multiplied too: a wait for the
+        // next ones that came before these have would not see the difference.)
+        ok = mbar_wait(a_full, a_use++ & 1, s_abort, a.err, 63, kAttWaitNs);
+        if (ok && total > 0) {
+          ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 64, kAttWaitNs);
           if (ok) {
             tc_fence_after();
             scores(use % ST);
@@ -256,7 +258,6 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_commit(r_full);
           if (++t == r.end) t = r.first;
         }
-        a_use++;
       }
       ok = __shfl_sync(~0u, ok, 0);
     }

@@ -219,7 +219,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
       const Range r = range_of(a, it);
-      if (lane == 0 && r.t0 < r.t1) {
+      // The queries are waited for where nothing is multiplied too: a wait for the
+      // next ones that came before these have would not see the difference.
+      for (int s = 0; s < 2 && ok; s++)
+        if (it.live[s]) ok = mbar_wait(&q_full[s], q_use[s]++ & 1, s_abort, a.err, 43, kAttWaitNs);
+      ok = __all_sync(~0u, ok);
+      if (ok && lane == 0 && r.t0 < r.t1) {
         auto scores = [&](int s, int st) {
 #pragma unroll
           for (int k = 0; k < DP / 16; k++)
@@ -227,10 +232,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                     idesc_s, k > 0);
           mma_commit(&s_full[s]);
         };
-        for (int s = 0; s < 2 && ok; s++)
-          if (r.first[s] < r.end[s]) ok = mbar_wait(&q_full[s], q_use[s] & 1, s_abort, a.err, 43, kAttWaitNs);
         // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
-        if (ok) ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 44, kAttWaitNs);
+        ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 44, kAttWaitNs);
         if (ok) {
           tc_fence_after();
           for (int s = 0; s < 2; s++)
@@ -274,12 +277,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         use += 2 * (r.t1 - r.t0);
-        for (int s = 0; s < 2; s++)
-          if (r.first[s] < r.end[s]) q_use[s]++;
       }
-      if (lane == 0)
-        for (int s = 0; s < 2; s++)
-          if (it.live[s] && r.first[s] >= r.end[s]) q_use[s]++;
       ok = __shfl_sync(~0u, ok, 0);
     }
     if (lane == 0 && *s_abort) {
