@@ -137,6 +137,23 @@ __device__ __forceinline__ void att_load_tile(uint8_t* to, const CUtensorMap* ma
     att_load(to + b * kAttBox, map, b * 64, tokens_last ? head : token, tokens_last ? token : head, bar);
 }
 
+// Bounded waits of one thread, and of a warp: one lane asks, since every question
+// is an access to the shared memory that the tensor cores read their operands from.
+__device__ __forceinline__ bool att_wait(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  return tc::mbar_wait(bar, parity, abort, err, code, kAttWaitNs);
+}
+// The products' warp goes on where a wait gave up (all that follow then return at
+// once, and what it multiplies is not used): control flow that hangs on what a wait
+// says would no longer be uniform.
+__device__ __forceinline__ void att_wait_uniform(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  tc::mbar_wait(bar, parity, abort, err, code, kAttWaitNs);
+}
+__device__ __forceinline__ bool att_wait_warp(uint64_t* bar, uint32_t parity, volatile int* abort, int* err, int code) {
+  bool ok = true;
+  if ((threadIdx.x & 31) == 0) ok = att_wait(bar, parity, abort, err, code);
+  return __shfl_sync(~0u, ok, 0);
+}
+
 // ---- operand descriptors of a tile (128 tokens x DP): its rows as M or N
 // (K-major, K = the elements), or its elements as N (MN-major, K = the tokens).
 __device__ __forceinline__ uint64_t att_desc_mn(const void* p) {
@@ -149,14 +166,37 @@ __device__ __forceinline__ uint64_t att_desc_mn(const void* p) {
 __device__ __forceinline__ uint32_t att_k_step(int k) { return (k >> 2) * (kAttBox >> 4) + (k & 3) * 2; }
 __device__ __forceinline__ uint32_t att_mn_step(int k) { return k * (2048 >> 4); }
 
-// D (+)= A B^T, A in tensor memory: a row a lane, two 16-bit values a column.
-__device__ __forceinline__ void att_mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+// D (+)= A B^T and its commit, by the lane whose `lead` is not 0; the whole warp
+// comes here, so that addresses and descriptors stay in uniform registers, where the
+// instruction wants them (a branch of one lane moves each of them there anew, some
+// 75 clocks an MMA of 64).
+__device__ __forceinline__ void att_mma_ss(uint32_t lead, uint32_t d_tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
                                            uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p, e;\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+// A in tensor memory: a row a lane, two 16-bit values a column.
+__device__ __forceinline__ void att_mma_ts(uint32_t lead, uint32_t d_tmem, uint32_t a_tmem, uint64_t bdesc, uint32_t idesc,
+                                           uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p, e;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "setp.ne.b32 e, %5, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "r"(a_tmem), "l"(bdesc), "r"(idesc), "r"(accumulate), "r"(lead)
+      : "memory");
+}
+__device__ __forceinline__ void att_commit(uint32_t lead, uint64_t* bar) {
+  asm volatile(
+      "{\n\t.reg .pred e;\n\t"
+      "setp.ne.b32 e, %1, 0;\n\t"
+      "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(tc::smem_u32(bar)),
+      "r"(lead)
       : "memory");
 }
 

@@ -97,9 +97,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(a_full, 1);
     mbar_init(a_empty, 8);
     mbar_init(s_full, 1);
-    mbar_init(p_full, kCompute);
+    mbar_init(p_full, kCompute / 32);
     mbar_init(dp_full, 1);
-    mbar_init(ds_full, kCompute);
+    mbar_init(ds_full, kCompute / 32);
     mbar_init(r_full, 1);
     mbar_init(drain, 1);
     *s_abort = 0;
@@ -138,7 +138,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (lane == 0) {
         const int n = max(0, r.end - r.first), total = n * per;
         auto rows = [&] {
-          ok = mbar_wait(a_empty, (a_use & 1) ^ 1, s_abort, a.err, 61, kAttWaitNs);
+          ok = att_wait(a_empty, (a_use & 1) ^ 1, s_abort, a.err, 61);
           if (!ok) return;
           mbar_expect_tx(a_full, 2 * TILE);
           att_load_tile<DP>(s_a, KEYS ? &maps.k : &maps.q, KEYS ? a.k_last : a.q_last, head, tile * kAttTile, a_full);
@@ -150,7 +150,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         int t = r.first, g = 0;
         for (int i = 0; ok && i < total; i++, use++) {
           const int st = use % ST;
-          ok = mbar_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 62, kAttWaitNs);
+          ok = att_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 62);
           if (!ok) break;
           uint8_t* to = s_b + 2 * st * TILE;
           if (KEYS) {
@@ -187,85 +187,78 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
     const uint64_t bk = smem_desc_sw128(s_b), bm = att_desc_mn(s_b);
     constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
+    const uint32_t lead = lane == 0, tm = __reduce_min_sync(~0u, tmem);
     constexpr uint32_t PAIR = 2 * TILE >> 4;
-    int use = 0, a_use = 0, p_use = 0, ds_use = 0;
+    int use = 0, a_use = 0, p_use = 0;
     uint32_t cleaned = 0;
-    bool ok = true;
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
     auto scores = [&](int st) {  // rows x (q or k)
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
-        mma_f16(tmem + kColS, a1 + att_k_step(k), bk + st * PAIR + att_k_step(k), idesc_s, k > 0);
-      mma_commit(s_full);
+        att_mma_ss(lead, tm + kColS, a1 + att_k_step(k), bk + st * PAIR + att_k_step(k), idesc_s, k > 0);
+      att_commit(lead, s_full);
     };
     auto dps = [&](int st) {  // rows x (dout or v)
 #pragma unroll
       for (int k = 0; k < DP / 16; k++)
-        mma_f16(tmem + kColDp, a2 + att_k_step(k), bk + st * PAIR + (TILE >> 4) + att_k_step(k), idesc_s, k > 0);
-      mma_commit(dp_full);
-      mma_commit(&done[st]);
+        att_mma_ss(lead, tm + kColDp, a2 + att_k_step(k), bk + st * PAIR + (TILE >> 4) + att_k_step(k), idesc_s, k > 0);
+      att_commit(lead, dp_full);
+      att_commit(lead, &done[st]);
     };
     // (p or ds over its own columns, each half of a row in its half of them) x (tile `second` of the pair)
     auto product = [&](uint32_t to, uint32_t from, int st, int second, bool add) {
 #pragma unroll
       for (int k = 0; k < kAttTile / 16; k++)
-        att_mma_ts(tmem + to, tmem + from + (k >> 2) * 64 + (k & 3) * 8,
+        att_mma_ts(lead, tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8,
                    bm + st * PAIR + second * (TILE >> 4) + att_mn_step(k), idesc_r, add || k > 0);
     };
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+    for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const AttSpan r = att_span<!KEYS>(a, tile_of(id));
-      if (lane == 0) {
-        const int n = max(0, r.end - r.first), total = n * per;
-        // (The rows are waited for where nothing is multiplied too: a wait for the
-        // next ones that came before these have would not see the difference.)
-        ok = mbar_wait(a_full, a_use++ & 1, s_abort, a.err, 63, kAttWaitNs);
-        if (ok && total > 0) {
-          ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 64, kAttWaitNs);
-          if (ok) {
-            tc_fence_after();
-            scores(use % ST);
-            dps(use % ST);
-          }
-        }
-        int t = r.first;
-        for (int i = 0; ok && i < total; i++, use++) {
-          const int st = use % ST, next = (use + 1) % ST;
-          const bool more = i + 1 < total, masked = att_masked(r.low_max, r.high_min, t);
-          ok = mbar_wait(p_full, p_use++ & 1, s_abort, a.err, 65, kAttWaitNs);
-          if (!ok) break;
-          if (KEYS) {
-            if (masked && !(ok = mbar_wait(&clean[2 * st + 1], cleaned >> st & 1, s_abort, a.err, 66, kAttWaitNs))) break;
-            tc_fence_after();
-            product(kCol2, kColS, st, 1, i > 0);
-          }
-          if (more) {
-            ok = mbar_wait(&full[next], (use + 1) / ST & 1, s_abort, a.err, 67, kAttWaitNs);
-            if (!ok) break;
-            tc_fence_after();
-            scores(next);
-          }
-          ok = mbar_wait(ds_full, ds_use++ & 1, s_abort, a.err, 68, kAttWaitNs);
-          if (ok && masked) {
-            ok = mbar_wait(&clean[2 * st], cleaned >> st & 1, s_abort, a.err, 69, kAttWaitNs);
-            cleaned ^= 1u << st;
-          }
-          if (!ok) break;
+      const int total = max(0, r.end - r.first) * per;
+      // (The rows are waited for where nothing is multiplied too: a wait for the
+      // next ones that came before these have would not see the difference.)
+      wait(a_full, a_use++, 63);
+      if (total == 0) continue;
+      wait(&full[use % ST], use / ST, 64);
+      tc_fence_after();
+      scores(use % ST);
+      dps(use % ST);
+      int t = r.first;
+#pragma unroll 1
+      for (int i = 0; i < total; i++, use++, p_use++) {
+        const int st = use % ST, next = (use + 1) % ST;
+        const bool more = i + 1 < total, masked = att_masked(r.low_max, r.high_min, t);
+        wait(p_full, p_use, 65);
+        if (KEYS) {
+          if (masked) wait(&clean[2 * st + 1], cleaned >> st, 66);
           tc_fence_after();
-          product(kCol1, kColDp, st, 0, i > 0);
-          mma_commit(&empty[st]);
-          if (more)
-            dps(next);
-          else
-            mma_commit(r_full);
-          if (++t == r.end) t = r.first;
+          product(kCol2, kColS, st, 1, i > 0);
         }
+        if (more) {
+          wait(&full[next], (use + 1) / ST, 67);
+          tc_fence_after();
+          scores(next);
+        }
+        wait(ds_full, p_use, 68);
+        if (masked) {
+          wait(&clean[2 * st], cleaned >> st, 69);
+          cleaned ^= 1u << st;
+        }
+        tc_fence_after();
+        product(kCol1, kColDp, st, 0, i > 0);
+        att_commit(lead, &empty[st]);
+        if (more)
+          dps(next);
+        else
+          att_commit(lead, r_full);
+        if (++t == r.end) t = r.first;
       }
-      ok = __shfl_sync(~0u, ok, 0);
     }
-    if (lane == 0 && *s_abort) {
+    if (*s_abort) {
       // MMAs in flight must not outlive the block's tensor memory: one more
       // commit, waited for (bounded).
       volatile int dummy = 0;
-      mma_commit(drain);
+      att_commit(lead, drain);
       mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
     }
   } else if (warp >= kCleanWarp) {
@@ -278,16 +271,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       int t = r.first;
       for (int i = 0; ok && i < total; i++, use++) {
         const int st = use % ST;
-        ok = mbar_wait(&full[st], use / ST & 1, s_abort, a.err, 70, kAttWaitNs);
-        ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(&full[st], use / ST & 1, s_abort, a.err, 70);
         if (!ok) break;
         // A later item's flag: the other cleaning warp is at most ST items ahead,
         // and the item eight before this one, which had the flag last, has its results.
         if (i == 0 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
         if (att_masked(r.low_max, r.high_min, t)) {
           // Scores and dp are of the values as they are.
-          ok = mbar_wait(&done[st], use / ST & 1, s_abort, a.err, 71, kAttWaitNs);
-          ok = __all_sync(~0u, ok);
+          ok = att_wait_warp(&done[st], use / ST & 1, s_abort, a.err, 71);
           if (!ok) break;
           bool any = false;
 #pragma unroll 1
@@ -330,8 +321,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int t = r.first;
       for (int i = 0; i < total; i++, use++) {
         const float* stat = s_stat + use % ST * 2 * kAttTile + half * 64;
-        ok = mbar_wait(s_full, s_use & 1, s_abort, a.err, 72, kAttWaitNs);
-        ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(s_full, s_use & 1, s_abort, a.err, 72);
         if (!ok) break;
         tc_fence_after();
         float p[64];
@@ -341,12 +331,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         att_tm_wait(p + 32);
         if (!KEYS) {
           tc_fence_before();
-          mbar_arrive(p_full);  // the next scores may come
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full);  // the next scores may come
         } else {
           // (The statistics came with the tiles, by the async proxy: this thread
           // has to have seen that barrier itself.)
-          ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 73, kAttWaitNs);
-          ok = __all_sync(~0u, ok);
+          ok = att_wait_warp(&full[use % ST], use / ST & 1, s_abort, a.err, 73);
           if (!ok) break;
         }
         const F2 cc = pack_f2(a.c2);
@@ -381,10 +371,10 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           att_tm_store_wait();
           tc_fence_before();
-          mbar_arrive(p_full);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full);
         }
-        ok = mbar_wait(dp_full, s_use & 1, s_abort, a.err, 74, kAttWaitNs);
-        ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(dp_full, s_use & 1, s_abort, a.err, 74);
         if (!ok) break;
         s_use++;
         tc_fence_after();
@@ -430,17 +420,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         att_tm_store16(tdp + 16, w + 16);
         att_tm_store_wait();
         tc_fence_before();
-        mbar_arrive(ds_full);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(ds_full);
         if (++t == r.end) t = r.first;
       }
       if (!ok) break;
       // Results: dk by the first four warps and dv by the others; dq by the first
       // four (d up to 64), or half its columns each.
       if (total == 0)
-        ok = mbar_wait(a_full, a_use & 1, s_abort, a.err, 75, kAttWaitNs);
+        ok = att_wait_warp(a_full, a_use & 1, s_abort, a.err, 75);
       else
-        ok = mbar_wait(r_full, r_use & 1, s_abort, a.err, 76, kAttWaitNs);
-      ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(r_full, r_use & 1, s_abort, a.err, 76);
       if (!ok) break;
       a_use++;
       if (total > 0) r_use++;

@@ -28,7 +28,11 @@ namespace {
 using namespace vrs::tc;
 
 constexpr int kThreads = 384;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;  // and 11
+constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10, kCleaners = 2;
+// Registers: 168 a thread at launch; the softmax warps hold a row of scores and
+// take what the others leave (256 x 192 + 128 x 120 of 384 x 168).
+constexpr int kSoftmaxRegs = 192, kOtherRegs = 120;
+constexpr int kParts = 2;       // of a row of P, handed over one by one
 constexpr int kColS = 0, kColO = 256;  // of tile 0; tile 1: 128 further
 
 template <int DP>
@@ -127,8 +131,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* q_full = clean + ST;    // [2]
   uint64_t* q_empty = q_full + 2;   // [2] the results have left
   uint64_t* s_full = q_empty + 2;   // [2] scores
-  uint64_t* p_full = s_full + 2;    // [2] P in tensor memory
-  uint64_t* o_full = p_full + 2;    // [2] all products
+  uint64_t* p_full = s_full + 2;    // [2][kParts] P in tensor memory
+  uint64_t* o_full = p_full + 2 * kParts;  // [2] all products
   uint64_t* drain = o_full + 2;     // of a run that gave up
   uint32_t* s_tmem = (uint32_t*)(drain + 1);
   volatile int* s_abort = (volatile int*)(s_tmem + 1);
@@ -138,14 +142,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < ST; s++) {
       mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 3);
-      mbar_init(&clean[s], 2);
+      mbar_init(&empty[s], 1 + kCleaners);
+      mbar_init(&clean[s], kCleaners);
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&q_full[s], 1);
       mbar_init(&q_empty[s], 4);
       mbar_init(&s_full[s], 1);
-      mbar_init(&p_full[s], 128);
+      for (int c = 0; c < kParts; c++) mbar_init(&p_full[s * kParts + c], 4);
       mbar_init(&o_full[s], 1);
     }
     mbar_init(drain, 1);
@@ -167,6 +171,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_launch();
   grid_wait();
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------ loads
     int use = 0, q_use[2] = {0, 0};
@@ -182,7 +188,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (i == min(i1, i0 + 2)) {
             for (int s = 0; s < 2 && ok; s++) {
               if (!it.live[s]) continue;
-              ok = mbar_wait(&q_empty[s], (q_use[s] & 1) ^ 1, s_abort, a.err, 41, kAttWaitNs);
+              ok = att_wait(&q_empty[s], (q_use[s] & 1) ^ 1, s_abort, a.err, 41);
               if (!ok) break;
               mbar_expect_tx(&q_full[s], TILE);
               att_load_tile<DP>(s_q + s * TILE, &maps.q, a.q_last, it.head[s], it.tile[s] * kAttTile, &q_full[s]);
@@ -191,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
           if (!ok || i >= i1) break;
           const int st = use % ST;
-          ok = mbar_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 42, kAttWaitNs);
+          ok = att_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 42);
           if (!ok) break;
           mbar_expect_tx(&full[st], TILE);
           const bool val = i & 1;
@@ -211,80 +217,80 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ products
+    // One warp for both tiles of queries, by turns: with a warp each their
+    // products interleave, both groups of warps wait and then take exponentials at
+    // the same time (8,192 x 8 heads: 335 us against 283).
     const uint64_t qd = smem_desc_sw128(s_q), kd = smem_desc_sw128(s_kv), vd = att_desc_mn(s_kv);
     constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_o = att_idesc<F16>(DP, true);
+    const uint32_t lead = lane == 0, tm = __reduce_min_sync(~0u, tmem);
     int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
     uint32_t cleaned = 0;  // parity of each stage's cleanings
-    bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
+    auto scores = [&](int s, int st) {
+#pragma unroll
+      for (int k = 0; k < DP / 16; k++)
+        att_mma_ss(lead, tm + kColS + s * 128, qd + s * (TILE >> 4) + att_k_step(k), kd + st * (TILE >> 4) + att_k_step(k),
+                   idesc_s, k > 0);
+      att_commit(lead, &s_full[s]);
+    };
+    for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
       const Range r = range_of(a, it);
       // The queries are waited for where nothing is multiplied too: a wait for the
       // next ones that came before these have would not see the difference.
-      for (int s = 0; s < 2 && ok; s++)
-        if (it.live[s]) ok = mbar_wait(&q_full[s], q_use[s]++ & 1, s_abort, a.err, 43, kAttWaitNs);
-      ok = __all_sync(~0u, ok);
-      if (ok && lane == 0 && r.t0 < r.t1) {
-        auto scores = [&](int s, int st) {
 #pragma unroll
-          for (int k = 0; k < DP / 16; k++)
-            mma_f16(tmem + kColS + s * 128, qd + s * (TILE >> 4) + att_k_step(k), kd + st * (TILE >> 4) + att_k_step(k),
-                    idesc_s, k > 0);
-          mma_commit(&s_full[s]);
-        };
-        // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
-        ok = mbar_wait(&full[use % ST], use / ST & 1, s_abort, a.err, 44, kAttWaitNs);
-        if (ok) {
-          tc_fence_after();
-          for (int s = 0; s < 2; s++)
-            if (r.active(s, r.t0)) scores(s, use % ST);
-          mma_commit(&empty[use % ST]);
+      for (int s = 0; s < 2; s++)
+        if (it.live[s]) wait(&q_full[s], q_use[s]++, 43);
+      if (r.t0 >= r.t1) continue;
+      // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
+      wait(&full[use % ST], use / ST, 44);
+      tc_fence_after();
+#pragma unroll
+      for (int s = 0; s < 2; s++)
+        if (r.active(s, r.t0)) scores(s, use % ST);
+      att_commit(lead, &empty[use % ST]);
+#pragma unroll 1
+      for (int t = r.t0; t < r.t1; t++, use += 2) {
+        const int uv = use + 1, uk = use + 2, sv = uv % ST, sk = uk % ST;
+        const bool more = t + 1 < r.t1;
+        wait(&full[sv], uv / ST, 45);
+        if (att_masked(r.low_max, r.high_min, t)) {
+          wait(&clean[sv], cleaned >> sv, 46);
+          cleaned ^= 1u << sv;
         }
-        for (int t = r.t0; ok && t < r.t1; t++) {
-          const int uv = use + 2 * (t - r.t0) + 1, uk = uv + 1, sv = uv % ST, sk = uk % ST;
-          const bool more = t + 1 < r.t1;
-          ok = mbar_wait(&full[sv], uv / ST & 1, s_abort, a.err, 45, kAttWaitNs);
-          if (ok && att_masked(r.low_max, r.high_min, t)) {
-            ok = mbar_wait(&clean[sv], cleaned >> sv & 1, s_abort, a.err, 46, kAttWaitNs);
-            cleaned ^= 1u << sv;
-          }
-          bool keys = false;
-          for (int s = 0; s < 2 && ok; s++) {
-            if (r.active(s, t)) {
-              ok = mbar_wait(&p_full[s], p_use[s] & 1, s_abort, a.err, 47, kAttWaitNs);
-              if (!ok) break;
-              p_use[s]++;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+          if (r.active(s, t)) {
+#pragma unroll
+            for (int c = 0; c < kParts; c++) {
+              wait(&p_full[s * kParts + c], p_use[s], 47);
               tc_fence_after();
 #pragma unroll
-              for (int k = 0; k < kAttTile / 16; k++)
-                att_mma_ts(tmem + kColO + s * 128, tmem + kColS + s * 128 + k * 8, vd + sv * (TILE >> 4) + att_mn_step(k),
+              for (int k = c * (8 / kParts); k < (c + 1) * (8 / kParts); k++)
+                att_mma_ts(lead, tm + kColO + s * 128, tm + kColS + s * 128 + k * 8, vd + sv * (TILE >> 4) + att_mn_step(k),
                            idesc_o, t > r.first[s] || k > 0);
-              if (t + 1 == r.end[s]) mma_commit(&o_full[s]);
             }
-            if (more && r.active(s, t + 1)) {
-              if (!keys) ok = mbar_wait(&full[sk], uk / ST & 1, s_abort, a.err, 48, kAttWaitNs);
-              if (!ok) break;
-              keys = true;
-              tc_fence_after();
-              scores(s, sk);
-            }
+            p_use[s]++;
+            if (t + 1 == r.end[s]) att_commit(lead, &o_full[s]);
           }
-          if (!ok) break;
-          mma_commit(&empty[sv]);
-          if (more) {
-            if (!keys) ok = mbar_wait(&full[sk], uk / ST & 1, s_abort, a.err, 48, kAttWaitNs);
-            mma_commit(&empty[sk]);
+          if (more && r.active(s, t + 1)) {
+            wait(&full[sk], uk / ST, 48);
+            tc_fence_after();
+            scores(s, sk);
           }
         }
-        use += 2 * (r.t1 - r.t0);
+        att_commit(lead, &empty[sv]);
+        if (more) {
+          wait(&full[sk], uk / ST, 48);
+          att_commit(lead, &empty[sk]);
+        }
       }
-      ok = __shfl_sync(~0u, ok, 0);
     }
-    if (lane == 0 && *s_abort) {
+    if (*s_abort) {
       // MMAs in flight must not outlive the block's tensor memory: one more
       // commit, waited for (bounded).
       volatile int dummy = 0;
-      mma_commit(drain);
+      att_commit(lead, drain);
       mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
     }
   } else if (warp >= kCleanWarp) {
@@ -298,16 +304,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int st = use % ST;
         // (Keys too are waited for: an arrival before the tile has come could
         // count for the tile before it.)
-        ok = mbar_wait(&full[st], use / ST & 1, s_abort, a.err, 49, kAttWaitNs);
-        ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(&full[st], use / ST & 1, s_abort, a.err, 49);
         if (!ok) break;
         if (i & 1) {
           // A later item's flag: the ring holds at most four tiles of values, so
-          // the other cleaning warp is at most four items ahead, and the item
+          // the other cleaning warps are at most four items ahead, and the item
           // eight before this one, which had the flag last, has its results.
           if (i == 2 * r.t0 + 1 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
           if (att_masked(r.low_max, r.high_min, i >> 1)) {
-            if (att_clean<DP, F16>(s_kv + st * TILE, warp - kCleanWarp, 2) && lane == 0) s_flag[count % kAttFlags] = 1;
+            if (att_clean<DP, F16>(s_kv + st * TILE, warp - kCleanWarp, kCleaners) && lane == 0) s_flag[count % kAttFlags] = 1;
             att_fence_async();
             __syncwarp();
             if (lane == 0) mbar_arrive(&clean[st]);
@@ -318,8 +323,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (r.t0 < r.t1) count++;
     }
+  }
   } else {
     // ------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int s = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + s * 128, to = tmem + lanes + kColO + s * 128;
@@ -337,8 +344,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int2 seen = att_interval<true>(a, i);
       float m = -INFINITY, l = 0.0f;
       for (int t = r.first[s]; t < r.end[s]; t++) {
-        ok = mbar_wait(&s_full[s], s_use & 1, s_abort, a.err, 50, kAttWaitNs);
-        ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(&s_full[s], s_use & 1, s_abort, a.err, 50);
         if (!ok) break;
         s_use++;
         tc_fence_after();
@@ -382,6 +388,15 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float sub = m == -INFINITY ? 0.0f : m;
         const F2 cc = pack_f2(a.c2), dd = pack_f2(kLift<F16> - sub);
         F2 sum[2] = {pack_f2(0.0f), pack_f2(0.0f)};
+        // P goes over in parts: the product with the first ones runs while the last
+        // ones are exponentiated. A part's store is waited for after the next
+        // part's exponentials.
+        const auto hand_over = [&](int c) {
+          att_tm_store_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[s * kParts + c]);
+        };
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           uint32_t p[16];
@@ -394,21 +409,19 @@ __global__ void __launch_bounds__(kThreads, 1)
             sum[j & 1] = add2(sum[j & 1], pack_f2(lo, hi));
             p[j] = att_pack2<F16>(lo, hi);
           }
+          if (c && c % (4 / kParts) == 0) hand_over(c / (4 / kParts) - 1);
           att_tm_store16(ts + 16 * c, p);
         }
+        hand_over(kParts - 1);
         l += sum_f2(add2(sum[0], sum[1]));
-        att_tm_store_wait();
-        tc_fence_before();
-        mbar_arrive(&p_full[s]);
       }
       if (!ok) break;
       // The row's result: sums over l; 0 for a row that sees nothing.
       const bool none = r.first[s] >= r.end[s];
       if (none)
-        ok = mbar_wait(&q_full[s], q_use & 1, s_abort, a.err, 51, kAttWaitNs);
+        ok = att_wait_warp(&q_full[s], q_use & 1, s_abort, a.err, 51);
       else
-        ok = mbar_wait(&o_full[s], o_use & 1, s_abort, a.err, 52, kAttWaitNs);
-      ok = __all_sync(~0u, ok);
+        ok = att_wait_warp(&o_full[s], o_use & 1, s_abort, a.err, 52);
       if (!ok) break;
       q_use++;
       tc_fence_after();
