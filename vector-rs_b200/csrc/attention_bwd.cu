@@ -187,30 +187,38 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
     const uint64_t bk = smem_desc_sw128(s_b), bm = att_desc_mn(s_b);
     constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
-    const uint32_t lead = lane == 0, tm = __reduce_min_sync(~0u, tmem);
+    // The whole warp goes through the loops, one lane issues.
+    const bool lead = att_elect();
+    const uint32_t tm = __reduce_min_sync(~0u, tmem);
     constexpr uint32_t PAIR = 2 * TILE >> 4;
     int use = 0, a_use = 0, p_use = 0;
     uint32_t cleaned = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
     auto scores = [&](int st) {  // rows x (q or k)
+      if (lead) {
+        const uint64_t bd = bk + st * PAIR;
 #pragma unroll
-      for (int k = 0; k < DP / 16; k++)
-        att_mma_ss(lead, tm + kColS, a1 + att_k_step(k), bk + st * PAIR + att_k_step(k), idesc_s, k > 0);
-      att_commit(lead, s_full);
+        for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColS, a1 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+        mma_commit(s_full);
+      }
     };
     auto dps = [&](int st) {  // rows x (dout or v)
+      if (lead) {
+        const uint64_t bd = bk + st * PAIR + (TILE >> 4);
 #pragma unroll
-      for (int k = 0; k < DP / 16; k++)
-        att_mma_ss(lead, tm + kColDp, a2 + att_k_step(k), bk + st * PAIR + (TILE >> 4) + att_k_step(k), idesc_s, k > 0);
-      att_commit(lead, dp_full);
-      att_commit(lead, &done[st]);
+        for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+        mma_commit(dp_full);
+        mma_commit(&done[st]);
+      }
     };
     // (p or ds over its own columns, each half of a row in its half of them) x (tile `second` of the pair)
     auto product = [&](uint32_t to, uint32_t from, int st, int second, bool add) {
+      if (lead) {
+        const uint64_t bd = bm + st * PAIR + second * (TILE >> 4);
 #pragma unroll
-      for (int k = 0; k < kAttTile / 16; k++)
-        att_mma_ts(lead, tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8,
-                   bm + st * PAIR + second * (TILE >> 4) + att_mn_step(k), idesc_r, add || k > 0);
+        for (int k = 0; k < kAttTile / 16; k++)
+          att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
+      }
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const AttSpan r = att_span<!KEYS>(a, tile_of(id));
@@ -246,11 +254,11 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         tc_fence_after();
         product(kCol1, kColDp, st, 0, i > 0);
-        att_commit(lead, &empty[st]);
+        if (lead) mma_commit(&empty[st]);
         if (more)
           dps(next);
         else
-          att_commit(lead, r_full);
+          if (lead) mma_commit(r_full);
         if (++t == r.end) t = r.first;
       }
     }
@@ -258,7 +266,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // MMAs in flight must not outlive the block's tensor memory: one more
       // commit, waited for (bounded).
       volatile int dummy = 0;
-      att_commit(lead, drain);
+      if (lead) mma_commit(drain);
       mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
     }
   } else if (warp >= kCleanWarp) {

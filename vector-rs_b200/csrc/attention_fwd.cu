@@ -222,16 +222,20 @@ __global__ void __launch_bounds__(kThreads, 1)
     // the same time (8,192 x 8 heads: 335 us against 283).
     const uint64_t qd = smem_desc_sw128(s_q), kd = smem_desc_sw128(s_kv), vd = att_desc_mn(s_kv);
     constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_o = att_idesc<F16>(DP, true);
-    const uint32_t lead = lane == 0, tm = __reduce_min_sync(~0u, tmem);
+    // The whole warp goes through the loops, one lane issues.
+    const bool lead = att_elect();
+    const uint32_t tm = __reduce_min_sync(~0u, tmem);
     int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
     uint32_t cleaned = 0;  // parity of each stage's cleanings
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
     auto scores = [&](int s, int st) {
+      if (lead) {
+        const uint64_t ad = qd + s * (TILE >> 4), bd = kd + st * (TILE >> 4);
 #pragma unroll
-      for (int k = 0; k < DP / 16; k++)
-        att_mma_ss(lead, tm + kColS + s * 128, qd + s * (TILE >> 4) + att_k_step(k), kd + st * (TILE >> 4) + att_k_step(k),
-                   idesc_s, k > 0);
-      att_commit(lead, &s_full[s]);
+        for (int k = 0; k < DP / 16; k++)
+          mma_f16(tm + kColS + s * 128, ad + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+        mma_commit(&s_full[s]);
+      }
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
@@ -248,7 +252,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
       for (int s = 0; s < 2; s++)
         if (r.active(s, r.t0)) scores(s, use % ST);
-      att_commit(lead, &empty[use % ST]);
+      if (lead) mma_commit(&empty[use % ST]);
 #pragma unroll 1
       for (int t = r.t0; t < r.t1; t++, use += 2) {
         const int uv = use + 1, uk = use + 2, sv = uv % ST, sk = uk % ST;
@@ -265,13 +269,16 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (int c = 0; c < kParts; c++) {
               wait(&p_full[s * kParts + c], p_use[s], 47);
               tc_fence_after();
+              if (lead) {
+                const uint64_t bd = vd + sv * (TILE >> 4);
 #pragma unroll
-              for (int k = c * (8 / kParts); k < (c + 1) * (8 / kParts); k++)
-                att_mma_ts(lead, tm + kColO + s * 128, tm + kColS + s * 128 + k * 8, vd + sv * (TILE >> 4) + att_mn_step(k),
-                           idesc_o, t > r.first[s] || k > 0);
+                for (int k = c * (8 / kParts); k < (c + 1) * (8 / kParts); k++)
+                  att_mma_ts(tm + kColO + s * 128, tm + kColS + s * 128 + k * 8, bd + att_mn_step(k), idesc_o,
+                             k > 0 || t > r.first[s]);
+              }
             }
             p_use[s]++;
-            if (t + 1 == r.end[s]) att_commit(lead, &o_full[s]);
+            if (t + 1 == r.end[s]) if (lead) mma_commit(&o_full[s]);
           }
           if (more && r.active(s, t + 1)) {
             wait(&full[sk], uk / ST, 48);
@@ -279,10 +286,10 @@ __global__ void __launch_bounds__(kThreads, 1)
             scores(s, sk);
           }
         }
-        att_commit(lead, &empty[sv]);
+        if (lead) mma_commit(&empty[sv]);
         if (more) {
           wait(&full[sk], uk / ST, 48);
-          att_commit(lead, &empty[sk]);
+          if (lead) mma_commit(&empty[sk]);
         }
       }
     }
@@ -290,7 +297,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // MMAs in flight must not outlive the block's tensor memory: one more
       // commit, waited for (bounded).
       volatile int dummy = 0;
-      att_commit(lead, drain);
+      if (lead) mma_commit(drain);
       mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
     }
   } else if (warp >= kCleanWarp) {
