@@ -53,6 +53,7 @@ struct Common {
   float unscale, max_norm;
   float* norm;
   int write_norm;
+  int in_place;    // all of them
 };
 
 template <int N>
@@ -191,41 +192,46 @@ __device__ __forceinline__ void store_one(O* o, T v, float f) {
   *o = from_f32<O>(to_f32(v) * f);
 }
 
-template <class T, class O, int VEC>
-__device__ __forceinline__ void scale_pack(const Pack<T, VEC>& p, O* o, float f, bool wide) {
-  if (!wide) {
+// Results are stored past the caches' reach (evict first): what is left of the
+// gradients in L2 stays there for the chunks before.
+template <class O, int VEC>
+__device__ __forceinline__ void stream_pack(O* o, const float* v) {
+  Pack<O, VEC> p;
 #pragma unroll
-    for (int j = 0; j < VEC; j++) store_one(o + j, p.v[j], f);
-    return;
-  }
-  constexpr int W = 16 / sizeof(O) < VEC ? 16 / sizeof(O) : VEC;
-#pragma unroll
-  for (int h = 0; h < VEC / W; h++) {
-    float v[W];
-#pragma unroll
-    for (int j = 0; j < W; j++) v[j] = to_f32(p.v[h * W + j]) * f;
-    store_pack<O, W>(o + h * W, v);
-  }
+  for (int j = 0; j < VEC; j += 2) round_pair(p.v + j, v[j], v[j + 1]);
+  __stcs(reinterpret_cast<uint4*>(o), *reinterpret_cast<uint4*>(&p));
 }
 
+// Accesses of 16 bytes on the result's side: of 16-bit gradients that become 32-bit
+// ones 8 bytes are read, so that neighbouring lanes store neighbouring 16 bytes.
 template <class T, class O>
 __device__ __forceinline__ void scale_chunk(const Grad& g, uint32_t chunk, float f) {
-  constexpr int VEC = 16 / sizeof(T);
+  constexpr int VEC = 16 / sizeof(T), W = 16 / sizeof(O), N = kLoads * VEC / W;
   const Part p = part_of<VEC>(g, chunk);
   const T* in = (const T*)g.in;
   O* out = (O*)g.out;
   const T* at = in + p.at;
   O* to = out + p.at;
   const int tid = threadIdx.x;
+  auto put = [&](int i, const Pack<T, W>& k) {
+    float v[W];
+#pragma unroll
+    for (int j = 0; j < W; j++) v[j] = to_f32(k.v[j]) * f;
+    if (g.wide) {
+      stream_pack<O, W>(to + i * W, v);
+    } else {
+#pragma unroll
+      for (int j = 0; j < W; j++) to[i * W + j] = from_f32<O>(v[j]);
+    }
+  };
   if (p.vecs == kChunkVecs) {
-    Pack<T, VEC> v[kLoads];
+    Pack<T, W> v[N];
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) v[i] = load_pack<T, VEC>(at + (i * kThreads + tid) * VEC);
+    for (int i = 0; i < N; i++) v[i] = load_pack<T, W>(at + (i * kThreads + tid) * W);
 #pragma unroll
-    for (int i = 0; i < kLoads; i++) scale_pack<T, O, VEC>(v[i], to + (i * kThreads + tid) * VEC, f, g.wide);
+    for (int i = 0; i < N; i++) put(i * kThreads + tid, v[i]);
   } else {
-    for (int i = tid; i < p.vecs; i += kThreads)
-      scale_pack<T, O, VEC>(load_pack<T, VEC>(at + i * VEC), to + i * VEC, f, g.wide);
+    for (int i = tid; i < p.vecs * (VEC / W); i += kThreads) put(i, load_pack<T, W>(at + i * W));
   }
   if (tid < p.before) store_one(out + tid, in[tid], f);
   if (tid < p.after) store_one(to + p.vecs * VEC + tid, at[p.vecs * VEC + tid], f);
@@ -243,6 +249,7 @@ __global__ void __launch_bounds__(kThreads) grad_scale_kernel(const __grid_const
   if (a.tensors == 0) return;
   const double q = (double)a.max_norm / (norm + 1e-6);
   const float f = (float)((q >= 1.0 ? 1.0 : q) * (double)a.unscale);  // (a NaN stays one)
+  if (f == 1.0f && a.in_place) return;
   uint32_t c0, c1;
   run_of(a.chunks, c0, c1);
   if (c0 >= c1) return;
@@ -333,6 +340,7 @@ int run(const char* who, const vrs_grad* grads, int64_t tensors, bool clip, floa
       Grad list[kMostTensors];
       uint32_t chunks = 0;
       int n = 0;
+      c.in_place = 1;
       for (; at < tensors && n < kMostTensors; at++) {
         const vrs_grad& v = grads[at];
         if (v.count == 0) continue;
@@ -344,6 +352,7 @@ int run(const char* who, const vrs_grad* grads, int64_t tensors, bool clip, floa
         g.n = v.count;
         g.type = (uint8_t)v.dtype;
         g.out_f32 = clip && v.out_dtype == VRS_F32;
+        if (v.out != v.grad) c.in_place = 0;
         g.head = (uint8_t)((16 - (uintptr_t)v.grad % 16) % 16 / bytes);
         g.wide = ((uintptr_t)v.out + (uintptr_t)g.head * ob) % 16 == 0;
         g.chunk = chunks;

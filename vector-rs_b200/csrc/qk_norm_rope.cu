@@ -16,6 +16,7 @@
 // Angles: position times frequency in 64 bits, in turns, of which the whole ones
 // are dropped before the sine is taken in 32 bits: positions of millions turn
 // the fastest pair by as many radians, of which 32 bits would leave two digits.
+#include <algorithm>
 #include <cmath>
 
 #include "ops_common.cuh"
@@ -27,7 +28,7 @@ namespace {
 constexpr int kThreads = 256;
 constexpr int kWarps = kThreads / 32;
 constexpr int kMostD = 256;
-constexpr int kMostBlocks = 148 * 6;   // of the backward pass: partial sums of the weights' gradients
+constexpr int kMostBlocks = 148 * 4;   // backward each block leaves partial sums
 constexpr int kFinishRows = 32;        // threads that share a column of those
 
 struct Heads {
@@ -43,7 +44,7 @@ struct Heads {
 struct RopeArgs {
   Heads q, k;
   int64_t tokens;
-  int d, rotary;
+  int d, rotary, w_f32;
   float eps, inv_d;
   const int64_t* pos;
   int splits, per;  // a token's heads are split for `splits` warps, `per` each
@@ -75,32 +76,18 @@ __device__ __forceinline__ Slot<V, INTER> slot_of(const RopeArgs& a, int slot) {
   return s;
 }
 
-// One head's pairs of a lane, as floats: e[0..V) from the first access, e[V..2V)
-// from the second.
+// V elements into shared memory, completing with the thread's group of copies.
 template <class T, int V>
-__device__ __forceinline__ void load_slot(const T* p, int a, int b, float (&e)[2 * V]) {
-  const Pack<T, V> x = load_pack<T, V>(p + a), y = load_pack<T, V>(p + b);
-#pragma unroll
-  for (int j = 0; j < V; j++) {
-    e[j] = to_f32(x.v[j]);
-    e[V + j] = to_f32(y.v[j]);
-  }
+__device__ __forceinline__ void copy_pack(Pack<T, V>* to, const T* from) {
+  if constexpr (sizeof(T) * V >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                 "n"(sizeof(T) * V)
+                 : "memory");
+  else
+    *to = load_pack<T, V>(from);  // (copies are of 4 bytes and more)
 }
-
-// Turns the pairs by (cos, sin); SIGN -1 turns back. Slots that are not turned
-// have cosine 1 and sine 0, which leaves finite values as they are; `turned`
-// keeps a 0 times an infinity out of them.
-template <int V, bool INTER>
-__device__ __forceinline__ void turn(float (&e)[2 * V], const float (&c)[V], const float (&s)[V], float sign, bool turned) {
-  if (!turned) return;
-#pragma unroll
-  for (int j = 0; j < V; j++) {
-    float &a = INTER ? e[2 * j] : e[j], &b = INTER ? e[2 * j + 1] : e[V + j];
-    const float x = a, y = b, sn = s[j] * sign;
-    a = x * c[j] - y * sn;
-    b = y * c[j] + x * sn;
-  }
-}
+template <int N>
+__device__ __forceinline__ void copies_but() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <int L>
 __device__ __forceinline__ float group_sum(float v) {
@@ -109,145 +96,329 @@ __device__ __forceinline__ float group_sum(float v) {
   return v;
 }
 
-// V pairs an access, L lanes a head, S accesses a lane; BACK: the gradients.
-template <class T, class P, int V, int L, int S, bool INTER, bool BACK>
-__global__ void __launch_bounds__(kThreads) qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
-  __shared__ float2 s_turn[kWarps][kMostD / 2];
-  __shared__ double s_freq[kMostD / 2];  // (lanes read different ones: constant memory would serve them in turn)
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane % L, group = lane / L;
-  constexpr int G = 32 / L;  // heads at a time
-  for (int p = threadIdx.x; p < a.rotary / 2; p += kThreads) s_freq[p] = a.turns[p];
-  __syncthreads();
-  grid_launch();
-  grid_wait();
-  Slot<V, INTER> slot[S];
-  float w[2][S][2 * V];   // weights of queries and keys
-  float dw[2][S][2 * V];
+// The 2 V elements of a slot as V pairs of floats: neighbours of one access (a pair
+// that turns together where those are neighbours), or one of each where V is 1.
+template <class T, int V>
+__device__ __forceinline__ void to_pairs(const Pack<T, V>& x, const Pack<T, V>& y, F2 (&e)[V]) {
+  if constexpr (V == 1) {
+    e[0] = pack_f2(to_f32(x.v[0]), to_f32(y.v[0]));
+  } else {
 #pragma unroll
-  for (int s = 0; s < S; s++) {
-    slot[s] = slot_of<V, INTER>(a, gl + s * L);
+    for (int q = 0; q < V / 2; q++) {
+      e[q] = pair_of(&x.v[2 * q]);
+      e[V / 2 + q] = pair_of(&y.v[2 * q]);
+    }
+  }
+}
+template <class T, int V>
+__device__ __forceinline__ void store_pairs(T* x, T* y, const F2 (&e)[V]) {
+  float v[2 * V];
 #pragma unroll
-    for (int h = 0; h < 2; h++) {
-      const P* from = (const P*)(h ? a.k.w : a.q.w);
+  for (int q = 0; q < V; q++) unpack_f2(e[q], v[2 * q], v[2 * q + 1]);
+  store_pack<T, V>(x, v);
+  store_pack<T, V>(y, v + V);
+}
+
+// A weight, in the heads' type or in 32 bits; ones where there are none.
+template <class T>
+__device__ __forceinline__ float weight_at(const void* w, int i, bool f32) {
+  return !w ? 1.0f : f32 ? static_cast<const float*>(w)[i] : to_f32(static_cast<const T*>(w)[i]);
+}
+
+struct alignas(16) TwoF2 {
+  F2 v[2];
+};
+
+// Turns a slot's pairs; BACK turns back. SIDE: a pair's two elements are next to
+// each other (in one F2), else its second ones are V / 2 F2s further.
+template <int V, bool SIDE>
+struct Angles {
+  F2 c[SIDE ? (V + 1) / 2 : V / 2], s[SIDE ? (V + 1) / 2 : V / 2];  // of pairs 2 q and 2 q + 1
+  __device__ __forceinline__ void set(const float2* turn) {
+    if constexpr (V == 1) {
+      c[0] = pack_f2(turn[0].x);
+      s[0] = pack_f2(turn[0].y);
+    } else {
 #pragma unroll
-      for (int j = 0; j < 2 * V; j++) {
-        const int at = j < V ? slot[s].a + j : slot[s].b + j - V;
-        w[h][s][j] = slot[s].a >= 0 && from ? to_f32(from[at]) : 1.0f;
-        dw[h][s][j] = 0.0f;
+      for (int q = 0; q < V / 2; q++) {
+        c[q] = pack_f2(turn[2 * q].x, turn[2 * q + 1].x);
+        s[q] = pack_f2(turn[2 * q].y, turn[2 * q + 1].y);
       }
     }
   }
-  const int heads = a.q.n + a.k.n, half = a.rotary / 2;
-  const int64_t units = a.tokens * a.splits;
-  for (int64_t u = (int64_t)blockIdx.x * kWarps + warp; u < units; u += (int64_t)gridDim.x * kWarps) {
-    const int64_t t = u / a.splits;
-    const int h0 = (int)(u % a.splits) * a.per, h1 = min(heads, h0 + a.per);
-    // The token's cosines and sines, each computed by one lane.
-    const double at = half ? (double)a.pos[t] : 0.0;
-    __syncwarp();
-    for (int p = lane; p < half; p += 32) {
-      const double turns = at * s_freq[p];
-      float sn, cs;
-      sincospif((float)(2.0 * (turns - rint(turns))), &sn, &cs);
-      s_turn[warp][p] = make_float2(cs, sn);
-    }
-    __syncwarp();
-    float cs[S][V], sn[S][V];
-    bool turned[S];
+  template <bool BACK>
+  __device__ __forceinline__ void turn(F2 (&e)[V]) const {
+    const F2 minus = pack_f2(-1.0f);
+    if constexpr (!SIDE) {
 #pragma unroll
-    for (int s = 0; s < S; s++) {
-      turned[s] = slot[s].a >= 0 && slot[s].first < half;
+      for (int q = 0; q < V / 2; q++) {
+        const F2 x = e[q], y = e[V / 2 + q], neg = mul2(s[q], minus);
+        e[q] = fma2(x, c[q], mul2(y, BACK ? s[q] : neg));
+        e[V / 2 + q] = fma2(y, c[q], mul2(x, BACK ? neg : s[q]));
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < V; q++) {
+        float x, y, c0, c1, s0, s1;
+        unpack_f2(e[q], x, y);
+        unpack_f2(c[q / 2], c0, c1);
+        unpack_f2(s[q / 2], s0, s1);
+        const float cs = q & 1 ? c1 : c0, sn = BACK ? -(q & 1 ? s1 : s0) : (q & 1 ? s1 : s0);
+        e[q] = pack_f2(fmaf(x, cs, -(y * sn)), fmaf(y, cs, x * sn));
+      }
+    }
+  }
+};
+
+// V pairs an access, L lanes a head, S accesses a lane; BACK: the gradients.
+// A warp's heads, of one token after another, pass through a ring in shared memory
+// that each lane fills for itself some turns ahead. What bounds it then is the number
+// of instructions, so the heads of queries and of keys are passes of their own whose
+// addresses only step, and arithmetic goes by pairs of floats (32,768 tokens of
+// 16 + 4 heads x 128 bf16: 240 instructions a turn and 97 us forward, 362 and 153
+// backward, with 8-byte accesses, single floats and addresses formed a head).
+template <class T, int S, int V>
+constexpr int ring_of() { return S * V * sizeof(T) <= 8 ? 4 : 2; }
+
+// Blocks an SM runs at a time: the grid is that and no more, since each block goes on
+// until the work is done.
+template <int S, int V, bool BACK>
+constexpr int blocks_of() { return (S * V >= 4 ? 2 : 3) + !BACK; }
+
+template <class T, int V, int L, int S, bool INTER, bool BACK>
+__global__ void __launch_bounds__(kThreads, (blocks_of<S, V, BACK>()))
+    qk_norm_rope_kernel(const __grid_constant__ RopeArgs a) {
+  constexpr int G = 32 / L, RING = ring_of<T, S, V>();  // G heads at a time
+  constexpr int ARRAYS = BACK ? 2 : 1, TURN = ARRAYS * S * 2 * 32;
+  using K = Pack<T, V>;
+  constexpr int kRingBytes = kWarps * RING * TURN * (int)sizeof(K);
+  constexpr int kSumBytes = BACK ? kWarps * kMostD * 4 : 16;
+  __shared__ __align__(16) uint8_t s_raw[kRingBytes > kSumBytes ? kRingBytes : kSumBytes];  // the ring, then the sums
+  __shared__ float2 s_turn[kWarps][kMostD / 2];
+  __shared__ double s_freq[kMostD / 2];  // (lanes read different ones: constant memory would serve them in turn)
+  __shared__ TwoF2 s_w[2][S][(V + 1) / 2][L];  // weights of queries and keys; neighbouring lanes side by side
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gl = lane % L, group = lane / L;
+  K* ring = reinterpret_cast<K*>(s_raw) + warp * RING * TURN + lane;
+  for (int p = threadIdx.x; p < a.rotary / 2; p += kThreads) s_freq[p] = a.turns[p];
+  grid_launch();
+  grid_wait();
+  Slot<V, INTER> slot[S];
+  F2 dw[2][S][V];
+  const int half = a.rotary / 2;
+  bool turned[S];
+#pragma unroll
+  for (int s = 0; s < S; s++) {
+    slot[s] = slot_of<V, INTER>(a, gl + s * L);
+    turned[s] = slot[s].a >= 0 && slot[s].first < half;
+#pragma unroll
+    for (int h = 0; h < 2; h++) {
+      const void* from = h ? a.k.w : a.q.w;
+      Pack<float, V> x, y;
 #pragma unroll
       for (int j = 0; j < V; j++) {
-        const float2 f = turned[s] ? s_turn[warp][slot[s].first + j] : make_float2(1.0f, 0.0f);
-        cs[s][j] = f.x;
-        sn[s][j] = f.y;
+        x.v[j] = slot[s].a >= 0 ? weight_at<T>(from, slot[s].a + j, a.w_f32) : 1.0f;
+        y.v[j] = slot[s].a >= 0 ? weight_at<T>(from, slot[s].b + j, a.w_f32) : 1.0f;
+      }
+      F2 w[V];
+      to_pairs<float, V>(x, y, w);
+#pragma unroll
+      for (int j = 0; j < V; j++) {
+        dw[h][s][j] = pack_f2(0.0f);
+        if (threadIdx.x < L) s_w[h][s][j / 2][gl].v[j % 2] = w[j];
       }
     }
-#pragma unroll 2
-    for (int i = h0; i < h1; i += G) {
-      const int head = i + group;
-      const bool live = head < h1, key = head >= a.q.n;
-      const int h = key ? head - a.q.n : head;
-      const T* x = (const T*)(key ? a.k.x : a.q.x) + t * (key ? a.k.stride : a.q.stride) + h * (key ? a.k.head : a.q.head);
-      T* y = (T*)(key ? a.k.y : a.q.y) + (t * (key ? a.k.n : a.q.n) + h) * a.d;
-      float e[S][2 * V], g[S][2 * V];
-      float sq = 0.0f;
+  }
+  // Lanes without elements read zeros for good.
+#pragma unroll
+  for (int i = 0; i < RING * ARRAYS * S * 2; i++) {
+    K z;
+#pragma unroll
+    for (int j = 0; j < V; j++) z.v[j] = from_f32<T>(0.0f);
+    ring[i * 32] = z;
+  }
+  __syncthreads();
+  const int heads = a.q.n + a.k.n;
+  const int64_t units = a.tokens * a.splits, step = (int64_t)gridDim.x * kWarps;
+
+  // The warp's work in order: per token (or part of its heads) a run of queries, then
+  // one of keys; `left` heads of it from this lane's group's on.
+  struct Run {
+    int64_t u, t;
+    int which, first, left;
+  };
+  auto enter = [&](Run& r) {  // the run `which` of unit u, or the next that is not empty
+    for (;; r.which = 0, r.u += step) {
+      if (r.u >= units) return;
+      r.t = r.u / a.splits;
+      const int h0 = (int)(r.u - r.t * a.splits) * a.per, h1 = min(heads, h0 + a.per);
+      for (; r.which < 2; r.which++) {
+        const int off = r.which ? a.q.n : 0, n = r.which ? a.k.n : a.q.n;
+        r.first = max(h0 - off, 0);
+        r.left = min(h1 - off, n) - r.first;
+        if (r.left > 0) {
+          r.first += group;
+          r.left -= group;
+          return;
+        }
+      }
+    }
+  };
+
+  // The copies run ahead.
+  Run ahead;
+  ahead.u = (int64_t)blockIdx.x * kWarps + warp;
+  ahead.which = 0;
+  const T *ax = nullptr, *ag = nullptr;
+  int64_t sx = 0, sg = 0;
+  auto point = [&] {
+    if (ahead.u >= units) return;
+    const Heads& h = ahead.which ? a.k : a.q;
+    ax = (const T*)h.x + ahead.t * h.stride + ahead.first * h.head;
+    sx = G * h.head;
+    if (BACK) {
+      ag = (const T*)h.dy + ahead.t * h.dstride + ahead.first * h.dhead;
+      sg = G * h.dhead;
+    }
+  };
+  enter(ahead);
+  Run now = ahead;
+  point();
+  auto fetch = [&](int r) {
+    if (ahead.u < units) {
+      K* to = ring + r * TURN;
+      if (ahead.left > 0) {
+#pragma unroll
+        for (int s = 0; s < S; s++)
+          if (slot[s].a >= 0) {
+            copy_pack<T, V>(to + 64 * s, ax + slot[s].a);
+            copy_pack<T, V>(to + 64 * s + 32, ax + slot[s].b);
+            if (BACK) {
+              copy_pack<T, V>(to + 64 * (S + s), ag + slot[s].a);
+              copy_pack<T, V>(to + 64 * (S + s) + 32, ag + slot[s].b);
+            }
+          }
+      }
+      ax += sx;
+      if (BACK) ag += sg;
+      ahead.left -= G;
+      if (ahead.left + group <= 0) {  // (the same for the whole warp)
+        ahead.which++;
+        enter(ahead);
+        point();
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll 1
+  for (int r = 0; r < RING; r++) fetch(r);
+
+  Angles<V, INTER || V == 1> angle[S];
+  int64_t token = -1;
+  int r = 0;
+  auto pass = [&](const Heads& hd, F2 (&sums)[S][V], const TwoF2 (&ws)[S][(V + 1) / 2][L]) {
+    T* y = (T*)hd.y + (now.t * hd.n + now.first) * a.d;
+#pragma unroll 1
+    for (int left = now.left; left + group > 0; left -= G) {
+      copies_but<RING - 1>();
+      const K* from = ring + r * TURN;
+      const bool live = left > 0;
+      F2 e[S][V], g[S][V], sq = pack_f2(0.0f);
 #pragma unroll
       for (int s = 0; s < S; s++) {
+        to_pairs<T, V>(from[64 * s], from[64 * s + 32], e[s]);
+        if (BACK) to_pairs<T, V>(from[64 * (S + s)], from[64 * (S + s) + 32], g[s]);
 #pragma unroll
-        for (int j = 0; j < 2 * V; j++) e[s][j] = g[s][j] = 0.0f;
-        if (live && slot[s].a >= 0) {
-          load_slot<T, V>(x, slot[s].a, slot[s].b, e[s]);
-          if (BACK) {
-            const T* dy = (const T*)(key ? a.k.dy : a.q.dy) + t * (key ? a.k.dstride : a.q.dstride) +
-                          h * (key ? a.k.dhead : a.q.dhead);
-            load_slot<T, V>(dy, slot[s].a, slot[s].b, g[s]);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < 2 * V; j++) sq = fmaf(e[s][j], e[s][j], sq);
+        for (int j = 0; j < V; j++) sq = fma2(e[s][j], e[s][j], sq);
       }
-      sq = group_sum<L>(sq);
-      const float rstd = 1.0f / sqrtf(sq * a.inv_d + a.eps);
-      if (BACK) {
-        float mean = 0.0f;
+      fetch(r);  // (each lane's own places, read above)
+      r = r + 1 == RING ? 0 : r + 1;
+      const F2 rstd = pack_f2(rsqrtf(group_sum<L>(sum_f2(sq)) * a.inv_d + a.eps));
+      if constexpr (BACK) {
+        F2 mean = pack_f2(0.0f);
 #pragma unroll
         for (int s = 0; s < S; s++) {
-          turn<V, INTER>(g[s], cs[s], sn[s], -1.0f, turned[s]);
+          if (turned[s]) angle[s].template turn<true>(g[s]);
 #pragma unroll
-          for (int j = 0; j < 2 * V; j++) {
-            e[s][j] *= rstd;
-            const float f = g[s][j] * e[s][j];
-            // (A select, so that each thread's sums stay in registers.)
-            dw[0][s][j] += live && !key ? f : 0.0f;
-            dw[1][s][j] += live && key ? f : 0.0f;
-            g[s][j] *= key ? w[1][s][j] : w[0][s][j];
-            mean = fmaf(g[s][j], e[s][j], mean);
+          for (int j = 0; j < V; j++) {
+            e[s][j] = mul2(e[s][j], rstd);
+            // (A group past the last head holds an earlier one's values.)
+            if (live) sums[s][j] = fma2(g[s][j], e[s][j], sums[s][j]);
+            g[s][j] = mul2(g[s][j], ws[s][j / 2][gl].v[j % 2]);
+            mean = fma2(g[s][j], e[s][j], mean);
           }
         }
-        mean = group_sum<L>(mean) * a.inv_d;
+        const F2 m = pack_f2(-group_sum<L>(sum_f2(mean)) * a.inv_d);
 #pragma unroll
         for (int s = 0; s < S; s++)
 #pragma unroll
-          for (int j = 0; j < 2 * V; j++) e[s][j] = (g[s][j] - e[s][j] * mean) * rstd;
+          for (int j = 0; j < V; j++) e[s][j] = mul2(fma2(e[s][j], m, g[s][j]), rstd);
       } else {
 #pragma unroll
         for (int s = 0; s < S; s++) {
 #pragma unroll
-          for (int j = 0; j < 2 * V; j++) e[s][j] = e[s][j] * rstd * (key ? w[1][s][j] : w[0][s][j]);
-          turn<V, INTER>(e[s], cs[s], sn[s], 1.0f, turned[s]);
+          for (int j = 0; j < V; j++) e[s][j] = mul2(mul2(e[s][j], rstd), ws[s][j / 2][gl].v[j % 2]);
+          if (turned[s]) angle[s].template turn<false>(e[s]);
         }
       }
+      if (live) {
+#pragma unroll
+        for (int s = 0; s < S; s++)
+          if (slot[s].a >= 0) store_pairs<T, V>(y + slot[s].a, y + slot[s].b, e[s]);
+      }
+      y += G * a.d;
+    }
+  };
+  while (now.u < units) {
+    if (now.t != token) {
+      // The token's cosines and sines, each computed by one lane.
+      token = now.t;
+      const double at = half ? (double)a.pos[token] : 0.0;
+      __syncwarp();
+      for (int p = lane; p < half; p += 32) {
+        const double turns = at * s_freq[p];
+        float sine, cosine;
+        sincospif((float)(2.0 * (turns - rint(turns))), &sine, &cosine);
+        s_turn[warp][p] = make_float2(cosine, sine);
+      }
+      __syncwarp();
 #pragma unroll
       for (int s = 0; s < S; s++)
-        if (live && slot[s].a >= 0) {
-          store_pack<T, V>(y + slot[s].a, &e[s][0]);
-          store_pack<T, V>(y + slot[s].b, &e[s][V]);
-        }
+        if (turned[s]) angle[s].set(&s_turn[warp][slot[s].first]);
     }
+    if (now.which == 0)
+      pass(a.q, dw[0], s_w[0]);
+    else
+      pass(a.k, dw[1], s_w[1]);
+    now.which++;
+    enter(now);
   }
-  if (!BACK || !a.partial) return;
-  // The block's sums for each column, its groups' in order.
-  __shared__ float s_dw[kWarps][kMostD];
+  copies_but<0>();
+  if constexpr (BACK) {
+    if (!a.partial) return;
+    // The block's sums for each column, its groups' in order.
+    float(*s_dw)[kMostD] = reinterpret_cast<float(*)[kMostD]>(s_raw);
 #pragma unroll
-  for (int h = 0; h < 2; h++) {
-    __syncthreads();
+    for (int h = 0; h < 2; h++) {
+      __syncthreads();
 #pragma unroll
-    for (int s = 0; s < S; s++)
+      for (int s = 0; s < S; s++) {
+        float v[2 * V];
 #pragma unroll
-      for (int j = 0; j < 2 * V; j++) {
-        float v = dw[h][s][j];
+        for (int q = 0; q < V; q++) unpack_f2(dw[h][s][q], v[2 * q], v[2 * q + 1]);
 #pragma unroll
-        for (int o = L; o < 32; o <<= 1) v += __shfl_xor_sync(~0u, v, o);
-        if (group == 0 && slot[s].a >= 0) s_dw[warp][j < V ? slot[s].a + j : slot[s].b + j - V] = v;
+        for (int j = 0; j < 2 * V; j++) {
+#pragma unroll
+          for (int o = L; o < 32; o <<= 1) v[j] += __shfl_xor_sync(~0u, v[j], o);
+          if (group == 0 && slot[s].a >= 0) s_dw[warp][j < V ? slot[s].a + j : slot[s].b + j - V] = v[j];
+        }
       }
-    __syncthreads();
-    for (int c = threadIdx.x; c < a.d; c += kThreads) {
-      float v = 0.0f;
+      __syncthreads();
+      for (int c = threadIdx.x; c < a.d; c += kThreads) {
+        float v = 0.0f;
 #pragma unroll
-      for (int i = 0; i < kWarps; i++) v += s_dw[i][c];
-      a.partial[((int64_t)blockIdx.x * 2 + h) * a.d + c] = v;
+        for (int i = 0; i < kWarps; i++) v += s_dw[i][c];
+        a.partial[((int64_t)blockIdx.x * 2 + h) * a.d + c] = v;
+      }
     }
   }
 }
@@ -261,8 +432,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_finish_kernel(const float* p
   grid_wait();
   const int c = blockIdx.x * 8 + (threadIdx.x & 7), r = threadIdx.x >> 3;
   float v = 0.0f;
-  if (c < 2 * d)
+  if (c < 2 * d) {
+#pragma unroll 8
     for (int b = r; b < blocks; b += kFinishRows) v += partial[(int64_t)b * 2 * d + c];
+  }
   s[r][threadIdx.x & 7] = v;
   __syncthreads();
   if (r == 0 && c < 2 * d) {
@@ -274,7 +447,7 @@ __global__ void __launch_bounds__(256) qk_norm_rope_finish_kernel(const float* p
   }
 }
 
-template <class T, class P, int V, int L, int S, bool INTER, bool BACK>
+template <class T, int V, int L, int S, bool INTER, bool BACK>
 int launch(RopeArgs& a, int sms, cudaStream_t s, int* blocks) {
   const int heads = a.q.n + a.k.n, at_once = 32 / L;
   // A warp takes all heads of a token where tokens are enough to fill the
@@ -286,49 +459,54 @@ int launch(RopeArgs& a, int sms, cudaStream_t s, int* blocks) {
   a.per = per * at_once;
   a.splits = (heads + a.per - 1) / a.per;
   int64_t grid = (a.tokens * a.splits + kWarps - 1) / kWarps;
-  const int64_t most = BACK ? kMostBlocks : (int64_t)sms * 32;
+  const int64_t most = std::min((int64_t)sms * blocks_of<S, V, BACK>(), (int64_t)kMostBlocks);
   if (grid > most) grid = most;
   *blocks = (int)grid;
-  VRS_TRY(launch_after(qk_norm_rope_kernel<T, P, V, L, S, INTER, BACK>, (unsigned)grid, kThreads, 0, s, a));
+  VRS_TRY(launch_after(qk_norm_rope_kernel<T, V, L, S, INTER, BACK>, (unsigned)grid, kThreads, 0, s, a));
   count_launch();
   return VRS_OK;
 }
 
-template <class T, class P, int V, bool INTER, bool BACK>
+template <class T, int V, bool INTER, bool BACK>
 int by_lanes(RopeArgs& a, int sms, cudaStream_t s, int* blocks) {
   const int slots = (a.d / 2 + V - 1) / V;
-  if (slots <= 8) return launch<T, P, V, 8, 1, INTER, BACK>(a, sms, s, blocks);
-  if (slots <= 16) return launch<T, P, V, 16, 1, INTER, BACK>(a, sms, s, blocks);
-  if (slots <= 32) return launch<T, P, V, 32, 1, INTER, BACK>(a, sms, s, blocks);
-  if constexpr (V <= 2) {
-    if (slots <= 64) return launch<T, P, V, 32, 2, INTER, BACK>(a, sms, s, blocks);
-    if constexpr (V == 1) return launch<T, P, V, 32, 4, INTER, BACK>(a, sms, s, blocks);
+  if constexpr (V == 1) {  // (off every wider boundary: one shape of lanes)
+    if (slots <= 32) return launch<T, 1, 32, 1, INTER, BACK>(a, sms, s, blocks);
+    return launch<T, 1, 32, 4, INTER, BACK>(a, sms, s, blocks);
+  } else {
+    if (slots <= 8) return launch<T, V, 8, 1, INTER, BACK>(a, sms, s, blocks);
+    if (slots <= 16) return launch<T, V, 16, 1, INTER, BACK>(a, sms, s, blocks);
+    if (slots <= 32) return launch<T, V, 32, 1, INTER, BACK>(a, sms, s, blocks);
+    if constexpr (V == 2) return launch<T, V, 32, 2, INTER, BACK>(a, sms, s, blocks);
+    return invalid("qk_norm_rope: d is too large");  // (checked before)
   }
-  return invalid("qk_norm_rope: d is too large");  // (checked before)
 }
 
-// V pairs an access where everything divides into it: 8 or 16 bytes a lane.
-template <class T, class P, bool BACK>
-int by_layout(RopeArgs& a, bool interleaved, bool wide, int sms, cudaStream_t s, int* blocks) {
-  constexpr int V = sizeof(T) == 2 ? 4 : 2;
-  if (wide)
-    return interleaved ? by_lanes<T, P, V, true, BACK>(a, sms, s, blocks) : by_lanes<T, P, V, false, BACK>(a, sms, s, blocks);
-  return interleaved ? by_lanes<T, P, 1, true, BACK>(a, sms, s, blocks) : by_lanes<T, P, 1, false, BACK>(a, sms, s, blocks);
+// Accesses of `wide` elements where everything divides into them: 16 bytes, 8, or one element.
+template <class T, bool BACK>
+int by_layout(RopeArgs& a, bool interleaved, int wide, int sms, cudaStream_t s, int* blocks) {
+  constexpr int V = 16 / sizeof(T);
+  if (wide >= V)
+    return interleaved ? by_lanes<T, V, true, BACK>(a, sms, s, blocks) : by_lanes<T, V, false, BACK>(a, sms, s, blocks);
+  if (wide >= V / 2)
+    return interleaved ? by_lanes<T, V / 2, true, BACK>(a, sms, s, blocks)
+                       : by_lanes<T, V / 2, false, BACK>(a, sms, s, blocks);
+  return interleaved ? by_lanes<T, 1, true, BACK>(a, sms, s, blocks) : by_lanes<T, 1, false, BACK>(a, sms, s, blocks);
 }
 
 template <bool BACK>
-int by_type(RopeArgs& a, int dtype, int param_dtype, bool interleaved, bool wide, int sms, cudaStream_t s, int* blocks) {
-  if (dtype == VRS_F32) return by_layout<float, float, BACK>(a, interleaved, wide, sms, s, blocks);
-  if (dtype == VRS_F16)
-    return param_dtype == VRS_F32 ? by_layout<f16, float, BACK>(a, interleaved, wide, sms, s, blocks)
-                                  : by_layout<f16, f16, BACK>(a, interleaved, wide, sms, s, blocks);
-  return param_dtype == VRS_F32 ? by_layout<bf16, float, BACK>(a, interleaved, wide, sms, s, blocks)
-                                : by_layout<bf16, bf16, BACK>(a, interleaved, wide, sms, s, blocks);
+int by_type(RopeArgs& a, int dtype, bool interleaved, int wide, int sms, cudaStream_t s, int* blocks) {
+  if (dtype == VRS_F32) return by_layout<float, BACK>(a, interleaved, wide, sms, s, blocks);
+  if (dtype == VRS_F16) return by_layout<f16, BACK>(a, interleaved, wide, sms, s, blocks);
+  return by_layout<bf16, BACK>(a, interleaved, wide, sms, s, blocks);
 }
 
-// One array: its alignment in elements is at least V in every stride that counts.
-bool fits(const void* p, int64_t stride, int64_t head, int64_t tokens, int n, int v, int bytes) {
-  return (uintptr_t)p % (v * bytes) == 0 && (tokens <= 1 || stride % v == 0) && (n <= 1 || head % v == 0);
+// The widest access, in elements up to 16 bytes, that every address and stride of
+// an array is a multiple of.
+int widest(const void* p, int64_t stride, int64_t head, int64_t tokens, int n, int bytes) {
+  int v = 16 / bytes;
+  while (v > 1 && ((uintptr_t)p % (v * bytes) || (tokens > 1 && stride % v) || (n > 1 && head % v))) v /= 2;
+  return v;
 }
 
 struct Call {
@@ -363,18 +541,20 @@ int check(const char* who, const Call& c, bool back) {
   return VRS_OK;
 }
 
-RopeArgs args_of(const Call& c, bool back, bool* wide) {
+RopeArgs args_of(const Call& c, bool back, int* wide) {
   RopeArgs a{};
-  const int bytes = dtype_bytes(c.dtype), v = c.dtype == VRS_F32 ? 2 : 4;
-  bool ok = c.d / 2 % v == 0 && c.rotary / 2 % v == 0;
+  const int bytes = dtype_bytes(c.dtype);
+  int v = 16 / bytes;
+  while (v > 1 && (c.d / 2 % v || c.rotary / 2 % v)) v /= 2;
   auto heads = [&](const vrs_heads& x, int64_t n, const void* w, void* y, const vrs_heads* dy) {
     Heads h{x.data, x.stride, x.head_stride, (int)n, w, y, nullptr, 0, 0};
-    ok = ok && fits(x.data, x.stride, x.head_stride, c.tokens, (int)n, v, bytes) && (uintptr_t)y % (v * bytes) == 0;
+    v = std::min({v, widest(x.data, x.stride, x.head_stride, c.tokens, (int)n, bytes),
+                  widest(y, c.d, c.d, c.tokens, (int)n, bytes)});
     if (back) {
       h.dy = dy->data;
       h.dstride = dy->stride;
       h.dhead = dy->head_stride;
-      ok = ok && fits(dy->data, dy->stride, dy->head_stride, c.tokens, (int)n, v, bytes);
+      v = std::min(v, widest(dy->data, dy->stride, dy->head_stride, c.tokens, (int)n, bytes));
     }
     return h;
   };
@@ -384,12 +564,13 @@ RopeArgs args_of(const Call& c, bool back, bool* wide) {
   a.d = (int)c.d;
   a.rotary = (int)c.rotary;
   a.eps = c.eps;
+  a.w_f32 = c.param_dtype == VRS_F32;
   a.inv_d = 1.0f / (float)c.d;
   a.pos = c.positions;
   // base^(-2 i / rotary) / 2 pi
   for (int i = 0; i < a.rotary / 2; i++)
     a.turns[i] = std::pow(c.base, -2.0 * i / (double)a.rotary) / 6.283185307179586476925286766559;
-  *wide = ok;
+  *wide = v;
   return a;
 }
 
@@ -408,13 +589,13 @@ extern "C" int vrs_qk_norm_rope_forward(const vrs_heads* q, int64_t heads, const
                q_weight, k_weight, param_dtype, base,    rotary, interleaved, eps,    q_out, k_out};
   VRS_TRY(check("vrs_qk_norm_rope_forward", c, false));
   if (tokens == 0) return VRS_OK;
-  bool wide = false;
+  int wide = 0;
   RopeArgs a = args_of(c, false, &wide);
   int sms = 0, blocks = 0;
   VRS_TRY(sm_count(&sms));
   cudaStream_t s = (cudaStream_t)cuda_stream;
   ProfToken t = prof_begin("qk_norm_rope_forward", s);
-  const int st = by_type<false>(a, dtype, param_dtype, interleaved != 0, wide, sms, s, &blocks);
+  const int st = by_type<false>(a, dtype, interleaved != 0, wide, sms, s, &blocks);
   prof_end(t, s);
   return st;
 }
@@ -451,13 +632,13 @@ extern "C" int vrs_qk_norm_rope_backward(const vrs_heads* dq_out, const vrs_head
     if (dk_weight) VRS_CUDA(cudaMemsetAsync(dk_weight, 0, bytes, s));
     return VRS_OK;
   }
-  bool wide = false;
+  int wide = 0;
   RopeArgs a = args_of(c, true, &wide);
   a.partial = params ? (float*)workspace : nullptr;
   int sms = 0, blocks = 0;
   VRS_TRY(sm_count(&sms));
   ProfToken t = prof_begin("qk_norm_rope_backward", s);
-  int st = by_type<true>(a, dtype, param_dtype, interleaved != 0, wide, sms, s, &blocks);
+  int st = by_type<true>(a, dtype, interleaved != 0, wide, sms, s, &blocks);
   if (st == VRS_OK && params) {
     const unsigned grid = (unsigned)((2 * d + 7) / 8);
     const float* from = a.partial;
