@@ -1,6 +1,7 @@
 // attention.cu -- the plan of an attention call: checks, tensor maps, each
 // token's sequence, and the launches of attention_fwd.cu and attention_bwd.cu.
 #include <algorithm>
+#include <climits>
 #include <cmath>
 
 #include "attention.cuh"
@@ -11,35 +12,63 @@ namespace {
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
+// A token's sequence, and two spans a tile.
+int64_t sequences_bytes(int64_t tokens) { return up(tokens * 8, 256) + up((tokens + kAttTile - 1) / kAttTile * 32, 256); }
+
 // Each token's sequence [first, past its last): the last bound at or below the
 // token, by bisection. Whatever cu holds, the interval contains the token and
-// lies within 0..tokens.
-__global__ void __launch_bounds__(256) attention_sequences_kernel(const int* cu, int sequences, int tokens, int2* seg,
-                                                                  unsigned* zero) {
+// lies within 0..tokens. A block has a tile and leaves what its rows meet beside it.
+__global__ void __launch_bounds__(kAttTile) attention_sequences_kernel(const int* cu, int sequences, int2* seg, int4* spans,
+                                                                       unsigned* zero, const AttArgs a) {
+  __shared__ int s_span[4][8];
   grid_launch();
   grid_wait();
-  const int t = blockIdx.x * 256 + threadIdx.x;
+  const int tile = blockIdx.x, t = tile * kAttTile + threadIdx.x;
   if (zero && t < 2) zero[t] = 0;
   if (!cu) return;
-  if (t >= tokens) return;
-  int lo = 0, hi = sequences;
-  if (sequences < 1 || cu[0] > t || cu[sequences] <= t) {
-    seg[t] = make_int2(0, 0);
-    return;
+  int2 mine = make_int2(0, 0);
+  if (t < a.tokens) {
+    if (sequences >= 1 && cu[0] <= t && cu[sequences] > t) {
+      int lo = 0, hi = sequences;
+      while (hi - lo > 1) {  // cu[lo] <= t < cu[hi]
+        const int mid = (lo + hi) >> 1;
+        if (cu[mid] <= t)
+          lo = mid;
+        else
+          hi = mid;
+      }
+      mine = make_int2(max(cu[lo], 0), min(cu[hi], a.tokens));
+    }
+    seg[t] = mine;
   }
-  while (hi - lo > 1) {  // cu[lo] <= t < cu[hi]
-    const int mid = (lo + hi) >> 1;
-    if (cu[mid] <= t)
-      lo = mid;
-    else
-      hi = mid;
+#pragma unroll
+  for (int way = 0; way < 2; way++) {
+    const int2 v = t >= a.tokens ? make_int2(0, 0) : way == 0 ? att_limited<true>(a, mine, t) : att_limited<false>(a, mine, t);
+    const bool some = v.x < v.y, none = !some && t < a.tokens;
+    const int r[4] = {__reduce_min_sync(~0u, some ? v.x : INT_MAX), __reduce_max_sync(~0u, some ? v.y : 0),
+                      __reduce_max_sync(~0u, some ? v.x : none ? INT_MAX : 0),  // (a row that meets nothing: no tile whole)
+                      __reduce_min_sync(~0u, some ? v.y : INT_MAX)};
+    if ((threadIdx.x & 31) == 0)
+      for (int i = 0; i < 4; i++) s_span[threadIdx.x >> 5][way * 4 + i] = r[i];
   }
-  seg[t] = make_int2(max(cu[lo], 0), min(cu[hi], tokens));
+  __syncthreads();
+  if (threadIdx.x < 2) {
+    const int w = threadIdx.x * 4;
+    int lo = INT_MAX, hi = 0, low_max = 0, high_min = INT_MAX;
+    for (int i = 0; i < 4; i++) {
+      lo = min(lo, s_span[i][w]);
+      hi = max(hi, s_span[i][w + 1]);
+      low_max = max(low_max, s_span[i][w + 2]);
+      high_min = min(high_min, s_span[i][w + 3]);
+    }
+    spans[threadIdx.x * a.tiles + tile] =
+        make_int4(hi > 0 ? lo / kAttTile : 0, (hi + kAttTile - 1) / kAttTile, low_max, high_min);
+  }
 }
 
 // d, heads and tokens as a 3-D map of 64 x 1 x `rows`, the smaller stride first.
-int make_map(CUtensorMap* m, bool f16, const vrs_heads& h, int64_t tokens, int64_t heads, int64_t d, int rows,
-             int* tokens_last) {
+int make_map(CUtensorMap* m, bool f16, const vrs_heads& h, int64_t tokens, int64_t heads, int64_t d, int* tokens_last) {
+  constexpr int rows = kAttTile;
   auto fn = tensor_map_encoder();
   if (!fn) {
     set_error(VRS_ERR_DRIVER, "cuTensorMapEncodeTiled unavailable");
@@ -113,9 +142,13 @@ int start(const Call& c, void* seg, unsigned* zero, AttArgs& a, cudaStream_t s) 
   a.seg = nullptr;
   VRS_TRY(error_word(&a.err));
   if (!c.cu && !zero) return VRS_OK;
-  if (c.cu) a.seg = (const int2*)seg;
-  VRS_TRY(launch_after(attention_sequences_kernel, c.cu ? (unsigned)((c.tokens + 255) / 256) : 1u, 256, 0, s,
-                       (const int*)c.cu, (int)c.sequences, (int)c.tokens, (int2*)seg, zero));
+  int4* spans = (int4*)((char*)seg + up(c.tokens * 8, 256));
+  if (c.cu) {
+    a.seg = (const int2*)seg;
+    a.spans = spans;
+  }
+  VRS_TRY(launch_after(attention_sequences_kernel, c.cu ? (unsigned)a.tiles : 1u, kAttTile, 0, s, (const int*)c.cu,
+                       (int)c.sequences, (int2*)seg, spans, zero, a));
   count_launch();
   return VRS_OK;
 }
@@ -133,7 +166,7 @@ extern "C" int vrs_attention_forward_workspace(int64_t tokens, int64_t* out_byte
   using namespace vrs::ops;
   if (tokens < 0 || tokens > (1ll << 31) - 512 || !out_bytes)
     return invalid("vrs_attention_forward_workspace: tokens must be in 0..2^31 - 512, out_bytes not null");
-  *out_bytes = up(tokens * 8, 256);
+  *out_bytes = sequences_bytes(tokens);
   return VRS_OK;
 }
 
@@ -161,14 +194,16 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
   const bool f16 = dtype == VRS_F16;
   AttFwdMaps maps;
   AttFwd a{};
-  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, kAttTile, &a.q_last));
-  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, kAttTile, &a.k_last));
-  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, kAttTile, &a.v_last));
-  VRS_TRY(make_map(&maps.out, f16, *out, tokens, heads, d, 32, &a.out_last));
+  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, &a.q_last));
+  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, &a.k_last));
+  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, &a.v_last));
   ProfToken t = prof_begin("attention_forward", s);
   int st = start(c, workspace, nullptr, a, s);
   if (st == VRS_OK) {
     a.lse = lse;
+    a.r1 = (uint16_t*)out->data;
+    a.r1s = out->stride;
+    a.r1h = out->head_stride;
     a.v = (const uint16_t*)v->data;
     a.vs = v->stride;
     a.vh = v->head_stride;
@@ -203,7 +238,7 @@ BwdSpace bwd_space(int64_t tokens, int64_t heads) {
   BwdSpace p;
   p.padded = up(tokens, kAttTile);
   p.seg = 0;
-  p.lse2 = up(tokens * 8, 256);
+  p.lse2 = sequences_bytes(tokens);
   p.delta = p.lse2 + heads * p.padded * 4;  // (padded: a multiple of 128)
   p.bound = p.delta + heads * p.padded * 4;
   p.bytes = p.bound + 256;
@@ -254,21 +289,12 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
   VRS_TRY(sm_count(&sms));
   const bool f16 = dtype == VRS_F16;
   char* ws = (char*)workspace;
-  AttBwdMaps maps{}, maps_q;
-  AttBwd a{}, aq;
-  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, kAttTile, &a.q_last));
-  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, kAttTile, &a.k_last));
-  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, kAttTile, &a.v_last));
-  VRS_TRY(make_map(&maps.dout, f16, *dout, tokens, heads, d, kAttTile, &a.dout_last));
-  a.out1_last = a.out2_last = 0;
-  maps.out1 = maps.out2 = maps.q;
-  maps_q = maps;
-  int dq_last = 0;
-  if (dq) VRS_TRY(make_map(&maps_q.out1, f16, *dq, tokens, heads, d, 32, &dq_last));
-  if (dk) {
-    VRS_TRY(make_map(&maps.out1, f16, *dk, tokens, kv_heads, d, 32, &a.out1_last));
-    VRS_TRY(make_map(&maps.out2, f16, *dv, tokens, kv_heads, d, 32, &a.out2_last));
-  }
+  AttBwdMaps maps;
+  AttBwd a{};
+  VRS_TRY(make_map(&maps.q, f16, *q, tokens, heads, d, &a.q_last));
+  VRS_TRY(make_map(&maps.k, f16, *k, tokens, kv_heads, d, &a.k_last));
+  VRS_TRY(make_map(&maps.v, f16, *v, tokens, kv_heads, d, &a.v_last));
+  VRS_TRY(make_map(&maps.dout, f16, *dout, tokens, heads, d, &a.dout_last));
   ProfToken t = prof_begin("attention_backward", s);
   unsigned* bound = f16 ? (unsigned*)(ws + p.bound) : nullptr;
   int st = start(c, ws + p.seg, bound, a, s);
@@ -299,13 +325,20 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
   const int dp = d <= 64 ? 64 : 128;
   if (st == VRS_OK && dk) {
     a.items = a.tiles * (int)kv_heads;
+    a.r1 = (uint16_t*)dk->data;
+    a.r1s = dk->stride;
+    a.r1h = dk->head_stride;
+    a.r2 = (uint16_t*)dv->data;
+    a.r2s = dv->stride;
+    a.r2h = dv->head_stride;
     st = launch_attention_backward(f16, dp, true, maps, a, sms, s);
   }
   if (st == VRS_OK && dq) {
-    aq = a;
-    aq.items = a.tiles * (int)heads;
-    aq.out1_last = dq_last;
-    st = launch_attention_backward(f16, dp, false, maps_q, aq, sms, s);
+    a.items = a.tiles * (int)heads;
+    a.r1 = (uint16_t*)dq->data;
+    a.r1s = dq->stride;
+    a.r1h = dq->head_stride;
+    st = launch_attention_backward(f16, dp, false, maps, a, sms, s);
   }
   prof_end(t, s);
   return st;

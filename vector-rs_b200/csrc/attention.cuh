@@ -33,9 +33,13 @@ struct AttArgs {
   int causal;
   int seq_len;        // of every sequence, where seg is null
   const int2* seg;    // per token: its sequence's first token and the one past its last
+  const int4* spans;  // beside seg: per tile what its rows meet, as queries, then as keys
   float c2;           // scale * log2 e
   float scale;
   float* lse;         // [heads][tokens]
+  // Results: out; dk or dq, and dv.
+  uint16_t *r1, *r2;
+  int64_t r1s, r1h, r2s, r2h;
   // Values that are not finite are read again from here.
   const uint16_t *q, *k, *v, *dout;
   int64_t qs, qh, ks, kh, vs, vh, dos, doh;
@@ -48,8 +52,21 @@ __device__ __forceinline__ float att_ex2(float x) {
   return r;
 }
 
-// Rows [lo, hi) that row i meets: the keys of a query (KEYS), or the queries of a
-// key. Empty for a row that no sequence holds. Whatever seg says, within 0..tokens.
+// Rows [lo, hi) that row i of a sequence meets: the keys of a query (KEYS), or the
+// queries of a key.
+template <bool KEYS>
+__device__ __forceinline__ int2 att_limited(const AttArgs& a, int2 r, int i) {
+  if (a.causal) {
+    if (KEYS)
+      r.y = min(r.y, i + 1);
+    else
+      r.x = max(r.x, i);
+  }
+  return r.x < r.y ? r : make_int2(0, 0);
+}
+
+// The same of row i, whose sequence is looked up. Empty for a row that no sequence
+// holds. Whatever seg says, within 0..tokens.
 template <bool KEYS>
 __device__ __forceinline__ int2 att_interval(const AttArgs& a, int i) {
   if (i >= a.tokens) return make_int2(0, 0);
@@ -60,46 +77,32 @@ __device__ __forceinline__ int2 att_interval(const AttArgs& a, int i) {
     r.x = i / a.seq_len * a.seq_len;
     r.y = r.x + a.seq_len;
   }
-  if (a.causal) {
-    if (KEYS)
-      r.y = min(r.y, i + 1);
-    else
-      r.x = max(r.x, i);
-  }
-  return r.x < r.y ? r : make_int2(0, 0);
+  return att_limited<KEYS>(a, r, i);
 }
 
-// What a tile of 128 rows meets; by a whole warp.
+// What a tile of 128 rows meets.
 struct AttSpan {
   int first, end;        // tiles [first, end) with a row that some row here meets
   int low_max, high_min;  // rows [low_max, high_min) are met by all rows here
 };
+// By a whole warp, to which the result is uniform.
 template <bool KEYS>
 __device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
-  const int lane = threadIdx.x & 31;
-  int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
-#pragma unroll
-  for (int r = 0; r < 4; r++) {
-    const int i = tile * kAttTile + r * 32 + lane;
-    const int2 v = att_interval<KEYS>(a, i);
-    if (v.x < v.y) {
-      lo_min = min(lo_min, v.x);
-      lo_max = max(lo_max, v.x);
-      hi_min = min(hi_min, v.y);
-      hi_max = max(hi_max, v.y);
-    } else if (i < a.tokens) {
-      lo_max = INT_MAX;  // a row that meets nothing
-    }
-  }
-  lo_min = __reduce_min_sync(~0u, lo_min);
-  lo_max = __reduce_max_sync(~0u, lo_max);
-  hi_min = __reduce_min_sync(~0u, hi_min);
-  hi_max = __reduce_max_sync(~0u, hi_max);
   AttSpan s;
-  s.first = hi_max > 0 ? lo_min / kAttTile : 0;
-  s.end = (hi_max + kAttTile - 1) / kAttTile;
-  s.low_max = lo_max;
-  s.high_min = hi_min;
+  if (a.seg) {
+    const int4 v = a.spans[KEYS ? tile : a.tiles + tile];
+    s.first = __reduce_min_sync(~0u, v.x);
+    s.end = __reduce_min_sync(~0u, v.y);
+    s.low_max = __reduce_min_sync(~0u, v.z);
+    s.high_min = __reduce_min_sync(~0u, v.w);
+    return s;
+  }
+  const int t0 = tile * kAttTile, last = min(a.tokens, t0 + kAttTile) - 1;
+  const int lo0 = t0 / a.seq_len * a.seq_len, lo1 = last / a.seq_len * a.seq_len;  // sequences of the first and last row
+  s.first = (a.causal && !KEYS ? t0 : lo0) / kAttTile;
+  s.end = ((a.causal && KEYS ? last + 1 : lo1 + a.seq_len) + kAttTile - 1) / kAttTile;
+  s.low_max = a.causal && !KEYS ? last : lo1;
+  s.high_min = a.causal && KEYS ? t0 + 1 : lo0 + a.seq_len;
   return s;
 }
 
@@ -109,7 +112,7 @@ __device__ __forceinline__ bool att_masked(int low_max, int high_min, int t) {
   return t * kAttTile < low_max || (t + 1) * kAttTile > high_min;
 }
 
-// 3-D tiles: 64 elements of one head of 128 (stored: 32) tokens. tokens_last: the
+// 3-D tiles: 64 elements of one head of 128 tokens. tokens_last: the
 // map's dimensions are d, heads, tokens, else d, tokens, heads.
 __device__ __forceinline__ void att_load(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
   asm volatile(
@@ -118,14 +121,6 @@ __device__ __forceinline__ void att_load(void* dst, const CUtensorMap* map, int 
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(bar))
       : "memory");
 }
-__device__ __forceinline__ void att_store(const CUtensorMap* map, const void* src, int x, int y, int z) {
-  asm volatile("cp.async.bulk.tensor.3d.global.shared::cta.bulk_group [%0, {%1, %2, %3}], [%4];" ::"l"(
-                   reinterpret_cast<uint64_t>(map)),
-               "r"(x), "r"(y), "r"(z), "r"(tc::smem_u32(src))
-               : "memory");
-}
-__device__ __forceinline__ void att_store_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
-__device__ __forceinline__ void att_store_wait() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
 __device__ __forceinline__ void att_fence_async() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 // A tile of one head: boxes of 64 elements, one after another.
@@ -264,23 +259,40 @@ __device__ __forceinline__ uint32_t att_clear(uint32_t u) {
   return u;
 }
 
+// x * 0 + acc for two values: stays 0 until one of them is not finite.
+template <bool F16>
+__device__ __forceinline__ void att_probe(uint32_t& acc, uint32_t u) {
+  if (F16)
+    asm("fma.rn.f16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(u), "r"(0u));
+  else
+    asm("fma.rn.bf16x2 %0, %1, %2, %0;" : "+r"(acc) : "r"(u), "r"(0u));
+}
+
 // A warp's share of a tile in shared memory, `part` of `parts`: values that are
 // not finite become 0. Whether there were any. (What the swizzle does within a
-// row is of no concern.)
+// row is of no concern.) Looking takes one instruction a word; only where it finds
+// something is the share gone through again.
 template <int DP, bool F16>
 __device__ __forceinline__ bool att_clean(uint8_t* tile, int part, int parts) {
   const int lane = threadIdx.x & 31;
   uint4* p = reinterpret_cast<uint4*>(tile);
   constexpr int kVecs = DP * kAttTile * 2 / 16;
-  uint32_t any = 0;
-#pragma unroll 4
+  uint32_t acc[4] = {0, 0, 0, 0};
+#pragma unroll 8
   for (int i = part * 32 + lane; i < kVecs; i += parts * 32) {
     const uint4 u = p[i];
-    const uint32_t bad = att_not_finite<F16>(u.x) | att_not_finite<F16>(u.y) | att_not_finite<F16>(u.z) | att_not_finite<F16>(u.w);
-    if (bad) p[i] = make_uint4(att_clear<F16>(u.x), att_clear<F16>(u.y), att_clear<F16>(u.z), att_clear<F16>(u.w));
-    any |= bad;
+    att_probe<F16>(acc[0], u.x);
+    att_probe<F16>(acc[1], u.y);
+    att_probe<F16>(acc[2], u.z);
+    att_probe<F16>(acc[3], u.w);
   }
-  return __any_sync(~0u, any != 0);
+  if (!__any_sync(~0u, ((acc[0] | acc[1] | acc[2] | acc[3]) & 0x7fff7fffu) != 0)) return false;
+#pragma unroll 1
+  for (int i = part * 32 + lane; i < kVecs; i += parts * 32) {
+    const uint4 u = p[i];
+    p[i] = make_uint4(att_clear<F16>(u.x), att_clear<F16>(u.y), att_clear<F16>(u.z), att_clear<F16>(u.w));
+  }
+  return true;
 }
 
 // Adds to 32 results of a row (elements [c0, c0 + 32) of d) the values that are
@@ -310,34 +322,33 @@ __device__ __forceinline__ void att_add_not_finite(float* o, const uint16_t* m, 
   }
 }
 
-// Row `row` of a staging tile (boxes of 64 elements, 128-byte swizzle): 32
-// results from element c0 on in 16 bits.
+// 32 results of a row, elements [c, c + 32) of d, in 16 bits. Whole 32-byte sectors
+// where rows start on them: a lane has a row, so nothing else makes up a sector.
 template <bool F16>
-__device__ __forceinline__ void att_stage_row(uint8_t* tile, int row, int c0, const float* w) {
-  uint8_t* to = tile + (c0 >> 6) * kAttBox + row * 128;
-  const int j0 = (c0 & 63) >> 3;
+__device__ __forceinline__ void att_store_row(uint16_t* row, int c, int d, const float* o) {
+  uint32_t w[16];
+#pragma unroll
+  for (int j = 0; j < 16; j++) w[j] = att_pack2<F16>(o[2 * j], o[2 * j + 1]);
+  uint16_t* to = row + c;
+  if (c + 32 <= d && ((uintptr_t)to & 31) == 0) {
+#pragma unroll
+    for (int h = 0; h < 2; h++)
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 16 * h), "r"(w[8 * h]),
+                   "r"(w[8 * h + 1]), "r"(w[8 * h + 2]), "r"(w[8 * h + 3]), "r"(w[8 * h + 4]), "r"(w[8 * h + 5]),
+                   "r"(w[8 * h + 6]), "r"(w[8 * h + 7])
+                   : "memory");
+    return;
+  }
 #pragma unroll
   for (int q = 0; q < 4; q++)
-    *reinterpret_cast<uint4*>(to + (((j0 + q) ^ (row & 7)) << 4)) =
-        make_uint4(att_pack2<F16>(w[8 * q], w[8 * q + 1]), att_pack2<F16>(w[8 * q + 2], w[8 * q + 3]),
-                   att_pack2<F16>(w[8 * q + 4], w[8 * q + 5]), att_pack2<F16>(w[8 * q + 6], w[8 * q + 7]));
+    if (c + 8 * q < d) *reinterpret_cast<uint4*>(to + 8 * q) = make_uint4(w[4 * q], w[4 * q + 1], w[4 * q + 2], w[4 * q + 3]);
 }
 
-// A warp's 32 rows of a staging tile to memory; the wait is for the reads only.
-template <int DP>
-__device__ __forceinline__ void att_store_rows(const AttArgs& a, const CUtensorMap* map, int tokens_last, uint8_t* tile,
-                                               int row, int head, int token) {
-  att_fence_async();
-  __syncwarp();
-  if ((threadIdx.x & 31) == 0 && token < a.tokens) {
-#pragma unroll
-    for (int b = 0; b < DP / 64; b++)
-      if (b * 64 < a.d)
-        att_store(map, tile + b * kAttBox + row * 128, b * 64, tokens_last ? head : token, tokens_last ? token : head);
-    att_store_commit();
-    att_store_wait();
-  }
-  __syncwarp();
+// Which of 32 columns from c0 on lie in [off, off + len): bit by bit.
+__device__ __forceinline__ uint32_t att_bits(int off, int len, int c0) {
+  const int lo = min(max(off - c0, 0), 32), hi = min(max(off + len - c0, 0), 32);
+  const uint32_t below_hi = hi < 32 ? (1u << hi) - 1 : ~0u, below_lo = lo < 32 ? (1u << lo) - 1 : ~0u;
+  return below_hi & ~below_lo;
 }
 
 // Set-up that the kernels share: dynamic shared memory on a 1,024-byte boundary.
@@ -352,22 +363,22 @@ __device__ __forceinline__ uint8_t* att_align(uint8_t* p) {
 enum AttPairing { kAttSingle = 0, kAttTwoHeads = 1, kAttTwoTiles = 2 };
 
 struct AttFwdMaps {
-  CUtensorMap q, k, v, out;
+  CUtensorMap q, k, v;
 };
 struct AttFwd : AttArgs {
   int pairing, items;
-  int q_last, k_last, v_last, out_last;  // maps whose last dimension is the tokens
+  int q_last, k_last, v_last;  // maps whose last dimension is the tokens
 };
 int launch_attention_forward(bool f16, int dp, const AttFwdMaps& maps, const AttFwd& a, int sms, cudaStream_t s);
 
 // The backward pass: statistics of the query rows, then a kernel for dk and dv
 // (items are tiles of keys) and one for dq (tiles of queries).
 struct AttBwdMaps {
-  CUtensorMap q, k, v, dout, out1, out2;  // out1: dk or dq, out2: dv
+  CUtensorMap q, k, v, dout;
 };
 struct AttBwd : AttArgs {
   int items;
-  int q_last, k_last, v_last, dout_last, out1_last, out2_last;
+  int q_last, k_last, v_last, dout_last;
   int padded;             // tokens, up to whole tiles
   const float* lse2;      // [heads][padded]: lse log2 e, +inf where nothing is seen
   const float* delta;     // [heads][padded]

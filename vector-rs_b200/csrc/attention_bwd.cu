@@ -65,7 +65,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t TILE = tile_bytes<DP>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = att_align(smem_raw);
-  uint8_t* s_a = smem;               // the rows' two tiles (k, v or q, dout); then the results
+  uint8_t* s_a = smem;               // the rows' two tiles (k, v or q, dout)
   uint8_t* s_b = smem + 2 * TILE;    // ring of pairs of tiles (q, dout or k, v)
   float* s_stat = (float*)(s_b + 2 * ST * TILE);  // [ST][lse2, delta][128]
   uint64_t* bars = (uint64_t*)((uint8_t*)s_stat + ST * kStatBytes);
@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   uint64_t* done = empty + ST;       // [ST] scores and dp are multiplied
   uint64_t* clean = done + ST;       // [ST][2] the pair's tiles are clean
   uint64_t* a_full = clean + 2 * ST;
-  uint64_t* a_empty = a_full + 1;    // the results have left
+  uint64_t* a_empty = a_full + 1;    // all scores and dp are multiplied
   uint64_t* s_full = a_empty + 1;
   uint64_t* p_full = s_full + 1;     // scores read, and p written (KEYS)
   uint64_t* dp_full = p_full + 1;
@@ -95,7 +95,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       mbar_init(&clean[2 * s + 1], 2);
     }
     mbar_init(a_full, 1);
-    mbar_init(a_empty, 8);
+    mbar_init(a_empty, 1);
     mbar_init(s_full, 1);
     mbar_init(p_full, kCompute / 32);
     mbar_init(dp_full, 1);
@@ -111,8 +111,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
     prefetch_tmap(&maps.dout);
-    prefetch_tmap(&maps.out1);
-    if (KEYS) prefetch_tmap(&maps.out2);
   }
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
   tc_fence_before();
@@ -202,13 +200,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         mma_commit(s_full);
       }
     };
-    auto dps = [&](int st) {  // rows x (dout or v)
+    auto dps = [&](int st, bool last) {  // rows x (dout or v)
       if (lead) {
         const uint64_t bd = bk + st * PAIR + (TILE >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(dp_full);
         mma_commit(&done[st]);
+        if (last) mma_commit(a_empty);
       }
     };
     // (p or ds over its own columns, each half of a row in its half of them) x (tile `second` of the pair)
@@ -226,11 +225,14 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (The rows are waited for where nothing is multiplied too: a wait for the
       // next ones that came before these have would not see the difference.)
       wait(a_full, a_use++, 63);
-      if (total == 0) continue;
+      if (total == 0) {
+        if (lead) mbar_arrive(a_empty);
+        continue;
+      }
       wait(&full[use % ST], use / ST, 64);
       tc_fence_after();
       scores(use % ST);
-      dps(use % ST);
+      dps(use % ST, total == 1);
       int t = r.first;
 #pragma unroll 1
       for (int i = 0; i < total; i++, use++, p_use++) {
@@ -256,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         product(kCol1, kColDp, st, 0, i > 0);
         if (lead) mma_commit(&empty[st]);
         if (more)
-          dps(next);
+          dps(next, i + 2 == total);
         else
           if (lead) mma_commit(r_full);
         if (++t == r.end) t = r.first;
@@ -311,27 +313,72 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + kColS + half * 64, tdp = tmem + lanes + kColDp + half * 64;
     const float gain = F16 ? gain_of(a.bound) : 1.0f;
     const float ds_scale = F16 ? gain * 0x1p-14f : 1.0f;
-    int use = 0, s_use = 0, a_use = 0, r_use = 0, count = 0;
+    int use = 0, s_use = 0, r_use = 0, count = 0;
     bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const int tile = tile_of(id), head = id % heads;
-      const AttSpan r = att_span<!KEYS>(a, tile);
-      const int total = max(0, r.end - r.first) * per;
-      const int i_row = tile * kAttTile + row;
-      const int2 seen = att_interval<!KEYS>(a, i_row);
-      const unsigned len = (unsigned)(seen.y - seen.x);
-      float lse2 = 0.0f, delta = 0.0f;
+    // What an item means to this thread. The next one's is found before this one's
+    // results are waited for.
+    struct Mine {
+      int tile, head, first, end, total, row;
+      int2 seen;
+      float lse2, delta;
+    };
+    auto mine_at = [&](int id) {
+      Mine m;
+      m.tile = tile_of(id);
+      m.head = id % heads;
+      const AttSpan r = att_span<!KEYS>(a, m.tile);
+      m.first = r.first;
+      m.end = r.end;
+      m.total = max(0, r.end - r.first) * per;
+      m.row = m.tile * kAttTile + row;
+      m.seen = att_interval<!KEYS>(a, m.row);
+      m.lse2 = m.delta = 0.0f;
       if (!KEYS) {
-        const int64_t at = (int64_t)head * a.padded + i_row;
-        lse2 = a.lse2[at];
-        delta = a.delta[at];
+        const int64_t at = (int64_t)m.head * a.padded + m.row;
+        m.lse2 = a.lse2[at];
+        m.delta = a.delta[at];
       }
-      int t = r.first;
+      return m;
+    };
+    Mine next = mine_at(blockIdx.x);
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Mine it = next;
+      const int head = it.head, total = it.total, i_row = it.row;
+      const int2 seen = it.seen;
+      const int len = seen.y - seen.x;
+      const float lse2 = it.lse2, delta = it.delta;
+      int t = it.first;
       for (int i = 0; i < total; i++, use++) {
         const float* stat = s_stat + use % ST * 2 * kAttTile + half * 64;
         ok = att_wait_warp(s_full, s_use & 1, s_abort, a.err, 72);
         if (!ok) break;
         tc_fence_after();
+        const int off = seen.x - t * kAttTile - half * 64;  // of this half of the tile
+        if (__all_sync(~0u, off >= 64 || off + len <= 0)) {
+          // None of these rows meets any of it.
+          const uint32_t zero[16] = {};
+          if (KEYS) {
+            att_tm_store16(ts, zero);
+            att_tm_store16(ts + 16, zero);
+            att_tm_store_wait();
+          }
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(p_full);
+          ok = att_wait_warp(dp_full, s_use & 1, s_abort, a.err, 74);
+          if (!ok) break;
+          s_use++;
+          tc_fence_after();
+          att_tm_store16(tdp, zero);
+          att_tm_store16(tdp + 16, zero);
+          att_tm_store_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(ds_full);
+          if (++t == it.end) t = it.first;
+          continue;
+        }
+        const bool whole = __all_sync(~0u, off <= 0 && off + len >= 64);
         float p[64];
         att_tm_load(ts, p);
         att_tm_load(ts + 32, p + 32);
@@ -364,10 +411,12 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
           for (int j = 0; j < 4; j++) p[c + j] = att_ex2(e[j]);
         }
-        const int off = seen.x - t * kAttTile;
-        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+        uint32_t in[2] = {~0u, ~0u};
+        if (!whole) {
+          in[0] = att_bits(off, len, 0);
+          in[1] = att_bits(off, len, 32);
 #pragma unroll
-          for (int c = 0; c < 64; c++) p[c] = (unsigned)(c + half * 64 - off) < len ? p[c] : 0.0f;
+          for (int c = 0; c < 64; c++) p[c] = in[c >> 5] & (1u << (c & 31)) ? p[c] : 0.0f;
         }
         if (KEYS) {
 #pragma unroll
@@ -417,11 +466,11 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // Masked places: p is 0, but dp and delta may hold anything.
-        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+        if (!whole) {
 #pragma unroll
           for (int c = 0; c < 32; c++) {
-            const bool x = (unsigned)(2 * c + half * 64 - off) < len, y = (unsigned)(2 * c + 1 + half * 64 - off) < len;
-            w[c] &= (x ? 0xffffu : 0u) | (y ? 0xffff0000u : 0u);
+            const uint32_t two = in[c >> 4] >> (2 * c & 31) & 3;
+            w[c] &= (two & 1 ? 0xffffu : 0u) | (two & 2 ? 0xffff0000u : 0u);
           }
         }
         att_tm_store16(tdp, w);
@@ -430,28 +479,25 @@ __global__ void __launch_bounds__(kThreads, 1)
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(ds_full);
-        if (++t == r.end) t = r.first;
+        if (++t == it.end) t = it.first;
       }
       if (!ok) break;
-      // Results: dk by the first four warps and dv by the others; dq by the first
-      // four (d up to 64), or half its columns each.
-      if (total == 0)
-        ok = att_wait_warp(a_full, a_use & 1, s_abort, a.err, 75);
-      else
-        ok = att_wait_warp(r_full, r_use & 1, s_abort, a.err, 76);
-      if (!ok) break;
-      a_use++;
-      if (total > 0) r_use++;
-      tc_fence_after();
+      // Results: dk by the first four warps and dv by the others, or half of dq's columns each.
+      if (id + (int)gridDim.x < a.items) next = mine_at(id + gridDim.x);
+      if (total > 0) {
+        ok = att_wait_warp(r_full, r_use++ & 1, s_abort, a.err, 76);
+        if (!ok) break;
+        tc_fence_after();
+      }
       const bool flagged = total > 0 && s_flag[count % kAttFlags];
       if (total > 0) count++;
       const bool dv = KEYS && half;
       const uint32_t from = tmem + lanes + (dv ? kCol2 : kCol1);
       const float f = dv ? (F16 ? 0x1p-14f : 1.0f) : a.scale / gain;
-      uint8_t* stage = s_a + (dv ? TILE : 0);
-      const int c0 = KEYS || DP == 64 ? 0 : half * 64, c1 = KEYS ? DP : DP == 64 ? (half ? 0 : 64) : c0 + 64;
+      uint16_t* to = dv ? a.r2 + i_row * a.r2s + head * a.r2h : a.r1 + i_row * a.r1s + head * a.r1h;
+      const int c0 = KEYS ? 0 : half * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
 #pragma unroll 1
-      for (int c = c0; c < c1; c += 32) {
+      for (int c = c0; c < c1 && c < a.d; c += 32) {
         float o[32];
         if (total == 0) {
 #pragma unroll
@@ -473,22 +519,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
           }
         }
-        att_stage_row<F16>(stage, row, c, o);
+        if (i_row < a.tokens) att_store_row<F16>(to, c, a.d, o);
       }
       tc_fence_before();
-      att_fence_async();
-      __syncwarp();
-      const int token = tile * kAttTile + quad * 32;
-      if (lane == 0 && token < a.tokens && c0 < c1) {
-        const CUtensorMap* map = dv ? &maps.out2 : &maps.out1;
-        const int last = dv ? a.out2_last : a.out1_last;
-        for (int c = c0; c < c1 && c < a.d; c += 64)
-          att_store(map, stage + (c >> 6) * kAttBox + quad * 32 * 128, c, last ? head : token, last ? token : head);
-        att_store_commit();
-        att_store_wait();
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(a_empty);
     }
   }
   tc_fence_before();

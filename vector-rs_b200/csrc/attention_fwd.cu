@@ -122,14 +122,14 @@ __global__ void __launch_bounds__(kThreads, 1)
   constexpr uint32_t TILE = tile_bytes<DP>();
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = att_align(smem_raw);
-  uint8_t* s_q = smem;              // two tiles; then the results
+  uint8_t* s_q = smem;              // two tiles
   uint8_t* s_kv = smem + 2 * TILE;  // ring of keys and values by turns
   uint64_t* bars = (uint64_t*)(s_kv + ST * TILE);
   uint64_t* full = bars;            // [ST] the tile has come
   uint64_t* empty = full + ST;      // [ST] multiplied, and looked through
   uint64_t* clean = empty + ST;     // [ST] a masked tile of values is clean
   uint64_t* q_full = clean + ST;    // [2]
-  uint64_t* q_empty = q_full + 2;   // [2] the results have left
+  uint64_t* q_empty = q_full + 2;   // [2] all scores are multiplied
   uint64_t* s_full = q_empty + 2;   // [2] scores
   uint64_t* p_full = s_full + 2;    // [2][kParts] P in tensor memory
   uint64_t* o_full = p_full + 2 * kParts;  // [2] all products
@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     for (int s = 0; s < 2; s++) {
       mbar_init(&q_full[s], 1);
-      mbar_init(&q_empty[s], 4);
+      mbar_init(&q_empty[s], 1);
       mbar_init(&s_full[s], 1);
       for (int c = 0; c < kParts; c++) mbar_init(&p_full[s * kParts + c], 4);
       mbar_init(&o_full[s], 1);
@@ -161,7 +161,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     prefetch_tmap(&maps.q);
     prefetch_tmap(&maps.k);
     prefetch_tmap(&maps.v);
-    prefetch_tmap(&maps.out);
   }
   if (warp == kMmaWarp) tmem_alloc(s_tmem, 512);
   tc_fence_before();
@@ -181,8 +180,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const Item it = item_at(a, id);
       const Range r = range_of(a, it);
       if (lane == 0) {
-        // The first keys and values before the queries: their places in the ring
-        // come free earlier than the queries', which the results leave through.
+        // (The first keys and values before the queries: their places are free.)
         const int i0 = 2 * r.t0, i1 = 2 * r.t1;
         for (int i = i0; ok && i <= max(i1 - 1, i0 + 2); i++) {
           if (i == min(i1, i0 + 2)) {
@@ -228,13 +226,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
     uint32_t cleaned = 0;  // parity of each stage's cleanings
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
-    auto scores = [&](int s, int st) {
+    auto scores = [&](int s, int st, bool last) {
       if (lead) {
         const uint64_t ad = qd + s * (TILE >> 4), bd = kd + st * (TILE >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; k++)
           mma_f16(tm + kColS + s * 128, ad + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(&s_full[s]);
+        if (last) mma_commit(&q_empty[s]);
       }
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
@@ -244,14 +243,17 @@ __global__ void __launch_bounds__(kThreads, 1)
       // next ones that came before these have would not see the difference.
 #pragma unroll
       for (int s = 0; s < 2; s++)
-        if (it.live[s]) wait(&q_full[s], q_use[s]++, 43);
+        if (it.live[s]) {
+          wait(&q_full[s], q_use[s]++, 43);
+          if (r.first[s] >= r.end[s] && lead) mbar_arrive(&q_empty[s]);
+        }
       if (r.t0 >= r.t1) continue;
       // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
       wait(&full[use % ST], use / ST, 44);
       tc_fence_after();
 #pragma unroll
       for (int s = 0; s < 2; s++)
-        if (r.active(s, r.t0)) scores(s, use % ST);
+        if (r.active(s, r.t0)) scores(s, use % ST, r.t0 + 1 == r.end[s]);
       if (lead) mma_commit(&empty[use % ST]);
 #pragma unroll 1
       for (int t = r.t0; t < r.t1; t++, use += 2) {
@@ -283,7 +285,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (more && r.active(s, t + 1)) {
             wait(&full[sk], uk / ST, 48);
             tc_fence_after();
-            scores(s, sk);
+            scores(s, sk, t + 2 == r.end[s]);
           }
         }
         if (lead) mma_commit(&empty[sv]);
@@ -337,34 +339,73 @@ __global__ void __launch_bounds__(kThreads, 1)
     const int s = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + s * 128, to = tmem + lanes + kColO + s * 128;
-    uint8_t* stage = s_q + s * TILE;
-    int s_use = 0, o_use = 0, q_use = 0, count = 0;
+    int s_use = 0, o_use = 0, count = 0;
     bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+    // What an item means to this thread. The next one's is found before this one's
+    // result is waited for.
+    struct Mine {
+      bool live, any;   // any: the item has tiles of keys
+      int first, end, head, kv, i;
+      int2 seen;
+    };
+    auto mine_at = [&](int id) {
       const Item it = item_at(a, id);
       const Range r = range_of(a, it);
-      if (!it.live[s]) {
-        if (r.t0 < r.t1) count++;
-        continue;
-      }
-      const int i = it.tile[s] * kAttTile + row;
-      const int2 seen = att_interval<true>(a, i);
+      Mine m;
+      m.live = s ? it.live[1] : it.live[0];
+      m.any = r.t0 < r.t1;
+      m.first = s ? r.first[1] : r.first[0];
+      m.end = s ? r.end[1] : r.end[0];
+      m.head = s ? it.head[1] : it.head[0];
+      m.kv = it.kv;
+      m.i = (s ? it.tile[1] : it.tile[0]) * kAttTile + row;
+      m.seen = att_interval<true>(a, m.i);
+      return m;
+    };
+    Mine next = mine_at(blockIdx.x);
+    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+      const Mine it = next;
+      const bool more = id + (int)gridDim.x < a.items;
       float m = -INFINITY, l = 0.0f;
-      for (int t = r.first[s]; t < r.end[s]; t++) {
+      const int2 seen = it.seen;
+      const int len = seen.y - seen.x;
+      for (int t = it.first; it.live && t < it.end; t++) {
         ok = att_wait_warp(&s_full[s], s_use & 1, s_abort, a.err, 50);
         if (!ok) break;
         s_use++;
         tc_fence_after();
+        // P goes over in parts: the product with the first ones runs while the last
+        // ones are exponentiated. A part's store is waited for after the next
+        // part's exponentials.
+        const auto hand_over = [&](int c) {
+          att_tm_store_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&p_full[s * kParts + c]);
+        };
+        const int off = seen.x - t * kAttTile;
+        if (__all_sync(~0u, off >= kAttTile || off + len <= 0)) {
+          // None of these rows sees any of the tile. (But for the first one, whose
+          // sums are set by the product, nothing is added.)
+          const uint32_t zero[16] = {};
+#pragma unroll
+          for (int c = 0; c < 4; c++) att_tm_store16(ts + 16 * c, zero);
+#pragma unroll
+          for (int c = 0; c < kParts; c++) hand_over(c);
+          continue;
+        }
         float v[128];
 #pragma unroll
         for (int c = 0; c < 4; c++) att_tm_load(ts + 32 * c, v + 32 * c);
 #pragma unroll
         for (int c = 0; c < 4; c++) att_tm_wait(v + 32 * c);
-        const int off = seen.x - t * kAttTile;
-        const unsigned len = (unsigned)(seen.y - seen.x);
-        if (!__all_sync(~0u, off <= 0 && off + (int)len >= kAttTile)) {
+        if (!__all_sync(~0u, off <= 0 && off + len >= kAttTile)) {
 #pragma unroll
-          for (int c = 0; c < 128; c++) v[c] = (unsigned)(c - off) < len ? v[c] : -INFINITY;
+          for (int c = 0; c < 4; c++) {
+            const uint32_t in = att_bits(off, len, 32 * c);
+#pragma unroll
+            for (int j = 0; j < 32; j++) v[32 * c + j] = in & (1u << j) ? v[32 * c + j] : -INFINITY;
+          }
         }
         float top[4];
 #pragma unroll
@@ -380,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           const float f = grow ? att_ex2(m - now) : 1.0f;
           if (grow) m = now;
           l *= f;
-          if (t > r.first[s]) {
+          if (t > it.first) {
 #pragma unroll 1
             for (int c = 0; c < DP; c += 32) {
               float o[32];
@@ -395,15 +436,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         const float sub = m == -INFINITY ? 0.0f : m;
         const F2 cc = pack_f2(a.c2), dd = pack_f2(kLift<F16> - sub);
         F2 sum[2] = {pack_f2(0.0f), pack_f2(0.0f)};
-        // P goes over in parts: the product with the first ones runs while the last
-        // ones are exponentiated. A part's store is waited for after the next
-        // part's exponentials.
-        const auto hand_over = [&](int c) {
-          att_tm_store_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(&p_full[s * kParts + c]);
-        };
 #pragma unroll
         for (int c = 0; c < 4; c++) {
           uint32_t p[16];
@@ -423,40 +455,39 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += sum_f2(add2(sum[0], sum[1]));
       }
       if (!ok) break;
+      if (more) next = mine_at(id + gridDim.x);
       // The row's result: sums over l; 0 for a row that sees nothing.
-      const bool none = r.first[s] >= r.end[s];
-      if (none)
-        ok = att_wait_warp(&q_full[s], q_use & 1, s_abort, a.err, 51);
-      else
-        ok = att_wait_warp(&o_full[s], o_use & 1, s_abort, a.err, 52);
-      if (!ok) break;
-      q_use++;
-      tc_fence_after();
-      if (!none) o_use++;
-      const float f = seen.x < seen.y ? 1.0f / l : 0.0f;
-      const bool flagged = r.t0 < r.t1 && s_flag[count % kAttFlags];
-#pragma unroll 1
-      for (int c = 0; c < DP; c += 32) {
-        float o[32];
-        if (none) {
-#pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = 0.0f;
-        } else {
-          att_tm_load(to + c, o);
-          att_tm_wait(o);
-#pragma unroll
-          for (int j = 0; j < 32; j++) o[j] *= f;
-          if (flagged) att_add_not_finite<F16>(o, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
-        }
-        att_stage_row<F16>(stage, row, c, o);
+      const bool none = it.first >= it.end;
+      if (it.live && !none) {
+        ok = att_wait_warp(&o_full[s], o_use++ & 1, s_abort, a.err, 52);
+        if (!ok) break;
+        tc_fence_after();
       }
-      tc_fence_before();
-      if (i < a.tokens)
-        a.lse[(int64_t)it.head[s] * a.tokens + i] =
-            seen.x < seen.y ? (m - kLift<F16> + log2f(l)) * 0.693147180559945309f : -INFINITY;
-      att_store_rows<DP>(a, &maps.out, a.out_last, stage, quad * 32, it.head[s], it.tile[s] * kAttTile + quad * 32);
-      if (lane == 0) mbar_arrive(&q_empty[s]);
-      if (r.t0 < r.t1) count++;
+      if (it.live) {
+        const float f = len > 0 ? 1.0f / l : 0.0f;
+        const bool flagged = it.any && s_flag[count % kAttFlags];
+        uint16_t* out = a.r1 + it.i * a.r1s + it.head * a.r1h;
+#pragma unroll 1
+        for (int c = 0; c < DP && c < a.d; c += 32) {
+          float o[32];
+          if (none) {
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[j] = 0.0f;
+          } else {
+            att_tm_load(to + c, o);
+            att_tm_wait(o);
+#pragma unroll
+            for (int j = 0; j < 32; j++) o[j] *= f;
+            if (flagged) att_add_not_finite<F16>(o, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
+          }
+          if (it.i < a.tokens) att_store_row<F16>(out, c, a.d, o);
+        }
+        tc_fence_before();
+        if (it.i < a.tokens)
+          a.lse[(int64_t)it.head * a.tokens + it.i] =
+              len > 0 ? (m - kLift<F16> + log2f(l)) * 0.693147180559945309f : -INFINITY;
+      }
+      if (it.any) count++;
     }
   }
   tc_fence_before();
