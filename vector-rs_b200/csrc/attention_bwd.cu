@@ -30,16 +30,25 @@ using namespace vrs::tc;
 constexpr int kThreads = 384;
 constexpr int kCompute = 256;
 constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;  // and 11
+// Registers: 168 a thread at launch; the computing warps take what the others leave
+// (256 x 192 + 128 x 120 of 384 x 168).
+constexpr int kComputeRegs = 192, kOtherRegs = 120;
 constexpr int kColS = 0, kColDp = 128, kCol1 = 256, kCol2 = 384;
 
+// Rings of the tiles that pass by. Each first one (q or k) is held from its scores to
+// the product with ds, each second one (dout or v) from dp to the product with p, or
+// only for dp: rings of their own let each be loaded again as soon as it is free.
 template <int DP>
-constexpr int stages() { return DP == 128 ? 2 : 4; }
+constexpr int stages1() { return DP == 128 ? 3 : 5; }
+template <int DP>
+constexpr int stages2() { return DP == 128 ? 2 : 4; }
 template <int DP>
 constexpr uint32_t tile_bytes() { return DP / 64 * kAttBox; }
-constexpr uint32_t kStatBytes = 2 * kAttTile * 4;
+constexpr uint32_t kStatBytes = kAttTile * 4;
 template <int DP>
 constexpr size_t smem_bytes() {
-  return 1024 + (2 + 2 * stages<DP>()) * (size_t)tile_bytes<DP>() + stages<DP>() * (size_t)kStatBytes + 512;
+  return (2 + stages1<DP>() + stages2<DP>()) * (size_t)tile_bytes<DP>() + (stages1<DP>() + stages2<DP>()) * (size_t)kStatBytes +
+         512;
 }
 static_assert(smem_bytes<128>() <= 232448 && smem_bytes<64>() <= 232448, "above the per-block limit");
 
@@ -61,19 +70,25 @@ __device__ __forceinline__ float gain_of(const unsigned* bound) {
 template <int DP, bool F16, bool KEYS>
 __global__ void __launch_bounds__(kThreads, 1)
     attention_backward_kernel(const __grid_constant__ AttBwdMaps maps, const __grid_constant__ AttBwd a) {
-  constexpr int ST = stages<DP>();
+  constexpr int S1 = stages1<DP>(), S2 = stages2<DP>();
   constexpr uint32_t TILE = tile_bytes<DP>();
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = att_align(smem_raw);
+  extern __shared__ __align__(1024) uint8_t smem[];  // (no byte to spare for aligning it here; checked below)
   uint8_t* s_a = smem;               // the rows' two tiles (k, v or q, dout)
-  uint8_t* s_b = smem + 2 * TILE;    // ring of pairs of tiles (q, dout or k, v)
-  float* s_stat = (float*)(s_b + 2 * ST * TILE);  // [ST][lse2, delta][128]
-  uint64_t* bars = (uint64_t*)((uint8_t*)s_stat + ST * kStatBytes);
-  uint64_t* full = bars;             // [ST] both tiles and the statistics have come
-  uint64_t* empty = full + ST;       // [ST] multiplied, and looked through
-  uint64_t* done = empty + ST;       // [ST] scores and dp are multiplied
-  uint64_t* clean = done + ST;       // [ST][2] the pair's tiles are clean
-  uint64_t* a_full = clean + 2 * ST;
+  uint8_t* s_b1 = smem + 2 * TILE;   // [S1] q or k
+  uint8_t* s_b2 = s_b1 + S1 * TILE;  // [S2] dout or v
+  // Statistics of the queries, each beside the tile that is held as long: delta is
+  // read for ds, lse for p.
+  float* s_delta = (float*)(s_b2 + S2 * TILE);  // [S1][128]
+  float* s_lse2 = s_delta + S1 * kAttTile;      // [S2][128]
+  uint64_t* full1 = (uint64_t*)(s_lse2 + S2 * kAttTile);  // [S1] the tile has come, and the statistic
+  uint64_t* full2 = full1 + S1;      // [S2]
+  uint64_t* empty1 = full2 + S2;     // [S1] multiplied, and looked through
+  uint64_t* empty2 = empty1 + S1;    // [S2]
+  uint64_t* done1 = empty2 + S2;     // [S1] scores are multiplied
+  uint64_t* done2 = done1 + S1;      // [S2] dp is multiplied
+  uint64_t* clean1 = done2 + S2;     // [S1] the tile is clean
+  uint64_t* clean2 = clean1 + S1;    // [S2]
+  uint64_t* a_full = clean2 + S2;
   uint64_t* a_empty = a_full + 1;    // all scores and dp are multiplied
   uint64_t* s_full = a_empty + 1;
   uint64_t* p_full = s_full + 1;     // scores read, and p written (KEYS)
@@ -86,13 +101,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   volatile int* s_flag = s_abort + 1;  // [kAttFlags]
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (smem_u32(smem) & 1023) {  // (the same for all threads; never seen)
+    if (threadIdx.x == 0) atomicCAS(a.err, 0, 60);
+    return;
+  }
   if (threadIdx.x == 0) {
-    for (int s = 0; s < ST; s++) {
-      mbar_init(&full[s], 1);
-      mbar_init(&empty[s], 3);
-      mbar_init(&done[s], 1);
-      mbar_init(&clean[2 * s], 2);
-      mbar_init(&clean[2 * s + 1], 2);
+    for (int s = 0; s < S1; s++) {
+      mbar_init(&full1[s], 1);
+      mbar_init(&empty1[s], 3);
+      mbar_init(&done1[s], 1);
+      mbar_init(&clean1[s], 2);
+    }
+    for (int s = 0; s < S2; s++) {
+      mbar_init(&full2[s], 1);
+      mbar_init(&empty2[s], KEYS ? 3 : 1);
+      mbar_init(&done2[s], 1);
+      mbar_init(&clean2[s], 2);
     }
     mbar_init(a_full, 1);
     mbar_init(a_empty, 1);
@@ -126,9 +150,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto tile_of = [&](int id) { return KEYS ? id / heads : a.tiles - 1 - id / heads; };
   const int per = KEYS ? a.group : 1;  // passes over the tiles: the query heads of a key's
 
+  if (warp >= 8) {
+  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
   if (warp == kLoadWarp) {
     // ------------------------------------------------------------ loads
-    int use = 0, a_use = 0;
+    int use = 0, a_use = 0, n1 = 0, n2 = 0;
     bool ok = true;
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const int tile = tile_of(id), head = id % heads;
@@ -144,25 +170,32 @@ __global__ void __launch_bounds__(kThreads, 1)
                             a_full);
           a_use++;
         };
-        const int kv = KEYS ? 0 : head / a.group;
         int t = r.first, g = 0;
         for (int i = 0; ok && i < total; i++, use++) {
-          const int st = use % ST;
-          ok = att_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 62);
+          const int s1 = use % S1, s2 = use % S2;
+          ok = att_wait(&empty1[s1], (use / S1 & 1) ^ 1, s_abort, a.err, 62);
           if (!ok) break;
-          uint8_t* to = s_b + 2 * st * TILE;
+          n1 = use + 1;
+          const int h = KEYS ? head * a.group + g : head / a.group;
+          const int64_t at = (int64_t)h * a.padded + t * kAttTile;
           if (KEYS) {
-            const int h = head * a.group + g;
-            mbar_expect_tx(&full[st], 2 * TILE + kStatBytes);
-            att_load_tile<DP>(to, &maps.q, a.q_last, h, t * kAttTile, &full[st]);
-            att_load_tile<DP>(to + TILE, &maps.dout, a.dout_last, h, t * kAttTile, &full[st]);
-            const int64_t at = (int64_t)h * a.padded + t * kAttTile;
-            bulk_copy_g2s(s_stat + st * 2 * kAttTile, a.lse2 + at, kAttTile * 4, &full[st]);
-            bulk_copy_g2s(s_stat + st * 2 * kAttTile + kAttTile, a.delta + at, kAttTile * 4, &full[st]);
+            mbar_expect_tx(&full1[s1], TILE + kStatBytes);
+            att_load_tile<DP>(s_b1 + s1 * TILE, &maps.q, a.q_last, h, t * kAttTile, &full1[s1]);
+            bulk_copy_g2s(s_delta + s1 * kAttTile, a.delta + at, kStatBytes, &full1[s1]);
           } else {
-            mbar_expect_tx(&full[st], 2 * TILE);
-            att_load_tile<DP>(to, &maps.k, a.k_last, kv, t * kAttTile, &full[st]);
-            att_load_tile<DP>(to + TILE, &maps.v, a.v_last, kv, t * kAttTile, &full[st]);
+            mbar_expect_tx(&full1[s1], TILE);
+            att_load_tile<DP>(s_b1 + s1 * TILE, &maps.k, a.k_last, h, t * kAttTile, &full1[s1]);
+          }
+          ok = att_wait(&empty2[s2], (use / S2 & 1) ^ 1, s_abort, a.err, 77);
+          if (!ok) break;
+          n2 = use + 1;
+          if (KEYS) {
+            mbar_expect_tx(&full2[s2], TILE + kStatBytes);
+            att_load_tile<DP>(s_b2 + s2 * TILE, &maps.dout, a.dout_last, h, t * kAttTile, &full2[s2]);
+            bulk_copy_g2s(s_lse2 + s2 * kAttTile, a.lse2 + at, kStatBytes, &full2[s2]);
+          } else {
+            mbar_expect_tx(&full2[s2], TILE);
+            att_load_tile<DP>(s_b2 + s2 * TILE, &maps.v, a.v_last, h, t * kAttTile, &full2[s2]);
           }
           if (++t == r.end) {
             t = r.first;
@@ -177,47 +210,52 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (lane == 0 && *s_abort) {
       // Drain (bounded) before shared memory goes.
       volatile int dummy = 0;
-      for (int i = max(0, use - ST); i < use; i++) mbar_wait(&full[i % ST], i / ST & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+      for (int i = max(0, n1 - S1); i < n1; i++) mbar_wait(&full1[i % S1], i / S1 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+      for (int i = max(0, n2 - S2); i < n2; i++) mbar_wait(&full2[i % S2], i / S2 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
       if (a_use) mbar_wait(a_full, (a_use - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
     }
   } else if (warp == kMmaWarp) {
     // ------------------------------------------------------------ products
     const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
-    const uint64_t bk = smem_desc_sw128(s_b), bm = att_desc_mn(s_b);
+    const uint64_t b1k = smem_desc_sw128(s_b1), b1m = att_desc_mn(s_b1);
+    const uint64_t b2k = smem_desc_sw128(s_b2), b2m = att_desc_mn(s_b2);
     constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
     // The whole warp goes through the loops, one lane issues.
     const bool lead = att_elect();
     const uint32_t tm = __reduce_min_sync(~0u, tmem);
-    constexpr uint32_t PAIR = 2 * TILE >> 4;
-    int use = 0, a_use = 0, p_use = 0;
-    uint32_t cleaned = 0;
+    int use = 0, a_use = 0;
+    uint32_t cleaned1 = 0, cleaned2 = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
-    auto scores = [&](int st) {  // rows x (q or k)
+    auto scores = [&](int u) {  // rows x (q or k)
+      const int st = u % S1;
+      wait(&full1[st], u / S1, 64);
+      tc_fence_after();
       if (lead) {
-        const uint64_t bd = bk + st * PAIR;
+        const uint64_t bd = b1k + st * (TILE >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColS, a1 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(s_full);
+        mma_commit(&done1[st]);
       }
     };
-    auto dps = [&](int st, bool last) {  // rows x (dout or v)
+    auto dps = [&](int u, bool last) {  // rows x (dout or v)
+      const int st = u % S2;
+      wait(&full2[st], u / S2, 67);
+      tc_fence_after();
       if (lead) {
-        const uint64_t bd = bk + st * PAIR + (TILE >> 4);
+        const uint64_t bd = b2k + st * (TILE >> 4);
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(dp_full);
-        mma_commit(&done[st]);
+        mma_commit(KEYS ? &done2[st] : &empty2[st]);
         if (last) mma_commit(a_empty);
       }
     };
-    // (p or ds over its own columns, each half of a row in its half of them) x (tile `second` of the pair)
-    auto product = [&](uint32_t to, uint32_t from, int st, int second, bool add) {
-      if (lead) {
-        const uint64_t bd = bm + st * PAIR + second * (TILE >> 4);
+    // (p or ds over its own columns, each half of a row in its half of them) x a tile
+    auto product = [&](uint32_t to, uint32_t from, uint64_t bd, bool add) {
 #pragma unroll
-        for (int k = 0; k < kAttTile / 16; k++)
-          att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
-      }
+      for (int k = 0; k < kAttTile / 16; k++)
+        att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const AttSpan r = att_span<!KEYS>(a, tile_of(id));
@@ -229,38 +267,38 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lead) mbar_arrive(a_empty);
         continue;
       }
-      wait(&full[use % ST], use / ST, 64);
-      tc_fence_after();
-      scores(use % ST);
-      dps(use % ST, total == 1);
+      scores(use);
+      dps(use, total == 1);
       int t = r.first;
 #pragma unroll 1
-      for (int i = 0; i < total; i++, use++, p_use++) {
-        const int st = use % ST, next = (use + 1) % ST;
+      for (int i = 0; i < total; i++, use++) {
+        const int s1 = use % S1, s2 = use % S2;
         const bool more = i + 1 < total, masked = att_masked(r.low_max, r.high_min, t);
-        wait(p_full, p_use, 65);
+        wait(p_full, use, 65);
         if (KEYS) {
-          if (masked) wait(&clean[2 * st + 1], cleaned >> st, 66);
+          if (masked) {
+            wait(&clean2[s2], cleaned2 >> s2, 66);
+            cleaned2 ^= 1u << s2;
+          }
           tc_fence_after();
-          product(kCol2, kColS, st, 1, i > 0);
+          if (lead) {
+            product(kCol2, kColS, b2m + s2 * (TILE >> 4), i > 0);
+            mma_commit(&empty2[s2]);
+          }
         }
-        if (more) {
-          wait(&full[next], (use + 1) / ST, 67);
-          tc_fence_after();
-          scores(next);
-        }
-        wait(ds_full, p_use, 68);
+        if (more) scores(use + 1);
+        wait(ds_full, use, 68);
         if (masked) {
-          wait(&clean[2 * st], cleaned >> st, 69);
-          cleaned ^= 1u << st;
+          wait(&clean1[s1], cleaned1 >> s1, 69);
+          cleaned1 ^= 1u << s1;
         }
         tc_fence_after();
-        product(kCol1, kColDp, st, 0, i > 0);
-        if (lead) mma_commit(&empty[st]);
-        if (more)
-          dps(next, i + 2 == total);
-        else
-          if (lead) mma_commit(r_full);
+        if (lead) {
+          product(kCol1, kColDp, b1m + s1 * (TILE >> 4), i > 0);
+          mma_commit(&empty1[s1]);
+          if (!more) mma_commit(r_full);
+        }
+        if (more) dps(use + 1, i + 2 == total);
         if (++t == r.end) t = r.first;
       }
     }
@@ -280,34 +318,39 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int total = max(0, r.end - r.first) * per;
       int t = r.first;
       for (int i = 0; ok && i < total; i++, use++) {
-        const int st = use % ST;
-        ok = att_wait_warp(&full[st], use / ST & 1, s_abort, a.err, 70);
+        const int s1 = use % S1, s2 = use % S2;
+        ok = att_wait_warp(&full1[s1], use / S1 & 1, s_abort, a.err, 70);
+        if (ok && KEYS) ok = att_wait_warp(&full2[s2], use / S2 & 1, s_abort, a.err, 78);
         if (!ok) break;
-        // A later item's flag: the other cleaning warp is at most ST items ahead,
+        // A later item's flag: the other cleaning warp is at most S1 items ahead,
         // and the item eight before this one, which had the flag last, has its results.
         if (i == 0 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
-        if (att_masked(r.low_max, r.high_min, t)) {
-          // Scores and dp are of the values as they are.
-          ok = att_wait_warp(&done[st], use / ST & 1, s_abort, a.err, 71);
+        const bool masked = att_masked(r.low_max, r.high_min, t);
+        // (Scores and dp are of the values as they are.)
+        auto look = [&](uint8_t* tile, uint64_t* done, uint64_t* clean, uint32_t parity) {
+          ok = att_wait_warp(done, parity, s_abort, a.err, 71);
+          if (!ok) return;
+          if (att_clean<DP, F16>(tile, warp - kCleanWarp, 2) && lane == 0) s_flag[count % kAttFlags] = 1;
+          att_fence_async();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(clean);
+        };
+        if (KEYS) {
+          if (masked) look(s_b2 + s2 * TILE, &done2[s2], &clean2[s2], use / S2 & 1);
           if (!ok) break;
-          bool any = false;
-#pragma unroll 1
-          for (int second = KEYS ? 1 : 0; second >= 0; second--) {
-            any |= att_clean<DP, F16>(s_b + (2 * st + second) * TILE, warp - kCleanWarp, 2);
-            if (any && lane == 0) s_flag[count % kAttFlags] = 1;
-            att_fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&clean[2 * st + second]);
-          }
+          if (lane == 0) mbar_arrive(&empty2[s2]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        if (masked) look(s_b1 + s1 * TILE, &done1[s1], &clean1[s1], use / S1 & 1);
+        if (!ok) break;
+        if (lane == 0) mbar_arrive(&empty1[s1]);
         if (++t == r.end) t = r.first;
       }
       if (total > 0) count++;
     }
+  }
   } else {
     // ------------------------------------------------------------ p, ds, results
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));
     const int half = warp >> 2, quad = warp & 3, row = quad * 32 + lane;
     const uint32_t lanes = (uint32_t)(quad * 32) << 16;
     const uint32_t ts = tmem + lanes + kColS + half * 64, tdp = tmem + lanes + kColDp + half * 64;
@@ -349,7 +392,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float lse2 = it.lse2, delta = it.delta;
       int t = it.first;
       for (int i = 0; i < total; i++, use++) {
-        const float* stat = s_stat + use % ST * 2 * kAttTile + half * 64;
+        const float* lses = s_lse2 + use % S2 * kAttTile + half * 64;
+        const float* deltas = s_delta + use % S1 * kAttTile + half * 64;
         ok = att_wait_warp(s_full, s_use & 1, s_abort, a.err, 72);
         if (!ok) break;
         tc_fence_after();
@@ -391,7 +435,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         } else {
           // (The statistics came with the tiles, by the async proxy: this thread
           // has to have seen that barrier itself.)
-          ok = att_wait_warp(&full[use % ST], use / ST & 1, s_abort, a.err, 73);
+          ok = att_wait_warp(&full2[use % S2], use / S2 & 1, s_abort, a.err, 73);
           if (!ok) break;
         }
         const F2 cc = pack_f2(a.c2);
@@ -400,7 +444,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           float e[4];
           F2 lo, hi;
           if (KEYS) {
-            const float4 z = *reinterpret_cast<const float4*>(stat + c);
+            const float4 z = *reinterpret_cast<const float4*>(lses + c);
             lo = pack_f2(kLift<F16> - z.x, kLift<F16> - z.y);
             hi = pack_f2(kLift<F16> - z.z, kLift<F16> - z.w);
           } else {
@@ -434,6 +478,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = att_wait_warp(dp_full, s_use & 1, s_abort, a.err, 74);
         if (!ok) break;
         s_use++;
+        if (KEYS) ok = att_wait_warp(&full1[use % S1], use / S1 & 1, s_abort, a.err, 79);
+        if (!ok) break;
         tc_fence_after();
         const F2 gg = pack_f2(ds_scale);
         uint32_t w[32];
@@ -446,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int c = 0; c < 32; c += 4) {
             F2 lo, hi;
             if (KEYS) {
-              const float4 z = *reinterpret_cast<const float4*>(stat + kAttTile + c0 + c);
+              const float4 z = *reinterpret_cast<const float4*>(deltas + c0 + c);
               lo = pack_f2(-z.x, -z.y);
               hi = pack_f2(-z.z, -z.w);
             } else {
