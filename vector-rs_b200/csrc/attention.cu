@@ -12,8 +12,14 @@ namespace {
 
 int64_t up(int64_t v, int64_t m) { return (v + m - 1) / m * m; }
 
-// A token's sequence, and two spans a tile.
-int64_t sequences_bytes(int64_t tokens) { return up(tokens * 8, 256) + up((tokens + kAttTile - 1) / kAttTile * 32, 256); }
+// A token's sequence, two spans a tile and two orders of the tiles.
+int64_t sequences_bytes(int64_t tokens) {
+  const int64_t tiles = (tokens + kAttTile - 1) / kAttTile;
+  return up(tokens * 8, 256) + up(tiles * 32, 256) + up(tiles * 8, 256);
+}
+int* order_in(void* seg, int64_t tokens) {
+  return (int*)((char*)seg + sequences_bytes(tokens) - up((tokens + kAttTile - 1) / kAttTile * 8, 256));
+}
 
 // Each token's sequence [first, past its last): the last bound at or below the
 // token, by bisection. Whatever cu holds, the interval contains the token and
@@ -64,6 +70,42 @@ __global__ void __launch_bounds__(kAttTile) attention_sequences_kernel(const int
     spans[threadIdx.x * a.tiles + tile] =
         make_int4(hi > 0 ? lo / kAttTile : 0, (hi + kAttTile - 1) / kAttTile, low_max, high_min);
   }
+}
+
+// Units of work, the longest first, where CTAs have several each: `step` neighbouring
+// tiles a unit, by what they meet. Block 0 for queries' rows, block 1 for keys'.
+// A counting sort; the order of equal ones does not matter (a result has one writer).
+constexpr int kBins = 1024;
+__global__ void __launch_bounds__(kBins) attention_order_kernel(const int4* spans, int tiles, int step, int* order) {
+  __shared__ int s_count[kBins], s_warp[kBins / 32];
+  grid_launch();
+  grid_wait();
+  const int4* at = spans + blockIdx.x * tiles;
+  const int units = (tiles + step - 1) / step, tid = threadIdx.x, lane = tid & 31;
+  order += blockIdx.x * tiles;
+  auto bin_of = [&](int u) {
+    int n = 0;
+    for (int t = u * step; t < min(tiles, u * step + step); t++) n += max(0, at[t].y - at[t].x);
+    return kBins - 1 - min(n, kBins - 1);
+  };
+  s_count[tid] = 0;
+  __syncthreads();
+  for (int u = tid; u < units; u += kBins) atomicAdd(&s_count[bin_of(u)], 1);
+  __syncthreads();
+  const int mine = s_count[tid];
+  int sum = mine;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int v = __shfl_up_sync(~0u, sum, o);
+    if (lane >= o) sum += v;
+  }
+  if (lane == 31) s_warp[tid >> 5] = sum;
+  __syncthreads();
+  int before = 0;
+  for (int w = 0; w < tid >> 5; w++) before += s_warp[w];
+  s_count[tid] = before + sum - mine;
+  __syncthreads();
+  for (int u = tid; u < units; u += kBins) order[atomicAdd(&s_count[bin_of(u)], 1)] = u;
 }
 
 // d, heads and tokens as a 3-D map of 64 x 1 x `rows`, the smaller stride first.
@@ -153,6 +195,16 @@ int start(const Call& c, void* seg, unsigned* zero, AttArgs& a, cudaStream_t s) 
   return VRS_OK;
 }
 
+// The order of work in a.order (queries' rows; keys' `tiles` further), for sequences
+// of several lengths.
+int sort_units(AttArgs& a, void* seg, int step, bool both, cudaStream_t s) {
+  int* order = order_in(seg, a.tokens);
+  VRS_TRY(launch_after(attention_order_kernel, both ? 2u : 1u, kBins, 0, s, a.spans, a.tiles, step, order));
+  count_launch();
+  a.order = order;
+  return VRS_OK;
+}
+
 int check_workspace(const std::string& w, const void* ws, int64_t have, int64_t need) {
   if (need && (!ws || (uintptr_t)ws % 256 || have < need)) return invalid(w + ": workspace missing, off 256 bytes or too small");
   return VRS_OK;
@@ -220,7 +272,9 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
       a.pairing = kAttTwoTiles;
       a.items = (int)((a.tiles + 1) / 2 * heads);
     }
-    st = launch_attention_forward(f16, d <= 64 ? 64 : 128, maps, a, sms, s);
+    if (cu_seqlens && a.items > sms)
+      st = sort_units(a, workspace, a.pairing == kAttTwoTiles ? 2 : 1, false, s);
+    if (st == VRS_OK) st = launch_attention_forward(f16, d <= 64 ? 64 : 128, maps, a, sms, s);
   }
   prof_end(t, s);
   return st;
@@ -323,8 +377,14 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
     st = launch_attention_stats(f16, b, sms, s);
   }
   const int dp = d <= 64 ? 64 : 128;
+  const int* order = nullptr;
+  if (st == VRS_OK && cu_seqlens && (int64_t)a.tiles * heads > sms) {
+    st = sort_units(a, ws + p.seg, 1, true, s);
+    order = a.order;
+  }
   if (st == VRS_OK && dk) {
     a.items = a.tiles * (int)kv_heads;
+    a.order = order ? order + a.tiles : nullptr;
     a.r1 = (uint16_t*)dk->data;
     a.r1s = dk->stride;
     a.r1h = dk->head_stride;
@@ -335,6 +395,7 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
   }
   if (st == VRS_OK && dq) {
     a.items = a.tiles * (int)heads;
+    a.order = order;
     a.r1 = (uint16_t*)dq->data;
     a.r1s = dq->stride;
     a.r1h = dq->head_stride;

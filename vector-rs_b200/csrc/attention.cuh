@@ -34,6 +34,7 @@ struct AttArgs {
   int seq_len;        // of every sequence, where seg is null
   const int2* seg;    // per token: its sequence's first token and the one past its last
   const int4* spans;  // beside seg: per tile what its rows meet, as queries, then as keys
+  const int* order;   // units of work (tiles, or pairs of them), the longest first; null: by number
   float c2;           // scale * log2 e
   float scale;
   float* lse;         // [heads][tokens]
@@ -85,12 +86,14 @@ struct AttSpan {
   int first, end;        // tiles [first, end) with a row that some row here meets
   int low_max, high_min;  // rows [low_max, high_min) are met by all rows here
 };
-// By a whole warp, to which the result is uniform.
-template <bool KEYS>
+// UNIFORM: by a whole warp, and in uniform registers (for which the load is waited
+// for).
+template <bool KEYS, bool UNIFORM>
 __device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
   AttSpan s;
   if (a.seg) {
     const int4 v = a.spans[KEYS ? tile : a.tiles + tile];
+    if (!UNIFORM) return AttSpan{v.x, v.y, v.z, v.w};
     s.first = __reduce_min_sync(~0u, v.x);
     s.end = __reduce_min_sync(~0u, v.y);
     s.low_max = __reduce_min_sync(~0u, v.z);
@@ -105,6 +108,9 @@ __device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
   s.high_min = a.causal && KEYS ? t0 + 1 : lo0 + a.seq_len;
   return s;
 }
+
+// The unit of work in place n.
+__device__ __forceinline__ int att_unit(const AttArgs& a, int n, int natural) { return a.order ? a.order[n] : natural; }
 
 // Whether some row of a span does not meet all of tile t. (The tile's rows past
 // the last token are zeros, and masked.)

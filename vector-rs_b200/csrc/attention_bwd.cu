@@ -147,7 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   // Items: causal, the tiles with the longest passes first (a key's queries are
   // those after it).
   const int heads = KEYS ? a.kv_heads : a.heads;
-  auto tile_of = [&](int id) { return KEYS ? id / heads : a.tiles - 1 - id / heads; };
+  auto tile_of = [&](int id) { return att_unit(a, id / heads, KEYS ? id / heads : a.tiles - 1 - id / heads); };
   const int per = KEYS ? a.group : 1;  // passes over the tiles: the query heads of a key's
 
   if (warp >= 8) {
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const int tile = tile_of(id), head = id % heads;
-      const AttSpan r = att_span<!KEYS>(a, tile);
+      const AttSpan r = att_span<!KEYS, true>(a, tile);
       if (lane == 0) {
         const int n = max(0, r.end - r.first), total = n * per;
         auto rows = [&] {
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
-      const AttSpan r = att_span<!KEYS>(a, tile_of(id));
+      const AttSpan r = att_span<!KEYS, true>(a, tile_of(id));
       const int total = max(0, r.end - r.first) * per;
       // (The rows are waited for where nothing is multiplied too: a wait for the
       // next ones that came before these have would not see the difference.)
@@ -314,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     int use = 0, count = 0;
     bool ok = true;
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const AttSpan r = att_span<!KEYS>(a, tile_of(id));
+      const AttSpan r = att_span<!KEYS, true>(a, tile_of(id));
       const int total = max(0, r.end - r.first) * per;
       int t = r.first;
       for (int i = 0; ok && i < total; i++, use++) {
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       Mine m;
       m.tile = tile_of(id);
       m.head = id % heads;
-      const AttSpan r = att_span<!KEYS>(a, m.tile);
+      const AttSpan r = att_span<!KEYS, false>(a, m.tile);
       m.first = r.first;
       m.end = r.end;
       m.total = max(0, r.end - r.first) * per;
@@ -391,7 +391,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = seen.y - seen.x;
       const float lse2 = it.lse2, delta = it.delta;
       int t = it.first;
+      const bool another = id + (int)gridDim.x < a.items;
+      if (another && total == 0) next = mine_at(id + gridDim.x);
       for (int i = 0; i < total; i++, use++) {
+        if (another && i + 1 == total) next = mine_at(id + gridDim.x);  // (its loads are on their way meanwhile)
         const float* lses = s_lse2 + use % S2 * kAttTile + half * 64;
         const float* deltas = s_delta + use % S1 * kAttTile + half * 64;
         ok = att_wait_warp(s_full, s_use & 1, s_abort, a.err, 72);
@@ -529,7 +532,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (!ok) break;
       // Results: dk by the first four warps and dv by the others, or half of dq's columns each.
-      if (id + (int)gridDim.x < a.items) next = mine_at(id + gridDim.x);
       if (total > 0) {
         ok = att_wait_warp(r_full, r_use++ & 1, s_abort, a.err, 76);
         if (!ok) break;
@@ -541,31 +543,35 @@ __global__ void __launch_bounds__(kThreads, 1)
       const uint32_t from = tmem + lanes + (dv ? kCol2 : kCol1);
       const float f = dv ? (F16 ? 0x1p-14f : 1.0f) : a.scale / gain;
       uint16_t* to = dv ? a.r2 + i_row * a.r2s + head * a.r2h : a.r1 + i_row * a.r1s + head * a.r1h;
-      const int c0 = KEYS ? 0 : half * (DP / 2), c1 = KEYS ? DP : c0 + DP / 2;
-#pragma unroll 1
-      for (int c = c0; c < c1 && c < a.d; c += 32) {
-        float o[32];
-        if (total == 0) {
+      const int c0 = KEYS ? 0 : half * (DP / 2);
+      constexpr int N = KEYS ? DP : DP / 2;
+      float o[N];
+      if (total == 0) {
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] = 0.0f;
-        } else {
-          att_tm_load(from + c, o);
-          att_tm_wait(o);
+        for (int j = 0; j < N; j++) o[j] = 0.0f;
+      } else {
 #pragma unroll
-          for (int j = 0; j < 32; j++) o[j] *= f;
-          if (flagged) {
-            if (!KEYS) {
-              att_add_not_finite<F16>(o, a.k + head / a.group * a.kh, a.ks, seen.x, seen.y, c, a.d);
-            } else {
+        for (int c = 0; c < N; c += 32) att_tm_load(from + c0 + c, o + c);
+#pragma unroll
+        for (int c = 0; c < N; c += 32) att_tm_wait(o + c);
+#pragma unroll
+        for (int j = 0; j < N; j++) o[j] *= f;
+        if (flagged) {
 #pragma unroll 1
-              for (int g = 0; g < per; g++) {
-                const int h = head * a.group + g;
-                att_add_not_finite<F16>(o, dv ? a.dout + h * a.doh : a.q + h * a.qh, dv ? a.dos : a.qs, seen.x, seen.y, c, a.d);
-              }
-            }
+          for (int g = 0; g < per; g++) {
+            const int h = KEYS ? head * a.group + g : head / a.group;
+            const uint16_t* m = dv ? a.dout + h * a.doh : KEYS ? a.q + h * a.qh : a.k + h * a.kh;
+#pragma unroll
+            for (int c = 0; c < N; c += 32)
+              if (c0 + c < a.d)
+                att_add_not_finite<F16>(o + c, m, dv ? a.dos : KEYS ? a.qs : a.ks, seen.x, seen.y, c0 + c, a.d);
           }
         }
-        if (i_row < a.tokens) att_store_row<F16>(to, c, a.d, o);
+      }
+      if (i_row < a.tokens) {
+#pragma unroll
+        for (int c = 0; c < N; c += 32)
+          if (c0 + c < a.d) att_store_row<F16>(to, c0 + c, a.d, o + c);
       }
       tc_fence_before();
     }

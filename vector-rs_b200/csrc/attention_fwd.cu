@@ -60,18 +60,18 @@ __device__ __forceinline__ Item item_at(const AttFwd& a, int id) {
   t.live[0] = true;
   if (a.pairing == kAttTwoHeads) {
     const int pairs = a.heads / 2;
-    t.tile[0] = t.tile[1] = a.tiles - 1 - id / pairs;
+    t.tile[0] = t.tile[1] = att_unit(a, id / pairs, a.tiles - 1 - id / pairs);
     t.head[0] = id % pairs * 2;
     t.head[1] = t.head[0] + 1;
     t.live[1] = true;
   } else if (a.pairing == kAttTwoTiles) {
-    const int n = (a.tiles + 1) / 2 - 1 - id / a.heads;
+    const int n = att_unit(a, id / a.heads, (a.tiles + 1) / 2 - 1 - id / a.heads);
     t.tile[0] = 2 * n;
     t.tile[1] = 2 * n + 1;
     t.head[0] = t.head[1] = id % a.heads;
     t.live[1] = t.tile[1] < a.tiles;
   } else {
-    t.tile[0] = t.tile[1] = a.tiles - 1 - id / a.heads;
+    t.tile[0] = t.tile[1] = att_unit(a, id / a.heads, a.tiles - 1 - id / a.heads);
     t.head[0] = t.head[1] = id % a.heads;
     t.live[1] = false;
   }
@@ -86,6 +86,7 @@ struct Range {
   int low_max, high_min;
   __device__ __forceinline__ bool active(int s, int t) const { return t >= first[s] && t < end[s]; }
 };
+template <bool UNIFORM>
 __device__ __forceinline__ Range range_of(const AttFwd& a, const Item& it) {
   Range r;
   r.t0 = INT_MAX;
@@ -101,7 +102,7 @@ __device__ __forceinline__ Range range_of(const AttFwd& a, const Item& it) {
       r.end[1] = r.end[0];
       continue;
     }
-    const AttSpan p = att_span<true>(a, it.tile[s]);
+    const AttSpan p = att_span<true, UNIFORM>(a, it.tile[s]);
     r.first[s] = p.first;
     r.end[s] = p.end;
     if (p.first < p.end) {
@@ -178,7 +179,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
-      const Range r = range_of(a, it);
+      const Range r = range_of<true>(a, it);
       if (lane == 0) {
         // (The first keys and values before the queries: their places are free.)
         const int i0 = 2 * r.t0, i1 = 2 * r.t1;
@@ -238,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
-      const Range r = range_of(a, it);
+      const Range r = range_of<true>(a, it);
       // The queries are waited for where nothing is multiplied too: a wait for the
       // next ones that came before these have would not see the difference.
 #pragma unroll
@@ -308,7 +309,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     bool ok = true;
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const Item it = item_at(a, id);
-      const Range r = range_of(a, it);
+      const Range r = range_of<true>(a, it);
       for (int i = 2 * r.t0; ok && i < 2 * r.t1; i++, use++) {
         const int st = use % ST;
         // (Keys too are waited for: an arrival before the tile has come could
@@ -350,7 +351,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     };
     auto mine_at = [&](int id) {
       const Item it = item_at(a, id);
-      const Range r = range_of(a, it);
+      const Range r = range_of<false>(a, it);
       Mine m;
       m.live = s ? it.live[1] : it.live[0];
       m.any = r.t0 < r.t1;
@@ -369,7 +370,10 @@ __global__ void __launch_bounds__(kThreads, 1)
       float m = -INFINITY, l = 0.0f;
       const int2 seen = it.seen;
       const int len = seen.y - seen.x;
+      const bool none = it.first >= it.end;
+      if (more && none) next = mine_at(id + gridDim.x);
       for (int t = it.first; it.live && t < it.end; t++) {
+        if (more && t + 1 == it.end) next = mine_at(id + gridDim.x);  // (its loads are on their way meanwhile)
         ok = att_wait_warp(&s_full[s], s_use & 1, s_abort, a.err, 50);
         if (!ok) break;
         s_use++;
@@ -455,9 +459,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         l += sum_f2(add2(sum[0], sum[1]));
       }
       if (!ok) break;
-      if (more) next = mine_at(id + gridDim.x);
       // The row's result: sums over l; 0 for a row that sees nothing.
-      const bool none = it.first >= it.end;
       if (it.live && !none) {
         ok = att_wait_warp(&o_full[s], o_use++ & 1, s_abort, a.err, 52);
         if (!ok) break;
@@ -465,22 +467,28 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       if (it.live) {
         const float f = len > 0 ? 1.0f / l : 0.0f;
-        const bool flagged = it.any && s_flag[count % kAttFlags];
         uint16_t* out = a.r1 + it.i * a.r1s + it.head * a.r1h;
-#pragma unroll 1
-        for (int c = 0; c < DP && c < a.d; c += 32) {
-          float o[32];
-          if (none) {
+        float o[DP];
+        if (none) {
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[j] = 0.0f;
-          } else {
-            att_tm_load(to + c, o);
-            att_tm_wait(o);
+          for (int j = 0; j < DP; j++) o[j] = 0.0f;
+        } else {
 #pragma unroll
-            for (int j = 0; j < 32; j++) o[j] *= f;
-            if (flagged) att_add_not_finite<F16>(o, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
+          for (int c = 0; c < DP; c += 32) att_tm_load(to + c, o + c);
+#pragma unroll
+          for (int c = 0; c < DP; c += 32) att_tm_wait(o + c);
+#pragma unroll
+          for (int j = 0; j < DP; j++) o[j] *= f;
+          if (it.any && s_flag[count % kAttFlags]) {
+#pragma unroll
+            for (int c = 0; c < DP; c += 32)
+              if (c < a.d) att_add_not_finite<F16>(o + c, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
           }
-          if (it.i < a.tokens) att_store_row<F16>(out, c, a.d, o);
+        }
+        if (it.i < a.tokens) {
+#pragma unroll
+          for (int c = 0; c < DP; c += 32)
+            if (c < a.d) att_store_row<F16>(out, c, a.d, o + c);
         }
         tc_fence_before();
         if (it.i < a.tokens)
