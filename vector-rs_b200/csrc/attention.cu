@@ -168,6 +168,10 @@ int check_heads(const std::string& w, const char* name, const vrs_heads* h, int6
   return VRS_OK;
 }
 
+bool sectors(const vrs_heads* h, int64_t tokens, int64_t heads) {
+  return (uintptr_t)h->data % 32 == 0 && (tokens == 1 || h->stride % 16 == 0) && (heads == 1 || h->head_stride % 16 == 0);
+}
+
 // What the passes share; cu_seqlens become a token's sequence in the workspace,
 // `zero` (two words, null: none) is cleared.
 int start(const Call& c, void* seg, unsigned* zero, AttArgs& a, cudaStream_t s) {
@@ -256,6 +260,7 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
     a.r1 = (uint16_t*)out->data;
     a.r1s = out->stride;
     a.r1h = out->head_stride;
+    a.sectors = sectors(out, tokens, heads);
     a.v = (const uint16_t*)v->data;
     a.vs = v->stride;
     a.vh = v->head_stride;
@@ -391,6 +396,7 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
     a.r2 = (uint16_t*)dv->data;
     a.r2s = dv->stride;
     a.r2h = dv->head_stride;
+    a.sectors = sectors(dk, tokens, kv_heads) && sectors(dv, tokens, kv_heads);
     st = launch_attention_backward(f16, dp, true, maps, a, sms, s);
   }
   if (st == VRS_OK && dq) {
@@ -399,6 +405,7 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
     a.r1 = (uint16_t*)dq->data;
     a.r1s = dq->stride;
     a.r1h = dq->head_stride;
+    a.sectors = sectors(dq, tokens, heads);
     st = launch_attention_backward(f16, dp, false, maps, a, sms, s);
   }
   prof_end(t, s);

@@ -41,6 +41,7 @@ struct AttArgs {
   // Results: out; dk or dq, and dv.
   uint16_t *r1, *r2;
   int64_t r1s, r1h, r2s, r2h;
+  int sectors;  // rows of all results start on 32 bytes
   // Values that are not finite are read again from here.
   const uint16_t *q, *k, *v, *dout;
   int64_t qs, qh, ks, kh, vs, vh, dos, doh;
@@ -328,15 +329,22 @@ __device__ __forceinline__ void att_add_not_finite(float* o, const uint16_t* m, 
   }
 }
 
-// 32 results of a row, elements [c, c + 32) of d, in 16 bits. Whole 32-byte sectors
-// where rows start on them: a lane has a row, so nothing else makes up a sector.
+// 32 results of a row times f, elements [c, c + 32) of d, in 16 bits. `sectors`: rows
+// start on 32 bytes, whose sectors are then stored whole (a lane has a row, so nothing
+// else makes up a sector). Called in loops that stay rolled: this code runs once an
+// item, and fetching it would take longer than running it.
 template <bool F16>
-__device__ __forceinline__ void att_store_row(uint16_t* row, int c, int d, const float* o) {
+__device__ __forceinline__ void att_store_row(uint16_t* row, int c, int d, const float* o, float f, bool sectors) {
+  const F2 ff = pack_f2(f);
   uint32_t w[16];
 #pragma unroll
-  for (int j = 0; j < 16; j++) w[j] = att_pack2<F16>(o[2 * j], o[2 * j + 1]);
+  for (int j = 0; j < 16; j++) {
+    float lo, hi;
+    unpack_f2(mul2(pack_f2(o[2 * j], o[2 * j + 1]), ff), lo, hi);
+    w[j] = att_pack2<F16>(lo, hi);
+  }
   uint16_t* to = row + c;
-  if (c + 32 <= d && ((uintptr_t)to & 31) == 0) {
+  if (sectors && c + 32 <= d) {
 #pragma unroll
     for (int h = 0; h < 2; h++)
       asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to + 16 * h), "r"(w[8 * h]),

@@ -358,8 +358,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const float ds_scale = F16 ? gain * 0x1p-14f : 1.0f;
     int use = 0, s_use = 0, r_use = 0, count = 0;
     bool ok = true;
-    // What an item means to this thread. The next one's is found before this one's
-    // results are waited for.
+    // What an item means to this thread; looked up an item ahead.
     struct Mine {
       int tile, head, first, end, total, row;
       int2 seen;
@@ -391,10 +390,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int len = seen.y - seen.x;
       const float lse2 = it.lse2, delta = it.delta;
       int t = it.first;
-      const bool another = id + (int)gridDim.x < a.items;
-      if (another && total == 0) next = mine_at(id + gridDim.x);
+      if (id + (int)gridDim.x < a.items) next = mine_at(id + gridDim.x);  // (its loads have this item's time)
       for (int i = 0; i < total; i++, use++) {
-        if (another && i + 1 == total) next = mine_at(id + gridDim.x);  // (its loads are on their way meanwhile)
         const float* lses = s_lse2 + use % S2 * kAttTile + half * 64;
         const float* deltas = s_delta + use % S1 * kAttTile + half * 64;
         ok = att_wait_warp(s_full, s_use & 1, s_abort, a.err, 72);
@@ -544,34 +541,25 @@ __global__ void __launch_bounds__(kThreads, 1)
       const float f = dv ? (F16 ? 0x1p-14f : 1.0f) : a.scale / gain;
       uint16_t* to = dv ? a.r2 + i_row * a.r2s + head * a.r2h : a.r1 + i_row * a.r1s + head * a.r1h;
       const int c0 = KEYS ? 0 : half * (DP / 2);
-      constexpr int N = KEYS ? DP : DP / 2;
-      float o[N];
-      if (total == 0) {
+#pragma unroll 1
+      for (int c = c0; c < min(a.d, c0 + (KEYS ? DP : DP / 2)); c += 32) {
+        float o[32];
+        if (total == 0) {
 #pragma unroll
-        for (int j = 0; j < N; j++) o[j] = 0.0f;
-      } else {
-#pragma unroll
-        for (int c = 0; c < N; c += 32) att_tm_load(from + c0 + c, o + c);
-#pragma unroll
-        for (int c = 0; c < N; c += 32) att_tm_wait(o + c);
-#pragma unroll
-        for (int j = 0; j < N; j++) o[j] *= f;
+          for (int j = 0; j < 32; j++) o[j] = 0.0f;
+        } else {
+          att_tm_load(from + c, o);
+          att_tm_wait(o);
+        }
         if (flagged) {
 #pragma unroll 1
           for (int g = 0; g < per; g++) {
             const int h = KEYS ? head * a.group + g : head / a.group;
-            const uint16_t* m = dv ? a.dout + h * a.doh : KEYS ? a.q + h * a.qh : a.k + h * a.kh;
-#pragma unroll
-            for (int c = 0; c < N; c += 32)
-              if (c0 + c < a.d)
-                att_add_not_finite<F16>(o + c, m, dv ? a.dos : KEYS ? a.qs : a.ks, seen.x, seen.y, c0 + c, a.d);
+            att_add_not_finite<F16>(o, dv ? a.dout + h * a.doh : KEYS ? a.q + h * a.qh : a.k + h * a.kh,
+                                    dv ? a.dos : KEYS ? a.qs : a.ks, seen.x, seen.y, c, a.d);
           }
         }
-      }
-      if (i_row < a.tokens) {
-#pragma unroll
-        for (int c = 0; c < N; c += 32)
-          if (c0 + c < a.d) att_store_row<F16>(to, c0 + c, a.d, o + c);
+        if (i_row < a.tokens) att_store_row<F16>(to, c, a.d, o, f, a.sectors);
       }
       tc_fence_before();
     }

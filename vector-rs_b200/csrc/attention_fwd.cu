@@ -342,8 +342,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + kColS + s * 128, to = tmem + lanes + kColO + s * 128;
     int s_use = 0, o_use = 0, count = 0;
     bool ok = true;
-    // What an item means to this thread. The next one's is found before this one's
-    // result is waited for.
+    // What an item means to this thread; looked up an item ahead.
     struct Mine {
       bool live, any;   // any: the item has tiles of keys
       int first, end, head, kv, i;
@@ -366,14 +365,12 @@ __global__ void __launch_bounds__(kThreads, 1)
     Mine next = mine_at(blockIdx.x);
     for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
       const Mine it = next;
-      const bool more = id + (int)gridDim.x < a.items;
       float m = -INFINITY, l = 0.0f;
       const int2 seen = it.seen;
       const int len = seen.y - seen.x;
       const bool none = it.first >= it.end;
-      if (more && none) next = mine_at(id + gridDim.x);
+      if (id + (int)gridDim.x < a.items) next = mine_at(id + gridDim.x);  // (its loads have this item's time)
       for (int t = it.first; it.live && t < it.end; t++) {
-        if (more && t + 1 == it.end) next = mine_at(id + gridDim.x);  // (its loads are on their way meanwhile)
         ok = att_wait_warp(&s_full[s], s_use & 1, s_abort, a.err, 50);
         if (!ok) break;
         s_use++;
@@ -468,27 +465,19 @@ __global__ void __launch_bounds__(kThreads, 1)
       if (it.live) {
         const float f = len > 0 ? 1.0f / l : 0.0f;
         uint16_t* out = a.r1 + it.i * a.r1s + it.head * a.r1h;
-        float o[DP];
-        if (none) {
+        const bool flagged = it.any && s_flag[count % kAttFlags];
+#pragma unroll 1
+        for (int c = 0; c < a.d; c += 32) {
+          float o[32];
+          if (none) {
 #pragma unroll
-          for (int j = 0; j < DP; j++) o[j] = 0.0f;
-        } else {
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) att_tm_load(to + c, o + c);
-#pragma unroll
-          for (int c = 0; c < DP; c += 32) att_tm_wait(o + c);
-#pragma unroll
-          for (int j = 0; j < DP; j++) o[j] *= f;
-          if (it.any && s_flag[count % kAttFlags]) {
-#pragma unroll
-            for (int c = 0; c < DP; c += 32)
-              if (c < a.d) att_add_not_finite<F16>(o + c, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
+            for (int j = 0; j < 32; j++) o[j] = 0.0f;
+          } else {
+            att_tm_load(to + c, o);
+            att_tm_wait(o);
           }
-        }
-        if (it.i < a.tokens) {
-#pragma unroll
-          for (int c = 0; c < DP; c += 32)
-            if (c < a.d) att_store_row<F16>(out, c, a.d, o + c);
+          if (flagged) att_add_not_finite<F16>(o, a.v + it.kv * a.vh, a.vs, seen.x, seen.y, c, a.d);
+          if (it.i < a.tokens) att_store_row<F16>(out, c, a.d, o, f, a.sectors);
         }
         tc_fence_before();
         if (it.i < a.tokens)
