@@ -29,7 +29,7 @@ using namespace vrs::tc;
 
 constexpr int kThreads = 384;
 constexpr int kCompute = 256;
-constexpr int kMmaWarp = 8, kLoadWarp = 9, kCleanWarp = 10;  // and 11
+constexpr int kMmaWarp = 8, kLoadWarp = 9;  // (10 and 11 make up their warpgroup)
 // Registers: 168 a thread at launch; the computing warps take what the others leave
 // (256 x 192 + 128 x 120 of 384 x 168).
 constexpr int kComputeRegs = 192, kOtherRegs = 120;
@@ -82,23 +82,20 @@ __global__ void __launch_bounds__(kThreads, 1)
   float* s_lse2 = s_delta + S1 * kAttTile;      // [S2][128]
   uint64_t* full1 = (uint64_t*)(s_lse2 + S2 * kAttTile);  // [S1] the tile has come, and the statistic
   uint64_t* full2 = full1 + S1;      // [S2]
-  uint64_t* empty1 = full2 + S2;     // [S1] multiplied, and looked through
+  uint64_t* empty1 = full2 + S2;     // [S1] multiplied
   uint64_t* empty2 = empty1 + S1;    // [S2]
-  uint64_t* done1 = empty2 + S2;     // [S1] scores are multiplied
-  uint64_t* done2 = done1 + S1;      // [S2] dp is multiplied
-  uint64_t* clean1 = done2 + S2;     // [S1] the tile is clean
-  uint64_t* clean2 = clean1 + S1;    // [S2]
-  uint64_t* a_full = clean2 + S2;
+  uint64_t* a_full = empty2 + S2;
   uint64_t* a_empty = a_full + 1;    // all scores and dp are multiplied
   uint64_t* s_full = a_empty + 1;
   uint64_t* p_full = s_full + 1;     // scores read, and p written (KEYS)
   uint64_t* dp_full = p_full + 1;
   uint64_t* ds_full = dp_full + 1;
   uint64_t* r_full = ds_full + 1;    // results
-  uint64_t* drain = r_full + 1;
+  uint64_t* voted = r_full + 1;      // the computing warps have voted
+  uint64_t* drain = voted + 1;
   uint32_t* s_tmem = (uint32_t*)(drain + 1);
   volatile int* s_abort = (volatile int*)(s_tmem + 1);
-  volatile int* s_flag = s_abort + 1;  // [kAttFlags]
+  volatile int* s_vote = s_abort + 1;  // [4] by turns
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {  // (the same for all threads; never seen)
@@ -108,15 +105,11 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (threadIdx.x == 0) {
     for (int s = 0; s < S1; s++) {
       mbar_init(&full1[s], 1);
-      mbar_init(&empty1[s], 3);
-      mbar_init(&done1[s], 1);
-      mbar_init(&clean1[s], 2);
+      mbar_init(&empty1[s], 1);
     }
     for (int s = 0; s < S2; s++) {
       mbar_init(&full2[s], 1);
-      mbar_init(&empty2[s], KEYS ? 3 : 1);
-      mbar_init(&done2[s], 1);
-      mbar_init(&clean2[s], 2);
+      mbar_init(&empty2[s], 1);
     }
     mbar_init(a_full, 1);
     mbar_init(a_empty, 1);
@@ -125,9 +118,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     mbar_init(dp_full, 1);
     mbar_init(ds_full, kCompute / 32);
     mbar_init(r_full, 1);
+    mbar_init(voted, kCompute / 32);
     mbar_init(drain, 1);
     *s_abort = 0;
-    for (int i = 0; i < kAttFlags; i++) s_flag[i] = 0;
+    for (int i = 0; i < 4; i++) s_vote[i] = 0;
     fence_mbar_init();
   }
   if (threadIdx.x == 32 * kLoadWarp) {
@@ -224,7 +218,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     const bool lead = att_elect();
     const uint32_t tm = __reduce_min_sync(~0u, tmem);
     int use = 0, a_use = 0;
-    uint32_t cleaned1 = 0, cleaned2 = 0;
     auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
     auto scores = [&](int u) {  // rows x (q or k)
       const int st = u % S1;
@@ -235,7 +228,6 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColS, a1 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(s_full);
-        mma_commit(&done1[st]);
       }
     };
     auto dps = [&](int u, bool last) {  // rows x (dout or v)
@@ -247,7 +239,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
         for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
         mma_commit(dp_full);
-        mma_commit(KEYS ? &done2[st] : &empty2[st]);
+        if (!KEYS) mma_commit(&empty2[st]);
         if (last) mma_commit(a_empty);
       }
     };
@@ -269,17 +261,12 @@ __global__ void __launch_bounds__(kThreads, 1)
       }
       scores(use);
       dps(use, total == 1);
-      int t = r.first;
 #pragma unroll 1
       for (int i = 0; i < total; i++, use++) {
         const int s1 = use % S1, s2 = use % S2;
-        const bool more = i + 1 < total, masked = att_masked(r.low_max, r.high_min, t);
+        const bool more = i + 1 < total;
         wait(p_full, use, 65);
         if (KEYS) {
-          if (masked) {
-            wait(&clean2[s2], cleaned2 >> s2, 66);
-            cleaned2 ^= 1u << s2;
-          }
           tc_fence_after();
           if (lead) {
             product(kCol2, kColS, b2m + s2 * (TILE >> 4), i > 0);
@@ -288,10 +275,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         if (more) scores(use + 1);
         wait(ds_full, use, 68);
-        if (masked) {
-          wait(&clean1[s1], cleaned1 >> s1, 69);
-          cleaned1 ^= 1u << s1;
-        }
         tc_fence_after();
         if (lead) {
           product(kCol1, kColDp, b1m + s1 * (TILE >> 4), i > 0);
@@ -299,7 +282,6 @@ __global__ void __launch_bounds__(kThreads, 1)
           if (!more) mma_commit(r_full);
         }
         if (more) dps(use + 1, i + 2 == total);
-        if (++t == r.end) t = r.first;
       }
     }
     if (*s_abort) {
@@ -308,44 +290,6 @@ __global__ void __launch_bounds__(kThreads, 1)
       volatile int dummy = 0;
       if (lead) mma_commit(drain);
       mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
-    }
-  } else if (warp >= kCleanWarp) {
-    // ------------------------------------------------------------ cleaning
-    int use = 0, count = 0;
-    bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const AttSpan r = att_span<!KEYS, true>(a, tile_of(id));
-      const int total = max(0, r.end - r.first) * per;
-      int t = r.first;
-      for (int i = 0; ok && i < total; i++, use++) {
-        const int s1 = use % S1, s2 = use % S2;
-        ok = att_wait_warp(&full1[s1], use / S1 & 1, s_abort, a.err, 70);
-        if (ok && KEYS) ok = att_wait_warp(&full2[s2], use / S2 & 1, s_abort, a.err, 78);
-        if (!ok) break;
-        // A later item's flag: the other cleaning warp is at most S1 items ahead,
-        // and the item eight before this one, which had the flag last, has its results.
-        if (i == 0 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
-        const bool masked = att_masked(r.low_max, r.high_min, t);
-        // (Scores and dp are of the values as they are.)
-        auto look = [&](uint8_t* tile, uint64_t* done, uint64_t* clean, uint32_t parity) {
-          ok = att_wait_warp(done, parity, s_abort, a.err, 71);
-          if (!ok) return;
-          if (att_clean<DP, F16>(tile, warp - kCleanWarp, 2) && lane == 0) s_flag[count % kAttFlags] = 1;
-          att_fence_async();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(clean);
-        };
-        if (KEYS) {
-          if (masked) look(s_b2 + s2 * TILE, &done2[s2], &clean2[s2], use / S2 & 1);
-          if (!ok) break;
-          if (lane == 0) mbar_arrive(&empty2[s2]);
-        }
-        if (masked) look(s_b1 + s1 * TILE, &done1[s1], &clean1[s1], use / S1 & 1);
-        if (!ok) break;
-        if (lane == 0) mbar_arrive(&empty1[s1]);
-        if (++t == r.end) t = r.first;
-      }
-      if (total > 0) count++;
     }
   }
   } else {
@@ -356,11 +300,22 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t ts = tmem + lanes + kColS + half * 64, tdp = tmem + lanes + kColDp + half * 64;
     const float gain = F16 ? gain_of(a.bound) : 1.0f;
     const float ds_scale = F16 ? gain * 0x1p-14f : 1.0f;
-    int use = 0, s_use = 0, r_use = 0, count = 0;
+    int use = 0, s_use = 0, r_use = 0, votes = 0;
     bool ok = true;
+    // Whether any of the computing warps says so. Between its two sides lies a barrier.
+    const auto vote = [&](bool mine) {
+      mine = __any_sync(~0u, mine);
+      if (lane == 0) {
+        if (warp == 0) s_vote[(votes + 2) & 3] = 0;  // (read two votes ago)
+        if (mine) s_vote[votes & 3] = 1;
+        mbar_arrive(voted);
+      }
+      ok = att_wait_warp(voted, votes & 1, s_abort, a.err, 70);
+      return s_vote[votes++ & 3] != 0;
+    };
     // What an item means to this thread; looked up an item ahead.
     struct Mine {
-      int tile, head, first, end, total, row;
+      int tile, head, first, end, total, row, low_max, high_min;
       int2 seen;
       float lse2, delta;
     };
@@ -372,6 +327,8 @@ __global__ void __launch_bounds__(kThreads, 1)
       m.first = r.first;
       m.end = r.end;
       m.total = max(0, r.end - r.first) * per;
+      m.low_max = r.low_max;
+      m.high_min = r.high_min;
       m.row = m.tile * kAttTile + row;
       m.seen = att_interval<!KEYS>(a, m.row);
       m.lse2 = m.delta = 0.0f;
@@ -389,6 +346,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const int2 seen = it.seen;
       const int len = seen.y - seen.x;
       const float lse2 = it.lse2, delta = it.delta;
+      bool flagged = false;  // values that are not finite were set to 0
       int t = it.first;
       if (id + (int)gridDim.x < a.items) next = mine_at(id + gridDim.x);  // (its loads have this item's time)
       for (int i = 0; i < total; i++, use++) {
@@ -398,36 +356,45 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
         const int off = seen.x - t * kAttTile - half * 64;  // of this half of the tile
-        if (__all_sync(~0u, off >= 64 || off + len <= 0)) {
-          // None of these rows meets any of it.
-          const uint32_t zero[16] = {};
-          if (KEYS) {
-            att_tm_store16(ts, zero);
-            att_tm_store16(ts + 16, zero);
-            att_tm_store_wait();
-          }
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(p_full);
-          ok = att_wait_warp(dp_full, s_use & 1, s_abort, a.err, 74);
-          if (!ok) break;
-          s_use++;
-          tc_fence_after();
-          att_tm_store16(tdp, zero);
-          att_tm_store16(tdp + 16, zero);
-          att_tm_store_wait();
-          tc_fence_before();
-          __syncwarp();
-          if (lane == 0) mbar_arrive(ds_full);
-          if (++t == it.end) t = it.first;
-          continue;
-        }
-        const bool whole = __all_sync(~0u, off <= 0 && off + len >= 64);
+        const bool whole = off <= 0 && off + len >= 64, all_whole = __all_sync(~0u, whole);
         float p[64];
         att_tm_load(ts, p);
         att_tm_load(ts + 32, p + 32);
         att_tm_wait(p);
         att_tm_wait(p + 32);
+        if (att_masked(it.low_max, it.high_min, t)) {
+          // Values of the passing tiles that are not finite would reach rows that do not
+          // meet them through the products with p and ds (0 times them). They show in
+          // every row of the scores and of dp. Where there are any, they become 0 in the
+          // tiles now that scores and dp are multiplied, and the results add them again.
+          F2 probe = pack_f2(0.0f);
+          const F2 zero = probe;
+#pragma unroll
+          for (int c = 0; c < 64; c += 2) probe = fma2(pack_f2(p[c], p[c + 1]), zero, probe);
+          if (KEYS) {
+            ok = att_wait_warp(dp_full, s_use & 1, s_abort, a.err, 73);
+            if (!ok) break;
+            tc_fence_after();
+#pragma unroll 1
+            for (int c0 = 0; c0 < 64; c0 += 32) {
+              float v[32];
+              att_tm_load(tdp + c0, v);
+              att_tm_wait(v);
+#pragma unroll
+              for (int c = 0; c < 32; c += 2) probe = fma2(pack_f2(v[c], v[c + 1]), zero, probe);
+            }
+          }
+          const bool any = vote(sum_f2(probe) != 0.0f);
+          if (!ok) break;
+          if (any) {
+            flagged = true;
+            att_clean<DP, F16>(s_b1 + use % S1 * TILE, warp, kCompute / 32);
+            if (KEYS) att_clean<DP, F16>(s_b2 + use % S2 * TILE, warp, kCompute / 32);
+            att_fence_async();
+            vote(false);
+            if (!ok) break;
+          }
+        }
         if (!KEYS) {
           tc_fence_before();
           __syncwarp();
@@ -456,7 +423,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int j = 0; j < 4; j++) p[c + j] = att_ex2(e[j]);
         }
         uint32_t in[2] = {~0u, ~0u};
-        if (!whole) {
+        if (!all_whole) {
           in[0] = att_bits(off, len, 0);
           in[1] = att_bits(off, len, 32);
 #pragma unroll
@@ -512,7 +479,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // Masked places: p is 0, but dp and delta may hold anything.
-        if (!whole) {
+        if (!all_whole) {
 #pragma unroll
           for (int c = 0; c < 32; c++) {
             const uint32_t two = in[c >> 4] >> (2 * c & 31) & 3;
@@ -534,8 +501,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (!ok) break;
         tc_fence_after();
       }
-      const bool flagged = total > 0 && s_flag[count % kAttFlags];
-      if (total > 0) count++;
       const bool dv = KEYS && half;
       const uint32_t from = tmem + lanes + (dv ? kCol2 : kCol1);
       const float f = dv ? (F16 ? 0x1p-14f : 1.0f) : a.scale / gain;
