@@ -570,3 +570,54 @@ def test_items_after_empty_ones(gpu, heads, kv, d, causal):
         out, lse = ops.attention_forward(q, k, v, cu, causal)
         got = (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu, causal))
         assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("causal", [False, True])
+@pytest.mark.parametrize("first,last", [(0, 300), (5, 300), (130, 131), (100, 260), (128, 256), (0, 0), (299, 300), (256, 300)])
+def test_one_sequence_within_the_tokens(gpu, first, last, causal):
+    """A single sequence that starts and ends anywhere: the tokens before and behind it see nothing."""
+    import torch
+    from vector_cuda import ops
+    q, k, v, do = _make([300], 4, 2, 64, "float16")
+    cu = torch.tensor([first, last], dtype=torch.int32, device="cuda")
+    out, lse = ops.attention_forward(q, k, v, cu, causal)
+    got = (out, *ops.attention_backward(do, q, k, v, out, lse, cu, causal))
+    part = slice(first, last)
+    if last > first:
+        # the same as three sequences, whose bounds are looked up the other way
+        three = torch.tensor([0, first, last, 300], dtype=torch.int32, device="cuda")
+        o3, l3 = ops.attention_forward(q, k, v, three, causal)
+        want = (o3, *ops.attention_backward(do, q, k, v, o3, l3, three, causal))
+        assert torch.equal(lse[:, part], l3[:, part])
+        for a, b in zip(got, want):
+            assert torch.equal(a[part], b[part])
+        _check(q[part].contiguous(), k[part].contiguous(), v[part].contiguous(), do[part].contiguous(), [last - first], causal)
+    outside = torch.ones(300, dtype=torch.bool)
+    outside[part] = False
+    assert all(not t[outside].any() for t in got) and (lse[:, outside] == -math.inf).all()
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(gpu):
+    """Tokens so far apart that their elements' numbers pass 2^32."""
+    import torch
+    from vector_cuda import ops
+    lengths, heads, kv, d = [1500, 600], 2, 1, 64
+    q, k, v, do = _make(lengths, heads, kv, d, "bfloat16")
+    cu = _bounds(lengths)
+    want = _check(q, k, v, do, lengths)
+    far = torch.empty(2100, 1 << 21, dtype=torch.bfloat16, device="cuda")  # 8.8 GB
+    x = [far[:, i * 256:i * 256 + t.shape[1] * d].view(2100, t.shape[1], d) for i, t in enumerate((q, k, v, do))]
+    for a, b in zip(x, (q, k, v, do)):
+        a.copy_(b)
+    x[1][1700, 0, 3] = float("nan")  # (the values that are read again, too)
+    k = k.clone()
+    k[1700, 0, 3] = float("nan")
+    out, lse = ops.attention_forward(q, k, v, cu)
+    near = (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu))
+    out, lse = ops.attention_forward(*x[:3], cu)
+    got = (out, lse, *ops.attention_backward(x[3], *x[:3], out, lse, cu))
+    for a, b in zip(near, got):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
+    assert torch.equal(got[0][:1500], want[0][:1500])

@@ -264,3 +264,18 @@ def test_c_refusals(vc):
                 dict(g=Grad(256, 514, 8, 1, 0)), dict(g=Grad(256, 512, -1, 1, 0)), dict(g=Grad(256, 512, 8, 3, 0)),
                 dict(g=Grad(256, 512, 8, 1, 2)), dict(g=Grad(256, 256, 8, 1, 0)), dict(g=Grad(256, 512, 1 << 43, 1, 0))):
         assert call(**bad) == 5, bad
+
+
+@pytest.mark.gpu
+def test_a_tensor_beyond_32_bits(gpu):
+    import torch
+    from vector_cuda import ops
+    n = (1 << 32) + 4099
+    t = torch.zeros(n, dtype=torch.float16, device="cuda")  # 8.6 GB
+    t[5] = t[(1 << 31) + 9] = t[(1 << 32) + 4098] = 2.0
+    t[(1 << 32) + 1] = -1.0
+    norm = ops.clip_grad_norm([t], 1.0)
+    _near_norm(norm, math.sqrt(13.0))
+    for at, was in ((5, 2.0), ((1 << 31) + 9, 2.0), ((1 << 32) + 4098, 2.0), ((1 << 32) + 1, -1.0)):
+        assert abs(t[at].item() - was / (math.sqrt(13.0) + 1e-6)) <= 2.0 ** -11
+    assert not t[6:(1 << 31) + 9].any() and not t[(1 << 31) + 10:(1 << 32) + 1].any()

@@ -297,3 +297,18 @@ def test_c_refusals(vc):
     a = n.value
     assert L.vrs_qk_norm_rope_backward_workspace(ctypes.c_int64(5000), ctypes.c_int64(128), ctypes.byref(n)) == 0
     assert n.value >= a > 0
+
+
+@pytest.mark.gpu
+def test_offsets_beyond_32_bits(gpu):
+    """Tokens so far apart that their elements' numbers pass 2^32."""
+    import torch
+    s = _make(2100, 2, 1, 64, "bfloat16", "bfloat16")
+    far = torch.empty(2100, 1 << 21, dtype=torch.bfloat16, device="cuda")  # 8.8 GB
+    v = dict(s)
+    for i, n in enumerate(("q", "k", "dq_out", "dk_out")):
+        v[n] = far[:, i * 256:i * 256 + s[n].shape[1] * 64].view(2100, s[n].shape[1], 64)
+        v[n].copy_(s[n])
+    want, wantg = _check(s)
+    got, gotg = _check(v)
+    assert all(torch.equal(want[n], got[n]) for n in want) and all(torch.equal(wantg[n], gotg[n]) for n in wantg)

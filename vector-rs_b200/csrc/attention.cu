@@ -185,16 +185,18 @@ int start(const Call& c, void* seg, unsigned* zero, AttArgs& a, cudaStream_t s) 
   a.scale = c.scale;
   a.c2 = c.scale * 1.44269504088896341f;
   a.seq_len = c.cu ? 0 : (int)(c.tokens / c.sequences);
+  a.two = c.cu && c.sequences == 1 ? (const int*)c.cu : nullptr;
   a.seg = nullptr;
   VRS_TRY(error_word(&a.err));
-  if (!c.cu && !zero) return VRS_OK;
+  const bool look = c.cu && !a.two;  // (a single sequence's bounds are read where they are needed)
+  if (!look && !zero) return VRS_OK;
   int4* spans = (int4*)((char*)seg + up(c.tokens * 8, 256));
-  if (c.cu) {
+  if (look) {
     a.seg = (const int2*)seg;
     a.spans = spans;
   }
-  VRS_TRY(launch_after(attention_sequences_kernel, c.cu ? (unsigned)a.tiles : 1u, kAttTile, 0, s, (const int*)c.cu,
-                       (int)c.sequences, (int2*)seg, spans, zero, a));
+  VRS_TRY(launch_after(attention_sequences_kernel, look ? (unsigned)a.tiles : 1u, kAttTile, 0, s,
+                       look ? (const int*)c.cu : nullptr, (int)c.sequences, (int2*)seg, spans, zero, a));
   count_launch();
   return VRS_OK;
 }
@@ -277,7 +279,7 @@ extern "C" int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, con
       a.pairing = kAttTwoTiles;
       a.items = (int)((a.tiles + 1) / 2 * heads);
     }
-    if (cu_seqlens && a.items > sms)
+    if (a.seg && a.items > sms)
       st = sort_units(a, workspace, a.pairing == kAttTwoTiles ? 2 : 1, false, s);
     if (st == VRS_OK) st = launch_attention_forward(f16, d <= 64 ? 64 : 128, maps, a, sms, s);
   }
@@ -383,7 +385,7 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
   }
   const int dp = d <= 64 ? 64 : 128;
   const int* order = nullptr;
-  if (st == VRS_OK && cu_seqlens && (int64_t)a.tiles * heads > sms) {
+  if (st == VRS_OK && a.seg && (int64_t)a.tiles * heads > sms) {
     st = sort_units(a, ws + p.seg, 1, true, s);
     order = a.order;
   }

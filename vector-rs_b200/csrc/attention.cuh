@@ -31,7 +31,8 @@ constexpr int kAttFlags = 16;                    // items that the "not finite" 
 struct AttArgs {
   int tokens, heads, kv_heads, group, d, tiles;
   int causal;
-  int seq_len;        // of every sequence, where seg is null
+  int seq_len;        // of every sequence, where two and seg are null
+  const int* two;     // the bounds of a single sequence
   const int2* seg;    // per token: its sequence's first token and the one past its last
   const int4* spans;  // beside seg: per tile what its rows meet, as queries, then as keys
   const int* order;   // units of work (tiles, or pairs of them), the longest first; null: by number
@@ -73,7 +74,10 @@ template <bool KEYS>
 __device__ __forceinline__ int2 att_interval(const AttArgs& a, int i) {
   if (i >= a.tokens) return make_int2(0, 0);
   int2 r;
-  if (a.seg) {
+  if (a.two) {
+    r = make_int2(max(a.two[0], 0), min(a.two[1], a.tokens));
+    if (i < r.x || i >= r.y) return make_int2(0, 0);
+  } else if (a.seg) {
     r = a.seg[i];
   } else {
     r.x = i / a.seq_len * a.seq_len;
@@ -92,6 +96,22 @@ struct AttSpan {
 template <bool KEYS, bool UNIFORM>
 __device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
   AttSpan s;
+  const int t0 = tile * kAttTile, last = min(a.tokens, t0 + kAttTile) - 1;
+  if (a.two) {
+    int lo = max(a.two[0], 0), hi = min(a.two[1], a.tokens);
+    if (UNIFORM) {
+      lo = __reduce_min_sync(~0u, lo);
+      hi = __reduce_min_sync(~0u, hi);
+    }
+    const int r0 = max(t0, lo), r1 = min(last + 1, hi);  // rows of the sequence
+    if (r0 >= r1) return AttSpan{0, 0, INT_MAX, 0};
+    const bool all = r0 == t0 && r1 == last + 1;
+    s.first = (a.causal && !KEYS ? r0 : lo) / kAttTile;
+    s.end = ((a.causal && KEYS ? r1 : hi) + kAttTile - 1) / kAttTile;
+    s.low_max = !all ? INT_MAX : a.causal && !KEYS ? r1 - 1 : lo;
+    s.high_min = a.causal && KEYS ? r0 + 1 : hi;
+    return s;
+  }
   if (a.seg) {
     const int4 v = a.spans[KEYS ? tile : a.tiles + tile];
     if (!UNIFORM) return AttSpan{v.x, v.y, v.z, v.w};
@@ -101,7 +121,6 @@ __device__ __forceinline__ AttSpan att_span(const AttArgs& a, int tile) {
     s.high_min = __reduce_min_sync(~0u, v.w);
     return s;
   }
-  const int t0 = tile * kAttTile, last = min(a.tokens, t0 + kAttTile) - 1;
   const int lo0 = t0 / a.seq_len * a.seq_len, lo1 = last / a.seq_len * a.seq_len;  // sequences of the first and last row
   s.first = (a.causal && !KEYS ? t0 : lo0) / kAttTile;
   s.end = ((a.causal && KEYS ? last + 1 : lo1 + a.seq_len) + kAttTile - 1) / kAttTile;
