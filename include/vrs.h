@@ -386,9 +386,9 @@ VRS_API int vrs_linear_cross_entropy_backward_with_loss(
  * norm: its attention with the norms and rotation of queries and keys before
  * it, and the norm and clipping of a training step's gradients. Everything said
  * of the training operators holds here: buffers, streams, workspaces (which
- * never shrink as a size grows), determinism, errors, capture. Stage names of vrs_profile_read: "attention_forward",
- * "attention_backward", "qk_norm_rope_forward", "qk_norm_rope_backward",
- * "grad_norm", "clip_grad_norm". */
+ * never shrink as a size grows), determinism, errors, capture. Stage names of
+ * vrs_profile_read: "attention_forward", "attention_backward",
+ * "qk_norm_rope_forward", "qk_norm_rope_backward", "grad_norm", "clip_grad_norm". */
 
 /* tokens x heads x d elements: `stride` between tokens, `head_stride` between
  * heads, both in elements; the d elements of a head are contiguous. */
@@ -408,8 +408,9 @@ typedef struct vrs_heads {
  * no other memory); cu_seqlens NULL: `sequences` of equal length. A token that no
  * sequence holds (behind the last one, say) has out 0 and lse -inf. What a row does
  * not see has no effect on it, infinities and NaN included. The weights e^(...) are
- * rounded to 16 bits for the product with v. The workspace (256-byte aligned) is
- * needed with cu_seqlens only. */
+ * rounded to 16 bits for the product with v. Fewer than 2^31 - 512 tokens, and
+ * heads x tokens below 2^37. The workspace (256-byte aligned) is needed with
+ * cu_seqlens only. */
 VRS_API int vrs_attention_forward_workspace(int64_t tokens, int64_t* out_bytes);
 VRS_API int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const vrs_heads* v, int64_t tokens,
                                   int64_t heads, int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,

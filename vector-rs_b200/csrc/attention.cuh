@@ -11,9 +11,11 @@
 //
 // Operands of a masked pair of tiles may hold values that are not finite in rows
 // that others do not see; their weight is 0, and 0 times such a value would reach
-// the others through the matrix product. The cleaning warps look such a tile
-// through in shared memory before it is multiplied, set what is not finite to 0
-// and raise a flag; rows of results then add the values that they do see.
+// the others through the matrix product. So such a tile is looked through, what is
+// not finite becomes 0 for the product, and rows of results then add the values that
+// they do see: forward by two warps of their own, in shared memory; backward, where
+// such a row shows as a score or a dp that is not finite, by the computing warps (935 us with
+// cleaning warps, 863 so: 8,192 tokens, 8 heads on 2 x 128, not causal).
 #pragma once
 #include <cuda.h>
 
@@ -26,7 +28,7 @@ namespace ops {
 constexpr int kAttTile = 128;                    // tokens of a tile
 constexpr uint32_t kAttBox = 64 * 2 * kAttTile;  // bytes of 64 elements of a tile's rows
 constexpr uint64_t kAttWaitNs = 2000000000ull;
-constexpr int kAttFlags = 16;                    // items that the "not finite" flags tell apart
+constexpr int kAttFlags = 16;                    // items that the forward pass's "not finite" flags tell apart
 
 struct AttArgs {
   int tokens, heads, kv_heads, group, d, tiles;

@@ -15,8 +15,9 @@
 // The tensor cores run in issue order, so the scores of the next tile are issued
 // after the product that reads this tile's p, and dp after the one that reads ds:
 // while the threads work on p, dp is multiplied, and while they work on ds, the
-// next scores are. Bound by the tensor cores: 4 x 512 clocks a pair of tiles for
-// dk and dv, 3 x 512 for dq (d = 128).
+// next scores are. Bound by that chain: a pair of tiles takes 3,500 clocks for dk and
+// dv, 2,300 for dq, of which products are 4 x 512 and 3 x 512 (d = 128). 8,192 tokens,
+// 8 heads on 2, not causal 863 us (796 TFLOP/s of the five products).
 #include <atomic>
 
 #include "attention.cuh"
@@ -145,153 +146,153 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int per = KEYS ? a.group : 1;  // passes over the tiles: the query heads of a key's
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kLoadWarp) {
-    // ------------------------------------------------------------ loads
-    int use = 0, a_use = 0, n1 = 0, n2 = 0;
-    bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const int tile = tile_of(id), head = id % heads;
-      const AttSpan r = att_span<!KEYS, true>(a, tile);
-      if (lane == 0) {
-        const int n = max(0, r.end - r.first), total = n * per;
-        auto rows = [&] {
-          ok = att_wait(a_empty, (a_use & 1) ^ 1, s_abort, a.err, 61);
-          if (!ok) return;
-          mbar_expect_tx(a_full, 2 * TILE);
-          att_load_tile<DP>(s_a, KEYS ? &maps.k : &maps.q, KEYS ? a.k_last : a.q_last, head, tile * kAttTile, a_full);
-          att_load_tile<DP>(s_a + TILE, KEYS ? &maps.v : &maps.dout, KEYS ? a.v_last : a.dout_last, head, tile * kAttTile,
-                            a_full);
-          a_use++;
-        };
-        int t = r.first, g = 0;
-        for (int i = 0; ok && i < total; i++, use++) {
-          const int s1 = use % S1, s2 = use % S2;
-          ok = att_wait(&empty1[s1], (use / S1 & 1) ^ 1, s_abort, a.err, 62);
-          if (!ok) break;
-          n1 = use + 1;
-          const int h = KEYS ? head * a.group + g : head / a.group;
-          const int64_t at = (int64_t)h * a.padded + t * kAttTile;
-          if (KEYS) {
-            mbar_expect_tx(&full1[s1], TILE + kStatBytes);
-            att_load_tile<DP>(s_b1 + s1 * TILE, &maps.q, a.q_last, h, t * kAttTile, &full1[s1]);
-            bulk_copy_g2s(s_delta + s1 * kAttTile, a.delta + at, kStatBytes, &full1[s1]);
-          } else {
-            mbar_expect_tx(&full1[s1], TILE);
-            att_load_tile<DP>(s_b1 + s1 * TILE, &maps.k, a.k_last, h, t * kAttTile, &full1[s1]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------ loads
+      int use = 0, a_use = 0, n1 = 0, n2 = 0;
+      bool ok = true;
+      for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+        const int tile = tile_of(id), head = id % heads;
+        const AttSpan r = att_span<!KEYS, true>(a, tile);
+        if (lane == 0) {
+          const int n = max(0, r.end - r.first), total = n * per;
+          auto rows = [&] {
+            ok = att_wait(a_empty, (a_use & 1) ^ 1, s_abort, a.err, 61);
+            if (!ok) return;
+            mbar_expect_tx(a_full, 2 * TILE);
+            att_load_tile<DP>(s_a, KEYS ? &maps.k : &maps.q, KEYS ? a.k_last : a.q_last, head, tile * kAttTile, a_full);
+            att_load_tile<DP>(s_a + TILE, KEYS ? &maps.v : &maps.dout, KEYS ? a.v_last : a.dout_last, head, tile * kAttTile,
+                              a_full);
+            a_use++;
+          };
+          int t = r.first, g = 0;
+          for (int i = 0; ok && i < total; i++, use++) {
+            const int s1 = use % S1, s2 = use % S2;
+            ok = att_wait(&empty1[s1], (use / S1 & 1) ^ 1, s_abort, a.err, 62);
+            if (!ok) break;
+            n1 = use + 1;
+            const int h = KEYS ? head * a.group + g : head / a.group;
+            const int64_t at = (int64_t)h * a.padded + t * kAttTile;
+            if (KEYS) {
+              mbar_expect_tx(&full1[s1], TILE + kStatBytes);
+              att_load_tile<DP>(s_b1 + s1 * TILE, &maps.q, a.q_last, h, t * kAttTile, &full1[s1]);
+              bulk_copy_g2s(s_delta + s1 * kAttTile, a.delta + at, kStatBytes, &full1[s1]);
+            } else {
+              mbar_expect_tx(&full1[s1], TILE);
+              att_load_tile<DP>(s_b1 + s1 * TILE, &maps.k, a.k_last, h, t * kAttTile, &full1[s1]);
+            }
+            ok = att_wait(&empty2[s2], (use / S2 & 1) ^ 1, s_abort, a.err, 77);
+            if (!ok) break;
+            n2 = use + 1;
+            if (KEYS) {
+              mbar_expect_tx(&full2[s2], TILE + kStatBytes);
+              att_load_tile<DP>(s_b2 + s2 * TILE, &maps.dout, a.dout_last, h, t * kAttTile, &full2[s2]);
+              bulk_copy_g2s(s_lse2 + s2 * kAttTile, a.lse2 + at, kStatBytes, &full2[s2]);
+            } else {
+              mbar_expect_tx(&full2[s2], TILE);
+              att_load_tile<DP>(s_b2 + s2 * TILE, &maps.v, a.v_last, h, t * kAttTile, &full2[s2]);
+            }
+            if (++t == r.end) {
+              t = r.first;
+              g++;
+            }
+            if (i == 0) rows();  // (the first pair's place comes free before the rows')
           }
-          ok = att_wait(&empty2[s2], (use / S2 & 1) ^ 1, s_abort, a.err, 77);
-          if (!ok) break;
-          n2 = use + 1;
-          if (KEYS) {
-            mbar_expect_tx(&full2[s2], TILE + kStatBytes);
-            att_load_tile<DP>(s_b2 + s2 * TILE, &maps.dout, a.dout_last, h, t * kAttTile, &full2[s2]);
-            bulk_copy_g2s(s_lse2 + s2 * kAttTile, a.lse2 + at, kStatBytes, &full2[s2]);
-          } else {
-            mbar_expect_tx(&full2[s2], TILE);
-            att_load_tile<DP>(s_b2 + s2 * TILE, &maps.v, a.v_last, h, t * kAttTile, &full2[s2]);
-          }
-          if (++t == r.end) {
-            t = r.first;
-            g++;
-          }
-          if (i == 0) rows();  // (the first pair's place comes free before the rows')
+          if (total == 0) rows();
         }
-        if (total == 0) rows();
+        ok = __shfl_sync(~0u, ok, 0);
       }
-      ok = __shfl_sync(~0u, ok, 0);
-    }
-    if (lane == 0 && *s_abort) {
-      // Drain (bounded) before shared memory goes.
-      volatile int dummy = 0;
-      for (int i = max(0, n1 - S1); i < n1; i++) mbar_wait(&full1[i % S1], i / S1 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
-      for (int i = max(0, n2 - S2); i < n2; i++) mbar_wait(&full2[i % S2], i / S2 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
-      if (a_use) mbar_wait(a_full, (a_use - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ products
-    const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
-    const uint64_t b1k = smem_desc_sw128(s_b1), b1m = att_desc_mn(s_b1);
-    const uint64_t b2k = smem_desc_sw128(s_b2), b2m = att_desc_mn(s_b2);
-    constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
-    // The whole warp goes through the loops, one lane issues.
-    const bool lead = att_elect();
-    const uint32_t tm = __reduce_min_sync(~0u, tmem);
-    int use = 0, a_use = 0;
-    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
-    auto scores = [&](int u) {  // rows x (q or k)
-      const int st = u % S1;
-      wait(&full1[st], u / S1, 64);
-      tc_fence_after();
-      if (lead) {
-        const uint64_t bd = b1k + st * (TILE >> 4);
-#pragma unroll
-        for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColS, a1 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
-        mma_commit(s_full);
+      if (lane == 0 && *s_abort) {
+        // Drain (bounded) before shared memory goes.
+        volatile int dummy = 0;
+        for (int i = max(0, n1 - S1); i < n1; i++) mbar_wait(&full1[i % S1], i / S1 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+        for (int i = max(0, n2 - S2); i < n2; i++) mbar_wait(&full2[i % S2], i / S2 & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+        if (a_use) mbar_wait(a_full, (a_use - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
       }
-    };
-    auto dps = [&](int u, bool last) {  // rows x (dout or v)
-      const int st = u % S2;
-      wait(&full2[st], u / S2, 67);
-      tc_fence_after();
-      if (lead) {
-        const uint64_t bd = b2k + st * (TILE >> 4);
-#pragma unroll
-        for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
-        mma_commit(dp_full);
-        if (!KEYS) mma_commit(&empty2[st]);
-        if (last) mma_commit(a_empty);
-      }
-    };
-    // (p or ds over its own columns, each half of a row in its half of them) x a tile
-    auto product = [&](uint32_t to, uint32_t from, uint64_t bd, bool add) {
-#pragma unroll
-      for (int k = 0; k < kAttTile / 16; k++)
-        att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
-    };
-    for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
-      const AttSpan r = att_span<!KEYS, true>(a, tile_of(id));
-      const int total = max(0, r.end - r.first) * per;
-      // (The rows are waited for where nothing is multiplied too: a wait for the
-      // next ones that came before these have would not see the difference.)
-      wait(a_full, a_use++, 63);
-      if (total == 0) {
-        if (lead) mbar_arrive(a_empty);
-        continue;
-      }
-      scores(use);
-      dps(use, total == 1);
-#pragma unroll 1
-      for (int i = 0; i < total; i++, use++) {
-        const int s1 = use % S1, s2 = use % S2;
-        const bool more = i + 1 < total;
-        wait(p_full, use, 65);
-        if (KEYS) {
-          tc_fence_after();
-          if (lead) {
-            product(kCol2, kColS, b2m + s2 * (TILE >> 4), i > 0);
-            mma_commit(&empty2[s2]);
-          }
-        }
-        if (more) scores(use + 1);
-        wait(ds_full, use, 68);
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------ products
+      const uint64_t a1 = smem_desc_sw128(s_a), a2 = a1 + (TILE >> 4);
+      const uint64_t b1k = smem_desc_sw128(s_b1), b1m = att_desc_mn(s_b1);
+      const uint64_t b2k = smem_desc_sw128(s_b2), b2m = att_desc_mn(s_b2);
+      constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_r = att_idesc<F16>(DP, true);
+      // The whole warp goes through the loops, one lane issues.
+      const bool lead = att_elect();
+      const uint32_t tm = __reduce_min_sync(~0u, tmem);
+      int use = 0, a_use = 0;
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
+      auto scores = [&](int u) {  // rows x (q or k)
+        const int st = u % S1;
+        wait(&full1[st], u / S1, 64);
         tc_fence_after();
         if (lead) {
-          product(kCol1, kColDp, b1m + s1 * (TILE >> 4), i > 0);
-          mma_commit(&empty1[s1]);
-          if (!more) mma_commit(r_full);
+          const uint64_t bd = b1k + st * (TILE >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColS, a1 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+          mma_commit(s_full);
         }
-        if (more) dps(use + 1, i + 2 == total);
+      };
+      auto dps = [&](int u, bool last) {  // rows x (dout or v)
+        const int st = u % S2;
+        wait(&full2[st], u / S2, 67);
+        tc_fence_after();
+        if (lead) {
+          const uint64_t bd = b2k + st * (TILE >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++) mma_f16(tm + kColDp, a2 + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+          mma_commit(dp_full);
+          if (!KEYS) mma_commit(&empty2[st]);
+          if (last) mma_commit(a_empty);
+        }
+      };
+      // (p or ds over its own columns, each half of a row in its half of them) x a tile
+      auto product = [&](uint32_t to, uint32_t from, uint64_t bd, bool add) {
+#pragma unroll
+        for (int k = 0; k < kAttTile / 16; k++)
+          att_mma_ts(tm + to, tm + from + (k >> 2) * 64 + (k & 3) * 8, bd + att_mn_step(k), idesc_r, k > 0 || add);
+      };
+      for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
+        const AttSpan r = att_span<!KEYS, true>(a, tile_of(id));
+        const int total = max(0, r.end - r.first) * per;
+        // (The rows are waited for where nothing is multiplied too: a wait for the
+        // next ones that came before these have would not see the difference.)
+        wait(a_full, a_use++, 63);
+        if (total == 0) {
+          if (lead) mbar_arrive(a_empty);
+          continue;
+        }
+        scores(use);
+        dps(use, total == 1);
+#pragma unroll 1
+        for (int i = 0; i < total; i++, use++) {
+          const int s1 = use % S1, s2 = use % S2;
+          const bool more = i + 1 < total;
+          wait(p_full, use, 65);
+          if (KEYS) {
+            tc_fence_after();
+            if (lead) {
+              product(kCol2, kColS, b2m + s2 * (TILE >> 4), i > 0);
+              mma_commit(&empty2[s2]);
+            }
+          }
+          if (more) scores(use + 1);
+          wait(ds_full, use, 68);
+          tc_fence_after();
+          if (lead) {
+            product(kCol1, kColDp, b1m + s1 * (TILE >> 4), i > 0);
+            mma_commit(&empty1[s1]);
+            if (!more) mma_commit(r_full);
+          }
+          if (more) dps(use + 1, i + 2 == total);
+        }
+      }
+      if (*s_abort) {
+        // MMAs in flight must not outlive the block's tensor memory: one more
+        // commit, waited for (bounded).
+        volatile int dummy = 0;
+        if (lead) mma_commit(drain);
+        mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
       }
     }
-    if (*s_abort) {
-      // MMAs in flight must not outlive the block's tensor memory: one more
-      // commit, waited for (bounded).
-      volatile int dummy = 0;
-      if (lead) mma_commit(drain);
-      mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
-    }
-  }
   } else {
     // ------------------------------------------------------------ p, ds, results
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kComputeRegs));

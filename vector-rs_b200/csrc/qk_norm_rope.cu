@@ -175,8 +175,9 @@ struct Angles {
 // that each lane fills for itself some turns ahead. What bounds it then is the number
 // of instructions, so the heads of queries and of keys are passes of their own whose
 // addresses only step, and arithmetic goes by pairs of floats (32,768 tokens of
-// 16 + 4 heads x 128 bf16: 240 instructions a turn and 97 us forward, 362 and 153
-// backward, with 8-byte accesses, single floats and addresses formed a head).
+// 16 + 4 heads x 128 bf16, a warp's instructions for 8 elements of each lane: 240 and 97 us
+// forward, 362 and 153 backward, with 8-byte accesses, single floats and addresses
+// formed a head; 150 and 75, 195 and 114, so. The bytes alone take 51 and 77 us).
 template <class T, int S, int V>
 constexpr int ring_of() { return S * V * sizeof(T) <= 8 ? 4 : 2; }
 

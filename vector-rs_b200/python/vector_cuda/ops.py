@@ -1,15 +1,17 @@
-"""vector_cuda.ops -- training operators over libvrs, on torch CUDA tensors.
+"""vector_cuda.ops -- training and encoder operators over libvrs, on torch CUDA
+tensors.
 
-What produces and trains the vectors that an index holds: the layer norm at
-an encoder's end, and the softmax cross entropy of a row's scores against
-every row of a table of vectors (the inner products that a dot-product search
-ranks), without keeping the scores. Neither has a counterpart in the
-reference, whose vectors come from outside.
+What produces and trains the vectors that an index holds: a text encoder's
+attention over packed sequences, with the norms and rotation of its queries and
+keys; the layer norm at its end; the softmax cross entropy of a row's scores
+against every row of a table of vectors (the inner products that a dot-product
+search ranks), without keeping the scores; and the norm and clipping of a step's
+gradients. None has a counterpart in the reference, whose vectors come from outside.
 
-``layer_norm`` and ``linear_cross_entropy`` take part in autograd; the
-``*_forward`` and ``*_backward`` functions are the passes by themselves.
-Every call queues its work on torch's current stream of the tensors' device
-and returns without waiting. There is no CPU fallback.
+``attention``, ``qk_norm_rope``, ``layer_norm`` and ``linear_cross_entropy`` take
+part in autograd; the ``*_forward`` and ``*_backward`` functions are the passes
+by themselves. Every call queues its work on torch's current stream of the
+tensors' device and returns without waiting. There is no CPU fallback.
 """
 from __future__ import annotations
 
