@@ -421,8 +421,8 @@ VRS_API int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const 
  * (NULL: not wanted), dk and dv (both or neither NULL), in dtype. Weights and
  * their gradients are formed again and rounded to 16 bits as operands of the
  * products: VRS_F16 keeps the latter relative to the largest row of dout times
- * the largest row of v, down to 2^-38 of that. Tokens that no sequence holds have
- * gradients 0. */
+ * the largest row of v (rows of sequences, values that are finite), down to 2^-38
+ * of that. Tokens that no sequence holds have gradients 0. */
 VRS_API int vrs_attention_backward_workspace(int64_t tokens, int64_t heads, int64_t* out_bytes);
 VRS_API int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q, const vrs_heads* k, const vrs_heads* v,
                                    const vrs_heads* out, const float* lse, int64_t tokens, int64_t heads,

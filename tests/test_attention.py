@@ -621,3 +621,54 @@ def test_offsets_beyond_32_bits(gpu):
     for a, b in zip(near, got):
         assert torch.equal(a.isnan(), b.isnan()) and torch.equal(a.nan_to_num(), b.nan_to_num())
     assert torch.equal(got[0][:1500], want[0][:1500])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), 60000.0, -3e4])
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("first,lengths,behind", [(0, [100, 60], 40), (130, [90, 200], 0), (7, [1, 0, 250], 300), (9, [150], 5)])
+def test_tokens_of_no_sequence_hold_anything(gpu, first, lengths, behind, dtype, value):
+    """Queries, keys, values and output gradients before the first sequence and
+    behind the last: the results are those of zeros there, bit for bit."""
+    import torch
+    from vector_cuda import ops
+    tokens = first + sum(lengths) + behind
+    cu = _bounds(lengths) + first
+    arrays = list(_make([tokens], 4, 2, 64, dtype))
+    none = torch.ones(tokens, dtype=torch.bool, device="cuda")
+    none[first:first + sum(lengths)] = False
+
+    def run(fill):
+        q, k, v, do = (torch.where(none[:, None, None], torch.full_like(t, fill), t) for t in arrays)
+        out, lse = ops.attention_forward(q, k, v, cu)
+        return (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu))
+
+    for a, b in zip(run(0.0), run(value)):
+        assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_calls_on_two_streams_at_once(gpu):
+    """Both passes of two calls, again and again on a stream each: every turn has
+    the bits of a call by itself."""
+    import torch
+    from vector_cuda import ops
+    calls = []
+    for lengths, dtype in (([300, 1, 700, 64], "float16"), ([50] * 30, "bfloat16")):
+        q, k, v, do = _make(lengths, 8, 2, 128, dtype)
+        calls.append((q, k, v, do, _bounds(lengths), torch.cuda.Stream()))
+
+    def run(q, k, v, do, cu, _):
+        out, lse = ops.attention_forward(q, k, v, cu)
+        return (out, lse, *ops.attention_backward(do, q, k, v, out, lse, cu))
+
+    want = [run(*c) for c in calls]
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(5):
+        for g, c in zip(got, calls):
+            with torch.cuda.stream(c[5]):
+                g.append(run(*c))
+    torch.cuda.synchronize()
+    for g, w in zip(got, want):
+        assert all(torch.equal(a, b) for turn in g for a, b in zip(turn, w))

@@ -578,6 +578,9 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
     const uint16_t* y = value ? x : b.out + h * b.oh;
     const int64_t xs = value ? a.vs : a.dos, ys = value ? a.vs : b.os;
     float mine = 0.0f, top = 0.0f;
+    // Rows that no sequence holds may hold anything; they bound nothing.
+    const bool none = att_interval<true>(a, t0 + lane).y == 0;
+    const uint32_t held = F16 ? __ballot_sync(~0u, !none) : 0;
 #pragma unroll 4
     for (int r = 0; r < 16; r++) {
       const int t = t0 + 2 * r + group;
@@ -589,7 +592,7 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
         xy += __shfl_xor_sync(~0u, xy, o);
         if (F16) xx += __shfl_xor_sync(~0u, xx, o);
       }
-      if (F16 && xx < INFINITY) top = fmaxf(top, xx);
+      if (F16 && (held >> (2 * r + group) & 1) && xx < INFINITY) top = fmaxf(top, xx);
       const float lo = __shfl_sync(~0u, xy, 0), hi = __shfl_sync(~0u, xy, 16);
       if (lane >> 1 == r) mine = lane & 1 ? hi : lo;
     }
@@ -601,7 +604,6 @@ __global__ void __launch_bounds__(256) attention_stats_kernel(const __grid_const
     const int t = t0 + lane;
     const int64_t at = (int64_t)h * b.padded + t;
     const float lse = t < a.tokens ? a.lse[(int64_t)h * a.tokens + t] : -INFINITY;
-    const bool none = att_interval<true>(a, t).y == 0;
     b.lse2[at] = none ? INFINITY : fabsf(lse) < INFINITY ? lse * 1.44269504088896341f : NAN;
     b.delta[at] = none ? 0.0f : fabsf(mine) < INFINITY ? mine : NAN;
   }
