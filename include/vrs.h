@@ -408,9 +408,9 @@ typedef struct vrs_heads {
  * no other memory); cu_seqlens NULL: `sequences` of equal length. A token that no
  * sequence holds (behind the last one, say) has out 0 and lse -inf. What a row does
  * not see has no effect on it, infinities and NaN included. The weights e^(...) are
- * rounded to 16 bits for the product with v. Fewer than 2^31 - 512 tokens, and
- * heads x tokens below 2^37. The workspace (256-byte aligned) is needed with
- * cu_seqlens only. */
+ * rounded to 16 bits for the product with v. scale is positive and below 2^127;
+ * at most 2^31 - 512 tokens, and heads x tokens below 2^37. The workspace
+ * (256-byte aligned) is needed with cu_seqlens only. */
 VRS_API int vrs_attention_forward_workspace(int64_t tokens, int64_t* out_bytes);
 VRS_API int vrs_attention_forward(const vrs_heads* q, const vrs_heads* k, const vrs_heads* v, int64_t tokens,
                                   int64_t heads, int64_t kv_heads, int64_t d, int32_t dtype, const int32_t* cu_seqlens,
@@ -474,7 +474,7 @@ VRS_API int vrs_grad_norm(const vrs_grad* grads, int64_t tensors, float unscale,
                           int64_t workspace_bytes, void* cuda_stream);
 /* The norm as above, and out = grad * unscale * min(1, max_norm / (norm + 1e-6)).
  * An infinite norm gives zeros, and NaN where the gradient is not finite; a NaN
- * norm gives NaN. In place nothing is written where the factor is 1. Results
+ * norm gives NaN, and so does an infinite one below an infinite max_norm. In place nothing is written where the factor is 1. Results
  * overlap neither one another nor other gradients. */
 VRS_API int vrs_clip_grad_norm(const vrs_grad* grads, int64_t tensors, float max_norm, float unscale, float* norm,
                                void* workspace, int64_t workspace_bytes, void* cuda_stream);

@@ -672,3 +672,13 @@ def test_calls_on_two_streams_at_once(gpu):
     torch.cuda.synchronize()
     for g, w in zip(got, want):
         assert all(torch.equal(a, b) for turn in g for a, b in zip(turn, w))
+
+
+def test_scales_whose_exponents_have_no_float(vc):
+    """scale times log2 e is a factor of the scores."""
+    L, i64 = vc.lib(), ctypes.c_int64
+    p = ctypes.c_void_p(256)
+    for scale in (2.4e38, 3.4e38):
+        assert L.vrs_attention_forward(None, None, None, i64(4), i64(1), i64(1), i64(64), 1, None, i64(1), 0,
+                                       ctypes.c_float(scale), None, p, p, i64(0), None) == 5
+        assert b"scale" in L.vrs_last_error()

@@ -279,3 +279,16 @@ def test_a_tensor_beyond_32_bits(gpu):
     for at, was in ((5, 2.0), ((1 << 31) + 9, 2.0), ((1 << 32) + 4098, 2.0), ((1 << 32) + 1, -1.0)):
         assert abs(t[at].item() - was / (math.sqrt(13.0) + 1e-6)) <= 2.0 ** -11
     assert not t[6:(1 << 31) + 9].any() and not t[(1 << 31) + 10:(1 << 32) + 1].any()
+
+
+@pytest.mark.gpu
+def test_infinite_limit(gpu):
+    """No limit: the factor is 1 and nothing is written; inf / inf for an infinite norm."""
+    import torch
+    from vector_cuda import ops
+    g = torch.randn(1000, device="cuda") * 1e6
+    want = g.clone()
+    norm = ops.clip_grad_norm([g], math.inf)
+    assert torch.equal(g, want) and abs(norm.item() / want.double().norm().item() - 1) < 2.0 ** -23
+    g[3] = math.inf
+    assert ops.clip_grad_norm([g], math.inf).item() == math.inf and g.isnan().all()

@@ -151,7 +151,8 @@ int check(const std::string& w, const Call& c) {
     return invalid(w + ": heads must be a multiple of kv_heads, both at least 1");
   if (c.tokens < 0 || c.tokens > (1ll << 31) - 512) return invalid(w + ": tokens must be in 0..2^31 - 512");
   if (c.heads * (c.tokens / kAttTile + 1) > (1ll << 30)) return invalid(w + ": heads x tokens must be below 2^37");
-  if (!(c.scale > 0.0f) || !(c.scale < INFINITY)) return invalid(w + ": scale must be positive and finite");
+  // (Its product with log2 e has to be a float.)
+  if (!(c.scale > 0.0f) || !(c.scale < 0x1p127f)) return invalid(w + ": scale must be positive and below 2^127");
   if (c.sequences < 0 || c.sequences > (1ll << 31) - 512) return invalid(w + ": sequences must be in 0..2^31 - 512");
   if (c.tokens && !c.cu && (c.sequences < 1 || c.tokens % c.sequences))
     return invalid(w + ": without cu_seqlens, tokens must divide into sequences");
