@@ -682,3 +682,30 @@ def test_scales_whose_exponents_have_no_float(vc):
         assert L.vrs_attention_forward(None, None, None, i64(4), i64(1), i64(1), i64(64), 1, None, i64(1), 0,
                                        ctypes.c_float(scale), None, p, p, i64(0), None) == 5
         assert b"scale" in L.vrs_last_error()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dtype", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lengths,heads,kv", [([1500], 2, 1), ([700, 20, 900], 12, 3), ([260] * 9, 8, 8)])
+def test_calls_that_follow_each_other(gpu, lengths, heads, kv, dtype):
+    """Calls queued one behind the other, whose workspaces are the same memory, and
+    a copy of dk behind each: the bits of calls that wait for each other."""
+    import torch
+    from vector_cuda import ops
+    cu = _bounds(lengths)
+    inputs = [_make(lengths, heads, kv, 64, dtype, seed=s) for s in range(12)]
+    passes = [ops.attention_forward(q, k, v, cu) for q, k, v, _ in inputs]
+
+    def back(i):
+        q, k, v, do = inputs[i]
+        dq, dk, dv = ops.attention_backward(do, q, k, v, *passes[i], cu)
+        return dk.clone(), dv.clone(), dq.clone()
+
+    want = []
+    for i in range(12):
+        torch.cuda.synchronize()
+        want.append(back(i))
+    torch.cuda.synchronize()
+    got = [back(i) for i in range(12)]
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))

@@ -405,6 +405,7 @@ extern "C" int vrs_attention_backward(const vrs_heads* dout, const vrs_heads* q,
   if (st == VRS_OK && dq) {
     a.items = a.tiles * (int)heads;
     a.order = order;
+    a.beside = dk != nullptr;
     a.r1 = (uint16_t*)dq->data;
     a.r1s = dq->stride;
     a.r1h = dq->head_stride;

@@ -418,6 +418,7 @@ struct AttBwd : AttArgs {
   const float* lse2;      // [heads][padded]: lse log2 e, +inf where nothing is seen
   const float* delta;     // [heads][padded]
   const unsigned* bound;  // f16: bits of the largest |dout row|^2 and |v row|^2
+  int beside;             // dq: launched behind the kernel of dk and dv
 };
 struct AttStats {
   AttArgs a;

@@ -17,7 +17,7 @@
 // while the threads work on p, dp is multiplied, and while they work on ds, the
 // next scores are. Bound by that chain: a pair of tiles takes 3,500 clocks for dk and
 // dv, 2,300 for dq, of which products are 4 x 512 and 3 x 512 (d = 128). 8,192 tokens,
-// 8 heads on 2, not causal 863 us (796 TFLOP/s of the five products).
+// 8 heads on 2, not causal 831 us (827 TFLOP/s of the five products).
 #include <atomic>
 
 #include "attention.cuh"
@@ -101,6 +101,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (smem_u32(smem) & 1023) {  // (the same for all threads; never seen)
     if (threadIdx.x == 0) atomicCAS(a.err, 0, 60);
+    grid_wait();
     return;
   }
   if (threadIdx.x == 0) {
@@ -136,8 +137,22 @@ __global__ void __launch_bounds__(kThreads, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *s_tmem;
-  grid_launch();
-  grid_wait();
+  // The kernel of dq begins on SMs that the one of dk and dv leaves, whose results it
+  // does not need (12 heads x 64, 4,096 tokens, causal: 208 us without, 168 so; 16 x 128,
+  // 8,192: 909, 833): that one lets it start once each of its blocks has waited for
+  // what both read. Fences on either side of that start order these reads. It waits for
+  // the kernel before it at its end, so that what follows on the stream has both.
+  if (KEYS) {
+    grid_wait();
+    __threadfence();
+    grid_launch();
+  } else {
+    grid_launch();
+    if (a.beside)
+      __threadfence();
+    else
+      grid_wait();
+  }
 
   // Items: causal, the tiles with the longest passes first (a key's queries are
   // those after it).
@@ -536,6 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     tmem_dealloc(tmem, 512);
   }
+  if (!KEYS && a.beside) grid_wait();
 }
 
 // Per query row: lse in powers of two, and delta = dout . out. A warp takes 32
