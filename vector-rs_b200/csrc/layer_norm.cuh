@@ -59,8 +59,8 @@ struct LnArgs {
 //   small    up to 256 elements: 4 to 32 threads, 8 elements each, two rows at
 //            a time (their loads and reductions overlap)
 //   narrow   up to 4,096: 32 to 256 threads, 16 elements each
-//   between  up to 3,072, many rows, forward only: 4 to 128 threads, 24 elements
-//            each, where that leaves fewer idle (45 M elements in bf16: width 136
+//   between  up to what 128 threads hold, many rows, forward only: 4 to 128
+//            threads, 24 elements each, where that leaves fewer idle (45 M elements in bf16: width 136
 //            36 us, as small 82; 768 33, as narrow 45; 1,536 35 and 44)
 //   wide     up to 8,192, forward only (the backward pass holds five values an
 //            element): 256 threads, 32 elements each
